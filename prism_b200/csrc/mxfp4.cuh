@@ -1,0 +1,52 @@
+// Microscaled 4-bit floating point (OCP MX): elements of 4 bits (E2M1: 0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives),
+// one power of two (E8M0: byte b stands for 2^(b - 127), 255 for not a number) for every 32 elements along a row.
+//
+//   codes   uint8 [..., R, Kp / 2]: Kp is K rounded up to 128; element 2i in the low half of byte i; zero beyond K
+//   scales  uint8 [..., ceil(R / 128), Kp / 128, 512]: a tile of 128 rows by four blocks, the layout in which the tensor
+//           cores' scale factors are copied to tensor memory: the byte of row r, block b at
+//           (r % 32) * 16 + r % 128 / 32 * 4 + b % 4; zero for blocks beyond K, anything for rows beyond R
+//
+// A block's exponent is that of its largest magnitude less two (6 = 1.5 * 2^2 is the largest element), at least -127;
+// elements round to nearest, ties to the even code, and saturate at 6.  Values are exact in bfloat16.  A block that
+// holds an infinity or NaN gets byte 255 and codes 0: all of its values are NaN.
+#pragma once
+
+#include "common.cuh"
+
+namespace prism {
+namespace mx {
+
+constexpr int BLOCK = 32, GROUP = 128, TILE_ROWS = 128, TILE_BYTES = 512;
+
+__host__ __device__ __forceinline__ int groups_of(int K) { return (K + GROUP - 1) / GROUP; }
+
+// place of the scale byte of row r, block b in a matrix of `groups` groups of four blocks
+__device__ __forceinline__ size_t scale_at(int r, int b, int groups) {
+    return ((size_t)(r / TILE_ROWS) * groups + b / 4) * TILE_BYTES + (r & 31) * 16 + (r & 127) / 32 * 4 + (b & 3);
+}
+
+// the scale byte of a block from the bits of its largest magnitude (an integer maximum: NaN and infinity win)
+__device__ __forceinline__ int scale_byte(uint32_t most) {
+    return most >= 0x7f800000u ? 255 : max((int)(most >> 23) - 2, 0);
+}
+// 2^(127 - byte), the factor that brings a block's values into the elements' range
+__device__ __forceinline__ float scale_inverse(int byte) { return __uint_as_float((uint32_t)(254 - min(byte, 253)) << 23); }
+// 2^(byte - 127), NaN for 255
+__device__ __forceinline__ float scale_value(int byte) {
+    return byte == 255 ? __uint_as_float(0x7fffffffu) : byte ? __uint_as_float((uint32_t)byte << 23) : __uint_as_float(0x00400000u);
+}
+// the value of a 4-bit code
+__device__ __forceinline__ float element(uint32_t code) {
+    const uint32_t m = code & 7;
+    const float a = m < 2 ? 0.5f * m : __uint_as_float(((m >> 1) + 126) << 23 | (m & 1) << 22);
+    return code & 8 ? -a : a;
+}
+// two values to 4 bits each, `lo` in the low half of the byte
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+    uint32_t r;
+    asm("{\n\t.reg .b8 t;\n\tcvt.rn.satfinite.e2m1x2.f32 t, %2, %1;\n\tcvt.u32.u8 %0, t;\n\t}" : "=r"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+
+}  // namespace mx
+}  // namespace prism

@@ -157,6 +157,11 @@ class _Sig:
                                   _f, _p, _i, _p, _p, _i, _p]
     prism_attention_merge_bf16 = [_p, _p, _i, _p, _i, _i, _i, _i, _p]
     prism_swiglu = [_p, _p, _i, _i, _i, _p]
+    prism_mxfp4_quantize = [_p, _i, _ll, _i, _i, _i, _p, _p, _p]
+    prism_mxfp4_dequantize = [_p, _p, _i, _i, _i, _p, _i, _p]
+    prism_mxfp4_linear = [_p, _ll, _p, _p, _p, _i, _p, _i, _ll, _i, _i, _i, _i, _p]
+    prism_mxfp4_moe = [_p, _ll, _p, _i, _p, _i, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _i, _i, _i, _f, _p, _i, _i, _i, _f, _f,
+                       _p, _i, _ll, _p, _p, _p, _p]
     prism_sgemm_nt = [_p, _i, _p, _i, _p, _i, _p, _i, _i, _i, _i, _p]
     prism_sample = [_p, _i, _i, _i, _p, _p, _p, _p]
     prism_argmax_split = [_p, _i, _i, _i, _i, _p, _p, _p, _p, _p]
@@ -2474,3 +2479,6 @@ def moe_feed_forward(ctx, x: torch.Tensor, logits: torch.Tensor, gate_up_w: torc
     if own is not None:
         _check(L.prism_moe_identity(_ptr(own), _ptr(sel_e), _ptr(sel_w), T, int(top), W, E, _ptr(y), _stream()), "moe_identity")
     return y
+
+
+from .mxfp4 import Mxfp4, mxfp4_linear, mxfp4_moe, mxfp4_quantize      # noqa: E402,F401

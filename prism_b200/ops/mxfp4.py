@@ -1,0 +1,153 @@
+"""Weights (and activations) in microscaled 4-bit floating point: elements of 4
+bits (E2M1), one power of two (E8M0) for every 32 of them along a row - 17/32
+of a byte an element, against 2 in bfloat16.  ``csrc/mxfp4.cuh`` has the format
+bit by bit.  andre-fu/prism has no such path (its weights are those of the
+file, engine/weight_pool.py:46-70).
+
+``mxfp4_quantize``    rows to 4 bits; ``Mxfp4.dequantize`` gives the values back
+``mxfp4_linear``      ``x @ w.T + bias`` with ``w`` in 4 bits, x as it is or brought to 4 bits too
+``mxfp4_moe``         a whole mixture-of-experts layer for a few tokens, its experts in 4 bits
+"""
+
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+
+from .. import ops
+
+BLOCK, GROUP, TILE_ROWS, TILE_BYTES = 32, 128, 128, 512      # csrc/mxfp4.cuh
+MOE_TOKENS = 64                                              # the most tokens of an ``mxfp4_moe`` call
+DTYPE = "mxfp4"
+
+
+def _need(ok, what: str):
+    if not ok:
+        raise ops.KernelError(what)
+
+
+class Mxfp4:
+    """A matrix ``[N, K]`` (or a stack ``[E, N, K]`` of them) in 4 bits.  ``codes``: uint8 ``[..., N, Kp / 2]`` with ``Kp``
+    the K rounded up to 128, element 2i in the low half of a byte, zero beyond K.  ``scales``: uint8 ``[..., ceil(N / 128),
+    Kp / 128, 512]``: the scale of row r and block b of a tile of 128 rows by four blocks is byte ``(r % 32) * 16 + r % 128
+    // 32 * 4 + b % 4``; zero for blocks beyond K, anything for rows beyond N."""
+
+    __slots__ = ("codes", "scales", "shape")
+    dtype = DTYPE
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, K: int):
+        cs, ss = codes.shape, scales.shape
+        groups = -(-K // GROUP)
+        if not (K > 0 and codes.dtype is torch.uint8 and scales.dtype is torch.uint8 and codes.is_contiguous() and scales.is_contiguous()
+                and len(cs) in (2, 3) and cs[-1] == groups * (GROUP // 2) and cs[-2] > 0
+                and ss == cs[:-2] + (-(-cs[-2] // TILE_ROWS), groups, TILE_BYTES)):
+            raise ops.KernelError(f"4-bit matrix of K = {K}: codes {tuple(cs)} {codes.dtype} and scales {tuple(ss)} {scales.dtype} do not belong together")
+        self.codes, self.scales, self.shape = codes, scales, cs[:-1] + (K,)
+
+    @property
+    def device(self):
+        return self.codes.device
+
+    @property
+    def nbytes(self) -> int:
+        return self.codes.numel() + self.scales.numel()
+
+    def dim(self) -> int:
+        return len(self.shape)
+
+    def __getitem__(self, e: int) -> "Mxfp4":
+        """One matrix of a stack."""
+        _need(len(self.shape) == 3, "only a stack of 4-bit matrices can be indexed")
+        return Mxfp4(self.codes[e], self.scales[e], self.shape[-1])
+
+    def dequantize(self, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+        """The values that the codes stand for, exact in bfloat16 and float32; NaN where the scale is 255."""
+        _need(dtype in (torch.bfloat16, torch.float32), f"4-bit values come back as bfloat16 or float32, not {dtype}")
+        ops._cuda(self.codes, self.scales)
+        out = torch.empty(self.shape, dtype=dtype, device=self.device)
+        N, K = self.shape[-2:]
+        ops._check(ops.lib().prism_mxfp4_dequantize(self.codes.data_ptr(), self.scales.data_ptr(), self.codes.numel() // self.codes.shape[-1],
+                                                    N, K, out.data_ptr(), ops._dt(out), ops._stream()), "mxfp4_dequantize")
+        return out
+
+
+def mxfp4_quantize(x: torch.Tensor) -> Mxfp4:
+    """``x [N, K]`` (rows may have a stride of their own) or a contiguous stack ``[E, N, K]``, bfloat16 or float32, to 4
+    bits: a block's exponent is that of its largest magnitude less two, elements round to nearest (ties to the even code) and
+    saturate at 6.  A block that holds an infinity or NaN becomes NaN as a whole."""
+    ops._cuda(x)
+    _need(x.dim() in (2, 3) and x.numel() > 0, f"rows to quantise: a matrix or a stack of them, got {tuple(x.shape)}")
+    _need(x.stride(-1) == 1 or x.shape[-1] == 1, "rows to quantise lie side by side in memory")
+    _need(x.dim() == 2 or x.is_contiguous(), "a stack to quantise is contiguous")
+    N, K = x.shape[-2:]
+    groups, lead = -(-K // GROUP), tuple(x.shape[:-2])
+    codes = torch.empty(lead + (N, groups * (GROUP // 2)), dtype=torch.uint8, device=x.device)
+    scales = torch.empty(lead + (-(-N // TILE_ROWS), groups, TILE_BYTES), dtype=torch.uint8, device=x.device)
+    rows = x.numel() // K
+    ops._check(ops.lib().prism_mxfp4_quantize(x.data_ptr(), ops._dt(x), x.stride(-2) if rows > 1 else K, rows, N, K, codes.data_ptr(),
+                                              scales.data_ptr(), ops._stream()), "mxfp4_quantize")
+    return Mxfp4(codes, scales, K)
+
+
+def mxfp4_linear(x: torch.Tensor, w: Mxfp4, bias: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
+                 out_dtype: Optional[torch.dtype] = None, act_bits: int = 16) -> torch.Tensor:
+    """``x @ w.T + bias`` for ``x [M, K]`` in bfloat16 (rows may have a stride of their own) and ``w [N, K]`` in 4 bits, sums
+    in float32.  ``act_bits`` 16: x as it is; 4: each row of x is brought to 4 bits first, as ``mxfp4_quantize`` does it.
+    ``out`` (row stride of its own) or ``out_dtype``: bfloat16 (default) or float32.  A row of x with an infinity or NaN in it
+    gives NaN."""
+    ops._cuda(x, w.codes, w.scales, bias, out)
+    _need(x.dim() == 2 and w.dim() == 2 and x.shape[1] == w.shape[1], f"product of {tuple(x.shape)} and {tuple(w.shape)}")
+    M, K = x.shape
+    N = w.shape[0]
+    _need(x.dtype is torch.bfloat16 and (x.stride(1) == 1 or K == 1), "activations are bfloat16 rows side by side in memory")
+    _need(act_bits in (4, 16), f"activations have 4 or 16 bits, not {act_bits}")
+    _need(bias is None or (bias.shape == (N,) and bias.is_contiguous()), "a bias has one entry per row of the weight")
+    if out is None:
+        out = torch.empty((M, N), dtype=out_dtype or torch.bfloat16, device=x.device)
+    _need(out.shape == (M, N) and (out.stride(1) == 1 or N == 1) and out_dtype in (None, out.dtype), "out does not fit the product")
+    ops._check(ops.lib().prism_mxfp4_linear(x.data_ptr(), x.stride(0), w.codes.data_ptr(), w.scales.data_ptr(), ops._ptr(bias),
+                                            ops.F32 if bias is None else ops._dt(bias), out.data_ptr(), ops._dt(out), out.stride(0), M, N, K,
+                                            act_bits, ops._stream()), "mxfp4_linear")
+    return out
+
+
+def mxfp4_moe(x: torch.Tensor, router: torch.Tensor, gate: Mxfp4, up: Mxfp4, down: Mxfp4, top: int, softmax: bool = False,
+              renorm: bool = False, scale_input: bool = True, act: str = "silu", limit: float = 0.0,
+              router_bias: Optional[torch.Tensor] = None, choice: Optional["ops.MoeChoice"] = None, out: Optional[torch.Tensor] = None,
+              out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """A mixture-of-experts layer for up to 64 tokens: ``x [T, H]`` bfloat16, ``router [E, H]`` (logits in float32),
+    ``gate``, ``up`` ``[E, F, H]`` and ``down`` ``[E, H, F]`` in 4 bits.  Each token takes the ``top`` experts with the largest
+    scores (sigmoid of the logits, or their softmax; the lower index of equal ones); a choice's weight is its score
+    (``renorm``: over the sum of the chosen) and multiplies the expert's input (``scale_input``) or its output.  ``act``:
+    silu, gelu_tanh or clamped (with ``limit``, as in ``ops.glu``).  ``choice``: an ``ops.MoeChoice``.  Returns the sum over a
+    token's choices, ``[T, H]`` bfloat16 or float32 (``out`` or ``out_dtype``)."""
+    ops._cuda(x, router, gate.codes, up.codes, down.codes, router_bias, out)
+    _need(x.dim() == 2 and x.dtype is torch.bfloat16 and x.stride(1) == 1, "activations are bfloat16 rows side by side in memory")
+    T, H = x.shape
+    E, F, _ = gate.shape if gate.dim() == 3 else (0, 0, 0)
+    _need(E > 0 and gate.shape == (E, F, H) and up.shape == gate.shape and down.shape == (E, H, F),
+          f"experts {tuple(gate.shape)}, {tuple(up.shape)}, {tuple(down.shape)} do not belong together or to rows of {H}")
+    _need(T <= MOE_TOKENS, f"{T} tokens: this layer is for up to {MOE_TOKENS}")
+    _need(1 <= top <= E, f"a token uses {top} of {E} experts: between 1 and all of them")
+    _need(router.shape == (E, H) and router.is_contiguous() and (router_bias is None or (router_bias.shape == (E,) and router_bias.is_contiguous())),
+          "the router has one row (and one bias) per expert")
+    _need(act in ops.GATED, f"a gated feed-forward's activation is one of {ops.GATED}, got {act!r}")
+    ch = choice or ops.MoeChoice()
+    _need(ch.correction is None or (ch.correction.shape == (E,) and ch.correction.is_contiguous() and ch.correction.is_cuda),
+          "the correction has one entry per expert")
+    _need(ch.groups >= 1 and E % ch.groups == 0 and 1 <= ch.keep <= ch.groups and ch.keep * (E // ch.groups) >= top,
+          f"{E} experts in {ch.groups} groups of which {ch.keep} are kept, {top} a token")
+    if out is None:
+        out = torch.empty((T, H), dtype=out_dtype or torch.bfloat16, device=x.device)
+    _need(out.shape == (T, H) and out.stride(1) == 1 and out_dtype in (None, out.dtype), "out does not fit the layer")
+    sel_e = torch.empty(T * top, dtype=torch.int32, device=x.device)
+    scratch = torch.empty(T * top * (F + 1), dtype=torch.float32, device=x.device)
+    ops._check(ops.lib().prism_mxfp4_moe(x.data_ptr(), x.stride(0), router.data_ptr(), ops._dt(router), ops._ptr(router_bias),
+                                         ops.F32 if router_bias is None else ops._dt(router_bias), gate.codes.data_ptr(), gate.scales.data_ptr(),
+                                         up.codes.data_ptr(), up.scales.data_ptr(), down.codes.data_ptr(), down.scales.data_ptr(), T, H, F, E,
+                                         top, int(softmax), int(renorm), int(scale_input), ops.MOE_ACTS[act], float(limit),
+                                         ops._ptr(ch.correction), ops.F32 if ch.correction is None else ops._dt(ch.correction), ch.groups, ch.keep,
+                                         ch.scale, ch.sum_eps, out.data_ptr(), ops._dt(out), out.stride(0), sel_e.data_ptr(),
+                                         scratch.data_ptr(), scratch.data_ptr() + 4 * T * top, ops._stream()), "mxfp4_moe")
+    return out
