@@ -1,85 +1,516 @@
-// y [M, N] = x [M, K] W [N, K]^T (+ bias) with W in microscaled 4-bit floating point (mxfp4.cuh), x in bfloat16 as it is or
-// brought to 4 bits first (a block of 32 along a row at a time, as W was).
+// y [M, N] = x [M, K] W [N, K]^T (+ bias) with W in microscaled 4-bit floating point (mxfp4.cuh), x in bfloat16 as it is
+// (act_bits 16) or brought to 4 bits first (act_bits 4: a block of 32 along a row at a time, as W was).
 //
-// CUDA cores: a CTA takes 64 rows of W and 32 of x, and walks K by blocks of 32, whose values both sides leave in shared
-// memory in float32; a thread has 4 x 2 sums.
+// Both run on the block-scaled tensor-core instructions, which take the codes and scale bytes as they lie in memory: no CUDA
+// core ever unpacks a weight.  128 rows of W are the M of a tcgen05.mma, tokens its N, the sums sit in tensor memory in
+// float32, the scales go from shared to tensor memory by tcgen05.cp.
+//
+//   act_bits 4   kind::mxf4: 4-bit codes on both sides, a scale for every 32 of either.
+//   act_bits 16  kind::mxf8f6f4 multiplies 4-bit codes by 8-bit ones (E4M3).  A bfloat16 value has 8 significant bits, two
+//                E4M3 terms of 4 each hold them: x = 2^s (hi + 2^-5 lo), s a block's own, hi the nearest E4M3 of x / 2^s and
+//                lo the (exact) rest times 2^5.  Exact for values within 2^-14 of their block's largest; below, off by at
+//                most 2^-22 of it.  Up to 64 tokens hi and lo are columns of one instruction, added at the end (W is
+//                then read from shared memory once); for tiles of 128 tokens two instructions add to the same sums.
+//
+// A first kernel brings x to terms or codes (a thread 8 values), in the workspace of the call, and clears its counters.  The
+// second is persistent, a CTA an SM: warp 0 issues TMA loads into a ring of stages (W: for 16 bits 128 codes a row, which
+// TMA spreads to a byte each, for 4 bits 256), warp 1 the scale copies and the products, the other warps take the sums out.
+// All of the product's blocks - (tile of W rows, tile of tokens, stage of K) - are dealt to the CTAs evenly as one long
+// line, so that every SM streams the same number of bytes whatever the sizes; a tile that several CTAs have part of is
+// added up by the one that comes last, in the order of the CTAs: results do not depend on timing.
+//
+// Every wait is bounded (tcgen05.cuh); on expiry the kernel sets the error word, frees tensor memory and returns.
 #include "mxfp4.cuh"
+#include "tcgen05.cuh"
+#include "vec.cuh"
 
 namespace prism {
 namespace mx {
 
-constexpr int TN = 64, TM = 32;
+using tc::mbar_expect_tx;
+using tc::mbar_init;
+using tc::mbar_wait;
+using tc::smem_addr;
+using tc::tma_load_2d;
+using tc::tmem_load;
+using tc::umma_commit;
+using tc::umma_desc;
 
-template <typename TO>
-__global__ void __launch_bounds__(256) linear_kernel(const __nv_bfloat16* __restrict__ x_in, long long ldx, const uint8_t* __restrict__ codes,
-                                                     const uint8_t* __restrict__ scales, const void* __restrict__ bias, int bias_bf16,
-                                                     TO* __restrict__ y, long long ldy, int M, int N, int K, int groups, int four) {
-    __shared__ float ws[TN][BLOCK + 1], xs[TM][BLOCK + 1];
-    pdl_wait();
+// ---- x to terms or codes ------------------------------------------------------------------------------------------------
+
+__device__ __forceinline__ uint32_t pack_e4m3(float lo, float hi) {
+    uint16_t r;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %2, %1;" : "=h"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ void unpack_e4m3(uint32_t p, float& lo, float& hi) {
+    uint32_t h;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((uint16_t)p));
+    asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.f32.f16 %0, a;\n\tcvt.f32.f16 %1, b;\n\t}" : "=f"(lo), "=f"(hi) : "r"(h));
+}
+
+// act 16: terms uint8 [token tile][2 tt][Kp], a tile's hi rows, then its lo rows; scales [token tile][groups][atoms][512],
+// the tiles of 128 such rows.  act 4: codes and scales as in mxfp4.cuh.  Rows that have no token are left as they are.
+template <bool A16>
+__global__ void __launch_bounds__(256) prepare_kernel(const __nv_bfloat16* __restrict__ x_in, long long ldx, int M, int K, int groups, int wide,
+                                                      int tt, uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, int* __restrict__ counters,
+                                                      int ncounters) {
+    pdl_wait();            // before the trigger: the product, which reads W at once, starts behind all that came before this kernel
     pdl_trigger();
     const __nv_bfloat16* x = pdl_fresh(x_in);
-    const int n0 = blockIdx.x * TN, m0 = blockIdx.y * TM, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int tn = threadIdx.x & 15, tm = threadIdx.x >> 4;
-    float acc[4][2] = {};
-    for (int b = 0; b * BLOCK < K; ++b) {
-        __syncthreads();
-        const int k = b * BLOCK + lane;
-        for (int i = warp; i < TN; i += 8) {
-            const int n = n0 + i;
-            float v = 0.f;
-            if (n < N) {
-                const uint32_t byte = codes[(size_t)n * (groups * (GROUP / 2)) + k / 2];
-                v = element(byte >> (4 * (k & 1)) & 15) * scale_value(scales[scale_at(n, b, groups)]);
-            }
-            ws[i][lane] = v;
-        }
-        for (int i = warp; i < TM; i += 8) {
-            float v = m0 + i < M && k < K ? __bfloat162float(x[(long long)(m0 + i) * ldx + k]) : 0.f;
-            if (four) {
-                const int byte = scale_byte(__reduce_max_sync(0xffffffffu, __float_as_uint(v) & 0x7fffffffu));
-                v = byte == 255 ? scale_value(255) : element(pack2(v * scale_inverse(byte), 0.f)) * scale_value(byte);
-            } else if (!isfinite(v)) {
-                v = scale_value(255);
-            }
-            xs[i][lane] = v;
-        }
-        __syncthreads();
-#pragma unroll 8
-        for (int j = 0; j < BLOCK; ++j) {
-            const float a0 = xs[tm][j], a1 = xs[tm + 16][j];
+    const int per_row = groups * (GROUP / 8);
+    const long long total = (long long)M * per_row;
+    const long long first = (long long)blockIdx.x * blockDim.x + threadIdx.x;
+    for (long long i = first; i < ncounters; i += (long long)gridDim.x * blockDim.x) counters[i] = 0;
+    for (long long i = first; i < total; i += (long long)gridDim.x * blockDim.x) {
+        const int r = (int)(i / per_row), c = (int)(i - (long long)r * per_row) * 8;
+        const __nv_bfloat16* p = x + (long long)r * ldx + c;
+        float v[8];
+        if (wide && c + 8 <= K) {
+            load8(p, v);
+        } else {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float w = ws[tn + 16 * i][j];
-                acc[i][0] = fmaf(a0, w, acc[i][0]);
-                acc[i][1] = fmaf(a1, w, acc[i][1]);
+            for (int j = 0; j < 8; ++j) v[j] = c + j < K ? to_float(p[j]) : 0.f;
+        }
+        uint32_t most = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) most = max(most, __float_as_uint(v[j]) & 0x7fffffffu);
+        const uint32_t four = 0xfu << (threadIdx.x & 28);
+        most = max(most, __shfl_xor_sync(four, most, 1));
+        most = max(most, __shfl_xor_sync(four, most, 2));
+        const bool bad = most >= 0x7f800000u;
+        if (A16) {
+            const int byte = max((int)(most >> 23) - 7, 5), lines = 2 * tt, atoms = (lines + 127) / 128;
+            const float f = __uint_as_float((uint32_t)(254 - byte) << 23);
+            uint32_t hi[2] = {0, 0}, lo[2] = {0, 0};
+            if (!bad) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float a = v[2 * j] * f, b = v[2 * j + 1] * f;
+                    const uint32_t h = pack_e4m3(a, b);
+                    float ha, hb;
+                    unpack_e4m3(h, ha, hb);
+                    hi[j / 2] |= h << (16 * (j & 1));
+                    lo[j / 2] |= pack_e4m3((a - ha) * 32.f, (b - hb) * 32.f) << (16 * (j & 1));
+                }
+            }
+            const int tile = r / tt, t = r - tile * tt;
+            uint8_t* at = codes + ((size_t)tile * lines + t) * ((size_t)groups * GROUP) + c;
+            *reinterpret_cast<uint2*>(at) = make_uint2(hi[0], hi[1]);
+            *reinterpret_cast<uint2*>(at + (size_t)tt * groups * GROUP) = make_uint2(lo[0], lo[1]);
+            if ((threadIdx.x & 3) == 0) {
+                uint8_t* s = scales + ((size_t)tile * groups + c / GROUP) * (atoms * TILE_BYTES) + c % GROUP / BLOCK;
+                const int u = t + tt;
+                s[t / 128 * TILE_BYTES + (t & 31) * 16 + (t & 127) / 32 * 4] = bad ? 255 : (uint8_t)byte;
+                s[u / 128 * TILE_BYTES + (u & 31) * 16 + (u & 127) / 32 * 4] = bad ? 255 : (uint8_t)(byte - 5);
+            }
+        } else {
+            const int byte = scale_byte(most);
+            const float inv = scale_inverse(byte);
+            uint32_t word = 0;
+            if (!bad)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) word |= pack2(v[2 * j] * inv, v[2 * j + 1] * inv) << (8 * j);
+            *reinterpret_cast<uint32_t*>(codes + (size_t)r * (groups * (GROUP / 2)) + c / 2) = word;
+            if ((threadIdx.x & 3) == 0) scales[scale_at(r, c / BLOCK, groups)] = (uint8_t)byte;
+        }
+    }
+}
+
+// ---- the product --------------------------------------------------------------------------------------------------------
+
+template <bool A16_, int TT_, int W_> struct Cfg {
+    static constexpr bool A16 = A16_;
+    static constexpr int TT = TT_, W = W_;                         // tokens of a tile; tiles of 128 rows of W that share it
+    static constexpr bool SIDE = A16 && TT <= 64;                  // hi and lo side by side as columns
+    static constexpr int GS = A16 ? 1 : 2;                         // groups of 128 along K in a stage (128 bytes of a row)
+    static constexpr int XR = A16 ? 2 * TT : TT;                   // rows of x's tile
+    static constexpr int NCOL = SIDE ? 2 * TT : TT;                // N of the instruction
+    static constexpr int ATOMS = (XR + 127) / 128;                 // tiles of scales of x
+    static constexpr int W_BYTES = W * 16384, X_BYTES = XR * 128, STAGE = W_BYTES + X_BYTES;
+    // bytes that a stage's loads report: codes that TMA spreads count as they are in memory, 64 bytes a row
+    static constexpr int ARRIVE = W * (A16 ? 8192 : 16384) + X_BYTES;
+    static constexpr int SF = GS * TILE_BYTES * (W + ATOMS);       // scale bytes of a stage
+    static constexpr int FIT = (216 * 1024) / (STAGE + SF);
+    static constexpr int SF_COLS = GS * 4 * (W + ATOMS);           // their columns in tensor memory: every stage has its own
+    static constexpr int STAGES = FIT > 10 ? 10 : FIT;
+    static constexpr int BUFS = 2 * W * NCOL + STAGES * SF_COLS <= 512 ? 2 : 1;
+    static constexpr int COLS_USED = BUFS * W * NCOL + STAGES * SF_COLS;
+    static constexpr int COLS = COLS_USED <= 64 ? 64 : COLS_USED <= 128 ? 128 : COLS_USED <= 256 ? 256 : 512;
+    static constexpr int EPI_WARPS = 4 * W, THREADS = 64 + 32 * EPI_WARPS;
+    static constexpr size_t SMEM = (size_t)STAGES * (STAGE + SF) + 1024 + 512;
+    static_assert(COLS_USED <= 512 && STAGES >= 3, "tensor memory or shared memory");
+};
+
+struct Split {                 // how the blocks are dealt: CTA c has the blocks [c total / P, (c + 1) total / P)
+    long long total;
+    int P, kb;                 // CTAs; stages of K of a unit
+    __device__ __forceinline__ long long start(int c) const { return (long long)c * total / P; }
+    __device__ __forceinline__ int owner(long long b) const { return (int)(((b + 1) * P - 1) / total); }
+};
+
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 ::"r"(smem_addr(dst)), "l"(src), "r"(bytes), "r"(smem_addr(bar)) : "memory");
+}
+// 512 bytes of scales, 32 rows of 16 without swizzle, to four columns of tensor memory, the same in every quarter of its lanes
+__device__ __forceinline__ void scales_to_tmem(uint32_t taddr, uint32_t saddr) {
+    const uint64_t d = (uint64_t)((saddr >> 4) & 0x3FFF) | (uint64_t)8 << 32 | (uint64_t)1 << 46;
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(d) : "memory");
+}
+template <bool A16>
+__device__ __forceinline__ void umma_scaled(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb, uint32_t accumulate) {
+    if (A16)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+            ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate) : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+            ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate) : "memory");
+}
+// Instruction descriptor: element kinds (mxf8f6f4: A E2M1 = 5, B E4M3 = 0; mxf4: E2M1 = 1 on both sides), N / 8, scales E8M0,
+// M / 128; `id`: which byte of a scale column the instruction begins at.
+template <typename C> __device__ __forceinline__ constexpr uint32_t idesc_of(int id) {
+    return (C::A16 ? 5u << 7 : 1u << 7 | 1u << 10) | (uint32_t)(C::NCOL >> 3) << 17 | 1u << 23 | 1u << 27 | (uint32_t)id << 4 | (uint32_t)id << 29;
+}
+
+struct Product {
+    const uint8_t *w_scales, *x_scales;
+    const void* bias;
+    void* y;
+    float* part;               // [P][2][W][TT][128]
+    int *counters, *err;
+    long long ldy;
+    Split split;
+    int M, N, groups, mtiles, ntiles, bias_bf16, out_bf16;
+};
+
+template <typename C>
+__global__ void __launch_bounds__(C::THREADS, 1)
+product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const __grid_constant__ Product p) {
+    constexpr int TT = C::TT, W = C::W, STAGES = C::STAGES;
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char* tiles = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    unsigned char* sf = tiles + (size_t)STAGES * C::STAGE;
+    uint64_t* full = reinterpret_cast<uint64_t*>(sf + STAGES * C::SF);
+    uint64_t *empty = full + STAGES, *acc_full = empty + STAGES, *acc_empty = acc_full + C::BUFS;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + C::BUFS);
+    __shared__ int abort_flag, is_last, gone;
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, cta = blockIdx.x;
+    if (threadIdx.x == 0) {
+        abort_flag = 0;
+        for (int s = 0; s < STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+        for (int s = 0; s < C::BUFS; ++s) { mbar_init(&acc_full[s], 1); mbar_init(&acc_empty[s], C::EPI_WARPS); }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(tmem_slot)), "r"(C::COLS));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem = *tmem_slot, tmem_sf = tmem + C::BUFS * W * C::NCOL;
+    volatile int* abortp = &abort_flag;
+    const long long b0 = p.split.start(cta), b1 = p.split.start(cta + 1);
+    const int n = (int)(b1 - b0), kb = p.split.kb;
+
+    // unit u: token tile u % mtiles of the W tiles W (u / mtiles) .. + W - 1
+    if (warp == 0) {
+        if (lane == 0) {
+            auto load_w = [&](int i) {
+                const long long b = b0 + i;
+                const int u = (int)(b / kb), k = (int)(b - (long long)u * kb), s = i % STAGES, t0 = u / p.mtiles * W;
+                const int gs = min(C::GS, p.groups - k * C::GS);         // groups that exist of this stage's
+                mbar_expect_tx(&full[s], C::ARRIVE + gs * TILE_BYTES * (W + C::ATOMS));
+#pragma unroll
+                for (int w = 0; w < W; ++w) {
+                    tma_load_2d(tiles + (size_t)s * C::STAGE + w * 16384, &map_w, &full[s], k * 128, (t0 + w) * 128);
+                    const int t = min(t0 + w, p.ntiles - 1);             // the last tile may have no partner: its scales again, never stored
+                    bulk_load(sf + s * C::SF + w * C::GS * TILE_BYTES, p.w_scales + ((size_t)t * p.groups + k * C::GS) * TILE_BYTES, gs * TILE_BYTES,
+                              &full[s]);
+                }
+            };
+            auto load_x = [&](int i) {
+                const long long b = b0 + i;
+                const int u = (int)(b / kb), k = (int)(b - (long long)u * kb), s = i % STAGES, m = u % p.mtiles;
+                const int gs = min(C::GS, p.groups - k * C::GS);
+                tma_load_2d(tiles + (size_t)s * C::STAGE + C::W_BYTES, &map_x, &full[s], k * 128, m * C::XR);
+                bulk_load(sf + s * C::SF + W * C::GS * TILE_BYTES, p.x_scales + ((size_t)m * p.groups + k * C::GS) * (C::ATOMS * TILE_BYTES),
+                          gs * C::ATOMS * TILE_BYTES, &full[s]);
+            };
+            const int pre = min(n, STAGES);
+            for (int i = 0; i < pre; ++i) load_w(i);
+            pdl_wait();
+            for (int i = 0; i < pre; ++i) load_x(i);
+            int issued = pre;
+            for (int i = pre; i < n; ++i) {
+                if (!mbar_wait(&empty[i % STAGES], (i / STAGES - 1) & 1, abortp)) break;
+                load_w(i);
+                load_x(i);
+                issued = i + 1;
+            }
+            pdl_trigger_gemm();
+            if (*abortp)
+                for (int i = max(0, issued - STAGES); i < issued; ++i) mbar_wait(&full[i % STAGES], (i / STAGES) & 1, abortp);
+        }
+    } else if (warp == 1) {
+        if (lane == 0) {
+            bool ok = true;
+            int seg = 0;
+            for (int i = 0; i < n && ok; ++i) {
+                const int k = (int)((b0 + i) % kb), s = i % STAGES;
+                const bool fresh = i == 0 || k == 0;
+                const int buf = seg % C::BUFS;
+                if (fresh && seg >= C::BUFS) ok = mbar_wait(&acc_empty[buf], (seg / C::BUFS - 1) & 1, abortp);
+                if (!ok) break;
+                ok = mbar_wait(&full[s], (i / STAGES) & 1, abortp);
+                if (!ok) break;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const uint32_t st = smem_addr(tiles + (size_t)s * C::STAGE), ss = smem_addr(sf + s * C::SF), tsf = tmem_sf + s * C::SF_COLS;
+                const int gs = min(C::GS, p.groups - k * C::GS);
+                for (int g = 0; g < gs; ++g) {
+#pragma unroll
+                    for (int w = 0; w < W; ++w) scales_to_tmem(tsf + (w * C::GS + g) * 4, ss + (w * C::GS + g) * TILE_BYTES);
+#pragma unroll
+                    for (int a = 0; a < C::ATOMS; ++a)
+                        scales_to_tmem(tsf + (W * C::GS + g * C::ATOMS + a) * 4, ss + (W * C::GS + g * C::ATOMS + a) * TILE_BYTES);
+                }
+                const uint64_t db = umma_desc(st + C::W_BYTES);
+                const int slices = C::A16 ? 4 : 2 * gs;                  // 32 bytes of a row each: 32 or 64 elements
+#pragma unroll
+                for (int w = 0; w < W; ++w) {
+                    const uint64_t da = umma_desc(st + w * 16384);
+                    const uint32_t d = tmem + (buf * W + w) * C::NCOL;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        if (j >= slices) break;
+                        const int g = C::A16 ? 0 : j / 2, id = C::A16 ? j : (j & 1) * 2;
+                        const uint32_t sa = tsf + (w * C::GS + g) * 4, sb = tsf + (W * C::GS + g * C::ATOMS) * 4;
+                        umma_scaled<C::A16>(d, da + 2 * j, db + 2 * j, idesc_of<C>(id), sa, sb, !fresh || j > 0);
+                        if (C::A16 && !C::SIDE)
+                            umma_scaled<C::A16>(d, da + 2 * j, db + (TT * 128 >> 4) + 2 * j, idesc_of<C>(id), sa, sb + 4, 1);
+                    }
+                }
+                umma_commit(&empty[s]);
+                if (i == n - 1 || k == kb - 1) {
+                    umma_commit(&acc_full[buf]);
+                    ++seg;
+                }
+            }
+        }
+    } else {
+        // warps of one tile of W rows: 2 + 4 w .. 5 + 4 w; TMEM lanes (warp % 4) * 32 .. + 31
+        const int w = (warp - 2) / 4, q = warp & 3, row = q * 32 + lane;
+        pdl_wait();
+        int seg = 0;
+        for (int i = 0; i < n; ++seg) {
+            const long long b = b0 + i;
+            const int u = (int)(b / kb), k0 = (int)(b - (long long)u * kb), k1 = min(kb, k0 + n - i), buf = seg % C::BUFS;
+            i += k1 - k0;
+            mbar_wait(&acc_full[buf], (seg / C::BUFS) & 1, abortp);
+            // one thread reads the flag for all of these warps: they leave together or not at all
+            asm volatile("bar.sync 1, %0;" ::"n"(C::EPI_WARPS * 32) : "memory");
+            if (threadIdx.x == 64) gone = *abortp;
+            asm volatile("bar.sync 1, %0;" ::"n"(C::EPI_WARPS * 32) : "memory");
+            if (gone) break;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            const int m0 = u % p.mtiles * TT, f = (u / p.mtiles * W + w) * 128 + row;      // first token, this thread's output feature
+            const int tokens = min(TT, p.M - m0);
+            const uint32_t d = tmem + ((uint32_t)(q * 32) << 16) + (buf * W + w) * C::NCOL;
+            const bool whole = k0 == 0 && k1 == kb;
+            const float bias = p.bias != nullptr && f < p.N ? load_param(p.bias, p.bias_bf16, f) : 0.f;
+            auto store = [&](int t0, const float (&v)[8]) {
+                if (f >= p.N) return;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    if (t0 + j >= tokens) return;
+                    const long long at = (long long)(m0 + t0 + j) * p.ldy + f;
+                    if (p.out_bf16) reinterpret_cast<__nv_bfloat16*>(p.y)[at] = __float2bfloat16_rn(v[j] + bias);
+                    else reinterpret_cast<float*>(p.y)[at] = v[j] + bias;
+                }
+            };
+            const int slot = (int)(p.split.start(cta) / kb) == u ? 0 : 1;
+            float* mine = p.part + (((size_t)cta * 2 + slot) * W + w) * (TT * 128) + row;
+#pragma unroll 1
+            for (int t0 = 0; t0 < tokens; t0 += 8) {
+                float v[8];
+                {
+                    uint32_t r[8], l[8];
+                    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]) : "r"(d + t0));
+                    if (C::SIDE)
+                        asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                                     : "=r"(l[0]), "=r"(l[1]), "=r"(l[2]), "=r"(l[3]), "=r"(l[4]), "=r"(l[5]), "=r"(l[6]), "=r"(l[7]) : "r"(d + TT + t0));
+                    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(r[j]) + (C::SIDE ? __uint_as_float(l[j]) : 0.f);
+                }
+                if (whole) store(t0, v);
+                else
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) mine[(t0 + j) * 128] = v[j];
+            }
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(&acc_empty[buf])) : "memory");
+            if (whole) continue;
+            const int c0 = p.split.owner((long long)u * kb), c1 = p.split.owner((long long)(u + 1) * kb - 1);
+            __threadfence();
+            asm volatile("bar.sync 1, %0;" ::"n"(C::EPI_WARPS * 32) : "memory");
+            if (threadIdx.x == 64) is_last = atomicAdd(&p.counters[u], 1) == c1 - c0;
+            asm volatile("bar.sync 1, %0;" ::"n"(C::EPI_WARPS * 32) : "memory");
+            if (!is_last) continue;
+            __threadfence();
+#pragma unroll 1
+            for (int t0 = 0; t0 < tokens; t0 += 8) {
+                float v[8] = {};
+                for (int c = c0; c <= c1; ++c) {
+                    const int sl = (int)(p.split.start(c) / kb) == u ? 0 : 1;
+                    const float* from = p.part + (((size_t)c * 2 + sl) * W + w) * (TT * 128) + row + t0 * 128;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) v[j] += __ldcg(from + j * 128);
+                }
+                store(t0, v);
             }
         }
     }
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int n = n0 + tn + 16 * i, m = m0 + tm + 16 * h;
-            if (n < N && m < M) y[(long long)m * ldy + n] = from_float<TO>(acc[i][h] + (bias != nullptr ? load_param(bias, bias_bf16, n) : 0.f));
-        }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    if (threadIdx.x == 0 && abort_flag) report_error(p.err, PRISM_ERR_WAIT_TIMEOUT);
+    if (warp == 1) {
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::COLS));
+    }
+}
+
+// ---- host side ----------------------------------------------------------------------------------------------------------
+
+// a matrix of bytes (or of 4-bit codes that TMA spreads to a byte each: `spread`, 128 of them a box row), boxes of 128 bytes in shared memory
+inline int byte_map(CUtensorMap* map, const void* ptr, long long rows, long long row_bytes, int box_rows, bool spread) {
+    tc::EncodeTiledFn fn = tc::encode_fn();
+    if (fn == nullptr) return (int)cudaErrorNotSupported;
+    cuuint64_t dims[2] = {(cuuint64_t)(spread ? row_bytes * 2 : row_bytes), (cuuint64_t)rows};
+    cuuint64_t strides[1] = {(cuuint64_t)row_bytes};
+    cuuint32_t box[2] = {128, (cuuint32_t)box_rows}, estr[2] = {1, 1};
+    CUresult r = fn(map, spread ? CU_TENSOR_MAP_DATA_TYPE_16U4_ALIGN16B : CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(ptr), dims, strides, box,
+                    estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? 0 : (int)cudaErrorInvalidValue;
+}
+
+inline int sm_count() {
+    static int n[64] = {};
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev < 0 || dev >= 64) return 148;
+    if (!n[dev]) cudaDeviceGetAttribute(&n[dev], cudaDevAttrMultiProcessorCount, dev);
+    return n[dev];
+}
+
+// tokens of a tile and tiles of W that share one
+inline void tiles_for(int M, int act_bits, int& tt, int& w) {
+    tt = M <= 8 && act_bits == 16 ? 8 : M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128;
+    w = tt >= 32 ? 2 : 1;
+}
+
+struct Plan {
+    int tt, w, groups, mtiles, ntiles, kb, P;
+    long long units, codes, scales, parts, counters, bytes;       // bytes from the workspace's start
+};
+inline Plan plan_for(int M, int N, int K, int act_bits) {
+    Plan q;
+    tiles_for(M, act_bits, q.tt, q.w);
+    q.groups = groups_of(K);
+    q.mtiles = (M + q.tt - 1) / q.tt;
+    q.ntiles = (N + 127) / 128;
+    q.kb = act_bits == 16 ? q.groups : (q.groups + 1) / 2;
+    q.units = (long long)((q.ntiles + q.w - 1) / q.w) * q.mtiles;
+    const long long total = q.units * q.kb;
+    q.P = (int)(total < sm_count() ? total : sm_count());
+    const int xr = act_bits == 16 ? 2 * q.tt : q.tt, atoms = (xr + 127) / 128;
+    auto up = [](long long b) { return (b + 1023) / 1024 * 1024; };
+    q.codes = 0;
+    q.scales = up(act_bits == 16 ? (long long)q.mtiles * xr * q.groups * GROUP : (long long)M * q.groups * (GROUP / 2));
+    q.parts = q.scales + up((long long)q.mtiles * q.groups * atoms * TILE_BYTES);
+    q.counters = q.parts + up((long long)q.P * 2 * q.w * q.tt * 128 * 4);
+    q.bytes = q.counters + up(q.units * 4);
+    return q;
+}
+
+template <typename C> int run_product(const CUtensorMap& mw, const CUtensorMap& mx, const Product& p, cudaStream_t stream) {
+    auto kern = product_kernel<C>;
+    cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::SMEM);
+    return (int)launch_kernel(kern, dim3(p.split.P), dim3(C::THREADS), C::SMEM, stream, mw, mx, p);
 }
 
 }  // namespace mx
 }  // namespace prism
 
-// x [M, K] bfloat16 (row stride ldx); codes, scales: W [N, K]; y [M, N] of `out_dtype` (row stride ldy); act_bits 16 or 4
+// bytes of workspace that prism_mxfp4_linear needs for these sizes, into *bytes
+PRISM_EXPORT int prism_mxfp4_linear_workspace(int M, int N, int K, int act_bits, long long* bytes) {
+    if (M <= 0 || N <= 0 || K <= 0 || (act_bits != 16 && act_bits != 4)) return (int)cudaErrorInvalidValue;
+    const prism::mx::Plan q = prism::mx::plan_for(M, N, K, act_bits);
+    *bytes = q.bytes;
+    return q.units > 0x7fffffffLL ? (int)cudaErrorInvalidValue : 0;
+}
+
+// x [M, K] bfloat16 (row stride ldx); codes, scales: W [N, K]; y [M, N] of `out_dtype` (row stride ldy); act_bits 16 or 4;
+// ws: workspace of the call (prism_mxfp4_linear_workspace), 1024-byte aligned
 PRISM_EXPORT int prism_mxfp4_linear(const void* x, long long ldx, const void* codes, const void* scales, const void* bias, int bias_dtype,
-                                    void* y, int out_dtype, long long ldy, int M, int N, int K, int act_bits, cudaStream_t stream) {
+                                    void* y, int out_dtype, long long ldy, int M, int N, int K, int act_bits, void* ws, int* err,
+                                    cudaStream_t stream) {
     using namespace prism;
+    using namespace prism::mx;
     if (M <= 0 || N <= 0) return 0;
-    if (K <= 0 || (act_bits != 16 && act_bits != 4) || ((uintptr_t)codes & 31)) return (int)cudaErrorInvalidValue;
-    const dim3 grid((N + mx::TN - 1) / mx::TN, (M + mx::TM - 1) / mx::TM), block(256);
-    const uint8_t *c = static_cast<const uint8_t*>(codes), *s = static_cast<const uint8_t*>(scales);
+    if (K <= 0 || (act_bits != 16 && act_bits != 4) || ((uintptr_t)codes & 31) || ((uintptr_t)scales & 15) || ((uintptr_t)ws & 255))
+        return (int)cudaErrorInvalidValue;
+    const Plan q = plan_for(M, N, K, act_bits);
+    if (q.units > 0x7fffffffLL) return (int)cudaErrorInvalidValue;
+    uint8_t* base = static_cast<uint8_t*>(ws);
+    const bool a16 = act_bits == 16;
+    const int xr = a16 ? 2 * q.tt : q.tt;
+    CUtensorMap mw, mx;
+    int rc = byte_map(&mw, codes, N, (long long)q.groups * (GROUP / 2), 128, a16);
+    if (rc) return rc;
+    rc = a16 ? byte_map(&mx, base + q.codes, (long long)q.mtiles * xr, (long long)q.groups * GROUP, xr, false)
+             : byte_map(&mx, base + q.codes, M, (long long)q.groups * (GROUP / 2), xr, false);
+    if (rc) return rc;
+    Product p;
+    p.w_scales = static_cast<const uint8_t*>(scales);
+    p.x_scales = base + q.scales;
+    p.bias = bias;
+    p.y = y;
+    p.part = reinterpret_cast<float*>(base + q.parts);
+    p.counters = reinterpret_cast<int*>(base + q.counters);
+    p.err = err;
+    p.ldy = ldy;
+    p.split = Split{q.units * q.kb, q.P, q.kb};
+    p.M = M, p.N = N, p.groups = q.groups, p.mtiles = q.mtiles, p.ntiles = q.ntiles;
+    p.bias_bf16 = bias_dtype == PRISM_DTYPE_BF16, p.out_bf16 = out_dtype == PRISM_DTYPE_BF16;
+    const long long threads = (long long)M * q.groups * 16, most = threads > q.units ? threads : q.units;
+    const int blocks = (int)((most + 255) / 256 < 148 * 8 ? (most + 255) / 256 : 148 * 8);
+    const int wide = ((uintptr_t)x & 15) == 0 && ldx % 8 == 0;
     const __nv_bfloat16* xb = static_cast<const __nv_bfloat16*>(x);
-    const int groups = mx::groups_of(K), bb = bias_dtype == PRISM_DTYPE_BF16, four = act_bits == 4;
-    if (out_dtype == PRISM_DTYPE_BF16)
-        return (int)launch_kernel(mx::linear_kernel<__nv_bfloat16>, grid, block, 0, stream, xb, ldx, c, s, bias, bb,
-                                  static_cast<__nv_bfloat16*>(y), ldy, M, N, K, groups, four);
-    return (int)launch_kernel(mx::linear_kernel<float>, grid, block, 0, stream, xb, ldx, c, s, bias, bb, static_cast<float*>(y), ldy, M, N, K,
-                              groups, four);
+    rc = (int)launch_kernel(a16 ? prepare_kernel<true> : prepare_kernel<false>, dim3(blocks), dim3(256), 0, stream, xb, ldx, M, K, q.groups, wide,
+                            q.tt, base + q.codes, base + q.scales, p.counters, (int)q.units);
+    if (rc) return rc;
+    if (a16) {
+        switch (q.tt) {
+            case 8: return run_product<Cfg<true, 8, 1>>(mw, mx, p, stream);
+            case 16: return run_product<Cfg<true, 16, 1>>(mw, mx, p, stream);
+            case 32: return run_product<Cfg<true, 32, 2>>(mw, mx, p, stream);
+            case 64: return run_product<Cfg<true, 64, 2>>(mw, mx, p, stream);
+            default: return run_product<Cfg<true, 128, 2>>(mw, mx, p, stream);
+        }
+    }
+    switch (q.tt) {
+        case 16: return run_product<Cfg<false, 16, 1>>(mw, mx, p, stream);
+        case 32: return run_product<Cfg<false, 32, 2>>(mw, mx, p, stream);
+        case 64: return run_product<Cfg<false, 64, 2>>(mw, mx, p, stream);
+        default: return run_product<Cfg<false, 128, 2>>(mw, mx, p, stream);
+    }
 }

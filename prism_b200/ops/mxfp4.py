@@ -11,6 +11,7 @@ file, engine/weight_pool.py:46-70).
 
 from __future__ import annotations
 
+import ctypes
 from typing import Optional
 
 import torch
@@ -90,6 +91,19 @@ def mxfp4_quantize(x: torch.Tensor) -> Mxfp4:
     return Mxfp4(codes, scales, K)
 
 
+_workspace_bytes = {}
+
+
+def _linear_workspace(M: int, N: int, K: int, act_bits: int) -> int:
+    key = (M, N, K, act_bits)
+    n = _workspace_bytes.get(key)
+    if n is None:
+        b = ctypes.c_longlong()
+        _need(ops.lib().prism_mxfp4_linear_workspace(M, N, K, act_bits, ctypes.addressof(b)) == 0, f"a product of {M} x {N} x {K} is not supported")
+        n = _workspace_bytes[key] = b.value
+    return n
+
+
 def mxfp4_linear(x: torch.Tensor, w: Mxfp4, bias: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
                  out_dtype: Optional[torch.dtype] = None, act_bits: int = 16) -> torch.Tensor:
     """``x @ w.T + bias`` for ``x [M, K]`` in bfloat16 (rows may have a stride of their own) and ``w [N, K]`` in 4 bits, sums
@@ -106,9 +120,12 @@ def mxfp4_linear(x: torch.Tensor, w: Mxfp4, bias: Optional[torch.Tensor] = None,
     if out is None:
         out = torch.empty((M, N), dtype=out_dtype or torch.bfloat16, device=x.device)
     _need(out.shape == (M, N) and (out.stride(1) == 1 or N == 1) and out_dtype in (None, out.dtype), "out does not fit the product")
+    if M == 0:
+        return out
+    ws = torch.empty(_linear_workspace(M, N, K, act_bits), dtype=torch.uint8, device=x.device)
     ops._check(ops.lib().prism_mxfp4_linear(x.data_ptr(), x.stride(0), w.codes.data_ptr(), w.scales.data_ptr(), ops._ptr(bias),
                                             ops.F32 if bias is None else ops._dt(bias), out.data_ptr(), ops._dt(out), out.stride(0), M, N, K,
-                                            act_bits, ops._stream()), "mxfp4_linear")
+                                            act_bits, ws.data_ptr(), ops._tc_err_word(x.device).data_ptr(), ops._stream()), "mxfp4_linear")
     return out
 
 
