@@ -20,34 +20,13 @@
 // added up by the one that comes last, in the order of the CTAs: results do not depend on timing.
 //
 // Every wait is bounded (tcgen05.cuh); on expiry the kernel sets the error word, frees tensor memory and returns.
-#include "mxfp4.cuh"
-#include "tcgen05.cuh"
+#include "mxfp4_mma.cuh"
 #include "vec.cuh"
 
 namespace prism {
 namespace mx {
 
-using tc::mbar_expect_tx;
-using tc::mbar_init;
-using tc::mbar_wait;
-using tc::smem_addr;
-using tc::tma_load_2d;
-using tc::tmem_load;
-using tc::umma_commit;
-using tc::umma_desc;
-
 // ---- x to terms or codes ------------------------------------------------------------------------------------------------
-
-__device__ __forceinline__ uint32_t pack_e4m3(float lo, float hi) {
-    uint16_t r;
-    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %2, %1;" : "=h"(r) : "f"(lo), "f"(hi));
-    return r;
-}
-__device__ __forceinline__ void unpack_e4m3(uint32_t p, float& lo, float& hi) {
-    uint32_t h;
-    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((uint16_t)p));
-    asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.f32.f16 %0, a;\n\tcvt.f32.f16 %1, b;\n\t}" : "=f"(lo), "=f"(hi) : "r"(h));
-}
 
 // act 16: terms uint8 [token tile][2 tt][Kp], a tile's hi rows, then its lo rows; scales [token tile][groups][atoms][512],
 // the tiles of 128 such rows.  act 4: codes and scales as in mxfp4.cuh.  Rows that have no token are left as they are.
@@ -78,22 +57,10 @@ __global__ void __launch_bounds__(256) prepare_kernel(const __nv_bfloat16* __res
         const uint32_t four = 0xfu << (threadIdx.x & 28);
         most = max(most, __shfl_xor_sync(four, most, 1));
         most = max(most, __shfl_xor_sync(four, most, 2));
-        const bool bad = most >= 0x7f800000u;
         if (A16) {
-            const int byte = max((int)(most >> 23) - 7, 5), lines = 2 * tt, atoms = (lines + 127) / 128;
-            const float f = __uint_as_float((uint32_t)(254 - byte) << 23);
-            uint32_t hi[2] = {0, 0}, lo[2] = {0, 0};
-            if (!bad) {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const float a = v[2 * j] * f, b = v[2 * j + 1] * f;
-                    const uint32_t h = pack_e4m3(a, b);
-                    float ha, hb;
-                    unpack_e4m3(h, ha, hb);
-                    hi[j / 2] |= h << (16 * (j & 1));
-                    lo[j / 2] |= pack_e4m3((a - ha) * 32.f, (b - hb) * 32.f) << (16 * (j & 1));
-                }
-            }
+            const int byte = term_byte(most), lines = 2 * tt, atoms = (lines + 127) / 128;
+            uint32_t hi[2], lo[2];
+            terms_of<8>(v, byte, hi, lo);
             const int tile = r / tt, t = r - tile * tt;
             uint8_t* at = codes + ((size_t)tile * lines + t) * ((size_t)groups * GROUP) + c;
             *reinterpret_cast<uint2*>(at) = make_uint2(hi[0], hi[1]);
@@ -101,14 +68,14 @@ __global__ void __launch_bounds__(256) prepare_kernel(const __nv_bfloat16* __res
             if ((threadIdx.x & 3) == 0) {
                 uint8_t* s = scales + ((size_t)tile * groups + c / GROUP) * (atoms * TILE_BYTES) + c % GROUP / BLOCK;
                 const int u = t + tt;
-                s[t / 128 * TILE_BYTES + (t & 31) * 16 + (t & 127) / 32 * 4] = bad ? 255 : (uint8_t)byte;
-                s[u / 128 * TILE_BYTES + (u & 31) * 16 + (u & 127) / 32 * 4] = bad ? 255 : (uint8_t)(byte - 5);
+                s[t / 128 * TILE_BYTES + (t & 31) * 16 + (t & 127) / 32 * 4] = (uint8_t)byte;
+                s[u / 128 * TILE_BYTES + (u & 31) * 16 + (u & 127) / 32 * 4] = low_byte(byte);
             }
         } else {
             const int byte = scale_byte(most);
             const float inv = scale_inverse(byte);
             uint32_t word = 0;
-            if (!bad)
+            if (byte != 255)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) word |= pack2(v[2 * j] * inv, v[2 * j + 1] * inv) << (8 * j);
             *reinterpret_cast<uint32_t*>(codes + (size_t)r * (groups * (GROUP / 2)) + c / 2) = word;
@@ -142,35 +109,6 @@ template <bool A16_, int TT_, int W_> struct Cfg {
     static_assert(COLS_USED <= 512 && STAGES >= 3, "tensor memory or shared memory");
 };
 
-struct Split {                 // how the blocks are dealt: CTA c has the blocks [c total / P, (c + 1) total / P)
-    long long total;
-    int P, kb;                 // CTAs; stages of K of a unit
-    __device__ __forceinline__ long long start(int c) const { return (long long)c * total / P; }
-    __device__ __forceinline__ int owner(long long b) const { return (int)(((b + 1) * P - 1) / total); }
-};
-
-__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-                 ::"r"(smem_addr(dst)), "l"(src), "r"(bytes), "r"(smem_addr(bar)) : "memory");
-}
-// 512 bytes of scales, 32 rows of 16 without swizzle, to four columns of tensor memory, the same in every quarter of its lanes
-__device__ __forceinline__ void scales_to_tmem(uint32_t taddr, uint32_t saddr) {
-    const uint64_t d = (uint64_t)((saddr >> 4) & 0x3FFF) | (uint64_t)8 << 32 | (uint64_t)1 << 46;
-    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(d) : "memory");
-}
-template <bool A16>
-__device__ __forceinline__ void umma_scaled(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb, uint32_t accumulate) {
-    if (A16)
-        asm volatile(
-            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
-            "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
-            ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate) : "memory");
-    else
-        asm volatile(
-            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
-            "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
-            ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate) : "memory");
-}
 // Instruction descriptor: element kinds (mxf8f6f4: A E2M1 = 5, B E4M3 = 0; mxf4: E2M1 = 1 on both sides), N / 8, scales E8M0,
 // M / 128; `id`: which byte of a scale column the instruction begins at.
 template <typename C> __device__ __forceinline__ constexpr uint32_t idesc_of(int id) {
@@ -388,28 +326,6 @@ product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
 }
 
 // ---- host side ----------------------------------------------------------------------------------------------------------
-
-// a matrix of bytes (or of 4-bit codes that TMA spreads to a byte each: `spread`, 128 of them a box row), boxes of 128 bytes in shared memory
-inline int byte_map(CUtensorMap* map, const void* ptr, long long rows, long long row_bytes, int box_rows, bool spread) {
-    tc::EncodeTiledFn fn = tc::encode_fn();
-    if (fn == nullptr) return (int)cudaErrorNotSupported;
-    cuuint64_t dims[2] = {(cuuint64_t)(spread ? row_bytes * 2 : row_bytes), (cuuint64_t)rows};
-    cuuint64_t strides[1] = {(cuuint64_t)row_bytes};
-    cuuint32_t box[2] = {128, (cuuint32_t)box_rows}, estr[2] = {1, 1};
-    CUresult r = fn(map, spread ? CU_TENSOR_MAP_DATA_TYPE_16U4_ALIGN16B : CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(ptr), dims, strides, box,
-                    estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    return r == CUDA_SUCCESS ? 0 : (int)cudaErrorInvalidValue;
-}
-
-inline int sm_count() {
-    static int n[64] = {};
-    int dev = 0;
-    cudaGetDevice(&dev);
-    if (dev < 0 || dev >= 64) return 148;
-    if (!n[dev]) cudaDeviceGetAttribute(&n[dev], cudaDevAttrMultiProcessorCount, dev);
-    return n[dev];
-}
 
 // tokens of a tile and tiles of W that share one
 inline void tiles_for(int M, int act_bits, int& tt, int& w) {

@@ -1,0 +1,112 @@
+// Block-scaled tensor-core products of 4-bit codes (tcgen05.mma kind::mxf4, kind::mxf8f6f4): two 8-bit terms that hold a 16-bit
+// value, scales on their way to tensor memory, how a product's blocks are dealt to CTAs, tensor maps.
+#pragma once
+
+#include "mxfp4.cuh"
+#include "tcgen05.cuh"
+
+namespace prism {
+namespace mx {
+
+using tc::mbar_expect_tx;
+using tc::mbar_init;
+using tc::mbar_wait;
+using tc::smem_addr;
+using tc::tma_load_2d;
+using tc::tmem_load;
+using tc::umma_commit;
+using tc::umma_desc;
+
+// ---- a bfloat16 value as two E4M3 terms: x = 2^(byte - 127) (hi + 2^-5 lo) -----------------------------------------------
+// The byte of a block of 32 from the bits of its largest magnitude: values scaled to below 256; at least 5, so that the low
+// terms' byte, 5 less, exists; 255 (both) for a block with an infinity or NaN.
+
+__device__ __forceinline__ uint32_t pack_e4m3(float lo, float hi) {
+    uint16_t r;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %2, %1;" : "=h"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ void unpack_e4m3(uint32_t p, float& lo, float& hi) {
+    uint32_t h;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((uint16_t)p));
+    asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.f32.f16 %0, a;\n\tcvt.f32.f16 %1, b;\n\t}" : "=f"(lo), "=f"(hi) : "r"(h));
+}
+
+__device__ __forceinline__ int term_byte(uint32_t most) { return most >= 0x7f800000u ? 255 : max((int)(most >> 23) - 7, 5); }
+__device__ __forceinline__ uint8_t low_byte(int byte) { return (uint8_t)(byte == 255 ? 255 : byte - 5); }
+// N values (N a multiple of 4) as N bytes of high and N of low terms
+template <int N> __device__ __forceinline__ void terms_of(const float (&v)[N], int byte, uint32_t (&hi)[N / 4], uint32_t (&lo)[N / 4]) {
+    const float f = byte == 255 ? 0.f : __uint_as_float((uint32_t)(254 - byte) << 23);
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i) {
+        hi[i] = lo[i] = 0;
+        if (byte == 255) continue;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const float a = v[4 * i + 2 * j] * f, b = v[4 * i + 2 * j + 1] * f;
+            const uint32_t h = pack_e4m3(a, b);
+            float ha, hb;
+            unpack_e4m3(h, ha, hb);
+            hi[i] |= h << (16 * j);
+            lo[i] |= pack_e4m3((a - ha) * 32.f, (b - hb) * 32.f) << (16 * j);
+        }
+    }
+}
+
+// ---- pieces of the products -----------------------------------------------------------------------------------------------
+
+struct Split {                 // how the blocks are dealt: CTA c has the blocks [c total / P, (c + 1) total / P)
+    long long total;
+    int P, kb;                 // CTAs; stages of K of a unit
+    __device__ __forceinline__ long long start(int c) const { return (long long)c * total / P; }
+    __device__ __forceinline__ int owner(long long b) const { return (int)(((b + 1) * P - 1) / total); }
+};
+
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 ::"r"(smem_addr(dst)), "l"(src), "r"(bytes), "r"(smem_addr(bar)) : "memory");
+}
+// 512 bytes of scales, 32 rows of 16 without swizzle, to four columns of tensor memory, the same in every quarter of its lanes
+__device__ __forceinline__ void scales_to_tmem(uint32_t taddr, uint32_t saddr) {
+    const uint64_t d = (uint64_t)((saddr >> 4) & 0x3FFF) | (uint64_t)8 << 32 | (uint64_t)1 << 46;
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(d) : "memory");
+}
+template <bool A16>
+__device__ __forceinline__ void umma_scaled(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb, uint32_t accumulate) {
+    if (A16)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+            ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate) : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+            ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate) : "memory");
+}
+// ---- host side ------------------------------------------------------------------------------------------------------------
+
+// a matrix of bytes (or of 4-bit codes that TMA spreads to a byte each: `spread`, 128 of them a box row), boxes of 128 bytes in shared memory
+inline int byte_map(CUtensorMap* map, const void* ptr, long long rows, long long row_bytes, int box_rows, bool spread) {
+    tc::EncodeTiledFn fn = tc::encode_fn();
+    if (fn == nullptr) return (int)cudaErrorNotSupported;
+    cuuint64_t dims[2] = {(cuuint64_t)(spread ? row_bytes * 2 : row_bytes), (cuuint64_t)rows};
+    cuuint64_t strides[1] = {(cuuint64_t)row_bytes};
+    cuuint32_t box[2] = {128, (cuuint32_t)box_rows}, estr[2] = {1, 1};
+    CUresult r = fn(map, spread ? CU_TENSOR_MAP_DATA_TYPE_16U4_ALIGN16B : CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(ptr), dims, strides, box,
+                    estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? 0 : (int)cudaErrorInvalidValue;
+}
+
+inline int sm_count() {
+    static int n[64] = {};
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev < 0 || dev >= 64) return 148;
+    if (!n[dev]) cudaDeviceGetAttribute(&n[dev], cudaDevAttrMultiProcessorCount, dev);
+    return n[dev];
+}
+
+}  // namespace mx
+}  // namespace prism

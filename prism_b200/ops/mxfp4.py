@@ -19,7 +19,7 @@ import torch
 from .. import ops
 
 BLOCK, GROUP, TILE_ROWS, TILE_BYTES = 32, 128, 128, 512      # csrc/mxfp4.cuh
-MOE_TOKENS = 64                                              # the most tokens of an ``mxfp4_moe`` call
+MOE_TOKENS, MOE_EXPERTS, MOE_TOP = 64, 256, 16               # the most of an ``mxfp4_moe`` call
 DTYPE = "mxfp4"
 
 
@@ -94,14 +94,30 @@ def mxfp4_quantize(x: torch.Tensor) -> Mxfp4:
 _workspace_bytes = {}
 
 
-def _linear_workspace(M: int, N: int, K: int, act_bits: int) -> int:
-    key = (M, N, K, act_bits)
-    n = _workspace_bytes.get(key)
+def _workspace(size_of: str, *sizes: int) -> int:
+    n = _workspace_bytes.get((size_of,) + sizes)
     if n is None:
         b = ctypes.c_longlong()
-        _need(ops.lib().prism_mxfp4_linear_workspace(M, N, K, act_bits, ctypes.addressof(b)) == 0, f"a product of {M} x {N} x {K} is not supported")
-        n = _workspace_bytes[key] = b.value
+        if getattr(ops.lib(), size_of)(*sizes, ctypes.addressof(b)) != 0:
+            raise ops.KernelError(f"{size_of}: sizes {sizes} are not supported")
+        n = _workspace_bytes[(size_of,) + sizes] = b.value
     return n
+
+
+_control_blocks = {}
+
+
+def _control(stream: int, device: torch.device) -> torch.Tensor:
+    """The counters that the experts' launch synchronises with and leaves at zero: a block of its own for each stream, as
+    launches of one stream follow each other; under graph capture one for the call, cleared by the graph, as graphs may run on
+    any stream."""
+    if torch.cuda.is_current_stream_capturing():
+        return torch.zeros(66, dtype=torch.int32, device=device)
+    key = (device.index, stream)
+    block = _control_blocks.get(key)
+    if block is None:
+        block = _control_blocks[key] = torch.zeros(66, dtype=torch.int32, device=device)
+    return block
 
 
 def mxfp4_linear(x: torch.Tensor, w: Mxfp4, bias: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
@@ -122,7 +138,7 @@ def mxfp4_linear(x: torch.Tensor, w: Mxfp4, bias: Optional[torch.Tensor] = None,
     _need(out.shape == (M, N) and (out.stride(1) == 1 or N == 1) and out_dtype in (None, out.dtype), "out does not fit the product")
     if M == 0:
         return out
-    ws = torch.empty(_linear_workspace(M, N, K, act_bits), dtype=torch.uint8, device=x.device)
+    ws = torch.empty(_workspace("prism_mxfp4_linear_workspace", M, N, K, act_bits), dtype=torch.uint8, device=x.device)
     ops._check(ops.lib().prism_mxfp4_linear(x.data_ptr(), x.stride(0), w.codes.data_ptr(), w.scales.data_ptr(), ops._ptr(bias),
                                             ops.F32 if bias is None else ops._dt(bias), out.data_ptr(), ops._dt(out), out.stride(0), M, N, K,
                                             act_bits, ws.data_ptr(), ops._tc_err_word(x.device).data_ptr(), ops._stream()), "mxfp4_linear")
@@ -133,7 +149,7 @@ def mxfp4_moe(x: torch.Tensor, router: torch.Tensor, gate: Mxfp4, up: Mxfp4, dow
               renorm: bool = False, scale_input: bool = True, act: str = "silu", limit: float = 0.0,
               router_bias: Optional[torch.Tensor] = None, choice: Optional["ops.MoeChoice"] = None, out: Optional[torch.Tensor] = None,
               out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
-    """A mixture-of-experts layer for up to 64 tokens: ``x [T, H]`` bfloat16, ``router [E, H]`` (logits in float32),
+    """A mixture-of-experts layer for up to 64 tokens, up to 256 experts and up to 16 of them a token, in one launch: ``x [T, H]`` bfloat16, ``router [E, H]`` (logits in float32),
     ``gate``, ``up`` ``[E, F, H]`` and ``down`` ``[E, H, F]`` in 4 bits.  Each token takes the ``top`` experts with the largest
     scores (sigmoid of the logits, or their softmax; the lower index of equal ones); a choice's weight is its score
     (``renorm``: over the sum of the chosen) and multiplies the expert's input (``scale_input``) or its output.  ``act``:
@@ -146,7 +162,7 @@ def mxfp4_moe(x: torch.Tensor, router: torch.Tensor, gate: Mxfp4, up: Mxfp4, dow
     _need(E > 0 and gate.shape == (E, F, H) and up.shape == gate.shape and down.shape == (E, H, F),
           f"experts {tuple(gate.shape)}, {tuple(up.shape)}, {tuple(down.shape)} do not belong together or to rows of {H}")
     _need(T <= MOE_TOKENS, f"{T} tokens: this layer is for up to {MOE_TOKENS}")
-    _need(1 <= top <= E, f"a token uses {top} of {E} experts: between 1 and all of them")
+    _need(1 <= top <= min(E, MOE_TOP) and E <= MOE_EXPERTS, f"a token uses {top} of {E} experts: up to {MOE_TOP} of up to {MOE_EXPERTS}")
     _need(router.shape == (E, H) and router.is_contiguous() and (router_bias is None or (router_bias.shape == (E,) and router_bias.is_contiguous())),
           "the router has one row (and one bias) per expert")
     _need(act in ops.GATED, f"a gated feed-forward's activation is one of {ops.GATED}, got {act!r}")
@@ -158,13 +174,16 @@ def mxfp4_moe(x: torch.Tensor, router: torch.Tensor, gate: Mxfp4, up: Mxfp4, dow
     if out is None:
         out = torch.empty((T, H), dtype=out_dtype or torch.bfloat16, device=x.device)
     _need(out.shape == (T, H) and out.stride(1) == 1 and out_dtype in (None, out.dtype), "out does not fit the layer")
-    sel_e = torch.empty(T * top, dtype=torch.int32, device=x.device)
-    scratch = torch.empty(T * top * (F + 1), dtype=torch.float32, device=x.device)
+    if T == 0:
+        return out
+    stream = ops._stream()
+    ws = torch.empty(_workspace("prism_mxfp4_moe_workspace", T, H, F, E, top), dtype=torch.uint8, device=x.device)
+    control = _control(stream, x.device)
     ops._check(ops.lib().prism_mxfp4_moe(x.data_ptr(), x.stride(0), router.data_ptr(), ops._dt(router), ops._ptr(router_bias),
                                          ops.F32 if router_bias is None else ops._dt(router_bias), gate.codes.data_ptr(), gate.scales.data_ptr(),
                                          up.codes.data_ptr(), up.scales.data_ptr(), down.codes.data_ptr(), down.scales.data_ptr(), T, H, F, E,
                                          top, int(softmax), int(renorm), int(scale_input), ops.MOE_ACTS[act], float(limit),
                                          ops._ptr(ch.correction), ops.F32 if ch.correction is None else ops._dt(ch.correction), ch.groups, ch.keep,
-                                         ch.scale, ch.sum_eps, out.data_ptr(), ops._dt(out), out.stride(0), sel_e.data_ptr(),
-                                         scratch.data_ptr(), scratch.data_ptr() + 4 * T * top, ops._stream()), "mxfp4_moe")
+                                         ch.scale, ch.sum_eps, out.data_ptr(), ops._dt(out), out.stride(0), ws.data_ptr(), control.data_ptr(),
+                                         ops._tc_err_word(x.device).data_ptr(), stream), "mxfp4_moe")
     return out

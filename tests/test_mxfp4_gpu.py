@@ -357,7 +357,7 @@ def test_refusals():
     bad += [
         moe(x, router[:3], gate, up, down, 2), moe(x, router, gate, up, down, 0), moe(x, router, gate, up, down, 5),
         moe(x, router, gate, down, down, 2), moe(x, router, gate, up, up, 2), moe(x, router, gate[0], up[0], down[0], 1),
-        moe(x[:, :100], router, gate, up, down, 2), moe(x.float(), router, gate, up, down, 2), moe(x, router, gate, up, down, 2, act="relu"),
+        moe(x, router, gate, up, down, 2, choice=ops.MoeChoice(None, 4, 1)), moe(x[:, :100], router, gate, up, down, 2), moe(x.float(), router, gate, up, down, 2), moe(x, router, gate, up, down, 2, act="relu"),
         moe(_acts(65, 200, 1), router, gate, up, down, 2), moe(x, router, gate, up, down, 2, choice=ops.MoeChoice(None, 3, 1)),
     ]
     for i, call in enumerate(bad):
