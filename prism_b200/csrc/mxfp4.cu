@@ -1,117 +1,142 @@
 // Rows to microscaled 4-bit floating point and back (mxfp4.cuh has the format).
 //
-// Bound by memory: 2 or 4 bytes read and 17/32 written an element, and back.  Four neighbouring threads share a block of 32:
-// each takes 8 values in one or two wide loads, the largest magnitude goes round by two shuffles, and each stores its 8 codes
-// as one word; a warp reads 512 consecutive bytes of a bfloat16 row and writes 128.
+// Bound by memory: 2 or 4 bytes read and 17/32 written an element, and back.  A CTA has one tile of scales, 128 rows by 128
+// columns: 16 threads share a row's 256 bytes (bfloat16), each with 8 values in one or two wide loads; all of a thread's rows
+// are asked for before the first is worked on.  Four neighbours share a block of 32: its largest magnitude goes round by two
+// shuffles, each stores its 8 codes as one word, and the tile's 512 scale bytes leave together through shared memory.
 #include "mxfp4.cuh"
 #include "vec.cuh"
 
 namespace prism {
 namespace mx {
 
-// x [rows, K] (row stride ld); rows_each: rows of one matrix of a stack, whose scales start at a tile of their own
+constexpr int THREADS = 256, AT_ONCE = 8, ROWS = THREADS / 16;      // rows of a round of the CTA
+
+__device__ __forceinline__ int scale_place(int r) { return (r & 31) * 16 + r / 32 * 4; }       // of row r of a tile, block 0
+
+// x: a stack of matrices [rows, K] (row stride ld); grid (groups, tiles of rows, matrices)
 template <typename T>
-__global__ void quantise_kernel(const T* __restrict__ x_in, long long ld, int rows, int rows_each, int K, int groups, int wide,
-                                uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
+__global__ void __launch_bounds__(THREADS) quantise_kernel(const T* __restrict__ x_in, long long ld, int rows, int K, int groups, int wide,
+                                                           uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
+    __shared__ __align__(16) uint8_t sc[TILE_BYTES];
     pdl_wait();
     pdl_trigger();
-    const T* x = pdl_fresh(x_in);
-    const int per_row = groups * (GROUP / 8);
-    const long long total = (long long)rows * per_row;
-    const size_t tiles_each = (size_t)((rows_each + TILE_ROWS - 1) / TILE_ROWS) * groups * TILE_BYTES;
-    for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (long long)gridDim.x * blockDim.x) {
-        // total is a multiple of 16 and threads of a block's four are neighbours: all four are here or none
-        const int r = (int)(i / per_row), c = (int)(i - (long long)r * per_row) * 8;
-        const T* p = x + (long long)r * ld + c;
-        float v[8];
-        if (wide && c + 8 <= K) {
-            load8(p, v);
-        } else {
+    const int g = blockIdx.x, r0 = blockIdx.y * TILE_ROWS, c = (threadIdx.x & 15) * 8, k = g * GROUP + c, first = threadIdx.x >> 4;
+    const size_t row0 = (size_t)blockIdx.z * rows + r0;
+    const T* x = pdl_fresh(x_in) + (long long)row0 * ld + k;
+    uint8_t* code = codes + row0 * (groups * (size_t)(GROUP / 2)) + k / 2;
+    const int here = min(TILE_ROWS, rows - r0);
+    for (int base = 0; base < here; base += ROWS * AT_ONCE) {
+        float v[AT_ONCE][8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = c + j < K ? to_float(p[j]) : 0.f;
+        for (int i = 0; i < AT_ONCE; ++i) {
+            const int r = base + i * ROWS + first;
+            const T* p = x + (long long)r * ld;
+            if (wide && r < here && k + 8 <= K) {
+                load8(p, v[i]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[i][j] = r < here && k + j < K ? to_float(p[j]) : 0.f;
+            }
         }
-        uint32_t most = 0;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) most = max(most, __float_as_uint(v[j]) & 0x7fffffffu);
-        const uint32_t four = 0xfu << (threadIdx.x & 28);
-        most = max(most, __shfl_xor_sync(four, most, 1));
-        most = max(most, __shfl_xor_sync(four, most, 2));
-        const int byte = scale_byte(most);
-        const float inv = byte == 255 ? 0.f : scale_inverse(byte);
-        uint32_t word = 0;
-        if (byte != 255)
+        for (int i = 0; i < AT_ONCE; ++i) {
+            const int r = base + i * ROWS + first;
+            uint32_t most = 0;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) word |= pack2(v[2 * j] * inv, v[2 * j + 1] * inv) << (8 * j);
-        *reinterpret_cast<uint32_t*>(codes + (size_t)r * (groups * (GROUP / 2)) + c / 2) = word;
-        if ((threadIdx.x & 3) == 0) {
-            const int m = r / rows_each;
-            scales[m * tiles_each + scale_at(r - m * rows_each, c / BLOCK, groups)] = (uint8_t)byte;
+            for (int j = 0; j < 8; ++j) most = max(most, __float_as_uint(v[i][j]) & 0x7fffffffu);
+            most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+            most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
+            const int byte = scale_byte(most);
+            const float inv = scale_inverse(byte);
+            uint32_t word = 0;
+            if (byte != 255)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) word |= pack2(v[i][2 * j] * inv, v[i][2 * j + 1] * inv) << (8 * j);
+            if (r < here) {
+                *reinterpret_cast<uint32_t*>(code + (size_t)r * (groups * (GROUP / 2))) = word;
+                if ((threadIdx.x & 3) == 0) sc[scale_place(r) + c / BLOCK] = (uint8_t)byte;
+            }
         }
     }
+    __syncthreads();
+    if (threadIdx.x < 32)
+        reinterpret_cast<uint4*>(scales + (((size_t)blockIdx.z * gridDim.y + blockIdx.y) * groups + g) * TILE_BYTES)[threadIdx.x] =
+            reinterpret_cast<const uint4*>(sc)[threadIdx.x];
 }
 
 template <typename T>
-__global__ void dequantise_kernel(const uint8_t* __restrict__ codes_in, const uint8_t* __restrict__ scales_in, int rows, int rows_each,
-                                  int K, int groups, T* __restrict__ out) {
+__global__ void __launch_bounds__(THREADS) dequantise_kernel(const uint8_t* __restrict__ codes_in, const uint8_t* __restrict__ scales_in, int rows,
+                                                             int K, int groups, T* __restrict__ out) {
+    __shared__ __align__(16) uint8_t sc[TILE_BYTES];
     pdl_wait();
     pdl_trigger();
-    const uint8_t *codes = pdl_fresh(codes_in), *scales = pdl_fresh(scales_in);
-    const int per_row = (K + 7) / 8;
-    const long long total = (long long)rows * per_row;
-    const size_t tiles_each = (size_t)((rows_each + TILE_ROWS - 1) / TILE_ROWS) * groups * TILE_BYTES;
-    for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (long long)gridDim.x * blockDim.x) {
-        const int r = (int)(i / per_row), c = (int)(i - (long long)r * per_row) * 8;
-        const uint32_t word = *reinterpret_cast<const uint32_t*>(codes + (size_t)r * (groups * (GROUP / 2)) + c / 2);
-        const int m = r / rows_each;
-        const float s = scale_value(scales[m * tiles_each + scale_at(r - m * rows_each, c / BLOCK, groups)]);
+    const int g = blockIdx.x, r0 = blockIdx.y * TILE_ROWS, c = (threadIdx.x & 15) * 8, k = g * GROUP + c, first = threadIdx.x >> 4;
+    const size_t row0 = (size_t)blockIdx.z * rows + r0;
+    const uint8_t* code = pdl_fresh(codes_in) + row0 * (groups * (size_t)(GROUP / 2)) + k / 2;
+    const int here = min(TILE_ROWS, rows - r0);
+    uint32_t word[AT_ONCE];
+    static_assert(ROWS * AT_ONCE == TILE_ROWS, "one round");
+#pragma unroll
+    for (int i = 0; i < AT_ONCE; ++i) {
+        const int r = i * ROWS + first;
+        word[i] = r < here ? *reinterpret_cast<const uint32_t*>(code + (size_t)r * (groups * (GROUP / 2))) : 0;
+    }
+    if (threadIdx.x < 32)
+        reinterpret_cast<uint4*>(sc)[threadIdx.x] =
+            reinterpret_cast<const uint4*>(pdl_fresh(scales_in) + (((size_t)blockIdx.z * gridDim.y + blockIdx.y) * groups + g) * TILE_BYTES)[threadIdx.x];
+    __syncthreads();
+    if (k >= K) return;
+#pragma unroll
+    for (int i = 0; i < AT_ONCE; ++i) {
+        const int r = i * ROWS + first;
+        if (r >= here) break;
+        const float s = scale_value(sc[scale_place(r) + c / BLOCK]);
         float v[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = element(word >> (4 * j) & 15) * s;
-        T* o = out + (long long)r * K + c;
+        for (int j = 0; j < 4; ++j) {
+            const float2 e = elements2(word[i] >> (8 * j));
+            v[2 * j] = e.x * s;
+            v[2 * j + 1] = e.y * s;
+        }
+        T* o = out + (row0 + r) * (size_t)K + k;
         if (K % 8 == 0) {
             store8(o, v);
         } else {
-            for (int j = 0; j < 8 && c + j < K; ++j) o[j] = from_float<T>(v[j]);
+            for (int j = 0; j < 8 && k + j < K; ++j) o[j] = from_float<T>(v[j]);
         }
     }
-}
-
-inline int blocks_for(long long threads) {
-    const long long b = (threads + 255) / 256;
-    return (int)(b < 148 * 8 ? b : 148 * 8);
 }
 
 }  // namespace mx
 }  // namespace prism
 
-// x [rows, K] of `dtype` (row stride ldx elements) -> codes [rows, Kp / 2], scales; rows: a stack of matrices of rows_each rows
-PRISM_EXPORT int prism_mxfp4_quantize(const void* x, int dtype, long long ldx, int rows, int rows_each, int K, void* codes, void* scales,
+// x: a stack of `matrices` [rows, K] of `dtype` (row stride ldx elements) -> codes [..., rows, Kp / 2], scales
+PRISM_EXPORT int prism_mxfp4_quantize(const void* x, int dtype, long long ldx, int matrices, int rows, int K, void* codes, void* scales,
                                       cudaStream_t stream) {
     using namespace prism;
-    if (rows <= 0 || K <= 0) return 0;
-    if (rows_each <= 0 || rows % rows_each || ((uintptr_t)codes & 15)) return (int)cudaErrorInvalidValue;
-    const int groups = mx::groups_of(K), bf = dtype == PRISM_DTYPE_BF16;
+    if (matrices <= 0 || rows <= 0 || K <= 0) return 0;
+    const int groups = mx::groups_of(K), bf = dtype == PRISM_DTYPE_BF16, tiles = (rows + mx::TILE_ROWS - 1) / mx::TILE_ROWS;
+    if (matrices > 65535 || tiles > 65535 || (((uintptr_t)codes | (uintptr_t)scales) & 15)) return (int)cudaErrorInvalidValue;
     const int wide = ((uintptr_t)x & 15) == 0 && ldx % (bf ? 8 : 4) == 0;
-    const dim3 grid(mx::blocks_for((long long)rows * groups * 16)), block(256);
+    const dim3 grid(groups, tiles, matrices), block(mx::THREADS);
     uint8_t *c = static_cast<uint8_t*>(codes), *s = static_cast<uint8_t*>(scales);
     if (bf)
-        return (int)launch_kernel(mx::quantise_kernel<__nv_bfloat16>, grid, block, 0, stream, static_cast<const __nv_bfloat16*>(x), ldx, rows,
-                                  rows_each, K, groups, wide, c, s);
-    return (int)launch_kernel(mx::quantise_kernel<float>, grid, block, 0, stream, static_cast<const float*>(x), ldx, rows, rows_each, K, groups,
-                              wide, c, s);
+        return (int)launch_kernel(mx::quantise_kernel<__nv_bfloat16>, grid, block, 0, stream, static_cast<const __nv_bfloat16*>(x), ldx, rows, K,
+                                  groups, wide, c, s);
+    return (int)launch_kernel(mx::quantise_kernel<float>, grid, block, 0, stream, static_cast<const float*>(x), ldx, rows, K, groups, wide, c, s);
 }
 
-// the values: out [rows, K] of `dtype`, contiguous, 16-byte aligned
-PRISM_EXPORT int prism_mxfp4_dequantize(const void* codes, const void* scales, int rows, int rows_each, int K, void* out, int dtype,
+// the values: out [..., rows, K] of `dtype`, contiguous, 16-byte aligned
+PRISM_EXPORT int prism_mxfp4_dequantize(const void* codes, const void* scales, int matrices, int rows, int K, void* out, int dtype,
                                         cudaStream_t stream) {
     using namespace prism;
-    if (rows <= 0 || K <= 0) return 0;
-    if (rows_each <= 0 || rows % rows_each || ((uintptr_t)codes & 15) || ((uintptr_t)out & 15)) return (int)cudaErrorInvalidValue;
-    const int groups = mx::groups_of(K);
-    const dim3 grid(mx::blocks_for((long long)rows * ((K + 7) / 8))), block(256);
+    if (matrices <= 0 || rows <= 0 || K <= 0) return 0;
+    const int groups = mx::groups_of(K), tiles = (rows + mx::TILE_ROWS - 1) / mx::TILE_ROWS;
+    if (matrices > 65535 || tiles > 65535 || (((uintptr_t)codes | (uintptr_t)scales | (uintptr_t)out) & 15)) return (int)cudaErrorInvalidValue;
+    const dim3 grid(groups, tiles, matrices), block(mx::THREADS);
     const uint8_t *c = static_cast<const uint8_t*>(codes), *s = static_cast<const uint8_t*>(scales);
     if (dtype == PRISM_DTYPE_BF16)
-        return (int)launch_kernel(mx::dequantise_kernel<__nv_bfloat16>, grid, block, 0, stream, c, s, rows, rows_each, K, groups,
-                                  static_cast<__nv_bfloat16*>(out));
-    return (int)launch_kernel(mx::dequantise_kernel<float>, grid, block, 0, stream, c, s, rows, rows_each, K, groups, static_cast<float*>(out));
+        return (int)launch_kernel(mx::dequantise_kernel<__nv_bfloat16>, grid, block, 0, stream, c, s, rows, K, groups, static_cast<__nv_bfloat16*>(out));
+    return (int)launch_kernel(mx::dequantise_kernel<float>, grid, block, 0, stream, c, s, rows, K, groups, static_cast<float*>(out));
 }

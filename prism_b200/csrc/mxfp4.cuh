@@ -35,11 +35,13 @@ __device__ __forceinline__ float scale_inverse(int byte) { return __uint_as_floa
 __device__ __forceinline__ float scale_value(int byte) {
     return byte == 255 ? __uint_as_float(0x7fffffffu) : byte ? __uint_as_float((uint32_t)byte << 23) : __uint_as_float(0x00400000u);
 }
-// the value of a 4-bit code
-__device__ __forceinline__ float element(uint32_t code) {
-    const uint32_t m = code & 7;
-    const float a = m < 2 ? 0.5f * m : __uint_as_float(((m >> 1) + 126) << 23 | (m & 1) << 22);
-    return code & 8 ? -a : a;
+// the values of a byte's two codes (the low half first), exact in half precision
+__device__ __forceinline__ float2 elements2(uint32_t byte) {
+    uint32_t h;
+    asm("{\n\t.reg .b8 t;\n\tcvt.u8.u32 t, %1;\n\tcvt.rn.f16x2.e2m1x2 %0, t;\n\t}" : "=r"(h) : "r"(byte));
+    float2 v;
+    asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.f32.f16 %0, a;\n\tcvt.f32.f16 %1, b;\n\t}" : "=f"(v.x), "=f"(v.y) : "r"(h));
+    return v;
 }
 // two values to 4 bits each, `lo` in the low half of the byte
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {

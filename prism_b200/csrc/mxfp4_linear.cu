@@ -154,43 +154,51 @@ product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = *tmem_slot, tmem_sf = tmem + C::BUFS * W * C::NCOL;
     volatile int* abortp = &abort_flag;
-    const long long b0 = p.split.start(cta), b1 = p.split.start(cta + 1);
-    const int n = (int)(b1 - b0), kb = p.split.kb;
+    const int b0 = p.split.start(cta), n = p.split.start(cta + 1) - b0, kb = p.split.kb;
 
-    // unit u: token tile u % mtiles of the W tiles W (u / mtiles) .. + W - 1
+    // unit u: token tile u % mtiles of the W tiles W (u / mtiles) .. + W - 1.  The loops below carry their place along: one
+    // thread's integer divisions would take longer than a block's products.
     if (warp == 0) {
         if (lane == 0) {
-            auto load_w = [&](int i) {
-                const long long b = b0 + i;
-                const int u = (int)(b / kb), k = (int)(b - (long long)u * kb), s = i % STAGES, t0 = u / p.mtiles * W;
-                const int gs = min(C::GS, p.groups - k * C::GS);         // groups that exist of this stage's
+            struct Place { int k, m, t0; };
+            const int u0 = b0 / kb;
+            Place pw{b0 - u0 * kb, u0 % p.mtiles, u0 / p.mtiles * W}, px = pw;
+            auto next = [&](Place& q) {
+                if (++q.k == kb) {
+                    q.k = 0;
+                    if (++q.m == p.mtiles) { q.m = 0; q.t0 += W; }
+                }
+            };
+            auto load_w = [&](int s) {
+                const int gs = C::GS == 1 ? 1 : min(C::GS, p.groups - pw.k * C::GS);         // groups that exist of this stage's
                 mbar_expect_tx(&full[s], C::ARRIVE + gs * TILE_BYTES * (W + C::ATOMS));
 #pragma unroll
                 for (int w = 0; w < W; ++w) {
-                    tma_load_2d(tiles + (size_t)s * C::STAGE + w * 16384, &map_w, &full[s], k * 128, (t0 + w) * 128);
-                    const int t = min(t0 + w, p.ntiles - 1);             // the last tile may have no partner: its scales again, never stored
-                    bulk_load(sf + s * C::SF + w * C::GS * TILE_BYTES, p.w_scales + ((size_t)t * p.groups + k * C::GS) * TILE_BYTES, gs * TILE_BYTES,
+                    tma_load_2d(tiles + s * C::STAGE + w * 16384, &map_w, &full[s], pw.k * 128, (pw.t0 + w) * 128);
+                    const int t = min(pw.t0 + w, p.ntiles - 1);          // the last tile may have no partner: its scales again, never stored
+                    bulk_load(sf + s * C::SF + w * C::GS * TILE_BYTES, p.w_scales + ((size_t)t * p.groups + pw.k * C::GS) * TILE_BYTES, gs * TILE_BYTES,
                               &full[s]);
                 }
+                next(pw);
             };
-            auto load_x = [&](int i) {
-                const long long b = b0 + i;
-                const int u = (int)(b / kb), k = (int)(b - (long long)u * kb), s = i % STAGES, m = u % p.mtiles;
-                const int gs = min(C::GS, p.groups - k * C::GS);
-                tma_load_2d(tiles + (size_t)s * C::STAGE + C::W_BYTES, &map_x, &full[s], k * 128, m * C::XR);
-                bulk_load(sf + s * C::SF + W * C::GS * TILE_BYTES, p.x_scales + ((size_t)m * p.groups + k * C::GS) * (C::ATOMS * TILE_BYTES),
+            auto load_x = [&](int s) {
+                const int gs = C::GS == 1 ? 1 : min(C::GS, p.groups - px.k * C::GS);
+                tma_load_2d(tiles + s * C::STAGE + C::W_BYTES, &map_x, &full[s], px.k * 128, px.m * C::XR);
+                bulk_load(sf + s * C::SF + W * C::GS * TILE_BYTES, p.x_scales + ((size_t)px.m * p.groups + px.k * C::GS) * (C::ATOMS * TILE_BYTES),
                           gs * C::ATOMS * TILE_BYTES, &full[s]);
+                next(px);
             };
             const int pre = min(n, STAGES);
             for (int i = 0; i < pre; ++i) load_w(i);
             pdl_wait();
             for (int i = 0; i < pre; ++i) load_x(i);
             int issued = pre;
-            for (int i = pre; i < n; ++i) {
-                if (!mbar_wait(&empty[i % STAGES], (i / STAGES - 1) & 1, abortp)) break;
-                load_w(i);
-                load_x(i);
-                issued = i + 1;
+            uint32_t parity = 0;
+            for (int s = 0; issued < n; ++issued) {
+                if (!mbar_wait(&empty[s], parity, abortp)) break;
+                load_w(s);
+                load_x(s);
+                if (++s == STAGES) { s = 0; parity ^= 1; }
             }
             pdl_trigger_gemm();
             if (*abortp)
@@ -198,47 +206,50 @@ product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
         }
     } else if (warp == 1) {
         if (lane == 0) {
-            bool ok = true;
-            int seg = 0;
-            for (int i = 0; i < n && ok; ++i) {
-                const int k = (int)((b0 + i) % kb), s = i % STAGES;
-                const bool fresh = i == 0 || k == 0;
-                const int buf = seg % C::BUFS;
-                if (fresh && seg >= C::BUFS) ok = mbar_wait(&acc_empty[buf], (seg / C::BUFS - 1) & 1, abortp);
-                if (!ok) break;
-                ok = mbar_wait(&full[s], (i / STAGES) & 1, abortp);
-                if (!ok) break;
+            const uint64_t desc0 = umma_desc(smem_addr(tiles));          // (offsets stay within the address field: 16-byte steps of 227 KB)
+            const uint32_t sf0 = smem_addr(sf);
+            int k = b0 % kb, s = 0, buf = 0;
+            uint32_t parity = 0, acc_parity = 1;                         // the first wait for each accumulator passes at once
+            bool fresh = true;
+            for (int i = 0; i < n; ++i) {
+                if (fresh && !mbar_wait(&acc_empty[buf], acc_parity, abortp)) break;
+                if (!mbar_wait(&full[s], parity, abortp)) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                const uint32_t st = smem_addr(tiles + (size_t)s * C::STAGE), ss = smem_addr(sf + s * C::SF), tsf = tmem_sf + s * C::SF_COLS;
-                const int gs = min(C::GS, p.groups - k * C::GS);
-                for (int g = 0; g < gs; ++g) {
+                const uint32_t ss = sf0 + s * C::SF, tsf = tmem_sf + s * C::SF_COLS;
+                const int gs = C::GS == 1 ? 1 : min(C::GS, p.groups - k * C::GS);
+#pragma unroll
+                for (int g = 0; g < C::GS; ++g) {
+                    if (g >= gs) break;
 #pragma unroll
                     for (int w = 0; w < W; ++w) scales_to_tmem(tsf + (w * C::GS + g) * 4, ss + (w * C::GS + g) * TILE_BYTES);
 #pragma unroll
                     for (int a = 0; a < C::ATOMS; ++a)
                         scales_to_tmem(tsf + (W * C::GS + g * C::ATOMS + a) * 4, ss + (W * C::GS + g * C::ATOMS + a) * TILE_BYTES);
                 }
-                const uint64_t db = umma_desc(st + C::W_BYTES);
+                const uint64_t da = desc0 + (uint32_t)(s * (C::STAGE >> 4)), db = da + (C::W_BYTES >> 4);
+                const uint32_t d = tmem + buf * W * C::NCOL;
                 const int slices = C::A16 ? 4 : 2 * gs;                  // 32 bytes of a row each: 32 or 64 elements
 #pragma unroll
-                for (int w = 0; w < W; ++w) {
-                    const uint64_t da = umma_desc(st + w * 16384);
-                    const uint32_t d = tmem + (buf * W + w) * C::NCOL;
+                for (int j = 0; j < 4; ++j) {
+                    if (j >= slices) break;
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        if (j >= slices) break;
+                    for (int w = 0; w < W; ++w) {
                         const int g = C::A16 ? 0 : j / 2, id = C::A16 ? j : (j & 1) * 2;
                         const uint32_t sa = tsf + (w * C::GS + g) * 4, sb = tsf + (W * C::GS + g * C::ATOMS) * 4;
-                        umma_scaled<C::A16>(d, da + 2 * j, db + 2 * j, idesc_of<C>(id), sa, sb, !fresh || j > 0);
+                        umma_scaled<C::A16>(d + w * C::NCOL, da + w * 1024 + 2 * j, db + 2 * j, idesc_of<C>(id), sa, sb, j > 0 || !fresh);
                         if (C::A16 && !C::SIDE)
-                            umma_scaled<C::A16>(d, da + 2 * j, db + (TT * 128 >> 4) + 2 * j, idesc_of<C>(id), sa, sb + 4, 1);
+                            umma_scaled<C::A16>(d + w * C::NCOL, da + w * 1024 + 2 * j, db + (TT * 128 >> 4) + 2 * j, idesc_of<C>(id), sa, sb + 4, 1);
                     }
                 }
                 umma_commit(&empty[s]);
-                if (i == n - 1 || k == kb - 1) {
+                fresh = false;
+                if (++k == kb || i == n - 1) {
                     umma_commit(&acc_full[buf]);
-                    ++seg;
+                    k = 0;
+                    fresh = true;
+                    if (++buf == C::BUFS) { buf = 0; acc_parity ^= 1; }
                 }
+                if (++s == STAGES) { s = 0; parity ^= 1; }
             }
         }
     } else {
@@ -247,8 +258,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
         pdl_wait();
         int seg = 0;
         for (int i = 0; i < n; ++seg) {
-            const long long b = b0 + i;
-            const int u = (int)(b / kb), k0 = (int)(b - (long long)u * kb), k1 = min(kb, k0 + n - i), buf = seg % C::BUFS;
+            const int u = (b0 + i) / kb, k0 = b0 + i - u * kb, k1 = min(kb, k0 + n - i), buf = seg % C::BUFS;
             i += k1 - k0;
             mbar_wait(&acc_full[buf], (seg / C::BUFS) & 1, abortp);
             // one thread reads the flag for all of these warps: they leave together or not at all
@@ -272,8 +282,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
                     else reinterpret_cast<float*>(p.y)[at] = v[j] + bias;
                 }
             };
-            const int slot = (int)(p.split.start(cta) / kb) == u ? 0 : 1;
-            float* mine = p.part + (((size_t)cta * 2 + slot) * W + w) * (TT * 128) + row;
+            float* mine = p.part + (((size_t)cta * 2 + p.split.place(cta, u)) * W + w) * (TT * 128) + row;
 #pragma unroll 1
             for (int t0 = 0; t0 < tokens; t0 += 8) {
                 float v[8];
@@ -296,7 +305,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(&acc_empty[buf])) : "memory");
             if (whole) continue;
-            const int c0 = p.split.owner((long long)u * kb), c1 = p.split.owner((long long)(u + 1) * kb - 1);
+            const int c0 = p.split.owner(u * kb), c1 = p.split.owner((u + 1) * kb - 1);
             __threadfence();
             asm volatile("bar.sync 1, %0;" ::"n"(C::EPI_WARPS * 32) : "memory");
             if (threadIdx.x == 64) is_last = atomicAdd(&p.counters[u], 1) == c1 - c0;
@@ -306,9 +315,10 @@ product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
 #pragma unroll 1
             for (int t0 = 0; t0 < tokens; t0 += 8) {
                 float v[8] = {};
+                // one CTA's after another's, four of them in a round of loads
+#pragma unroll 4
                 for (int c = c0; c <= c1; ++c) {
-                    const int sl = (int)(p.split.start(c) / kb) == u ? 0 : 1;
-                    const float* from = p.part + (((size_t)c * 2 + sl) * W + w) * (TT * 128) + row + t0 * 128;
+                    const float* from = p.part + (((size_t)c * 2 + p.split.place(c, u)) * W + w) * (TT * 128) + row + t0 * 128;
 #pragma unroll
                     for (int j = 0; j < 8; ++j) v[j] += __ldcg(from + j * 128);
                 }
@@ -371,7 +381,7 @@ PRISM_EXPORT int prism_mxfp4_linear_workspace(int M, int N, int K, int act_bits,
     if (M <= 0 || N <= 0 || K <= 0 || (act_bits != 16 && act_bits != 4)) return (int)cudaErrorInvalidValue;
     const prism::mx::Plan q = prism::mx::plan_for(M, N, K, act_bits);
     *bytes = q.bytes;
-    return q.units > 0x7fffffffLL ? (int)cudaErrorInvalidValue : 0;
+    return q.units * q.kb > 0x7fffffffLL ? (int)cudaErrorInvalidValue : 0;
 }
 
 // x [M, K] bfloat16 (row stride ldx); codes, scales: W [N, K]; y [M, N] of `out_dtype` (row stride ldy); act_bits 16 or 4;
@@ -385,7 +395,7 @@ PRISM_EXPORT int prism_mxfp4_linear(const void* x, long long ldx, const void* co
     if (K <= 0 || (act_bits != 16 && act_bits != 4) || ((uintptr_t)codes & 31) || ((uintptr_t)scales & 15) || ((uintptr_t)ws & 255))
         return (int)cudaErrorInvalidValue;
     const Plan q = plan_for(M, N, K, act_bits);
-    if (q.units > 0x7fffffffLL) return (int)cudaErrorInvalidValue;
+    if (q.units * q.kb > 0x7fffffffLL) return (int)cudaErrorInvalidValue;
     uint8_t* base = static_cast<uint8_t*>(ws);
     const bool a16 = act_bits == 16;
     const int xr = a16 ? 2 * q.tt : q.tt;
@@ -404,7 +414,7 @@ PRISM_EXPORT int prism_mxfp4_linear(const void* x, long long ldx, const void* co
     p.counters = reinterpret_cast<int*>(base + q.counters);
     p.err = err;
     p.ldy = ldy;
-    p.split = Split{q.units * q.kb, q.P, q.kb};
+    p.split = Split((int)(q.units * q.kb), q.P, q.kb);
     p.M = M, p.N = N, p.groups = q.groups, p.mtiles = q.mtiles, p.ntiles = q.ntiles;
     p.bias_bf16 = bias_dtype == PRISM_DTYPE_BF16, p.out_bf16 = out_dtype == PRISM_DTYPE_BF16;
     const long long threads = (long long)M * q.groups * 16, most = threads > q.units ? threads : q.units;

@@ -55,11 +55,19 @@ template <int N> __device__ __forceinline__ void terms_of(const float (&v)[N], i
 
 // ---- pieces of the products -----------------------------------------------------------------------------------------------
 
-struct Split {                 // how the blocks are dealt: CTA c has the blocks [c total / P, (c + 1) total / P)
-    long long total;
-    int P, kb;                 // CTAs; stages of K of a unit
-    __device__ __forceinline__ long long start(int c) const { return (long long)c * total / P; }
-    __device__ __forceinline__ int owner(long long b) const { return (int)(((b + 1) * P - 1) / total); }
+// How `total` blocks are dealt to P CTAs as one line: the first `more` have one block more than the others.  A unit is kb
+// neighbouring blocks; a CTA that does not begin within a unit has its first blocks in the second of its two places for
+// sums that are not whole (it can only share the unit it begins in and the unit it ends in with others).
+struct Split {
+    int total, P, kb, base, more;
+    __host__ __device__ Split() {}
+    __host__ __device__ Split(int total_, int P_, int kb_) : total(total_), P(P_), kb(kb_), base(total_ / P_), more(total_ - total_ / P_ * P_) {}
+    __device__ __forceinline__ int start(int c) const { return c * base + min(c, more); }
+    __device__ __forceinline__ int owner(int b) const {
+        const int edge = more * (base + 1);
+        return b < edge ? b / (base + 1) : more + (b - edge) / base;
+    }
+    __device__ __forceinline__ int place(int c, int unit) const { return start(c) >= unit * kb ? 0 : 1; }
 };
 
 __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {

@@ -242,7 +242,7 @@ __device__ __forceinline__ void moe_lists(const Moe& p, Lists& q) {
 struct Walk {
     int l, tile, k, n, tiles, kb;
     __device__ __forceinline__ Walk(const Split& s, int cta, int tiles_, int kb_) : tiles(tiles_), kb(kb_) {
-        const int b0 = cta < s.P ? (int)s.start(cta) : 0, b1 = cta < s.P ? (int)s.start(cta + 1) : 0, u = b0 / kb;
+        const int b0 = cta < s.P ? s.start(cta) : 0, b1 = cta < s.P ? s.start(cta + 1) : 0, u = b0 / kb;
         l = u / tiles, tile = u - l * tiles, k = b0 - u * kb, n = b1 - b0;
     }
     __device__ __forceinline__ void next() { step(1); }
@@ -293,7 +293,7 @@ moe_kernel(const __grid_constant__ CUtensorMap map_gate, const __grid_constant__
         moe_lists(p, q);
         const int g1 = groups_of(p.H), g2 = groups_of(p.F), tiles1 = g2, tiles_h = (p.H + 127) / 128, tiles2 = (tiles_h + 1) / 2;
         const int total1 = q.live * tiles1 * g1, total2 = q.live * tiles2 * g2;
-        const Split s1{total1, min(P, total1), g1}, s2{total2, min(P, total2), g2};
+        const Split s1(total1, min(P, total1), g1), s2(total2, min(P, total2), g2);
         Walk a(s1, cta, tiles1, g1), b(s2, cta, tiles2, g2);
         const int n1 = a.n, n = a.n + b.n;
         int* units2 = p.counters + q.live * tiles1;
@@ -368,33 +368,37 @@ moe_kernel(const __grid_constant__ CUtensorMap map_gate, const __grid_constant__
             }
         } else if (warp == 1) {
             if (lane == 0) {
-                int seg = 0;
+                const uint64_t desc0 = umma_desc(smem_addr(tiles));
+                const uint32_t sf0 = smem_addr(sf);
+                int s = 0, buf = 0;
+                uint32_t parity = 0, acc_parity = 1;             // the first wait for each accumulator passes at once
+                bool fresh = true;
                 for (int i = 0; i < n; ++i) {
-                    const int s = i % STAGES, buf = seg % C::BUFS, k = i < n1 ? a.k : b.k;
-                    const bool fresh = i == 0 || i == n1 || k == 0;
-                    if (fresh && seg >= C::BUFS && !mbar_wait(&acc_empty[buf], (seg / C::BUFS - 1) & 1, abortp)) break;
-                    if (!mbar_wait(&full[s], (i / STAGES) & 1, abortp)) break;
+                    if (fresh && !mbar_wait(&acc_empty[buf], acc_parity, abortp)) break;
+                    if (!mbar_wait(&full[s], parity, abortp)) break;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    const uint32_t st = smem_addr(tiles + (size_t)s * C::STAGE), ss = smem_addr(sf + s * C::SF), tsf = tmem_sf + s * C::SF_COLS;
+                    const uint32_t ss = sf0 + s * C::SF, tsf = tmem_sf + s * C::SF_COLS;
 #pragma unroll
                     for (int c = 0; c < 3; ++c) scales_to_tmem(tsf + c * 4, ss + c * TILE_BYTES);
                     const int cols = i < n1 ? NCOL : (q.count[b.l] + 7) / 8 * 16;
                     const uint32_t idesc = 5u << 7 | (uint32_t)(cols >> 3) << 17 | 1u << 23 | 1u << 27;       // E2M1 by E4M3, scales E8M0
-                    const uint64_t db = umma_desc(st + C::W_BYTES);
+                    const uint64_t da = desc0 + (uint32_t)(s * (C::STAGE >> 4)), db = da + (C::W_BYTES >> 4);
+                    const uint32_t d = tmem + buf * 2 * NCOL;
 #pragma unroll
-                    for (int w = 0; w < 2; ++w)
+                    for (uint32_t j = 0; j < 4; ++j)
 #pragma unroll
-                        for (uint32_t j = 0; j < 4; ++j)
-                            umma_scaled<true>(tmem + (buf * 2 + w) * NCOL, umma_desc(st + w * 16384) + 2 * j, db + 2 * j, idesc | j << 4 | j << 29,
-                                              tsf + w * 4, tsf + 8, !fresh || j > 0);
+                        for (int w = 0; w < 2; ++w)
+                            umma_scaled<true>(d + w * NCOL, da + w * 1024 + 2 * j, db + 2 * j, idesc | j << 4 | j << 29, tsf + w * 4, tsf + 8, j > 0 || !fresh);
                     umma_commit(&empty[s]);
-                    const bool done = i == n1 - 1 || i == n - 1 || k == (i < n1 ? g1 : g2) - 1;
+                    const bool done = i == n1 - 1 || i == n - 1 || (i < n1 ? a.k == g1 - 1 : b.k == g2 - 1);
                     if (i < n1) a.next();
                     else b.next();
+                    fresh = done;
                     if (done) {
                         umma_commit(&acc_full[buf]);
-                        ++seg;
+                        if (++buf == C::BUFS) { buf = 0; acc_parity ^= 1; }
                     }
+                    if (++s == STAGES) { s = 0; parity ^= 1; }
                 }
             }
         } else if (warp >= 4) {
@@ -448,7 +452,7 @@ moe_kernel(const __grid_constant__ CUtensorMap map_gate, const __grid_constant__
                         s[(v & 31) * 16 + v / 32 * 4] = low_byte(byte);
                     }
                 };
-                float* mine = p.part1 + (size_t)(cta * 2 + ((int)(s1.start(cta) / g1) == unit ? 0 : 1)) * (2 * TT * 128) + row;
+                float* mine = p.part1 + (size_t)(cta * 2 + s1.place(cta, unit)) * (2 * TT * 128) + row;
                 for (int r0 = half * 4; r0 < count; r0 += 8) {
                     float g[4][2], u[4][2];
 #pragma unroll
@@ -470,12 +474,13 @@ moe_kernel(const __grid_constant__ CUtensorMap map_gate, const __grid_constant__
                 release();
                 ++seg;
                 if (!whole) {
-                    const int c0 = s1.owner((long long)unit * g1), c1 = s1.owner((long long)(unit + 1) * g1 - 1);
+                    const int c0 = s1.owner(unit * g1), c1 = s1.owner((unit + 1) * g1 - 1);
                     if (!last_of(&p.counters[unit], c1 - c0)) continue;
                     for (int r = half; r < count; r += 2) {
                         float g = 0.f, u = 0.f;
+#pragma unroll 8
                         for (int c = c0; c <= c1; ++c) {
-                            const float* from = p.part1 + (size_t)(c * 2 + ((int)(s1.start(c) / g1) == unit ? 0 : 1)) * (2 * TT * 128) + r * 128 + row;
+                            const float* from = p.part1 + (size_t)(c * 2 + s1.place(c, unit)) * (2 * TT * 128) + r * 128 + row;
                             g += __ldcg(from), u += __ldcg(from + TT * 128);
                         }
                         hidden(r, g, u);
@@ -497,7 +502,7 @@ moe_kernel(const __grid_constant__ CUtensorMap map_gate, const __grid_constant__
                 if (!begin()) break;
                 const int count = q.count[l], first = q.first[l], nt = (count + 7) / 8 * 8, f = (tile * 2 + half) * 128 + row;
                 const uint32_t d = tmem + lanes + ((seg % C::BUFS) * 2 + half) * NCOL;
-                float* mine = p.part2 + ((size_t)(cta * 2 + ((int)(s2.start(cta) / g2) == unit ? 0 : 1)) * 2 + half) * (TT * 128) + row;
+                float* mine = p.part2 + ((size_t)(cta * 2 + s2.place(cta, unit)) * 2 + half) * (TT * 128) + row;
                 auto store = [&](int r, float v) {
                     if (f < p.H) p.planes[(size_t)q.plane[first + r] * p.H + f] = v;
                 };
@@ -520,12 +525,13 @@ moe_kernel(const __grid_constant__ CUtensorMap map_gate, const __grid_constant__
                 release();
                 ++seg;
                 if (whole) continue;
-                const int c0 = s2.owner((long long)unit * g2), c1 = s2.owner((long long)(unit + 1) * g2 - 1);
+                const int c0 = s2.owner(unit * g2), c1 = s2.owner((unit + 1) * g2 - 1);
                 if (!last_of(&units2[unit], c1 - c0)) continue;
                 for (int r = 0; r < count; ++r) {
                     float v = 0.f;
+#pragma unroll 8
                     for (int c = c0; c <= c1; ++c)
-                        v += __ldcg(p.part2 + ((size_t)(c * 2 + ((int)(s2.start(c) / g2) == unit ? 0 : 1)) * 2 + half) * (TT * 128) + r * 128 + row);
+                        v += __ldcg(p.part2 + ((size_t)(c * 2 + s2.place(c, unit)) * 2 + half) * (TT * 128) + r * 128 + row);
                     store(r, v);
                 }
             }

@@ -23,11 +23,6 @@ MOE_TOKENS, MOE_EXPERTS, MOE_TOP = 64, 256, 16               # the most of an ``
 DTYPE = "mxfp4"
 
 
-def _need(ok, what: str):
-    if not ok:
-        raise ops.KernelError(what)
-
-
 class Mxfp4:
     """A matrix ``[N, K]`` (or a stack ``[E, N, K]`` of them) in 4 bits.  ``codes``: uint8 ``[..., N, Kp / 2]`` with ``Kp``
     the K rounded up to 128, element 2i in the low half of a byte, zero beyond K.  ``scales``: uint8 ``[..., ceil(N / 128),
@@ -41,7 +36,7 @@ class Mxfp4:
         cs, ss = codes.shape, scales.shape
         groups = -(-K // GROUP)
         if not (K > 0 and codes.dtype is torch.uint8 and scales.dtype is torch.uint8 and codes.is_contiguous() and scales.is_contiguous()
-                and len(cs) in (2, 3) and cs[-1] == groups * (GROUP // 2) and cs[-2] > 0
+                and codes.device == scales.device and len(cs) in (2, 3) and cs[-1] == groups * (GROUP // 2) and cs[-2] > 0
                 and ss == cs[:-2] + (-(-cs[-2] // TILE_ROWS), groups, TILE_BYTES)):
             raise ops.KernelError(f"4-bit matrix of K = {K}: codes {tuple(cs)} {codes.dtype} and scales {tuple(ss)} {scales.dtype} do not belong together")
         self.codes, self.scales, self.shape = codes, scales, cs[:-1] + (K,)
@@ -59,16 +54,18 @@ class Mxfp4:
 
     def __getitem__(self, e: int) -> "Mxfp4":
         """One matrix of a stack."""
-        _need(len(self.shape) == 3, "only a stack of 4-bit matrices can be indexed")
+        if len(self.shape) != 3:
+            raise ops.KernelError("only a stack of 4-bit matrices can be indexed")
         return Mxfp4(self.codes[e], self.scales[e], self.shape[-1])
 
     def dequantize(self, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
         """The values that the codes stand for, exact in bfloat16 and float32; NaN where the scale is 255."""
-        _need(dtype in (torch.bfloat16, torch.float32), f"4-bit values come back as bfloat16 or float32, not {dtype}")
-        ops._cuda(self.codes, self.scales)
+        if dtype not in (torch.bfloat16, torch.float32):
+            raise ops.KernelError(f"4-bit values come back as bfloat16 or float32, not {dtype}")
+        ops._cuda(self.codes)
         out = torch.empty(self.shape, dtype=dtype, device=self.device)
         N, K = self.shape[-2:]
-        ops._check(ops.lib().prism_mxfp4_dequantize(self.codes.data_ptr(), self.scales.data_ptr(), self.codes.numel() // self.codes.shape[-1],
+        ops._check(ops.lib().prism_mxfp4_dequantize(self.codes.data_ptr(), self.scales.data_ptr(), self.shape[0] if len(self.shape) == 3 else 1,
                                                     N, K, out.data_ptr(), ops._dt(out), ops._stream()), "mxfp4_dequantize")
         return out
 
@@ -77,17 +74,17 @@ def mxfp4_quantize(x: torch.Tensor) -> Mxfp4:
     """``x [N, K]`` (rows may have a stride of their own) or a contiguous stack ``[E, N, K]``, bfloat16 or float32, to 4
     bits: a block's exponent is that of its largest magnitude less two, elements round to nearest (ties to the even code) and
     saturate at 6.  A block that holds an infinity or NaN becomes NaN as a whole."""
-    ops._cuda(x)
-    _need(x.dim() in (2, 3) and x.numel() > 0, f"rows to quantise: a matrix or a stack of them, got {tuple(x.shape)}")
-    _need(x.stride(-1) == 1 or x.shape[-1] == 1, "rows to quantise lie side by side in memory")
-    _need(x.dim() == 2 or x.is_contiguous(), "a stack to quantise is contiguous")
-    N, K = x.shape[-2:]
-    groups, lead = -(-K // GROUP), tuple(x.shape[:-2])
+    if not x.is_cuda:
+        ops._cuda(x)
+    lead, (N, K) = x.shape[:-2], x.shape[-2:] if x.dim() in (2, 3) else (0, 0)
+    if not (N and K and (x.stride(-1) == 1 or K == 1) and (not lead or (lead[0] and x.is_contiguous()))):
+        raise ops.KernelError(f"rows to quantise: a matrix whose rows lie side by side in memory or a contiguous stack of them, got {tuple(x.shape)} "
+                              f"with strides {x.stride()}")
+    groups = -(-K // GROUP)
     codes = torch.empty(lead + (N, groups * (GROUP // 2)), dtype=torch.uint8, device=x.device)
     scales = torch.empty(lead + (-(-N // TILE_ROWS), groups, TILE_BYTES), dtype=torch.uint8, device=x.device)
-    rows = x.numel() // K
-    ops._check(ops.lib().prism_mxfp4_quantize(x.data_ptr(), ops._dt(x), x.stride(-2) if rows > 1 else K, rows, N, K, codes.data_ptr(),
-                                              scales.data_ptr(), ops._stream()), "mxfp4_quantize")
+    ops._check(ops.lib().prism_mxfp4_quantize(x.data_ptr(), ops._dt(x), x.stride(-2) if N > 1 else K, lead[0] if lead else 1, N, K,
+                                              codes.data_ptr(), scales.data_ptr(), ops._stream()), "mxfp4_quantize")
     return Mxfp4(codes, scales, K)
 
 
@@ -102,6 +99,17 @@ def _workspace(size_of: str, *sizes: int) -> int:
             raise ops.KernelError(f"{size_of}: sizes {sizes} are not supported")
         n = _workspace_bytes[(size_of,) + sizes] = b.value
     return n
+
+
+_err_words = {}
+
+
+def _err_word(device: torch.device) -> int:
+    """Address of the device's error word of bounded waits (``ops.check_tc_errors`` reads it)."""
+    p = _err_words.get(device.index)
+    if p is None:
+        p = _err_words[device.index] = ops._tc_err_word(device).data_ptr()
+    return p
 
 
 _control_blocks = {}
@@ -126,23 +134,32 @@ def mxfp4_linear(x: torch.Tensor, w: Mxfp4, bias: Optional[torch.Tensor] = None,
     in float32.  ``act_bits`` 16: x as it is; 4: each row of x is brought to 4 bits first, as ``mxfp4_quantize`` does it.
     ``out`` (row stride of its own) or ``out_dtype``: bfloat16 (default) or float32.  A row of x with an infinity or NaN in it
     gives NaN."""
-    ops._cuda(x, w.codes, w.scales, bias, out)
-    _need(x.dim() == 2 and w.dim() == 2 and x.shape[1] == w.shape[1], f"product of {tuple(x.shape)} and {tuple(w.shape)}")
-    M, K = x.shape
-    N = w.shape[0]
-    _need(x.dtype is torch.bfloat16 and (x.stride(1) == 1 or K == 1), "activations are bfloat16 rows side by side in memory")
-    _need(act_bits in (4, 16), f"activations have 4 or 16 bits, not {act_bits}")
-    _need(bias is None or (bias.shape == (N,) and bias.is_contiguous()), "a bias has one entry per row of the weight")
+    if not (x.is_cuda and w.codes.is_cuda and (bias is None or bias.is_cuda) and (out is None or out.is_cuda)):
+        ops._cuda(x, w.codes, bias, out)
+    xs, ws = x.shape, w.shape
+    if len(xs) != 2 or len(ws) != 2 or xs[1] != ws[1]:
+        raise ops.KernelError(f"product of {tuple(xs)} and {tuple(ws)}")
+    M, K = xs
+    N = ws[0]
+    if x.dtype is not torch.bfloat16 or (x.stride(1) != 1 and K > 1) or act_bits not in (4, 16):
+        raise ops.KernelError(f"activations are bfloat16 rows side by side in memory, used with 4 or 16 bits: got {x.dtype}, strides {x.stride()}, {act_bits}")
+    if bias is not None and (bias.shape != (N,) or not bias.is_contiguous()):
+        raise ops.KernelError(f"a bias has one entry per row of the weight, got {tuple(bias.shape)}")
     if out is None:
         out = torch.empty((M, N), dtype=out_dtype or torch.bfloat16, device=x.device)
-    _need(out.shape == (M, N) and (out.stride(1) == 1 or N == 1) and out_dtype in (None, out.dtype), "out does not fit the product")
+    elif out.shape != (M, N) or (out.stride(1) != 1 and N > 1) or out_dtype not in (None, out.dtype):
+        raise ops.KernelError(f"the result of {tuple(xs)} and {tuple(ws)} does not go into {tuple(out.shape)} {out.dtype}")
     if M == 0:
         return out
-    ws = torch.empty(_workspace("prism_mxfp4_linear_workspace", M, N, K, act_bits), dtype=torch.uint8, device=x.device)
-    ops._check(ops.lib().prism_mxfp4_linear(x.data_ptr(), x.stride(0), w.codes.data_ptr(), w.scales.data_ptr(), ops._ptr(bias),
-                                            ops.F32 if bias is None else ops._dt(bias), out.data_ptr(), ops._dt(out), out.stride(0), M, N, K,
-                                            act_bits, ws.data_ptr(), ops._tc_err_word(x.device).data_ptr(), ops._stream()), "mxfp4_linear")
+    work = torch.empty(_workspace("prism_mxfp4_linear_workspace", M, N, K, act_bits), dtype=torch.uint8, device=x.device)
+    ops._check(ops.lib().prism_mxfp4_linear(x.data_ptr(), x.stride(0), w.codes.data_ptr(), w.scales.data_ptr(),
+                                            None if bias is None else bias.data_ptr(), 0 if bias is None else ops._dt(bias), out.data_ptr(),
+                                            ops._dt(out), out.stride(0), M, N, K, act_bits, work.data_ptr(), _err_word(x.device), ops._stream()),
+               "mxfp4_linear")
     return out
+
+
+_ANY_CHOICE = ops.MoeChoice()
 
 
 def mxfp4_moe(x: torch.Tensor, router: torch.Tensor, gate: Mxfp4, up: Mxfp4, down: Mxfp4, top: int, softmax: bool = False,
@@ -155,35 +172,42 @@ def mxfp4_moe(x: torch.Tensor, router: torch.Tensor, gate: Mxfp4, up: Mxfp4, dow
     (``renorm``: over the sum of the chosen) and multiplies the expert's input (``scale_input``) or its output.  ``act``:
     silu, gelu_tanh or clamped (with ``limit``, as in ``ops.glu``).  ``choice``: an ``ops.MoeChoice``.  Returns the sum over a
     token's choices, ``[T, H]`` bfloat16 or float32 (``out`` or ``out_dtype``)."""
-    ops._cuda(x, router, gate.codes, up.codes, down.codes, router_bias, out)
-    _need(x.dim() == 2 and x.dtype is torch.bfloat16 and x.stride(1) == 1, "activations are bfloat16 rows side by side in memory")
+    for t in (x, router, gate.codes, up.codes, down.codes, router_bias, out):
+        if t is not None and not t.is_cuda:
+            ops._cuda(t)
+    if x.dim() != 2 or x.dtype is not torch.bfloat16 or x.stride(1) != 1:
+        raise ops.KernelError(f"activations are bfloat16 rows side by side in memory, got {tuple(x.shape)} {x.dtype}")
     T, H = x.shape
-    E, F, _ = gate.shape if gate.dim() == 3 else (0, 0, 0)
-    _need(E > 0 and gate.shape == (E, F, H) and up.shape == gate.shape and down.shape == (E, H, F),
-          f"experts {tuple(gate.shape)}, {tuple(up.shape)}, {tuple(down.shape)} do not belong together or to rows of {H}")
-    _need(T <= MOE_TOKENS, f"{T} tokens: this layer is for up to {MOE_TOKENS}")
-    _need(1 <= top <= min(E, MOE_TOP) and E <= MOE_EXPERTS, f"a token uses {top} of {E} experts: up to {MOE_TOP} of up to {MOE_EXPERTS}")
-    _need(router.shape == (E, H) and router.is_contiguous() and (router_bias is None or (router_bias.shape == (E,) and router_bias.is_contiguous())),
-          "the router has one row (and one bias) per expert")
-    _need(act in ops.GATED, f"a gated feed-forward's activation is one of {ops.GATED}, got {act!r}")
-    ch = choice or ops.MoeChoice()
-    _need(ch.correction is None or (ch.correction.shape == (E,) and ch.correction.is_contiguous() and ch.correction.is_cuda),
-          "the correction has one entry per expert")
-    _need(ch.groups >= 1 and E % ch.groups == 0 and 1 <= ch.keep <= ch.groups and ch.keep * (E // ch.groups) >= top,
-          f"{E} experts in {ch.groups} groups of which {ch.keep} are kept, {top} a token")
+    E, F, _ = gate.shape if len(gate.shape) == 3 else (0, 0, 0)
+    if not E or gate.shape != (E, F, H) or up.shape != gate.shape or down.shape != (E, H, F):
+        raise ops.KernelError(f"experts {tuple(gate.shape)}, {tuple(up.shape)}, {tuple(down.shape)} do not belong together or to rows of {H}")
+    if T > MOE_TOKENS or E > MOE_EXPERTS or not 1 <= top <= min(E, MOE_TOP):
+        raise ops.KernelError(f"{T} tokens that use {top} of {E} experts: this layer is for up to {MOE_TOKENS} tokens, {MOE_EXPERTS} experts and "
+                              f"{MOE_TOP} of them a token")
+    if router.shape != (E, H) or not router.is_contiguous() or (router_bias is not None and (router_bias.shape != (E,) or not router_bias.is_contiguous())):
+        raise ops.KernelError("the router has one row (and one bias) per expert")
+    if act not in ops.GATED:
+        raise ops.KernelError(f"a gated feed-forward's activation is one of {ops.GATED}, got {act!r}")
+    ch = choice or _ANY_CHOICE
+    corr = ch.correction
+    if corr is not None and (corr.shape != (E,) or not corr.is_contiguous() or not corr.is_cuda):
+        raise ops.KernelError("the correction has one entry per expert, on the device")
+    if ch.groups < 1 or E % ch.groups or not 1 <= ch.keep <= ch.groups or ch.keep * (E // ch.groups) < top:
+        raise ops.KernelError(f"{E} experts in {ch.groups} groups of which {ch.keep} are kept, {top} a token")
     if out is None:
         out = torch.empty((T, H), dtype=out_dtype or torch.bfloat16, device=x.device)
-    _need(out.shape == (T, H) and out.stride(1) == 1 and out_dtype in (None, out.dtype), "out does not fit the layer")
+    elif out.shape != (T, H) or out.stride(1) != 1 or out_dtype not in (None, out.dtype):
+        raise ops.KernelError(f"the result of {T} rows of {H} does not go into {tuple(out.shape)} {out.dtype}")
     if T == 0:
         return out
     stream = ops._stream()
-    ws = torch.empty(_workspace("prism_mxfp4_moe_workspace", T, H, F, E, top), dtype=torch.uint8, device=x.device)
+    work = torch.empty(_workspace("prism_mxfp4_moe_workspace", T, H, F, E, top), dtype=torch.uint8, device=x.device)
     control = _control(stream, x.device)
-    ops._check(ops.lib().prism_mxfp4_moe(x.data_ptr(), x.stride(0), router.data_ptr(), ops._dt(router), ops._ptr(router_bias),
-                                         ops.F32 if router_bias is None else ops._dt(router_bias), gate.codes.data_ptr(), gate.scales.data_ptr(),
-                                         up.codes.data_ptr(), up.scales.data_ptr(), down.codes.data_ptr(), down.scales.data_ptr(), T, H, F, E,
-                                         top, int(softmax), int(renorm), int(scale_input), ops.MOE_ACTS[act], float(limit),
-                                         ops._ptr(ch.correction), ops.F32 if ch.correction is None else ops._dt(ch.correction), ch.groups, ch.keep,
-                                         ch.scale, ch.sum_eps, out.data_ptr(), ops._dt(out), out.stride(0), ws.data_ptr(), control.data_ptr(),
-                                         ops._tc_err_word(x.device).data_ptr(), stream), "mxfp4_moe")
+    ops._check(ops.lib().prism_mxfp4_moe(x.data_ptr(), x.stride(0), router.data_ptr(), ops._dt(router),
+                                         None if router_bias is None else router_bias.data_ptr(), 0 if router_bias is None else ops._dt(router_bias),
+                                         gate.codes.data_ptr(), gate.scales.data_ptr(), up.codes.data_ptr(), up.scales.data_ptr(),
+                                         down.codes.data_ptr(), down.scales.data_ptr(), T, H, F, E, top, softmax, renorm, scale_input,
+                                         ops.MOE_ACTS[act], limit, None if corr is None else corr.data_ptr(), 0 if corr is None else ops._dt(corr),
+                                         ch.groups, ch.keep, ch.scale, ch.sum_eps, out.data_ptr(), ops._dt(out), out.stride(0), work.data_ptr(),
+                                         control.data_ptr(), _err_word(x.device), stream), "mxfp4_moe")
     return out
