@@ -3,7 +3,7 @@
 //
 // Both run on the block-scaled tensor-core instructions, which take the codes and scale bytes as they lie in memory: no CUDA
 // core ever unpacks a weight.  128 rows of W are the M of a tcgen05.mma, tokens its N, the sums sit in tensor memory in
-// float32, the scales go from shared to tensor memory by tcgen05.cp.
+// float32, the scales beside them (tcgen05.cp).
 //
 //   act_bits 4   kind::mxf4: 4-bit codes on both sides, a scale for every 32 of either.
 //   act_bits 16  kind::mxf8f6f4 multiplies 4-bit codes by 8-bit ones (E4M3).  A bfloat16 value has 8 significant bits, two
@@ -13,8 +13,9 @@
 //                then read from shared memory once); for tiles of 128 tokens two instructions add to the same sums.
 //
 // A first kernel brings x to terms or codes (a thread 8 values), in the workspace of the call, and clears its counters.  The
-// second is persistent, a CTA an SM: warp 0 issues TMA loads into a ring of stages (W: for 16 bits 128 codes a row, which
-// TMA spreads to a byte each, for 4 bits 256), warp 1 the scale copies and the products, the other warps take the sums out.
+// second is persistent, a CTA an SM: warps 0 and 2 issue TMA loads into a ring of stages (W: for 16 bits 128 codes a row, which
+// TMA spreads to a byte each, for 4 bits 256; x), warp 1 the scale copies and the products, the warps from 4 on take the sums
+// out.
 // All of the product's blocks - (tile of W rows, tile of tokens, stage of K) - are dealt to the CTAs evenly as one long
 // line, so that every SM streams the same number of bytes whatever the sizes; a tile that several CTAs have part of is
 // added up by the one that comes last, in the order of the CTAs: results do not depend on timing.
@@ -95,8 +96,8 @@ template <bool A16_, int TT_, int W_> struct Cfg {
     static constexpr int NCOL = SIDE ? 2 * TT : TT;                // N of the instruction
     static constexpr int ATOMS = (XR + 127) / 128;                 // tiles of scales of x
     static constexpr int W_BYTES = W * 16384, X_BYTES = XR * 128, STAGE = W_BYTES + X_BYTES;
-    // bytes that a stage's loads report: codes that TMA spreads count as they are in memory, 64 bytes a row
-    static constexpr int ARRIVE = W * (A16 ? 8192 : 16384) + X_BYTES;
+    // bytes that W's loads of a stage report: codes that TMA spreads count as they are in memory, 64 bytes a row
+    static constexpr int W_ARRIVE = W * (A16 ? 8192 : 16384);
     static constexpr int SF = GS * TILE_BYTES * (W + ATOMS);       // scale bytes of a stage
     static constexpr int FIT = (216 * 1024) / (STAGE + SF);
     static constexpr int SF_COLS = GS * 4 * (W + ATOMS);           // their columns in tensor memory: every stage has its own
@@ -104,7 +105,7 @@ template <bool A16_, int TT_, int W_> struct Cfg {
     static constexpr int BUFS = 2 * W * NCOL + STAGES * SF_COLS <= 512 ? 2 : 1;
     static constexpr int COLS_USED = BUFS * W * NCOL + STAGES * SF_COLS;
     static constexpr int COLS = COLS_USED <= 64 ? 64 : COLS_USED <= 128 ? 128 : COLS_USED <= 256 ? 256 : 512;
-    static constexpr int EPI_WARPS = 4 * W, THREADS = 64 + 32 * EPI_WARPS;
+    static constexpr int EPI_WARPS = 4 * W, THREADS = 128 + 32 * EPI_WARPS;
     static constexpr size_t SMEM = (size_t)STAGES * (STAGE + SF) + 1024 + 512;
     static_assert(COLS_USED <= 512 && STAGES >= 3, "tensor memory or shared memory");
 };
@@ -141,7 +142,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, cta = blockIdx.x;
     if (threadIdx.x == 0) {
         abort_flag = 0;
-        for (int s = 0; s < STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+        for (int s = 0; s < STAGES; ++s) { mbar_init(&full[s], 2); mbar_init(&empty[s], 1); }
         for (int s = 0; s < C::BUFS; ++s) { mbar_init(&acc_full[s], 1); mbar_init(&acc_empty[s], C::EPI_WARPS); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -158,65 +159,60 @@ product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
 
     // unit u: token tile u % mtiles of the W tiles W (u / mtiles) .. + W - 1.  The loops below carry their place along: one
     // thread's integer divisions would take longer than a block's products.
-    if (warp == 0) {
-        if (lane == 0) {
-            struct Place { int k, m, t0; };
-            const int u0 = b0 / kb;
-            Place pw{b0 - u0 * kb, u0 % p.mtiles, u0 / p.mtiles * W}, px = pw;
-            auto next = [&](Place& q) {
-                if (++q.k == kb) {
-                    q.k = 0;
-                    if (++q.m == p.mtiles) { q.m = 0; q.t0 += W; }
-                }
-            };
-            auto load_w = [&](int s) {
-                const int gs = C::GS == 1 ? 1 : min(C::GS, p.groups - pw.k * C::GS);         // groups that exist of this stage's
-                mbar_expect_tx(&full[s], C::ARRIVE + gs * TILE_BYTES * (W + C::ATOMS));
+    if (warp == 0 || warp == 2) {
+        // warp 0: W and its scales, from the start; warp 2: x's, once they exist
+        const bool is_w = warp == 0;
+        const int u0 = b0 / kb;
+        int k = b0 - u0 * kb, m = u0 % p.mtiles, t0 = u0 / p.mtiles * W;
+        if (!is_w) pdl_wait();
+        uint32_t parity = 1;                                             // the first round passes at once
+        int s = 0, i = 0;
+        for (; i < n; ++i) {
+            if (!warp_wait(&empty[s], parity, abortp)) break;
+            const int gs = C::GS == 1 ? 1 : min(C::GS, p.groups - k * C::GS);             // groups that exist of this stage's
+            unsigned char *st = tiles + s * C::STAGE, *ss = sf + s * C::SF;
+            if (is_w) {
+                if (elect_one()) {
+                    mbar_expect_tx(&full[s], C::W_ARRIVE + gs * TILE_BYTES * W);
 #pragma unroll
-                for (int w = 0; w < W; ++w) {
-                    tma_load_2d(tiles + s * C::STAGE + w * 16384, &map_w, &full[s], pw.k * 128, (pw.t0 + w) * 128);
-                    const int t = min(pw.t0 + w, p.ntiles - 1);          // the last tile may have no partner: its scales again, never stored
-                    bulk_load(sf + s * C::SF + w * C::GS * TILE_BYTES, p.w_scales + ((size_t)t * p.groups + pw.k * C::GS) * TILE_BYTES, gs * TILE_BYTES,
-                              &full[s]);
+                    for (int w = 0; w < W; ++w) {
+                        tma_load_2d(st + w * 16384, &map_w, &full[s], k * 128, (t0 + w) * 128);
+                        const int t = min(t0 + w, p.ntiles - 1);         // the last tile may have no partner: its scales again, never stored
+                        bulk_load(ss + w * C::GS * TILE_BYTES, p.w_scales + ((size_t)t * p.groups + k * C::GS) * TILE_BYTES, gs * TILE_BYTES, &full[s]);
+                    }
                 }
-                next(pw);
-            };
-            auto load_x = [&](int s) {
-                const int gs = C::GS == 1 ? 1 : min(C::GS, p.groups - px.k * C::GS);
-                tma_load_2d(tiles + s * C::STAGE + C::W_BYTES, &map_x, &full[s], px.k * 128, px.m * C::XR);
-                bulk_load(sf + s * C::SF + W * C::GS * TILE_BYTES, p.x_scales + ((size_t)px.m * p.groups + px.k * C::GS) * (C::ATOMS * TILE_BYTES),
+            } else if (elect_one()) {
+                mbar_expect_tx(&full[s], C::X_BYTES + gs * TILE_BYTES * C::ATOMS);
+                tma_load_2d(st + C::W_BYTES, &map_x, &full[s], k * 128, m * C::XR);
+                bulk_load(ss + W * C::GS * TILE_BYTES, p.x_scales + ((size_t)m * p.groups + k * C::GS) * (C::ATOMS * TILE_BYTES),
                           gs * C::ATOMS * TILE_BYTES, &full[s]);
-                next(px);
-            };
-            const int pre = min(n, STAGES);
-            for (int i = 0; i < pre; ++i) load_w(i);
-            pdl_wait();
-            for (int i = 0; i < pre; ++i) load_x(i);
-            int issued = pre;
-            uint32_t parity = 0;
-            for (int s = 0; issued < n; ++issued) {
-                if (!mbar_wait(&empty[s], parity, abortp)) break;
-                load_w(s);
-                load_x(s);
-                if (++s == STAGES) { s = 0; parity ^= 1; }
             }
-            pdl_trigger_gemm();
-            if (*abortp)
-                for (int i = max(0, issued - STAGES); i < issued; ++i) mbar_wait(&full[i % STAGES], (i / STAGES) & 1, abortp);
+            __syncwarp();
+            if (++k == kb) {
+                k = 0;
+                if (++m == p.mtiles) { m = 0; t0 += W; }
+            }
+            if (++s == STAGES) { s = 0; parity ^= 1; }
         }
+        if (is_w) pdl_trigger_gemm();
+        if (*abortp)                                                     // what is in flight gets a bounded chance to land
+            for (int j = max(0, i - STAGES); j < i; ++j) mbar_wait(&full[j % STAGES], (j / STAGES) & 1, abortp);
     } else if (warp == 1) {
-        if (lane == 0) {
-            const uint64_t desc0 = umma_desc(smem_addr(tiles));          // (offsets stay within the address field: 16-byte steps of 227 KB)
-            const uint32_t sf0 = smem_addr(sf);
-            int k = b0 % kb, s = 0, buf = 0;
-            uint32_t parity = 0, acc_parity = 1;                         // the first wait for each accumulator passes at once
-            bool fresh = true;
-            for (int i = 0; i < n; ++i) {
-                if (fresh && !mbar_wait(&acc_empty[buf], acc_parity, abortp)) break;
-                if (!mbar_wait(&full[s], parity, abortp)) break;
-                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                const uint32_t ss = sf0 + s * C::SF, tsf = tmem_sf + s * C::SF_COLS;
-                const int gs = C::GS == 1 ? 1 : min(C::GS, p.groups - k * C::GS);
+        const uint64_t desc0 = umma_desc(smem_addr(tiles));              // (offsets stay within the address field: 16-byte steps of 227 KB)
+        const uint32_t sf0 = smem_addr(sf);
+        int k = b0 % kb, s = 0, buf = 0;
+        uint32_t parity = 0, acc_parity = 1;                             // the first wait for each accumulator passes at once
+        bool fresh = true;
+        for (int i = 0; i < n; ++i) {
+            if (fresh && !warp_wait(&acc_empty[buf], acc_parity, abortp)) break;
+            if (!warp_wait(&full[s], parity, abortp)) break;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            const uint32_t ss = sf0 + s * C::SF, tsf = tmem_sf + s * C::SF_COLS;
+            const int gs = C::GS == 1 ? 1 : min(C::GS, p.groups - k * C::GS);
+            const uint64_t da = desc0 + (uint32_t)(s * (C::STAGE >> 4)), db = da + (C::W_BYTES >> 4);
+            const uint32_t d = tmem + buf * W * C::NCOL;
+            const bool done = ++k == kb || i == n - 1;
+            if (elect_one()) {
 #pragma unroll
                 for (int g = 0; g < C::GS; ++g) {
                     if (g >= gs) break;
@@ -225,36 +221,31 @@ product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
 #pragma unroll
                     for (int a = 0; a < C::ATOMS; ++a)
                         scales_to_tmem(tsf + (W * C::GS + g * C::ATOMS + a) * 4, ss + (W * C::GS + g * C::ATOMS + a) * TILE_BYTES);
-                }
-                const uint64_t da = desc0 + (uint32_t)(s * (C::STAGE >> 4)), db = da + (C::W_BYTES >> 4);
-                const uint32_t d = tmem + buf * W * C::NCOL;
-                const int slices = C::A16 ? 4 : 2 * gs;                  // 32 bytes of a row each: 32 or 64 elements
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    if (j >= slices) break;
+                    for (int j = 0; j < 4 / C::GS; ++j)                  // 32 bytes of a row each: 32 or 64 elements
 #pragma unroll
-                    for (int w = 0; w < W; ++w) {
-                        const int g = C::A16 ? 0 : j / 2, id = C::A16 ? j : (j & 1) * 2;
-                        const uint32_t sa = tsf + (w * C::GS + g) * 4, sb = tsf + (W * C::GS + g * C::ATOMS) * 4;
-                        umma_scaled<C::A16>(d + w * C::NCOL, da + w * 1024 + 2 * j, db + 2 * j, idesc_of<C>(id), sa, sb, j > 0 || !fresh);
-                        if (C::A16 && !C::SIDE)
-                            umma_scaled<C::A16>(d + w * C::NCOL, da + w * 1024 + 2 * j, db + (TT * 128 >> 4) + 2 * j, idesc_of<C>(id), sa, sb + 4, 1);
-                    }
+                        for (int w = 0; w < W; ++w) {
+                            const int id = C::A16 ? j : j * 2, at = 2 * (g * (4 / C::GS) + j);
+                            const uint32_t sa = tsf + (w * C::GS + g) * 4, sb = tsf + (W * C::GS + g * C::ATOMS) * 4;
+                            umma_scaled<C::A16>(d + w * C::NCOL, da + w * 1024 + at, db + at, idesc_of<C>(id), sa, sb, g > 0 || j > 0 || !fresh);
+                            if (C::A16 && !C::SIDE)
+                                umma_scaled<C::A16>(d + w * C::NCOL, da + w * 1024 + at, db + (TT * 128 >> 4) + at, idesc_of<C>(id), sa, sb + 4, 1);
+                        }
                 }
                 umma_commit(&empty[s]);
-                fresh = false;
-                if (++k == kb || i == n - 1) {
-                    umma_commit(&acc_full[buf]);
-                    k = 0;
-                    fresh = true;
-                    if (++buf == C::BUFS) { buf = 0; acc_parity ^= 1; }
-                }
-                if (++s == STAGES) { s = 0; parity ^= 1; }
+                if (done) umma_commit(&acc_full[buf]);
             }
+            __syncwarp();
+            fresh = done;
+            if (done) {
+                k = 0;
+                if (++buf == C::BUFS) { buf = 0; acc_parity ^= 1; }
+            }
+            if (++s == STAGES) { s = 0; parity ^= 1; }
         }
-    } else {
-        // warps of one tile of W rows: 2 + 4 w .. 5 + 4 w; TMEM lanes (warp % 4) * 32 .. + 31
-        const int w = (warp - 2) / 4, q = warp & 3, row = q * 32 + lane;
+    } else if (warp >= 4) {
+        // warps of one tile of W rows: 4 + 4 w .. 7 + 4 w; TMEM lanes (warp % 4) * 32 .. + 31
+        const int w = (warp - 4) / 4, q = warp & 3, row = q * 32 + lane;
         pdl_wait();
         int seg = 0;
         for (int i = 0; i < n; ++seg) {
@@ -263,7 +254,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
             mbar_wait(&acc_full[buf], (seg / C::BUFS) & 1, abortp);
             // one thread reads the flag for all of these warps: they leave together or not at all
             asm volatile("bar.sync 1, %0;" ::"n"(C::EPI_WARPS * 32) : "memory");
-            if (threadIdx.x == 64) gone = *abortp;
+            if (threadIdx.x == 128) gone = *abortp;
             asm volatile("bar.sync 1, %0;" ::"n"(C::EPI_WARPS * 32) : "memory");
             if (gone) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -303,12 +294,13 @@ product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
                     for (int j = 0; j < 8; ++j) mine[(t0 + j) * 128] = v[j];
             }
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-            if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(&acc_empty[buf])) : "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&acc_empty[buf]);
             if (whole) continue;
             const int c0 = p.split.owner(u * kb), c1 = p.split.owner((u + 1) * kb - 1);
             __threadfence();
             asm volatile("bar.sync 1, %0;" ::"n"(C::EPI_WARPS * 32) : "memory");
-            if (threadIdx.x == 64) is_last = atomicAdd(&p.counters[u], 1) == c1 - c0;
+            if (threadIdx.x == 128) is_last = atomicAdd(&p.counters[u], 1) == c1 - c0;
             asm volatile("bar.sync 1, %0;" ::"n"(C::EPI_WARPS * 32) : "memory");
             if (!is_last) continue;
             __threadfence();

@@ -74,10 +74,24 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
                  ::"r"(smem_addr(dst)), "l"(src), "r"(bytes), "r"(smem_addr(bar)) : "memory");
 }
+// The warps that issue loads and products run their loops as a whole, and one lane of them issues: operands then stay in the
+// uniform registers that these instructions take them from.  A single lane's loop moves them over for every instruction (a
+// product of 128 x 32 x 32: 115 cycles against 42, of 128 x 128 x 32 65).
+__device__ __forceinline__ bool elect_one() {
+    uint32_t e;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(e));
+    return e != 0;
+}
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abortp) {
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity, abortp));
+}
 // 512 bytes of scales, 32 rows of 16 without swizzle, to four columns of tensor memory, the same in every quarter of its lanes
 __device__ __forceinline__ void scales_to_tmem(uint32_t taddr, uint32_t saddr) {
     const uint64_t d = (uint64_t)((saddr >> 4) & 0x3FFF) | (uint64_t)8 << 32 | (uint64_t)1 << 46;
     asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(d) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(bar)) : "memory");
 }
 template <bool A16>
 __device__ __forceinline__ void umma_scaled(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb, uint32_t accumulate) {

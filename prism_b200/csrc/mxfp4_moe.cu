@@ -299,107 +299,104 @@ moe_kernel(const __grid_constant__ CUtensorMap map_gate, const __grid_constant__
         int* units2 = p.counters + q.live * tiles1;
 
         if (warp == 0) {
-            if (lane == 0) {
-                int i = 0;
-                for (; i < n; ++i) {
-                    const int s = i % STAGES;
-                    if (i >= STAGES && !mbar_wait(&empty[s], (i / STAGES - 1) & 1, abortp)) break;
-                    unsigned char *st = tiles + (size_t)s * C::STAGE, *ss = sf + s * C::SF;
-                    mbar_expect_tx(&full[s], 2 * 8192 + 2 * TILE_BYTES);         // spread codes count as they are in memory
-                    if (i < n1) {
-                        const int e = q.expert[a.l], row = e * p.F + a.tile * 128;
-                        const size_t at = ((size_t)(e * tiles1 + a.tile) * g1 + a.k) * TILE_BYTES;
+            uint32_t parity = 1;                                 // the first round passes at once
+            int i = 0;
+            for (int s = 0; i < n; ++i) {
+                if (!warp_wait(&empty[s], parity, abortp)) break;
+                unsigned char *st = tiles + s * C::STAGE, *ss = sf + s * C::SF;
+                if (i < n1) {
+                    const int e = q.expert[a.l], row = e * p.F + a.tile * 128;
+                    const size_t at = ((size_t)(e * tiles1 + a.tile) * g1 + a.k) * TILE_BYTES;
+                    if (elect_one()) {
+                        mbar_expect_tx(&full[s], 2 * 8192 + 2 * TILE_BYTES);     // spread codes count as they are in memory
                         tma_load_2d(st, &map_gate, &full[s], a.k * 128, row);
                         tma_load_2d(st + 16384, &map_up, &full[s], a.k * 128, row);
                         bulk_load(ss, p.gate_s + at, TILE_BYTES, &full[s]);
                         bulk_load(ss + TILE_BYTES, p.up_s + at, TILE_BYTES, &full[s]);
-                        a.next();
-                    } else {
-                        const int e = q.expert[b.l], t0 = b.tile * 2, row = e * p.H + t0 * 128;
+                    }
+                    a.next();
+                } else {
+                    const int e = q.expert[b.l], t0 = b.tile * 2, row = e * p.H + t0 * 128;
+                    if (elect_one()) {
+                        mbar_expect_tx(&full[s], 2 * 8192 + 2 * TILE_BYTES);
                         tma_load_2d(st, &map_down, &full[s], b.k * 128, row);
                         tma_load_2d(st + 16384, &map_down, &full[s], b.k * 128, row + 128);
                         bulk_load(ss, p.down_s + ((size_t)(e * tiles_h + t0) * g2 + b.k) * TILE_BYTES, TILE_BYTES, &full[s]);
                         // the last tile may have no partner: its scales again, never stored
                         bulk_load(ss + TILE_BYTES, p.down_s + ((size_t)(e * tiles_h + min(t0 + 1, tiles_h - 1)) * g2 + b.k) * TILE_BYTES, TILE_BYTES,
                                   &full[s]);
-                        b.next();
                     }
+                    b.next();
                 }
-                if (*abortp)
-                    for (int j = max(0, i - STAGES); j < i; ++j) mbar_wait(&full[j % STAGES], (j / STAGES) & 1, abortp);
+                __syncwarp();
+                if (++s == STAGES) { s = 0; parity ^= 1; }
             }
+            if (*abortp)
+                for (int j = max(0, i - STAGES); j < i; ++j) mbar_wait(&full[j % STAGES], (j / STAGES) & 1, abortp);
         } else if (warp == 2) {
             int seen = -1;
-            if (lane == 0) fence_async();
-            for (int i = 0; i < n; ++i) {
-                const int s = i % STAGES;
-                unsigned char *st = tiles + (size_t)s * C::STAGE + C::W_BYTES, *ss = sf + s * C::SF + 2 * TILE_BYTES;
-                int ok = 1;
-                if (lane == 0) {
-                    if (i >= STAGES) ok = mbar_wait(&empty[s], (i / STAGES - 1) & 1, abortp);
-                    if (ok && i >= n1 && b.l != seen) {
-                        ok = wait_count(&p.ready[b.l], tiles1, abortp);
-                        fence_async();
-                    }
-                }
-                if (!__shfl_sync(0xffffffffu, ok, 0)) break;
+            uint32_t parity = 1;
+            fence_async();
+            for (int i = 0, s = 0; i < n; ++i) {
+                if (!warp_wait(&empty[s], parity, abortp)) break;
+                unsigned char *st = tiles + s * C::STAGE + C::W_BYTES, *ss = sf + s * C::SF + 2 * TILE_BYTES;
                 if (i < n1) {
-                    if (lane == 0) {
+                    if (elect_one()) {
                         mbar_expect_tx(&full[s], C::X_BYTES + TILE_BYTES);
                         tma_load_2d(st, &map_x, &full[s], a.k * 128, 0);
                         bulk_load(ss, p.xs + (size_t)a.k * TILE_BYTES, TILE_BYTES, &full[s]);
                     }
                     a.next();
                 } else {
-                    seen = b.l;
+                    if (b.l != seen) {                           // all of this expert's h is there
+                        if (!__all_sync(0xffffffffu, wait_count(&p.ready[b.l], tiles1, abortp))) break;
+                        fence_async();
+                        seen = b.l;
+                    }
                     const int boxes = (q.count[b.l] + 7) / 8 * 2;
-                    if (lane == 0) {
+                    if (elect_one()) {
                         mbar_expect_tx(&full[s], boxes * 1024 + TILE_BYTES);
                         bulk_load(ss, p.hs + ((size_t)b.l * g2 + b.k) * TILE_BYTES, TILE_BYTES, &full[s]);
-                    }
-                    __syncwarp();
-                    if (lane < boxes) {
-                        fence_async();
-                        tma_load_2d(st + lane * 1024, &map_h, &full[s], b.k * 128, (q.hrow8[b.l] + lane) * 8);
+                        for (int j = 0; j < boxes; ++j) tma_load_2d(st + j * 1024, &map_h, &full[s], b.k * 128, (q.hrow8[b.l] + j) * 8);
                     }
                     b.next();
                 }
                 __syncwarp();
+                if (++s == STAGES) { s = 0; parity ^= 1; }
             }
         } else if (warp == 1) {
-            if (lane == 0) {
-                const uint64_t desc0 = umma_desc(smem_addr(tiles));
-                const uint32_t sf0 = smem_addr(sf);
-                int s = 0, buf = 0;
-                uint32_t parity = 0, acc_parity = 1;             // the first wait for each accumulator passes at once
-                bool fresh = true;
-                for (int i = 0; i < n; ++i) {
-                    if (fresh && !mbar_wait(&acc_empty[buf], acc_parity, abortp)) break;
-                    if (!mbar_wait(&full[s], parity, abortp)) break;
-                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    const uint32_t ss = sf0 + s * C::SF, tsf = tmem_sf + s * C::SF_COLS;
+            const uint64_t desc0 = umma_desc(smem_addr(tiles));
+            const uint32_t sf0 = smem_addr(sf);
+            int s = 0, buf = 0;
+            uint32_t parity = 0, acc_parity = 1;                 // the first wait for each accumulator passes at once
+            bool fresh = true;
+            for (int i = 0; i < n; ++i) {
+                if (fresh && !warp_wait(&acc_empty[buf], acc_parity, abortp)) break;
+                if (!warp_wait(&full[s], parity, abortp)) break;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const uint32_t ss = sf0 + s * C::SF, tsf = tmem_sf + s * C::SF_COLS;
+                const int cols = i < n1 ? NCOL : (q.count[b.l] + 7) / 8 * 16;
+                const uint32_t idesc = 5u << 7 | (uint32_t)(cols >> 3) << 17 | 1u << 23 | 1u << 27;           // E2M1 by E4M3, scales E8M0
+                const uint64_t da = desc0 + (uint32_t)(s * (C::STAGE >> 4)), db = da + (C::W_BYTES >> 4);
+                const uint32_t d = tmem + buf * 2 * NCOL;
+                const bool done = i == n1 - 1 || i == n - 1 || (i < n1 ? a.k == g1 - 1 : b.k == g2 - 1);
+                if (elect_one()) {
 #pragma unroll
                     for (int c = 0; c < 3; ++c) scales_to_tmem(tsf + c * 4, ss + c * TILE_BYTES);
-                    const int cols = i < n1 ? NCOL : (q.count[b.l] + 7) / 8 * 16;
-                    const uint32_t idesc = 5u << 7 | (uint32_t)(cols >> 3) << 17 | 1u << 23 | 1u << 27;       // E2M1 by E4M3, scales E8M0
-                    const uint64_t da = desc0 + (uint32_t)(s * (C::STAGE >> 4)), db = da + (C::W_BYTES >> 4);
-                    const uint32_t d = tmem + buf * 2 * NCOL;
 #pragma unroll
                     for (uint32_t j = 0; j < 4; ++j)
 #pragma unroll
                         for (int w = 0; w < 2; ++w)
                             umma_scaled<true>(d + w * NCOL, da + w * 1024 + 2 * j, db + 2 * j, idesc | j << 4 | j << 29, tsf + w * 4, tsf + 8, j > 0 || !fresh);
                     umma_commit(&empty[s]);
-                    const bool done = i == n1 - 1 || i == n - 1 || (i < n1 ? a.k == g1 - 1 : b.k == g2 - 1);
-                    if (i < n1) a.next();
-                    else b.next();
-                    fresh = done;
-                    if (done) {
-                        umma_commit(&acc_full[buf]);
-                        if (++buf == C::BUFS) { buf = 0; acc_parity ^= 1; }
-                    }
-                    if (++s == STAGES) { s = 0; parity ^= 1; }
+                    if (done) umma_commit(&acc_full[buf]);
                 }
+                __syncwarp();
+                if (i < n1) a.next();
+                else b.next();
+                fresh = done;
+                if (done && ++buf == C::BUFS) { buf = 0; acc_parity ^= 1; }
+                if (++s == STAGES) { s = 0; parity ^= 1; }
             }
         } else if (warp >= 4) {
             const int half = (warp - 4) / 4, quarter = warp & 3, row = quarter * 32 + lane;
@@ -417,7 +414,7 @@ moe_kernel(const __grid_constant__ CUtensorMap map_gate, const __grid_constant__
             auto release = [&]() {
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                 __syncwarp();
-                if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(&acc_empty[seg % C::BUFS])) : "memory");
+                if (lane == 0) mbar_arrive(&acc_empty[seg % C::BUFS]);
             };
             auto last_of = [&](int* counter, int others) {        // of the CTAs that share a tile
                 __threadfence();
