@@ -12,8 +12,8 @@
 //                most 2^-22 of it.  Up to 64 tokens hi and lo are columns of one instruction, added at the end (W is
 //                then read from shared memory once); for tiles of 128 tokens two instructions add to the same sums.
 //
-// A first kernel brings x to terms or codes (a thread 8 values), in the workspace of the call, and clears its counters.  The
-// second is persistent, a CTA an SM: warps 0 and 2 issue TMA loads into a ring of stages (W: for 16 bits 128 codes a row, which
+// Up to 32 tokens it is one kernel, whose CTAs each bring the parts of x that they meet to terms or codes on the way.  For more, a
+// first kernel does that once (a thread 8 values), in the workspace of the call, and clears its counters.  The product is persistent, a CTA an SM: warps 0 and 2 issue TMA loads into a ring of stages (W: for 16 bits 128 codes a row, which
 // TMA spreads to a byte each, for 4 bits 256; x), warp 1 the scale copies and the products, the warps from 4 on take the sums
 // out.
 // All of the product's blocks - (tile of W rows, tile of tokens, stage of K) - are dealt to the CTAs evenly as one long
@@ -30,7 +30,8 @@ namespace mx {
 // ---- x to terms or codes ------------------------------------------------------------------------------------------------
 
 // act 16: terms uint8 [token tile][2 tt][Kp], a tile's hi rows, then its lo rows; scales [token tile][groups][atoms][512],
-// the tiles of 128 such rows.  act 4: codes and scales as in mxfp4.cuh.  Rows that have no token are left as they are.
+// the tiles of 128 such rows.  act 4: codes as in mxfp4.cuh, scales [token tile][groups][512].  Rows that have no token are left as
+// they are.
 template <bool A16>
 __global__ void __launch_bounds__(256) prepare_kernel(const __nv_bfloat16* __restrict__ x_in, long long ldx, int M, int K, int groups, int wide,
                                                       int tt, uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, int* __restrict__ counters,
@@ -80,24 +81,28 @@ __global__ void __launch_bounds__(256) prepare_kernel(const __nv_bfloat16* __res
 #pragma unroll
                 for (int j = 0; j < 4; ++j) word |= pack2(v[2 * j] * inv, v[2 * j + 1] * inv) << (8 * j);
             *reinterpret_cast<uint32_t*>(codes + (size_t)r * (groups * (GROUP / 2)) + c / 2) = word;
-            if ((threadIdx.x & 3) == 0) scales[scale_at(r, c / BLOCK, groups)] = (uint8_t)byte;
+            const int tile = r / tt, t = r - tile * tt;
+            if ((threadIdx.x & 3) == 0)
+                scales[((size_t)tile * groups + c / GROUP) * TILE_BYTES + (t & 31) * 16 + t / 32 * 4 + c % GROUP / BLOCK] = (uint8_t)byte;
         }
     }
 }
 
 // ---- the product --------------------------------------------------------------------------------------------------------
 
-template <bool A16_, int TT_, int W_> struct Cfg {
-    static constexpr bool A16 = A16_;
+// FUSED: the product brings x to terms itself (no first kernel)
+template <bool A16_, int TT_, int W_, int GS_, bool FUSED_> struct Cfg {
+    static constexpr bool A16 = A16_, FUSED = FUSED_;
     static constexpr int TT = TT_, W = W_;                         // tokens of a tile; tiles of 128 rows of W that share it
     static constexpr bool SIDE = A16 && TT <= 64;                  // hi and lo side by side as columns
-    static constexpr int GS = A16 ? 1 : 2;                         // groups of 128 along K in a stage (128 bytes of a row)
+    static constexpr int GS = GS_;                                 // groups of 128 along K in a stage
+    static constexpr int SUBS = A16 ? GS : GS / 2;                 // tiles of 128 bytes a row that hold them
     static constexpr int XR = A16 ? 2 * TT : TT;                   // rows of x's tile
     static constexpr int NCOL = SIDE ? 2 * TT : TT;                // N of the instruction
     static constexpr int ATOMS = (XR + 127) / 128;                 // tiles of scales of x
-    static constexpr int W_BYTES = W * 16384, X_BYTES = XR * 128, STAGE = W_BYTES + X_BYTES;
+    static constexpr int W_BYTES = W * SUBS * 16384, X_BYTES = SUBS * XR * 128, STAGE = W_BYTES + X_BYTES;
     // bytes that W's loads of a stage report: codes that TMA spreads count as they are in memory, 64 bytes a row
-    static constexpr int W_ARRIVE = W * (A16 ? 8192 : 16384);
+    static constexpr int W_ARRIVE = W * SUBS * (A16 ? 8192 : 16384);
     static constexpr int SF = GS * TILE_BYTES * (W + ATOMS);       // scale bytes of a stage
     static constexpr int FIT = (216 * 1024) / (STAGE + SF);
     static constexpr int SF_COLS = GS * 4 * (W + ATOMS);           // their columns in tensor memory: every stage has its own
@@ -105,9 +110,10 @@ template <bool A16_, int TT_, int W_> struct Cfg {
     static constexpr int BUFS = 2 * W * NCOL + STAGES * SF_COLS <= 512 ? 2 : 1;
     static constexpr int COLS_USED = BUFS * W * NCOL + STAGES * SF_COLS;
     static constexpr int COLS = COLS_USED <= 64 ? 64 : COLS_USED <= 128 ? 128 : COLS_USED <= 256 ? 256 : 512;
-    static constexpr int EPI_WARPS = 4 * W, THREADS = 128 + 32 * EPI_WARPS;
+    static constexpr int EPI_WARPS = 4 * W, FIRST_X = 4 + EPI_WARPS, X_WARPS = 8;
+    static constexpr int THREADS = 32 * (4 + EPI_WARPS + (FUSED ? X_WARPS : 0));
     static constexpr size_t SMEM = (size_t)STAGES * (STAGE + SF) + 1024 + 512;
-    static_assert(COLS_USED <= 512 && STAGES >= 3, "tensor memory or shared memory");
+    static_assert(COLS_USED <= 512 && STAGES >= 3 && (A16 || GS % 2 == 0) && (!FUSED || TT <= 32) && (!FUSED || GS * TT / 2 % X_WARPS == 0), "tensor memory, shared memory or form");
 };
 
 // Instruction descriptor: element kinds (mxf8f6f4: A E2M1 = 5, B E4M3 = 0; mxf4: E2M1 = 1 on both sides), N / 8, scales E8M0,
@@ -118,6 +124,9 @@ template <typename C> __device__ __forceinline__ constexpr uint32_t idesc_of(int
 
 struct Product {
     const uint8_t *w_scales, *x_scales;
+    const __nv_bfloat16* x;    // (fused) as it is
+    long long ldx;
+    int K, wide;
     const void* bias;
     void* y;
     float* part;               // [P][2][W][TT][128]
@@ -142,7 +151,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, cta = blockIdx.x;
     if (threadIdx.x == 0) {
         abort_flag = 0;
-        for (int s = 0; s < STAGES; ++s) { mbar_init(&full[s], 2); mbar_init(&empty[s], 1); }
+        for (int s = 0; s < STAGES; ++s) { mbar_init(&full[s], C::FUSED ? 1 + C::X_WARPS : 2); mbar_init(&empty[s], 1); }
         for (int s = 0; s < C::BUFS; ++s) { mbar_init(&acc_full[s], 1); mbar_init(&acc_empty[s], C::EPI_WARPS); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -159,12 +168,13 @@ product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
 
     // unit u: token tile u % mtiles of the W tiles W (u / mtiles) .. + W - 1.  The loops below carry their place along: one
     // thread's integer divisions would take longer than a block's products.
-    if (warp == 0 || warp == 2) {
-        // warp 0: W and its scales, from the start; warp 2: x's, once they exist
-        const bool is_w = warp == 0;
+    if (warp == 0 || (warp == 2 && !C::FUSED)) {
+        // warp 0: W and its scales; warp 2: x's.  W waits for nobody where the kernel before this one is x's own, which began
+        // after everything before it had ended
+        const bool is_w = C::FUSED || warp == 0;
         const int u0 = b0 / kb;
         int k = b0 - u0 * kb, m = u0 % p.mtiles, t0 = u0 / p.mtiles * W;
-        if (!is_w) pdl_wait();
+        if (C::FUSED || !is_w) pdl_wait();
         uint32_t parity = 1;                                             // the first round passes at once
         int s = 0, i = 0;
         for (; i < n; ++i) {
@@ -176,14 +186,18 @@ product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
                     mbar_expect_tx(&full[s], C::W_ARRIVE + gs * TILE_BYTES * W);
 #pragma unroll
                     for (int w = 0; w < W; ++w) {
-                        tma_load_2d(st + w * 16384, &map_w, &full[s], k * 128, (t0 + w) * 128);
+#pragma unroll
+                        for (int b = 0; b < C::SUBS; ++b)
+                            tma_load_2d(st + (w * C::SUBS + b) * 16384, &map_w, &full[s], (k * C::SUBS + b) * 128, (t0 + w) * 128);
                         const int t = min(t0 + w, p.ntiles - 1);         // the last tile may have no partner: its scales again, never stored
                         bulk_load(ss + w * C::GS * TILE_BYTES, p.w_scales + ((size_t)t * p.groups + k * C::GS) * TILE_BYTES, gs * TILE_BYTES, &full[s]);
                     }
                 }
             } else if (elect_one()) {
                 mbar_expect_tx(&full[s], C::X_BYTES + gs * TILE_BYTES * C::ATOMS);
-                tma_load_2d(st + C::W_BYTES, &map_x, &full[s], k * 128, m * C::XR);
+#pragma unroll
+                for (int b = 0; b < C::SUBS; ++b)
+                    tma_load_2d(st + C::W_BYTES + b * (C::XR * 128), &map_x, &full[s], (k * C::SUBS + b) * 128, m * C::XR);
                 bulk_load(ss + W * C::GS * TILE_BYTES, p.x_scales + ((size_t)m * p.groups + k * C::GS) * (C::ATOMS * TILE_BYTES),
                           gs * C::ATOMS * TILE_BYTES, &full[s]);
             }
@@ -197,21 +211,107 @@ product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
         if (is_w) pdl_trigger_gemm();
         if (*abortp)                                                     // what is in flight gets a bounded chance to land
             for (int j = max(0, i - STAGES); j < i; ++j) mbar_wait(&full[j % STAGES], (j / STAGES) & 1, abortp);
+    } else if (C::FUSED && warp >= C::FIRST_X) {
+        // All of these warps share a stage: an item is two tokens' values of a group, 8 to a lane; those of AHEAD stages are on their way.
+        constexpr int ITEMS = C::GS * TT / 2 / C::X_WARPS, AHEAD = 3;
+        pdl_wait();
+        const __nv_bfloat16* x = pdl_fresh(p.x);
+        const int c = (lane & 15) * 8, first = warp - C::FIRST_X;
+        uint4 raw[AHEAD][ITEMS];
+        int kl = b0 % kb, il = 0;                                        // the next stage to be asked for
+        auto ask = [&](uint4 (&to)[ITEMS]) {
+            if (il >= n) return;
+#pragma unroll
+            for (int j = 0; j < ITEMS; ++j) {
+                const int item = first + C::X_WARPS * j, t = item % (TT / 2) * 2 + (lane >> 4), at = (kl * C::GS + item / (TT / 2)) * GROUP + c;
+                const __nv_bfloat16* from = x + (long long)t * p.ldx + at;
+                if (p.wide && t < p.M && at + 8 <= p.K) {
+                    to[j] = *reinterpret_cast<const uint4*>(from);
+                } else {
+                    __nv_bfloat16 v[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[e] = t < p.M && at + e < p.K ? from[e] : __nv_bfloat16(0.f);
+                    to[j] = *reinterpret_cast<const uint4*>(v);
+                }
+            }
+            ++il;
+            if (++kl == kb) kl = 0;
+        };
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) ask(raw[u]);
+        uint32_t parity = 1;
+        int s = 0;
+        bool ok = true;
+        for (int i0 = 0; i0 < n && ok; i0 += AHEAD) {
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u) {
+                if (i0 + u >= n) break;
+                ok = warp_wait(&empty[s], parity, abortp);
+                if (!ok) break;
+                unsigned char *xt = tiles + s * C::STAGE + C::W_BYTES, *ss = sf + s * C::SF + W * C::GS * TILE_BYTES;
+#pragma unroll
+                for (int j = 0; j < ITEMS; ++j) {
+                    const int item = first + C::X_WARPS * j, t = item % (TT / 2) * 2 + (lane >> 4), g = item / (TT / 2);
+                    float v[8];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float2 f = __bfloat1622float2(reinterpret_cast<const __nv_bfloat162*>(&raw[u][j])[e]);
+                        v[2 * e] = f.x, v[2 * e + 1] = f.y;
+                    }
+                    uint32_t most = 0;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) most = max(most, __float_as_uint(v[e]) & 0x7fffffffu);
+                    most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+                    most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
+                    unsigned char* sc = ss + g * C::ATOMS * TILE_BYTES + (lane & 15) / 4;
+                    if (C::A16) {                                        // 16-byte pieces of a row change places by the row's number
+                        const int byte = term_byte(most);
+                        uint32_t hi[2], lo[2];
+                        terms_of<8>(v, byte, hi, lo);
+                        unsigned char* to = xt + g * (C::XR * 128) + t * 128 + ((((lane & 15) >> 1) ^ (t & 7)) << 4) + (lane & 1) * 8;
+                        *reinterpret_cast<uint2*>(to) = make_uint2(hi[0], hi[1]);
+                        *reinterpret_cast<uint2*>(to + TT * 128) = make_uint2(lo[0], lo[1]);
+                        if ((lane & 3) == 0) {
+                            sc[(t & 31) * 16 + t / 32 * 4] = (uint8_t)byte;
+                            sc[((t + TT) & 31) * 16 + (t + TT) / 32 * 4] = low_byte(byte);
+                        }
+                    } else {
+                        const int byte = scale_byte(most);
+                        const float inv = scale_inverse(byte);
+                        uint32_t word = 0;
+                        if (byte != 255)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) word |= pack2(v[2 * e] * inv, v[2 * e + 1] * inv) << (8 * e);
+                        *reinterpret_cast<uint32_t*>(xt + g / 2 * (C::XR * 128) + t * 128 + ((((g & 1) * 4 + (lane & 15) / 4) ^ (t & 7)) << 4) +
+                                                     (lane & 3) * 4) = word;
+                        if ((lane & 3) == 0) sc[(t & 31) * 16 + t / 32 * 4] = (uint8_t)byte;
+                    }
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&full[s]);
+                ask(raw[u]);
+                if (++s == STAGES) { s = 0; parity ^= 1; }
+            }
+        }
     } else if (warp == 1) {
         const uint64_t desc0 = umma_desc(smem_addr(tiles));              // (offsets stay within the address field: 16-byte steps of 227 KB)
         const uint32_t sf0 = smem_addr(sf);
         int k = b0 % kb, s = 0, buf = 0;
         uint32_t parity = 0, acc_parity = 1;                             // the first wait for each accumulator passes at once
-        bool fresh = true;
+        bool fresh = true, ready = false;
         for (int i = 0; i < n; ++i) {
             if (fresh && !warp_wait(&acc_empty[buf], acc_parity, abortp)) break;
-            if (!warp_wait(&full[s], parity, abortp)) break;
+            if (!__all_sync(0xffffffffu, ready) && !warp_wait(&full[s], parity, abortp)) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const uint32_t ss = sf0 + s * C::SF, tsf = tmem_sf + s * C::SF_COLS;
             const int gs = C::GS == 1 ? 1 : min(C::GS, p.groups - k * C::GS);
             const uint64_t da = desc0 + (uint32_t)(s * (C::STAGE >> 4)), db = da + (C::W_BYTES >> 4);
             const uint32_t d = tmem + buf * W * C::NCOL;
             const bool done = ++k == kb || i == n - 1;
+            const int s_now = s;
+            if (++s == STAGES) { s = 0; parity ^= 1; }
+            ready = mbar_try_wait(&full[s], parity);                     // of the next stage: the answer comes while products are issued
             if (elect_one()) {
 #pragma unroll
                 for (int g = 0; g < C::GS; ++g) {
@@ -221,18 +321,20 @@ product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
 #pragma unroll
                     for (int a = 0; a < C::ATOMS; ++a)
                         scales_to_tmem(tsf + (W * C::GS + g * C::ATOMS + a) * 4, ss + (W * C::GS + g * C::ATOMS + a) * TILE_BYTES);
+                    const int sub = C::A16 ? g : g / 2;
 #pragma unroll
-                    for (int j = 0; j < 4 / C::GS; ++j)                  // 32 bytes of a row each: 32 or 64 elements
+                    for (int j = 0; j < (C::A16 ? 4 : 2); ++j)           // 32 bytes of a row each: 32 or 64 elements
 #pragma unroll
                         for (int w = 0; w < W; ++w) {
-                            const int id = C::A16 ? j : j * 2, at = 2 * (g * (4 / C::GS) + j);
+                            const int id = C::A16 ? j : j * 2, at = C::A16 ? 2 * j : 2 * ((g & 1) * 2 + j);
+                            const uint64_t a = da + (w * C::SUBS + sub) * 1024 + at, b = db + sub * (C::XR * 128 >> 4) + at;
                             const uint32_t sa = tsf + (w * C::GS + g) * 4, sb = tsf + (W * C::GS + g * C::ATOMS) * 4;
-                            umma_scaled<C::A16>(d + w * C::NCOL, da + w * 1024 + at, db + at, idesc_of<C>(id), sa, sb, g > 0 || j > 0 || !fresh);
+                            umma_scaled<C::A16>(d + w * C::NCOL, a, b, idesc_of<C>(id), sa, sb, g > 0 || j > 0 || !fresh);
                             if (C::A16 && !C::SIDE)
-                                umma_scaled<C::A16>(d + w * C::NCOL, da + w * 1024 + at, db + (TT * 128 >> 4) + at, idesc_of<C>(id), sa, sb + 4, 1);
+                                umma_scaled<C::A16>(d + w * C::NCOL, a, b + (TT * 128 >> 4), idesc_of<C>(id), sa, sb + 4, 1);
                         }
                 }
-                umma_commit(&empty[s]);
+                umma_commit(&empty[s_now]);
                 if (done) umma_commit(&acc_full[buf]);
             }
             __syncwarp();
@@ -241,9 +343,8 @@ product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
                 k = 0;
                 if (++buf == C::BUFS) { buf = 0; acc_parity ^= 1; }
             }
-            if (++s == STAGES) { s = 0; parity ^= 1; }
         }
-    } else if (warp >= 4) {
+    } else if (warp >= 4 && warp < C::FIRST_X) {
         // warps of one tile of W rows: 4 + 4 w .. 7 + 4 w; TMEM lanes (warp % 4) * 32 .. + 31
         const int w = (warp - 4) / 4, q = warp & 3, row = q * 32 + lane;
         pdl_wait();
@@ -303,6 +404,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
             if (threadIdx.x == 128) is_last = atomicAdd(&p.counters[u], 1) == c1 - c0;
             asm volatile("bar.sync 1, %0;" ::"n"(C::EPI_WARPS * 32) : "memory");
             if (!is_last) continue;
+            if (C::FUSED && threadIdx.x == 128) p.counters[u] = 0;        // as the next launch expects it
             __threadfence();
 #pragma unroll 1
             for (int t0 = 0; t0 < tokens; t0 += 8) {
@@ -329,33 +431,57 @@ product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
 
 // ---- host side ----------------------------------------------------------------------------------------------------------
 
-// tokens of a tile and tiles of W that share one
-inline void tiles_for(int M, int act_bits, int& tt, int& w) {
-    tt = M <= 8 && act_bits == 16 ? 8 : M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128;
-    w = tt >= 32 ? 2 : 1;
-}
+constexpr int MOST_COUNTERS = 4096;       // tiles of the fused form: counters of the stream's, which the kernel leaves at zero
 
+// A form of the product and how many CTAs share its blocks
 struct Plan {
-    int tt, w, groups, mtiles, ntiles, kb, P;
+    int tt, w, gs, groups, mtiles, ntiles, kb, P;
+    bool fused;
     long long units, codes, scales, parts, counters, bytes;       // bytes from the workspace's start
 };
+// Tiles of 8 to 64 tokens take all tokens at once; more tokens go by tiles of 128, or 64 where that leaves SMs without work.
+// A unit's K is shared by so many CTAs that the blocks of the busiest (block: what one takes) and the joining of partial sums (1.5 us
+// for handing over, then the bytes of each share) take least: 159 x 777 x 4,407: 173 us dealt to all SMs, 4,608 x 3,584 by 1 token ... 
 inline Plan plan_for(int M, int N, int K, int act_bits) {
-    Plan q;
-    tiles_for(M, act_bits, q.tt, q.w);
-    q.groups = groups_of(K);
-    q.mtiles = (M + q.tt - 1) / q.tt;
-    q.ntiles = (N + 127) / 128;
-    q.kb = act_bits == 16 ? q.groups : (q.groups + 1) / 2;
-    q.units = (long long)((q.ntiles + q.w - 1) / q.w) * q.mtiles;
-    const long long total = q.units * q.kb;
-    q.P = (int)(total < sm_count() ? total : sm_count());
-    const int xr = act_bits == 16 ? 2 * q.tt : q.tt, atoms = (xr + 127) / 128;
+    Plan best;
+    float best_us = 1e30f;
+    const bool a16 = act_bits == 16;
+    const int sms = sm_count();
+    const bool many_tiles = N > MOST_COUNTERS * 128LL;              // more than the fused form has counters for
+    for (int tt = many_tiles ? 64 : a16 && M <= 8 ? 8 : M <= 16 ? 16 : M <= 32 ? 32 : 64;; tt *= 2) {
+        Plan q;
+        q.tt = tt;
+        q.w = tt >= 32 ? 2 : 1;
+        q.gs = (a16 ? 1 : 2) * (tt <= 16 ? 2 : 1);
+        q.fused = tt <= 32;
+        q.groups = groups_of(K);
+        q.mtiles = (M + tt - 1) / tt;
+        q.ntiles = (N + 127) / 128;
+        q.kb = (q.groups + q.gs - 1) / q.gs;
+        q.units = (long long)((q.ntiles + q.w - 1) / q.w) * q.mtiles;
+        const long long total = q.units * q.kb;
+        const float block = tt <= 16 ? 0.40f : tt == 32 ? 0.42f : tt == 64 ? 0.48f : (a16 ? 0.75f : 0.55f);
+        const float share = (float)(tt * q.w) / 256.f;
+        for (int split = 1; split <= q.kb; split += split < 4 ? 1 : split / 4) {
+            const long long want = q.units * split;
+            q.P = (int)(want < sms ? want : sms);
+            if (q.P > total) q.P = (int)total;
+            const long long each = (total + q.P - 1) / q.P;
+            const int shares = each >= q.kb && total % q.P == 0 ? 1 : (int)((q.kb + each - 1) / each) + (want > sms);
+            const float us = each * block + (shares > 1 ? 1.5f + shares * share : 0.f);
+            if (us < best_us) { best_us = us; best = q; }
+            if (want >= sms) break;
+        }
+        if (tt >= (M <= 64 ? tt : 128)) break;
+    }
+    Plan& q = best;
+    const int xr = a16 ? 2 * q.tt : q.tt, atoms = (xr + 127) / 128;
     auto up = [](long long b) { return (b + 1023) / 1024 * 1024; };
     q.codes = 0;
-    q.scales = up(act_bits == 16 ? (long long)q.mtiles * xr * q.groups * GROUP : (long long)M * q.groups * (GROUP / 2));
-    q.parts = q.scales + up((long long)q.mtiles * q.groups * atoms * TILE_BYTES);
+    q.scales = q.fused ? 0 : up(a16 ? (long long)q.mtiles * xr * q.groups * GROUP : (long long)M * q.groups * (GROUP / 2));
+    q.parts = q.scales + (q.fused ? 0 : up((long long)q.mtiles * q.groups * atoms * TILE_BYTES));
     q.counters = q.parts + up((long long)q.P * 2 * q.w * q.tt * 128 * 4);
-    q.bytes = q.counters + up(q.units * 4);
+    q.bytes = q.counters + (q.fused ? 0 : up(q.units * 4));
     return q;
 }
 
@@ -377,9 +503,10 @@ PRISM_EXPORT int prism_mxfp4_linear_workspace(int M, int N, int K, int act_bits,
 }
 
 // x [M, K] bfloat16 (row stride ldx); codes, scales: W [N, K]; y [M, N] of `out_dtype` (row stride ldy); act_bits 16 or 4;
-// ws: workspace of the call (prism_mxfp4_linear_workspace), 1024-byte aligned
+// ws: workspace of the call (prism_mxfp4_linear_workspace), 256-byte aligned; counters: at least ceil(N / 128) ints (4,096 always
+// suffice), zero before the first launch (the kernel leaves them zero), of one stream's launches at a time
 PRISM_EXPORT int prism_mxfp4_linear(const void* x, long long ldx, const void* codes, const void* scales, const void* bias, int bias_dtype,
-                                    void* y, int out_dtype, long long ldy, int M, int N, int K, int act_bits, void* ws, int* err,
+                                    void* y, int out_dtype, long long ldy, int M, int N, int K, int act_bits, void* ws, int* counters, int* err,
                                     cudaStream_t stream) {
     using namespace prism;
     using namespace prism::mx;
@@ -390,45 +517,44 @@ PRISM_EXPORT int prism_mxfp4_linear(const void* x, long long ldx, const void* co
     if (q.units * q.kb > 0x7fffffffLL) return (int)cudaErrorInvalidValue;
     uint8_t* base = static_cast<uint8_t*>(ws);
     const bool a16 = act_bits == 16;
-    const int xr = a16 ? 2 * q.tt : q.tt;
     CUtensorMap mw, mx;
     int rc = byte_map(&mw, codes, N, (long long)q.groups * (GROUP / 2), 128, a16);
-    if (rc) return rc;
-    rc = a16 ? byte_map(&mx, base + q.codes, (long long)q.mtiles * xr, (long long)q.groups * GROUP, xr, false)
-             : byte_map(&mx, base + q.codes, M, (long long)q.groups * (GROUP / 2), xr, false);
     if (rc) return rc;
     Product p;
     p.w_scales = static_cast<const uint8_t*>(scales);
     p.x_scales = base + q.scales;
+    p.x = static_cast<const __nv_bfloat16*>(x);
+    p.ldx = ldx;
+    p.K = K;
+    p.wide = ((uintptr_t)x & 15) == 0 && ldx % 8 == 0;
     p.bias = bias;
     p.y = y;
     p.part = reinterpret_cast<float*>(base + q.parts);
-    p.counters = reinterpret_cast<int*>(base + q.counters);
+    p.counters = q.fused ? counters : reinterpret_cast<int*>(base + q.counters);
     p.err = err;
     p.ldy = ldy;
     p.split = Split((int)(q.units * q.kb), q.P, q.kb);
     p.M = M, p.N = N, p.groups = q.groups, p.mtiles = q.mtiles, p.ntiles = q.ntiles;
     p.bias_bf16 = bias_dtype == PRISM_DTYPE_BF16, p.out_bf16 = out_dtype == PRISM_DTYPE_BF16;
+    if (q.fused) {
+        if (a16) {
+            switch (q.tt) {
+                case 8: return run_product<Cfg<true, 8, 1, 2, true>>(mw, mw, p, stream);
+                case 16: return run_product<Cfg<true, 16, 1, 2, true>>(mw, mw, p, stream);
+                default: return run_product<Cfg<true, 32, 2, 1, true>>(mw, mw, p, stream);
+            }
+        }
+        return q.tt == 16 ? run_product<Cfg<false, 16, 1, 4, true>>(mw, mw, p, stream) : run_product<Cfg<false, 32, 2, 2, true>>(mw, mw, p, stream);
+    }
+    const int xr = a16 ? 2 * q.tt : q.tt;
+    rc = a16 ? byte_map(&mx, base + q.codes, (long long)q.mtiles * xr, (long long)q.groups * GROUP, xr, false)
+             : byte_map(&mx, base + q.codes, M, (long long)q.groups * (GROUP / 2), xr, false);
+    if (rc) return rc;
     const long long threads = (long long)M * q.groups * 16, most = threads > q.units ? threads : q.units;
     const int blocks = (int)((most + 255) / 256 < 148 * 8 ? (most + 255) / 256 : 148 * 8);
-    const int wide = ((uintptr_t)x & 15) == 0 && ldx % 8 == 0;
-    const __nv_bfloat16* xb = static_cast<const __nv_bfloat16*>(x);
-    rc = (int)launch_kernel(a16 ? prepare_kernel<true> : prepare_kernel<false>, dim3(blocks), dim3(256), 0, stream, xb, ldx, M, K, q.groups, wide,
+    rc = (int)launch_kernel(a16 ? prepare_kernel<true> : prepare_kernel<false>, dim3(blocks), dim3(256), 0, stream, p.x, ldx, M, K, q.groups, p.wide,
                             q.tt, base + q.codes, base + q.scales, p.counters, (int)q.units);
     if (rc) return rc;
-    if (a16) {
-        switch (q.tt) {
-            case 8: return run_product<Cfg<true, 8, 1>>(mw, mx, p, stream);
-            case 16: return run_product<Cfg<true, 16, 1>>(mw, mx, p, stream);
-            case 32: return run_product<Cfg<true, 32, 2>>(mw, mx, p, stream);
-            case 64: return run_product<Cfg<true, 64, 2>>(mw, mx, p, stream);
-            default: return run_product<Cfg<true, 128, 2>>(mw, mx, p, stream);
-        }
-    }
-    switch (q.tt) {
-        case 16: return run_product<Cfg<false, 16, 1>>(mw, mx, p, stream);
-        case 32: return run_product<Cfg<false, 32, 2>>(mw, mx, p, stream);
-        case 64: return run_product<Cfg<false, 64, 2>>(mw, mx, p, stream);
-        default: return run_product<Cfg<false, 128, 2>>(mw, mx, p, stream);
-    }
+    if (a16) return q.tt == 64 ? run_product<Cfg<true, 64, 2, 1, false>>(mw, mx, p, stream) : run_product<Cfg<true, 128, 2, 1, false>>(mw, mx, p, stream);
+    return q.tt == 64 ? run_product<Cfg<false, 64, 2, 2, false>>(mw, mx, p, stream) : run_product<Cfg<false, 128, 2, 2, false>>(mw, mx, p, stream);
 }

@@ -10,6 +10,7 @@ namespace mx {
 
 using tc::mbar_expect_tx;
 using tc::mbar_init;
+using tc::mbar_try_wait;
 using tc::mbar_wait;
 using tc::smem_addr;
 using tc::tma_load_2d;

@@ -159,7 +159,7 @@ class _Sig:
     prism_swiglu = [_p, _p, _i, _i, _i, _p]
     prism_mxfp4_quantize = [_p, _i, _ll, _i, _i, _i, _p, _p, _p]
     prism_mxfp4_dequantize = [_p, _p, _i, _i, _i, _p, _i, _p]
-    prism_mxfp4_linear = [_p, _ll, _p, _p, _p, _i, _p, _i, _ll, _i, _i, _i, _i, _p, _p, _p]
+    prism_mxfp4_linear = [_p, _ll, _p, _p, _p, _i, _p, _i, _ll, _i, _i, _i, _i, _p, _p, _p, _p]
     prism_mxfp4_linear_workspace = [_i, _i, _i, _i, _p]
     prism_mxfp4_moe = [_p, _ll, _p, _i, _p, _i, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _i, _i, _i, _f, _p, _i, _i, _i, _f, _f,
                        _p, _i, _ll, _p, _p, _p, _p]
@@ -435,6 +435,7 @@ def check_tc_errors():
         code = int(word.item())
         if code:
             word.zero_()
+            mxfp4._clear_counters()
             raise KernelError(f"tensor-core GEMM: device error {code} (a bounded wait ran out)")
 
 
@@ -2483,4 +2484,5 @@ def moe_feed_forward(ctx, x: torch.Tensor, logits: torch.Tensor, gate_up_w: torc
     return y
 
 
+from . import mxfp4      # noqa: E402
 from .mxfp4 import Mxfp4, mxfp4_linear, mxfp4_moe, mxfp4_quantize      # noqa: E402,F401

@@ -112,20 +112,43 @@ def _err_word(device: torch.device) -> int:
     return p
 
 
-_control_blocks = {}
+_COUNTERS = 4096             # of a stream: tiles of a product (csrc/mxfp4_linear.cu), or 66 of an experts' layer
+_SCRATCH = 16 << 20          # a larger workspace is the call's own
+_ARENA = 1 << 20
+_streams = {}                # (device, stream) -> [counters, workspace]: launches of one stream follow each other
+_arenas = {}                 # device -> [counters for captured calls, how many are given away]
 
 
-def _control(stream: int, device: torch.device) -> torch.Tensor:
-    """The counters that the experts' launch synchronises with and leaves at zero: a block of its own for each stream, as
-    launches of one stream follow each other; under graph capture one for the call, cleared by the graph, as graphs may run on
-    any stream."""
-    if torch.cuda.is_current_stream_capturing():
-        return torch.zeros(66, dtype=torch.int32, device=device)
-    key = (device.index, stream)
-    block = _control_blocks.get(key)
-    if block is None:
-        block = _control_blocks[key] = torch.zeros(66, dtype=torch.int32, device=device)
-    return block
+def _call_memory(stream: int, device: torch.device, nbytes: int, counters: int):
+    """``(workspace, counters)`` of a call.  Counters are zero before a launch and left so.  Under graph capture a call gets
+    counters of its own for good, as graphs may run on any stream, and a workspace of the graph's."""
+    if torch._C._cuda_isCurrentStreamCapturing():
+        arena = _arenas.get(device.index)
+        counters = (counters + 63) // 64 * 64
+        if arena is None or arena[1] + counters > _ARENA:
+            block = torch.zeros(counters, dtype=torch.int32, device=device)            # cleared by the graph
+        else:
+            block = arena[0][arena[1]:arena[1] + counters]
+            arena[1] += counters
+        return torch.empty(nbytes, dtype=torch.uint8, device=device), block
+    own = _streams.get((device.index, stream))
+    if own is None:
+        if device.index not in _arenas:
+            _arenas[device.index] = [torch.zeros(_ARENA, dtype=torch.int32, device=device), 0]
+            torch.cuda.current_stream(device).synchronize()      # captured calls of any stream find it cleared
+        own = _streams[(device.index, stream)] = [torch.zeros(_COUNTERS, dtype=torch.int32, device=device), None]
+    if nbytes > _SCRATCH:
+        return torch.empty(nbytes, dtype=torch.uint8, device=device), own[0]
+    if own[1] is None or own[1].numel() < nbytes:
+        own[1] = torch.empty(max(nbytes, 4 << 20), dtype=torch.uint8, device=device)
+    return own[1], own[0]
+
+
+def _clear_counters():
+    """After a launch that gave up its counters may be anything (``ops.check_tc_errors``, which has waited for the device)."""
+    for block in list(_streams.values()) + list(_arenas.values()):
+        block[0].zero_()
+    torch.cuda.synchronize()
 
 
 def mxfp4_linear(x: torch.Tensor, w: Mxfp4, bias: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
@@ -151,11 +174,12 @@ def mxfp4_linear(x: torch.Tensor, w: Mxfp4, bias: Optional[torch.Tensor] = None,
         raise ops.KernelError(f"the result of {tuple(xs)} and {tuple(ws)} does not go into {tuple(out.shape)} {out.dtype}")
     if M == 0:
         return out
-    work = torch.empty(_workspace("prism_mxfp4_linear_workspace", M, N, K, act_bits), dtype=torch.uint8, device=x.device)
+    stream = ops._stream()
+    work, counters = _call_memory(stream, x.device, _workspace("prism_mxfp4_linear_workspace", M, N, K, act_bits), min(-(-N // 128), _COUNTERS))
     ops._check(ops.lib().prism_mxfp4_linear(x.data_ptr(), x.stride(0), w.codes.data_ptr(), w.scales.data_ptr(),
                                             None if bias is None else bias.data_ptr(), 0 if bias is None else ops._dt(bias), out.data_ptr(),
-                                            ops._dt(out), out.stride(0), M, N, K, act_bits, work.data_ptr(), _err_word(x.device), ops._stream()),
-               "mxfp4_linear")
+                                            ops._dt(out), out.stride(0), M, N, K, act_bits, work.data_ptr(), counters.data_ptr(),
+                                            _err_word(x.device), stream), "mxfp4_linear")
     return out
 
 
@@ -201,8 +225,7 @@ def mxfp4_moe(x: torch.Tensor, router: torch.Tensor, gate: Mxfp4, up: Mxfp4, dow
     if T == 0:
         return out
     stream = ops._stream()
-    work = torch.empty(_workspace("prism_mxfp4_moe_workspace", T, H, F, E, top), dtype=torch.uint8, device=x.device)
-    control = _control(stream, x.device)
+    work, control = _call_memory(stream, x.device, _workspace("prism_mxfp4_moe_workspace", T, H, F, E, top), 66)
     ops._check(ops.lib().prism_mxfp4_moe(x.data_ptr(), x.stride(0), router.data_ptr(), ops._dt(router),
                                          None if router_bias is None else router_bias.data_ptr(), 0 if router_bias is None else ops._dt(router_bias),
                                          gate.codes.data_ptr(), gate.scales.data_ptr(), up.codes.data_ptr(), up.scales.data_ptr(),
