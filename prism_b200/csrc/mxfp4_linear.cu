@@ -110,8 +110,8 @@ template <bool A16_, int TT_, int W_, int GS_, bool FUSED_> struct Cfg {
     static constexpr int BUFS = 2 * W * NCOL + STAGES * SF_COLS <= 512 ? 2 : 1;
     static constexpr int COLS_USED = BUFS * W * NCOL + STAGES * SF_COLS;
     static constexpr int COLS = COLS_USED <= 64 ? 64 : COLS_USED <= 128 ? 128 : COLS_USED <= 256 ? 256 : 512;
-    static constexpr int EPI_WARPS = 4 * W, FIRST_X = 4 + EPI_WARPS, X_WARPS = 8;
-    static constexpr int THREADS = 32 * (4 + EPI_WARPS + (FUSED ? X_WARPS : 0));
+    static constexpr int EPI_WARPS = 4 * W, FIRST_X = 4 + EPI_WARPS, X_WARPS = 8, TEAMS = 2;       // teams of X_WARPS take the stages in turn
+    static constexpr int THREADS = 32 * (4 + EPI_WARPS + (FUSED ? TEAMS * X_WARPS : 0));
     static constexpr size_t SMEM = (size_t)STAGES * (STAGE + SF) + 1024 + 512;
     static_assert(COLS_USED <= 512 && STAGES >= 3 && (A16 || GS % 2 == 0) && (!FUSED || TT <= 32) && (!FUSED || GS * TT / 2 % X_WARPS == 0), "tensor memory, shared memory or form");
 };
@@ -212,13 +212,13 @@ product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
         if (*abortp)                                                     // what is in flight gets a bounded chance to land
             for (int j = max(0, i - STAGES); j < i; ++j) mbar_wait(&full[j % STAGES], (j / STAGES) & 1, abortp);
     } else if (C::FUSED && warp >= C::FIRST_X) {
-        // All of these warps share a stage: an item is two tokens' values of a group, 8 to a lane; those of AHEAD stages are on their way.
-        constexpr int ITEMS = C::GS * TT / 2 / C::X_WARPS, AHEAD = 3;
+        // A team's warps share a stage: an item is two tokens' values of a group, 8 to a lane; its next stage's are on their way.
+        constexpr int ITEMS = C::GS * TT / 2 / C::X_WARPS;
         pdl_wait();
         const __nv_bfloat16* x = pdl_fresh(p.x);
-        const int c = (lane & 15) * 8, first = warp - C::FIRST_X;
-        uint4 raw[AHEAD][ITEMS];
-        int kl = b0 % kb, il = 0;                                        // the next stage to be asked for
+        const int c = (lane & 15) * 8, first = (warp - C::FIRST_X) % C::X_WARPS, team = (warp - C::FIRST_X) / C::X_WARPS;
+        uint4 raw[2][ITEMS];
+        int kl = (b0 + team) % kb, il = team;                            // the next stage to be asked for
         auto ask = [&](uint4 (&to)[ITEMS]) {
             if (il >= n) return;
 #pragma unroll
@@ -234,40 +234,34 @@ product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
                     to[j] = *reinterpret_cast<const uint4*>(v);
                 }
             }
-            ++il;
-            if (++kl == kb) kl = 0;
+            il += C::TEAMS;
+            kl = (kl + C::TEAMS) % kb;
         };
-#pragma unroll
-        for (int u = 0; u < AHEAD; ++u) ask(raw[u]);
+        ask(raw[0]);
         uint32_t parity = 1;
-        int s = 0;
+        int s = team;
         bool ok = true;
-        for (int i0 = 0; i0 < n && ok; i0 += AHEAD) {
+#pragma unroll 1
+        for (int i = team; i < n && ok; i += 2 * C::TEAMS) {
 #pragma unroll
-            for (int u = 0; u < AHEAD; ++u) {
-                if (i0 + u >= n) break;
+            for (int h = 0; h < 2; ++h) {
+                if (i + h * C::TEAMS >= n) break;
+                ask(raw[1 - h]);
                 ok = warp_wait(&empty[s], parity, abortp);
                 if (!ok) break;
                 unsigned char *xt = tiles + s * C::STAGE + C::W_BYTES, *ss = sf + s * C::SF + W * C::GS * TILE_BYTES;
 #pragma unroll
                 for (int j = 0; j < ITEMS; ++j) {
                     const int item = first + C::X_WARPS * j, t = item % (TT / 2) * 2 + (lane >> 4), g = item / (TT / 2);
-                    float v[8];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const float2 f = __bfloat1622float2(reinterpret_cast<const __nv_bfloat162*>(&raw[u][j])[e]);
-                        v[2 * e] = f.x, v[2 * e + 1] = f.y;
-                    }
-                    uint32_t most = 0;
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) most = max(most, __float_as_uint(v[e]) & 0x7fffffffu);
-                    most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
-                    most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
+                    uint32_t most = magnitude(raw[h][j]);
+                    most = __vmaxu2(most, __shfl_xor_sync(0xffffffffu, most, 1));
+                    most = __vmaxu2(most, __shfl_xor_sync(0xffffffffu, most, 2));
+                    most = max(most << 16, most & 0xffff0000u);          // as float32 bits
                     unsigned char* sc = ss + g * C::ATOMS * TILE_BYTES + (lane & 15) / 4;
                     if (C::A16) {                                        // 16-byte pieces of a row change places by the row's number
                         const int byte = term_byte(most);
                         uint32_t hi[2], lo[2];
-                        terms_of<8>(v, byte, hi, lo);
+                        terms_of_bf16(raw[h][j], byte, hi, lo);
                         unsigned char* to = xt + g * (C::XR * 128) + t * 128 + ((((lane & 15) >> 1) ^ (t & 7)) << 4) + (lane & 1) * 8;
                         *reinterpret_cast<uint2*>(to) = make_uint2(hi[0], hi[1]);
                         *reinterpret_cast<uint2*>(to + TT * 128) = make_uint2(lo[0], lo[1]);
@@ -277,21 +271,20 @@ product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
                         }
                     } else {
                         const int byte = scale_byte(most);
-                        const float inv = scale_inverse(byte);
+                        const float inv = byte == 255 ? 0.f : scale_inverse(byte);
+                        const uint32_t r[4] = {raw[h][j].x, raw[h][j].y, raw[h][j].z, raw[h][j].w};
                         uint32_t word = 0;
-                        if (byte != 255)
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) word |= pack2(v[2 * e] * inv, v[2 * e + 1] * inv) << (8 * e);
+                        for (int e = 0; e < 4; ++e) word |= pack2(__uint_as_float(r[e] << 16) * inv, __uint_as_float(r[e] & 0xffff0000u) * inv) << (8 * e);
                         *reinterpret_cast<uint32_t*>(xt + g / 2 * (C::XR * 128) + t * 128 + ((((g & 1) * 4 + (lane & 15) / 4) ^ (t & 7)) << 4) +
-                                                     (lane & 3) * 4) = word;
+                                                     (lane & 3) * 4) = byte == 255 ? 0 : word;
                         if ((lane & 3) == 0) sc[(t & 31) * 16 + t / 32 * 4] = (uint8_t)byte;
                     }
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&full[s]);
-                ask(raw[u]);
-                if (++s == STAGES) { s = 0; parity ^= 1; }
+                if ((s += C::TEAMS) >= STAGES) { s -= STAGES; parity ^= 1; }
             }
         }
     } else if (warp == 1) {
@@ -313,26 +306,32 @@ product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
             if (++s == STAGES) { s = 0; parity ^= 1; }
             ready = mbar_try_wait(&full[s], parity);                     // of the next stage: the answer comes while products are issued
             if (elect_one()) {
-#pragma unroll
-                for (int g = 0; g < C::GS; ++g) {
-                    if (g >= gs) break;
+                uint32_t more = !fresh;
+#pragma unroll 1
+                for (int g = 0; g < gs; ++g) {
 #pragma unroll
                     for (int w = 0; w < W; ++w) scales_to_tmem(tsf + (w * C::GS + g) * 4, ss + (w * C::GS + g) * TILE_BYTES);
 #pragma unroll
                     for (int a = 0; a < C::ATOMS; ++a)
                         scales_to_tmem(tsf + (W * C::GS + g * C::ATOMS + a) * 4, ss + (W * C::GS + g * C::ATOMS + a) * TILE_BYTES);
                     const int sub = C::A16 ? g : g / 2;
+                    const uint32_t sa = tsf + g * 4, sb = tsf + (W * C::GS + g * C::ATOMS) * 4;
+                    uint64_t a = da + sub * 1024 + (C::A16 ? 0 : (g & 1) * 4), b = db + sub * (C::XR * 128 >> 4) + (C::A16 ? 0 : (g & 1) * 4);
+                    uint32_t id = 0;
 #pragma unroll
-                    for (int j = 0; j < (C::A16 ? 4 : 2); ++j)           // 32 bytes of a row each: 32 or 64 elements
+                    for (int j = 0; j < (C::A16 ? 4 : 2); ++j) {         // 32 bytes of a row each: 32 or 64 elements
+                        const uint32_t idesc = idesc_of<C>(0) | id << 4 | id << 29;
 #pragma unroll
                         for (int w = 0; w < W; ++w) {
-                            const int id = C::A16 ? j : j * 2, at = C::A16 ? 2 * j : 2 * ((g & 1) * 2 + j);
-                            const uint64_t a = da + (w * C::SUBS + sub) * 1024 + at, b = db + sub * (C::XR * 128 >> 4) + at;
-                            const uint32_t sa = tsf + (w * C::GS + g) * 4, sb = tsf + (W * C::GS + g * C::ATOMS) * 4;
-                            umma_scaled<C::A16>(d + w * C::NCOL, a, b, idesc_of<C>(id), sa, sb, g > 0 || j > 0 || !fresh);
+                            umma_scaled<C::A16>(d + w * C::NCOL, a + w * (C::SUBS * 1024), b, idesc, sa + w * (C::GS * 4), sb, more);
                             if (C::A16 && !C::SIDE)
-                                umma_scaled<C::A16>(d + w * C::NCOL, a, b + (TT * 128 >> 4), idesc_of<C>(id), sa, sb + 4, 1);
+                                umma_scaled<C::A16>(d + w * C::NCOL, a + w * (C::SUBS * 1024), b + (TT * 128 >> 4), idesc, sa + w * (C::GS * 4), sb + 4, 1);
                         }
+                        more = 1;
+                        id += C::A16 ? 1 : 2;
+                        a += 2;
+                        b += 2;
+                    }
                 }
                 umma_commit(&empty[s_now]);
                 if (done) umma_commit(&acc_full[buf]);
@@ -364,10 +363,10 @@ product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
             const uint32_t d = tmem + ((uint32_t)(q * 32) << 16) + (buf * W + w) * C::NCOL;
             const bool whole = k0 == 0 && k1 == kb;
             const float bias = p.bias != nullptr && f < p.N ? load_param(p.bias, p.bias_bf16, f) : 0.f;
-            auto store = [&](int t0, const float (&v)[8]) {
+            auto store = [&](int t0, const auto& v) {
                 if (f >= p.N) return;
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
+                for (int j = 0; j < (int)(sizeof(v) / sizeof(float)); ++j) {
                     if (t0 + j >= tokens) return;
                     const long long at = (long long)(m0 + t0 + j) * p.ldy + f;
                     if (p.out_bf16) reinterpret_cast<__nv_bfloat16*>(p.y)[at] = __float2bfloat16_rn(v[j] + bias);
@@ -406,15 +405,26 @@ product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
             if (!is_last) continue;
             if (C::FUSED && threadIdx.x == 128) p.counters[u] = 0;        // as the next launch expects it
             __threadfence();
+            // one CTA's share after another's, the loads of eight of them at once
+            constexpr int SHARES = 8;
 #pragma unroll 1
             for (int t0 = 0; t0 < tokens; t0 += 8) {
                 float v[8] = {};
-                // one CTA's after another's, four of them in a round of loads
-#pragma unroll 4
-                for (int c = c0; c <= c1; ++c) {
-                    const float* from = p.part + (((size_t)c * 2 + p.split.place(c, u)) * W + w) * (TT * 128) + row + t0 * 128;
+#pragma unroll 1
+                for (int c = c0; c <= c1; c += SHARES) {
+                    float part[SHARES][8];
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) v[j] += __ldcg(from + j * 128);
+                    for (int k = 0; k < SHARES; ++k) {
+                        const int from_cta = min(c + k, c1);
+                        const float* from = p.part + (((size_t)from_cta * 2 + p.split.place(from_cta, u)) * W + w) * (TT * 128) + row + t0 * 128;
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) part[k][j] = __ldcg(from + j * 128);
+                    }
+#pragma unroll
+                    for (int k = 0; k < SHARES; ++k)
+#pragma unroll
+                        for (int j = 0; j < 8; ++j)
+                            if (c + k <= c1) v[j] += part[k][j];
                 }
                 store(t0, v);
             }
@@ -439,40 +449,44 @@ struct Plan {
     bool fused;
     long long units, codes, scales, parts, counters, bytes;       // bytes from the workspace's start
 };
-// Tiles of 8 to 64 tokens take all tokens at once; more tokens go by tiles of 128, or 64 where that leaves SMs without work.
-// A unit's K is shared by so many CTAs that the blocks of the busiest (block: what one takes) and the joining of partial sums (1.5 us
-// for handing over, then the bytes of each share) take least: 159 x 777 x 4,407: 173 us dealt to all SMs, 4,608 x 3,584 by 1 token ... 
+// Up to 32 tokens go through the fused form of their size; for more, tiles of 32 to 128 tokens by one or two of W.  What is chosen, tile
+// and CTAs that share a unit's K, takes least by this estimate (us): blocks of the busiest CTA times a block's time (W and x from
+// memory, or the products), and where K is shared 2 for handing over and the bytes of the shares at 100 KB a us.  Measured: 159 tokens
+// x 777 x 4,407 dealt to all SMs in tiles of 128 x 256 173 us, of which 110 joining; ...
 inline Plan plan_for(int M, int N, int K, int act_bits) {
+    struct Form { int tt, w; float block16, block4; };
+    static const Form few[] = {{8, 1, .40f, 0.f}, {16, 1, .50f, .40f}, {32, 2, .45f, .45f}};
+    static const Form many[] = {{32, 1, .26f, .38f}, {64, 1, .30f, .40f}, {64, 2, .48f, .48f}, {128, 2, .72f, .55f}};
     Plan best;
     float best_us = 1e30f;
     const bool a16 = act_bits == 16;
     const int sms = sm_count();
-    const bool many_tiles = N > MOST_COUNTERS * 128LL;              // more than the fused form has counters for
-    for (int tt = many_tiles ? 64 : a16 && M <= 8 ? 8 : M <= 16 ? 16 : M <= 32 ? 32 : 64;; tt *= 2) {
+    const bool fused = M <= 32 && N <= MOST_COUNTERS * 128LL;       // as many tiles as the fused form has counters for
+    const Form* forms = fused ? &few[M <= 8 && a16 ? 0 : M <= 16 ? 1 : 2] : many;
+    for (int i = 0; i < (fused ? 1 : 4); ++i) {
         Plan q;
-        q.tt = tt;
-        q.w = tt >= 32 ? 2 : 1;
-        q.gs = (a16 ? 1 : 2) * (tt <= 16 ? 2 : 1);
-        q.fused = tt <= 32;
+        q.tt = forms[i].tt;
+        q.w = forms[i].w;
+        q.gs = !a16 || q.tt <= 16 ? 2 : 1;
+        q.fused = fused;
         q.groups = groups_of(K);
-        q.mtiles = (M + tt - 1) / tt;
+        q.mtiles = (M + q.tt - 1) / q.tt;
         q.ntiles = (N + 127) / 128;
         q.kb = (q.groups + q.gs - 1) / q.gs;
         q.units = (long long)((q.ntiles + q.w - 1) / q.w) * q.mtiles;
         const long long total = q.units * q.kb;
-        const float block = tt <= 16 ? 0.40f : tt == 32 ? 0.42f : tt == 64 ? 0.48f : (a16 ? 0.75f : 0.55f);
-        const float share = (float)(tt * q.w) / 256.f;
+        const float block = a16 ? forms[i].block16 : forms[i].block4;
+        const float share = (float)(q.tt * q.w) * (512.f / 100e3f);
         for (int split = 1; split <= q.kb; split += split < 4 ? 1 : split / 4) {
             const long long want = q.units * split;
             q.P = (int)(want < sms ? want : sms);
             if (q.P > total) q.P = (int)total;
             const long long each = (total + q.P - 1) / q.P;
             const int shares = each >= q.kb && total % q.P == 0 ? 1 : (int)((q.kb + each - 1) / each) + (want > sms);
-            const float us = each * block + (shares > 1 ? 1.5f + shares * share : 0.f);
+            const float us = each * block + (shares > 1 ? 2.f + shares * share : 0.f);
             if (us < best_us) { best_us = us; best = q; }
             if (want >= sms) break;
         }
-        if (tt >= (M <= 64 ? tt : 128)) break;
     }
     Plan& q = best;
     const int xr = a16 ? 2 * q.tt : q.tt, atoms = (xr + 127) / 128;
@@ -544,7 +558,7 @@ PRISM_EXPORT int prism_mxfp4_linear(const void* x, long long ldx, const void* co
                 default: return run_product<Cfg<true, 32, 2, 1, true>>(mw, mw, p, stream);
             }
         }
-        return q.tt == 16 ? run_product<Cfg<false, 16, 1, 4, true>>(mw, mw, p, stream) : run_product<Cfg<false, 32, 2, 2, true>>(mw, mw, p, stream);
+        return q.tt == 16 ? run_product<Cfg<false, 16, 1, 2, true>>(mw, mw, p, stream) : run_product<Cfg<false, 32, 2, 2, true>>(mw, mw, p, stream);
     }
     const int xr = a16 ? 2 * q.tt : q.tt;
     rc = a16 ? byte_map(&mx, base + q.codes, (long long)q.mtiles * xr, (long long)q.groups * GROUP, xr, false)
@@ -555,6 +569,19 @@ PRISM_EXPORT int prism_mxfp4_linear(const void* x, long long ldx, const void* co
     rc = (int)launch_kernel(a16 ? prepare_kernel<true> : prepare_kernel<false>, dim3(blocks), dim3(256), 0, stream, p.x, ldx, M, K, q.groups, p.wide,
                             q.tt, base + q.codes, base + q.scales, p.counters, (int)q.units);
     if (rc) return rc;
-    if (a16) return q.tt == 64 ? run_product<Cfg<true, 64, 2, 1, false>>(mw, mx, p, stream) : run_product<Cfg<true, 128, 2, 1, false>>(mw, mx, p, stream);
-    return q.tt == 64 ? run_product<Cfg<false, 64, 2, 2, false>>(mw, mx, p, stream) : run_product<Cfg<false, 128, 2, 2, false>>(mw, mx, p, stream);
+    const int form = q.tt * 10 + q.w;
+    if (a16) {
+        switch (form) {
+            case 321: return run_product<Cfg<true, 32, 1, 1, false>>(mw, mx, p, stream);
+            case 641: return run_product<Cfg<true, 64, 1, 1, false>>(mw, mx, p, stream);
+            case 642: return run_product<Cfg<true, 64, 2, 1, false>>(mw, mx, p, stream);
+            default: return run_product<Cfg<true, 128, 2, 1, false>>(mw, mx, p, stream);
+        }
+    }
+    switch (form) {
+        case 321: return run_product<Cfg<false, 32, 1, 2, false>>(mw, mx, p, stream);
+        case 641: return run_product<Cfg<false, 64, 1, 2, false>>(mw, mx, p, stream);
+        case 642: return run_product<Cfg<false, 64, 2, 2, false>>(mw, mx, p, stream);
+        default: return run_product<Cfg<false, 128, 2, 2, false>>(mw, mx, p, stream);
+    }
 }

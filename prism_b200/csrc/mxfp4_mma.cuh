@@ -54,6 +54,33 @@ template <int N> __device__ __forceinline__ void terms_of(const float (&v)[N], i
     }
 }
 
+// The same of eight bfloat16 values as they lie in memory, in half precision where two share an instruction (exact: a scaled
+// value has 8 significant bits and is below 256; what half precision drops is below 2^-24, which no E4M3 term of it holds).
+__device__ __forceinline__ uint32_t magnitude(const uint4& raw) {       // the largest, as bfloat16 bits, in either half of the word
+    const uint32_t m = 0x7fff7fffu;
+    return __vmaxu2(__vmaxu2(raw.x & m, raw.y & m), __vmaxu2(raw.z & m, raw.w & m));
+}
+__device__ __forceinline__ void terms_of_bf16(const uint4& raw, int byte, uint32_t (&hi)[2], uint32_t (&lo)[2]) {
+    const float f = byte == 255 ? 0.f : __uint_as_float((uint32_t)(254 - byte) << 23);
+    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+    uint16_t h8[4], l8[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float a = __uint_as_float(w[i] << 16) * f, b = __uint_as_float(w[i] & 0xffff0000u) * f;
+        uint32_t x, back, rest;
+        asm("cvt.rn.f16x2.f32 %0, %2, %1;" : "=r"(x) : "f"(a), "f"(b));
+        asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(h8[i]) : "r"(x));
+        asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(back) : "h"(h8[i]));
+        asm("{\n\t.reg .b32 d;\n\tsub.f16x2 d, %1, %2;\n\tmul.f16x2 %0, d, %3;\n\t}" : "=r"(rest) : "r"(x), "r"(back), "r"(0x50005000u));     // 32, 32
+        asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(l8[i]) : "r"(rest));
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        hi[i] = byte == 255 ? 0 : h8[2 * i] | (uint32_t)h8[2 * i + 1] << 16;
+        lo[i] = byte == 255 ? 0 : l8[2 * i] | (uint32_t)l8[2 * i + 1] << 16;
+    }
+}
+
 // ---- pieces of the products -----------------------------------------------------------------------------------------------
 
 // How `total` blocks are dealt to P CTAs as one line: the first `more` have one block more than the others.  A unit is kb
