@@ -22,18 +22,22 @@
 #include "mxfp4_mma.cuh"
 #include "vec.cuh"
 
+#include <climits>
+
 namespace prism {
 namespace mx {
 
 constexpr int MOE_THREADS = 384, MOE_WARPS = 12, MOE_MOST_EXPERTS = 256, MOE_MOST_ENTRIES = 1024;
 
+// TT: tokens there is room for.  COMPACT: the columns of gate and up are an expert's own tokens, whose rows of x are laid out anew for
+// it; otherwise all tokens (there are few).
 template <int TT_> struct MoeCfg {
     static constexpr int TT = TT_, NCOL = 2 * TT;
+    static constexpr bool COMPACT = TT > 16;
     static constexpr int W_BYTES = 2 * 16384, X_BYTES = NCOL * 128, STAGE = W_BYTES + X_BYTES, SF = 3 * TILE_BYTES, SF_COLS = 12;
     static constexpr int FIT = 200 * 1024 / (STAGE + SF), STAGES = FIT > 8 ? 8 : FIT;
-    static constexpr int BUFS = 4 * NCOL + STAGES * SF_COLS <= 512 ? 2 : 1;
-    static constexpr int USED = BUFS * 2 * NCOL + STAGES * SF_COLS;
-    static constexpr int COLS = USED <= 128 ? 128 : USED <= 256 ? 256 : 512;
+    static constexpr int USED = 2 * NCOL + STAGES * SF_COLS, BOTH = 4 * NCOL + STAGES * SF_COLS;       // columns with one set of sums, with two
+    static constexpr int COLS = BOTH <= 128 ? 128 : BOTH <= 256 ? 256 : 512;
     static constexpr size_t SMEM = (size_t)STAGES * (STAGE + SF) + 1024 + 512;
     static_assert(USED <= 512 && STAGES >= 3, "tensor memory or shared memory");
 };
@@ -42,12 +46,13 @@ struct Moe {
     const __nv_bfloat16* x;
     const void *router, *rbias, *corr;
     const uint8_t *gate_s, *up_s, *down_s;
-    uint8_t *xt, *xs, *h, *hs;             // x's terms [2 TT][Hp] and scales, h's [rows][Fp] and scales [live][groups][512]
+    // x's terms [2 TT][Hp] and scales [groups][512] (compact: [rows][Hp] and [live][groups][512]), h's [rows][Fp] and [live][groups][512]
+    uint8_t *xt, *xs, *h, *hs;
     float *z, *sel_w, *part1, *part2, *planes;
-    int *sel_e, *counters, *ready, *control, *err;      // control: barrier, leavers, a counter per token
+    int *sel_e, *counters, *ready, *control, *err;      // ready: h, then x (compact); control: barrier, leavers, a counter per token
     void* y;
     long long ldx, ldy;
-    int T, H, F, E, top, softmax, renorm, scale_in, act, groups_of_experts, keep, experts_a_warp, ncounters;
+    int T, H, F, E, top, softmax, renorm, scale_in, act, groups_of_experts, keep, dots, most_live, ncounters;
     int router_bf16, rbias_bf16, corr_bf16, out_bf16, wide;
     float limit, wscale, sum_eps;
 };
@@ -58,8 +63,9 @@ struct Lists {                             // of the experts that have tokens, i
     // an expert's tokens from first[] on, ascending
     float weight[MOE_MOST_ENTRIES];
     short plane[MOE_MOST_ENTRIES], first_plane[MOE_MOST_ENTRIES];
+    short expert_of[MOE_MOST_ENTRIES];     // by choice, token after token
     unsigned char token[MOE_MOST_ENTRIES];
-    int live;
+    int live, entries, most;               // experts with tokens, their tokens in all, the most of one
 };
 
 // until *p >= want, within the limit of every wait here
@@ -81,9 +87,9 @@ __device__ __forceinline__ bool wait_count(const int* p, int want, volatile int*
     }
 }
 __device__ __forceinline__ void grid_barrier(int* bar, int want, volatile int* abortp) {
-    __threadfence();
     __syncthreads();
     if (threadIdx.x == 0) {
+        __threadfence();                                       // for all that this CTA's threads wrote before they met here
         atomicAdd(bar, 1);
         wait_count(bar, want, abortp);
     }
@@ -91,89 +97,156 @@ __device__ __forceinline__ void grid_barrier(int* bar, int want, volatile int* a
 }
 __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async;" ::: "memory"); }
 
-__device__ __forceinline__ float tmem_one(uint32_t taddr) {
-    uint32_t r;
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(r) : "r"(taddr));
-    return __uint_as_float(r);
+__device__ __forceinline__ void tmem_one(uint32_t& v, uint32_t taddr) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(v) : "r"(taddr));
 }
 
-// 1: logits, choices, x's terms
-__device__ __forceinline__ void moe_route_and_terms(const Moe& p, float* scratch, int tt) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, gw = blockIdx.x * MOE_WARPS + warp, warps = gridDim.x * MOE_WARPS;
-    const int groups = groups_of(p.H), per_row = groups * (GROUP / 8);
+// eight of a row's values from column c, zero beyond K
+__device__ __forceinline__ uint4 row8(const __nv_bfloat16* row, int c, int K, int wide) {
+    if (wide && c + 8 <= K) return *reinterpret_cast<const uint4*>(row + c);
+    __nv_bfloat16 v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = c + j < K ? row[c + j] : __nv_bfloat16(0.f);
+    return *reinterpret_cast<const uint4*>(v);
+}
+// Terms of eight values of a row (neighbouring threads have a block's others) to the rows `hi`, `lo` of a matrix of rows of
+// `pitch` bytes and to its scales; su, sl: the rows' numbers there.
+__device__ __forceinline__ void row_terms(const uint4& raw, int c, uint8_t* hi_row, uint8_t* lo_row, uint8_t* scales, int su, int sl) {
+    const uint32_t four = 0xfu << (threadIdx.x & 28);
+    uint32_t most = magnitude(raw);
+    most = __vmaxu2(most, __shfl_xor_sync(four, most, 1));
+    most = __vmaxu2(most, __shfl_xor_sync(four, most, 2));
+    const int byte = term_byte(max(most << 16, most & 0xffff0000u));
+    uint32_t hi[2], lo[2];
+    terms_of_bf16(raw, byte, hi, lo);
+    *reinterpret_cast<uint2*>(hi_row + c) = make_uint2(hi[0], hi[1]);
+    *reinterpret_cast<uint2*>(lo_row + c) = make_uint2(lo[0], lo[1]);
+    if ((threadIdx.x & 3) == 0) {
+        uint8_t* s = scales + (size_t)(c / GROUP) * TILE_BYTES + c % GROUP / BLOCK;
+        s[(su & 31) * 16 + su / 32 * 4] = (uint8_t)byte;
+        s[(sl & 31) * 16 + sl / 32 * 4] = low_byte(byte);
+    }
+}
+
+// A token's choice by one warp whose lanes keep its scores (lane, lane + 32, ...): as moe_route_token, without groups.
+__device__ __forceinline__ void choose(const Moe& p, int t) {
+    constexpr int EACH = MOE_MOST_EXPERTS / 32;
+    const int lane = threadIdx.x & 31;
+    float s[EACH], mx = -INFINITY, den = 0.f;
+    int key[EACH];
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {
+        s[i] = lane + 32 * i < p.E ? __ldcg(p.z + t * p.E + lane + 32 * i) : -INFINITY;
+        mx = fmaxf(mx, s[i]);
+    }
+    mx = warp_max(mx);
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {
+        if (32 * i >= p.E) break;
+        if (lane + 32 * i >= p.E) continue;
+        s[i] = p.softmax ? expf(s[i] - mx) : moe_sigmoid(s[i]);
+        den += s[i];
+    }
+    den = p.softmax ? warp_sum(den) : 1.f;
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {
+        const int e = lane + 32 * i;
+        key[i] = INT_MIN;                                      // what cannot be chosen: no expert, no number, minus infinity
+        if (e >= p.E) continue;
+        if (p.softmax) s[i] = s[i] / den;
+        const float c = p.corr != nullptr ? s[i] + load_param(p.corr, p.corr_bf16, e) : s[i];
+        const int bits = __float_as_int(c);
+        if (c > -INFINITY) key[i] = bits ^ (bits >> 31 & 0x7fffffff);          // ordered as the numbers are
+        if (c == 0.f) key[i] = 0;
+    }
+    float chosen = 0.f, mine = 0.f;
+#pragma unroll 1
+    for (int j = 0; j < p.top; ++j) {
+        int best = INT_MIN, at = p.E;
+#pragma unroll
+        for (int i = EACH - 1; i >= 0; --i)
+            if (key[i] >= best && key[i] != INT_MIN) { best = key[i]; at = lane + 32 * i; }
+        const int most = __reduce_max_sync(0xffffffffu, best);
+        at = __reduce_min_sync(0xffffffffu, best == most && most != INT_MIN ? at : INT_MAX);
+        if (at == INT_MAX) at = 0;                             // every score NaN: keep the indices legal
+        float w = 0.f;
+#pragma unroll
+        for (int i = 0; i < EACH; ++i)
+            if (lane + 32 * i == at) { w = s[i]; key[i] = INT_MIN; }
+        w = __shfl_sync(0xffffffffu, w, at & 31);
+        chosen += w;
+        if (lane == j) mine = w;
+        if (lane == 0) p.sel_e[t * p.top + j] = at;
+    }
+    if (lane < p.top) p.sel_w[t * p.top + lane] = (p.renorm ? mine / (chosen + p.sum_eps) : mine) * p.wscale;
+}
+
+// 1: logits, choices, x's terms.  A CTA has `dots` neighbouring logits (of one token or two); where they are few, several warps
+// share a row.
+template <typename C> __device__ __forceinline__ void moe_route_and_terms(const Moe& p, float* scratch) {
+    __shared__ int finished[2];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int gtid = blockIdx.x * MOE_THREADS + threadIdx.x, threads = gridDim.x * MOE_THREADS;
     for (int i = gtid; i < p.ncounters; i += threads) p.ready[i] = 0;             // and the tiles' counters behind them
-    for (int i = gtid; i < p.T * per_row; i += threads) {
-        const int r = i / per_row, c = (i - r * per_row) * 8;
-        const __nv_bfloat16* at = p.x + (long long)r * p.ldx + c;
-        float v[8];
-        if (p.wide && c + 8 <= p.H) {
-            load8(at, v);
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = c + j < p.H ? to_float(at[j]) : 0.f;
+    if (!C::COMPACT) {
+        const int groups = groups_of(p.H), per_row = groups * (GROUP / 8);
+        const size_t pitch = (size_t)groups * GROUP;
+#pragma unroll 1
+        for (int i = gtid; i < p.T * per_row; i += threads) {
+            const int r = i / per_row, c = (i - r * per_row) * 8;
+            row_terms(row8(p.x + (long long)r * p.ldx, c, p.H, p.wide), c, p.xt + r * pitch, p.xt + (r + C::TT) * pitch, p.xs, r, r + C::TT);
         }
-        uint32_t most = 0;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) most = max(most, __float_as_uint(v[j]) & 0x7fffffffu);
-        const uint32_t four = 0xfu << (threadIdx.x & 28);
-        most = max(most, __shfl_xor_sync(four, most, 1));
-        most = max(most, __shfl_xor_sync(four, most, 2));
-        const int byte = term_byte(most);
-        uint32_t hi[2], lo[2];
-        terms_of<8>(v, byte, hi, lo);
-        uint8_t* to = p.xt + (size_t)r * groups * GROUP + c;
-        *reinterpret_cast<uint2*>(to) = make_uint2(hi[0], hi[1]);
-        *reinterpret_cast<uint2*>(to + (size_t)tt * groups * GROUP) = make_uint2(lo[0], lo[1]);
-        if ((threadIdx.x & 3) == 0) {
-            uint8_t* s = p.xs + (size_t)(c / GROUP) * TILE_BYTES + c % GROUP / BLOCK;
-            const int u = r + tt;
-            s[(r & 31) * 16 + r / 32 * 4] = (uint8_t)byte;
-            s[(u & 31) * 16 + u / 32 * 4] = low_byte(byte);
-        }
+        fence_async();                                         // the terms are read by TMA, of all CTAs
     }
-    fence_async();                                             // the terms are read by TMA, of all CTAs
-    constexpr int MOST = 4;
-    const int chunks = (p.E + p.experts_a_warp - 1) / p.experts_a_warp, items = p.T * chunks;
-    for (int i = gw; i < items; i += warps) {
-        const int t = i / chunks, e0 = (i - t * chunks) * p.experts_a_warp, ne = min(p.experts_a_warp, p.E - e0);
+    const int first = blockIdx.x * p.dots, count = min(p.dots, p.T * p.E - first);
+    if (count <= 0) return;
+    const int parts = p.dots >= MOE_WARPS ? 1 : MOE_WARPS / p.dots, at_once = MOE_WARPS / parts, part = warp % parts;
+    const int len = ((p.H + parts - 1) / parts + 7) / 8 * 8, k0 = part * len, k1 = min(p.H, k0 + len);
+    const bool wide = p.wide && p.H % 8 == 0;
+#pragma unroll 1
+    for (int i = warp / parts; i < count; i += at_once) {
+        const int t = (first + i) / p.E, e = first + i - t * p.E;
         const __nv_bfloat16* row = p.x + (long long)t * p.ldx;
-        float sum[MOST] = {};
-        if (p.wide && p.H % 8 == 0) {
-#pragma unroll 2
-            for (int k = lane * 8; k < p.H; k += 256) {
+        float sum = 0.f;
+        if (wide) {
+#pragma unroll 4
+            for (int k = k0 + lane * 8; k < k1; k += 256) {
                 float a[8], w[8];
                 load8(row + k, a);
+                load_param8(p.router, p.router_bf16, (size_t)e * p.H + k, w);
 #pragma unroll
-                for (int j = 0; j < MOST; ++j)
-                    if (j < ne) {
-                        load_param8(p.router, p.router_bf16, (size_t)(e0 + j) * p.H + k, w);
-#pragma unroll
-                        for (int l = 0; l < 8; ++l) sum[j] = fmaf(a[l], w[l], sum[j]);
-                    }
+                for (int l = 0; l < 8; ++l) sum = fmaf(a[l], w[l], sum);
             }
         } else {
-            for (int k = lane; k < p.H; k += 32) {
-                const float a = to_float(row[k]);
-#pragma unroll
-                for (int j = 0; j < MOST; ++j)
-                    if (j < ne) sum[j] = fmaf(a, load_param(p.router, p.router_bf16, (size_t)(e0 + j) * p.H + k), sum[j]);
-            }
+#pragma unroll 8
+            for (int k = k0 + lane; k < k1; k += 32) sum = fmaf(to_float(row[k]), load_param(p.router, p.router_bf16, (size_t)e * p.H + k), sum);
         }
-#pragma unroll
-        for (int j = 0; j < MOST; ++j) {
-            if (j >= ne) break;
-            const float s = warp_sum(sum[j]);
-            if (lane == 0) p.z[t * p.E + e0 + j] = s + (p.rbias != nullptr ? load_param(p.rbias, p.rbias_bf16, e0 + j) : 0.f);
-        }
-        int last = 0;
-        if (lane == 0) {
+        sum = warp_sum(sum);
+        if (lane == 0) scratch[i * parts + part] = sum;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < count; i += MOE_THREADS) {
+        const int t = (first + i) / p.E, e = first + i - t * p.E;
+        float sum = p.rbias != nullptr ? load_param(p.rbias, p.rbias_bf16, e) : 0.f;
+        for (int j = 0; j < parts; ++j) sum += scratch[i * parts + j];
+        p.z[first + i] = sum;
+    }
+    __syncthreads();
+    const int t0 = first / p.E, t1 = (first + count - 1) / p.E;             // no more than E logits: two tokens at most
+    if (threadIdx.x < 2) {
+        const int t = t0 + threadIdx.x;
+        finished[threadIdx.x] = 0;
+        if (t <= t1) {
+            const int here = min(first + count, (t + 1) * p.E) - max(first, t * p.E);
             __threadfence();
-            last = atomicAdd(&p.control[2 + t], 1) == chunks - 1;
+            finished[threadIdx.x] = atomicAdd(&p.control[2 + t], here) == p.E - here;
             __threadfence();
         }
-        if (!__shfl_sync(0xffffffffu, last, 0)) continue;
-        __threadfence();
+    }
+    __syncthreads();
+    if (warp >= 2 || !finished[warp]) return;
+    const int t = t0 + warp;
+    if (p.groups_of_experts > 1 && p.keep < p.groups_of_experts) {
         float* zs = scratch + (size_t)warp * (4 * p.E + 2 * p.groups_of_experts + 16);
         int* counts = reinterpret_cast<int*>(zs + 3 * p.E + 2 * p.groups_of_experts);
         for (int e = lane; e < p.E; e += 32) {
@@ -183,59 +256,88 @@ __device__ __forceinline__ void moe_route_and_terms(const Moe& p, float* scratch
         __syncwarp();
         moe_route_token(zs, zs + p.E, zs + 2 * p.E, zs + 3 * p.E, p.E, p.top, p.softmax, p.renorm, lane, counts, p.sel_e + t * p.top,
                         p.sel_w + t * p.top, counts + p.E, p.corr, p.corr_bf16, p.groups_of_experts, p.keep, p.wscale, p.sum_eps);
-        __syncwarp();
+    } else {
+        choose(p, t);
     }
 }
 
 // 2: who has tokens
 __device__ __forceinline__ void moe_lists(const Moe& p, Lists& q) {
     const int n = p.T * p.top;
+    for (int i = threadIdx.x; i < n; i += MOE_THREADS) {
+        q.expert_of[i] = (short)__ldcg(p.sel_e + i);
+        q.weight[i] = __ldcg(p.sel_w + i);
+    }
     for (int e = threadIdx.x; e < p.E; e += MOE_THREADS) q.mask[e] = 0;
     __syncthreads();
     for (int i = threadIdx.x; i < n; i += MOE_THREADS) {
         const int t = i / p.top;
-        atomicOr(reinterpret_cast<unsigned int*>(&q.mask[__ldcg(p.sel_e + i)]) + t / 32, 1u << (t & 31));
+        atomicOr(reinterpret_cast<unsigned int*>(&q.mask[q.expert_of[i]]) + t / 32, 1u << (t & 31));
     }
     __syncthreads();
     if (threadIdx.x < 32) {
         const int lane = threadIdx.x;
-        int live = 0, first = 0, row8 = 0;
+        int live = 0, first = 0, row8 = 0, most = 0;
+#pragma unroll 1
         for (int e0 = 0; e0 < p.E; e0 += 32) {
             const int e = e0 + lane, c = e < p.E ? __popcll(q.mask[e]) : 0;
-            int l = c > 0, f = c, r = (c + 7) / 8 * 2;            // inclusive sums over the lanes: experts, tokens, rows of h / 8
+            const unsigned any = __ballot_sync(0xffffffffu, c > 0);
+            int v = c | (c + 7) / 8 * 2 << 16;                    // inclusive sums over the lanes: tokens, rows of h / 8
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
-                const int a = __shfl_up_sync(0xffffffffu, l, o), b = __shfl_up_sync(0xffffffffu, f, o), d = __shfl_up_sync(0xffffffffu, r, o);
-                if (lane >= o) { l += a; f += b; r += d; }
+                const int a = __shfl_up_sync(0xffffffffu, v, o);
+                if (lane >= o) v += a;
             }
             if (c > 0) {
-                const int at = live + l - 1;
+                const int at = live + __popc(any & ((1u << lane) - 1));
                 q.slot[e] = (short)at;
                 q.expert[at] = (short)e;
                 q.count[at] = (short)c;
-                q.first[at] = (short)(first + f - c);
-                q.hrow8[at] = (short)(row8 + r - (c + 7) / 8 * 2);
+                q.first[at] = (short)(first + (v & 0xffff) - c);
+                q.hrow8[at] = (short)(row8 + (v >> 16) - (c + 7) / 8 * 2);
             }
-            live += __shfl_sync(0xffffffffu, l, 31);
-            first += __shfl_sync(0xffffffffu, f, 31);
-            row8 += __shfl_sync(0xffffffffu, r, 31);
+            v = __shfl_sync(0xffffffffu, v, 31);
+            live += __popc(any);
+            first += v & 0xffff;
+            row8 += v >> 16;
+            most = max(most, __reduce_max_sync(0xffffffffu, c));
         }
-        if (lane == 0) q.live = live;
+        if (lane == 0) { q.live = live; q.entries = first; q.most = most; }
     }
     __syncthreads();
     for (int i = threadIdx.x; i < n; i += MOE_THREADS) {
-        const int t = i / p.top, j = i - t * p.top, e = __ldcg(p.sel_e + i);
+        const int t = i / p.top, j = i - t * p.top, e = q.expert_of[i];
         int same = j;                                            // scores that are not numbers can choose an expert twice
-        for (int o = 0; o < j; ++o)
-            if (__ldcg(p.sel_e + t * p.top + o) == e) { same = o; break; }
+        for (int o = j - 1; o >= 0; --o)
+            if (q.expert_of[t * p.top + o] == e) same = o;
         q.first_plane[i] = (short)(t * p.top + same);
         if (same != j) continue;
         const int at = q.first[q.slot[e]] + __popcll(q.mask[e] & ((1ull << t) - 1));
         q.token[at] = (unsigned char)t;
-        q.weight[at] = __ldcg(p.sel_w + i);
         q.plane[at] = (short)i;
     }
     __syncthreads();
+}
+
+// (compact) rows of x, as terms, laid out for the experts that read them; an expert's counter says how many of its rows are there
+__device__ __forceinline__ void moe_compact(const Moe& p, const Lists& q) {
+    const int groups = groups_of(p.H);
+    const size_t pitch = (size_t)groups * GROUP;
+    int l = 0;
+    for (int i = blockIdx.x; i < q.entries; i += gridDim.x) {
+        while (i >= q.first[l] + q.count[l]) ++l;
+        const int r = i - q.first[l], nt = (q.count[l] + 7) / 8 * 8;
+        const __nv_bfloat16* row = p.x + (long long)q.token[i] * p.ldx;
+        uint8_t* to = p.xt + (size_t)(q.hrow8[l] * 8 + r) * pitch;
+        for (int c = (threadIdx.x - 128) * 8; c < groups * GROUP; c += 256 * 8)
+            row_terms(row8(row, c, p.H, p.wide), c, to, to + nt * pitch, p.xs + (size_t)l * groups * TILE_BYTES, r, nt + r);
+        fence_async();
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        if (threadIdx.x == 128) {
+            __threadfence();
+            atomicAdd(&p.ready[p.most_live + l], 1);
+        }
+    }
 }
 
 // a walk over a CTA's blocks: live expert l, tile, stage k; n blocks left
@@ -266,26 +368,26 @@ moe_kernel(const __grid_constant__ CUtensorMap map_gate, const __grid_constant__
     unsigned char* tiles = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     unsigned char* sf = tiles + (size_t)STAGES * C::STAGE;
     uint64_t* full = reinterpret_cast<uint64_t*>(sf + STAGES * C::SF);
-    uint64_t *empty = full + STAGES, *acc_full = empty + STAGES, *acc_empty = acc_full + C::BUFS;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + C::BUFS);
+    uint64_t *empty = full + STAGES, *acc_full = empty + STAGES, *acc_empty = acc_full + 2;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, cta = blockIdx.x, P = gridDim.x;
     volatile int* abortp = &abort_flag;
     if (threadIdx.x == 0) {
         abort_flag = 0;
         for (int s = 0; s < STAGES; ++s) { mbar_init(&full[s], 2); mbar_init(&empty[s], 1); }
-        for (int s = 0; s < C::BUFS; ++s) { mbar_init(&acc_full[s], 1); mbar_init(&acc_empty[s], 8); }
+        for (int s = 0; s < 2; ++s) { mbar_init(&acc_full[s], 1); mbar_init(&acc_empty[s], 8); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(tmem_slot)), "r"(C::COLS));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
     }
-    moe_route_and_terms(p, reinterpret_cast<float*>(tiles), TT);
+    moe_route_and_terms<C>(p, reinterpret_cast<float*>(tiles));
     fence_async();                          // the scratch becomes stages
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     grid_barrier(p.control, P, abortp);
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    const uint32_t tmem = *tmem_slot, tmem_sf = tmem + C::BUFS * 2 * NCOL;
+    const uint32_t tmem = *tmem_slot, tmem_sf = tmem + C::COLS - STAGES * C::SF_COLS;
     if (threadIdx.x == 0) gone = *abortp;
     __syncthreads();
 
@@ -293,10 +395,13 @@ moe_kernel(const __grid_constant__ CUtensorMap map_gate, const __grid_constant__
         moe_lists(p, q);
         const int g1 = groups_of(p.H), g2 = groups_of(p.F), tiles1 = g2, tiles_h = (p.H + 127) / 128, tiles2 = (tiles_h + 1) / 2;
         const int total1 = q.live * tiles1 * g1, total2 = q.live * tiles2 * g2;
-        const Split s1(total1, min(P, total1), g1), s2(total2, min(P, total2), g2);
+        // no more than about eight CTAs share a tile: joining more costs more than their blocks
+        const Split s1(total1, min(min(P, total1), q.live * tiles1 * 7), g1), s2(total2, min(min(P, total2), q.live * tiles2 * 7), g2);
         Walk a(s1, cta, tiles1, g1), b(s2, cta, tiles2, g2);
         const int n1 = a.n, n = a.n + b.n;
         int* units2 = p.counters + q.live * tiles1;
+        // columns of a tile's sums; two sets of them where they fit
+        const int cols = C::COMPACT ? (q.most + 7) / 8 * 16 : NCOL, bufs = 4 * cols + STAGES * C::SF_COLS <= C::COLS ? 2 : 1;
 
         if (warp == 0) {
             uint32_t parity = 1;                                 // the first round passes at once
@@ -340,27 +445,30 @@ moe_kernel(const __grid_constant__ CUtensorMap map_gate, const __grid_constant__
             for (int i = 0, s = 0; i < n; ++i) {
                 if (!warp_wait(&empty[s], parity, abortp)) break;
                 unsigned char *st = tiles + s * C::STAGE + C::W_BYTES, *ss = sf + s * C::SF + 2 * TILE_BYTES;
-                if (i < n1) {
+                const bool one = i < n1;
+                const int l = one ? a.l : b.l, k = one ? a.k : b.k;
+                if (one && !C::COMPACT) {
                     if (elect_one()) {
                         mbar_expect_tx(&full[s], C::X_BYTES + TILE_BYTES);
-                        tma_load_2d(st, &map_x, &full[s], a.k * 128, 0);
-                        bulk_load(ss, p.xs + (size_t)a.k * TILE_BYTES, TILE_BYTES, &full[s]);
+                        tma_load_2d(st, &map_x, &full[s], k * 128, 0);
+                        bulk_load(ss, p.xs + (size_t)k * TILE_BYTES, TILE_BYTES, &full[s]);
                     }
-                    a.next();
                 } else {
-                    if (b.l != seen) {                           // all of this expert's h is there
-                        if (!__all_sync(0xffffffffu, wait_count(&p.ready[b.l], tiles1, abortp))) break;
+                    if (i == n1) seen = -1;
+                    if (l != seen) {                             // all of this expert's rows are there
+                        if (!__all_sync(0xffffffffu, wait_count(one ? &p.ready[p.most_live + l] : &p.ready[l], one ? q.count[l] : tiles1, abortp))) break;
                         fence_async();
-                        seen = b.l;
+                        seen = l;
                     }
-                    const int boxes = (q.count[b.l] + 7) / 8 * 2;
+                    const int boxes = (q.count[l] + 7) / 8 * 2, row0 = q.hrow8[l] * 8;
                     if (elect_one()) {
                         mbar_expect_tx(&full[s], boxes * 1024 + TILE_BYTES);
-                        bulk_load(ss, p.hs + ((size_t)b.l * g2 + b.k) * TILE_BYTES, TILE_BYTES, &full[s]);
-                        for (int j = 0; j < boxes; ++j) tma_load_2d(st + j * 1024, &map_h, &full[s], b.k * 128, (q.hrow8[b.l] + j) * 8);
+                        bulk_load(ss, (one ? p.xs + ((size_t)l * g1 + k) * TILE_BYTES : p.hs + ((size_t)l * g2 + k) * TILE_BYTES), TILE_BYTES, &full[s]);
+                        for (int j = 0; j < boxes; ++j) tma_load_2d(st + j * 1024, one ? &map_x : &map_h, &full[s], k * 128, row0 + j * 8);
                     }
-                    b.next();
                 }
+                if (one) a.next();
+                else b.next();
                 __syncwarp();
                 if (++s == STAGES) { s = 0; parity ^= 1; }
             }
@@ -375,10 +483,10 @@ moe_kernel(const __grid_constant__ CUtensorMap map_gate, const __grid_constant__
                 if (!warp_wait(&full[s], parity, abortp)) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const uint32_t ss = sf0 + s * C::SF, tsf = tmem_sf + s * C::SF_COLS;
-                const int cols = i < n1 ? NCOL : (q.count[b.l] + 7) / 8 * 16;
-                const uint32_t idesc = 5u << 7 | (uint32_t)(cols >> 3) << 17 | 1u << 23 | 1u << 27;           // E2M1 by E4M3, scales E8M0
+                const int n_cols = i < n1 ? (C::COMPACT ? (q.count[a.l] + 7) / 8 * 16 : NCOL) : (q.count[b.l] + 7) / 8 * 16;
+                const uint32_t idesc = 5u << 7 | (uint32_t)(n_cols >> 3) << 17 | 1u << 23 | 1u << 27;           // E2M1 by E4M3, scales E8M0
                 const uint64_t da = desc0 + (uint32_t)(s * (C::STAGE >> 4)), db = da + (C::W_BYTES >> 4);
-                const uint32_t d = tmem + buf * 2 * NCOL;
+                const uint32_t d = tmem + buf * 2 * cols;
                 const bool done = i == n1 - 1 || i == n - 1 || (i < n1 ? a.k == g1 - 1 : b.k == g2 - 1);
                 if (elect_one()) {
 #pragma unroll
@@ -387,7 +495,7 @@ moe_kernel(const __grid_constant__ CUtensorMap map_gate, const __grid_constant__
                     for (uint32_t j = 0; j < 4; ++j)
 #pragma unroll
                         for (int w = 0; w < 2; ++w)
-                            umma_scaled<true>(d + w * NCOL, da + w * 1024 + 2 * j, db + 2 * j, idesc | j << 4 | j << 29, tsf + w * 4, tsf + 8, j > 0 || !fresh);
+                            umma_scaled<true>(d + w * cols, da + w * 1024 + 2 * j, db + 2 * j, idesc | j << 4 | j << 29, tsf + w * 4, tsf + 8, j > 0 || !fresh);
                     umma_commit(&empty[s]);
                     if (done) umma_commit(&acc_full[buf]);
                 }
@@ -395,16 +503,17 @@ moe_kernel(const __grid_constant__ CUtensorMap map_gate, const __grid_constant__
                 if (i < n1) a.next();
                 else b.next();
                 fresh = done;
-                if (done && ++buf == C::BUFS) { buf = 0; acc_parity ^= 1; }
+                if (done && ++buf == bufs) { buf = 0; acc_parity ^= 1; }
                 if (++s == STAGES) { s = 0; parity ^= 1; }
             }
         } else if (warp >= 4) {
             const int half = (warp - 4) / 4, quarter = warp & 3, row = quarter * 32 + lane;
             const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+            constexpr int SHARES = 8;
             int seg = 0;
             bool out = false;
             auto begin = [&]() {                                  // the sums of a segment are there; false: a wait ran out
-                mbar_wait(&acc_full[seg % C::BUFS], (seg / C::BUFS) & 1, abortp);
+                mbar_wait(&acc_full[seg % bufs], (seg / bufs) & 1, abortp);
                 asm volatile("bar.sync 1, 256;" ::: "memory");
                 if (threadIdx.x == 128) gone = *abortp;
                 asm volatile("bar.sync 1, 256;" ::: "memory");
@@ -414,8 +523,9 @@ moe_kernel(const __grid_constant__ CUtensorMap map_gate, const __grid_constant__
             auto release = [&]() {
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&acc_empty[seg % C::BUFS]);
+                if (lane == 0) mbar_arrive(&acc_empty[seg % bufs]);
             };
+            if (C::COMPACT) moe_compact(p, q);
             auto last_of = [&](int* counter, int others) {        // of the CTAs that share a tile
                 __threadfence();
                 asm volatile("bar.sync 1, 256;" ::: "memory");
@@ -424,16 +534,16 @@ moe_kernel(const __grid_constant__ CUtensorMap map_gate, const __grid_constant__
                 __threadfence();
                 return is_last != 0;
             };
-            // ---- gate and up: the halves take four of the expert's tokens in turn
+            // ---- gate and up: the halves take the expert's tokens in turn
             while (a.n > 0) {
                 const int l = a.l, tile = a.tile, unit = l * tiles1 + tile, take = min(a.n, g1 - a.k);
                 const bool whole = take == g1;
                 a.step(take);
                 if (!begin()) { out = true; break; }
                 const int count = q.count[l], first = q.first[l], nt = (count + 7) / 8 * 8, f = tile * 128 + row;
-                const uint32_t dg = tmem + lanes + (seg % C::BUFS) * 2 * NCOL, du = dg + NCOL;
+                const uint32_t dg = tmem + lanes + (seg % bufs) * 2 * cols, du = dg + cols;
                 auto hidden = [&](int r, float g, float u) {      // all lanes of a warp: a block of 32 of row r of the expert's h
-                    const float w = q.weight[first + r];
+                    const float w = q.weight[q.plane[first + r]];
                     if (p.scale_in) { g *= w; u *= w; }
                     float h[4] = {f < p.F ? moe_glu(g, u, p.act, p.limit) * (p.scale_in ? 1.f : w) : 0.f, 0.f, 0.f, 0.f};
                     const int byte = term_byte(__reduce_max_sync(0xffffffffu, __float_as_uint(h[0]) & 0x7fffffffu));
@@ -450,20 +560,23 @@ moe_kernel(const __grid_constant__ CUtensorMap map_gate, const __grid_constant__
                     }
                 };
                 float* mine = p.part1 + (size_t)(cta * 2 + s1.place(cta, unit)) * (2 * TT * 128) + row;
+#pragma unroll 1
                 for (int r0 = half * 4; r0 < count; r0 += 8) {
-                    float g[4][2], u[4][2];
+                    uint32_t g[4][2], u[4][2];
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        const int t = r0 + j < count ? q.token[first + r0 + j] : 0;
-                        g[j][0] = tmem_one(dg + t), g[j][1] = tmem_one(dg + TT + t);
-                        u[j][0] = tmem_one(du + t), u[j][1] = tmem_one(du + TT + t);
+                        const int t = C::COMPACT ? min(r0 + j, nt - 1) : r0 + j < count ? q.token[first + r0 + j] : 0, lo = C::COMPACT ? nt : TT;
+                        tmem_one(g[j][0], dg + t), tmem_one(g[j][1], dg + lo + t);
+                        tmem_one(u[j][0], du + t), tmem_one(u[j][1], du + lo + t);
                     }
                     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        asm volatile("" : "+f"(g[j][0]), "+f"(g[j][1]), "+f"(u[j][0]), "+f"(u[j][1]));       // not before the wait
-                        if (r0 + j >= count) break;
-                        const float gs = g[j][0] + g[j][1], us = u[j][0] + u[j][1];
+                    for (int j = 0; j < 4; ++j) asm volatile("" : "+r"(g[j][0]), "+r"(g[j][1]), "+r"(u[j][0]), "+r"(u[j][1]));   // not before the wait
+#pragma unroll 1
+                    for (int j = 0; j < 4 && r0 + j < count; ++j) {
+                        const float gs = __uint_as_float(g[0][0]) + __uint_as_float(g[0][1]), us = __uint_as_float(u[0][0]) + __uint_as_float(u[0][1]);
+#pragma unroll
+                        for (int k = 0; k < 3; ++k) g[k][0] = g[k + 1][0], g[k][1] = g[k + 1][1], u[k][0] = u[k + 1][0], u[k][1] = u[k + 1][1];
                         if (whole) hidden(r0 + j, gs, us);
                         else mine[(r0 + j) * 128] = gs, mine[(TT + r0 + j) * 128] = us;
                     }
@@ -473,18 +586,27 @@ moe_kernel(const __grid_constant__ CUtensorMap map_gate, const __grid_constant__
                 if (!whole) {
                     const int c0 = s1.owner(unit * g1), c1 = s1.owner((unit + 1) * g1 - 1);
                     if (!last_of(&p.counters[unit], c1 - c0)) continue;
+                    // one CTA's share after another's, the loads of eight at once
+#pragma unroll 1
                     for (int r = half; r < count; r += 2) {
                         float g = 0.f, u = 0.f;
-#pragma unroll 8
-                        for (int c = c0; c <= c1; ++c) {
-                            const float* from = p.part1 + (size_t)(c * 2 + s1.place(c, unit)) * (2 * TT * 128) + r * 128 + row;
-                            g += __ldcg(from), u += __ldcg(from + TT * 128);
+#pragma unroll 1
+                        for (int c = c0; c <= c1; c += SHARES) {
+                            float gp[SHARES], up[SHARES];
+#pragma unroll
+                            for (int k = 0; k < SHARES; ++k) {
+                                const int cc = min(c + k, c1);
+                                const float* from = p.part1 + (size_t)(cc * 2 + s1.place(cc, unit)) * (2 * TT * 128) + r * 128 + row;
+                                gp[k] = __ldcg(from), up[k] = __ldcg(from + TT * 128);
+                            }
+#pragma unroll
+                            for (int k = 0; k < SHARES; ++k)
+                                if (c + k <= c1) g += gp[k], u += up[k];
                         }
                         hidden(r, g, u);
                     }
                 }
                 fence_async();
-                __threadfence();
                 asm volatile("bar.sync 1, 256;" ::: "memory");
                 if (threadIdx.x == 128) {
                     __threadfence();
@@ -498,7 +620,7 @@ moe_kernel(const __grid_constant__ CUtensorMap map_gate, const __grid_constant__
                 b.step(take);
                 if (!begin()) break;
                 const int count = q.count[l], first = q.first[l], nt = (count + 7) / 8 * 8, f = (tile * 2 + half) * 128 + row;
-                const uint32_t d = tmem + lanes + ((seg % C::BUFS) * 2 + half) * NCOL;
+                const uint32_t d = tmem + lanes + ((seg % bufs) * 2 + half) * cols;
                 float* mine = p.part2 + ((size_t)(cta * 2 + s2.place(cta, unit)) * 2 + half) * (TT * 128) + row;
                 auto store = [&](int r, float v) {
                     if (f < p.H) p.planes[(size_t)q.plane[first + r] * p.H + f] = v;
@@ -524,12 +646,28 @@ moe_kernel(const __grid_constant__ CUtensorMap map_gate, const __grid_constant__
                 if (whole) continue;
                 const int c0 = s2.owner(unit * g2), c1 = s2.owner((unit + 1) * g2 - 1);
                 if (!last_of(&units2[unit], c1 - c0)) continue;
-                for (int r = 0; r < count; ++r) {
-                    float v = 0.f;
-#pragma unroll 8
-                    for (int c = c0; c <= c1; ++c)
-                        v += __ldcg(p.part2 + ((size_t)(c * 2 + s2.place(c, unit)) * 2 + half) * (TT * 128) + r * 128 + row);
-                    store(r, v);
+#pragma unroll 1
+                for (int r = 0; r < count; r += 4) {
+                    float v[4] = {};
+#pragma unroll 1
+                    for (int c = c0; c <= c1; c += SHARES) {
+                        float part[SHARES][4];
+#pragma unroll
+                        for (int k = 0; k < SHARES; ++k) {
+                            const int cc = min(c + k, c1);
+                            const float* from = p.part2 + ((size_t)(cc * 2 + s2.place(cc, unit)) * 2 + half) * (TT * 128) + r * 128 + row;
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) part[k][j] = __ldcg(from + j * 128);
+                        }
+#pragma unroll
+                        for (int k = 0; k < SHARES; ++k)
+#pragma unroll
+                            for (int j = 0; j < 4; ++j)
+                                if (c + k <= c1) v[j] += part[k][j];
+                    }
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        if (r + j < count) store(r + j, v[j]);
                 }
             }
         }
@@ -565,6 +703,7 @@ moe_kernel(const __grid_constant__ CUtensorMap map_gate, const __grid_constant__
 
 struct MoePlan {
     int tt, P, most_live, most_rows, ncounters;
+    bool compact;
     long long xt, xs, h, hs, z, sel_e, sel_w, part1, part2, planes, counters, bytes;
 };
 inline MoePlan moe_plan(int T, int H, int F, int E, int top) {
@@ -574,11 +713,12 @@ inline MoePlan moe_plan(int T, int H, int F, int E, int top) {
     q.most_live = E < T * top ? E : T * top;
     q.most_rows = 2 * (T * top + 7 * q.most_live);
     const long long g1 = groups_of(H), g2 = groups_of(F), tiles2 = ((H + 127) / 128 + 1) / 2;
-    q.ncounters = (int)(q.most_live * (g2 + tiles2) + q.most_live);
+    q.ncounters = (int)(q.most_live * (g2 + tiles2) + 2 * q.most_live);
     long long at = 0;
     auto take = [&](long long bytes) { const long long o = at; at += (bytes + 1023) / 1024 * 1024; return o; };
-    q.xt = take(2LL * q.tt * g1 * GROUP);
-    q.xs = take(g1 * TILE_BYTES);
+    q.compact = q.tt > 16;
+    q.xt = take((q.compact ? (long long)q.most_rows : 2LL * q.tt) * g1 * GROUP);
+    q.xs = take((q.compact ? q.most_live : 1) * g1 * TILE_BYTES);
     q.h = take((long long)q.most_rows * g2 * GROUP);
     q.hs = take(q.most_live * g2 * TILE_BYTES);
     q.z = take(4LL * T * E);
@@ -644,7 +784,7 @@ PRISM_EXPORT int prism_mxfp4_moe(const void* x, long long ldx, const void* route
     int rc = byte_map(&m[0], gate_codes, (long long)E * F, (long long)g1 * 64, 128, true);
     if (!rc) rc = byte_map(&m[1], up_codes, (long long)E * F, (long long)g1 * 64, 128, true);
     if (!rc) rc = byte_map(&m[2], down_codes, (long long)E * H, (long long)g2 * 64, 128, true);
-    if (!rc) rc = byte_map(&m[3], base + q.xt, 2 * q.tt, (long long)g1 * GROUP, 2 * q.tt, false);
+    if (!rc) rc = byte_map(&m[3], base + q.xt, q.compact ? q.most_rows : 2 * q.tt, (long long)g1 * GROUP, q.compact ? 8 : 2 * q.tt, false);
     if (!rc) rc = byte_map(&m[4], base + q.h, q.most_rows, (long long)g2 * GROUP, 8, false);
     if (rc) return rc;
     Moe p;
@@ -661,14 +801,14 @@ PRISM_EXPORT int prism_mxfp4_moe(const void* x, long long ldx, const void* route
     p.part2 = reinterpret_cast<float*>(base + q.part2);
     p.planes = reinterpret_cast<float*>(base + q.planes);
     p.ready = reinterpret_cast<int*>(base + q.counters);
-    p.counters = p.ready + q.most_live;
+    p.counters = p.ready + 2 * q.most_live;
     p.control = control, p.err = err;
     p.y = y;
     p.ldx = ldx, p.ldy = ldy;
     p.T = T, p.H = H, p.F = F, p.E = E, p.top = top, p.softmax = softmax, p.renorm = renorm, p.scale_in = scale_in, p.act = act;
     p.groups_of_experts = groups, p.keep = keep;
-    const int warps = q.P * MOE_WARPS, each = (T * E + warps - 1) / warps;
-    p.experts_a_warp = each < 4 ? each : 4;
+    p.dots = (T * E + q.P - 1) / q.P;
+    p.most_live = q.most_live;
     p.ncounters = q.ncounters;
     p.router_bf16 = router_dtype == PRISM_DTYPE_BF16, p.rbias_bf16 = rbias_dtype == PRISM_DTYPE_BF16, p.corr_bf16 = corr_dtype == PRISM_DTYPE_BF16;
     p.out_bf16 = out_dtype == PRISM_DTYPE_BF16;
