@@ -62,8 +62,9 @@ struct Lists {                             // of the experts that have tokens, i
     short slot[MOE_MOST_EXPERTS], expert[MOE_MOST_EXPERTS], count[MOE_MOST_EXPERTS], hrow8[MOE_MOST_EXPERTS], first[MOE_MOST_EXPERTS];
     // an expert's tokens from first[] on, ascending
     float weight[MOE_MOST_ENTRIES];
-    short plane[MOE_MOST_ENTRIES], first_plane[MOE_MOST_ENTRIES];
-    short expert_of[MOE_MOST_ENTRIES];     // by choice, token after token
+    short plane[MOE_MOST_ENTRIES], owner[MOE_MOST_ENTRIES];
+    // by choice, token after token
+    short expert_of[MOE_MOST_ENTRIES], first_plane[MOE_MOST_ENTRIES];
     unsigned char token[MOE_MOST_ENTRIES];
     int live, entries, most;               // experts with tokens, their tokens in all, the most of one
 };
@@ -129,14 +130,14 @@ __device__ __forceinline__ void row_terms(const uint4& raw, int c, uint8_t* hi_r
 }
 
 // A token's choice by one warp whose lanes keep its scores (lane, lane + 32, ...): as moe_route_token, without groups.
-__device__ __forceinline__ void choose(const Moe& p, int t) {
+__device__ __forceinline__ void choose(const Moe& p, int t, const float* z) {       // z: shared memory
     constexpr int EACH = MOE_MOST_EXPERTS / 32;
     const int lane = threadIdx.x & 31;
     float s[EACH], mx = -INFINITY, den = 0.f;
     int key[EACH];
 #pragma unroll
     for (int i = 0; i < EACH; ++i) {
-        s[i] = lane + 32 * i < p.E ? __ldcg(p.z + t * p.E + lane + 32 * i) : -INFINITY;
+        s[i] = lane + 32 * i < p.E ? z[lane + 32 * i] : -INFINITY;
         mx = fmaxf(mx, s[i]);
     }
     mx = warp_max(mx);
@@ -181,12 +182,13 @@ __device__ __forceinline__ void choose(const Moe& p, int t) {
     if (lane < p.top) p.sel_w[t * p.top + lane] = (p.renorm ? mine / (chosen + p.sum_eps) : mine) * p.wscale;
 }
 
-// 1: logits, choices, x's terms.  A CTA has `dots` neighbouring logits (of one token or two); where they are few, several warps
-// share a row.
+// 1: logits, choices, x's terms.  A CTA has all logits of a token, or, where a router's rows are too many for that, `dots`
+// neighbouring ones (of one token or two), and the CTA that finishes a token's makes its choice.  Several warps share a row where
+// there are few.
 template <typename C> __device__ __forceinline__ void moe_route_and_terms(const Moe& p, float* scratch) {
     __shared__ int finished[2];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int gtid = blockIdx.x * MOE_THREADS + threadIdx.x, threads = gridDim.x * MOE_THREADS;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, back = gridDim.x - 1 - blockIdx.x;
+    const int gtid = back * MOE_THREADS + threadIdx.x, threads = gridDim.x * MOE_THREADS;       // the last CTAs, which have no logits, first
     for (int i = gtid; i < p.ncounters; i += threads) p.ready[i] = 0;             // and the tiles' counters behind them
     if (!C::COMPACT) {
         const int groups = groups_of(p.H), per_row = groups * (GROUP / 8);
@@ -202,20 +204,32 @@ template <typename C> __device__ __forceinline__ void moe_route_and_terms(const 
     if (count <= 0) return;
     const int parts = p.dots >= MOE_WARPS ? 1 : MOE_WARPS / p.dots, at_once = MOE_WARPS / parts, part = warp % parts;
     const int len = ((p.H + parts - 1) / parts + 7) / 8 * 8, k0 = part * len, k1 = min(p.H, k0 + len);
-    const bool wide = p.wide && p.H % 8 == 0;
+    const bool wide = p.wide && p.H % 8 == 0, whole = p.dots == p.E;
 #pragma unroll 1
     for (int i = warp / parts; i < count; i += at_once) {
         const int t = (first + i) / p.E, e = first + i - t * p.E;
         const __nv_bfloat16* row = p.x + (long long)t * p.ldx;
         float sum = 0.f;
-        if (wide) {
-#pragma unroll 4
-            for (int k = k0 + lane * 8; k < k1; k += 256) {
-                float a[8], w[8];
-                load8(row + k, a);
-                load_param8(p.router, p.router_bf16, (size_t)e * p.H + k, w);
+        if (wide && p.router_bf16) {
+            const __nv_bfloat16* r = static_cast<const __nv_bfloat16*>(p.router) + (size_t)e * p.H;
+#pragma unroll 1
+            for (int k = k0 + lane * 8; k < k1; k += 8 * 256) {              // eight pieces of either row on their way at once
+                uint4 a[8], w[8];
 #pragma unroll
-                for (int l = 0; l < 8; ++l) sum = fmaf(a[l], w[l], sum);
+                for (int j = 0; j < 8; ++j) {
+                    const int at = k + j * 256;
+                    a[j] = at < k1 ? *reinterpret_cast<const uint4*>(row + at) : make_uint4(0, 0, 0, 0);
+                    w[j] = at < k1 ? *reinterpret_cast<const uint4*>(r + at) : make_uint4(0, 0, 0, 0);
+                }
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+#pragma unroll
+                    for (int l = 0; l < 4; ++l) {
+                        const float2 f = __bfloat1622float2(reinterpret_cast<const __nv_bfloat162*>(&a[j])[l]);
+                        const float2 g = __bfloat1622float2(reinterpret_cast<const __nv_bfloat162*>(&w[j])[l]);
+                        sum = fmaf(f.x, g.x, sum);
+                        sum = fmaf(f.y, g.y, sum);
+                    }
             }
         } else {
 #pragma unroll 8
@@ -225,39 +239,44 @@ template <typename C> __device__ __forceinline__ void moe_route_and_terms(const 
         if (lane == 0) scratch[i * parts + part] = sum;
     }
     __syncthreads();
+    float* zs = scratch + p.dots * parts;                      // the logits, of a token or (then for two warps) of two
     for (int i = threadIdx.x; i < count; i += MOE_THREADS) {
         const int t = (first + i) / p.E, e = first + i - t * p.E;
         float sum = p.rbias != nullptr ? load_param(p.rbias, p.rbias_bf16, e) : 0.f;
         for (int j = 0; j < parts; ++j) sum += scratch[i * parts + j];
-        p.z[first + i] = sum;
+        if (whole) zs[i] = sum;
+        else p.z[first + i] = sum;
     }
     __syncthreads();
     const int t0 = first / p.E, t1 = (first + count - 1) / p.E;             // no more than E logits: two tokens at most
-    if (threadIdx.x < 2) {
-        const int t = t0 + threadIdx.x;
-        finished[threadIdx.x] = 0;
-        if (t <= t1) {
-            const int here = min(first + count, (t + 1) * p.E) - max(first, t * p.E);
-            __threadfence();
-            finished[threadIdx.x] = atomicAdd(&p.control[2 + t], here) == p.E - here;
-            __threadfence();
+    if (!whole) {
+        if (threadIdx.x < 2) {
+            const int t = t0 + threadIdx.x;
+            finished[threadIdx.x] = 0;
+            if (t <= t1) {
+                const int here = min(first + count, (t + 1) * p.E) - max(first, t * p.E);
+                __threadfence();
+                finished[threadIdx.x] = atomicAdd(&p.control[2 + t], here) == p.E - here;
+                __threadfence();
+            }
         }
+        __syncthreads();
     }
-    __syncthreads();
-    if (warp >= 2 || !finished[warp]) return;
+    if (warp >= 2 || (whole ? warp > 0 : !finished[warp])) return;
     const int t = t0 + warp;
+    zs += warp * (4 * p.E + 2 * p.groups_of_experts + 16);
+    if (!whole) {
+        for (int e = lane; e < p.E; e += 32) zs[e] = __ldcg(p.z + t * p.E + e);
+        __syncwarp();
+    }
     if (p.groups_of_experts > 1 && p.keep < p.groups_of_experts) {
-        float* zs = scratch + (size_t)warp * (4 * p.E + 2 * p.groups_of_experts + 16);
         int* counts = reinterpret_cast<int*>(zs + 3 * p.E + 2 * p.groups_of_experts);
-        for (int e = lane; e < p.E; e += 32) {
-            zs[e] = __ldcg(p.z + t * p.E + e);
-            counts[e] = 0;
-        }
+        for (int e = lane; e < p.E; e += 32) counts[e] = 0;
         __syncwarp();
         moe_route_token(zs, zs + p.E, zs + 2 * p.E, zs + 3 * p.E, p.E, p.top, p.softmax, p.renorm, lane, counts, p.sel_e + t * p.top,
                         p.sel_w + t * p.top, counts + p.E, p.corr, p.corr_bf16, p.groups_of_experts, p.keep, p.wscale, p.sum_eps);
     } else {
-        choose(p, t);
+        choose(p, t, zs);
     }
 }
 
@@ -315,6 +334,7 @@ __device__ __forceinline__ void moe_lists(const Moe& p, Lists& q) {
         const int at = q.first[q.slot[e]] + __popcll(q.mask[e] & ((1ull << t) - 1));
         q.token[at] = (unsigned char)t;
         q.plane[at] = (short)i;
+        q.owner[at] = q.slot[e];
     }
     __syncthreads();
 }
@@ -323,20 +343,18 @@ __device__ __forceinline__ void moe_lists(const Moe& p, Lists& q) {
 __device__ __forceinline__ void moe_compact(const Moe& p, const Lists& q) {
     const int groups = groups_of(p.H);
     const size_t pitch = (size_t)groups * GROUP;
-    int l = 0;
-    for (int i = blockIdx.x; i < q.entries; i += gridDim.x) {
-        while (i >= q.first[l] + q.count[l]) ++l;
+    const int chunks = groups * (GROUP / 8), mine = (q.entries - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x;
+    for (int w = threadIdx.x - 128; w < mine * chunks; w += 256) {
+        const int j = w / chunks, c = (w - j * chunks) * 8, i = blockIdx.x + j * gridDim.x, l = q.owner[i];
         const int r = i - q.first[l], nt = (q.count[l] + 7) / 8 * 8;
-        const __nv_bfloat16* row = p.x + (long long)q.token[i] * p.ldx;
         uint8_t* to = p.xt + (size_t)(q.hrow8[l] * 8 + r) * pitch;
-        for (int c = (threadIdx.x - 128) * 8; c < groups * GROUP; c += 256 * 8)
-            row_terms(row8(row, c, p.H, p.wide), c, to, to + nt * pitch, p.xs + (size_t)l * groups * TILE_BYTES, r, nt + r);
-        fence_async();
-        asm volatile("bar.sync 1, 256;" ::: "memory");
-        if (threadIdx.x == 128) {
-            __threadfence();
-            atomicAdd(&p.ready[p.most_live + l], 1);
-        }
+        row_terms(row8(p.x + (long long)q.token[i] * p.ldx, c, p.H, p.wide), c, to, to + nt * pitch, p.xs + (size_t)l * groups * TILE_BYTES, r, nt + r);
+    }
+    fence_async();
+    asm volatile("bar.sync 1, 256;" ::: "memory");
+    for (int j = threadIdx.x - 128; j < mine; j += 256) {
+        __threadfence();
+        atomicAdd(&p.ready[p.most_live + q.owner[blockIdx.x + j * gridDim.x]], 1);
     }
 }
 
@@ -377,6 +395,10 @@ moe_kernel(const __grid_constant__ CUtensorMap map_gate, const __grid_constant__
         for (int s = 0; s < STAGES; ++s) { mbar_init(&full[s], 2); mbar_init(&empty[s], 1); }
         for (int s = 0; s < 2; ++s) { mbar_init(&acc_full[s], 1); mbar_init(&acc_empty[s], 8); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 2 && lane < 5) {
+        const CUtensorMap* m = lane == 0 ? &map_gate : lane == 1 ? &map_up : lane == 2 ? &map_down : lane == 3 ? &map_x : &map_h;
+        asm volatile("prefetch.tensormap [%0];" ::"l"(m) : "memory");
     }
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(tmem_slot)), "r"(C::COLS));
@@ -588,22 +610,27 @@ moe_kernel(const __grid_constant__ CUtensorMap map_gate, const __grid_constant__
                     if (!last_of(&p.counters[unit], c1 - c0)) continue;
                     // one CTA's share after another's, the loads of eight at once
 #pragma unroll 1
-                    for (int r = half; r < count; r += 2) {
-                        float g = 0.f, u = 0.f;
+                    for (int r = half * 2; r < count; r += 4) {
+                        float g[2] = {}, u[2] = {};
 #pragma unroll 1
                         for (int c = c0; c <= c1; c += SHARES) {
-                            float gp[SHARES], up[SHARES];
+                            float gp[SHARES][2], up[SHARES][2];
 #pragma unroll
                             for (int k = 0; k < SHARES; ++k) {
                                 const int cc = min(c + k, c1);
                                 const float* from = p.part1 + (size_t)(cc * 2 + s1.place(cc, unit)) * (2 * TT * 128) + r * 128 + row;
-                                gp[k] = __ldcg(from), up[k] = __ldcg(from + TT * 128);
+                                gp[k][0] = __ldcg(from), gp[k][1] = __ldcg(from + 128);
+                                up[k][0] = __ldcg(from + TT * 128), up[k][1] = __ldcg(from + TT * 128 + 128);
                             }
 #pragma unroll
                             for (int k = 0; k < SHARES; ++k)
-                                if (c + k <= c1) g += gp[k], u += up[k];
+                                if (c + k <= c1) g[0] += gp[k][0], g[1] += gp[k][1], u[0] += up[k][0], u[1] += up[k][1];
                         }
-                        hidden(r, g, u);
+#pragma unroll 1
+                        for (int j = 0; j < 2 && r + j < count; ++j) {
+                            hidden(r + j, g[0], u[0]);
+                            g[0] = g[1], u[0] = u[1];
+                        }
                     }
                 }
                 fence_async();
@@ -807,7 +834,9 @@ PRISM_EXPORT int prism_mxfp4_moe(const void* x, long long ldx, const void* route
     p.ldx = ldx, p.ldy = ldy;
     p.T = T, p.H = H, p.F = F, p.E = E, p.top = top, p.softmax = softmax, p.renorm = renorm, p.scale_in = scale_in, p.act = act;
     p.groups_of_experts = groups, p.keep = keep;
-    p.dots = (T * E + q.P - 1) / q.P;
+    // a token's logits in one CTA save a pass through memory (1 token, 8 experts of 2,048: 1.1 us) while there is a warp for each of
+    // them and their rows are not long for one SM (64 experts: 9.7 us over all SMs, 11.6 a token an SM)
+    p.dots = E <= MOE_WARPS && (long long)E * H <= (1 << 18) && T <= q.P ? E : (T * E + q.P - 1) / q.P;
     p.most_live = q.most_live;
     p.ncounters = q.ncounters;
     p.router_bf16 = router_dtype == PRISM_DTYPE_BF16, p.rbias_bf16 = rbias_dtype == PRISM_DTYPE_BF16, p.corr_bf16 = corr_dtype == PRISM_DTYPE_BF16;
