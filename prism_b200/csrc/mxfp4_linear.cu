@@ -501,7 +501,8 @@ inline Plan plan_for(int M, int N, int K, int act_bits) {
 
 template <typename C> int run_product(const CUtensorMap& mw, const CUtensorMap& mx, const Product& p, cudaStream_t stream) {
     auto kern = product_kernel<C>;
-    cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::SMEM);
+    static unsigned char done[64] = {};
+    open_once(kern, C::SMEM, done);
     return (int)launch_kernel(kern, dim3(p.split.P), dim3(C::THREADS), C::SMEM, stream, mw, mx, p);
 }
 

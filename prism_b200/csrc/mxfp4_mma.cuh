@@ -149,13 +149,23 @@ inline int byte_map(CUtensorMap* map, const void* ptr, long long rows, long long
     return r == CUDA_SUCCESS ? 0 : (int)cudaErrorInvalidValue;
 }
 
-inline int sm_count() {
-    static int n[64] = {};
+inline int current_device() {
     int dev = 0;
     cudaGetDevice(&dev);
+    return dev;
+}
+inline int sm_count() {
+    static int n[64] = {};
+    const int dev = current_device();
     if (dev < 0 || dev >= 64) return 148;
     if (!n[dev]) cudaDeviceGetAttribute(&n[dev], cudaDevAttrMultiProcessorCount, dev);
     return n[dev];
+}
+// A kernel's limit of shared memory, always the same value: asked for once on a device
+template <typename... KArgs> inline void open_once(void (*kern)(KArgs...), size_t smem, unsigned char (&done)[64]) {
+    const int dev = current_device();
+    if (dev >= 0 && dev < 64 && done[dev]) return;
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) == cudaSuccess && dev >= 0 && dev < 64) done[dev] = 1;
 }
 
 }  // namespace mx

@@ -766,7 +766,8 @@ inline bool moe_sizes_ok(int T, int H, int F, int E, int top) {
 
 template <typename C> int run_moe(const CUtensorMap (&m)[5], const Moe& p, int P, cudaStream_t stream) {
     auto kern = moe_kernel<C>;
-    cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::SMEM);
+    static unsigned char done[64] = {};
+    open_once(kern, C::SMEM, done);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(P);
     cfg.blockDim = dim3(MOE_THREADS);

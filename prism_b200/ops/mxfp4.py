@@ -34,12 +34,19 @@ class Mxfp4:
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, K: int):
         cs, ss = codes.shape, scales.shape
-        groups = -(-K // GROUP)
-        if not (K > 0 and codes.dtype is torch.uint8 and scales.dtype is torch.uint8 and codes.is_contiguous() and scales.is_contiguous()
-                and codes.device == scales.device and len(cs) in (2, 3) and cs[-1] == groups * (GROUP // 2) and cs[-2] > 0
-                and ss == cs[:-2] + (-(-cs[-2] // TILE_ROWS), groups, TILE_BYTES)):
+        groups, d = -(-K // GROUP), len(cs)
+        if not (K > 0 and (d == 2 or d == 3) and len(ss) == d + 1 and cs[-1] == groups * (GROUP // 2) and cs[-2] > 0
+                and ss[-1] == TILE_BYTES and ss[-2] == groups and ss[-3] == -(-cs[-2] // TILE_ROWS) and ss[0] == (cs[0] if d == 3 else ss[-3])
+                and codes.dtype is torch.uint8 and scales.dtype is torch.uint8 and codes.is_contiguous() and scales.is_contiguous()
+                and codes.device == scales.device):
             raise ops.KernelError(f"4-bit matrix of K = {K}: codes {tuple(cs)} {codes.dtype} and scales {tuple(ss)} {scales.dtype} do not belong together")
-        self.codes, self.scales, self.shape = codes, scales, cs[:-1] + (K,)
+        self.codes, self.scales, self.shape = codes, scales, (cs[0], K) if d == 2 else (cs[0], cs[1], K)
+
+    @classmethod
+    def _of(cls, codes, scales, shape) -> "Mxfp4":
+        q = object.__new__(cls)
+        q.codes, q.scales, q.shape = codes, scales, shape
+        return q
 
     @property
     def device(self):
@@ -56,17 +63,19 @@ class Mxfp4:
         """One matrix of a stack."""
         if len(self.shape) != 3:
             raise ops.KernelError("only a stack of 4-bit matrices can be indexed")
-        return Mxfp4(self.codes[e], self.scales[e], self.shape[-1])
+        return Mxfp4._of(self.codes[e], self.scales[e], self.shape[1:])
 
     def dequantize(self, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
         """The values that the codes stand for, exact in bfloat16 and float32; NaN where the scale is 255."""
         if dtype not in (torch.bfloat16, torch.float32):
             raise ops.KernelError(f"4-bit values come back as bfloat16 or float32, not {dtype}")
-        ops._cuda(self.codes)
-        out = torch.empty(self.shape, dtype=dtype, device=self.device)
-        N, K = self.shape[-2:]
-        ops._check(ops.lib().prism_mxfp4_dequantize(self.codes.data_ptr(), self.scales.data_ptr(), self.shape[0] if len(self.shape) == 3 else 1,
-                                                    N, K, out.data_ptr(), ops._dt(out), ops._stream()), "mxfp4_dequantize")
+        codes, shape = self.codes, self.shape
+        if not codes.is_cuda:
+            ops._cuda(codes)
+        out = codes.new_empty(shape, dtype=dtype)
+        ops._check(ops.lib().prism_mxfp4_dequantize(codes.data_ptr(), self.scales.data_ptr(), shape[0] if len(shape) == 3 else 1, shape[-2], shape[-1],
+                                                    out.data_ptr(), ops.F32 if dtype is torch.float32 else ops.BF16, ops._stream()),
+                   "mxfp4_dequantize")
         return out
 
 
@@ -76,16 +85,23 @@ def mxfp4_quantize(x: torch.Tensor) -> Mxfp4:
     saturate at 6.  A block that holds an infinity or NaN becomes NaN as a whole."""
     if not x.is_cuda:
         ops._cuda(x)
-    lead, (N, K) = x.shape[:-2], x.shape[-2:] if x.dim() in (2, 3) else (0, 0)
-    if not (N and K and (x.stride(-1) == 1 or K == 1) and (not lead or (lead[0] and x.is_contiguous()))):
+    xs = x.shape
+    d = len(xs)
+    N, K = (xs[-2], xs[-1]) if d == 2 or d == 3 else (0, 0)
+    if not (N and K and xs[0] and (x.stride(-1) == 1 or K == 1) and (d == 2 or x.is_contiguous())):
         raise ops.KernelError(f"rows to quantise: a matrix whose rows lie side by side in memory or a contiguous stack of them, got {tuple(x.shape)} "
                               f"with strides {x.stride()}")
-    groups = -(-K // GROUP)
-    codes = torch.empty(lead + (N, groups * (GROUP // 2)), dtype=torch.uint8, device=x.device)
-    scales = torch.empty(lead + (-(-N // TILE_ROWS), groups, TILE_BYTES), dtype=torch.uint8, device=x.device)
-    ops._check(ops.lib().prism_mxfp4_quantize(x.data_ptr(), ops._dt(x), x.stride(-2) if N > 1 else K, lead[0] if lead else 1, N, K,
-                                              codes.data_ptr(), scales.data_ptr(), ops._stream()), "mxfp4_quantize")
-    return Mxfp4(codes, scales, K)
+    groups, tiles = -(-K // GROUP), -(-N // TILE_ROWS)
+    if d == 2:
+        shape, matrices = (N, K), 1
+        codes, scales = x.new_empty((N, groups * 64), dtype=torch.uint8), x.new_empty((tiles, groups, TILE_BYTES), dtype=torch.uint8)
+    else:
+        shape, matrices = (xs[0], N, K), xs[0]
+        codes = x.new_empty((matrices, N, groups * 64), dtype=torch.uint8)
+        scales = x.new_empty((matrices, tiles, groups, TILE_BYTES), dtype=torch.uint8)
+    ops._check(ops.lib().prism_mxfp4_quantize(x.data_ptr(), ops._dt(x), x.stride(-2) if N > 1 else K, matrices, N, K, codes.data_ptr(),
+                                              scales.data_ptr(), ops._stream()), "mxfp4_quantize")
+    return Mxfp4._of(codes, scales, shape)
 
 
 _workspace_bytes = {}
@@ -169,7 +185,7 @@ def mxfp4_linear(x: torch.Tensor, w: Mxfp4, bias: Optional[torch.Tensor] = None,
     if bias is not None and (bias.shape != (N,) or not bias.is_contiguous()):
         raise ops.KernelError(f"a bias has one entry per row of the weight, got {tuple(bias.shape)}")
     if out is None:
-        out = torch.empty((M, N), dtype=out_dtype or torch.bfloat16, device=x.device)
+        out = x.new_empty((M, N), dtype=out_dtype)
     elif out.shape != (M, N) or (out.stride(1) != 1 and N > 1) or out_dtype not in (None, out.dtype):
         raise ops.KernelError(f"the result of {tuple(xs)} and {tuple(ws)} does not go into {tuple(out.shape)} {out.dtype}")
     if M == 0:
@@ -219,7 +235,7 @@ def mxfp4_moe(x: torch.Tensor, router: torch.Tensor, gate: Mxfp4, up: Mxfp4, dow
     if ch.groups < 1 or E % ch.groups or not 1 <= ch.keep <= ch.groups or ch.keep * (E // ch.groups) < top:
         raise ops.KernelError(f"{E} experts in {ch.groups} groups of which {ch.keep} are kept, {top} a token")
     if out is None:
-        out = torch.empty((T, H), dtype=out_dtype or torch.bfloat16, device=x.device)
+        out = x.new_empty((T, H), dtype=out_dtype)
     elif out.shape != (T, H) or out.stride(1) != 1 or out_dtype not in (None, out.dtype):
         raise ops.KernelError(f"the result of {T} rows of {H} does not go into {tuple(out.shape)} {out.dtype}")
     if T == 0:
