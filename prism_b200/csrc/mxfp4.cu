@@ -14,6 +14,8 @@ constexpr int THREADS = 256, AT_ONCE = 8, ROWS = THREADS / 16;      // rows of a
 
 __device__ __forceinline__ int scale_place(int r) { return (r & 31) * 16 + r / 32 * 4; }       // of row r of a tile, block 0
 
+template <typename T> struct alignas(16) Eight { T v[8]; };
+
 // x: a stack of matrices [rows, K] (row stride ld); grid (groups, tiles of rows, matrices)
 template <typename T>
 __global__ void __launch_bounds__(THREADS) quantise_kernel(const T* __restrict__ x_in, long long ld, int rows, int K, int groups, int wide,
@@ -26,37 +28,44 @@ __global__ void __launch_bounds__(THREADS) quantise_kernel(const T* __restrict__
     const T* x = pdl_fresh(x_in) + (long long)row0 * ld + k;
     uint8_t* code = codes + row0 * (groups * (size_t)(GROUP / 2)) + k / 2;
     const int here = min(TILE_ROWS, rows - r0);
-    for (int base = 0; base < here; base += ROWS * AT_ONCE) {
-        float v[AT_ONCE][8];
+    auto finish = [&](const float (&v)[8], int r) {
+        uint32_t most = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) most = max(most, __float_as_uint(v[j]) & 0x7fffffffu);
+        most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+        most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
+        const int byte = scale_byte(most);
+        const float inv = scale_inverse(byte);
+        uint32_t word = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) word |= pack2(v[2 * j] * inv, v[2 * j + 1] * inv) << (8 * j);
+        if (r < here) {
+            *reinterpret_cast<uint32_t*>(code + (size_t)r * (groups * (GROUP / 2))) = byte == 255 ? 0 : word;
+            if ((threadIdx.x & 3) == 0) sc[scale_place(r) + c / BLOCK] = (uint8_t)byte;
+        }
+    };
+    if (wide && here == TILE_ROWS && (g + 1) * GROUP <= K) {               // a whole tile: all of a thread's loads, then its work
+        Eight<T> raw[AT_ONCE];
+#pragma unroll
+        for (int i = 0; i < AT_ONCE; ++i) raw[i] = *reinterpret_cast<const Eight<T>*>(x + (long long)(i * ROWS + first) * ld);
 #pragma unroll
         for (int i = 0; i < AT_ONCE; ++i) {
-            const int r = base + i * ROWS + first;
+            float v[8];
+            load8(reinterpret_cast<const T*>(&raw[i]), v);
+            finish(v, i * ROWS + first);
+        }
+    } else {
+#pragma unroll 1
+        for (int r = first; r < ROWS * ((here + ROWS - 1) / ROWS); r += ROWS) {          // whole warps go round together
             const T* p = x + (long long)r * ld;
+            float v[8];
             if (wide && r < here && k + 8 <= K) {
-                load8(p, v[i]);
+                load8(p, v);
             } else {
 #pragma unroll
-                for (int j = 0; j < 8; ++j) v[i][j] = r < here && k + j < K ? to_float(p[j]) : 0.f;
+                for (int j = 0; j < 8; ++j) v[j] = r < here && k + j < K ? to_float(p[j]) : 0.f;
             }
-        }
-#pragma unroll
-        for (int i = 0; i < AT_ONCE; ++i) {
-            const int r = base + i * ROWS + first;
-            uint32_t most = 0;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) most = max(most, __float_as_uint(v[i][j]) & 0x7fffffffu);
-            most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
-            most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
-            const int byte = scale_byte(most);
-            const float inv = scale_inverse(byte);
-            uint32_t word = 0;
-            if (byte != 255)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) word |= pack2(v[i][2 * j] * inv, v[i][2 * j + 1] * inv) << (8 * j);
-            if (r < here) {
-                *reinterpret_cast<uint32_t*>(code + (size_t)r * (groups * (GROUP / 2))) = word;
-                if ((threadIdx.x & 3) == 0) sc[scale_place(r) + c / BLOCK] = (uint8_t)byte;
-            }
+            finish(v, r);
         }
     }
     __syncthreads();
@@ -86,12 +95,14 @@ __global__ void __launch_bounds__(THREADS) dequantise_kernel(const uint8_t* __re
         reinterpret_cast<uint4*>(sc)[threadIdx.x] =
             reinterpret_cast<const uint4*>(pdl_fresh(scales_in) + (((size_t)blockIdx.z * gridDim.y + blockIdx.y) * groups + g) * TILE_BYTES)[threadIdx.x];
     __syncthreads();
-    if (k >= K) return;
+    __shared__ T line[THREADS / 32][2][GROUP];                           // rows that no wide store fits go out element by element, side by side
+    T(*mine)[GROUP] = line[threadIdx.x / 32];
+    const int lane = threadIdx.x & 31;
 #pragma unroll
     for (int i = 0; i < AT_ONCE; ++i) {
         const int r = i * ROWS + first;
-        if (r >= here) break;
-        const float s = scale_value(sc[scale_place(r) + c / BLOCK]);
+        if (i * ROWS >= here) break;
+        const float s = r < here ? scale_value(sc[scale_place(r) + c / BLOCK]) : 0.f;
         float v[8];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -99,11 +110,18 @@ __global__ void __launch_bounds__(THREADS) dequantise_kernel(const uint8_t* __re
             v[2 * j] = e.x * s;
             v[2 * j + 1] = e.y * s;
         }
-        T* o = out + (row0 + r) * (size_t)K + k;
         if (K % 8 == 0) {
-            store8(o, v);
+            if (r < here && k < K) store8(out + (row0 + r) * (size_t)K + k, v);
         } else {
-            for (int j = 0; j < 8 && k + j < K; ++j) o[j] = from_float<T>(v[j]);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) mine[lane / 16][c + j] = from_float<T>(v[j]);
+            __syncwarp();
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int at = lane + 32 * (j & 3), row = r - lane / 16 + j / 4;
+                if (row < here && g * GROUP + at < K) out[(row0 + row) * (size_t)K + g * GROUP + at] = mine[j / 4][at];
+            }
+            __syncwarp();
         }
     }
 }
