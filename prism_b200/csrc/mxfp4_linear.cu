@@ -12,7 +12,7 @@
 //                most 2^-22 of it.  Up to 64 tokens hi and lo are columns of one instruction, added at the end (W is
 //                then read from shared memory once); for tiles of 128 tokens two instructions add to the same sums.
 //
-// Up to 32 tokens it is one kernel, whose CTAs each bring the parts of x that they meet to terms or codes on the way.  For more, a
+// Up to 16 tokens it is one kernel, whose CTAs each bring the parts of x that they meet to terms or codes on the way.  For more, a
 // first kernel does that once (a thread 8 values), in the workspace of the call, and clears its counters.  The product is persistent, a CTA an SM: warps 0 and 2 issue TMA loads into a ring of stages (W: for 16 bits 128 codes a row, which
 // TMA spreads to a byte each, for 4 bits 256; x), warp 1 the scale copies and the products, the warps from 4 on take the sums
 // out.
@@ -113,9 +113,19 @@ template <bool A16_, int TT_, int W_, int GS_, bool FUSED_> struct Cfg {
     static constexpr int EPI_WARPS = 4 * W, FIRST_X = 4 + EPI_WARPS, X_WARPS = 8, TEAMS = 2;       // teams of X_WARPS take the stages in turn
     static constexpr int THREADS = 32 * (4 + EPI_WARPS + (FUSED ? TEAMS * X_WARPS : 0));
     static constexpr size_t SMEM = (size_t)STAGES * (STAGE + SF) + 1024 + 512;
-    static_assert(COLS_USED <= 512 && STAGES >= 3 && (A16 || GS % 2 == 0) && (!FUSED || TT <= 32) && (!FUSED || GS * TT / 2 % X_WARPS == 0), "tensor memory, shared memory or form");
+    static_assert(COLS_USED <= 512 && STAGES >= 3 && (A16 || GS % 2 == 0) && (!FUSED || TT <= 16) && (!FUSED || GS * TT / 2 % X_WARPS == 0), "tensor memory, shared memory or form");
 };
 
+// 8 or 16 columns of a warp's lanes, without the wait
+__device__ __forceinline__ void tmem_get(uint32_t (&r)[8], uint32_t taddr) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]) : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_get(uint32_t (&r)[16], uint32_t taddr) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+                   "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]) : "r"(taddr));
+}
 // Instruction descriptor: element kinds (mxf8f6f4: A E2M1 = 5, B E4M3 = 0; mxf4: E2M1 = 1 on both sides), N / 8, scales E8M0,
 // M / 128; `id`: which byte of a scale column the instruction begins at.
 template <typename C> __device__ __forceinline__ constexpr uint32_t idesc_of(int id) {
@@ -374,24 +384,24 @@ product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
                 }
             };
             float* mine = p.part + (((size_t)cta * 2 + p.split.place(cta, u)) * W + w) * (TT * 128) + row;
+            constexpr int TAKE = C::FUSED ? 8 : 16;
 #pragma unroll 1
-            for (int t0 = 0; t0 < tokens; t0 += 8) {
-                float v[8];
-                {
-                    uint32_t r[8], l[8];
-                    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
-                                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]) : "r"(d + t0));
-                    if (C::SIDE)
-                        asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
-                                     : "=r"(l[0]), "=r"(l[1]), "=r"(l[2]), "=r"(l[3]), "=r"(l[4]), "=r"(l[5]), "=r"(l[6]), "=r"(l[7]) : "r"(d + TT + t0));
-                    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+            for (int t0 = 0; t0 < tokens; t0 += TAKE) {
+                uint32_t r[TAKE], l[TAKE];
+                tmem_get(r, d + t0);
+                if (C::SIDE) tmem_get(l, d + TT + t0);
+                asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                float v[TAKE];
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(r[j]) + (C::SIDE ? __uint_as_float(l[j]) : 0.f);
+                for (int j = 0; j < TAKE; ++j) {
+                    asm volatile("" : "+r"(r[j]));                       // not before the wait
+                    if (C::SIDE) asm volatile("" : "+r"(l[j]));
+                    v[j] = __uint_as_float(r[j]) + (C::SIDE ? __uint_as_float(l[j]) : 0.f);
                 }
                 if (whole) store(t0, v);
                 else
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) mine[(t0 + j) * 128] = v[j];
+                    for (int j = 0; j < TAKE; ++j) mine[(t0 + j) * 128] = v[j];
             }
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             __syncwarp();
@@ -406,24 +416,24 @@ product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
             if (C::FUSED && threadIdx.x == 128) p.counters[u] = 0;        // as the next launch expects it
             __threadfence();
             // one CTA's share after another's, the loads of eight of them at once
-            constexpr int SHARES = 8;
+            constexpr int SHARES = 8, JOIN = C::FUSED ? 4 : 8;          // as many registers as there are
 #pragma unroll 1
-            for (int t0 = 0; t0 < tokens; t0 += 8) {
-                float v[8] = {};
+            for (int t0 = 0; t0 < tokens; t0 += JOIN) {
+                float v[JOIN] = {};
 #pragma unroll 1
                 for (int c = c0; c <= c1; c += SHARES) {
-                    float part[SHARES][8];
+                    float part[SHARES][JOIN];
 #pragma unroll
                     for (int k = 0; k < SHARES; ++k) {
                         const int from_cta = min(c + k, c1);
                         const float* from = p.part + (((size_t)from_cta * 2 + p.split.place(from_cta, u)) * W + w) * (TT * 128) + row + t0 * 128;
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) part[k][j] = __ldcg(from + j * 128);
+                        for (int j = 0; j < JOIN; ++j) part[k][j] = __ldcg(from + j * 128);
                     }
 #pragma unroll
                     for (int k = 0; k < SHARES; ++k)
 #pragma unroll
-                        for (int j = 0; j < 8; ++j)
+                        for (int j = 0; j < JOIN; ++j)
                             if (c + k <= c1) v[j] += part[k][j];
                 }
                 store(t0, v);
@@ -449,20 +459,20 @@ struct Plan {
     bool fused;
     long long units, codes, scales, parts, counters, bytes;       // bytes from the workspace's start
 };
-// Up to 32 tokens go through the fused form of their size; for more, tiles of 32 to 128 tokens by one or two of W.  What is chosen, tile
+// Up to 16 tokens go through the fused form of their size; for more, tiles of 32 to 128 tokens by one or two of W.  What is chosen, tile
 // and CTAs that share a unit's K, takes least by this estimate (us): blocks of the busiest CTA times a block's time (W and x from
 // memory, or the products), and where K is shared 2 for handing over and the bytes of the shares at 100 KB a us.  Measured: 159 tokens
 // x 777 x 4,407 dealt to all SMs in tiles of 128 x 256 173 us, of which 110 joining; ...
 inline Plan plan_for(int M, int N, int K, int act_bits) {
     struct Form { int tt, w; float block16, block4; };
-    static const Form few[] = {{8, 1, .40f, 0.f}, {16, 1, .50f, .40f}, {32, 2, .45f, .45f}};
+    static const Form few[] = {{8, 1, .40f, 0.f}, {16, 1, .50f, .40f}};
     static const Form many[] = {{32, 1, .26f, .38f}, {64, 1, .30f, .40f}, {64, 2, .48f, .48f}, {128, 2, .72f, .55f}};
     Plan best;
     float best_us = 1e30f;
     const bool a16 = act_bits == 16;
     const int sms = sm_count();
-    const bool fused = M <= 32 && N <= MOST_COUNTERS * 128LL;       // as many tiles as the fused form has counters for
-    const Form* forms = fused ? &few[M <= 8 && a16 ? 0 : M <= 16 ? 1 : 2] : many;
+    const bool fused = M <= 16 && N <= MOST_COUNTERS * 128LL;       // as many tiles as the fused form has counters for
+    const Form* forms = fused ? &few[M <= 8 && a16 ? 0 : 1] : many;
     for (int i = 0; i < (fused ? 1 : 4); ++i) {
         Plan q;
         q.tt = forms[i].tt;
@@ -552,14 +562,8 @@ PRISM_EXPORT int prism_mxfp4_linear(const void* x, long long ldx, const void* co
     p.M = M, p.N = N, p.groups = q.groups, p.mtiles = q.mtiles, p.ntiles = q.ntiles;
     p.bias_bf16 = bias_dtype == PRISM_DTYPE_BF16, p.out_bf16 = out_dtype == PRISM_DTYPE_BF16;
     if (q.fused) {
-        if (a16) {
-            switch (q.tt) {
-                case 8: return run_product<Cfg<true, 8, 1, 2, true>>(mw, mw, p, stream);
-                case 16: return run_product<Cfg<true, 16, 1, 2, true>>(mw, mw, p, stream);
-                default: return run_product<Cfg<true, 32, 2, 1, true>>(mw, mw, p, stream);
-            }
-        }
-        return q.tt == 16 ? run_product<Cfg<false, 16, 1, 2, true>>(mw, mw, p, stream) : run_product<Cfg<false, 32, 2, 2, true>>(mw, mw, p, stream);
+        if (!a16) return run_product<Cfg<false, 16, 1, 2, true>>(mw, mw, p, stream);
+        return q.tt == 8 ? run_product<Cfg<true, 8, 1, 2, true>>(mw, mw, p, stream) : run_product<Cfg<true, 16, 1, 2, true>>(mw, mw, p, stream);
     }
     const int xr = a16 ? 2 * q.tt : q.tt;
     rc = a16 ? byte_map(&mx, base + q.codes, (long long)q.mtiles * xr, (long long)q.groups * GROUP, xr, false)
