@@ -30,7 +30,7 @@ namespace mx {
 // ---- x to terms or codes ------------------------------------------------------------------------------------------------
 
 // act 16: terms uint8 [token tile][2 tt][Kp], a tile's hi rows, then its lo rows; scales [token tile][groups][atoms][512],
-// the tiles of 128 such rows.  act 4: codes as in mxfp4.cuh, scales [token tile][groups][512].  Rows that have no token are left as
+// the tiles of 128 such rows.  act 4: codes as in mxfp4.cuh, scales [token tile][groups][atoms][512].  Rows that have no token are left as
 // they are.
 template <bool A16>
 __global__ void __launch_bounds__(256) prepare_kernel(const __nv_bfloat16* __restrict__ x_in, long long ldx, int M, int K, int groups, int wide,
@@ -81,14 +81,17 @@ __global__ void __launch_bounds__(256) prepare_kernel(const __nv_bfloat16* __res
 #pragma unroll
                 for (int j = 0; j < 4; ++j) word |= pack2(v[2 * j] * inv, v[2 * j + 1] * inv) << (8 * j);
             *reinterpret_cast<uint32_t*>(codes + (size_t)r * (groups * (GROUP / 2)) + c / 2) = word;
-            const int tile = r / tt, t = r - tile * tt;
+            const int tile = r / tt, t = r - tile * tt, atoms = (tt + 127) / 128;
             if ((threadIdx.x & 3) == 0)
-                scales[((size_t)tile * groups + c / GROUP) * TILE_BYTES + (t & 31) * 16 + t / 32 * 4 + c % GROUP / BLOCK] = (uint8_t)byte;
+                scales[(((size_t)tile * groups + c / GROUP) * atoms + t / 128) * TILE_BYTES + (t & 31) * 16 + (t & 127) / 32 * 4 + c % GROUP / BLOCK] =
+                    (uint8_t)byte;
         }
     }
 }
 
 // ---- the product --------------------------------------------------------------------------------------------------------
+
+constexpr int STAGE_OUT = 16 * 128 * 2;        // bytes of sixteen tokens' results of 128 features in bfloat16
 
 // FUSED: the product brings x to terms itself (no first kernel)
 template <bool A16_, int TT_, int W_, int GS_, bool FUSED_> struct Cfg {
@@ -112,7 +115,7 @@ template <bool A16_, int TT_, int W_, int GS_, bool FUSED_> struct Cfg {
     static constexpr int COLS = COLS_USED <= 64 ? 64 : COLS_USED <= 128 ? 128 : COLS_USED <= 256 ? 256 : 512;
     static constexpr int EPI_WARPS = 4 * W, FIRST_X = 4 + EPI_WARPS, X_WARPS = 8, TEAMS = 2;       // teams of X_WARPS take the stages in turn
     static constexpr int THREADS = 32 * (4 + EPI_WARPS + (FUSED ? TEAMS * X_WARPS : 0));
-    static constexpr size_t SMEM = (size_t)STAGES * (STAGE + SF) + 1024 + 512;
+    static constexpr size_t SMEM = (size_t)STAGES * (STAGE + SF) + 1024 + 512 + W * STAGE_OUT;
     static_assert(COLS_USED <= 512 && STAGES >= 3 && (A16 || GS % 2 == 0) && (!FUSED || TT <= 16) && (!FUSED || GS * TT / 2 % X_WARPS == 0), "tensor memory, shared memory or form");
 };
 
@@ -143,8 +146,37 @@ struct Product {
     int *counters, *err;
     long long ldy;
     Split split;
-    int M, N, groups, mtiles, ntiles, bias_bf16, out_bf16;
+    int M, N, groups, mtiles, ntiles, bias_bf16, out_bf16, wide_out;       // wide_out: rows of the result in bfloat16 at multiples of 16 bytes
 };
+
+// Sixteen tokens' results of 128 features, a feature a thread of four warps, to memory: as bfloat16 through `stage` (4 KB), so that
+// 16 threads store a token's 256 bytes 16 bytes each.  Stores of 2 bytes a lane took 16 cycles a warp: 11,000 cycles a tile of 256 x 128
+// beside 166,000 of products in 12 tiles.  `bar`: a barrier of the four warps.
+__device__ __forceinline__ void store_sixteen(const Product& p, unsigned char* stage, int bar, int m0, int t0, int tokens, int f0, int row, const float (&v)[16]) {
+    if (p.wide_out) {
+        __nv_bfloat16* to = reinterpret_cast<__nv_bfloat16*>(stage) + row;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) to[j * 128] = __float2bfloat16_rn(v[j]);
+        asm volatile("bar.sync %0, 128;" ::"r"(bar) : "memory");
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int t = h * 8 + row / 16, f = f0 + row % 16 * 8;
+            if (t0 + t < tokens && f < p.N)
+                *reinterpret_cast<uint4*>(reinterpret_cast<__nv_bfloat16*>(p.y) + (long long)(m0 + t0 + t) * p.ldy + f) =
+                    *reinterpret_cast<const uint4*>(stage + t * 256 + row % 16 * 16);
+        }
+        asm volatile("bar.sync %0, 128;" ::"r"(bar) : "memory");
+        return;
+    }
+    if (f0 + row >= p.N) return;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+        if (t0 + j >= tokens) return;
+        const long long at = (long long)(m0 + t0 + j) * p.ldy + f0 + row;
+        if (p.out_bf16) reinterpret_cast<__nv_bfloat16*>(p.y)[at] = __float2bfloat16_rn(v[j]);
+        else reinterpret_cast<float*>(p.y)[at] = v[j];
+    }
+}
 
 template <typename C>
 __global__ void __launch_bounds__(C::THREADS, 1)
@@ -156,6 +188,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
     uint64_t* full = reinterpret_cast<uint64_t*>(sf + STAGES * C::SF);
     uint64_t *empty = full + STAGES, *acc_full = empty + STAGES, *acc_empty = acc_full + C::BUFS;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + C::BUFS);
+    unsigned char* staging = reinterpret_cast<unsigned char*>(full) + 512;
     __shared__ int abort_flag, is_last, gone;
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, cta = blockIdx.x;
@@ -373,39 +406,76 @@ product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
             const uint32_t d = tmem + ((uint32_t)(q * 32) << 16) + (buf * W + w) * C::NCOL;
             const bool whole = k0 == 0 && k1 == kb;
             const float bias = p.bias != nullptr && f < p.N ? load_param(p.bias, p.bias_bf16, f) : 0.f;
-            auto store = [&](int t0, const auto& v) {
-                if (f >= p.N) return;
+            auto store = [&](int t0, auto& v) {
+                constexpr int count = (int)(sizeof(v) / sizeof(float));
 #pragma unroll
-                for (int j = 0; j < (int)(sizeof(v) / sizeof(float)); ++j) {
-                    if (t0 + j >= tokens) return;
-                    const long long at = (long long)(m0 + t0 + j) * p.ldy + f;
-                    if (p.out_bf16) reinterpret_cast<__nv_bfloat16*>(p.y)[at] = __float2bfloat16_rn(v[j] + bias);
-                    else reinterpret_cast<float*>(p.y)[at] = v[j] + bias;
+                for (int j = 0; j < count; ++j) v[j] += bias;
+                if constexpr (count == 16) {
+                    store_sixteen(p, staging + w * STAGE_OUT, 2 + w, m0, t0, tokens, f - row, row, v);
+                } else {
+                    if (f >= p.N) return;
+#pragma unroll
+                    for (int j = 0; j < count; ++j) {
+                        if (t0 + j >= tokens) return;
+                        const long long at = (long long)(m0 + t0 + j) * p.ldy + f;
+                        if (p.out_bf16) reinterpret_cast<__nv_bfloat16*>(p.y)[at] = __float2bfloat16_rn(v[j]);
+                        else reinterpret_cast<float*>(p.y)[at] = v[j];
+                    }
                 }
             };
             float* mine = p.part + (((size_t)cta * 2 + p.split.place(cta, u)) * W + w) * (TT * 128) + row;
-            constexpr int TAKE = C::FUSED ? 8 : 16;
-#pragma unroll 1
-            for (int t0 = 0; t0 < tokens; t0 += TAKE) {
-                uint32_t r[TAKE], l[TAKE];
-                tmem_get(r, d + t0);
-                if (C::SIDE) tmem_get(l, d + TT + t0);
-                asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-                float v[TAKE];
+            auto release = [&]() {                                       // the sums are out: the next unit's may begin
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&acc_empty[buf]);
+            };
+            if constexpr (TT == 128) {
+                // one set of sums, and many: all into registers before the first is stored (2,048 tokens x (28,672 x 4,096) in 4
+                // bits 173 -> 152 us; tiles of 64 tokens, of fewer blocks each, lost by as much to the code that this takes)
+                uint32_t r[TT / 16][16];
 #pragma unroll
-                for (int j = 0; j < TAKE; ++j) {
-                    asm volatile("" : "+r"(r[j]));                       // not before the wait
-                    if (C::SIDE) asm volatile("" : "+r"(l[j]));
-                    v[j] = __uint_as_float(r[j]) + (C::SIDE ? __uint_as_float(l[j]) : 0.f);
+                for (int c = 0; c < TT / 16; ++c) {
+                    tmem_get(r[c], d + 16 * c);
                 }
-                if (whole) store(t0, v);
-                else
+                asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-                    for (int j = 0; j < TAKE; ++j) mine[(t0 + j) * 128] = v[j];
+                for (int c = 0; c < TT / 16; ++c)
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) asm volatile("" : "+r"(r[c][j]));       // not before the wait
+                release();
+#pragma unroll
+                for (int c = 0; c < TT / 16; ++c) {
+                    if (16 * c >= tokens) break;
+                    float v[16];
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(r[c][j]);
+                    if (whole) store(16 * c, v);
+                    else
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) mine[(16 * c + j) * 128] = v[j];
+                }
+            } else {
+                constexpr int TAKE = C::FUSED ? 8 : 16;
+#pragma unroll 1
+                for (int t0 = 0; t0 < tokens; t0 += TAKE) {
+                    uint32_t r[TAKE], l[TAKE];
+                    tmem_get(r, d + t0);
+                    if (C::SIDE) tmem_get(l, d + TT + t0);
+                    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                    float v[TAKE];
+#pragma unroll
+                    for (int j = 0; j < TAKE; ++j) {
+                        asm volatile("" : "+r"(r[j]));                   // not before the wait
+                        if (C::SIDE) asm volatile("" : "+r"(l[j]));
+                        v[j] = __uint_as_float(r[j]) + (C::SIDE ? __uint_as_float(l[j]) : 0.f);
+                    }
+                    if (whole) store(t0, v);
+                    else
+#pragma unroll
+                        for (int j = 0; j < TAKE; ++j) mine[(t0 + j) * 128] = v[j];
+                }
+                release();
             }
-            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&acc_empty[buf]);
             if (whole) continue;
             const int c0 = p.split.owner(u * kb), c1 = p.split.owner((u + 1) * kb - 1);
             __threadfence();
@@ -425,16 +495,15 @@ product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
                     float part[SHARES][JOIN];
 #pragma unroll
                     for (int k = 0; k < SHARES; ++k) {
-                        const int from_cta = min(c + k, c1);
-                        const float* from = p.part + (((size_t)from_cta * 2 + p.split.place(from_cta, u)) * W + w) * (TT * 128) + row + t0 * 128;
+                        const bool there = c + k <= c1;
+                        const float* from = p.part + (((size_t)(c + k) * 2 + p.split.place(c + k, u)) * W + w) * (TT * 128) + row + t0 * 128;
 #pragma unroll
-                        for (int j = 0; j < JOIN; ++j) part[k][j] = __ldcg(from + j * 128);
+                        for (int j = 0; j < JOIN; ++j) part[k][j] = there ? __ldcg(from + j * 128) : 0.f;
                     }
 #pragma unroll
                     for (int k = 0; k < SHARES; ++k)
 #pragma unroll
-                        for (int j = 0; j < JOIN; ++j)
-                            if (c + k <= c1) v[j] += part[k][j];
+                        for (int j = 0; j < JOIN; ++j) v[j] += part[k][j];
                 }
                 store(t0, v);
             }
@@ -466,7 +535,7 @@ struct Plan {
 inline Plan plan_for(int M, int N, int K, int act_bits) {
     struct Form { int tt, w; float block16, block4; };
     static const Form few[] = {{8, 1, .40f, 0.f}, {16, 1, .50f, .40f}};
-    static const Form many[] = {{32, 1, .26f, .38f}, {64, 1, .30f, .40f}, {64, 2, .48f, .48f}, {128, 2, .72f, .55f}};
+    static const Form many[] = {{32, 1, .26f, .30f}, {64, 1, .32f, .38f}, {64, 2, .58f, .63f}, {128, 2, 1.0f, .80f}};
     Plan best;
     float best_us = 1e30f;
     const bool a16 = act_bits == 16;
@@ -493,7 +562,7 @@ inline Plan plan_for(int M, int N, int K, int act_bits) {
             if (q.P > total) q.P = (int)total;
             const long long each = (total + q.P - 1) / q.P;
             const int shares = each >= q.kb && total % q.P == 0 ? 1 : (int)((q.kb + each - 1) / each) + (want > sms);
-            const float us = each * block + (shares > 1 ? 2.f + shares * share : 0.f);
+            const float us = each * block + (shares > 1 ? 2 * (1.5f + (1 + shares) * share) : 0.f);
             if (us < best_us) { best_us = us; best = q; }
             if (want >= sms) break;
         }
@@ -561,6 +630,7 @@ PRISM_EXPORT int prism_mxfp4_linear(const void* x, long long ldx, const void* co
     p.split = Split((int)(q.units * q.kb), q.P, q.kb);
     p.M = M, p.N = N, p.groups = q.groups, p.mtiles = q.mtiles, p.ntiles = q.ntiles;
     p.bias_bf16 = bias_dtype == PRISM_DTYPE_BF16, p.out_bf16 = out_dtype == PRISM_DTYPE_BF16;
+    p.wide_out = p.out_bf16 && N % 8 == 0 && ldy % 8 == 0 && ((uintptr_t)y & 15) == 0;
     if (q.fused) {
         if (!a16) return run_product<Cfg<false, 16, 1, 2, true>>(mw, mw, p, stream);
         return q.tt == 8 ? run_product<Cfg<true, 8, 1, 2, true>>(mw, mw, p, stream) : run_product<Cfg<true, 16, 1, 2, true>>(mw, mw, p, stream);

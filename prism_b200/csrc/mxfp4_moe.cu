@@ -617,14 +617,14 @@ moe_kernel(const __grid_constant__ CUtensorMap map_gate, const __grid_constant__
                             float gp[SHARES][2], up[SHARES][2];
 #pragma unroll
                             for (int k = 0; k < SHARES; ++k) {
-                                const int cc = min(c + k, c1);
-                                const float* from = p.part1 + (size_t)(cc * 2 + s1.place(cc, unit)) * (2 * TT * 128) + r * 128 + row;
-                                gp[k][0] = __ldcg(from), gp[k][1] = __ldcg(from + 128);
-                                up[k][0] = __ldcg(from + TT * 128), up[k][1] = __ldcg(from + TT * 128 + 128);
+                                const bool there = c + k <= c1;
+                                const float* from = p.part1 + (size_t)((c + k) * 2 + s1.place(c + k, unit)) * (2 * TT * 128) + r * 128 + row;
+                                gp[k][0] = there ? __ldcg(from) : 0.f, gp[k][1] = there ? __ldcg(from + 128) : 0.f;
+                                up[k][0] = there ? __ldcg(from + TT * 128) : 0.f, up[k][1] = there ? __ldcg(from + TT * 128 + 128) : 0.f;
                             }
 #pragma unroll
                             for (int k = 0; k < SHARES; ++k)
-                                if (c + k <= c1) g[0] += gp[k][0], g[1] += gp[k][1], u[0] += up[k][0], u[1] += up[k][1];
+                                g[0] += gp[k][0], g[1] += gp[k][1], u[0] += up[k][0], u[1] += up[k][1];
                         }
 #pragma unroll 1
                         for (int j = 0; j < 2 && r + j < count; ++j) {
@@ -681,16 +681,16 @@ moe_kernel(const __grid_constant__ CUtensorMap map_gate, const __grid_constant__
                         float part[SHARES][4];
 #pragma unroll
                         for (int k = 0; k < SHARES; ++k) {
-                            const int cc = min(c + k, c1);
-                            const float* from = p.part2 + ((size_t)(cc * 2 + s2.place(cc, unit)) * 2 + half) * (TT * 128) + r * 128 + row;
+                            const bool there = c + k <= c1;
+                            const float* from = p.part2 + ((size_t)((c + k) * 2 + s2.place(c + k, unit)) * 2 + half) * (TT * 128) + r * 128 + row;
 #pragma unroll
-                            for (int j = 0; j < 4; ++j) part[k][j] = __ldcg(from + j * 128);
+                            for (int j = 0; j < 4; ++j) part[k][j] = there ? __ldcg(from + j * 128) : 0.f;
                         }
 #pragma unroll
                         for (int k = 0; k < SHARES; ++k)
 #pragma unroll
                             for (int j = 0; j < 4; ++j)
-                                if (c + k <= c1) v[j] += part[k][j];
+                                v[j] += part[k][j];
                     }
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
