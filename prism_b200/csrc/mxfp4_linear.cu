@@ -13,7 +13,7 @@
 //                then read from shared memory once); for tiles of 128 tokens two instructions add to the same sums.
 //
 // Up to 16 tokens it is one kernel, whose CTAs each bring the parts of x that they meet to terms or codes on the way.  For more, a
-// first kernel does that once (a thread 8 values), in the workspace of the call, and clears its counters.  The product is persistent, a CTA an SM: warps 0 and 2 issue TMA loads into a ring of stages (W: for 16 bits 128 codes a row, which
+// first kernel does that once, in the workspace of the call, and clears its counters.  The product is persistent, a CTA an SM: warps 0 and 2 issue TMA loads into a ring of stages (W: for 16 bits 128 codes a row, which
 // TMA spreads to a byte each, for 4 bits 256; x), warp 1 the scale copies and the products, the warps from 4 on take the sums
 // out.
 // All of the product's blocks - (tile of W rows, tile of tokens, stage of K) - are dealt to the CTAs evenly as one long
@@ -30,8 +30,8 @@ namespace mx {
 // ---- x to terms or codes ------------------------------------------------------------------------------------------------
 
 // act 16: terms uint8 [token tile][2 tt][Kp], a tile's hi rows, then its lo rows; scales [token tile][groups][atoms][512],
-// the tiles of 128 such rows.  act 4: codes as in mxfp4.cuh, scales [token tile][groups][atoms][512].  Rows that have no token are left as
-// they are.
+// the tiles of 128 such rows.  act 4: codes as in mxfp4.cuh, scales [token tile][groups][512].  Rows that have no token are left as
+// they are.  A CTA has a group of 128 columns of 32 rows: 16 threads share a row, each has 8 values of two.
 template <bool A16>
 __global__ void __launch_bounds__(256) prepare_kernel(const __nv_bfloat16* __restrict__ x_in, long long ldx, int M, int K, int groups, int wide,
                                                       int tt, uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, int* __restrict__ counters,
@@ -39,52 +39,41 @@ __global__ void __launch_bounds__(256) prepare_kernel(const __nv_bfloat16* __res
     pdl_wait();            // before the trigger: the product, which reads W at once, starts behind all that came before this kernel
     pdl_trigger();
     const __nv_bfloat16* x = pdl_fresh(x_in);
-    const int per_row = groups * (GROUP / 8);
-    const long long total = (long long)M * per_row;
-    const long long first = (long long)blockIdx.x * blockDim.x + threadIdx.x;
-    for (long long i = first; i < ncounters; i += (long long)gridDim.x * blockDim.x) counters[i] = 0;
-    for (long long i = first; i < total; i += (long long)gridDim.x * blockDim.x) {
-        const int r = (int)(i / per_row), c = (int)(i - (long long)r * per_row) * 8;
-        const __nv_bfloat16* p = x + (long long)r * ldx + c;
-        float v[8];
-        if (wide && c + 8 <= K) {
-            load8(p, v);
-        } else {
+    const int g = blockIdx.x, c = (threadIdx.x & 15) * 8, k = g * GROUP + c, first = blockIdx.y * 32 + (threadIdx.x >> 4);
+    const int cta = blockIdx.y * gridDim.x + blockIdx.x;
+    for (int i = cta * 256 + threadIdx.x; i < ncounters; i += gridDim.x * gridDim.y * 256) counters[i] = 0;
+    uint4 raw[2];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = c + j < K ? to_float(p[j]) : 0.f;
-        }
-        uint32_t most = 0;
+    for (int h = 0; h < 2; ++h) {
+        const int r = first + 16 * h;
+        raw[h] = r < M ? row8(x + (long long)r * ldx, k, K, wide) : make_uint4(0, 0, 0, 0);
+    }
 #pragma unroll
-        for (int j = 0; j < 8; ++j) most = max(most, __float_as_uint(v[j]) & 0x7fffffffu);
-        const uint32_t four = 0xfu << (threadIdx.x & 28);
-        most = max(most, __shfl_xor_sync(four, most, 1));
-        most = max(most, __shfl_xor_sync(four, most, 2));
+    for (int h = 0; h < 2; ++h) {
+        const int r = first + 16 * h, tile = r / tt, t = r - tile * tt;
+        uint32_t most = magnitude(raw[h]);
+        most = __vmaxu2(most, __shfl_xor_sync(0xffffffffu, most, 1));
+        most = __vmaxu2(most, __shfl_xor_sync(0xffffffffu, most, 2));
+        most = max(most << 16, most & 0xffff0000u);
+        if (r >= M) continue;
         if (A16) {
             const int byte = term_byte(most), lines = 2 * tt, atoms = (lines + 127) / 128;
             uint32_t hi[2], lo[2];
-            terms_of<8>(v, byte, hi, lo);
-            const int tile = r / tt, t = r - tile * tt;
-            uint8_t* at = codes + ((size_t)tile * lines + t) * ((size_t)groups * GROUP) + c;
+            terms_of_bf16(raw[h], byte, hi, lo);
+            uint8_t* at = codes + ((size_t)tile * lines + t) * ((size_t)groups * GROUP) + k;
             *reinterpret_cast<uint2*>(at) = make_uint2(hi[0], hi[1]);
             *reinterpret_cast<uint2*>(at + (size_t)tt * groups * GROUP) = make_uint2(lo[0], lo[1]);
             if ((threadIdx.x & 3) == 0) {
-                uint8_t* s = scales + ((size_t)tile * groups + c / GROUP) * (atoms * TILE_BYTES) + c % GROUP / BLOCK;
+                uint8_t* s = scales + ((size_t)tile * groups + g) * (atoms * TILE_BYTES) + c / BLOCK;
                 const int u = t + tt;
                 s[t / 128 * TILE_BYTES + (t & 31) * 16 + (t & 127) / 32 * 4] = (uint8_t)byte;
                 s[u / 128 * TILE_BYTES + (u & 31) * 16 + (u & 127) / 32 * 4] = low_byte(byte);
             }
         } else {
             const int byte = scale_byte(most);
-            const float inv = scale_inverse(byte);
-            uint32_t word = 0;
-            if (byte != 255)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) word |= pack2(v[2 * j] * inv, v[2 * j + 1] * inv) << (8 * j);
-            *reinterpret_cast<uint32_t*>(codes + (size_t)r * (groups * (GROUP / 2)) + c / 2) = word;
-            const int tile = r / tt, t = r - tile * tt, atoms = (tt + 127) / 128;
+            *reinterpret_cast<uint32_t*>(codes + (size_t)r * (groups * (GROUP / 2)) + k / 2) = codes_of_bf16(raw[h], byte);
             if ((threadIdx.x & 3) == 0)
-                scales[(((size_t)tile * groups + c / GROUP) * atoms + t / 128) * TILE_BYTES + (t & 31) * 16 + (t & 127) / 32 * 4 + c % GROUP / BLOCK] =
-                    (uint8_t)byte;
+                scales[((size_t)tile * groups + g) * TILE_BYTES + (t & 31) * 16 + t / 32 * 4 + c / BLOCK] = (uint8_t)byte;
         }
     }
 }
@@ -267,15 +256,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
 #pragma unroll
             for (int j = 0; j < ITEMS; ++j) {
                 const int item = first + C::X_WARPS * j, t = item % (TT / 2) * 2 + (lane >> 4), at = (kl * C::GS + item / (TT / 2)) * GROUP + c;
-                const __nv_bfloat16* from = x + (long long)t * p.ldx + at;
-                if (p.wide && t < p.M && at + 8 <= p.K) {
-                    to[j] = *reinterpret_cast<const uint4*>(from);
-                } else {
-                    __nv_bfloat16 v[8];
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) v[e] = t < p.M && at + e < p.K ? from[e] : __nv_bfloat16(0.f);
-                    to[j] = *reinterpret_cast<const uint4*>(v);
-                }
+                to[j] = t < p.M ? row8(x + (long long)t * p.ldx, at, p.K, p.wide) : make_uint4(0, 0, 0, 0);
             }
             il += C::TEAMS;
             kl = (kl + C::TEAMS) % kb;
@@ -314,13 +295,8 @@ product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
                         }
                     } else {
                         const int byte = scale_byte(most);
-                        const float inv = byte == 255 ? 0.f : scale_inverse(byte);
-                        const uint32_t r[4] = {raw[h][j].x, raw[h][j].y, raw[h][j].z, raw[h][j].w};
-                        uint32_t word = 0;
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) word |= pack2(__uint_as_float(r[e] << 16) * inv, __uint_as_float(r[e] & 0xffff0000u) * inv) << (8 * e);
                         *reinterpret_cast<uint32_t*>(xt + g / 2 * (C::XR * 128) + t * 128 + ((((g & 1) * 4 + (lane & 15) / 4) ^ (t & 7)) << 4) +
-                                                     (lane & 3) * 4) = byte == 255 ? 0 : word;
+                                                     (lane & 3) * 4) = codes_of_bf16(raw[h][j], byte);
                         if ((lane & 3) == 0) sc[(t & 31) * 16 + t / 32 * 4] = (uint8_t)byte;
                     }
                 }
@@ -639,10 +615,9 @@ PRISM_EXPORT int prism_mxfp4_linear(const void* x, long long ldx, const void* co
     rc = a16 ? byte_map(&mx, base + q.codes, (long long)q.mtiles * xr, (long long)q.groups * GROUP, xr, false)
              : byte_map(&mx, base + q.codes, M, (long long)q.groups * (GROUP / 2), xr, false);
     if (rc) return rc;
-    const long long threads = (long long)M * q.groups * 16, most = threads > q.units ? threads : q.units;
-    const int blocks = (int)((most + 255) / 256 < 148 * 8 ? (most + 255) / 256 : 148 * 8);
-    rc = (int)launch_kernel(a16 ? prepare_kernel<true> : prepare_kernel<false>, dim3(blocks), dim3(256), 0, stream, p.x, ldx, M, K, q.groups, p.wide,
-                            q.tt, base + q.codes, base + q.scales, p.counters, (int)q.units);
+    if ((M + 31) / 32 > 65535) return (int)cudaErrorInvalidValue;
+    rc = (int)launch_kernel(a16 ? prepare_kernel<true> : prepare_kernel<false>, dim3(q.groups, (M + 31) / 32), dim3(256), 0, stream, p.x, ldx, M, K,
+                            q.groups, p.wide, q.tt, base + q.codes, base + q.scales, p.counters, (int)q.units);
     if (rc) return rc;
     const int form = q.tt * 10 + q.w;
     if (a16) {

@@ -35,26 +35,15 @@ __device__ __forceinline__ void unpack_e4m3(uint32_t p, float& lo, float& hi) {
 
 __device__ __forceinline__ int term_byte(uint32_t most) { return most >= 0x7f800000u ? 255 : max((int)(most >> 23) - 7, 5); }
 __device__ __forceinline__ uint8_t low_byte(int byte) { return (uint8_t)(byte == 255 ? 255 : byte - 5); }
-// N values (N a multiple of 4) as N bytes of high and N of low terms
-template <int N> __device__ __forceinline__ void terms_of(const float (&v)[N], int byte, uint32_t (&hi)[N / 4], uint32_t (&lo)[N / 4]) {
-    const float f = byte == 255 ? 0.f : __uint_as_float((uint32_t)(254 - byte) << 23);
-#pragma unroll
-    for (int i = 0; i < N / 4; ++i) {
-        hi[i] = lo[i] = 0;
-        if (byte == 255) continue;
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const float a = v[4 * i + 2 * j] * f, b = v[4 * i + 2 * j + 1] * f;
-            const uint32_t h = pack_e4m3(a, b);
-            float ha, hb;
-            unpack_e4m3(h, ha, hb);
-            hi[i] |= h << (16 * j);
-            lo[i] |= pack_e4m3((a - ha) * 32.f, (b - hb) * 32.f) << (16 * j);
-        }
-    }
+// a value (of h's) as a byte of a high and one of a low term
+__device__ __forceinline__ void terms_of_one(float v, int byte, uint32_t& hi, uint32_t& lo) {
+    const float a = byte == 255 ? 0.f : v * __uint_as_float((uint32_t)(254 - byte) << 23);
+    float ha, none;
+    hi = pack_e4m3(a, 0.f);
+    unpack_e4m3(hi, ha, none);
+    lo = byte == 255 ? 0 : pack_e4m3((a - ha) * 32.f, 0.f);
 }
-
-// The same of eight bfloat16 values as they lie in memory, in half precision where two share an instruction (exact: a scaled
+// The terms of eight bfloat16 values as they lie in memory, in half precision where two share an instruction (exact: a scaled
 // value has 8 significant bits and is below 256; what half precision drops is below 2^-24, which no E4M3 term of it holds).
 __device__ __forceinline__ uint32_t magnitude(const uint4& raw) {       // the largest, as bfloat16 bits, in either half of the word
     const uint32_t m = 0x7fff7fffu;
@@ -79,6 +68,24 @@ __device__ __forceinline__ void terms_of_bf16(const uint4& raw, int byte, uint32
         hi[i] = byte == 255 ? 0 : h8[2 * i] | (uint32_t)h8[2 * i + 1] << 16;
         lo[i] = byte == 255 ? 0 : l8[2 * i] | (uint32_t)l8[2 * i + 1] << 16;
     }
+}
+
+// the same eight as 4-bit codes under their block's scale byte
+__device__ __forceinline__ uint32_t codes_of_bf16(const uint4& raw, int byte) {
+    const float inv = scale_inverse(byte);
+    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+    uint32_t word = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) word |= pack2(__uint_as_float(w[i] << 16) * inv, __uint_as_float(w[i] & 0xffff0000u) * inv) << (8 * i);
+    return byte == 255 ? 0 : word;
+}
+// eight of a row's values from column c, zero beyond K
+__device__ __forceinline__ uint4 row8(const __nv_bfloat16* row, int c, int K, int wide) {
+    if (wide && c + 8 <= K) return *reinterpret_cast<const uint4*>(row + c);
+    __nv_bfloat16 v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = c + j < K ? row[c + j] : __nv_bfloat16(0.f);
+    return *reinterpret_cast<const uint4*>(v);
 }
 
 // ---- pieces of the products -----------------------------------------------------------------------------------------------

@@ -102,14 +102,6 @@ __device__ __forceinline__ void tmem_one(uint32_t& v, uint32_t taddr) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(v) : "r"(taddr));
 }
 
-// eight of a row's values from column c, zero beyond K
-__device__ __forceinline__ uint4 row8(const __nv_bfloat16* row, int c, int K, int wide) {
-    if (wide && c + 8 <= K) return *reinterpret_cast<const uint4*>(row + c);
-    __nv_bfloat16 v[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = c + j < K ? row[c + j] : __nv_bfloat16(0.f);
-    return *reinterpret_cast<const uint4*>(v);
-}
 // Terms of eight values of a row (neighbouring threads have a block's others) to the rows `hi`, `lo` of a matrix of rows of
 // `pitch` bytes and to its scales; su, sl: the rows' numbers there.
 __device__ __forceinline__ void row_terms(const uint4& raw, int c, uint8_t* hi_row, uint8_t* lo_row, uint8_t* scales, int su, int sl) {
@@ -567,13 +559,13 @@ moe_kernel(const __grid_constant__ CUtensorMap map_gate, const __grid_constant__
                 auto hidden = [&](int r, float g, float u) {      // all lanes of a warp: a block of 32 of row r of the expert's h
                     const float w = q.weight[q.plane[first + r]];
                     if (p.scale_in) { g *= w; u *= w; }
-                    float h[4] = {f < p.F ? moe_glu(g, u, p.act, p.limit) * (p.scale_in ? 1.f : w) : 0.f, 0.f, 0.f, 0.f};
-                    const int byte = term_byte(__reduce_max_sync(0xffffffffu, __float_as_uint(h[0]) & 0x7fffffffu));
-                    uint32_t hi[1], lo[1];
-                    terms_of<4>(h, byte, hi, lo);
+                    const float h = f < p.F ? moe_glu(g, u, p.act, p.limit) * (p.scale_in ? 1.f : w) : 0.f;
+                    const int byte = term_byte(__reduce_max_sync(0xffffffffu, __float_as_uint(h) & 0x7fffffffu));
+                    uint32_t hi, lo;
+                    terms_of_one(h, byte, hi, lo);
                     uint8_t* to = p.h + (size_t)(q.hrow8[l] * 8 + r) * ((size_t)g2 * GROUP) + f;
-                    to[0] = (uint8_t)hi[0];
-                    to[(size_t)nt * g2 * GROUP] = (uint8_t)lo[0];
+                    to[0] = (uint8_t)hi;
+                    to[(size_t)nt * g2 * GROUP] = (uint8_t)lo;
                     if (lane == 0) {
                         uint8_t* s = p.hs + ((size_t)l * g2 + tile) * TILE_BYTES + quarter;
                         const int v = nt + r;
