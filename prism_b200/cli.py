@@ -41,6 +41,9 @@ def build_parser() -> argparse.ArgumentParser:
     p.add_argument("--max-num-seqs", type=int, default=64)
     p.add_argument("--max-seq-len", type=int, default=None)
     p.add_argument("--no-cuda-graph", action="store_true")
+    p.add_argument("--weight-format", default=None, choices=["mxfp4"], help="keep the layers' matrices in 4 bits")
+    p.add_argument("--act-bits", type=int, default=16, choices=[16, 4],
+                   help="with --weight-format: activations of the products as they are (16) or in 4 bits too")
     return p
 
 
@@ -70,7 +73,8 @@ def main(argv=None) -> int:
     ec = EngineConfig(gpu_id=args.gpu, kv_page_size=args.page_size, num_pages=args.num_pages,
                       kv_cache_budget_gb=args.kv_budget_gb, max_seq_len=args.max_seq_len,
                       use_cuda_graph=not args.no_cuda_graph, seed=args.sample_seed,
-                      scheduler=SchedulerConfig(args.max_batch_tokens, args.max_num_seqs, args.prefill_chunk))
+                      scheduler=SchedulerConfig(args.max_batch_tokens, args.max_num_seqs, args.prefill_chunk),
+                      weight_format=args.weight_format, act_bits=args.act_bits)
     t0 = time.perf_counter()
     if raw is not None:
         eng = Engine(None, ec, dtype=args.dtype, config=raw, random_seed=args.seed)

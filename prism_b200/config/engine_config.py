@@ -47,3 +47,9 @@ class EngineConfig:
     graph_batch_sizes: Sequence[int] = (1, 2, 4, 8, 16, 32, 64)
     seed: int = 0
     scheduler: SchedulerConfig = field(default_factory=SchedulerConfig)
+    weight_format: Optional[str] = None  # "mxfp4": the layers' matrices in microscaled 4-bit floating point
+    act_bits: int = 16                  # with it: products take activations as they are (16) or brought to 4 bits too
+
+    def __post_init__(self):
+        from ..weights.four_bit import check_weight_format
+        check_weight_format(self.weight_format, self.act_bits)

@@ -76,13 +76,14 @@ __global__ void __launch_bounds__(THREADS) quantise_kernel(const T* __restrict__
 
 template <typename T>
 __global__ void __launch_bounds__(THREADS) dequantise_kernel(const uint8_t* __restrict__ codes_in, const uint8_t* __restrict__ scales_in, int rows,
-                                                             int K, int groups, T* __restrict__ out) {
+                                                             int K, int groups, T* __restrict__ out, long long ldm) {
     __shared__ __align__(16) uint8_t sc[TILE_BYTES];
     pdl_wait();
     pdl_trigger();
     const int g = blockIdx.x, r0 = blockIdx.y * TILE_ROWS, c = (threadIdx.x & 15) * 8, k = g * GROUP + c, first = threadIdx.x >> 4;
     const size_t row0 = (size_t)blockIdx.z * rows + r0;
     const uint8_t* code = pdl_fresh(codes_in) + row0 * (groups * (size_t)(GROUP / 2)) + k / 2;
+    out += blockIdx.z * ldm + (long long)r0 * K;
     const int here = min(TILE_ROWS, rows - r0);
     uint32_t word[AT_ONCE];
     static_assert(ROWS * AT_ONCE == TILE_ROWS, "one round");
@@ -111,7 +112,7 @@ __global__ void __launch_bounds__(THREADS) dequantise_kernel(const uint8_t* __re
             v[2 * j + 1] = e.y * s;
         }
         if (K % 8 == 0) {
-            if (r < here && k < K) store8(out + (row0 + r) * (size_t)K + k, v);
+            if (r < here && k < K) store8(out + (size_t)r * K + k, v);
         } else {
 #pragma unroll
             for (int j = 0; j < 8; ++j) mine[lane / 16][c + j] = from_float<T>(v[j]);
@@ -119,7 +120,7 @@ __global__ void __launch_bounds__(THREADS) dequantise_kernel(const uint8_t* __re
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const int at = lane + 32 * (j & 3), row = r - lane / 16 + j / 4;
-                if (row < here && g * GROUP + at < K) out[(row0 + row) * (size_t)K + g * GROUP + at] = mine[j / 4][at];
+                if (row < here && g * GROUP + at < K) out[(size_t)row * K + g * GROUP + at] = mine[j / 4][at];
             }
             __syncwarp();
         }
@@ -145,16 +146,18 @@ PRISM_EXPORT int prism_mxfp4_quantize(const void* x, int dtype, long long ldx, i
     return (int)launch_kernel(mx::quantise_kernel<float>, grid, block, 0, stream, static_cast<const float*>(x), ldx, rows, K, groups, wide, c, s);
 }
 
-// the values: out [..., rows, K] of `dtype`, contiguous, 16-byte aligned
-PRISM_EXPORT int prism_mxfp4_dequantize(const void* codes, const void* scales, int matrices, int rows, int K, void* out, int dtype,
+// the values: out, a matrix [rows, K] of `dtype` every ldm elements
+PRISM_EXPORT int prism_mxfp4_dequantize(const void* codes, const void* scales, int matrices, int rows, int K, void* out, long long ldm, int dtype,
                                         cudaStream_t stream) {
     using namespace prism;
     if (matrices <= 0 || rows <= 0 || K <= 0) return 0;
     const int groups = mx::groups_of(K), tiles = (rows + mx::TILE_ROWS - 1) / mx::TILE_ROWS;
-    if (matrices > 65535 || tiles > 65535 || (((uintptr_t)codes | (uintptr_t)scales | (uintptr_t)out) & 15)) return (int)cudaErrorInvalidValue;
+    if (matrices > 65535 || tiles > 65535 || (((uintptr_t)codes | (uintptr_t)scales) & 15)) return (int)cudaErrorInvalidValue;
+    if (K % 8 == 0 && ((uintptr_t)out & 15 || (matrices > 1 && ldm % 8))) return (int)cudaErrorInvalidValue;
     const dim3 grid(groups, tiles, matrices), block(mx::THREADS);
     const uint8_t *c = static_cast<const uint8_t*>(codes), *s = static_cast<const uint8_t*>(scales);
     if (dtype == PRISM_DTYPE_BF16)
-        return (int)launch_kernel(mx::dequantise_kernel<__nv_bfloat16>, grid, block, 0, stream, c, s, rows, K, groups, static_cast<__nv_bfloat16*>(out));
-    return (int)launch_kernel(mx::dequantise_kernel<float>, grid, block, 0, stream, c, s, rows, K, groups, static_cast<float*>(out));
+        return (int)launch_kernel(mx::dequantise_kernel<__nv_bfloat16>, grid, block, 0, stream, c, s, rows, K, groups, static_cast<__nv_bfloat16*>(out),
+                                  ldm);
+    return (int)launch_kernel(mx::dequantise_kernel<float>, grid, block, 0, stream, c, s, rows, K, groups, static_cast<float*>(out), ldm);
 }

@@ -20,6 +20,7 @@ from ..config.engine_config import EngineConfig, ModelConfig
 from ..cache.manager import pool_sizes
 from ..model_registry import build_model
 from ..sampling.sampler import Sampler, SamplingParams
+from ..weights.four_bit import check_weight_format, to_four_bits
 from ..weights.loader import load_model_folder
 from ..weights.random_init import random_pool
 from .request import GenerationResult
@@ -35,10 +36,13 @@ class Engine:
         """``model``: a folder with config.json and model.safetensors (or a
         ``ModelConfig`` naming one).  Random-weights mode instead: ``config``
         (a raw config.json dict) and ``random_seed``; the weights are drawn on
-        the device and no file is written."""
+        the device and no file is written.  With ``engine_config.weight_format`` the layers' matrices are
+        brought to that format once they are loaded."""
+        ec = engine_config or EngineConfig()
+        check_weight_format(ec.weight_format, ec.act_bits, dtype or getattr(model, "dtype", "bfloat16"))
         if not torch.cuda.is_available():
             raise RuntimeError("prism_b200 needs a CUDA device; there is no CPU path")
-        self.engine_config = ec = engine_config or EngineConfig()
+        self.engine_config = ec
         if isinstance(model, str):
             model = ModelConfig(model_id=model, dtype=dtype or "bfloat16")
         self.model_config = model
@@ -54,6 +58,8 @@ class Engine:
                 raise ValueError("give a model folder, or config= and random_seed= for random weights")
             self.config, self.model = build_model(config)
             self.pool = random_pool(self.model, random_seed or 0, self.device, self.dtype)
+        if ec.weight_format is not None:
+            self.pool = to_four_bits(self.model, self.pool, self.device, self.dtype, ec.act_bits)
         spec = self.model.spec
         max_seq_len = min(ec.max_seq_len or spec.max_positions, spec.max_positions)
         num_pages = self._pages_per_group(ec, max_seq_len)

@@ -158,7 +158,7 @@ class _Sig:
     prism_attention_merge_bf16 = [_p, _p, _i, _p, _i, _i, _i, _i, _p]
     prism_swiglu = [_p, _p, _i, _i, _i, _p]
     prism_mxfp4_quantize = [_p, _i, _ll, _i, _i, _i, _p, _p, _p]
-    prism_mxfp4_dequantize = [_p, _p, _i, _i, _i, _p, _i, _p]
+    prism_mxfp4_dequantize = [_p, _p, _i, _i, _i, _p, _ll, _i, _p]
     prism_mxfp4_linear = [_p, _ll, _p, _p, _p, _i, _p, _i, _ll, _i, _i, _i, _i, _p, _p, _p, _p]
     prism_mxfp4_linear_workspace = [_i, _i, _i, _i, _p]
     prism_mxfp4_moe = [_p, _ll, _p, _i, _p, _i, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _i, _i, _i, _f, _p, _i, _i, _i, _f, _f,
@@ -460,7 +460,14 @@ def linear(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = None
     file.  float32 activations, or a float32 weight under bf16 activations
     (a tensor the model file stores in 32-bit), go through the true-float32
     kernel; bf16 x bf16 goes to the library matrix product (cuBLAS through
-    torch), as in andre-fu/prism (executor.py:109)."""
+    torch), as in andre-fu/prism (executor.py:109).  ``w`` may be an
+    ``Mxfp4``: bf16 activations by ``mxfp4_linear``, with its ``act_bits``."""
+    if isinstance(w, Mxfp4):
+        want = out_dtype or (out.dtype if out is not None else x.dtype)
+        if out is None or out.dtype == want:
+            return mxfp4_linear(x, w, bias, out, want, w.act_bits)
+        out.copy_(mxfp4_linear(x, w, bias, None, want, w.act_bits))
+        return out
     _cuda(x, w, bias)
     M, N = x.shape[0], w.shape[0]
     want = out_dtype or (out.dtype if out is not None else x.dtype)
@@ -623,7 +630,7 @@ def qkv_rotate_store(ctx, x: torch.Tensor, qkv_w: torch.Tensor, qkv_b: Optional[
             rope_kv_write_partial(parts, qkv_b, q, ctx.positions, ctx.tok_seg, table, rot.rotary_dim, kc, vc,
                                   cache.block_table, cache.num_pages, ctx.max_positions, nkv, ctx.err)
             return q
-    if QKV_LIBRARY and x.dtype == torch.bfloat16:
+    if QKV_LIBRARY and x.dtype == torch.bfloat16 and not isinstance(qkv_w, Mxfp4):
         b = qkv_b if (qkv_b is None or qkv_b.dtype == torch.bfloat16) else qkv_b.to(torch.bfloat16)
         qkv = torch.nn.functional.linear(x, qkv_w, b)
     else:

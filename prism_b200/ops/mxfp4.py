@@ -27,9 +27,10 @@ class Mxfp4:
     """A matrix ``[N, K]`` (or a stack ``[E, N, K]`` of them) in 4 bits.  ``codes``: uint8 ``[..., N, Kp / 2]`` with ``Kp``
     the K rounded up to 128, element 2i in the low half of a byte, zero beyond K.  ``scales``: uint8 ``[..., ceil(N / 128),
     Kp / 128, 512]``: the scale of row r and block b of a tile of 128 rows by four blocks is byte ``(r % 32) * 16 + r % 128
-    // 32 * 4 + b % 4``; zero for blocks beyond K, anything for rows beyond N."""
+    // 32 * 4 + b % 4``; zero for blocks beyond K, anything for rows beyond N.  ``act_bits``: what ``ops.linear`` does with the
+    activations (``mxfp4_linear``)."""
 
-    __slots__ = ("codes", "scales", "shape")
+    __slots__ = ("codes", "scales", "shape", "act_bits")
     dtype = DTYPE
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, K: int):
@@ -40,12 +41,12 @@ class Mxfp4:
                 and codes.dtype is torch.uint8 and scales.dtype is torch.uint8 and codes.is_contiguous() and scales.is_contiguous()
                 and codes.device == scales.device):
             raise ops.KernelError(f"4-bit matrix of K = {K}: codes {tuple(cs)} {codes.dtype} and scales {tuple(ss)} {scales.dtype} do not belong together")
-        self.codes, self.scales, self.shape = codes, scales, (cs[0], K) if d == 2 else (cs[0], cs[1], K)
+        self.codes, self.scales, self.shape, self.act_bits = codes, scales, (cs[0], K) if d == 2 else (cs[0], cs[1], K), 16
 
     @classmethod
     def _of(cls, codes, scales, shape) -> "Mxfp4":
         q = object.__new__(cls)
-        q.codes, q.scales, q.shape = codes, scales, shape
+        q.codes, q.scales, q.shape, q.act_bits = codes, scales, shape, 16
         return q
 
     @property
@@ -65,16 +66,23 @@ class Mxfp4:
             raise ops.KernelError("only a stack of 4-bit matrices can be indexed")
         return Mxfp4._of(self.codes[e], self.scales[e], self.shape[1:])
 
-    def dequantize(self, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
-        """The values that the codes stand for, exact in bfloat16 and float32; NaN where the scale is 255."""
+    def dequantize(self, dtype: Optional[torch.dtype] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """The values that the codes stand for, exact in bfloat16 (default) and float32; NaN where the scale is 255.  ``out``:
+        a place of this shape for them; a stack's matrices may lie apart in it."""
+        dtype = dtype or (torch.bfloat16 if out is None else out.dtype)
         if dtype not in (torch.bfloat16, torch.float32):
             raise ops.KernelError(f"4-bit values come back as bfloat16 or float32, not {dtype}")
         codes, shape = self.codes, self.shape
         if not codes.is_cuda:
             ops._cuda(codes)
-        out = codes.new_empty(shape, dtype=dtype)
+        K = shape[-1]
+        if out is None:
+            out = codes.new_empty(shape, dtype=dtype)
+        elif out.shape != shape or out.dtype is not dtype or not out[0:1].is_contiguous() or not out.is_cuda or (
+                len(shape) == 2 and not out.is_contiguous()) or (K % 8 == 0 and (out.data_ptr() % 16 or (len(shape) == 3 and out.stride(0) % 8))):
+            raise ops.KernelError(f"4-bit values of {shape} do not go into {tuple(out.shape)} {out.dtype} with strides {out.stride()}")
         ops._check(ops.lib().prism_mxfp4_dequantize(codes.data_ptr(), self.scales.data_ptr(), shape[0] if len(shape) == 3 else 1, shape[-2], shape[-1],
-                                                    out.data_ptr(), ops.F32 if dtype is torch.float32 else ops.BF16, ops._stream()),
+                                                    out.data_ptr(), out.stride(0), ops.F32 if dtype is torch.float32 else ops.BF16, ops._stream()),
                    "mxfp4_dequantize")
         return out
 

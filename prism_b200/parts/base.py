@@ -26,6 +26,8 @@ from __future__ import annotations
 from dataclasses import dataclass, field
 from typing import Callable, Dict, List, Optional, Tuple
 
+from .. import ops
+
 
 # --------------------------------------------------------------------------
 # weights a part asks for
@@ -186,6 +188,7 @@ class Part:
 
     category = ""
     prefix = ""
+    four_bit: Tuple[str, ...] = ()       # own parameters that may be kept in 4 bits (``ops.Mxfp4``)
 
     @property
     def children(self) -> Dict[str, "Part"]:
@@ -221,6 +224,10 @@ class Part:
 
     def on_bound(self) -> None:
         """Hook: create device buffers that are not weights (tables, scratch)."""
+
+    def in_four_bits(self, name: str, tensor):
+        """Parameter ``name`` as this part wants to be bound to it in 4 bits: an ``ops.Mxfp4`` or a tuple of them."""
+        return ops.mxfp4_quantize(tensor)
 
     def handed_over(self, *sources: WeightSource) -> Tuple[WeightSource, ...]:
         """Own file tensors under their full names, for a ``DetachedProjection``."""

@@ -18,6 +18,8 @@ class SwiGLU(FeedForward):
     through, ``silu`` or ``gelu_tanh``; or ``clamped``, the form with both projections limited by ``limit``
     (``ops.glu``).  ``biases``: the names of the gate's, the up and the down projection's biases, or None."""
 
+    four_bit = ("gate_up_w", "down_w")
+
     def __init__(self, hidden_size: int, intermediate_size: int,
                  names=("gate_proj.weight", "up_proj.weight", "down_proj.weight"), activation: str = "silu",
                  limit: Optional[float] = None, biases=None):
@@ -56,6 +58,8 @@ class SwiGLU(FeedForward):
 class ActMLP(FeedForward):
     """``down(act(up(x)))`` without gate.  ``activation``: one of ``ops.ACTIVATIONS`` (``relu2``: the square of
     relu; ``gelu_tanh``; ``silu``; ``relu``).  ``names``: the up and down tensors' names in the model file."""
+
+    four_bit = ("up_w", "down_w")
 
     def __init__(self, hidden_size: int, intermediate_size: int, activation: str = "relu2",
                  names=("up_proj.weight", "down_proj.weight")):
@@ -166,10 +170,48 @@ class MixtureOfExperts(FeedForward):
             ps.append(ParamSpec("correction", (WeightSource(self.correction, (self.routed,), "bias"),)))
         return ps
 
+    @property
+    def four_bit(self):
+        fits = (self.gated and not self.identity and self.activation in ops.GATED and self.experts <= ops.mxfp4.MOE_EXPERTS
+                and self.top <= ops.mxfp4.MOE_TOP)
+        return ("gate_up_w", "down_w") if fits else ()
+
+    def in_four_bits(self, name, tensor):
+        """The gate/up parameter as two stacks of matrices, the down parameter as one."""
+        H, I, E = self.hidden_size, self.intermediate_size, self.experts
+        if name == "down_w":
+            return ops.mxfp4_quantize(tensor.view(E, H, I))
+        gate_up = tensor.view(E, 2, I, H)
+        return tuple(ops.mxfp4_quantize(gate_up[:, i].contiguous()) for i in range(2))
+
     def on_bound(self):
         self.choice = ops.MoeChoice(self.w.get("correction"), self.groups, self.keep, self.weight_scale, self.sum_eps)
 
+    def _forward_four_bits(self, ctx, x):
+        """Experts in 4 bits: up to 64 tokens as one launch, a plane of sums; a longer step brings the step's layer back to
+        bfloat16 for the grouped products, which is right where every weight is used many times."""
+        T, H = x.shape
+        E, I = self.experts, self.intermediate_size
+        (gate, up), down = self.w["gate_up_w"], self.w["down_w"]
+        extra = 0 if self.shared is None else 1
+        if T <= ops.mxfp4.MOE_TOKENS:
+            y = ctx.alloc((1 + extra, T, H), ops.torch.float32)
+            ops.mxfp4_moe(x, self.w["router_w"], gate, up, down, self.top, self.softmax, self.renorm, self.scale_input, self.activation,
+                          self.limit, self.w.get("router_b"), self.choice, out=y[0])
+        else:
+            gate_up = ctx.alloc((E, 2, I, H), x.dtype)
+            gate.dequantize(out=gate_up[:, 0])
+            up.dequantize(out=gate_up[:, 1])
+            logits = ops.linear(x, self.w["router_w"], self.w.get("router_b"), out_dtype=ops.torch.float32)
+            y = ops.moe_feed_forward(ctx, x, logits, gate_up.view(E, 2 * I, H), down.dequantize(x.dtype), self.top, self.softmax, self.renorm,
+                                     self.scale_input, self.activation, True, self.choice, extra_planes=extra, limit=self.limit)
+        if extra:
+            self.shared.forward_to(ctx, x, y[-1])
+        return y
+
     def forward(self, ctx, x, rows32=None):
+        if isinstance(self.w["gate_up_w"], tuple):
+            return self._forward_four_bits(ctx, x)
         H, I, E = self.hidden_size, self.intermediate_size, self.experts
         # a gated shared expert with the experts' own activation runs with them
         alike = (isinstance(self.shared, SwiGLU) and self.gated and self.shared.activation == self.activation
