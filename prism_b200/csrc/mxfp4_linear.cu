@@ -323,7 +323,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
             const bool done = ++k == kb || i == n - 1;
             const int s_now = s;
             if (++s == STAGES) { s = 0; parity ^= 1; }
-            ready = mbar_try_wait(&full[s], parity);                     // of the next stage: the answer comes while products are issued
+            ready = i + 1 < n && mbar_test(&full[s], parity);            // the next stage: the answer comes while products are issued
             if (elect_one()) {
                 uint32_t more = !fresh;
 #pragma unroll 1
