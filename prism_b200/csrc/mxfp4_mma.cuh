@@ -109,6 +109,15 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
                  ::"r"(smem_addr(dst)), "l"(src), "r"(bytes), "r"(smem_addr(bar)) : "memory");
 }
+// To a counter in memory, behind all that the calling thread's CTA wrote before it met at a barrier that the thread was at; and (acq)
+// ahead of all that is read behind the barrier after it.  A barrier and one thread's release order as much as a fence of every
+// thread does and cost less.
+__device__ __forceinline__ void add_release(int* p, int v) { asm volatile("red.release.gpu.global.add.s32 [%0], %1;" ::"l"(p), "r"(v) : "memory"); }
+__device__ __forceinline__ int add_acq_rel(int* p, int v) {
+    int before;
+    asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], %2;" : "=r"(before) : "l"(p), "r"(v) : "memory");
+    return before;
+}
 // The warps that issue loads and products run their loops as a whole, and one lane of them issues: operands then stay in the
 // uniform registers that these instructions take them from.  A single lane's loop moves them over for every instruction (a
 // product of 128 x 32 x 32: 115 cycles against 42, of 128 x 128 x 32 65).

@@ -90,8 +90,7 @@ __device__ __forceinline__ bool wait_count(const int* p, int want, volatile int*
 __device__ __forceinline__ void grid_barrier(int* bar, int want, volatile int* abortp) {
     __syncthreads();
     if (threadIdx.x == 0) {
-        __threadfence();                                       // for all that this CTA's threads wrote before they met here
-        atomicAdd(bar, 1);
+        add_release(bar, 1);                                   // for all that this CTA's threads wrote before they met here
         wait_count(bar, want, abortp);
     }
     __syncthreads();
@@ -247,9 +246,7 @@ template <typename C> __device__ __forceinline__ void moe_route_and_terms(const 
             finished[threadIdx.x] = 0;
             if (t <= t1) {
                 const int here = min(first + count, (t + 1) * p.E) - max(first, t * p.E);
-                __threadfence();
-                finished[threadIdx.x] = atomicAdd(&p.control[2 + t], here) == p.E - here;
-                __threadfence();
+                finished[threadIdx.x] = add_acq_rel(&p.control[2 + t], here) == p.E - here;
             }
         }
         __syncthreads();
@@ -345,8 +342,7 @@ __device__ __forceinline__ void moe_compact(const Moe& p, const Lists& q) {
     fence_async();
     asm volatile("bar.sync 1, 256;" ::: "memory");
     for (int j = threadIdx.x - 128; j < mine; j += 256) {
-        __threadfence();
-        atomicAdd(&p.ready[p.most_live + q.owner[blockIdx.x + j * gridDim.x]], 1);
+        add_release(&p.ready[p.most_live + q.owner[blockIdx.x + j * gridDim.x]], 1);
     }
 }
 
@@ -541,11 +537,9 @@ moe_kernel(const __grid_constant__ CUtensorMap map_gate, const __grid_constant__
             };
             if (C::COMPACT) moe_compact(p, q);
             auto last_of = [&](int* counter, int others) {        // of the CTAs that share a tile
-                __threadfence();
                 asm volatile("bar.sync 1, 256;" ::: "memory");
-                if (threadIdx.x == 128) is_last = atomicAdd(counter, 1) == others;
+                if (threadIdx.x == 128) is_last = add_acq_rel(counter, 1) == others;
                 asm volatile("bar.sync 1, 256;" ::: "memory");
-                __threadfence();
                 return is_last != 0;
             };
             // ---- gate and up: the halves take the expert's tokens in turn
@@ -627,10 +621,7 @@ moe_kernel(const __grid_constant__ CUtensorMap map_gate, const __grid_constant__
                 }
                 fence_async();
                 asm volatile("bar.sync 1, 256;" ::: "memory");
-                if (threadIdx.x == 128) {
-                    __threadfence();
-                    atomicAdd(&p.ready[l], 1);
-                }
+                if (threadIdx.x == 128) add_release(&p.ready[l], 1);
             }
             // ---- down: a half has 128 of the 256 rows
             while (!out && b.n > 0) {
