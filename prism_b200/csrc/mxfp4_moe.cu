@@ -269,18 +269,25 @@ template <typename C> __device__ __forceinline__ void moe_route_and_terms(const 
     }
 }
 
-// 2: who has tokens
+// 2: who has tokens (the masks are zero)
 __device__ __forceinline__ void moe_lists(const Moe& p, Lists& q) {
     const int n = p.T * p.top;
-    for (int i = threadIdx.x; i < n; i += MOE_THREADS) {
-        q.expert_of[i] = (short)__ldcg(p.sel_e + i);
-        q.weight[i] = __ldcg(p.sel_w + i);
+    constexpr int EACH = (MOE_MOST_ENTRIES + MOE_THREADS - 1) / MOE_THREADS;
+    int expert[EACH];
+    float weight[EACH];
+#pragma unroll
+    for (int h = 0; h < EACH; ++h) {
+        const int i = threadIdx.x + h * MOE_THREADS;
+        if (i >= n) break;
+        expert[h] = __ldcg(p.sel_e + i), weight[h] = __ldcg(p.sel_w + i);
     }
-    for (int e = threadIdx.x; e < p.E; e += MOE_THREADS) q.mask[e] = 0;
-    __syncthreads();
-    for (int i = threadIdx.x; i < n; i += MOE_THREADS) {
-        const int t = i / p.top;
-        atomicOr(reinterpret_cast<unsigned int*>(&q.mask[q.expert_of[i]]) + t / 32, 1u << (t & 31));
+#pragma unroll
+    for (int h = 0; h < EACH; ++h) {
+        const int i = threadIdx.x + h * MOE_THREADS, t = i / p.top;
+        if (i >= n) break;
+        q.expert_of[i] = (short)expert[h];
+        q.weight[i] = weight[h];
+        atomicOr(reinterpret_cast<unsigned int*>(&q.mask[expert[h]]) + t / 32, 1u << (t & 31));
     }
     __syncthreads();
     if (threadIdx.x < 32) {
@@ -392,6 +399,7 @@ moe_kernel(const __grid_constant__ CUtensorMap map_gate, const __grid_constant__
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(tmem_slot)), "r"(C::COLS));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
     }
+    for (int e = threadIdx.x; e < p.E; e += MOE_THREADS) q.mask[e] = 0;
     moe_route_and_terms<C>(p, reinterpret_cast<float*>(tiles));
     fence_async();                          // the scratch becomes stages
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
