@@ -214,9 +214,9 @@ def mxfp4_moe(x: torch.Tensor, router: torch.Tensor, gate: Mxfp4, up: Mxfp4, dow
               renorm: bool = False, scale_input: bool = True, act: str = "silu", limit: float = 0.0,
               router_bias: Optional[torch.Tensor] = None, choice: Optional["ops.MoeChoice"] = None, out: Optional[torch.Tensor] = None,
               out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
-    """A mixture-of-experts layer for up to 64 tokens, up to 256 experts and up to 16 of them a token, in one launch: ``x [T, H]`` bfloat16, ``router [E, H]`` (logits in float32),
-    ``gate``, ``up`` ``[E, F, H]`` and ``down`` ``[E, H, F]`` in 4 bits.  Each token takes the ``top`` experts with the largest
-    scores (sigmoid of the logits, or their softmax; the lower index of equal ones); a choice's weight is its score
+    """A mixture-of-experts layer for up to 64 tokens, up to 256 experts and up to 16 of them a token, in one launch: ``x [T, H]``
+    bfloat16, ``router [E, H]`` (logits in float32), ``gate``, ``up`` ``[E, F, H]`` and ``down`` ``[E, H, F]`` in 4 bits.  Each
+    token takes the ``top`` experts with the largest scores (sigmoid of the logits, or their softmax; the lower index of equal ones); a choice's weight is its score
     (``renorm``: over the sum of the chosen) and multiplies the expert's input (``scale_input``) or its output.  ``act``:
     silu, gelu_tanh or clamped (with ``limit``, as in ``ops.glu``).  ``choice``: an ``ops.MoeChoice``.  Returns the sum over a
     token's choices, ``[T, H]`` bfloat16 or float32 (``out`` or ``out_dtype``)."""
