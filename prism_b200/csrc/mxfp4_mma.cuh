@@ -33,13 +33,19 @@ __device__ __forceinline__ void unpack_e4m3(uint32_t p, float& lo, float& hi) {
 
 __device__ __forceinline__ int term_byte(uint32_t most) { return most >= 0x7f800000u ? 255 : max((int)(most >> 23) - 7, 5); }
 __device__ __forceinline__ uint8_t low_byte(int byte) { return (uint8_t)(byte == 255 ? 255 : byte - 5); }
-// a value (of h's) as a byte of a high and one of a low term
-__device__ __forceinline__ void terms_of_one(float v, int byte, uint32_t& hi, uint32_t& lo) {
-    const float a = byte == 255 ? 0.f : v * __uint_as_float((uint32_t)(254 - byte) << 23);
-    float ha, none;
-    hi = pack_e4m3(a, 0.f);
-    unpack_e4m3(hi, ha, none);
-    lo = byte == 255 ? 0 : pack_e4m3((a - ha) * 32.f, 0.f);
+// A float32 value as three such terms, 2^(byte - 127) (t0 + 2^-5 t1 + 2^-10 t2): each takes what the one before left over, at most
+// half a step of it, 8 of 256.  So off by at most 2^-14 of the value (8 of 2^10 beside 128), or, where the last is below E4M3's
+// normal numbers, by 2^-27 of the block's largest.  The last one's byte is 10 less, so a block's is at least 10.
+__device__ __forceinline__ int three_term_byte(uint32_t most) { return most >= 0x7f800000u ? 255 : max((int)(most >> 23) - 7, 10); }
+__device__ __forceinline__ void three_terms(float v, int byte, uint32_t (&term)[3]) {
+    float rest = byte == 255 ? 0.f : v * __uint_as_float((uint32_t)(254 - byte) << 23);
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+        float held, none;
+        term[i] = pack_e4m3(rest, 0.f);
+        unpack_e4m3(term[i], held, none);
+        rest = (rest - held) * 32.f;
+    }
 }
 // The terms of eight bfloat16 values as they lie in memory, in half precision where two share an instruction (exact: a scaled
 // value has 8 significant bits and is below 256; what half precision drops is below 2^-24, which no E4M3 term of it holds).

@@ -10,16 +10,19 @@
 //      two 8-bit terms (mxfp4_mma.cuh); barrier over the grid
 //   2. every CTA reads the choices and lists the experts that have tokens
 //   3. gate and up: 128 rows of either and all tokens (high terms, low terms) as columns of one tcgen05.mma each; the sums of
-//      an expert's tokens become h, again as two terms (a warp's 32 lanes are one block)
+//      an expert's tokens become h, as three terms (a warp's 32 lanes are one block): h is not of bfloat16's 8 significant bits as x
+//      is, and two terms would round it to about those; three hold it to 2^-14 of itself and 2^-27 of its block's largest.  With two
+//      a whole layer's result was off by 0.0018 of its scale instead of 0.0017, bfloat16's own rounding; the third costs nothing at 1
+//      token, 1 % at 16 and 5 % at 64 (below: 84.9 us with two)
 //   4. down: 256 rows, the expert's own tokens as columns, once all of its h is there (a counter per expert)
 //   5. barrier over the grid; y is the sum of a token's choices in their order
 // In 3 and 4 the blocks (expert, rows, 128 of K) are dealt to the CTAs evenly as one line; a tile that several CTAs have part of
 // is added up by the last to come, in the CTAs' order: results do not depend on timing.
 //
-// 1 token through 2 of 8 experts of 3 x 672 x 2,048: 21.4 us, of which routing and its barrier 5.7, lists 2, the first weights 3,
+// 1 token through 2 of 8 experts of 3 x 672 x 2,048: 21.8 us, of which routing and its barrier 5.7, lists 2, the first weights 3,
 // two hand-overs of a tile's shares some 4 each, the last barrier and sums 1.5.  16 tokens through 8 of 3 x 1,184 x 4,096: 40.8 us.  64
-// tokens through 64 of 3 x 1,024 x 2,048, 8 a token: 84.6 us for 214 MB, of which 28 until the first products (routing over 64 experts,
-// lists, x laid out), 29 gate and up at 4.9 TB/s, 12 until an expert's h is whole, 15 down.
+// tokens through 64 of 3 x 1,024 x 2,048, 8 a token: 89.4 us for 214 MB, of which 28 until the first products (routing over 64 experts,
+// lists, x laid out), 29 gate and up at 4.9 TB/s, some 14 until an expert's h is whole, some 18 down.
 //
 // Warp 0 streams weights and their scales, warp 2 x and h, warp 1 issues the products, warps 4-11 take the sums out.  Every
 // wait is bounded; on expiry the error word is set, tensor memory is freed, the control block is cleared and the kernel returns.
@@ -39,9 +42,10 @@ constexpr int MOE_THREADS = 384, MOE_WARPS = 12, MOE_MOST_EXPERTS = 256, MOE_MOS
 template <int TT_> struct MoeCfg {
     static constexpr int TT = TT_, NCOL = 2 * TT;
     static constexpr bool COMPACT = TT > 16;
-    static constexpr int W_BYTES = 2 * 16384, X_BYTES = NCOL * 128, STAGE = W_BYTES + X_BYTES, SF = 3 * TILE_BYTES, SF_COLS = 12;
+    // of x two terms a token, of h three: up to 192 rows, whose scales are two tiles
+    static constexpr int W_BYTES = 2 * 16384, X_BYTES = 3 * TT * 128, STAGE = W_BYTES + X_BYTES, SF = 4 * TILE_BYTES, SF_COLS = 16;
     static constexpr int FIT = 200 * 1024 / (STAGE + SF), STAGES = FIT > 8 ? 8 : FIT;
-    static constexpr int USED = 2 * NCOL + STAGES * SF_COLS, BOTH = 4 * NCOL + STAGES * SF_COLS;       // columns with one set of sums, with two
+    static constexpr int USED = 6 * TT + STAGES * SF_COLS, BOTH = 12 * TT + STAGES * SF_COLS;       // columns with one set of sums, with two
     static constexpr int COLS = BOTH <= 128 ? 128 : BOTH <= 256 ? 256 : 512;
     static constexpr size_t SMEM = (size_t)STAGES * (STAGE + SF) + 1024 + 512;
     static_assert(USED <= 512 && STAGES >= 3, "tensor memory or shared memory");
@@ -51,7 +55,7 @@ struct Moe {
     const __nv_bfloat16* x;
     const void *router, *rbias, *corr;
     const uint8_t *gate_s, *up_s, *down_s;
-    // x's terms [2 TT][Hp] and scales [groups][512] (compact: [rows][Hp] and [live][groups][512]), h's [rows][Fp] and [live][groups][512]
+    // x's terms [2 TT][Hp] and scales [groups][512] (compact: [rows][Hp] and [live][groups][512]), h's [rows][Fp] and [live][groups][2][512]
     uint8_t *xt, *xs, *h, *hs;
     float *z, *sel_w, *part1, *part2, *planes;
     int *sel_e, *counters, *ready, *control, *err;      // ready: h, then x (compact); control: barrier, leavers, a counter per token
@@ -302,7 +306,7 @@ __device__ __forceinline__ void moe_lists(const Moe& p, Lists& q) {
         for (int e0 = 0; e0 < p.E; e0 += 32) {
             const int e = e0 + lane, c = e < p.E ? __popcll(q.mask[e]) : 0;
             const unsigned any = __ballot_sync(0xffffffffu, c > 0);
-            int v = c | (c + 7) / 8 * 2 << 16;                    // inclusive sums over the lanes: tokens, rows of h / 8
+            int v = c | (c + 7) / 8 * 3 << 16;                    // inclusive sums over the lanes: tokens, rows of h / 8
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
                 const int a = __shfl_up_sync(0xffffffffu, v, o);
@@ -314,7 +318,7 @@ __device__ __forceinline__ void moe_lists(const Moe& p, Lists& q) {
                 q.expert[at] = (short)e;
                 q.count[at] = (short)c;
                 q.first[at] = (short)(first + (v & 0xffff) - c);
-                q.hrow8[at] = (short)(row8 + (v >> 16) - (c + 7) / 8 * 2);
+                q.hrow8[at] = (short)(row8 + (v >> 16) - (c + 7) / 8 * 3);
             }
             v = __shfl_sync(0xffffffffu, v, 31);
             live += __popc(any);
@@ -424,7 +428,7 @@ moe_kernel(const __grid_constant__ CUtensorMap map_gate, const __grid_constant__
         const int n1 = a.n, n = a.n + b.n;
         int* units2 = p.counters + q.live * tiles1;
         // columns of a tile's sums; two sets of them where they fit
-        const int cols = C::COMPACT ? (q.most + 7) / 8 * 16 : NCOL, bufs = 4 * cols + STAGES * C::SF_COLS <= C::COLS ? 2 : 1;
+        const int cols = max((q.most + 7) / 8 * 24, C::COMPACT ? 0 : NCOL), bufs = 4 * cols + STAGES * C::SF_COLS <= C::COLS ? 2 : 1;
 
         if (warp == 0) {
             uint32_t parity = 1;                                 // the first round passes at once
@@ -472,7 +476,7 @@ moe_kernel(const __grid_constant__ CUtensorMap map_gate, const __grid_constant__
                 const int l = one ? a.l : b.l, k = one ? a.k : b.k;
                 if (one && !C::COMPACT) {
                     if (elect_one()) {
-                        mbar_expect_tx(&full[s], C::X_BYTES + TILE_BYTES);
+                        mbar_expect_tx(&full[s], NCOL * 128 + TILE_BYTES);
                         tma_load_2d(st, &map_x, &full[s], k * 128, 0);
                         bulk_load(ss, p.xs + (size_t)k * TILE_BYTES, TILE_BYTES, &full[s]);
                     }
@@ -483,10 +487,10 @@ moe_kernel(const __grid_constant__ CUtensorMap map_gate, const __grid_constant__
                         fence_async();
                         seen = l;
                     }
-                    const int boxes = (q.count[l] + 7) / 8 * 2, row0 = q.hrow8[l] * 8;
+                    const int boxes = (q.count[l] + 7) / 8 * (one ? 2 : 3), row0 = q.hrow8[l] * 8, scales = boxes * 8 > 128 && !one ? 2 * TILE_BYTES : TILE_BYTES;
                     if (elect_one()) {
-                        mbar_expect_tx(&full[s], boxes * 1024 + TILE_BYTES);
-                        bulk_load(ss, (one ? p.xs + ((size_t)l * g1 + k) * TILE_BYTES : p.hs + ((size_t)l * g2 + k) * TILE_BYTES), TILE_BYTES, &full[s]);
+                        mbar_expect_tx(&full[s], boxes * 1024 + scales);
+                        bulk_load(ss, one ? p.xs + ((size_t)l * g1 + k) * TILE_BYTES : p.hs + ((size_t)l * g2 + k) * (2 * TILE_BYTES), scales, &full[s]);
                         for (int j = 0; j < boxes; ++j) tma_load_2d(st + j * 1024, one ? &map_x : &map_h, &full[s], k * 128, row0 + j * 8);
                     }
                 }
@@ -506,7 +510,7 @@ moe_kernel(const __grid_constant__ CUtensorMap map_gate, const __grid_constant__
                 if (!warp_wait(&full[s], parity, abortp)) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const uint32_t ss = sf0 + s * C::SF, tsf = tmem_sf + s * C::SF_COLS;
-                const int n_cols = i < n1 ? (C::COMPACT ? (q.count[a.l] + 7) / 8 * 16 : NCOL) : (q.count[b.l] + 7) / 8 * 16;
+                const int n_cols = i < n1 ? (C::COMPACT ? (q.count[a.l] + 7) / 8 * 16 : NCOL) : (q.count[b.l] + 7) / 8 * 24;
                 const uint32_t idesc = 5u << 7 | (uint32_t)(n_cols >> 3) << 17 | 1u << 23 | 1u << 27;           // E2M1 by E4M3, scales E8M0
                 const uint64_t da = desc0 + (uint32_t)(s * (C::STAGE >> 4)), db = da + (C::W_BYTES >> 4);
                 const uint32_t d = tmem + buf * 2 * cols;
@@ -514,6 +518,7 @@ moe_kernel(const __grid_constant__ CUtensorMap map_gate, const __grid_constant__
                 if (elect_one()) {
 #pragma unroll
                     for (int c = 0; c < 3; ++c) scales_to_tmem(tsf + c * 4, ss + c * TILE_BYTES);
+                    if (n_cols > 128) scales_to_tmem(tsf + 12, ss + 3 * TILE_BYTES);
 #pragma unroll
                     for (uint32_t j = 0; j < 4; ++j)
 #pragma unroll
@@ -567,17 +572,16 @@ moe_kernel(const __grid_constant__ CUtensorMap map_gate, const __grid_constant__
                     const float w = q.weight[q.plane[first + r]];
                     if (p.scale_in) { g *= w; u *= w; }
                     const float h = f < p.F ? moe_glu(g, u, p.act, p.limit) * (p.scale_in ? 1.f : w) : 0.f;
-                    const int byte = term_byte(__reduce_max_sync(0xffffffffu, __float_as_uint(h) & 0x7fffffffu));
-                    uint32_t hi, lo;
-                    terms_of_one(h, byte, hi, lo);
+                    const int byte = three_term_byte(__reduce_max_sync(0xffffffffu, __float_as_uint(h) & 0x7fffffffu));
+                    uint32_t term[3];
+                    three_terms(h, byte, term);
                     uint8_t* to = p.h + (size_t)(q.hrow8[l] * 8 + r) * ((size_t)g2 * GROUP) + f;
-                    to[0] = (uint8_t)hi;
-                    to[(size_t)nt * g2 * GROUP] = (uint8_t)lo;
-                    if (lane == 0) {
-                        uint8_t* s = p.hs + ((size_t)l * g2 + tile) * TILE_BYTES + quarter;
-                        const int v = nt + r;
-                        s[(r & 31) * 16 + r / 32 * 4] = (uint8_t)byte;
-                        s[(v & 31) * 16 + v / 32 * 4] = low_byte(byte);
+                    const size_t next = (size_t)nt * g2 * GROUP;
+                    to[0] = (uint8_t)term[0], to[next] = (uint8_t)term[1], to[2 * next] = (uint8_t)term[2];
+                    if (lane < 3) {                               // a term's scale each
+                        const int v = lane * nt + r;
+                        p.hs[((size_t)l * g2 + tile) * (2 * TILE_BYTES) + quarter + v / 128 * TILE_BYTES + (v & 31) * 16 + (v & 127) / 32 * 4] =
+                            byte == 255 ? 255 : (uint8_t)(byte - 5 * lane);
                     }
                 };
                 float* mine = p.part1 + (size_t)(cta * 2 + s1.place(cta, unit)) * (2 * TT * 128) + row;
@@ -649,17 +653,18 @@ moe_kernel(const __grid_constant__ CUtensorMap map_gate, const __grid_constant__
                     if (f < p.H) p.planes[(size_t)q.plane[first + r] * p.H + f] = v;
                 };
                 for (int r0 = 0; r0 < count; r0 += 8) {
-                    uint32_t r[8], o[8];
-                    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
-                                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]) : "r"(d + r0));
-                    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
-                                 : "=r"(o[0]), "=r"(o[1]), "=r"(o[2]), "=r"(o[3]), "=r"(o[4]), "=r"(o[5]), "=r"(o[6]), "=r"(o[7]) : "r"(d + nt + r0));
+                    uint32_t r[3][8];
+#pragma unroll
+                    for (int i = 0; i < 3; ++i)
+                        asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                                     : "=r"(r[i][0]), "=r"(r[i][1]), "=r"(r[i][2]), "=r"(r[i][3]), "=r"(r[i][4]), "=r"(r[i][5]), "=r"(r[i][6]), "=r"(r[i][7])
+                                     : "r"(d + i * nt + r0));
                     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
-                        asm volatile("" : "+r"(r[j]), "+r"(o[j]));
+                        asm volatile("" : "+r"(r[0][j]), "+r"(r[1][j]), "+r"(r[2][j]));
                         if (r0 + j >= count) break;
-                        const float v = __uint_as_float(r[j]) + __uint_as_float(o[j]);
+                        const float v = __uint_as_float(r[0][j]) + (__uint_as_float(r[1][j]) + __uint_as_float(r[2][j]));
                         if (whole) store(r0 + j, v);
                         else mine[(r0 + j) * 128] = v;
                     }
@@ -734,7 +739,7 @@ inline MoePlan moe_plan(int T, int H, int F, int E, int top) {
     q.tt = T <= 8 ? 8 : T <= 16 ? 16 : T <= 32 ? 32 : 64;
     q.P = sm_count();
     q.most_live = E < T * top ? E : T * top;
-    q.most_rows = 2 * (T * top + 7 * q.most_live);
+    q.most_rows = 3 * (T * top + 7 * q.most_live);
     const long long g1 = groups_of(H), g2 = groups_of(F), tiles2 = ((H + 127) / 128 + 1) / 2;
     q.ncounters = (int)(q.most_live * (g2 + tiles2) + 2 * q.most_live);
     long long at = 0;
@@ -743,7 +748,7 @@ inline MoePlan moe_plan(int T, int H, int F, int E, int top) {
     q.xt = take((q.compact ? (long long)q.most_rows : 2LL * q.tt) * g1 * GROUP);
     q.xs = take((q.compact ? q.most_live : 1) * g1 * TILE_BYTES);
     q.h = take((long long)q.most_rows * g2 * GROUP);
-    q.hs = take(q.most_live * g2 * TILE_BYTES);
+    q.hs = take(q.most_live * g2 * (2 * TILE_BYTES));
     q.z = take(4LL * T * E);
     q.sel_e = take(4LL * T * top);
     q.sel_w = take(4LL * T * top);

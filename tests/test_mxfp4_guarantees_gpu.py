@@ -1,0 +1,41 @@
+"""What the 4-bit operators promise beyond their values at ordinary inputs: how far an expert's hidden values are held.
+
+Tolerances.  A product's float32 sum is within 2^-18 of the sum of |x w| of the 64-bit one (``test_mxfp4_gpu``)."""
+
+import pytest
+import torch
+
+from test_mxfp4_gpu import DEV, _acts, _experts, _gen, _ops, decode
+
+pytestmark = pytest.mark.gpu
+
+SUM = 2.0 ** -18
+
+
+@pytest.mark.parametrize("T,E,F,H", [(1, 2, 32, 64), (5, 3, 100, 256), (16, 2, 672, 700), (20, 2, 130, 256), (64, 2, 200, 256), (64, 1, 256, 512), (64, 16, 64, 128)])
+def test_hidden_values_keep_fourteen_bits(T, E, F, H):
+    """One choice of weight 1 a token, and down products that each read one hidden value: so the result shows what is
+    held of it, 2^-14 of itself and 2^-27 of the largest of its block of 32 (two 8-bit terms would hold 2^-9).  Beside that
+    only the errors of g and u, through silu (slope below 1.1) and the product."""
+    ops = _ops()
+    x = _acts(T, H, T + F)
+    router = (_acts(E, H, 4) * H ** -0.5).to(torch.bfloat16)
+    gate, up, _ = _experts(E, F, H, F)
+    sparse = torch.zeros(E, H, F)
+    sparse[:, torch.arange(H), torch.arange(H) % F] = torch.where(torch.rand(E, H, generator=_gen(3)) < 0.5, -1.0, 1.0)
+    down = ops.mxfp4_quantize(sparse.to(DEV))
+    assert torch.equal(down.dequantize(torch.float32).cpu(), sparse)
+    got = ops.mxfp4_moe(x, router, gate, up, down, 1, True, True, False, out_dtype=torch.float32).double()
+    pick = torch.argsort(-torch.softmax(x.double() @ router.double().t(), -1), dim=1, stable=True)[:, 0]
+    for t in range(T):
+        e, a = int(pick[t]), x[t].double()
+        wg, wu = decode(gate[e]).to(DEV), decode(up[e]).to(DEV)
+        g, u = wg @ a, wu @ a
+        eg, eu = (wg.abs() @ a.abs()) * SUM, (wu.abs() @ a.abs()) * SUM
+        s = torch.nn.functional.silu(g)
+        h = s * u
+        block = torch.nn.functional.pad(h.abs(), (0, -F % 32)).view(-1, 32).amax(1).repeat_interleave(32)[:F]
+        bound = h.abs() * (2.0 ** -14 + 2.0 ** -20) + block * 2.0 ** -27 + 1.1 * eg * (u.abs() + eu) + s.abs() * eu
+        at = torch.arange(H, device=DEV) % F
+        far = (got[t] - sparse[e, torch.arange(H), at.cpu()].to(DEV).double() * h[at]).abs() - bound[at]
+        assert (far <= 0).all(), (t, far.max().item(), (far > 0).double().mean().item())
