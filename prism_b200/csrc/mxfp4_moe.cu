@@ -25,7 +25,8 @@
 // lists, x laid out), 29 gate and up at 4.9 TB/s, some 14 until an expert's h is whole, some 18 down.
 //
 // Warp 0 streams weights and their scales, warp 2 x and h, warp 1 issues the products, warps 4-11 take the sums out.  Every
-// wait is bounded; on expiry the error word is set, tensor memory is freed, the control block is cleared and the kernel returns.
+// wait is bounded; on expiry all CTAs learn of it and leave without a result: the error word is set, tensor memory is freed, the
+// control block is cleared and the kernel returns.
 #include "moe_route.cuh"
 #include "mxfp4_mma.cuh"
 #include "vec.cuh"
@@ -58,13 +59,17 @@ struct Moe {
     // x's terms [2 TT][Hp] and scales [groups][512] (compact: [rows][Hp] and [live][groups][512]), h's [rows][Fp] and [live][groups][2][512]
     uint8_t *xt, *xs, *h, *hs;
     float *z, *sel_w, *part1, *part2, *planes;
-    int *sel_e, *counters, *ready, *control, *err;      // ready: h, then x (compact); control: barrier, leavers, a counter per token
+    int *sel_e, *counters, *ready, *control, *err;      // ready: h, then x (compact); control: see Control
     void* y;
     long long ldx, ldy;
     int T, H, F, E, top, softmax, renorm, scale_in, act, groups_of_experts, keep, dots, most_live, ncounters;
     int router_bf16, rbias_bf16, corr_bf16, out_bf16, wide;
     float limit, wscale, sum_eps;
 };
+
+// Words of the control block.  A barrier's word counts its own arrivals only, and a CTA that gave up arrives nowhere any more but
+// raises GAVE_UP, which whoever waits in memory reads too: so nobody passes a barrier before all that it stands for is there.
+enum Control { FIRST, SECOND, GAVE_UP, LEAVERS, TOKEN, CONTROL_WORDS = TOKEN + 64 };     // TOKEN: logits that are there, a word each
 
 struct Lists {                             // of the experts that have tokens, in their order
     unsigned long long mask[MOE_MOST_EXPERTS];
@@ -78,29 +83,35 @@ struct Lists {                             // of the experts that have tokens, i
     int live, entries, most;               // experts with tokens, their tokens in all, the most of one
 };
 
-// until *p >= want, within the limit of every wait here
-__device__ __forceinline__ bool wait_count(const int* p, int want, volatile int* abortp) {
+// until *p >= want, within the limit of every wait here and as long as no CTA has given up
+__device__ __forceinline__ int load_acquire(const int* p) {
+    int v;
+    asm volatile("ld.acquire.gpu.global.b32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
+    return v;
+}
+__device__ __forceinline__ bool wait_count(const int* p, int want, const int* control, volatile int* abortp) {
     unsigned long long t0 = 0;
     for (int i = 0;; ++i) {
-        int v;
-        asm volatile("ld.acquire.gpu.global.b32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
-        if (v >= want) return true;
+        if (load_acquire(p) >= want) return true;
         if (i % 64 == 63) {
             const unsigned long long now = tc::globaltimer();
             if (t0 == 0) t0 = now;
             if (*abortp) return false;
-            if (now - t0 > tc::WAIT_LIMIT_NS) {
+            if (now - t0 > tc::WAIT_LIMIT_NS || load_acquire(control + GAVE_UP)) {
                 *abortp = 1;
                 return false;
             }
         }
     }
 }
-__device__ __forceinline__ void grid_barrier(int* bar, int want, volatile int* abortp) {
+__device__ __forceinline__ void grid_barrier(int* control, int which, volatile int* abortp) {
     __syncthreads();
     if (threadIdx.x == 0) {
-        add_release(bar, 1);                                   // for all that this CTA's threads wrote before they met here
-        wait_count(bar, want, abortp);
+        if (!*abortp) {
+            add_release(control + which, 1);                   // for all that this CTA's threads wrote before they met here
+            wait_count(control + which, gridDim.x, control, abortp);
+        }
+        if (*abortp) add_release(control + GAVE_UP, 1);
     }
     __syncthreads();
 }
@@ -255,7 +266,7 @@ template <typename C> __device__ __forceinline__ void moe_route_and_terms(const 
             finished[threadIdx.x] = 0;
             if (t <= t1) {
                 const int here = min(first + count, (t + 1) * p.E) - max(first, t * p.E);
-                finished[threadIdx.x] = add_acq_rel(&p.control[2 + t], here) == p.E - here;
+                finished[threadIdx.x] = add_acq_rel(&p.control[TOKEN + t], here) == p.E - here;
             }
         }
         __syncthreads();
@@ -278,11 +289,11 @@ template <typename C> __device__ __forceinline__ void moe_route_and_terms(const 
     }
 }
 
-// 2: who has tokens (the masks are zero)
-__device__ __forceinline__ void moe_lists(const Moe& p, Lists& q) {
+// 2: who has tokens (the masks are zero).  False, for all threads: what was read are not choices.
+__device__ __forceinline__ bool moe_lists(const Moe& p, Lists& q) {
     const int n = p.T * p.top;
     constexpr int EACH = (MOE_MOST_ENTRIES + MOE_THREADS - 1) / MOE_THREADS;
-    int expert[EACH];
+    int expert[EACH], wrong = 0;
     float weight[EACH];
 #pragma unroll
     for (int h = 0; h < EACH; ++h) {
@@ -294,11 +305,15 @@ __device__ __forceinline__ void moe_lists(const Moe& p, Lists& q) {
     for (int h = 0; h < EACH; ++h) {
         const int i = threadIdx.x + h * MOE_THREADS, t = i / p.top;
         if (i >= n) break;
+        if ((unsigned)expert[h] >= (unsigned)p.E) {              // (numbers index shared memory from here on)
+            wrong = 1;
+            continue;
+        }
         q.expert_of[i] = (short)expert[h];
         q.weight[i] = weight[h];
         atomicOr(reinterpret_cast<unsigned int*>(&q.mask[expert[h]]) + t / 32, 1u << (t & 31));
     }
-    __syncthreads();
+    if (__syncthreads_or(wrong)) return false;
     if (threadIdx.x < 32) {
         const int lane = threadIdx.x;
         int live = 0, first = 0, row8 = 0, most = 0;
@@ -342,6 +357,7 @@ __device__ __forceinline__ void moe_lists(const Moe& p, Lists& q) {
         q.owner[at] = q.slot[e];
     }
     __syncthreads();
+    return true;
 }
 
 // (compact) rows of x, as terms, laid out for the experts that read them; an expert's counter says how many of its rows are there
@@ -412,14 +428,15 @@ moe_kernel(const __grid_constant__ CUtensorMap map_gate, const __grid_constant__
     moe_route_and_terms<C>(p, reinterpret_cast<float*>(tiles));
     fence_async();                          // the scratch becomes stages
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-    grid_barrier(p.control, P, abortp);
+    grid_barrier(p.control, FIRST, abortp);
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = *tmem_slot, tmem_sf = tmem + C::COLS - STAGES * C::SF_COLS;
     if (threadIdx.x == 0) gone = *abortp;
     __syncthreads();
 
-    if (!gone) {
-        moe_lists(p, q);
+    if (gone || !moe_lists(p, q)) {
+        if (threadIdx.x == 0) abort_flag = 1;
+    } else {
         const int g1 = groups_of(p.H), g2 = groups_of(p.F), tiles1 = g2, tiles_h = (p.H + 127) / 128, tiles2 = (tiles_h + 1) / 2;
         const int total1 = q.live * tiles1 * g1, total2 = q.live * tiles2 * g2;
         // no more than about eight CTAs share a tile: joining more costs more than their blocks
@@ -483,7 +500,7 @@ moe_kernel(const __grid_constant__ CUtensorMap map_gate, const __grid_constant__
                 } else {
                     if (i == n1) seen = -1;
                     if (l != seen) {                             // all of this expert's rows are there
-                        if (!__all_sync(0xffffffffu, wait_count(one ? &p.ready[p.most_live + l] : &p.ready[l], one ? q.count[l] : tiles1, abortp))) break;
+                        if (!__all_sync(0xffffffffu, wait_count(one ? &p.ready[p.most_live + l] : &p.ready[l], one ? q.count[l] : tiles1, p.control, abortp))) break;
                         fence_async();
                         seen = l;
                     }
@@ -701,7 +718,7 @@ moe_kernel(const __grid_constant__ CUtensorMap map_gate, const __grid_constant__
         }
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-    grid_barrier(p.control, 2 * P, abortp);
+    grid_barrier(p.control, SECOND, abortp);
     if (threadIdx.x == 0) gone = *abortp;
     __syncthreads();
     if (!gone) {
@@ -716,10 +733,8 @@ moe_kernel(const __grid_constant__ CUtensorMap map_gate, const __grid_constant__
     if (threadIdx.x == 0) {
         if (gone) report_error(p.err, PRISM_ERR_WAIT_TIMEOUT);
         __threadfence();
-        if (atomicAdd(&p.control[1], 1) == P - 1) {               // the last to leave clears the control block for the next launch
-            for (int t = 0; t < p.T; ++t) p.control[2 + t] = 0;
-            p.control[0] = p.control[1] = 0;
-        }
+        if (atomicAdd(&p.control[LEAVERS], 1) == P - 1)           // the last to leave clears the control block for the next launch
+            for (int i = 0; i < TOKEN + p.T; ++i) p.control[i] = 0;
     }
     if (warp == 1) {
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -793,7 +808,7 @@ PRISM_EXPORT int prism_mxfp4_moe_workspace(int T, int H, int F, int E, int top, 
 }
 
 // x [T, H] bfloat16; router [E, H] (+ rbias [E]); gate, up [E, F, H] and down [E, H, F] in 4 bits; corr [E] or null.
-// ws: workspace of the call; control: 66 ints, zero before the first launch (the kernel leaves them zero), of one stream's
+// ws: workspace of the call; control: 68 ints, zero before the first launch (the kernel leaves them zero), of one stream's
 // launches at a time.  y [T, H] of `out_dtype` (row stride ldy).
 PRISM_EXPORT int prism_mxfp4_moe(const void* x, long long ldx, const void* router, int router_dtype, const void* rbias, int rbias_dtype,
                                  const void* gate_codes, const void* gate_scales, const void* up_codes, const void* up_scales,

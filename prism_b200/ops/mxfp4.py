@@ -136,7 +136,8 @@ def _err_word(device: torch.device) -> int:
     return p
 
 
-_COUNTERS = 4096             # of a stream: tiles of a product (csrc/mxfp4_linear.cu), or 66 of an experts' layer
+_COUNTERS = 4096             # of a stream: tiles of a product (csrc/mxfp4_linear.cu), or an experts' layer's control words
+_CONTROL = 68                # csrc/mxfp4_moe.cu: Control
 _SCRATCH = 16 << 20          # a larger workspace is the call's own
 _ARENA = 1 << 20
 _streams = {}                # (device, stream) -> [counters, workspace]: launches of one stream follow each other
@@ -249,7 +250,7 @@ def mxfp4_moe(x: torch.Tensor, router: torch.Tensor, gate: Mxfp4, up: Mxfp4, dow
     if T == 0:
         return out
     stream = ops._stream()
-    work, control = _call_memory(stream, x.device, _workspace("prism_mxfp4_moe_workspace", T, H, F, E, top), 66)
+    work, control = _call_memory(stream, x.device, _workspace("prism_mxfp4_moe_workspace", T, H, F, E, top), _CONTROL)
     ops._check(ops.lib().prism_mxfp4_moe(x.data_ptr(), x.stride(0), router.data_ptr(), ops._dt(router),
                                          None if router_bias is None else router_bias.data_ptr(), 0 if router_bias is None else ops._dt(router_bias),
                                          gate.codes.data_ptr(), gate.scales.data_ptr(), up.codes.data_ptr(), up.scales.data_ptr(),

@@ -1,4 +1,5 @@
-"""What the 4-bit operators promise beyond their values at ordinary inputs: how far an expert's hidden values are held.
+"""What the 4-bit operators promise beyond their values at ordinary inputs: how far an expert's hidden values are held; that a
+wait that runs out is an error and nothing else.
 
 Tolerances.  A product's float32 sum is within 2^-18 of the sum of |x w| of the 64-bit one (``test_mxfp4_gpu``)."""
 
@@ -39,3 +40,29 @@ def test_hidden_values_keep_fourteen_bits(T, E, F, H):
         at = torch.arange(H, device=DEV) % F
         far = (got[t] - sparse[e, torch.arange(H), at.cpu()].to(DEV).double() * h[at]).abs() - bound[at]
         assert (far <= 0).all(), (t, far.max().item(), (far > 0).double().mean().item())
+
+
+def _moe_args(T, H=256, F=200, E=6, seed=1):
+    router = (_acts(E, H, 4) * H ** -0.5).to(torch.bfloat16)
+    return (_acts(T, H, seed), router, *_experts(E, F, H, 2), 2, True, True, False)
+
+
+@pytest.mark.parametrize("T", [1, 12, 40])
+def test_a_wait_that_runs_out_leaves_no_result_and_no_trace(T):
+    """One arrival short at the barrier behind the router: every block gives up after the wait's limit, the result stays
+    untouched, the error is raised once, and the next call is right."""
+    ops = _ops()
+    args = _moe_args(T)
+    want = ops.mxfp4_moe(*args)
+    out = torch.full_like(want, 7.0)
+    torch.cuda.synchronize()
+    control = ops.mxfp4._streams[(torch.cuda.current_device(), ops._stream())][0]
+    assert not control.any()
+    control[0] = -1
+    ops.mxfp4_moe(*args, out=out)
+    torch.cuda.synchronize()
+    with pytest.raises(ops.KernelError, match="wait"):
+        ops.check_tc_errors()
+    assert (out == 7).all() and not control.any()
+    assert torch.equal(ops.mxfp4_moe(*args), want)
+    ops.check_tc_errors()
