@@ -17,6 +17,7 @@ namespace prism {
 namespace mx {
 
 constexpr int BLOCK = 32, GROUP = 128, TILE_ROWS = 128, TILE_BYTES = 512;
+constexpr int WORKSPACE_TOO_SMALL = -1;        // an entry's answer before it launches anything
 
 __host__ __device__ __forceinline__ int groups_of(int K) { return (K + GROUP - 1) / GROUP; }
 

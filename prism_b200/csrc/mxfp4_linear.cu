@@ -587,10 +587,11 @@ PRISM_EXPORT int prism_mxfp4_linear_workspace(int M, int N, int K, int act_bits,
 }
 
 // x [M, K] bfloat16 (row stride ldx); codes, scales: W [N, K]; y [M, N] of `out_dtype` (row stride ldy); act_bits 16 or 4;
-// ws: workspace of the call (prism_mxfp4_linear_workspace), 256-byte aligned; counters: at least ceil(N / 128) ints (4,096 always
+// ws: workspace of the call, 256-byte aligned; nothing is launched and -1 returned where its ws_bytes are fewer than
+// prism_mxfp4_linear_workspace says on this device; counters: at least ceil(N / 128) ints (4,096 always
 // suffice), zero before the first launch (the kernel leaves them zero), of one stream's launches at a time
 PRISM_EXPORT int prism_mxfp4_linear(const void* x, long long ldx, const void* codes, const void* scales, const void* bias, int bias_dtype,
-                                    void* y, int out_dtype, long long ldy, int M, int N, int K, int act_bits, void* ws, int* counters, int* err,
+                                    void* y, int out_dtype, long long ldy, int M, int N, int K, int act_bits, void* ws, long long ws_bytes, int* counters, int* err,
                                     cudaStream_t stream) {
     using namespace prism;
     using namespace prism::mx;
@@ -599,6 +600,7 @@ PRISM_EXPORT int prism_mxfp4_linear(const void* x, long long ldx, const void* co
         return (int)cudaErrorInvalidValue;
     const Plan q = plan_for(M, N, K, act_bits);
     if (q.units * q.kb > 0x7fffffffLL) return (int)cudaErrorInvalidValue;
+    if (ws_bytes < q.bytes) return WORKSPACE_TOO_SMALL;
     uint8_t* base = static_cast<uint8_t*>(ws);
     const bool a16 = act_bits == 16;
     CUtensorMap mw, mx;

@@ -808,13 +808,14 @@ PRISM_EXPORT int prism_mxfp4_moe_workspace(int T, int H, int F, int E, int top, 
 }
 
 // x [T, H] bfloat16; router [E, H] (+ rbias [E]); gate, up [E, F, H] and down [E, H, F] in 4 bits; corr [E] or null.
-// ws: workspace of the call; control: 68 ints, zero before the first launch (the kernel leaves them zero), of one stream's
+// ws: workspace of the call; nothing is launched and -1 returned where its ws_bytes are too few; control: 68 ints, zero before the first launch (the kernel leaves them zero), of one stream's
 // launches at a time.  y [T, H] of `out_dtype` (row stride ldy).
 PRISM_EXPORT int prism_mxfp4_moe(const void* x, long long ldx, const void* router, int router_dtype, const void* rbias, int rbias_dtype,
                                  const void* gate_codes, const void* gate_scales, const void* up_codes, const void* up_scales,
                                  const void* down_codes, const void* down_scales, int T, int H, int F, int E, int top, int softmax, int renorm,
                                  int scale_in, int act, float limit, const void* corr, int corr_dtype, int groups, int keep, float wscale,
-                                 float sum_eps, void* y, int out_dtype, long long ldy, void* ws, int* control, int* err, cudaStream_t stream) {
+                                 float sum_eps, void* y, int out_dtype, long long ldy, void* ws, long long ws_bytes, int* control, int* err,
+                                 cudaStream_t stream) {
     using namespace prism;
     using namespace prism::mx;
     if (T <= 0) return 0;
@@ -822,6 +823,7 @@ PRISM_EXPORT int prism_mxfp4_moe(const void* x, long long ldx, const void* route
         (((uintptr_t)gate_scales | (uintptr_t)up_scales | (uintptr_t)down_scales) & 15) || ((uintptr_t)ws & 255))
         return (int)cudaErrorInvalidValue;
     const MoePlan q = moe_plan(T, H, F, E, top);
+    if (ws_bytes < q.bytes) return WORKSPACE_TOO_SMALL;
     const int g1 = groups_of(H), g2 = groups_of(F);
     uint8_t* base = static_cast<uint8_t*>(ws);
     CUtensorMap m[5];

@@ -112,17 +112,11 @@ def mxfp4_quantize(x: torch.Tensor) -> Mxfp4:
     return Mxfp4._of(codes, scales, shape)
 
 
-_workspace_bytes = {}
-
-
-def _workspace(size_of: str, *sizes: int) -> int:
-    n = _workspace_bytes.get((size_of,) + sizes)
-    if n is None:
-        b = ctypes.c_longlong()
-        if getattr(ops.lib(), size_of)(*sizes, ctypes.addressof(b)) != 0:
-            raise ops.KernelError(f"{size_of}: sizes {sizes} are not supported")
-        n = _workspace_bytes[(size_of,) + sizes] = b.value
-    return n
+def _workspace(size_of: str, sizes) -> int:
+    b = ctypes.c_longlong()
+    if getattr(ops.lib(), size_of)(*sizes, ctypes.addressof(b)) != 0:
+        raise ops.KernelError(f"{size_of}: sizes {sizes} are not supported")
+    return b.value
 
 
 _err_words = {}
@@ -138,15 +132,18 @@ def _err_word(device: torch.device) -> int:
 
 _COUNTERS = 4096             # of a stream: tiles of a product (csrc/mxfp4_linear.cu), or an experts' layer's control words
 _CONTROL = 68                # csrc/mxfp4_moe.cu: Control
+_TOO_SMALL = -1              # csrc/mxfp4.cuh: WORKSPACE_TOO_SMALL
 _SCRATCH = 16 << 20          # a larger workspace is the call's own
 _ARENA = 1 << 20
 _streams = {}                # (device, stream) -> [counters, workspace]: launches of one stream follow each other
 _arenas = {}                 # device -> [counters for captured calls, how many are given away]
 
 
-def _call_memory(stream: int, device: torch.device, nbytes: int, counters: int):
-    """``(workspace, counters)`` of a call.  Counters are zero before a launch and left so.  Under graph capture a call gets
-    counters of its own for good, as graphs may run on any stream, and a workspace of the graph's."""
+def _with_memory(launch, size_of: str, sizes, stream: int, device: torch.device, counters: int) -> int:
+    """``launch(workspace, its bytes, counters)`` with memory for the call; its answer.  It is asked to run in the stream's workspace at
+    once and says, before it launches anything, where that is too small: how much a call needs is for the device that it runs on to say.
+    Counters are zero before a launch and left so.  Under graph capture a call gets counters of its own for good, as graphs may
+    run on any stream, and a workspace of the graph's."""
     if torch._C._cuda_isCurrentStreamCapturing():
         arena = _arenas.get(device.index)
         counters = (counters + 63) // 64 * 64
@@ -155,18 +152,23 @@ def _call_memory(stream: int, device: torch.device, nbytes: int, counters: int):
         else:
             block = arena[0][arena[1]:arena[1] + counters]
             arena[1] += counters
-        return torch.empty(nbytes, dtype=torch.uint8, device=device), block
+        work = torch.empty(_workspace(size_of, sizes), dtype=torch.uint8, device=device)
+        return launch(work.data_ptr(), work.numel(), block.data_ptr())
     own = _streams.get((device.index, stream))
     if own is None:
         if device.index not in _arenas:
             _arenas[device.index] = [torch.zeros(_ARENA, dtype=torch.int32, device=device), 0]
             torch.cuda.current_stream(device).synchronize()      # captured calls of any stream find it cleared
-        own = _streams[(device.index, stream)] = [torch.zeros(_COUNTERS, dtype=torch.int32, device=device), None]
-    if nbytes > _SCRATCH:
-        return torch.empty(nbytes, dtype=torch.uint8, device=device), own[0]
-    if own[1] is None or own[1].numel() < nbytes:
-        own[1] = torch.empty(max(nbytes, 4 << 20), dtype=torch.uint8, device=device)
-    return own[1], own[0]
+        own = _streams[(device.index, stream)] = [torch.zeros(_COUNTERS, dtype=torch.int32, device=device),
+                                                  torch.empty(4 << 20, dtype=torch.uint8, device=device)]
+    work = own[1]
+    code = launch(work.data_ptr(), work.numel(), own[0].data_ptr())
+    if code == _TOO_SMALL:
+        work = torch.empty(_workspace(size_of, sizes), dtype=torch.uint8, device=device)
+        if work.numel() <= _SCRATCH:
+            own[1] = work
+        code = launch(work.data_ptr(), work.numel(), own[0].data_ptr())
+    return code
 
 
 def _clear_counters():
@@ -200,11 +202,14 @@ def mxfp4_linear(x: torch.Tensor, w: Mxfp4, bias: Optional[torch.Tensor] = None,
     if M == 0:
         return out
     stream = ops._stream()
-    work, counters = _call_memory(stream, x.device, _workspace("prism_mxfp4_linear_workspace", M, N, K, act_bits), min(-(-N // 128), _COUNTERS))
-    ops._check(ops.lib().prism_mxfp4_linear(x.data_ptr(), x.stride(0), w.codes.data_ptr(), w.scales.data_ptr(),
-                                            None if bias is None else bias.data_ptr(), 0 if bias is None else ops._dt(bias), out.data_ptr(),
-                                            ops._dt(out), out.stride(0), M, N, K, act_bits, work.data_ptr(), counters.data_ptr(),
-                                            _err_word(x.device), stream), "mxfp4_linear")
+    run = ops.lib().prism_mxfp4_linear
+
+    def launch(work, nbytes, counters):
+        return run(x.data_ptr(), x.stride(0), w.codes.data_ptr(), w.scales.data_ptr(), None if bias is None else bias.data_ptr(),
+                   0 if bias is None else ops._dt(bias), out.data_ptr(), ops._dt(out), out.stride(0), M, N, K, act_bits, work, nbytes, counters,
+                   _err_word(x.device), stream)
+    ops._check(_with_memory(launch, "prism_mxfp4_linear_workspace", (M, N, K, act_bits), stream, x.device, min(-(-N // 128), _COUNTERS)),
+               "mxfp4_linear")
     return out
 
 
@@ -250,12 +255,13 @@ def mxfp4_moe(x: torch.Tensor, router: torch.Tensor, gate: Mxfp4, up: Mxfp4, dow
     if T == 0:
         return out
     stream = ops._stream()
-    work, control = _call_memory(stream, x.device, _workspace("prism_mxfp4_moe_workspace", T, H, F, E, top), _CONTROL)
-    ops._check(ops.lib().prism_mxfp4_moe(x.data_ptr(), x.stride(0), router.data_ptr(), ops._dt(router),
-                                         None if router_bias is None else router_bias.data_ptr(), 0 if router_bias is None else ops._dt(router_bias),
-                                         gate.codes.data_ptr(), gate.scales.data_ptr(), up.codes.data_ptr(), up.scales.data_ptr(),
-                                         down.codes.data_ptr(), down.scales.data_ptr(), T, H, F, E, top, softmax, renorm, scale_input,
-                                         ops.MOE_ACTS[act], limit, None if corr is None else corr.data_ptr(), 0 if corr is None else ops._dt(corr),
-                                         ch.groups, ch.keep, ch.scale, ch.sum_eps, out.data_ptr(), ops._dt(out), out.stride(0), work.data_ptr(),
-                                         control.data_ptr(), _err_word(x.device), stream), "mxfp4_moe")
+    run = ops.lib().prism_mxfp4_moe
+
+    def launch(work, nbytes, control):
+        return run(x.data_ptr(), x.stride(0), router.data_ptr(), ops._dt(router), None if router_bias is None else router_bias.data_ptr(),
+                   0 if router_bias is None else ops._dt(router_bias), gate.codes.data_ptr(), gate.scales.data_ptr(), up.codes.data_ptr(),
+                   up.scales.data_ptr(), down.codes.data_ptr(), down.scales.data_ptr(), T, H, F, E, top, softmax, renorm, scale_input,
+                   ops.MOE_ACTS[act], limit, None if corr is None else corr.data_ptr(), 0 if corr is None else ops._dt(corr), ch.groups, ch.keep,
+                   ch.scale, ch.sum_eps, out.data_ptr(), ops._dt(out), out.stride(0), work, nbytes, control, _err_word(x.device), stream)
+    ops._check(_with_memory(launch, "prism_mxfp4_moe_workspace", (T, H, F, E, top), stream, x.device, _CONTROL), "mxfp4_moe")
     return out

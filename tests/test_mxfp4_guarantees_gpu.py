@@ -1,7 +1,9 @@
 """What the 4-bit operators promise beyond their values at ordinary inputs: how far an expert's hidden values are held; that a
-wait that runs out is an error and nothing else.
+wait that runs out is an error and nothing else; that no kernel runs in a workspace that is too small for it.
 
 Tolerances.  A product's float32 sum is within 2^-18 of the sum of |x w| of the 64-bit one (``test_mxfp4_gpu``)."""
+
+import ctypes
 
 import pytest
 import torch
@@ -66,3 +68,39 @@ def test_a_wait_that_runs_out_leaves_no_result_and_no_trace(T):
     assert (out == 7).all() and not control.any()
     assert torch.equal(ops.mxfp4_moe(*args), want)
     ops.check_tc_errors()
+
+
+@pytest.mark.parametrize("M,act_bits", [(1, 16), (8, 4), (40, 16), (300, 4), (300, 16)])
+def test_a_product_s_workspace_that_is_too_small_is_refused(M, act_bits):
+    ops = _ops()
+    N, K = 700, 2000
+    x, w, out = _acts(M, K, 1), ops.mxfp4_quantize(_acts(N, K, 2)), torch.full((M, N), 7.0, device=DEV)
+    need = ctypes.c_longlong()
+    assert ops.lib().prism_mxfp4_linear_workspace(M, N, K, act_bits, ctypes.addressof(need)) == 0
+    work, counters = torch.empty(need.value, dtype=torch.uint8, device=DEV), torch.zeros(4096, dtype=torch.int32, device=DEV)
+
+    def call(nbytes):
+        return ops.lib().prism_mxfp4_linear(x.data_ptr(), K, w.codes.data_ptr(), w.scales.data_ptr(), None, 0, out.data_ptr(), ops.F32, N, M, N, K, act_bits,
+                                            work.data_ptr(), nbytes, counters.data_ptr(), ops._tc_err_word(x.device).data_ptr(), ops._stream())
+    assert call(need.value - 1) == call(0) == -1
+    torch.cuda.synchronize()
+    assert (out == 7).all()
+    assert call(need.value) == 0
+    assert torch.equal(out, ops.mxfp4_linear(x, w, out_dtype=torch.float32, act_bits=act_bits))
+
+
+def test_workspaces_grow_with_the_calls():
+    """A stream's first call is small and a later one needs more than the stream has, or more than it keeps."""
+    ops = _ops()
+    side = torch.cuda.Stream()
+    for M, N, K in ((1, 200, 300), (400, 2100, 1200), (2048, 1024, 8192), (1, 200, 300)):
+        x, w = _acts(M, K, 1), ops.mxfp4_quantize(_acts(N, K, 2))
+        want = ops.mxfp4_linear(x, w)
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            got = ops.mxfp4_linear(x, w)
+        torch.cuda.current_stream().wait_stream(side)
+        assert torch.equal(got, want)
+        assert all(own[1].numel() <= ops.mxfp4._SCRATCH for own in ops.mxfp4._streams.values())
+    args = _moe_args(64, 2048, 1024, 8)
+    assert torch.equal(ops.mxfp4_moe(*args), ops.mxfp4_moe(*args))
