@@ -31,6 +31,7 @@
 #include "mxfp4_mma.cuh"
 #include "vec.cuh"
 
+#include <algorithm>
 #include <climits>
 
 namespace prism {
@@ -194,8 +195,8 @@ __device__ __forceinline__ void choose(const Moe& p, int t, const float* z) {   
 }
 
 // 1: logits, choices, x's terms.  A CTA has all logits of a token, or, where a router's rows are too many for that, `dots`
-// neighbouring ones (of one token or two), and the CTA that finishes a token's makes its choice.  Several warps share a row where
-// there are few.
+// neighbouring ones (no more than E: of one token or two), and the CTA that finishes a token's makes its choice.  Several warps
+// share a row where there are few.
 template <typename C> __device__ __forceinline__ void moe_route_and_terms(const Moe& p, float* scratch) {
     __shared__ int finished[2];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, back = gridDim.x - 1 - blockIdx.x;
@@ -211,81 +212,86 @@ template <typename C> __device__ __forceinline__ void moe_route_and_terms(const 
         }
         fence_async();                                         // the terms are read by TMA, of all CTAs
     }
-    const int first = blockIdx.x * p.dots, count = min(p.dots, p.T * p.E - first);
-    if (count <= 0) return;
     const int parts = p.dots >= MOE_WARPS ? 1 : MOE_WARPS / p.dots, at_once = MOE_WARPS / parts, part = warp % parts;
     const int len = ((p.H + parts - 1) / parts + 7) / 8 * 8, k0 = part * len, k1 = min(p.H, k0 + len);
     const bool wide = p.wide && p.H % 8 == 0, whole = p.dots == p.E;
+    // once for most CTAs; where there are more tokens than CTAs, several times
 #pragma unroll 1
-    for (int i = warp / parts; i < count; i += at_once) {
-        const int t = (first + i) / p.E, e = first + i - t * p.E;
-        const __nv_bfloat16* row = p.x + (long long)t * p.ldx;
-        float sum = 0.f;
-        if (wide && p.router_bf16) {
-            const __nv_bfloat16* r = static_cast<const __nv_bfloat16*>(p.router) + (size_t)e * p.H;
+    for (int first = blockIdx.x * p.dots; first < p.T * p.E; first += gridDim.x * p.dots) {
+        const int count = min(p.dots, p.T * p.E - first);
+        if (first != blockIdx.x * p.dots) __syncthreads();     // the scratch has been read
 #pragma unroll 1
-            for (int k = k0 + lane * 8; k < k1; k += 8 * 256) {              // eight pieces of either row on their way at once
-                uint4 a[8], w[8];
+        for (int i = warp / parts; i < count; i += at_once) {
+            const int t = (first + i) / p.E, e = first + i - t * p.E;
+            const __nv_bfloat16* row = p.x + (long long)t * p.ldx;
+            float sum = 0.f;
+            if (wide && p.router_bf16) {
+                const __nv_bfloat16* r = static_cast<const __nv_bfloat16*>(p.router) + (size_t)e * p.H;
+#pragma unroll 1
+                for (int k = k0 + lane * 8; k < k1; k += 8 * 256) {              // eight pieces of either row on their way at once
+                    uint4 a[8], w[8];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const int at = k + j * 256;
-                    a[j] = at < k1 ? *reinterpret_cast<const uint4*>(row + at) : make_uint4(0, 0, 0, 0);
-                    w[j] = at < k1 ? *reinterpret_cast<const uint4*>(r + at) : make_uint4(0, 0, 0, 0);
-                }
-#pragma unroll
-                for (int j = 0; j < 8; ++j)
-#pragma unroll
-                    for (int l = 0; l < 4; ++l) {
-                        const float2 f = __bfloat1622float2(reinterpret_cast<const __nv_bfloat162*>(&a[j])[l]);
-                        const float2 g = __bfloat1622float2(reinterpret_cast<const __nv_bfloat162*>(&w[j])[l]);
-                        sum = fmaf(f.x, g.x, sum);
-                        sum = fmaf(f.y, g.y, sum);
+                    for (int j = 0; j < 8; ++j) {
+                        const int at = k + j * 256;
+                        a[j] = at < k1 ? *reinterpret_cast<const uint4*>(row + at) : make_uint4(0, 0, 0, 0);
+                        w[j] = at < k1 ? *reinterpret_cast<const uint4*>(r + at) : make_uint4(0, 0, 0, 0);
                     }
-            }
-        } else {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+#pragma unroll
+                        for (int l = 0; l < 4; ++l) {
+                            const float2 f = __bfloat1622float2(reinterpret_cast<const __nv_bfloat162*>(&a[j])[l]);
+                            const float2 g = __bfloat1622float2(reinterpret_cast<const __nv_bfloat162*>(&w[j])[l]);
+                            sum = fmaf(f.x, g.x, sum);
+                            sum = fmaf(f.y, g.y, sum);
+                        }
+                }
+            } else {
 #pragma unroll 8
-            for (int k = k0 + lane; k < k1; k += 32) sum = fmaf(to_float(row[k]), load_param(p.router, p.router_bf16, (size_t)e * p.H + k), sum);
-        }
-        sum = warp_sum(sum);
-        if (lane == 0) scratch[i * parts + part] = sum;
-    }
-    __syncthreads();
-    float* zs = scratch + p.dots * parts;                      // the logits, of a token or (then for two warps) of two
-    for (int i = threadIdx.x; i < count; i += MOE_THREADS) {
-        const int t = (first + i) / p.E, e = first + i - t * p.E;
-        float sum = p.rbias != nullptr ? load_param(p.rbias, p.rbias_bf16, e) : 0.f;
-        for (int j = 0; j < parts; ++j) sum += scratch[i * parts + j];
-        if (whole) zs[i] = sum;
-        else p.z[first + i] = sum;
-    }
-    __syncthreads();
-    const int t0 = first / p.E, t1 = (first + count - 1) / p.E;             // no more than E logits: two tokens at most
-    if (!whole) {
-        if (threadIdx.x < 2) {
-            const int t = t0 + threadIdx.x;
-            finished[threadIdx.x] = 0;
-            if (t <= t1) {
-                const int here = min(first + count, (t + 1) * p.E) - max(first, t * p.E);
-                finished[threadIdx.x] = add_acq_rel(&p.control[TOKEN + t], here) == p.E - here;
+                for (int k = k0 + lane; k < k1; k += 32) sum = fmaf(to_float(row[k]), load_param(p.router, p.router_bf16, (size_t)e * p.H + k), sum);
             }
+            sum = warp_sum(sum);
+            if (lane == 0) scratch[i * parts + part] = sum;
         }
         __syncthreads();
-    }
-    if (warp >= 2 || (whole ? warp > 0 : !finished[warp])) return;
-    const int t = t0 + warp;
-    zs += warp * (4 * p.E + 2 * p.groups_of_experts + 16);
-    if (!whole) {
-        for (int e = lane; e < p.E; e += 32) zs[e] = __ldcg(p.z + t * p.E + e);
-        __syncwarp();
-    }
-    if (p.groups_of_experts > 1 && p.keep < p.groups_of_experts) {
-        int* counts = reinterpret_cast<int*>(zs + 3 * p.E + 2 * p.groups_of_experts);
-        for (int e = lane; e < p.E; e += 32) counts[e] = 0;
-        __syncwarp();
-        moe_route_token(zs, zs + p.E, zs + 2 * p.E, zs + 3 * p.E, p.E, p.top, p.softmax, p.renorm, lane, counts, p.sel_e + t * p.top,
-                        p.sel_w + t * p.top, counts + p.E, p.corr, p.corr_bf16, p.groups_of_experts, p.keep, p.wscale, p.sum_eps);
-    } else {
-        choose(p, t, zs);
+        float* zs = scratch + p.dots * parts;                      // the logits, of a token or (then for two warps) of two
+        for (int i = threadIdx.x; i < count; i += MOE_THREADS) {
+            const int t = (first + i) / p.E, e = first + i - t * p.E;
+            float sum = p.rbias != nullptr ? load_param(p.rbias, p.rbias_bf16, e) : 0.f;
+            for (int j = 0; j < parts; ++j) sum += scratch[i * parts + j];
+            if (whole) zs[i] = sum;
+            else p.z[first + i] = sum;
+        }
+        __syncthreads();
+        const int t0 = first / p.E, t1 = (first + count - 1) / p.E;             // no more than E logits: two tokens at most
+        if (!whole) {
+            if (threadIdx.x < 2) {
+                const int t = t0 + threadIdx.x;
+                finished[threadIdx.x] = 0;
+                if (t <= t1) {
+                    const int here = min(first + count, (t + 1) * p.E) - max(first, t * p.E);
+                    finished[threadIdx.x] = add_acq_rel(&p.control[TOKEN + t], here) == p.E - here;
+                }
+            }
+            __syncthreads();
+        }
+        if (warp < 2 && (whole ? warp == 0 : finished[warp] != 0)) {
+            const int t = t0 + warp;
+            float* s = zs + warp * (4 * p.E + 2 * p.groups_of_experts + 16);
+            if (!whole) {
+                for (int e = lane; e < p.E; e += 32) s[e] = __ldcg(p.z + t * p.E + e);
+                __syncwarp();
+            }
+            if (p.groups_of_experts > 1 && p.keep < p.groups_of_experts) {
+                int* counts = reinterpret_cast<int*>(s + 3 * p.E + 2 * p.groups_of_experts);
+                for (int e = lane; e < p.E; e += 32) counts[e] = 0;
+                __syncwarp();
+                moe_route_token(s, s + p.E, s + 2 * p.E, s + 3 * p.E, p.E, p.top, p.softmax, p.renorm, lane, counts, p.sel_e + t * p.top,
+                                p.sel_w + t * p.top, counts + p.E, p.corr, p.corr_bf16, p.groups_of_experts, p.keep, p.wscale, p.sum_eps);
+            } else {
+                choose(p, t, s);
+            }
+        }
     }
 }
 
@@ -749,10 +755,11 @@ struct MoePlan {
     bool compact;
     long long xt, xs, h, hs, z, sel_e, sel_w, part1, part2, planes, counters, bytes;
 };
-inline MoePlan moe_plan(int T, int H, int F, int E, int top) {
+// ctas: at most so many (0: one an SM)
+inline MoePlan moe_plan(int T, int H, int F, int E, int top, int ctas) {
     MoePlan q;
     q.tt = T <= 8 ? 8 : T <= 16 ? 16 : T <= 32 ? 32 : 64;
-    q.P = sm_count();
+    q.P = ctas > 0 && ctas < sm_count() ? ctas : sm_count();
     q.most_live = E < T * top ? E : T * top;
     q.most_rows = 3 * (T * top + 7 * q.most_live);
     const long long g1 = groups_of(H), g2 = groups_of(F), tiles2 = ((H + 127) / 128 + 1) / 2;
@@ -801,20 +808,20 @@ template <typename C> int run_moe(const CUtensorMap (&m)[5], const Moe& p, int P
 }  // namespace prism
 
 // bytes of workspace that prism_mxfp4_moe needs for these sizes, into *bytes
-PRISM_EXPORT int prism_mxfp4_moe_workspace(int T, int H, int F, int E, int top, long long* bytes) {
+PRISM_EXPORT int prism_mxfp4_moe_workspace(int T, int H, int F, int E, int top, int ctas, long long* bytes) {
     if (!prism::mx::moe_sizes_ok(T, H, F, E, top)) return (int)cudaErrorInvalidValue;
-    *bytes = prism::mx::moe_plan(T, H, F, E, top).bytes;
+    *bytes = prism::mx::moe_plan(T, H, F, E, top, ctas).bytes;
     return 0;
 }
 
 // x [T, H] bfloat16; router [E, H] (+ rbias [E]); gate, up [E, F, H] and down [E, H, F] in 4 bits; corr [E] or null.
-// ws: workspace of the call; nothing is launched and -1 returned where its ws_bytes are too few; control: 68 ints, zero before the first launch (the kernel leaves them zero), of one stream's
-// launches at a time.  y [T, H] of `out_dtype` (row stride ldy).
+// ws: workspace of the call; nothing is launched and -1 returned where its ws_bytes are too few; control: 68 ints, zero before the
+// first launch (the kernel leaves them zero), of one stream's launches at a time.  y [T, H] of `out_dtype` (row stride ldy).  ctas: at most so many share the work (0: one an SM).
 PRISM_EXPORT int prism_mxfp4_moe(const void* x, long long ldx, const void* router, int router_dtype, const void* rbias, int rbias_dtype,
                                  const void* gate_codes, const void* gate_scales, const void* up_codes, const void* up_scales,
                                  const void* down_codes, const void* down_scales, int T, int H, int F, int E, int top, int softmax, int renorm,
                                  int scale_in, int act, float limit, const void* corr, int corr_dtype, int groups, int keep, float wscale,
-                                 float sum_eps, void* y, int out_dtype, long long ldy, void* ws, long long ws_bytes, int* control, int* err,
+                                 float sum_eps, void* y, int out_dtype, long long ldy, int ctas, void* ws, long long ws_bytes, int* control, int* err,
                                  cudaStream_t stream) {
     using namespace prism;
     using namespace prism::mx;
@@ -822,7 +829,7 @@ PRISM_EXPORT int prism_mxfp4_moe(const void* x, long long ldx, const void* route
     if (!moe_sizes_ok(T, H, F, E, top) || groups < 1 || groups > E || (((uintptr_t)gate_codes | (uintptr_t)up_codes | (uintptr_t)down_codes) & 31) ||
         (((uintptr_t)gate_scales | (uintptr_t)up_scales | (uintptr_t)down_scales) & 15) || ((uintptr_t)ws & 255))
         return (int)cudaErrorInvalidValue;
-    const MoePlan q = moe_plan(T, H, F, E, top);
+    const MoePlan q = moe_plan(T, H, F, E, top, ctas);
     if (ws_bytes < q.bytes) return WORKSPACE_TOO_SMALL;
     const int g1 = groups_of(H), g2 = groups_of(F);
     uint8_t* base = static_cast<uint8_t*>(ws);
@@ -855,7 +862,7 @@ PRISM_EXPORT int prism_mxfp4_moe(const void* x, long long ldx, const void* route
     p.groups_of_experts = groups, p.keep = keep;
     // a token's logits in one CTA save a pass through memory (1 token, 8 experts of 2,048: 1.1 us) while there is a warp for each of
     // them and their rows are not long for one SM (64 experts: 9.7 us over all SMs, 11.6 a token an SM)
-    p.dots = E <= MOE_WARPS && (long long)E * H <= (1 << 18) && T <= q.P ? E : (T * E + q.P - 1) / q.P;
+    p.dots = E <= MOE_WARPS && (long long)E * H <= (1 << 18) && T <= q.P ? E : std::min(E, (T * E + q.P - 1) / q.P);
     p.most_live = q.most_live;
     p.ncounters = q.ncounters;
     p.router_bf16 = router_dtype == PRISM_DTYPE_BF16, p.rbias_bf16 = rbias_dtype == PRISM_DTYPE_BF16, p.corr_bf16 = corr_dtype == PRISM_DTYPE_BF16;

@@ -162,8 +162,8 @@ class _Sig:
     prism_mxfp4_linear = [_p, _ll, _p, _p, _p, _i, _p, _i, _ll, _i, _i, _i, _i, _p, _ll, _p, _p, _p]
     prism_mxfp4_linear_workspace = [_i, _i, _i, _i, _p]
     prism_mxfp4_moe = [_p, _ll, _p, _i, _p, _i, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _i, _i, _i, _f, _p, _i, _i, _i, _f, _f,
-                       _p, _i, _ll, _p, _ll, _p, _p, _p]
-    prism_mxfp4_moe_workspace = [_i, _i, _i, _i, _i, _p]
+                       _p, _i, _ll, _i, _p, _ll, _p, _p, _p]
+    prism_mxfp4_moe_workspace = [_i, _i, _i, _i, _i, _i, _p]
     prism_sgemm_nt = [_p, _i, _p, _i, _p, _i, _p, _i, _i, _i, _i, _p]
     prism_sample = [_p, _i, _i, _i, _p, _p, _p, _p]
     prism_argmax_split = [_p, _i, _i, _i, _i, _p, _p, _p, _p, _p]

@@ -21,6 +21,7 @@ from .. import ops
 BLOCK, GROUP, TILE_ROWS, TILE_BYTES = 32, 128, 128, 512      # csrc/mxfp4.cuh
 MOE_TOKENS, MOE_EXPERTS, MOE_TOP = 64, 256, 16               # the most of an ``mxfp4_moe`` call
 DTYPE = "mxfp4"
+MOE_CTAS = 0                # at most so many blocks share an ``mxfp4_moe`` call; 0: one an SM
 
 
 class Mxfp4:
@@ -262,6 +263,6 @@ def mxfp4_moe(x: torch.Tensor, router: torch.Tensor, gate: Mxfp4, up: Mxfp4, dow
                    0 if router_bias is None else ops._dt(router_bias), gate.codes.data_ptr(), gate.scales.data_ptr(), up.codes.data_ptr(),
                    up.scales.data_ptr(), down.codes.data_ptr(), down.scales.data_ptr(), T, H, F, E, top, softmax, renorm, scale_input,
                    ops.MOE_ACTS[act], limit, None if corr is None else corr.data_ptr(), 0 if corr is None else ops._dt(corr), ch.groups, ch.keep,
-                   ch.scale, ch.sum_eps, out.data_ptr(), ops._dt(out), out.stride(0), work, nbytes, control, _err_word(x.device), stream)
-    ops._check(_with_memory(launch, "prism_mxfp4_moe_workspace", (T, H, F, E, top), stream, x.device, _CONTROL), "mxfp4_moe")
+                   ch.scale, ch.sum_eps, out.data_ptr(), ops._dt(out), out.stride(0), MOE_CTAS, work, nbytes, control, _err_word(x.device), stream)
+    ops._check(_with_memory(launch, "prism_mxfp4_moe_workspace", (T, H, F, E, top, MOE_CTAS), stream, x.device, _CONTROL), "mxfp4_moe")
     return out

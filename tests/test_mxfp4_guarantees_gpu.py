@@ -1,5 +1,6 @@
 """What the 4-bit operators promise beyond their values at ordinary inputs: how far an expert's hidden values are held; that a
-wait that runs out is an error and nothing else; that no kernel runs in a workspace that is too small for it.
+wait that runs out is an error and nothing else; that no kernel runs in a workspace that is too small for it; that an experts' layer is right on any
+number of SMs.
 
 Tolerances.  A product's float32 sum is within 2^-18 of the sum of |x w| of the 64-bit one (``test_mxfp4_gpu``)."""
 
@@ -8,7 +9,7 @@ import ctypes
 import pytest
 import torch
 
-from test_mxfp4_gpu import DEV, _acts, _experts, _gen, _ops, decode
+from test_mxfp4_gpu import DEV, _acts, _experts, _gen, _ops, decode, plain_moe
 
 pytestmark = pytest.mark.gpu
 
@@ -104,3 +105,23 @@ def test_workspaces_grow_with_the_calls():
         assert all(own[1].numel() <= ops.mxfp4._SCRATCH for own in ops.mxfp4._streams.values())
     args = _moe_args(64, 2048, 1024, 8)
     assert torch.equal(ops.mxfp4_moe(*args), ops.mxfp4_moe(*args))
+
+
+@pytest.mark.parametrize("ctas", [1, 5, 16, 60])
+@pytest.mark.parametrize("T,E,F,H,top", [(64, 40, 40, 200, 3), (64, 6, 70, 256, 2), (33, 1, 33, 96, 1), (7, 9, 200, 130, 4)])
+def test_fewer_blocks_than_tokens_choose_for_every_token(ctas, T, E, F, H, top, monkeypatch):
+    """As on a part of a GPU: a block then has the logits of more than two tokens, one share after another."""
+    ops = _ops()
+    x, router = _acts(T, H, T), (_acts(E, H, 4) * H ** -0.5).to(torch.bfloat16)
+    gate, up, down = _experts(E, F, H, 2)
+    dv = [decode(w).to(DEV) for w in (gate, up, down)]
+    want, bound = plain_moe(x, router, *dv, top, True, True, False)
+    monkeypatch.setattr(ops.mxfp4, "MOE_CTAS", ctas)
+    got = ops.mxfp4_moe(x, router, gate, up, down, top, True, True, False, out_dtype=torch.float32)
+    ops.check_tc_errors()
+    assert ((got.double() - want).abs() <= bound * 2.0 ** -8).all()
+    choice = ops.MoeChoice(None, 2, 1) if E % 2 == 0 and E // 2 >= top else None
+    if choice is not None:
+        want, bound = plain_moe(x, router, *dv, top, False, False, True, choice=choice)
+        got = ops.mxfp4_moe(x, router, gate, up, down, top, False, False, True, choice=choice, out_dtype=torch.float32)
+        assert ((got.double() - want).abs() <= bound * 2.0 ** -8).all()
