@@ -590,9 +590,9 @@ PRISM_EXPORT int prism_mxfp4_linear_workspace(int M, int N, int K, int act_bits,
 // ws: workspace of the call, 256-byte aligned; nothing is launched and -1 returned where its ws_bytes are fewer than
 // prism_mxfp4_linear_workspace says on this device; counters: at least ceil(N / 128) ints (4,096 always
 // suffice), zero before the first launch (the kernel leaves them zero), of one stream's launches at a time
-PRISM_EXPORT int prism_mxfp4_linear(const void* x, long long ldx, const void* codes, const void* scales, const void* bias, int bias_dtype,
-                                    void* y, int out_dtype, long long ldy, int M, int N, int K, int act_bits, void* ws, long long ws_bytes, int* counters, int* err,
-                                    cudaStream_t stream) {
+PRISM_EXPORT int prism_mxfp4_linear(void* ws, long long ws_bytes, int* counters, const void* x, long long ldx, const void* codes, const void* scales,
+                                    const void* bias, int bias_dtype, void* y, int out_dtype, long long ldy, int M, int N, int K, int act_bits,
+                                    int* err, cudaStream_t stream) {
     using namespace prism;
     using namespace prism::mx;
     if (M <= 0 || N <= 0) return 0;

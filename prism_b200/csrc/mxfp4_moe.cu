@@ -817,12 +817,12 @@ PRISM_EXPORT int prism_mxfp4_moe_workspace(int T, int H, int F, int E, int top, 
 // x [T, H] bfloat16; router [E, H] (+ rbias [E]); gate, up [E, F, H] and down [E, H, F] in 4 bits; corr [E] or null.
 // ws: workspace of the call; nothing is launched and -1 returned where its ws_bytes are too few; control: 68 ints, zero before the
 // first launch (the kernel leaves them zero), of one stream's launches at a time.  y [T, H] of `out_dtype` (row stride ldy).  ctas: at most so many share the work (0: one an SM).
-PRISM_EXPORT int prism_mxfp4_moe(const void* x, long long ldx, const void* router, int router_dtype, const void* rbias, int rbias_dtype,
+PRISM_EXPORT int prism_mxfp4_moe(void* ws, long long ws_bytes, int* control, const void* x, long long ldx, const void* router, int router_dtype,
+                                 const void* rbias, int rbias_dtype,
                                  const void* gate_codes, const void* gate_scales, const void* up_codes, const void* up_scales,
                                  const void* down_codes, const void* down_scales, int T, int H, int F, int E, int top, int softmax, int renorm,
                                  int scale_in, int act, float limit, const void* corr, int corr_dtype, int groups, int keep, float wscale,
-                                 float sum_eps, void* y, int out_dtype, long long ldy, int ctas, void* ws, long long ws_bytes, int* control, int* err,
-                                 cudaStream_t stream) {
+                                 float sum_eps, void* y, int out_dtype, long long ldy, int ctas, int* err, cudaStream_t stream) {
     using namespace prism;
     using namespace prism::mx;
     if (T <= 0) return 0;

@@ -159,10 +159,10 @@ class _Sig:
     prism_swiglu = [_p, _p, _i, _i, _i, _p]
     prism_mxfp4_quantize = [_p, _i, _ll, _i, _i, _i, _p, _p, _p]
     prism_mxfp4_dequantize = [_p, _p, _i, _i, _i, _p, _ll, _i, _p]
-    prism_mxfp4_linear = [_p, _ll, _p, _p, _p, _i, _p, _i, _ll, _i, _i, _i, _i, _p, _ll, _p, _p, _p]
+    prism_mxfp4_linear = [_p, _ll, _p, _p, _ll, _p, _p, _p, _i, _p, _i, _ll, _i, _i, _i, _i, _p, _p]
     prism_mxfp4_linear_workspace = [_i, _i, _i, _i, _p]
-    prism_mxfp4_moe = [_p, _ll, _p, _i, _p, _i, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _i, _i, _i, _f, _p, _i, _i, _i, _f, _f,
-                       _p, _i, _ll, _i, _p, _ll, _p, _p, _p]
+    prism_mxfp4_moe = [_p, _ll, _p, _p, _ll, _p, _i, _p, _i, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _i, _i, _i, _f, _p, _i, _i, _i, _f, _f,
+                       _p, _i, _ll, _i, _p, _p]
     prism_mxfp4_moe_workspace = [_i, _i, _i, _i, _i, _i, _p]
     prism_sgemm_nt = [_p, _i, _p, _i, _p, _i, _p, _i, _i, _i, _i, _p]
     prism_sample = [_p, _i, _i, _i, _p, _p, _p, _p]

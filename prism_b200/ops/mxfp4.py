@@ -12,6 +12,7 @@ file, engine/weight_pool.py:46-70).
 from __future__ import annotations
 
 import ctypes
+import threading
 from typing import Optional
 
 import torch
@@ -136,47 +137,62 @@ _CONTROL = 68                # csrc/mxfp4_moe.cu: Control
 _TOO_SMALL = -1              # csrc/mxfp4.cuh: WORKSPACE_TOO_SMALL
 _SCRATCH = 16 << 20          # a larger workspace is the call's own
 _ARENA = 1 << 20
-_streams = {}                # (device, stream) -> [counters, workspace]: launches of one stream follow each other
+_streams = {}                # (device, stream) -> _Own: launches of one stream follow each other
+_memory = threading.Lock()   # held from the choice of a call's memory until its last launch is on its way: threads share streams
 _arenas = {}                 # device -> [counters for captured calls, how many are given away]
 
 
-def _with_memory(launch, size_of: str, sizes, stream: int, device: torch.device, counters: int) -> int:
-    """``launch(workspace, its bytes, counters)`` with memory for the call; its answer.  It is asked to run in the stream's workspace at
-    once and says, before it launches anything, where that is too small: how much a call needs is for the device that it runs on to say.
-    Counters are zero before a launch and left so.  Under graph capture a call gets counters of its own for good, as graphs may
-    run on any stream, and a workspace of the graph's."""
-    if torch._C._cuda_isCurrentStreamCapturing():
-        arena = _arenas.get(device.index)
-        counters = (counters + 63) // 64 * 64
-        if arena is None or arena[1] + counters > _ARENA:
-            block = torch.zeros(counters, dtype=torch.int32, device=device)            # cleared by the graph
-        else:
-            block = arena[0][arena[1]:arena[1] + counters]
-            arena[1] += counters
-        work = torch.empty(_workspace(size_of, sizes), dtype=torch.uint8, device=device)
-        return launch(work.data_ptr(), work.numel(), block.data_ptr())
-    own = _streams.get((device.index, stream))
-    if own is None:
-        if device.index not in _arenas:
-            _arenas[device.index] = [torch.zeros(_ARENA, dtype=torch.int32, device=device), 0]
-            torch.cuda.current_stream(device).synchronize()      # captured calls of any stream find it cleared
-        own = _streams[(device.index, stream)] = [torch.zeros(_COUNTERS, dtype=torch.int32, device=device),
-                                                  torch.empty(4 << 20, dtype=torch.uint8, device=device)]
-    work = own[1]
-    code = launch(work.data_ptr(), work.numel(), own[0].data_ptr())
-    if code == _TOO_SMALL:
-        work = torch.empty(_workspace(size_of, sizes), dtype=torch.uint8, device=device)
-        if work.numel() <= _SCRATCH:
-            own[1] = work
-        code = launch(work.data_ptr(), work.numel(), own[0].data_ptr())
-    return code
+class _Own:
+    """A stream's counters and workspace, and where they are."""
+
+    __slots__ = ("counters", "work", "at")
+
+    def __init__(self, counters: torch.Tensor, work: torch.Tensor):
+        self.counters = counters
+        self.use(work)
+
+    def use(self, work: torch.Tensor) -> None:
+        self.work, self.at = work, (work.data_ptr(), work.numel(), self.counters.data_ptr())
+
+
+def _with_memory(run, args, size_of: str, sizes, stream: int, device: torch.device, counters: int) -> int:
+    """``run(workspace, its bytes, counters, *args)`` with memory that no other thread's call has meanwhile; its answer.  It is asked to
+    run in the stream's workspace at once and says, before it launches anything, where that is too small: how much a call needs is
+    for the device that it runs on to say.  Counters are zero before a launch and left so.  Under graph capture a call gets
+    counters of its own for good, as graphs may run on any stream, and a workspace of the graph's."""
+    with _memory:
+        if torch._C._cuda_isCurrentStreamCapturing():
+            arena = _arenas.get(device.index)
+            counters = (counters + 63) // 64 * 64
+            if arena is None or arena[1] + counters > _ARENA:
+                block = torch.zeros(counters, dtype=torch.int32, device=device)            # cleared by the graph
+            else:
+                block = arena[0][arena[1]:arena[1] + counters]
+                arena[1] += counters
+            work = torch.empty(_workspace(size_of, sizes), dtype=torch.uint8, device=device)
+            return run(work.data_ptr(), work.numel(), block.data_ptr(), *args)
+        own = _streams.get((device.index, stream))
+        if own is None:
+            if device.index not in _arenas:
+                _arenas[device.index] = [torch.zeros(_ARENA, dtype=torch.int32, device=device), 0]
+                torch.cuda.current_stream(device).synchronize()      # captured calls of any stream find it cleared
+            own = _streams[(device.index, stream)] = _Own(torch.zeros(_COUNTERS, dtype=torch.int32, device=device),
+                                                          torch.empty(4 << 20, dtype=torch.uint8, device=device))
+        code = run(*own.at, *args)
+        if code == _TOO_SMALL:
+            work = torch.empty(_workspace(size_of, sizes), dtype=torch.uint8, device=device)
+            if work.numel() <= _SCRATCH:
+                own.use(work)
+            code = run(work.data_ptr(), work.numel(), own.at[2], *args)
+        return code
 
 
 def _clear_counters():
     """After a launch that gave up its counters may be anything (``ops.check_tc_errors``, which has waited for the device)."""
-    for block in list(_streams.values()) + list(_arenas.values()):
-        block[0].zero_()
-    torch.cuda.synchronize()
+    with _memory:
+        for block in [own.counters for own in _streams.values()] + [arena[0] for arena in _arenas.values()]:
+            block.zero_()
+        torch.cuda.synchronize()
 
 
 def mxfp4_linear(x: torch.Tensor, w: Mxfp4, bias: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
@@ -203,14 +219,10 @@ def mxfp4_linear(x: torch.Tensor, w: Mxfp4, bias: Optional[torch.Tensor] = None,
     if M == 0:
         return out
     stream = ops._stream()
-    run = ops.lib().prism_mxfp4_linear
-
-    def launch(work, nbytes, counters):
-        return run(x.data_ptr(), x.stride(0), w.codes.data_ptr(), w.scales.data_ptr(), None if bias is None else bias.data_ptr(),
-                   0 if bias is None else ops._dt(bias), out.data_ptr(), ops._dt(out), out.stride(0), M, N, K, act_bits, work, nbytes, counters,
-                   _err_word(x.device), stream)
-    ops._check(_with_memory(launch, "prism_mxfp4_linear_workspace", (M, N, K, act_bits), stream, x.device, min(-(-N // 128), _COUNTERS)),
-               "mxfp4_linear")
+    args = (x.data_ptr(), x.stride(0), w.codes.data_ptr(), w.scales.data_ptr(), None if bias is None else bias.data_ptr(),
+            0 if bias is None else ops._dt(bias), out.data_ptr(), ops._dt(out), out.stride(0), M, N, K, act_bits, _err_word(x.device), stream)
+    ops._check(_with_memory(ops.lib().prism_mxfp4_linear, args, "prism_mxfp4_linear_workspace", (M, N, K, act_bits), stream, x.device,
+                            min(-(-N // 128), _COUNTERS)), "mxfp4_linear")
     return out
 
 
@@ -256,13 +268,11 @@ def mxfp4_moe(x: torch.Tensor, router: torch.Tensor, gate: Mxfp4, up: Mxfp4, dow
     if T == 0:
         return out
     stream = ops._stream()
-    run = ops.lib().prism_mxfp4_moe
-
-    def launch(work, nbytes, control):
-        return run(x.data_ptr(), x.stride(0), router.data_ptr(), ops._dt(router), None if router_bias is None else router_bias.data_ptr(),
-                   0 if router_bias is None else ops._dt(router_bias), gate.codes.data_ptr(), gate.scales.data_ptr(), up.codes.data_ptr(),
-                   up.scales.data_ptr(), down.codes.data_ptr(), down.scales.data_ptr(), T, H, F, E, top, softmax, renorm, scale_input,
-                   ops.MOE_ACTS[act], limit, None if corr is None else corr.data_ptr(), 0 if corr is None else ops._dt(corr), ch.groups, ch.keep,
-                   ch.scale, ch.sum_eps, out.data_ptr(), ops._dt(out), out.stride(0), MOE_CTAS, work, nbytes, control, _err_word(x.device), stream)
-    ops._check(_with_memory(launch, "prism_mxfp4_moe_workspace", (T, H, F, E, top, MOE_CTAS), stream, x.device, _CONTROL), "mxfp4_moe")
+    args = (x.data_ptr(), x.stride(0), router.data_ptr(), ops._dt(router), None if router_bias is None else router_bias.data_ptr(),
+            0 if router_bias is None else ops._dt(router_bias), gate.codes.data_ptr(), gate.scales.data_ptr(), up.codes.data_ptr(), up.scales.data_ptr(),
+            down.codes.data_ptr(), down.scales.data_ptr(), T, H, F, E, top, softmax, renorm, scale_input, ops.MOE_ACTS[act], limit,
+            None if corr is None else corr.data_ptr(), 0 if corr is None else ops._dt(corr), ch.groups, ch.keep, ch.scale, ch.sum_eps, out.data_ptr(),
+            ops._dt(out), out.stride(0), MOE_CTAS, _err_word(x.device), stream)
+    ops._check(_with_memory(ops.lib().prism_mxfp4_moe, args, "prism_mxfp4_moe_workspace", (T, H, F, E, top, MOE_CTAS), stream, x.device, _CONTROL),
+               "mxfp4_moe")
     return out

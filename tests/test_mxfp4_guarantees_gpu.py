@@ -1,10 +1,11 @@
 """What the 4-bit operators promise beyond their values at ordinary inputs: how far an expert's hidden values are held; that a
 wait that runs out is an error and nothing else; that no kernel runs in a workspace that is too small for it; that an experts' layer is right on any
-number of SMs.
+number of SMs; that threads and streams do not disturb one another.
 
 Tolerances.  A product's float32 sum is within 2^-18 of the sum of |x w| of the 64-bit one (``test_mxfp4_gpu``)."""
 
 import ctypes
+import threading
 
 import pytest
 import torch
@@ -59,7 +60,7 @@ def test_a_wait_that_runs_out_leaves_no_result_and_no_trace(T):
     want = ops.mxfp4_moe(*args)
     out = torch.full_like(want, 7.0)
     torch.cuda.synchronize()
-    control = ops.mxfp4._streams[(torch.cuda.current_device(), ops._stream())][0]
+    control = ops.mxfp4._streams[(torch.cuda.current_device(), ops._stream())].counters
     assert not control.any()
     control[0] = -1
     ops.mxfp4_moe(*args, out=out)
@@ -81,8 +82,8 @@ def test_a_product_s_workspace_that_is_too_small_is_refused(M, act_bits):
     work, counters = torch.empty(need.value, dtype=torch.uint8, device=DEV), torch.zeros(4096, dtype=torch.int32, device=DEV)
 
     def call(nbytes):
-        return ops.lib().prism_mxfp4_linear(x.data_ptr(), K, w.codes.data_ptr(), w.scales.data_ptr(), None, 0, out.data_ptr(), ops.F32, N, M, N, K, act_bits,
-                                            work.data_ptr(), nbytes, counters.data_ptr(), ops._tc_err_word(x.device).data_ptr(), ops._stream())
+        return ops.lib().prism_mxfp4_linear(work.data_ptr(), nbytes, counters.data_ptr(), x.data_ptr(), K, w.codes.data_ptr(), w.scales.data_ptr(), None, 0, out.data_ptr(), ops.F32, N, M, N, K, act_bits,
+                                            ops._tc_err_word(x.device).data_ptr(), ops._stream())
     assert call(need.value - 1) == call(0) == -1
     torch.cuda.synchronize()
     assert (out == 7).all()
@@ -102,7 +103,7 @@ def test_workspaces_grow_with_the_calls():
             got = ops.mxfp4_linear(x, w)
         torch.cuda.current_stream().wait_stream(side)
         assert torch.equal(got, want)
-        assert all(own[1].numel() <= ops.mxfp4._SCRATCH for own in ops.mxfp4._streams.values())
+        assert all(own.work.numel() <= ops.mxfp4._SCRATCH for own in ops.mxfp4._streams.values())
     args = _moe_args(64, 2048, 1024, 8)
     assert torch.equal(ops.mxfp4_moe(*args), ops.mxfp4_moe(*args))
 
@@ -125,3 +126,47 @@ def test_fewer_blocks_than_tokens_choose_for_every_token(ctas, T, E, F, H, top, 
         want, bound = plain_moe(x, router, *dv, top, False, False, True, choice=choice)
         got = ops.mxfp4_moe(x, router, gate, up, down, top, False, False, True, choice=choice, out_dtype=torch.float32)
         assert ((got.double() - want).abs() <= bound * 2.0 ** -8).all()
+
+
+@pytest.mark.parametrize("M,act_bits", [(64, 16), (200, 16), (64, 4), (200, 4), (3, 16)])
+def test_two_threads_on_one_stream(M, act_bits):
+    """Threads that share the default stream get the bits of their own inputs, whatever the order of their launches."""
+    ops = _ops()
+    w = ops.mxfp4_quantize(_acts(1500, 2100, 2))
+    xs = [_acts(M, 2100, 30 + i) for i in range(2)]
+    want = [ops.mxfp4_linear(x, w, act_bits=act_bits) for x in xs]
+    got = [[], []]
+
+    def work(i):
+        for _ in range(200):
+            got[i].append(ops.mxfp4_linear(xs[i], w, act_bits=act_bits))
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    ops.check_tc_errors()
+    for i in range(2):
+        assert len(got[i]) == 200 and all(torch.equal(y, want[i]) for y in got[i])
+
+
+def test_two_streams_at_once():
+    """Different inputs on two streams with no wait between them: the bits of each alone."""
+    ops = _ops()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    w = ops.mxfp4_quantize(_acts(1500, 2100, 2))
+    cases = [[(_acts(M, 2100, 10 * i + M), bits) for M in (1, 9, 64, 200) for bits in (16, 4)] for i in range(2)]
+    want = [[ops.mxfp4_linear(x, w, act_bits=b) for x, b in c] for c in cases]
+    args = [[_moe_args(T, seed=50 + i) for T in (1, 12, 40)] for i in range(2)]
+    layers = [[ops.mxfp4_moe(*a) for a in c] for c in args]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(20):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(([ops.mxfp4_linear(x, w, act_bits=b) for x, b in cases[i]], [ops.mxfp4_moe(*a) for a in args[i]]))
+    torch.cuda.synchronize()
+    ops.check_tc_errors()
+    for i in range(2):
+        for products, moes in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(products, want[i])) and all(torch.equal(a, b) for a, b in zip(moes, layers[i]))

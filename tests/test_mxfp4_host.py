@@ -1,0 +1,57 @@
+"""The host side of the 4-bit operators, without a GPU: who gets which memory, and when."""
+
+import threading
+import time
+
+import pytest
+import torch
+
+
+@pytest.fixture
+def mx(monkeypatch):
+    """``ops.mxfp4`` with one stream's memory in place, on the CPU."""
+    from prism_b200.ops import mxfp4
+    monkeypatch.setattr(torch._C, "_cuda_isCurrentStreamCapturing", lambda: False, raising=False)
+    monkeypatch.setattr(mxfp4, "_streams", {(None, 7): mxfp4._Own(torch.zeros(64, dtype=torch.int32), torch.empty(1024, dtype=torch.uint8))})
+    monkeypatch.setattr(mxfp4, "_arenas", {None: [torch.zeros(1 << 12, dtype=torch.int32), 0]})
+    monkeypatch.setattr(mxfp4, "_workspace", lambda size_of, sizes: sizes[0])
+    return mxfp4
+
+
+def in_threads(n, f):
+    threads = [threading.Thread(target=f, args=(i,)) for i in range(n)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(30)
+    assert not any(t.is_alive() for t in threads)
+
+
+def test_calls_of_two_threads_do_not_share_a_stream_s_memory_at_once(mx):
+    """A call of several launches has the stream's workspace and counters to itself until the last of them is on its way."""
+    inside, most = [], []
+
+    def launch(work, nbytes, counters):
+        inside.append(work)
+        most.append(len(inside))
+        time.sleep(0.02)                                     # between a call's first launch and its second
+        inside.remove(work)
+        return 0
+
+    in_threads(4, lambda i: [mx._with_memory(launch, (), "f", (100,), 7, torch.device("cpu"), 8) for _ in range(3)])
+    assert len(most) == 12 and max(most) == 1
+
+
+def test_captures_of_two_threads_get_counters_of_their_own(mx, monkeypatch):
+    monkeypatch.setattr(torch._C, "_cuda_isCurrentStreamCapturing", lambda: True, raising=False)
+    given = []
+
+    class Arena(list):                                       # a thread may be interrupted between reading the place and moving it on
+        def __getitem__(self, i):
+            v = super().__getitem__(i)
+            if i == 1:
+                time.sleep(0.002)
+            return v
+    mx._arenas[None] = Arena(mx._arenas[None])
+    in_threads(4, lambda i: [mx._with_memory(lambda w, n, c: given.append(c) or 0, (), "f", (100,), 7, torch.device("cpu"), 8) for _ in range(5)])
+    assert len(given) == 20 == len(set(given))
