@@ -188,11 +188,16 @@ def _with_memory(run, args, size_of: str, sizes, stream: int, device: torch.devi
 
 
 def _clear_counters():
-    """After a launch that gave up its counters may be anything (``ops.check_tc_errors``, which has waited for the device)."""
+    """After a launch that gave up (``ops.check_tc_errors``) its counters may be anything, and launches on other streams may still be
+    counting: each device is waited for as a whole, then its counters are cleared."""
     with _memory:
+        devices = sorted({key[0] for key in _streams} | set(_arenas), key=str)
+        for device in devices:
+            torch.cuda.synchronize(device)
         for block in [own.counters for own in _streams.values()] + [arena[0] for arena in _arenas.values()]:
             block.zero_()
-        torch.cuda.synchronize()
+        for device in devices:
+            torch.cuda.synchronize(device)
 
 
 def mxfp4_linear(x: torch.Tensor, w: Mxfp4, bias: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,

@@ -55,3 +55,19 @@ def test_captures_of_two_threads_get_counters_of_their_own(mx, monkeypatch):
     mx._arenas[None] = Arena(mx._arenas[None])
     in_threads(4, lambda i: [mx._with_memory(lambda w, n, c: given.append(c) or 0, (), "f", (100,), 7, torch.device("cpu"), 8) for _ in range(5)])
     assert len(given) == 20 == len(set(given))
+
+
+def test_counters_are_cleared_behind_all_streams_work(mx, monkeypatch):
+    """After a wait that ran out a launch on another stream may still be counting: the whole device is waited for first."""
+    done = []
+    monkeypatch.setattr(torch.cuda, "synchronize", lambda device=None: done.append(("wait", device)))
+
+    class Counters(torch.Tensor):
+        def zero_(self):
+            done.append(("clear", None))
+            return super().zero_()
+    for own in mx._streams.values():
+        own.counters = own.counters.add(3).as_subclass(Counters)
+    mx._clear_counters()
+    assert done[0] == ("wait", None) and ("clear", None) in done and done[-1][0] == "wait"
+    assert not any(own.counters.any() for own in mx._streams.values())
