@@ -213,9 +213,10 @@ class MixtureOfExperts(FeedForward):
         if isinstance(self.w["gate_up_w"], tuple):
             return self._forward_four_bits(ctx, x)
         H, I, E = self.hidden_size, self.intermediate_size, self.experts
-        # a gated shared expert with the experts' own activation runs with them
+        # a gated shared expert with the experts' own activation runs with them, where it is not in 4 bits beside experts that are not
         alike = (isinstance(self.shared, SwiGLU) and self.gated and self.shared.activation == self.activation
-                 and self.shared.biases is None and self.shared.limit == self.limit)
+                 and self.shared.biases is None and self.shared.limit == self.limit
+                 and not isinstance(self.shared.w["gate_up_w"], ops.Mxfp4) and not isinstance(self.shared.w["down_w"], ops.Mxfp4))
         logits = ops.linear(x, self.w["router_w"], self.w.get("router_b"), out_dtype=ops.torch.float32)
         y = ops.moe_feed_forward(ctx, x, logits, self.w["gate_up_w"].view(E, (2 if self.gated else 1) * I, H),
                                  self.w["down_w"].view(E, H, I), self.top, self.softmax, self.renorm, self.scale_input,

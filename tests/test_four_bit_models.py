@@ -1,0 +1,70 @@
+"""Models in 4 bits whose parts mix formats: what a part hands to another (CPU), and whole models against the same models
+with the 4-bit values written out (GPU)."""
+
+import pytest
+import torch
+
+import helpers
+import limatar_helpers as LH
+from test_four_bit_engine import engine, folder_of, logits, page_size, rms, write_out
+
+
+def four_bits(N, K):
+    from prism_b200 import ops
+    return ops.Mxfp4(torch.zeros(N, -(-K // 128) * 64, dtype=torch.uint8), torch.zeros(-(-N // 128), -(-K // 128), 512, dtype=torch.uint8), K)
+
+
+def test_a_shared_expert_in_four_bits_runs_on_its_own(monkeypatch):
+    """Experts that stay in bfloat16 run their shared expert with them only where it has stayed in bfloat16 too."""
+    from prism_b200 import ops
+    from prism_b200.parts.base import PartSpec, build_part
+    H, I, E = 64, 32, 300
+    part = build_part("feed_forward", PartSpec("moe", dict(hidden_size=H, intermediate_size=I, experts=E, top=2, shared=PartSpec(
+        "swiglu", dict(hidden_size=H, intermediate_size=I)))))
+    assert part.four_bit == () and part.shared.four_bit
+    part.w = {"router_w": torch.zeros(E, H), "gate_up_w": torch.zeros(E * 2 * I, H), "down_w": torch.zeros(E * H, I)}
+    part.choice = None
+    calls = []
+    monkeypatch.setattr(ops, "linear", lambda x, w, *a, **k: torch.zeros(x.shape[0], w.shape[0]))
+    monkeypatch.setattr(ops, "moe_feed_forward", lambda ctx, x, z, gu, dn, top, *a, extra_planes=0, shared=None, **k: calls.append(
+        (extra_planes, shared)) or torch.zeros(top + extra_planes + (shared is not None), x.shape[0], H))
+    monkeypatch.setattr(part.shared, "forward_to", lambda ctx, x, out: calls.append(out.shape))
+    x = torch.zeros(3, H)
+    part.shared.w = {"gate_up_w": torch.zeros(2 * I, H), "down_w": torch.zeros(H, I)}
+    assert part.forward(None, x).shape == (3, 3, H) and calls[0][0] == 0 and calls[0][1] is not None and len(calls) == 1
+    calls.clear()
+    part.shared.w = {"gate_up_w": four_bits(2 * I, H), "down_w": four_bits(H, I)}
+    assert part.forward(None, x).shape == (3, 3, H)
+    assert calls == [(1, None), (3, H)]
+
+
+# ---- whole models ----------------------------------------------------------------------------------------------------
+
+MANY = LH.model(120, 64, [
+    LH.layer("latent", LH.latent(2, 16, 8, 16, 24, 32), LH.moe(16, 260, 260, shared=16)),
+    LH.layer("retention", LH.retain(2, 16, 16, (0.9, 0.98)), LH.moe(16, 258, 258, shared=24)),
+])
+
+
+def compare(family, name, **kw):
+    """As ``test_a_model_in_four_bits_is_the_model_with_those_values``: twice the bfloat16 engine's error and 2^-8 of the logits."""
+    folder, ps = folder_of(family, name), page_size(family, name)
+    four, b16, f32 = engine(folder, ps, weight_format="mxfp4", **kw), engine(folder, ps), engine(folder, ps, "float32")
+    vocab = four.model.spec.vocab_size
+    seqs = {"a": helpers.random_tokens(vocab, 73, 5), "b": helpers.random_tokens(vocab, 11, 6)}
+    n = write_out(four, b16)
+    assert n == write_out(four, f32) > 0
+    cuts = (0, 1, 1, 2)
+    want = logits(f32, seqs, cuts)
+    own, ref = rms(logits(four, seqs, cuts) - want), rms(logits(b16, seqs, cuts) - want)
+    assert own <= 2 * ref + 2 ** -8 * rms(want), (own, ref, rms(want))
+    return four
+
+
+@pytest.mark.gpu
+def test_a_model_of_many_experts_with_shared_ones(monkeypatch):
+    monkeypatch.setitem(LH.CONFIGS, "many", (MANY, 21, 16))
+    four = compare("limatar_helpers", "many")
+    from prism_b200 import ops
+    kept = [isinstance(w, (ops.Mxfp4, tuple)) for q, w in four.pool.tensors.items() if q.endswith("gate_up_w")]
+    assert sorted(kept) == [False, False, True, True]            # the experts', the shared ones'
