@@ -43,7 +43,7 @@ def build_parser() -> argparse.ArgumentParser:
     p.add_argument("--no-cuda-graph", action="store_true")
     p.add_argument("--weight-format", default=None, choices=["mxfp4"], help="keep the layers' matrices in 4 bits")
     p.add_argument("--act-bits", type=int, default=16, choices=[16, 4],
-                   help="with --weight-format: activations of the products as they are (16) or in 4 bits too")
+                   help="with --weight-format: activations of the products as they are (16) or in 4 bits too (those of experts stay in 16)")
     return p
 
 

@@ -48,7 +48,8 @@ class EngineConfig:
     seed: int = 0
     scheduler: SchedulerConfig = field(default_factory=SchedulerConfig)
     weight_format: Optional[str] = None  # "mxfp4": the layers' matrices in microscaled 4-bit floating point
-    act_bits: int = 16                  # with it: products take activations as they are (16) or brought to 4 bits too
+    act_bits: int = 16                  # with it: products take activations as they are (16) or brought to 4 bits too;
+                                        # layers of experts take them as they are in any case
 
     def __post_init__(self):
         from ..weights.four_bit import check_weight_format

@@ -30,7 +30,7 @@ class Mxfp4:
     the K rounded up to 128, element 2i in the low half of a byte, zero beyond K.  ``scales``: uint8 ``[..., ceil(N / 128),
     Kp / 128, 512]``: the scale of row r and block b of a tile of 128 rows by four blocks is byte ``(r % 32) * 16 + r % 128
     // 32 * 4 + b % 4``; zero for blocks beyond K, anything for rows beyond N.  ``act_bits``: what ``ops.linear`` does with the
-    activations (``mxfp4_linear``)."""
+    activations (``mxfp4_linear``); ``mxfp4_moe`` takes them as they are, so a stack's is 16."""
 
     __slots__ = ("codes", "scales", "shape", "act_bits")
     dtype = DTYPE

@@ -40,7 +40,8 @@ def four_bit_params(part, path: str = "") -> Iterator[Tuple[str, object]]:
 
 
 def to_four_bits(model, pool: StaticWeightPool, device, dtype: torch.dtype, act_bits: int = 16) -> StaticWeightPool:
-    """Bind ``model`` to a new pool with those matrices in 4 bits and everything else copied; ``pool`` may be dropped."""
+    """Bind ``model`` to a new pool with those matrices in 4 bits and everything else copied; ``pool`` may be dropped.  ``act_bits``:
+    of the products with single matrices; layers of experts take activations of 16 bits in any case."""
     chosen: Dict[str, object] = {q: part for q, part in four_bit_params(model) if pool.tensors.get(q) is not None}
     # an absent parameter keeps its name without memory of its own (an alias or nothing), one filled with zeros is float32
     plan = [(q, spec, None if pool.tensors[q] is None or (spec.alias_of and pool.tensors[q] is pool.tensors.get(spec.alias_of))
@@ -53,7 +54,8 @@ def to_four_bits(model, pool: StaticWeightPool, device, dtype: torch.dtype, act_
         kept.specs[q] = pool.specs[q]
         kept.tensors[q] = part.in_four_bits(q.rsplit(".", 1)[-1], pool.tensors[q])
         for w in kept.tensors[q] if isinstance(kept.tensors[q], tuple) else (kept.tensors[q],):
-            w.act_bits = act_bits
+            if w.dim() == 2:                     # a stack's products (ops.mxfp4_moe) take activations as they are
+                w.act_bits = act_bits
             kept.total_bytes += w.nbytes
     model.bind(kept.tensors, torch.device(device), dtype)
     return kept

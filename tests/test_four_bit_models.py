@@ -38,6 +38,35 @@ def test_a_shared_expert_in_four_bits_runs_on_its_own(monkeypatch):
     assert calls == [(1, None), (3, H)]
 
 
+def fake_pool(model, dtype=torch.bfloat16):
+    from prism_b200.weights.pool import StaticWeightPool
+    return StaticWeightPool([(q, spec, dtype) for q, spec in model.named_params()], "cpu")
+
+
+def test_experts_keep_sixteen_bit_activations(monkeypatch):
+    """``act_bits`` 4 is for products with a matrix; a layer of experts takes its activations as they are, and its stacks say so."""
+    from prism_b200 import ops
+    from prism_b200.cli import build_parser
+    from prism_b200.model_registry import build_model
+    from prism_b200.weights import four_bit
+
+    def quantise(x):
+        q = four_bits(x.shape[-2], x.shape[-1])
+        if x.dim() == 3:
+            q = ops.Mxfp4(torch.stack([q.codes] * x.shape[0]), torch.stack([q.scales] * x.shape[0]), x.shape[-1])
+        return q
+    monkeypatch.setattr(ops, "mxfp4_quantize", quantise)
+    _, model = build_model(LH.CONFIGS["B"][0])
+    pool = four_bit.to_four_bits(model, fake_pool(model), "cpu", torch.bfloat16, 4)
+    seen = set()
+    for w in pool.tensors.values():
+        for q in w if isinstance(w, tuple) else (w,):
+            if isinstance(q, ops.Mxfp4):
+                seen.add((q.dim(), q.act_bits))
+    assert seen == {(2, 4), (3, 16)}
+    assert "experts" in " ".join(a.help or "" for a in build_parser()._actions if "--act-bits" in a.option_strings)
+
+
 # ---- whole models ----------------------------------------------------------------------------------------------------
 
 MANY = LH.model(120, 64, [
