@@ -12,6 +12,7 @@ file, engine/weight_pool.py:46-70).
 from __future__ import annotations
 
 import ctypes
+import operator
 import threading
 from typing import Optional
 
@@ -64,9 +65,12 @@ class Mxfp4:
 
     def __getitem__(self, e: int) -> "Mxfp4":
         """One matrix of a stack."""
-        if len(self.shape) != 3:
-            raise ops.KernelError("only a stack of 4-bit matrices can be indexed")
-        return Mxfp4._of(self.codes[e], self.scales[e], self.shape[1:])
+        if len(self.shape) != 3 or not hasattr(e, "__index__"):
+            raise ops.KernelError("only a stack of 4-bit matrices can be indexed, by the number of one of them")
+        e = operator.index(e)
+        one = Mxfp4._of(self.codes[e], self.scales[e], self.shape[1:])
+        one.act_bits = self.act_bits
+        return one
 
     def dequantize(self, dtype: Optional[torch.dtype] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """The values that the codes stand for, exact in bfloat16 (default) and float32; NaN where the scale is 255.  ``out``:

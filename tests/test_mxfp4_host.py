@@ -71,3 +71,19 @@ def test_counters_are_cleared_behind_all_streams_work(mx, monkeypatch):
     mx._clear_counters()
     assert done[0] == ("wait", None) and ("clear", None) in done and done[-1][0] == "wait"
     assert not any(own.counters.any() for own in mx._streams.values())
+
+
+def test_one_matrix_of_a_stack_and_nothing_else():
+    from prism_b200 import ops
+    w = ops.Mxfp4(torch.arange(3 * 5 * 64, dtype=torch.int64).remainder(251).to(torch.uint8).view(3, 5, 64), torch.zeros(3, 1, 1, 512, dtype=torch.uint8), 100)
+    w.act_bits = 4
+    for e in (0, 2, -1, torch.tensor(1)):
+        one = w[e]
+        assert one.shape == (5, 100) and one.act_bits == 4 and torch.equal(one.codes, w.codes[int(e)])
+    for bad in (slice(0, 2), (0, 1), [0, 1], None, Ellipsis, 1.0):
+        with pytest.raises(ops.KernelError):
+            w[bad]
+    for far in (3, -4):
+        with pytest.raises(IndexError):
+            w[far]
+    assert [one.shape for one in w] == [(5, 100)] * 3
