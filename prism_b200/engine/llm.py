@@ -60,6 +60,7 @@ class Engine:
             self.pool = random_pool(self.model, random_seed or 0, self.device, self.dtype)
         if ec.weight_format is not None:
             self.pool = to_four_bits(self.model, self.pool, self.device, self.dtype, ec.act_bits)
+            torch.cuda.empty_cache()             # the matrices as they were: free memory, not torch's, when the cache is sized
         spec = self.model.spec
         max_seq_len = min(ec.max_seq_len or spec.max_positions, spec.max_positions)
         num_pages = self._pages_per_group(ec, max_seq_len)

@@ -43,6 +43,12 @@ def fake_pool(model, dtype=torch.bfloat16):
     return StaticWeightPool([(q, spec, dtype) for q, spec in model.named_params()], "cpu")
 
 
+def quantise_on_the_cpu(x):
+    from prism_b200 import ops
+    q = four_bits(x.shape[-2], x.shape[-1])
+    return q if x.dim() == 2 else ops.Mxfp4(torch.stack([q.codes] * x.shape[0]), torch.stack([q.scales] * x.shape[0]), x.shape[-1])
+
+
 def test_experts_keep_sixteen_bit_activations(monkeypatch):
     """``act_bits`` 4 is for products with a matrix; a layer of experts takes its activations as they are, and its stacks say so."""
     from prism_b200 import ops
@@ -50,12 +56,7 @@ def test_experts_keep_sixteen_bit_activations(monkeypatch):
     from prism_b200.model_registry import build_model
     from prism_b200.weights import four_bit
 
-    def quantise(x):
-        q = four_bits(x.shape[-2], x.shape[-1])
-        if x.dim() == 3:
-            q = ops.Mxfp4(torch.stack([q.codes] * x.shape[0]), torch.stack([q.scales] * x.shape[0]), x.shape[-1])
-        return q
-    monkeypatch.setattr(ops, "mxfp4_quantize", quantise)
+    monkeypatch.setattr(ops, "mxfp4_quantize", quantise_on_the_cpu)
     _, model = build_model(LH.CONFIGS["B"][0])
     pool = four_bit.to_four_bits(model, fake_pool(model), "cpu", torch.bfloat16, 4)
     seen = set()
@@ -97,3 +98,20 @@ def test_a_model_of_many_experts_with_shared_ones(monkeypatch):
     from prism_b200 import ops
     kept = [isinstance(w, (ops.Mxfp4, tuple)) for q, w in four.pool.tensors.items() if q.endswith("gate_up_w")]
     assert sorted(kept) == [False, False, True, True]            # the experts', the shared ones'
+
+
+@pytest.mark.gpu
+def test_the_matrices_of_the_file_are_given_back_before_the_cache_is_sized(monkeypatch):
+    """What the 16-bit weights held is the device's again, not torch's, when the cache's share of the free memory is taken."""
+    import gc
+    from prism_b200 import Engine, EngineConfig
+    raw = dict(helpers.TINY_B, hidden_size=1024, head_dim=64, intermediate_size=8192, num_hidden_layers=8)
+    held = []
+    sized = Engine._pages_per_group
+    monkeypatch.setattr(Engine, "_pages_per_group", lambda self, *a: held.append(torch.cuda.memory_reserved()) or sized(self, *a))
+    gc.collect()
+    torch.cuda.empty_cache()
+    before = torch.cuda.memory_reserved()
+    four = Engine(None, EngineConfig(kv_page_size=16, num_pages=8, use_cuda_graph=False, weight_format="mxfp4"), config=raw, random_seed=1)
+    matrices = 8 * 2 * 3 * 1024 * 8192                            # bytes of the feed-forwards' in bfloat16
+    assert four.pool.total_bytes < matrices // 2 and held[0] - before < matrices // 2
