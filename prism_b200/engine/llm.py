@@ -20,7 +20,7 @@ from ..config.engine_config import EngineConfig, ModelConfig
 from ..cache.manager import pool_sizes
 from ..model_registry import build_model
 from ..sampling.sampler import Sampler, SamplingParams
-from ..weights.four_bit import check_weight_format, to_four_bits
+from ..weights.four_bit import check_weight_format, to_four_bits, written_out_bytes
 from ..weights.loader import load_model_folder
 from ..weights.random_init import random_pool
 from .request import GenerationResult
@@ -72,11 +72,13 @@ class Engine:
 
     def _pages_per_group(self, ec: EngineConfig, max_seq_len: int) -> List[int]:
         """Pool size of every cache group: ``ec.num_pages`` if given, else from the byte budget
-        ``min(budget, 0.7 * free)`` (engine/scheduler.py:100-103); see ``cache.manager.pool_sizes``."""
+        ``min(budget, 0.7 * free)`` (engine/scheduler.py:100-103), less what a step writes out of
+        matrices in 4 bits; see ``cache.manager.pool_sizes``."""
         groups, _ = cache_groups(self.model)
         budget = None
         if not ec.num_pages:
-            budget = min(ec.kv_cache_budget_gb * 1e9, 0.7 * torch.cuda.mem_get_info(self.device)[0])
+            free = torch.cuda.mem_get_info(self.device)[0] - written_out_bytes(self.model)
+            budget = min(ec.kv_cache_budget_gb * 1e9, 0.7 * free)
         return pool_sizes(groups, ec.kv_page_size, 4 if self.dtype == torch.float32 else 2, max_seq_len,
                           ec.scheduler.max_num_seqs, ec.scheduler.prefill_chunk, ec.num_pages, budget)
 

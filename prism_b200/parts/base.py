@@ -229,6 +229,10 @@ class Part:
         """Parameter ``name`` as this part wants to be bound to it in 4 bits: an ``ops.Mxfp4`` or a tuple of them."""
         return ops.mxfp4_quantize(tensor)
 
+    def written_out_bytes(self) -> int:
+        """Bytes that a step may take to write matrices in 4 bits out, while it is in this part."""
+        return 0
+
     def handed_over(self, *sources: WeightSource) -> Tuple[WeightSource, ...]:
         """Own file tensors under their full names, for a ``DetachedProjection``."""
         return tuple(WeightSource(s.name if s.absolute else self.prefix + s.name, s.shape, s.init, True) for s in sources)

@@ -184,6 +184,10 @@ class MixtureOfExperts(FeedForward):
         gate_up = tensor.view(E, 2, I, H)
         return tuple(ops.mxfp4_quantize(gate_up[:, i].contiguous()) for i in range(2))
 
+    def written_out_bytes(self):
+        four = isinstance(self.w["gate_up_w"], tuple)
+        return 2 * 3 * self.experts * self.intermediate_size * self.hidden_size if four else 0       # as _forward_four_bits does
+
     def on_bound(self):
         self.choice = ops.MoeChoice(self.w.get("correction"), self.groups, self.keep, self.weight_scale, self.sum_eps)
 

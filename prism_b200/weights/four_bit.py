@@ -39,6 +39,11 @@ def four_bit_params(part, path: str = "") -> Iterator[Tuple[str, object]]:
         yield from four_bit_params(child, f"{path}{cname}.")
 
 
+def written_out_bytes(part) -> int:
+    """The most that any part below ``part`` writes out of its matrices in 4 bits at once."""
+    return max([part.written_out_bytes()] + [written_out_bytes(child) for child in part.children.values()])
+
+
 def to_four_bits(model, pool: StaticWeightPool, device, dtype: torch.dtype, act_bits: int = 16) -> StaticWeightPool:
     """Bind ``model`` to a new pool with those matrices in 4 bits and everything else copied; ``pool`` may be dropped.  ``act_bits``:
     of the products with single matrices; layers of experts take activations of 16 bits in any case."""

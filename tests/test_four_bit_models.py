@@ -68,6 +68,28 @@ def test_experts_keep_sixteen_bit_activations(monkeypatch):
     assert "experts" in " ".join(a.help or "" for a in build_parser()._actions if "--act-bits" in a.option_strings)
 
 
+def test_the_cache_s_budget_leaves_room_for_experts_written_out(monkeypatch):
+    """A step of more than 64 tokens writes a layer's experts out in bfloat16; the largest layer's are no room for keys."""
+    from types import SimpleNamespace
+    from prism_b200 import EngineConfig, ops
+    from prism_b200.engine import llm
+    from prism_b200.model_registry import build_model
+    from prism_b200.weights import four_bit
+    budgets = []
+    monkeypatch.setattr(llm, "pool_sizes", lambda *a: budgets.append(a[-1]))
+    monkeypatch.setattr(torch.cuda, "mem_get_info", lambda device=None: (10 ** 9, 2 * 10 ** 9))
+    monkeypatch.setattr(ops, "mxfp4_quantize", quantise_on_the_cpu)
+    _, model = build_model(LH.CONFIGS["B"][0])
+    pool = fake_pool(model)
+    model.bind(pool.tensors, "cpu", torch.bfloat16)
+    self = SimpleNamespace(model=model, device="cpu", dtype=torch.bfloat16)
+    llm.Engine._pages_per_group(self, EngineConfig(), 128)
+    four_bit.to_four_bits(model, pool, "cpu", torch.bfloat16)
+    llm.Engine._pages_per_group(self, EngineConfig(), 128)
+    written_out = 2 * 8 * 3 * 128 * 64                            # the larger of the two layers: 8 experts of 3 x 64 x 128
+    assert budgets == [0.7 * 10 ** 9, 0.7 * (10 ** 9 - written_out)]
+
+
 # ---- whole models ----------------------------------------------------------------------------------------------------
 
 MANY = LH.model(120, 64, [
