@@ -52,6 +52,7 @@ def main(argv=None) -> int:
     import torch
     from .config.engine_config import EngineConfig, ModelConfig, SchedulerConfig
     from .sampling.sampler import SamplingParams
+    from .weights.four_bit import four_bit_share
 
     raw = None
     if args.random_weights:
@@ -99,7 +100,8 @@ def main(argv=None) -> int:
             print(f"no tokenizer in the model folder ({e}); use --prompt-ids or --prompt-len", file=sys.stderr)
             return 2
         prompts = [tokenizer.encode(text).ids] * args.num_prompts
-    print(f"\nPrompt: {len(prompts)} x {len(prompts[0])} tokens; weights {eng.pool.total_gb:.2f} GB loaded in {t_load:.1f}s")
+    four = "" if args.weight_format is None else f" ({four_bit_share(eng.model):.0%} of the parameters in 4 bits)"
+    print(f"\nPrompt: {len(prompts)} x {len(prompts[0])} tokens; weights {eng.pool.total_gb:.2f} GB{four} loaded in {t_load:.1f}s")
 
     sp = SamplingParams(max_new_tokens=args.max_tokens, temperature=args.temperature, seed=args.sample_seed,
                         ignore_eos=args.ignore_eos)

@@ -9,6 +9,7 @@ matrices of parts that name none and those that a block has taken over from its 
 
 from __future__ import annotations
 
+from math import prod
 from typing import Dict, Iterator, Tuple
 
 import torch
@@ -37,6 +38,13 @@ def four_bit_params(part, path: str = "") -> Iterator[Tuple[str, object]]:
             yield path + name, part
     for cname, child in part.children.items():
         yield from four_bit_params(child, f"{path}{cname}.")
+
+
+def four_bit_share(model) -> float:
+    """The share of ``model``'s parameters that may be kept in 4 bits: from nine tenths of a dense design to a twentieth of one
+    whose blocks run their matrices jointly."""
+    count = {q: prod(spec.shape) for q, spec in model.named_params() if not spec.alias_of}
+    return sum(count[q] for q, _ in four_bit_params(model)) / sum(count.values())
 
 
 def written_out_bytes(part) -> int:

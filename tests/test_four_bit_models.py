@@ -68,6 +68,19 @@ def test_experts_keep_sixteen_bit_activations(monkeypatch):
     assert "experts" in " ".join(a.help or "" for a in build_parser()._actions if "--act-bits" in a.option_strings)
 
 
+@pytest.mark.parametrize("module,name,low,high", [("helpers", "D", 0.8, 0.9), ("limatar_helpers", "B", 0.5, 0.6), ("dolezen_helpers", "Y", 0.0, 0.1)])
+def test_the_share_in_four_bits_is_known(module, name, low, high):
+    """Part of some designs' parameters is never taken; how much is for the user to see."""
+    import importlib
+    from prism_b200.model_registry import build_model
+    from prism_b200.weights.four_bit import four_bit_params, four_bit_share
+    mod = importlib.import_module(module)
+    _, model = build_model((mod.TINY if module == "helpers" else mod.CONFIGS)[name][0])
+    share = four_bit_share(model)
+    count = {q: torch.Size(spec.shape).numel() for q, spec in model.named_params() if not spec.alias_of}
+    assert low < share < high and share == sum(count[q] for q, _ in four_bit_params(model)) / sum(count.values())
+
+
 def test_the_cache_s_budget_leaves_room_for_experts_written_out(monkeypatch):
     """A step of more than 64 tokens writes a layer's experts out in bfloat16; the largest layer's are no room for keys."""
     from types import SimpleNamespace
