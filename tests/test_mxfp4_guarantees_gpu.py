@@ -170,3 +170,85 @@ def test_two_streams_at_once():
     for i in range(2):
         for products, moes in got[i]:
             assert all(torch.equal(a, b) for a, b in zip(products, want[i])) and all(torch.equal(a, b) for a, b in zip(moes, layers[i]))
+
+
+@pytest.mark.parametrize("T", [1, 16, 33, 64])
+def test_a_layer_of_experts_replays_and_repeats(T):
+    """The same bits again, among other calls and from a captured graph, whose inputs may change between replays."""
+    ops = _ops()
+    args = _moe_args(T, 512, 300, 9)
+    want = ops.mxfp4_moe(*args)
+    other = (_acts(T, 512, 99),) + args[1:]
+    want_other = ops.mxfp4_moe(*other)
+    assert not torch.equal(want, want_other)
+    x = args[0].clone()
+    g = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(g):
+        y = ops.mxfp4_moe(x, *args[1:])
+        z = ops.mxfp4_moe(x, *args[1:])
+    for i in range(6):
+        assert torch.equal(ops.mxfp4_moe(*args), want)
+        x.copy_(other[0] if i % 2 else args[0])
+        g.replay()
+        g.replay()
+        assert torch.equal(y, want_other if i % 2 else want) and torch.equal(z, y)
+    ops.check_tc_errors()
+
+
+def test_graphs_of_two_streams_at_once():
+    """Two captured steps of several calls, replayed on two streams with no wait between them."""
+    ops = _ops()
+    w = ops.mxfp4_quantize(_acts(1500, 2100, 2))
+    steps = []
+    for i in range(2):
+        xs, layer = [_acts(M, 2100, 10 * i + M) for M in (1, 64)], _moe_args(12, seed=40 + i)
+        want = [ops.mxfp4_linear(x, w, act_bits=b) for x in xs for b in (16, 4)] + [ops.mxfp4_moe(*layer)]
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            got = [ops.mxfp4_linear(x, w, act_bits=b) for x in xs for b in (16, 4)] + [ops.mxfp4_moe(*layer)]
+        steps.append((g, torch.cuda.Stream(), got, want, xs, layer))
+    torch.cuda.synchronize()
+    for _ in range(30):
+        for g, stream, *_ in steps:
+            with torch.cuda.stream(stream):
+                g.replay()
+    torch.cuda.synchronize()
+    ops.check_tc_errors()
+    assert all(torch.equal(a, b) for _, _, got, want, *_ in steps for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("T,E,top,H,F", [(64, 256, 16, 128, 32), (64, 16, 16, 96, 40), (1, 256, 16, 200, 64), (64, 256, 1, 64, 33), (64, 64, 16, 1003, 31)])
+def test_the_most_experts_and_choices(T, E, top, H, F):
+    ops = _ops()
+    x, router = _acts(T, H, T), (_acts(E, H, 4) * H ** -0.5).to(torch.bfloat16)
+    gate, up, down = _experts(E, F, H, 2)
+    want, bound = plain_moe(x, router, *[decode(w).to(DEV) for w in (gate, up, down)], top, True, True, False)
+    got = ops.mxfp4_moe(x, router, gate, up, down, top, True, True, False, out_dtype=torch.float32)
+    assert ((got.double() - want).abs() <= bound * 2.0 ** -8).all()
+
+
+@pytest.mark.parametrize("M", [1, 16, 40, 200])
+@pytest.mark.parametrize("below", [6, 13, 18, 21])
+def test_activations_far_below_their_block_s_largest(M, below):
+    """Every block of x holds one large value, which meets weights of zero, and values some 2^-``below`` of it: these are read
+    exactly down to 2^-14 of the largest and to within 2^-22 of it below."""
+    ops = _ops()
+    N, K = 200, 640
+    g = _gen(M + below)
+    x = (torch.rand(M, K, generator=g) * 2 + 2) * 2.0 ** -below * torch.where(torch.rand(M, K, generator=g) < 0.5, -1.0, 1.0)
+    x[:, ::32] = 1 + torch.rand(M, K // 32, generator=g)
+    x = x.to(torch.bfloat16).to(DEV)
+    wf = torch.randn(N, K, generator=g)
+    wf[:, ::32] = 0
+    w = ops.mxfp4_quantize(wf.to(DEV))
+    wv = decode(w).to(DEV)
+    want = x.double() @ wv.t()
+    small = torch.ones(K, dtype=torch.float64, device=DEV)
+    small[::32] = 0
+    bound = (x.double().abs() * small) @ wv.abs().t() * SUM
+    if below > 13:
+        bound = bound + x.double()[:, ::32].abs().repeat_interleave(32, 1) @ wv.abs().t() * 2.0 ** -22
+    far = (ops.mxfp4_linear(x, w, out_dtype=torch.float32).double() - want).abs() - bound
+    assert (far <= 0).all(), (far.max().item(), (far > 0).double().mean().item())
