@@ -578,17 +578,18 @@ template <typename C> int run_product(const CUtensorMap& mw, const CUtensorMap& 
 }  // namespace mx
 }  // namespace prism
 
-// bytes of workspace that prism_mxfp4_linear needs for these sizes, into *bytes
-PRISM_EXPORT int prism_mxfp4_linear_workspace(int M, int N, int K, int act_bits, long long* bytes) {
+// what prism_mxfp4_linear needs for these sizes: bytes of workspace, into need[0], and counters, into need[1]
+PRISM_EXPORT int prism_mxfp4_linear_workspace(int M, int N, int K, int act_bits, long long* need) {
     if (M <= 0 || N <= 0 || K <= 0 || (act_bits != 16 && act_bits != 4)) return (int)cudaErrorInvalidValue;
     const prism::mx::Plan q = prism::mx::plan_for(M, N, K, act_bits);
-    *bytes = q.bytes;
+    need[0] = q.bytes;
+    need[1] = q.fused ? q.units : 0;
     return q.units * q.kb > 0x7fffffffLL ? (int)cudaErrorInvalidValue : 0;
 }
 
 // x [M, K] bfloat16 (row stride ldx); codes, scales: W [N, K]; y [M, N] of `out_dtype` (row stride ldy); act_bits 16 or 4;
 // ws: workspace of the call, 256-byte aligned; nothing is launched and -1 returned where its ws_bytes are fewer than
-// prism_mxfp4_linear_workspace says on this device; counters: at least ceil(N / 128) ints (4,096 always
+// prism_mxfp4_linear_workspace says on this device; counters: as many ints as it says there (4,096 always
 // suffice), zero before the first launch (the kernel leaves them zero), of one stream's launches at a time
 PRISM_EXPORT int prism_mxfp4_linear(void* ws, long long ws_bytes, int* counters, const void* x, long long ldx, const void* codes, const void* scales,
                                     const void* bias, int bias_dtype, void* y, int out_dtype, long long ldy, int M, int N, int K, int act_bits,

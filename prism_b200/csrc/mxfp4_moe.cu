@@ -807,10 +807,11 @@ template <typename C> int run_moe(const CUtensorMap (&m)[5], const Moe& p, int P
 }  // namespace mx
 }  // namespace prism
 
-// bytes of workspace that prism_mxfp4_moe needs for these sizes, into *bytes
-PRISM_EXPORT int prism_mxfp4_moe_workspace(int T, int H, int F, int E, int top, int ctas, long long* bytes) {
+// what prism_mxfp4_moe needs for these sizes: bytes of workspace, into need[0], and words of control, into need[1]
+PRISM_EXPORT int prism_mxfp4_moe_workspace(int T, int H, int F, int E, int top, int ctas, long long* need) {
     if (!prism::mx::moe_sizes_ok(T, H, F, E, top)) return (int)cudaErrorInvalidValue;
-    *bytes = prism::mx::moe_plan(T, H, F, E, top, ctas).bytes;
+    need[0] = prism::mx::moe_plan(T, H, F, E, top, ctas).bytes;
+    need[1] = prism::mx::CONTROL_WORDS;
     return 0;
 }
 

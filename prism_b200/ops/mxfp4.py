@@ -118,11 +118,12 @@ def mxfp4_quantize(x: torch.Tensor) -> Mxfp4:
     return Mxfp4._of(codes, scales, shape)
 
 
-def _workspace(size_of: str, sizes) -> int:
-    b = ctypes.c_longlong()
+def _workspace(size_of: str, sizes):
+    """``(bytes of workspace, counters)`` of a call."""
+    b = (ctypes.c_longlong * 2)()
     if getattr(ops.lib(), size_of)(*sizes, ctypes.addressof(b)) != 0:
         raise ops.KernelError(f"{size_of}: sizes {sizes} are not supported")
-    return b.value
+    return b[0], b[1]
 
 
 _err_words = {}
@@ -136,8 +137,7 @@ def _err_word(device: torch.device) -> int:
     return p
 
 
-_COUNTERS = 4096             # of a stream: tiles of a product (csrc/mxfp4_linear.cu), or an experts' layer's control words
-_CONTROL = 68                # csrc/mxfp4_moe.cu: Control
+_COUNTERS = 4096             # of a stream, the most of a call: tiles of a product in one launch (csrc/mxfp4_linear.cu), an experts' layer's control words
 _TOO_SMALL = -1              # csrc/mxfp4.cuh: WORKSPACE_TOO_SMALL
 _SCRATCH = 16 << 20          # a larger workspace is the call's own
 _ARENA = 1 << 20
@@ -159,7 +159,7 @@ class _Own:
         self.work, self.at = work, (work.data_ptr(), work.numel(), self.counters.data_ptr())
 
 
-def _with_memory(run, args, size_of: str, sizes, stream: int, device: torch.device, counters: int) -> int:
+def _with_memory(run, args, size_of: str, sizes, stream: int, device: torch.device) -> int:
     """``run(workspace, its bytes, counters, *args)`` with memory that no other thread's call has meanwhile; its answer.  It is asked to
     run in the stream's workspace at once and says, before it launches anything, where that is too small: how much a call needs is
     for the device that it runs on to say.  Counters are zero before a launch and left so.  Under graph capture a call gets
@@ -167,14 +167,18 @@ def _with_memory(run, args, size_of: str, sizes, stream: int, device: torch.devi
     with _memory:
         if torch._C._cuda_isCurrentStreamCapturing():
             arena = _arenas.get(device.index)
+            nbytes, counters = _workspace(size_of, sizes)
             counters = (counters + 63) // 64 * 64
-            if arena is None or arena[1] + counters > _ARENA:
+            if counters == 0:                                        # its first kernel clears those in its workspace
+                at = 0
+            elif arena is None or arena[1] + counters > _ARENA:
                 block = torch.zeros(counters, dtype=torch.int32, device=device)            # cleared by the graph
+                at = block.data_ptr()
             else:
-                block = arena[0][arena[1]:arena[1] + counters]
+                at = arena[0].data_ptr() + 4 * arena[1]
                 arena[1] += counters
-            work = torch.empty(_workspace(size_of, sizes), dtype=torch.uint8, device=device)
-            return run(work.data_ptr(), work.numel(), block.data_ptr(), *args)
+            work = torch.empty(nbytes, dtype=torch.uint8, device=device)
+            return run(work.data_ptr(), work.numel(), at, *args)
         own = _streams.get((device.index, stream))
         if own is None:
             if device.index not in _arenas:
@@ -184,7 +188,7 @@ def _with_memory(run, args, size_of: str, sizes, stream: int, device: torch.devi
                                                           torch.empty(4 << 20, dtype=torch.uint8, device=device))
         code = run(*own.at, *args)
         if code == _TOO_SMALL:
-            work = torch.empty(_workspace(size_of, sizes), dtype=torch.uint8, device=device)
+            work = torch.empty(_workspace(size_of, sizes)[0], dtype=torch.uint8, device=device)
             if work.numel() <= _SCRATCH:
                 own.use(work)
             code = run(work.data_ptr(), work.numel(), own.at[2], *args)
@@ -230,8 +234,8 @@ def mxfp4_linear(x: torch.Tensor, w: Mxfp4, bias: Optional[torch.Tensor] = None,
     stream = ops._stream()
     args = (x.data_ptr(), x.stride(0), w.codes.data_ptr(), w.scales.data_ptr(), None if bias is None else bias.data_ptr(),
             0 if bias is None else ops._dt(bias), out.data_ptr(), ops._dt(out), out.stride(0), M, N, K, act_bits, _err_word(x.device), stream)
-    ops._check(_with_memory(ops.lib().prism_mxfp4_linear, args, "prism_mxfp4_linear_workspace", (M, N, K, act_bits), stream, x.device,
-                            min(-(-N // 128), _COUNTERS)), "mxfp4_linear")
+    ops._check(_with_memory(ops.lib().prism_mxfp4_linear, args, "prism_mxfp4_linear_workspace", (M, N, K, act_bits), stream, x.device),
+               "mxfp4_linear")
     return out
 
 
@@ -282,6 +286,6 @@ def mxfp4_moe(x: torch.Tensor, router: torch.Tensor, gate: Mxfp4, up: Mxfp4, dow
             down.codes.data_ptr(), down.scales.data_ptr(), T, H, F, E, top, softmax, renorm, scale_input, ops.MOE_ACTS[act], limit,
             None if corr is None else corr.data_ptr(), 0 if corr is None else ops._dt(corr), ch.groups, ch.keep, ch.scale, ch.sum_eps, out.data_ptr(),
             ops._dt(out), out.stride(0), MOE_CTAS, _err_word(x.device), stream)
-    ops._check(_with_memory(ops.lib().prism_mxfp4_moe, args, "prism_mxfp4_moe_workspace", (T, H, F, E, top, MOE_CTAS), stream, x.device, _CONTROL),
+    ops._check(_with_memory(ops.lib().prism_mxfp4_moe, args, "prism_mxfp4_moe_workspace", (T, H, F, E, top, MOE_CTAS), stream, x.device),
                "mxfp4_moe")
     return out

@@ -10,7 +10,7 @@ import threading
 import pytest
 import torch
 
-from test_mxfp4_gpu import DEV, _acts, _experts, _gen, _ops, decode, plain_moe
+from test_mxfp4_gpu import DEV, _acts, _check_linear, _experts, _gen, _ops, decode, plain_moe
 
 pytestmark = pytest.mark.gpu
 
@@ -77,17 +77,17 @@ def test_a_product_s_workspace_that_is_too_small_is_refused(M, act_bits):
     ops = _ops()
     N, K = 700, 2000
     x, w, out = _acts(M, K, 1), ops.mxfp4_quantize(_acts(N, K, 2)), torch.full((M, N), 7.0, device=DEV)
-    need = ctypes.c_longlong()
+    need = (ctypes.c_longlong * 2)()
     assert ops.lib().prism_mxfp4_linear_workspace(M, N, K, act_bits, ctypes.addressof(need)) == 0
-    work, counters = torch.empty(need.value, dtype=torch.uint8, device=DEV), torch.zeros(4096, dtype=torch.int32, device=DEV)
+    work, counters = torch.empty(need[0], dtype=torch.uint8, device=DEV), torch.zeros(4096, dtype=torch.int32, device=DEV)
 
     def call(nbytes):
         return ops.lib().prism_mxfp4_linear(work.data_ptr(), nbytes, counters.data_ptr(), x.data_ptr(), K, w.codes.data_ptr(), w.scales.data_ptr(), None, 0, out.data_ptr(), ops.F32, N, M, N, K, act_bits,
                                             ops._tc_err_word(x.device).data_ptr(), ops._stream())
-    assert call(need.value - 1) == call(0) == -1
+    assert call(need[0] - 1) == call(0) == -1
     torch.cuda.synchronize()
     assert (out == 7).all()
-    assert call(need.value) == 0
+    assert need[1] == (6 if M <= 8 else 0) and call(need[0]) == 0
     assert torch.equal(out, ops.mxfp4_linear(x, w, out_dtype=torch.float32, act_bits=act_bits))
 
 
@@ -252,3 +252,16 @@ def test_activations_far_below_their_block_s_largest(M, below):
         bound = bound + x.double()[:, ::32].abs().repeat_interleave(32, 1) @ wv.abs().t() * 2.0 ** -22
     far = (ops.mxfp4_linear(x, w, out_dtype=torch.float32).double() - want).abs() - bound
     assert (far <= 0).all(), (far.max().item(), (far > 0).double().mean().item())
+
+
+@pytest.mark.parametrize("N", [4096 * 128, 4096 * 128 + 1])
+@pytest.mark.parametrize("act_bits", [16, 4])
+def test_as_many_rows_as_the_stream_s_counters_and_one_more(N, act_bits):
+    """Beyond 4,096 tiles a few tokens go through the form of many."""
+    ops = _ops()
+    x, w = _acts(2, 40, 1), ops.mxfp4_quantize(_acts(N, 40, 2))
+    got = ops.mxfp4_linear(x, w, act_bits=act_bits)
+    at = torch.cat([torch.arange(300), torch.arange(N - 300, N)]).to(DEV)
+    few = ops.mxfp4_quantize(_acts(N, 40, 2)[at])
+    assert torch.equal(got[:, at], ops.mxfp4_linear(x, few, act_bits=act_bits))
+    _check_linear(x, few, None, act_bits, got=got[:, at].contiguous())

@@ -14,7 +14,7 @@ def mx(monkeypatch):
     monkeypatch.setattr(torch._C, "_cuda_isCurrentStreamCapturing", lambda: False, raising=False)
     monkeypatch.setattr(mxfp4, "_streams", {(None, 7): mxfp4._Own(torch.zeros(64, dtype=torch.int32), torch.empty(1024, dtype=torch.uint8))})
     monkeypatch.setattr(mxfp4, "_arenas", {None: [torch.zeros(1 << 12, dtype=torch.int32), 0]})
-    monkeypatch.setattr(mxfp4, "_workspace", lambda size_of, sizes: sizes[0])
+    monkeypatch.setattr(mxfp4, "_workspace", lambda size_of, sizes: (sizes[0], 8))
     return mxfp4
 
 
@@ -38,7 +38,7 @@ def test_calls_of_two_threads_do_not_share_a_stream_s_memory_at_once(mx):
         inside.remove(work)
         return 0
 
-    in_threads(4, lambda i: [mx._with_memory(launch, (), "f", (100,), 7, torch.device("cpu"), 8) for _ in range(3)])
+    in_threads(4, lambda i: [mx._with_memory(launch, (), "f", (100,), 7, torch.device("cpu")) for _ in range(3)])
     assert len(most) == 12 and max(most) == 1
 
 
@@ -53,7 +53,7 @@ def test_captures_of_two_threads_get_counters_of_their_own(mx, monkeypatch):
                 time.sleep(0.002)
             return v
     mx._arenas[None] = Arena(mx._arenas[None])
-    in_threads(4, lambda i: [mx._with_memory(lambda w, n, c: given.append(c) or 0, (), "f", (100,), 7, torch.device("cpu"), 8) for _ in range(5)])
+    in_threads(4, lambda i: [mx._with_memory(lambda w, n, c: given.append(c) or 0, (), "f", (100,), 7, torch.device("cpu")) for _ in range(5)])
     assert len(given) == 20 == len(set(given))
 
 
@@ -87,3 +87,22 @@ def test_one_matrix_of_a_stack_and_nothing_else():
         with pytest.raises(IndexError):
             w[far]
     assert [one.shape for one in w] == [(5, 100)] * 3
+
+
+def test_captured_calls_take_the_counters_that_they_use(mx, monkeypatch):
+    """A call whose first kernel clears counters in its workspace takes none; behind the last ones a graph clears its own."""
+    monkeypatch.setattr(torch._C, "_cuda_isCurrentStreamCapturing", lambda: True, raising=False)
+    given = []
+
+    def call():
+        assert mx._with_memory(lambda w, n, c: given.append(c) or 0, (), "f", (100,), 7, torch.device("cpu")) == 0
+    arena = mx._arenas[None]
+    monkeypatch.setattr(mx, "_workspace", lambda size_of, sizes: (100, 0))
+    call()
+    assert arena[1] == 0 and not given[-1]
+    monkeypatch.setattr(mx, "_workspace", lambda size_of, sizes: (100, 70))
+    call()
+    assert arena[1] == 128 and given[-1] == arena[0].data_ptr()
+    monkeypatch.setattr(mx, "_ARENA", 250)
+    call()
+    assert arena[1] == 128 and given[-1] and not arena[0].data_ptr() <= given[-1] < arena[0].data_ptr() + 4 * arena[0].numel()
