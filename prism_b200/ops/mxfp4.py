@@ -85,7 +85,7 @@ class Mxfp4:
         if out is None:
             out = codes.new_empty(shape, dtype=dtype)
         elif out.shape != shape or out.dtype is not dtype or not out[0:1].is_contiguous() or not out.is_cuda or (
-                len(shape) == 2 and not out.is_contiguous()) or (K % 8 == 0 and (out.data_ptr() % 16 or (len(shape) == 3 and out.stride(0) % 8))):
+                len(shape) == 2 and not out.is_contiguous()) or (len(shape) == 3 and shape[0] > 1 and out.stride(0) < shape[1] * K) or (K % 8 == 0 and (out.data_ptr() % 16 or (len(shape) == 3 and out.stride(0) % 8))):
             raise ops.KernelError(f"4-bit values of {shape} do not go into {tuple(out.shape)} {out.dtype} with strides {out.stride()}")
         ops._check(ops.lib().prism_mxfp4_dequantize(codes.data_ptr(), self.scales.data_ptr(), shape[0] if len(shape) == 3 else 1, shape[-2], shape[-1],
                                                     out.data_ptr(), out.stride(0), ops.F32 if dtype is torch.float32 else ops.BF16, ops._stream()),
@@ -227,8 +227,8 @@ def mxfp4_linear(x: torch.Tensor, w: Mxfp4, bias: Optional[torch.Tensor] = None,
         raise ops.KernelError(f"a bias has one entry per row of the weight, got {tuple(bias.shape)}")
     if out is None:
         out = x.new_empty((M, N), dtype=out_dtype)
-    elif out.shape != (M, N) or (out.stride(1) != 1 and N > 1) or out_dtype not in (None, out.dtype):
-        raise ops.KernelError(f"the result of {tuple(xs)} and {tuple(ws)} does not go into {tuple(out.shape)} {out.dtype}")
+    elif out.shape != (M, N) or (out.stride(1) != 1 and N > 1) or (M > 1 and out.stride(0) < N) or out_dtype not in (None, out.dtype):
+        raise ops.KernelError(f"the result of {tuple(xs)} and {tuple(ws)} does not go into {tuple(out.shape)} {out.dtype} with strides {out.stride()}")
     if M == 0:
         return out
     stream = ops._stream()
@@ -276,8 +276,8 @@ def mxfp4_moe(x: torch.Tensor, router: torch.Tensor, gate: Mxfp4, up: Mxfp4, dow
         raise ops.KernelError(f"{E} experts in {ch.groups} groups of which {ch.keep} are kept, {top} a token")
     if out is None:
         out = x.new_empty((T, H), dtype=out_dtype)
-    elif out.shape != (T, H) or out.stride(1) != 1 or out_dtype not in (None, out.dtype):
-        raise ops.KernelError(f"the result of {T} rows of {H} does not go into {tuple(out.shape)} {out.dtype}")
+    elif out.shape != (T, H) or out.stride(1) != 1 or (T > 1 and out.stride(0) < H) or out_dtype not in (None, out.dtype):
+        raise ops.KernelError(f"the result of {T} rows of {H} does not go into {tuple(out.shape)} {out.dtype} with strides {out.stride()}")
     if T == 0:
         return out
     stream = ops._stream()

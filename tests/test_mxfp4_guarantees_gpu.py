@@ -265,3 +265,30 @@ def test_as_many_rows_as_the_stream_s_counters_and_one_more(N, act_bits):
     few = ops.mxfp4_quantize(_acts(N, 40, 2)[at])
     assert torch.equal(got[:, at], ops.mxfp4_linear(x, few, act_bits=act_bits))
     _check_linear(x, few, None, act_bits, got=got[:, at].contiguous())
+
+
+def test_results_whose_rows_overlap_are_refused():
+    ops = _ops()
+    x, w, stack = _acts(4, 200, 1), ops.mxfp4_quantize(_acts(96, 200, 2)), ops.mxfp4_quantize(torch.stack([_acts(8, 64, i) for i in range(3)]))
+    line = torch.empty(4 * 300, dtype=torch.bfloat16, device=DEV)
+    layer = _moe_args(4, 256)
+    for call in (lambda: ops.mxfp4_linear(x, w, out=line[:96].expand(4, 96)), lambda: ops.mxfp4_linear(x, w, out=line.as_strided((4, 96), (95, 1))),
+                 lambda: stack.dequantize(out=line[:512].view(1, 8, 64).expand(3, 8, 64)), lambda: stack.dequantize(out=line.as_strided((3, 8, 64), (256, 64, 1))),
+                 lambda: ops.mxfp4_moe(*layer, out=line[:256].expand(4, 256)), lambda: ops.mxfp4_moe(*layer, out=line.as_strided((4, 256), (128, 1)))):
+        with pytest.raises(ops.KernelError):
+            call()
+    one = line.as_strided((1, 96), (1, 1))                         # a single row's stride says nothing
+    assert torch.equal(ops.mxfp4_linear(x[:1], w, out=one), ops.mxfp4_linear(x[:1], w))
+
+
+@pytest.mark.parametrize("T", [16, 40, 64])
+def test_a_token_that_is_not_a_number_among_many(T):
+    """It is a row of NaN, and the other tokens' bits are as without it (every expert has tokens either way)."""
+    ops = _ops()
+    x, *rest = _moe_args(T, 256, 96, 2)
+    clean = ops.mxfp4_moe(x, *rest)
+    y = x.clone()
+    y[5, 200], y[T - 1, 0] = float("nan"), float("inf")
+    got = ops.mxfp4_moe(y, *rest)
+    keep = [t for t in range(T) if t not in (5, T - 1)]
+    assert torch.isnan(got[[5, T - 1]]).all() and torch.equal(got[keep], clean[keep])
