@@ -47,7 +47,8 @@ class EngineConfig:
     graph_batch_sizes: Sequence[int] = (1, 2, 4, 8, 16, 32, 64)
     seed: int = 0
     scheduler: SchedulerConfig = field(default_factory=SchedulerConfig)
-    weight_format: Optional[str] = None  # "mxfp4": the layers' matrices in microscaled 4-bit floating point
+    weight_format: Optional[str] = None  # "mxfp4": the layers' matrices in microscaled 4-bit floating point, brought to it once the
+                                        # model is loaded as its file has it (both have room on the device for a moment)
     act_bits: int = 16                  # with it: products take activations as they are (16) or brought to 4 bits too;
                                         # layers of experts take them as they are in any case
 

@@ -251,7 +251,8 @@ def mxfp4_moe(x: torch.Tensor, router: torch.Tensor, gate: Mxfp4, up: Mxfp4, dow
     token takes the ``top`` experts with the largest scores (sigmoid of the logits, or their softmax; the lower index of equal ones); a choice's weight is its score
     (``renorm``: over the sum of the chosen) and multiplies the expert's input (``scale_input``) or its output.  ``act``:
     silu, gelu_tanh or clamped (with ``limit``, as in ``ops.glu``).  ``choice``: an ``ops.MoeChoice``.  Returns the sum over a
-    token's choices, ``[T, H]`` bfloat16 or float32 (``out`` or ``out_dtype``)."""
+    token's choices, ``[T, H]`` bfloat16 or float32 (``out`` or ``out_dtype``).  Activations are taken as they are, hidden values are
+    held to 2^-14 of themselves; a row of x, or 32 neighbouring hidden values, with an infinity or NaN among them are NaN as a whole."""
     for t in (x, router, gate.codes, up.codes, down.codes, router_bias, out):
         if t is not None and not t.is_cuda:
             ops._cuda(t)

@@ -192,8 +192,9 @@ class MixtureOfExperts(FeedForward):
         self.choice = ops.MoeChoice(self.w.get("correction"), self.groups, self.keep, self.weight_scale, self.sum_eps)
 
     def _forward_four_bits(self, ctx, x):
-        """Experts in 4 bits: up to 64 tokens as one launch, a plane of sums; a longer step brings the step's layer back to
-        bfloat16 for the grouped products, which is right where every weight is used many times."""
+        """Experts in 4 bits: up to 64 tokens as one launch, a plane of sums; a longer step brings the layer back to bfloat16 for the
+        grouped products.  That costs some 4.5 bytes a weight and step, and room for the copy (``written_out_bytes``): little where
+        every expert has many tokens, much where a step is a little longer than 64 or the experts are many."""
         T, H = x.shape
         E, I = self.experts, self.intermediate_size
         (gate, up), down = self.w["gate_up_w"], self.w["down_w"]
