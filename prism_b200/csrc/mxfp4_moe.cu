@@ -19,10 +19,11 @@
 // In 3 and 4 the blocks (expert, rows, 128 of K) are dealt to the CTAs evenly as one line; a tile that several CTAs have part of
 // is added up by the last to come, in the CTAs' order: results do not depend on timing.
 //
-// 1 token through 2 of 8 experts of 3 x 672 x 2,048: 21.8 us, of which routing and its barrier 5.7, lists 2, the first weights 3,
-// two hand-overs of a tile's shares some 4 each, the last barrier and sums 1.5.  16 tokens through 8 of 3 x 1,184 x 4,096: 40.8 us.  64
-// tokens through 64 of 3 x 1,024 x 2,048, 8 a token: 89.4 us for 214 MB, of which 28 until the first products (routing over 64 experts,
-// lists, x laid out), 29 gate and up at 4.9 TB/s, some 14 until an expert's h is whole, some 18 down.
+// 1 token through 2 of 8 experts of 3 x 672 x 2,048: 22.7 us, of which (taken at 21.4) routing and its barrier 5.7, lists 2, the
+// first weights 3, two hand-overs of a tile's shares some 4 each, the last barrier and sums 1.5.  16 tokens through 8 of 3 x 1,184 x
+// 4,096: 40.5 us.  64 tokens through 64 of 3 x 1,024 x 2,048, 8 a token: 89.4 us for 214 MB, of which 28 until the first products
+// (routing over 64 experts, lists, x laid out), 29 gate and up at 4.9 TB/s, and, taken before h had its third term, which added 4.5
+// to them, 12 until an expert's h is whole and 15 down.
 //
 // Warp 0 streams weights and their scales, warp 2 x and h, warp 1 issues the products, warps 4-11 take the sums out.  Every
 // wait is bounded; on expiry all CTAs learn of it and leave without a result: the error word is set, tensor memory is freed, the
