@@ -308,9 +308,8 @@ _tc_err = {}
 def _tc_err_word(device) -> torch.Tensor:
     """Device error word for the tensor-core GEMM's bounded waits (one per device)."""
     key = torch.device(device).index or 0
-    if key not in _tc_err:
-        _tc_err[key] = torch.zeros(1, dtype=torch.int32, device=device)
-    return _tc_err[key]
+    word = _tc_err.get(key)
+    return word if word is not None else _tc_err.setdefault(key, torch.zeros(1, dtype=torch.int32, device=device))       # of threads, the first one's
 
 
 _tc_ws = {}

@@ -106,3 +106,18 @@ def test_captured_calls_take_the_counters_that_they_use(mx, monkeypatch):
     monkeypatch.setattr(mx, "_ARENA", 250)
     call()
     assert arena[1] == 128 and given[-1] and not arena[0].data_ptr() <= given[-1] < arena[0].data_ptr() + 4 * arena[0].numel()
+
+
+def test_threads_share_one_error_word(monkeypatch):
+    """The word whose address is kept is the word that is read."""
+    from prism_b200 import ops
+    zeros = torch.zeros
+    monkeypatch.setattr(ops, "_tc_err", {})
+
+    def slow(*a, **k):
+        time.sleep(0.02)
+        return zeros(*a, **k)
+    monkeypatch.setattr(torch, "zeros", slow)
+    words = []
+    in_threads(4, lambda i: words.append(ops._tc_err_word(torch.device("cpu"))))
+    assert len(words) == 4 and all(w is ops._tc_err[0] for w in words)
