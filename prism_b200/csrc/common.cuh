@@ -25,6 +25,8 @@
 #define PRISM_ERR_PAGE_RANGE 2
 #define PRISM_ERR_POSITION_RANGE 3
 #define PRISM_ERR_WAIT_TIMEOUT 4
+#define PRISM_ERR_ADAPTER_RANGE 5
+#define PRISM_ERR_ROW_RANGE 6
 
 // which keys a position sees (all causal): every key, the last `size`, or its own block of `size` positions
 #define PRISM_MASK_CAUSAL 0

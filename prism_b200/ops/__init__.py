@@ -166,6 +166,8 @@ class _Sig:
     prism_mxfp4_moe_workspace = [_i, _i, _i, _i, _i, _i, _p]
     prism_sgemm_nt = [_p, _i, _p, _i, _p, _i, _p, _i, _i, _i, _i, _p]
     prism_sample = [_p, _i, _i, _i, _p, _p, _p, _p]
+    prism_sample_filtered = [_p, _ll, _i, _i, _i, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p]
+    prism_low_rank = [_p, _ll, _i, _p, _p, _p, _p, _p, _ll, _p, _ll, _i, _i, _i, _i, _i, _i, _i, _p, _i, _p, _p]
     prism_argmax_split = [_p, _i, _i, _i, _i, _p, _p, _p, _p, _p]
     prism_set_pdl = [_i]
     prism_gemm_tcgen05_supported = [_i, _i, _i]
@@ -190,6 +192,12 @@ def _cuda(*ts):
 
 
 launch_count = 0      # kernels of this library launched (or captured) by this process
+
+
+def _here(t: torch.Tensor, what: str):
+    """Launches go to the current device's current stream: a call for another device's tensors is refused."""
+    if t.device.index != torch._C._cuda_getDevice():
+        raise KernelError(f"{what}: tensors on {t.device} while the current device is cuda:{torch._C._cuda_getDevice()}")
 
 
 def _check(code: int, what: str):
@@ -428,13 +436,18 @@ def tc_ksplit_paired(N: int, K: int, sms: Optional[int] = None, M: Optional[int]
     return max(1, min((sms or num_sms()) // tiles, kblocks // 8))
 
 
+_ERR_TEXT = {5: "an adapter's number outside its stack", 6: "a row outside the logits"}       # csrc/common.cuh
+
+
 def check_tc_errors():
-    """Raise if a bounded wait of the tensor-core GEMM ran out (synchronises)."""
+    """Raise if a bounded wait of the tensor-core GEMM ran out, or a kernel met a number that it must not follow (synchronises)."""
     for word in _tc_err.values():
         code = int(word.item())
         if code:
             word.zero_()
             mxfp4._clear_counters()
+            if code in _ERR_TEXT:
+                raise KernelError(f"device error {code}: {_ERR_TEXT[code]}")
             raise KernelError(f"tensor-core GEMM: device error {code} (a bounded wait ran out)")
 
 
@@ -695,6 +708,44 @@ def sample(logits: torch.Tensor, temperature: Optional[torch.Tensor], u: Optiona
         return
     _check(lib().prism_sample(_ptr(logits), logits.stride(0), R, V, _ptr(temperature), _ptr(u),
                               _ptr(out), _stream()), "sample")
+
+
+def sample_filtered(logits: torch.Tensor, temperature: Optional[torch.Tensor], u: torch.Tensor, out: torch.Tensor,
+                    top_k: Optional[torch.Tensor] = None, top_p: Optional[torch.Tensor] = None, min_p: Optional[torch.Tensor] = None,
+                    rows: Optional[torch.Tensor] = None, kept: Optional[torch.Tensor] = None, logprob: Optional[torch.Tensor] = None):
+    """Per row: a token of ``softmax(logits / temperature)`` among those that the row's filters keep, at the uniform number ``u`` (in
+    ``[0, 1)``) of the inverse CDF.  ``top_k`` (int32; 0 or less: off) keeps the largest logits (the lower index of equal ones);
+    ``top_p`` (float32; 1 or more: off) the shortest run of the likeliest of these whose probability reaches that share of theirs, one at least;
+    ``min_p`` (float32; 0 or less: off) of these the ones at least ``min_p`` times as likely as the likeliest.  Temperature 0 or less
+    (or None for all rows): the largest, lowest index on ties.  NaN counts as -infinity, which is never kept; rows of nothing else give token
+    0.  +infinity leaves the probability to such logits alone.  Decided in 64-bit arithmetic and whole-number sums: a row's result
+    depends on its own logits and settings only.  ``rows`` (int32): only these rows of ``logits``, each at most once; the others' results are
+    left as they are.  Results by row of ``logits``: ``out`` (int32); ``kept`` (int32): how many tokens it was drawn from (1 if greedy; 0
+    for a row of nothing); ``logprob`` (float32): the logarithm of the probability that the token had among them (0 if greedy, -infinity
+    for a row of nothing)."""
+    _cuda(logits, temperature, u, out, top_k, top_p, min_p, rows, kept, logprob)
+    if logits.dim() != 2 or logits.dtype != torch.float32 or (logits.stride(1) != 1 and logits.shape[1] > 1) or logits.shape[1] < 1:
+        raise KernelError(f"sample_filtered: logits are float32 rows side by side in memory, got {tuple(logits.shape)} {logits.dtype}, strides "
+                          f"{logits.stride()}")
+    R, V = logits.shape
+    for name, t, dtype in (("temperature", temperature, torch.float32), ("u", u, torch.float32), ("out", out, torch.int32),
+                           ("top_k", top_k, torch.int32), ("top_p", top_p, torch.float32), ("min_p", min_p, torch.float32),
+                           ("kept", kept, torch.int32), ("logprob", logprob, torch.float32), ("rows", rows, torch.int32)):
+        if t is None:
+            if name in ("u", "out"):
+                raise KernelError(f"sample_filtered: no {name}")
+            continue
+        if t.dtype != dtype or not t.is_contiguous() or t.dim() != 1 or (t.shape[0] != R if name != "rows" else t.shape[0] > R) \
+                or t.device != logits.device:
+            raise KernelError(f"sample_filtered: {name} is {dtype} for each of the {R} rows, contiguous, on {logits.device}: got {t.dtype} "
+                              f"{tuple(t.shape)} on {t.device}")
+    _here(logits, "sample_filtered")
+    n = R if rows is None else rows.shape[0]
+    if n == 0:
+        return
+    _check(lib().prism_sample_filtered(_ptr(logits), logits.stride(0), n, R, V, _ptr(temperature), _ptr(u), _ptr(top_k), _ptr(top_p), _ptr(min_p),
+                                       _ptr(rows), _ptr(out), _ptr(kept), _ptr(logprob), _ptr(_tc_err_word(logits.device)), _stream()),
+           "sample_filtered")
 
 
 # --------------------------------------------------------------------------
@@ -2492,3 +2543,4 @@ def moe_feed_forward(ctx, x: torch.Tensor, logits: torch.Tensor, gate_up_w: torc
 
 from . import mxfp4      # noqa: E402
 from .mxfp4 import Mxfp4, mxfp4_linear, mxfp4_moe, mxfp4_quantize      # noqa: E402,F401
+from .low_rank import LowRank, low_rank      # noqa: E402,F401

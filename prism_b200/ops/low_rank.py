@@ -1,0 +1,125 @@
+"""Low-rank adapters of many requests at once, beside a projection that they
+share: ``out[t] = base[t] + s_l (x[t] A_l^T) B_l^T`` with l the adapter of
+token t's request.  andre-fu/prism has no adapters: a model with one of its own
+is a model of its own there (engine/weight_manager.py:45).
+
+``LowRank``     the adapters of one projection, stacked
+``low_rank``    their part of the projection's result, added to the shared part
+``Adapted``     a projection's matrix with its adapters: what ``linear`` and its kin take in place of the matrix
+"""
+
+from __future__ import annotations
+
+import ctypes
+from typing import Optional, Sequence
+
+import torch
+
+from .. import ops
+
+MOST_RANK, MOST_SLICES = 128, 8      # csrc/low_rank.cu
+RANK_UNIT, WIDTH_UNIT = 16, 8        # an adapter's rank in memory, and its A's rows, are whole numbers of these
+
+
+def _up(n: int, unit: int) -> int:
+    return -(-n // unit) * unit
+
+
+class LowRank:
+    """Adapters of one projection ``[N, K]``.  ``a [L, G, r, Kp]``: the A of each of the L adapters for each of the G slices of the
+    projection's rows (the matrices that it stacks: q, k and v, say), r rows each.  ``b [L, N, r]``: the rows of their B, all slices'
+    below each other.  ``rows``: how many of the N rows each slice has.  r is a multiple of 16 up to 128, with zeros beyond an adapter's
+    own rank; Kp is K rounded up to a multiple of 8 at least, with zeros beyond K.  ``scale``: float32 ``[L]``."""
+
+    __slots__ = ("a", "b", "scale", "rows", "k", "rank", "count", "n", "_first", "_address")
+
+    def __init__(self, a: torch.Tensor, b: torch.Tensor, scale: torch.Tensor, rows: Sequence[int], k: Optional[int] = None):
+        rows = tuple(int(n) for n in rows)
+        if a.dim() != 4 or b.dim() != 3 or not rows or min(rows) < 1 or len(rows) > MOST_SLICES:
+            raise ops.KernelError(f"adapters: A is [adapters, slices, rank, width] and B [adapters, rows, rank], of 1 to {MOST_SLICES} slices: got "
+                                  f"{tuple(a.shape)}, {tuple(b.shape)} and rows {rows}")
+        L, G, r, kp = a.shape
+        k = kp if k is None else int(k)
+        if G != len(rows) or b.shape != (L, sum(rows), r) or L < 1:
+            raise ops.KernelError(f"adapters: A {tuple(a.shape)}, B {tuple(b.shape)} and rows {rows} do not belong together")
+        if r % RANK_UNIT or not RANK_UNIT <= r <= MOST_RANK or kp % WIDTH_UNIT or not 1 <= k <= kp:
+            raise ops.KernelError(f"adapters: a rank in memory is a multiple of {RANK_UNIT} up to {MOST_RANK} and a row of A a multiple of {WIDTH_UNIT} "
+                                  f"that holds its {k} entries: got rank {r}, rows of {kp}")
+        if a.dtype not in (torch.bfloat16, torch.float32) or b.dtype != a.dtype or scale.dtype != torch.float32 or scale.shape != (L,):
+            raise ops.KernelError(f"adapters: A and B are both bfloat16 or both float32 and the scales float32 [{L}]: got {a.dtype}, {b.dtype}, "
+                                  f"{scale.dtype} {tuple(scale.shape)}")
+        if not (a.is_contiguous() and b.is_contiguous() and scale.is_contiguous()) or a.data_ptr() % 16 or b.data_ptr() % 16 \
+                or not a.device == b.device == scale.device:
+            raise ops.KernelError("adapters: A, B and the scales lie contiguous on one device, A and B from a 16-byte border on")
+        self.a, self.b, self.scale, self.rows, self.k, self.rank, self.count, self.n = a, b, scale, rows, k, r, L, sum(rows)
+        first = [sum(rows[:g]) for g in range(G + 1)]
+        self._first = (ctypes.c_int * (G + 1))(*first)
+        self._address = ctypes.addressof(self._first)
+
+    @classmethod
+    def empty(cls, count: int, rank: int, rows: Sequence[int], k: int, dtype: torch.dtype, device) -> "LowRank":
+        """Room for ``count`` adapters of ranks up to ``rank``, all zero (an adapter of zeros adds nothing)."""
+        r, kp = _up(int(rank), RANK_UNIT), _up(int(k), WIDTH_UNIT)
+        return cls(torch.zeros((count, len(rows), r, kp), dtype=dtype, device=device), torch.zeros((count, sum(rows), r), dtype=dtype, device=device),
+                   torch.zeros(count, dtype=torch.float32, device=device), rows, k)
+
+    @property
+    def nbytes(self) -> int:
+        return sum(t.numel() * t.element_size() for t in (self.a, self.b, self.scale))
+
+    def put(self, index: int, slices, scale: float) -> None:
+        """Adapter ``index``: per slice its ``(A [rank, K], B [rows, rank])``, or None where it has none."""
+        if not 0 <= index < self.count or len(slices) != len(self.rows):
+            raise ops.KernelError(f"adapter {index} of {self.count} with {len(slices)} of {len(self.rows)} slices")
+        for g, ab in enumerate(slices):
+            if ab is not None and not (ab[0].dim() == 2 and ab[0].shape[0] <= self.rank and ab[0].shape[1] == self.k
+                                       and ab[1].shape == (self.rows[g], ab[0].shape[0])):
+                raise ops.KernelError(f"adapter {index}: A {tuple(ab[0].shape)} and B {tuple(ab[1].shape)} for a matrix [{self.rows[g]}, {self.k}] and "
+                                      f"ranks up to {self.rank}")
+        self.a[index].zero_()
+        self.b[index].zero_()
+        self.scale[index] = float(scale)
+        for g, ab in enumerate(slices):
+            if ab is not None:
+                rank, at = ab[0].shape[0], self._first[g]
+                self.a[index, g, :rank, :self.k].copy_(ab[0])
+                self.b[index, at:at + self.rows[g], :rank].copy_(ab[1])
+
+
+SINGLES = 64                 # without a word from the caller, so many tokens are taken one by one
+
+
+def low_rank(x: torch.Tensor, low: LowRank, ids: torch.Tensor, base: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
+             singles: Optional[int] = None) -> torch.Tensor:
+    """``out[t] = base[t] + scale[l] (x[t] A_l^T) B_l^T`` with ``l = ids[t]`` (int32 ``[T]`` on the device; negative: ``out[t] = base[t]``).
+    ``x [T, K]`` in the adapters' dtype; ``base`` and ``out [T, N]`` both bfloat16 or both float32, rows may have strides of their own;
+    ``base`` None: zeros; ``out`` may be ``base`` itself.  Sums in float32, one rounding.  ``singles``: so many tokens from the first on are
+    each a request of its own, and the others stand in runs of one adapter (as in a step: decoding requests, then portions of
+    prompts); this says how the work is laid out and changes no result's meaning.  An id outside the stack adds nothing and is reported by
+    ``check_tc_errors``."""
+    a = low.a
+    if not (x.is_cuda and a.is_cuda and ids.is_cuda and (base is None or base.is_cuda) and (out is None or out.is_cuda)):
+        ops._cuda(x, a, ids, base, out)
+    if x.dim() != 2 or x.shape[1] != low.k or x.dtype is not a.dtype or (x.stride(1) != 1 and low.k > 1):
+        raise ops.KernelError(f"adapters in {a.dtype} for rows of {low.k} side by side in memory: got {tuple(x.shape)} {x.dtype}, strides {x.stride()}")
+    T, N = x.shape[0], low.n
+    if ids.shape != (T,) or ids.dtype is not torch.int32 or not ids.is_contiguous():
+        raise ops.KernelError(f"adapters' numbers are int32 [{T}], contiguous: got {ids.dtype} {tuple(ids.shape)}")
+    if out is None:
+        out = x.new_empty((T, N), dtype=None if base is None else base.dtype)
+    for t, name in ((base, "base"), (out, "out")):
+        if t is not None and (t.shape != (T, N) or t.dtype not in (torch.bfloat16, torch.float32) or (t.stride(1) != 1 and N > 1)
+                              or (T > 1 and t.stride(0) < N) or t.device != x.device or t.dtype is not out.dtype):
+            raise ops.KernelError(f"{name} of {T} rows and {N} columns, bfloat16 or float32 as the other: got {tuple(t.shape)} {t.dtype}, strides "
+                                  f"{t.stride()} on {t.device}")
+    if a.device != x.device or ids.device != x.device:
+        raise ops.KernelError(f"adapters on {a.device} and their numbers on {ids.device} beside rows on {x.device}")
+    ops._here(x, "low_rank")
+    if T == 0:
+        return out
+    singles = (T if T <= SINGLES else 0) if singles is None else max(0, min(int(singles), T))
+    ops._check(ops.lib().prism_low_rank(x.data_ptr(), x.stride(0), ops._dt(x), a.data_ptr(), low.b.data_ptr(), low.scale.data_ptr(), ids.data_ptr(),
+                                        None if base is None else base.data_ptr(), 0 if base is None else base.stride(0), out.data_ptr(), out.stride(0),
+                                        ops._dt(out), T, low.k, a.shape[3], low.rank, low.count, len(low.rows), low._address, singles,
+                                        ops.mxfp4._err_word(x.device), ops._stream()), "low_rank")
+    return out
