@@ -120,6 +120,6 @@ def low_rank(x: torch.Tensor, low: LowRank, ids: torch.Tensor, base: Optional[to
     singles = (T if T <= SINGLES else 0) if singles is None else max(0, min(int(singles), T))
     ops._check(ops.lib().prism_low_rank(x.data_ptr(), x.stride(0), ops._dt(x), a.data_ptr(), low.b.data_ptr(), low.scale.data_ptr(), ids.data_ptr(),
                                         None if base is None else base.data_ptr(), 0 if base is None else base.stride(0), out.data_ptr(), out.stride(0),
-                                        ops._dt(out), T, low.k, a.shape[3], low.rank, low.count, len(low.rows), low._address, singles,
+                                        ops._dt(out), T, low.k, a.shape[3], low.rank, low.count, len(low.rows), low._address, singles, ops.num_sms(x.device),
                                         ops.mxfp4._err_word(x.device), ops._stream()), "low_rank")
     return out
