@@ -1,0 +1,475 @@
+// Low-rank adapters (low_rank.cu has the formula) for portions of prompts: tiles of 128 tokens on the 5th-generation tensor cores, bfloat16 adapters.
+//
+// Two launches.  The first forms the hidden values: a cluster of eight CTAs has a tile of tokens, each CTA every eighth block of 64 k of x and of all
+// slices' A (TMA, 128-byte swizzle, tcgen05.mma with the tokens as M); their sums meet through distributed shared memory, are scaled and leave as
+// two bfloat16 terms, high and low (2^-16 of a hidden value is lost; one term alone would lose 2^-8, as much as rounding the result does).  The
+// second multiplies them with B, 128 columns at a time, and adds the shared result: it is bound by reading and writing that - the 7B shape's gate
+// and up for 2,048 tokens are 310 MB against 28 MB of everything else.
+//
+// A tile's tokens may have several adapters: it is gone through once for each of them, and only that adapter's rows are stored.
+#include "tcgen05.cuh"
+#include "vec.cuh"
+
+namespace prism {
+namespace lowrank {
+
+using namespace prism::tc;
+constexpr int TILE = 128;                     // tokens of a tile, and columns of one of B
+constexpr int BLOCK_BYTES = TILE * TILE_K * 2;
+constexpr int CTAS = 8;                       // that share a tile's K
+constexpr int EPI_WARPS = 8, EPI_THREADS = EPI_WARPS * 32, ALL_THREADS = EPI_THREADS + 64;
+constexpr int MOST_RANK = 128, MOST_SLICES = 8, MOST_HIDDEN = 512;
+constexpr int CHUNK = 64, CHUNK_LD = CHUNK + 4;                   // columns of sums on their way through shared memory, and their pitch
+
+struct Tiles {
+    int n, first[MOST_SLICES + 1];            // slice g has the result columns first[g] .. first[g + 1] - 1
+    int units[MOST_SLICES + 1];               // of the second launch: slice g has the CTAs units[g] .. units[g + 1] - 1 of a tile
+};
+
+// The tokens' adapters (-1: none, or beyond the end) and the different ones among them, in order.  By one warp.
+__device__ __forceinline__ void list_adapters(const int* ids, int t0, int tokens, int L, int* own, int* list, int* count, int* err) {
+    const int lane = threadIdx.x & 31;
+    int n = 0;
+    for (int q = 0; q < TILE / 32; ++q) {
+        const int t = t0 + q * 32 + lane;
+        int id = t < tokens ? ids[t] : -1;
+        if (id >= L) {
+            report_error(err, PRISM_ERR_ADAPTER_RANGE);
+            id = -1;
+        }
+        id = max(id, -1);
+        own[q * 32 + lane] = id;
+        const uint32_t same = __match_any_sync(0xffffffffu, id);
+        bool first = id >= 0 && __ffs(same) - 1 == lane;
+        for (int i = 0; i < n; ++i) first = first && list[i] != id;
+        const uint32_t found = __ballot_sync(0xffffffffu, first);
+        if (first) list[n + __popc(found & ((1u << lane) - 1))] = id;
+        n += __popc(found);
+        __syncwarp();
+    }
+    if (lane == 0) *count = n;
+}
+
+__device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(bar)) : "memory");
+}
+__device__ __forceinline__ uint32_t instruction(int n) {
+    return (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(TILE >> 4) << 24);
+}
+__device__ __forceinline__ void epilogue_barrier() { asm volatile("bar.sync 1, %0;" ::"n"(EPI_THREADS) : "memory"); }
+
+// ---- hidden values ------------------------------------------------------------------------------------------
+
+// hidden: [2][tokens][G r], high terms and low ones
+__global__ void __launch_bounds__(ALL_THREADS)
+low_rank_hidden_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_a, const float* __restrict__ scale,
+                       const int* __restrict__ ids_, __nv_bfloat16* __restrict__ hidden, int tokens, int K, int r, int G, int L, int stages,
+                       int tmem_cols, int* err) {
+    extern __shared__ unsigned char raw[];
+    unsigned char* ring = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
+    const int H = G * r, stage_bytes = BLOCK_BYTES + H * TILE_K * 2;
+    float* sums = reinterpret_cast<float*>(ring + (size_t)stages * stage_bytes);
+    __shared__ uint64_t full[8], empty[8], done;
+    __shared__ uint32_t tmem_slot;
+    __shared__ int abort_flag, own[TILE], list[TILE], count;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, me = blockIdx.x, t0 = blockIdx.y * TILE;
+    const int blocks = (K + TILE_K - 1) / TILE_K, mine = blocks > me ? (blocks - me + CTAS - 1) / CTAS : 0;
+    volatile int* abortp = &abort_flag;
+
+    if (threadIdx.x == 0) {
+        abort_flag = 0;
+        for (int s = 0; s < stages; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+        mbar_init(&done, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&tmem_slot)), "r"(tmem_cols));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
+    }
+    pdl_wait();
+    if (warp == 2) list_adapters(pdl_fresh(ids_), t0, tokens, L, own, list, &count, me == 0 ? err : nullptr);
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem = tmem_slot;
+    const int passes = count;
+    pdl_trigger();                            // not before this CTA has its tensor memory: a kernel that waits for this one may hold the rest
+
+    int it = 0;                               // blocks so far, over all passes
+    bool go = true;                           // no wait of this warp has run out
+    for (int p = 0; p < passes; ++p) {
+        const int l = list[p];
+        if (warp == 0) {
+            if (lane == 0) {
+                int issued = 0;
+                for (int i = 0; i < mine; ++i) {
+                    const int s = (it + i) % stages, round = (it + i) / stages;
+                    if (round > 0 && !mbar_wait(&empty[s], (round - 1) & 1, abortp)) break;
+                    unsigned char* st = ring + (size_t)s * stage_bytes;
+                    mbar_expect_tx(&full[s], stage_bytes);
+                    const int k = (me + i * CTAS) * TILE_K;
+                    tma_load_2d(st, &map_x, &full[s], k, t0);
+                    for (int g = 0; g < G; ++g)
+                        tma_load_2d(st + BLOCK_BYTES + (size_t)g * r * TILE_K * 2, &map_a, &full[s], k, (l * G + g) * r);
+                    issued = i + 1;
+                }
+                if (*abortp)                  // copies in flight get a bounded chance to land before the memory is used otherwise
+                    for (int i = max(0, issued - stages); i < issued; ++i) mbar_wait(&full[(it + i) % stages], ((it + i) / stages) & 1, abortp);
+            }
+        } else if (warp == 1) {
+            if (lane == 0) {
+                const uint32_t idesc = instruction(r);
+                bool ok = true;
+                for (int i = 0; i < mine && ok; ++i) {
+                    const int s = (it + i) % stages;
+                    ok = mbar_wait(&full[s], ((it + i) / stages) & 1, abortp);
+                    if (!ok) break;
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    const uint32_t st = smem_addr(ring + (size_t)s * stage_bytes);
+                    const uint64_t dx = umma_desc(st);
+                    for (int g = 0; g < G; ++g) {
+                        // a slice's rows start on 8 rows of 128 bytes, as r is a multiple of 16
+                        const uint64_t da = umma_desc(st + BLOCK_BYTES + g * r * TILE_K * 2);
+#pragma unroll
+                        for (int k = 0; k < TILE_K / UMMA_K; ++k)
+                            umma_bf16(tmem + g * r, dx + (uint64_t)(k * UMMA_K * 2 >> 4), da + (uint64_t)(k * UMMA_K * 2 >> 4), idesc, (i > 0 || k > 0) ? 1u : 0u);
+                    }
+                    umma_commit(&empty[s]);
+                }
+                umma_commit(&done);
+            }
+        }
+        __syncwarp();
+        const int q = warp & 3, half = (warp - 2) >> 2, tid = threadIdx.x - 64;        // of the epilogue's warps
+        if (warp >= 2) {
+            if (mine > 0) go = __all_sync(0xffffffffu, mbar_wait(&done, p & 1, abortp)) && go;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        }
+        for (int c0 = 0; c0 < H; c0 += CHUNK) {
+            if (warp >= 2) {
+                // this CTA's sums: a thread's row is its tensor memory lane
+                const int c = c0 + half * 32;
+                if (c < H) {
+                    float v[32];
+                    if (mine > 0 && go) {
+                        tmem_load<32>(tmem + ((uint32_t)(q * 32) << 16) + c, v);       // columns beyond H are allocated, and not used
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) v[i] = 0.f;
+                    }
+                    float* row = sums + (q * 32 + lane) * CHUNK_LD + half * 32;
+#pragma unroll
+                    for (int i = 0; i < 32; i += 4) *reinterpret_cast<float4*>(row + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+                }
+            }
+            asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+            if (warp >= 2) {
+                // sixteen rows of all CTAs' sums: four columns a thread
+                const int row = me * (TILE / CTAS) + tid / (CHUNK / 4), c = tid % (CHUNK / 4) * 4, t = t0 + row;
+                if (c0 + c < H && own[row] == l && go) {
+                    const uint32_t at = smem_addr(sums + row * CHUNK_LD + c);
+                    float4 part[CTAS];
+#pragma unroll
+                    for (int j = 0; j < CTAS; ++j) {
+                        uint32_t peer;
+                        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(peer) : "r"(at), "r"(j));
+                        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                                     : "=f"(part[j].x), "=f"(part[j].y), "=f"(part[j].z), "=f"(part[j].w) : "r"(peer) : "memory");
+                    }
+                    float v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int j = 0; j < CTAS; ++j) v[0] += part[j].x, v[1] += part[j].y, v[2] += part[j].z, v[3] += part[j].w;
+                    const float s = scale[l];
+                    __nv_bfloat16 hi[4], lo[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float h = v[i] * s;
+                        hi[i] = __float2bfloat16_rn(h);
+                        const float rest = h - __bfloat162float(hi[i]);
+                        lo[i] = __float2bfloat16_rn(rest == rest ? rest : 0.f);        // an infinity's rest is none
+                    }
+                    __nv_bfloat16* to = hidden + (size_t)t * H + c0 + c;
+                    *reinterpret_cast<uint2*>(to) = *reinterpret_cast<uint2*>(hi);
+                    *reinterpret_cast<uint2*>(to + (size_t)tokens * H) = *reinterpret_cast<uint2*>(lo);
+                }
+            }
+            asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+        }
+        it += mine;
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+        __syncthreads();                      // the sums have been read: the next pass may write them
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    }
+    if (threadIdx.x == 0 && abort_flag) report_error(err, PRISM_ERR_WAIT_TIMEOUT);
+    if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(tmem_cols));
+}
+
+// ---- results ------------------------------------------------------------------------------------------------
+
+template <typename O> struct Eight;           // eight neighbouring results, 16 or 32 bytes
+template <> struct Eight<__nv_bfloat16> {
+    uint4 raw;
+    __device__ __forceinline__ void load(const __nv_bfloat16* p) { raw = *reinterpret_cast<const uint4*>(p); }
+    __device__ __forceinline__ void zero() { raw = make_uint4(0, 0, 0, 0); }
+    __device__ __forceinline__ void get(float (&v)[8]) const { load8(reinterpret_cast<const __nv_bfloat16*>(&raw), v); }
+};
+template <> struct Eight<float> {
+    float4 a, b;
+    __device__ __forceinline__ void load(const float* p) { a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1]; }
+    __device__ __forceinline__ void zero() { a = b = make_float4(0, 0, 0, 0); }
+    __device__ __forceinline__ void get(float (&v)[8]) const {
+        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+    }
+};
+
+template <typename O>
+__global__ void __launch_bounds__(ALL_THREADS)
+low_rank_result_kernel(const __grid_constant__ CUtensorMap map_b, const __nv_bfloat16* __restrict__ hidden_, const int* __restrict__ ids_,
+                       const O* base, long long ldb, O* out, long long ldo, int aligned, int tokens, int r, int N, int L, Tiles tiles, int* err) {
+    constexpr int STAGES = 2;
+    extern __shared__ unsigned char raw[];
+    unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
+    const int kblocks = (r + TILE_K - 1) / TILE_K;
+    unsigned char* h_hi = smem;
+    unsigned char* ring = smem + 2 * kblocks * BLOCK_BYTES;                            // behind the low terms
+    float* sums = reinterpret_cast<float*>(ring + STAGES * kblocks * BLOCK_BYTES);
+    __shared__ uint64_t full[STAGES], empty[STAGES], acc_full[2], acc_empty[2], h_full;
+    __shared__ uint32_t tmem_slot;
+    __shared__ int abort_flag, own[TILE], list[TILE], count;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, t0 = blockIdx.y * TILE;
+    volatile int* abortp = &abort_flag;
+    int g = 0;
+    while (g + 1 < tiles.n && (int)blockIdx.x >= tiles.units[g + 1]) ++g;
+    // this CTA's tiles of the slice's columns
+    const int n_first = tiles.first[g], n_end = tiles.first[g + 1], all = (n_end - n_first + TILE - 1) / TILE;
+    const int units = tiles.units[g + 1] - tiles.units[g], unit = blockIdx.x - tiles.units[g];
+    const int j0 = (int)((long long)all * unit / units), j1 = (int)((long long)all * (unit + 1) / units);
+
+    if (threadIdx.x == 0) {
+        abort_flag = 0;
+        for (int s = 0; s < STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+        for (int s = 0; s < 2; ++s) { mbar_init(&acc_full[s], 1); mbar_init(&acc_empty[s], EPI_WARPS); }
+        mbar_init(&h_full, EPI_THREADS);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&tmem_slot)), "r"(2 * TILE));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
+    }
+    pdl_wait();
+    if (warp == 2) list_adapters(pdl_fresh(ids_), t0, tokens, L, own, list, &count, nullptr);
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem = tmem_slot;
+    const int passes = count;
+    pdl_trigger();                            // not before this CTA has its tensor memory: a kernel that waits for this one may hold the rest
+
+    if (warp == 0) {
+        if (lane == 0) {
+            int i = 0;
+            for (int p = 0; p < passes && !*abortp; ++p)
+                for (int j = j0; j < j1; ++j, ++i) {
+                    const int s = i % STAGES;
+                    if (i >= STAGES && !mbar_wait(&empty[s], (i / STAGES - 1) & 1, abortp)) break;
+                    mbar_expect_tx(&full[s], kblocks * BLOCK_BYTES);
+                    for (int k = 0; k < kblocks; ++k)
+                        tma_load_2d(ring + (s * kblocks + k) * BLOCK_BYTES, &map_b, &full[s], k * TILE_K, list[p] * N + n_first + j * TILE);
+                }
+            if (*abortp)
+                for (int k = max(0, i - STAGES); k < i; ++k) mbar_wait(&full[k % STAGES], (k / STAGES) & 1, abortp);
+        }
+    } else if (warp == 1) {
+        if (lane == 0) {
+            const uint32_t idesc = instruction(TILE);
+            int i = 0;
+            bool ok = true;
+            for (int p = 0; p < passes && ok; ++p) {
+                ok = mbar_wait(&h_full, p & 1, abortp);
+                for (int j = j0; j < j1 && ok; ++j, ++i) {
+                    const int s = i % STAGES, buf = i & 1;
+                    ok = mbar_wait(&full[s], (i / STAGES) & 1, abortp) && (i < 2 || mbar_wait(&acc_empty[buf], (i / 2 - 1) & 1, abortp));
+                    if (!ok) break;
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    const uint32_t d = tmem + buf * TILE;
+                    for (int k = 0; k < r / UMMA_K; ++k) {
+                        const int block = k / 4, in = k % 4;
+                        const uint64_t db = umma_desc(smem_addr(ring + (s * kblocks + block) * BLOCK_BYTES)) + (uint64_t)(in * UMMA_K * 2 >> 4);
+                        const uint64_t dh = umma_desc(smem_addr(h_hi + block * BLOCK_BYTES)) + (uint64_t)(in * UMMA_K * 2 >> 4);
+                        const uint64_t dl = umma_desc(smem_addr(h_hi + (kblocks + block) * BLOCK_BYTES)) + (uint64_t)(in * UMMA_K * 2 >> 4);
+                        umma_bf16(d, dh, db, idesc, k > 0 ? 1u : 0u);
+                        umma_bf16(d, dl, db, idesc, 1u);
+                    }
+                    umma_commit(&empty[s]);
+                    umma_commit(&acc_full[buf]);
+                }
+            }
+        }
+    } else {
+        const int tid = threadIdx.x - 64, q = warp & 3, part = (warp - 2) >> 2;
+        const int H = tiles.n * r;
+        // after a wait that ran out the loops go on, as the barriers of these threads count on all of them, but touch nothing
+        int i = 0;
+        bool ok = true;
+        for (int p = 0; p < passes; ++p) {
+            const int l = list[p];
+            {
+                // the adapter's hidden rows as operands, the others zero: high terms by one half of the threads, low ones by the other
+                const int row = tid % TILE, term = tid / TILE;
+                const bool mine = own[row] == l;
+                const uint4* from = reinterpret_cast<const uint4*>(pdl_fresh(hidden_) + ((size_t)term * tokens + (mine ? t0 + row : 0)) * H + g * r);
+                unsigned char* to = h_hi + term * kblocks * BLOCK_BYTES + row * 128;
+#pragma unroll 4
+                for (int c = 0; c < r / 8; ++c)
+                    *reinterpret_cast<uint4*>(to + c / 8 * BLOCK_BYTES + ((c % 8) ^ (row & 7)) * 16) = mine ? from[c] : make_uint4(0, 0, 0, 0);
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                mbar_arrive(&h_full);
+            }
+            for (int j = j0; j < j1; ++j, ++i) {
+                const int buf = i & 1;
+#pragma unroll 1
+                for (int c0 = 0; c0 < TILE; c0 += CHUNK) {
+                    const int n0 = n_first + j * TILE + c0, wide = min(CHUNK, n_end - n0);
+                    // what the result is added to, asked for before the sums are waited for: eight columns of four rows a thread
+                    const int c = tid % 8 * 8, row0 = tid / 8;
+                    const bool whole = aligned && n0 % 8 == 0 && c + 8 <= wide;
+                    Eight<O> old[4];
+#pragma unroll
+                    for (int m = 0; m < 4; ++m) {
+                        const int row = row0 + 32 * m;
+                        old[m].zero();
+                        if (whole && base && own[row] == l) old[m].load(base + (size_t)(t0 + row) * ldb + n0 + c);
+                    }
+                    if (c0 == 0) {
+                        ok = __all_sync(0xffffffffu, mbar_wait(&acc_full[buf], (i / 2) & 1, abortp)) && ok;
+                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    }
+                    if (wide > 0 && ok) {
+                        float v[32];
+                        tmem_load<32>(tmem + ((uint32_t)(q * 32) << 16) + buf * TILE + c0 + part * 32, v);
+                        float* row = sums + (q * 32 + lane) * CHUNK_LD + part * 32;
+#pragma unroll
+                        for (int e = 0; e < 32; e += 4) *reinterpret_cast<float4*>(row + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+                    }
+                    if (c0 + CHUNK >= TILE) {                      // the accumulator has been read
+                        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&acc_empty[buf]);
+                    }
+                    epilogue_barrier();
+                    if (ok)
+#pragma unroll
+                        for (int m = 0; m < 4; ++m) {
+                            const int row = row0 + 32 * m;
+                            if (own[row] != l || c >= wide) continue;
+                            float v[8], s[8];
+                            load8(sums + row * CHUNK_LD + c, s);
+                            O* to = out + (size_t)(t0 + row) * ldo + n0 + c;
+                            if (whole) {
+                                old[m].get(v);
+#pragma unroll
+                                for (int e = 0; e < 8; ++e) v[e] += s[e];
+                                store8(to, v);
+                            } else {
+                                for (int e = 0; e < min(8, wide - c); ++e)
+                                    to[e] = from_float<O>(base ? to_float(base[(size_t)(t0 + row) * ldb + n0 + c + e]) + s[e] : s[e]);
+                            }
+                        }
+                    epilogue_barrier();
+                }
+            }
+        }
+        if ((const O*)out != base) {          // tokens without an adapter
+            const int n0 = n_first + j0 * TILE, n1 = min(n_end, n_first + j1 * TILE);
+            for (int row = warp - 2; row < TILE; row += EPI_WARPS)
+                if (own[row] < 0 && t0 + row < tokens)
+                    for (int n = n0 + lane; n < n1; n += 32)
+                        out[(size_t)(t0 + row) * ldo + n] = base ? base[(size_t)(t0 + row) * ldb + n] : from_float<O>(0.f);
+        }
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    if (threadIdx.x == 0 && abort_flag) report_error(err, PRISM_ERR_WAIT_TIMEOUT);
+    if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * TILE));
+}
+
+}  // namespace lowrank
+}  // namespace prism
+
+// Whether the tiles take these sizes: x rows that TMA can read, hidden values of all slices in tensor memory.
+PRISM_EXPORT int prism_low_rank_tile_supported(int K, int r, int G, int x_aligned) {
+    using namespace prism::lowrank;
+    return x_aligned && K >= 1 && r >= 16 && r % 16 == 0 && r <= MOST_RANK && G >= 1 && G <= MOST_SLICES && G * r <= MOST_HIDDEN;
+}
+
+// bfloat16 x and adapters, all T tokens in tiles; arguments as prism_low_rank's.  hidden: 2 T G r bfloat16 of workspace.
+PRISM_EXPORT int prism_low_rank_tile(const void* x, long long ldx, const void* a, const void* b, const float* scale, const int* ids, const void* base,
+                                     long long ldb, void* out, long long ldo, int out_dtype, int T, int K, int Kp, int r, int L, int G, const int* first,
+                                     void* hidden, int sms, int* err, cudaStream_t stream) {
+    using namespace prism::lowrank;
+    typedef __nv_bfloat16 bf16;
+    if (T <= 0) return 0;
+    const bool x_aligned = reinterpret_cast<uintptr_t>(x) % 16 == 0 && (ldx % 8 == 0 || T == 1);
+    if (!prism_low_rank_tile_supported(K, r, G, x_aligned) || Kp < K || Kp % 8 || L < 1 || sms < 1 || (T + TILE - 1) / TILE > 65535)
+        return (int)cudaErrorInvalidValue;
+    Tiles s;
+    s.n = G;
+    for (int g = 0; g <= G; ++g) s.first[g] = first[g];
+    long long all = 0;
+    for (int g = 0; g < G; ++g) {
+        if (s.first[g] >= s.first[g + 1]) return (int)cudaErrorInvalidValue;
+        all += (s.first[g + 1] - s.first[g] + TILE - 1) / TILE;
+    }
+    const int N = first[G], tiles = (T + TILE - 1) / TILE, H = G * r;
+    if ((long long)L * N >= 1ll << 31 || (long long)L * H >= 1ll << 31) return (int)cudaErrorInvalidValue;
+    CUtensorMap map_x, map_a, map_b;
+    // a box of r rows of A: a slice's
+    int code = prism::tc::make_map(&map_x, x, T, K, T > 1 ? ldx : (K + 7) / 8 * 8, TILE);
+    if (code == 0) code = prism::tc::make_map(&map_a, a, (long long)L * H, Kp, Kp, r);
+    if (code == 0) code = prism::tc::make_map(&map_b, b, (long long)L * N, r, r, TILE);
+    if (code != 0) return code;
+
+    const int stage = BLOCK_BYTES + H * prism::tc::TILE_K * 2, sums = TILE * CHUNK_LD * 4;
+    const int stages = min(6, (190 * 1024 - sums) / stage);
+    int cols = 32;
+    while (cols < H) cols *= 2;
+    size_t smem = 1024 + (size_t)stages * stage + sums;
+    prism::open_smem(low_rank_hidden_kernel, smem);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(CTAS, tiles);
+    cfg.blockDim = dim3(ALL_THREADS);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = CTAS, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = prism::pdl_enabled() ? 2 : 1;
+    code = (int)cudaLaunchKernelEx(&cfg, low_rank_hidden_kernel, map_x, map_a, scale, ids, (bf16*)hidden, T, K, r, G, L, stages, cols, err);
+    if (code != 0) return code;
+
+    // the second launch: two CTAs an SM, as their shared memory allows, share the tiles of results; a CTA has some columns of one slice
+    const int kblocks = (r + prism::tc::TILE_K - 1) / prism::tc::TILE_K;
+    smem = 1024 + (size_t)(2 + 2) * kblocks * BLOCK_BYTES + sums;
+    const int slots = (smem <= 110 * 1024 ? 2 : 1) * sms;
+    const double per = all <= slots / tiles ? 1.0 : (double)all * tiles / slots;       // tiles of columns a CTA
+    s.units[0] = 0;
+    for (int g = 0; g < G; ++g) {
+        const int mine = (s.first[g + 1] - s.first[g] + TILE - 1) / TILE;
+        s.units[g + 1] = s.units[g] + max(1, min(mine, (int)(mine / per)));
+    }
+    const int aligned = reinterpret_cast<uintptr_t>(out) % 16 == 0 && reinterpret_cast<uintptr_t>(base) % 16 == 0 &&
+                        (T == 1 || (ldo % 8 == 0 && (base == nullptr || ldb % 8 == 0)));
+    const dim3 grid(s.units[G], tiles);
+    if (out_dtype == PRISM_DTYPE_F32) {
+        prism::open_smem(low_rank_result_kernel<float>, smem);
+        return (int)prism::launch_kernel(low_rank_result_kernel<float>, grid, dim3(ALL_THREADS), smem, stream, map_b, (const bf16*)hidden, ids, (const float*)base,
+                                         ldb, (float*)out, ldo, aligned, T, r, N, L, s, err);
+    }
+    prism::open_smem(low_rank_result_kernel<bf16>, smem);
+    return (int)prism::launch_kernel(low_rank_result_kernel<bf16>, grid, dim3(ALL_THREADS), smem, stream, map_b, (const bf16*)hidden, ids, (const bf16*)base, ldb,
+                                     (bf16*)out, ldo, aligned, T, r, N, L, s, err);
+}

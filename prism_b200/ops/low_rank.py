@@ -87,6 +87,7 @@ class LowRank:
 
 
 SINGLES = 64                 # without a word from the caller, so many tokens are taken one by one
+TILE_FROM = 16               # so many tokens of portions, and they are taken in tiles of 128
 
 
 def low_rank(x: torch.Tensor, low: LowRank, ids: torch.Tensor, base: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
@@ -118,8 +119,25 @@ def low_rank(x: torch.Tensor, low: LowRank, ids: torch.Tensor, base: Optional[to
     if T == 0:
         return out
     singles = (T if T <= SINGLES else 0) if singles is None else max(0, min(int(singles), T))
-    ops._check(ops.lib().prism_low_rank(x.data_ptr(), x.stride(0), ops._dt(x), a.data_ptr(), low.b.data_ptr(), low.scale.data_ptr(), ids.data_ptr(),
-                                        None if base is None else base.data_ptr(), 0 if base is None else base.stride(0), out.data_ptr(), out.stride(0),
-                                        ops._dt(out), T, low.k, a.shape[3], low.rank, low.count, len(low.rows), low._address, singles, ops.num_sms(x.device),
-                                        ops.mxfp4._err_word(x.device), ops._stream()), "low_rank")
+    L = ops.lib()
+    xp, xs, bp, bs, op, os_ = x.data_ptr(), x.stride(0), 0 if base is None else base.data_ptr(), 0 if base is None else base.stride(0), out.data_ptr(), \
+        out.stride(0)
+    what = (low.scale.data_ptr(), ids.data_ptr())
+    sizes = (low.k, a.shape[3], low.rank, low.count, len(low.rows), low._address)
+    sms, err, stream, dt, odt = ops.num_sms(x.device), ops.mxfp4._err_word(x.device), ops._stream(), ops._dt(x), ops._dt(out)
+    tiled = 0
+    if T - singles >= TILE_FROM and dt == ops.BF16:
+        skip = singles * xs * 2
+        if L.prism_low_rank_tile_supported(low.k, low.rank, len(low.rows), (xp + skip) % 16 == 0 and (xs % 8 == 0 or T - singles == 1)):
+            tiled = T - singles
+    if T > tiled:
+        ops._check(L.prism_low_rank(xp, xs, dt, a.data_ptr(), low.b.data_ptr(), *what, bp or None, bs, op, os_, odt, T - tiled, *sizes,
+                                    min(singles, T - tiled), sms, err, stream), "low_rank")
+    if tiled:
+        size = 2 if odt == ops.BF16 else 4
+        hidden = torch.empty(2 * tiled * len(low.rows) * low.rank, dtype=torch.bfloat16, device=x.device)
+        ops._check(L.prism_low_rank_tile(xp + singles * xs * 2, xs, a.data_ptr(), low.b.data_ptr(), what[0], what[1] + 4 * singles,
+                                         bp + singles * bs * size if bp else None, bs, op + singles * os_ * size, os_, odt, tiled, *sizes,
+                                         hidden.data_ptr(), sms, err, stream), "low_rank_tile")
+        ops.launch_count += 1                # two kernels
     return out
