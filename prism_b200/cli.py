@@ -27,6 +27,10 @@ def build_parser() -> argparse.ArgumentParser:
     p.add_argument("--max-tokens", type=int, default=100, help="Max new tokens")
     p.add_argument("--dtype", default="bfloat16", choices=["bfloat16", "float32"], help="Model dtype")
     p.add_argument("--temperature", type=float, default=0.0)
+    p.add_argument("--top-k", type=int, default=0, help="with --temperature: draw from the k likeliest tokens (0: all)")
+    p.add_argument("--top-p", type=float, default=1.0, help="with --temperature: from the fewest of these that have this share of their probability")
+    p.add_argument("--min-p", type=float, default=0.0, help="with --temperature: from those of these at least so likely beside the likeliest")
+    p.add_argument("--adapter", default=None, metavar="DIR", help="low-rank adapter folder: adapter_config.json + adapter_model.safetensors")
     p.add_argument("--sample-seed", type=int, default=0)
     p.add_argument("--ignore-eos", action="store_true")
     p.add_argument("--random-weights", action="store_true", help="draw weights from --seed instead of reading them")
@@ -52,6 +56,7 @@ def main(argv=None) -> int:
     import torch
     from .config.engine_config import EngineConfig, ModelConfig, SchedulerConfig
     from .sampling.sampler import SamplingParams
+    from .weights.adapters import read_adapter_config
     from .weights.four_bit import four_bit_share
 
     raw = None
@@ -75,12 +80,16 @@ def main(argv=None) -> int:
                       kv_cache_budget_gb=args.kv_budget_gb, max_seq_len=args.max_seq_len,
                       use_cuda_graph=not args.no_cuda_graph, seed=args.sample_seed,
                       scheduler=SchedulerConfig(args.max_batch_tokens, args.max_num_seqs, args.prefill_chunk),
-                      weight_format=args.weight_format, act_bits=args.act_bits)
+                      weight_format=args.weight_format, act_bits=args.act_bits, max_adapters=int(args.adapter is not None),
+                      max_adapter_rank=read_adapter_config(args.adapter)[0] if args.adapter else 16)
     t0 = time.perf_counter()
     if raw is not None:
         eng = Engine(None, ec, dtype=args.dtype, config=raw, random_seed=args.seed)
     else:
         eng = Engine(ModelConfig(args.model, args.name, args.dtype), ec)
+    adapter = None if args.adapter is None else "adapter"
+    if adapter:
+        eng.load_adapter(adapter, args.adapter)
     t_load = time.perf_counter() - t0
     vocab = eng.model.spec.vocab_size
 
@@ -104,13 +113,13 @@ def main(argv=None) -> int:
     print(f"\nPrompt: {len(prompts)} x {len(prompts[0])} tokens; weights {eng.pool.total_gb:.2f} GB{four} loaded in {t_load:.1f}s")
 
     sp = SamplingParams(max_new_tokens=args.max_tokens, temperature=args.temperature, seed=args.sample_seed,
-                        ignore_eos=args.ignore_eos)
+                        ignore_eos=args.ignore_eos, top_k=args.top_k, top_p=args.top_p, min_p=args.min_p)
     print("Warming up...")
-    eng.generate(prompts[:1], SamplingParams(max_new_tokens=min(5, args.max_tokens), ignore_eos=True))
+    eng.generate(prompts[:1], SamplingParams(max_new_tokens=min(5, args.max_tokens), ignore_eos=True), adapter)
     print("Generating...\n")
     torch.cuda.synchronize()
     t_start = time.perf_counter()
-    results = eng.generate(prompts, sp)
+    results = eng.generate(prompts, sp, adapter)
     torch.cuda.synchronize()
     t_total = time.perf_counter() - t_start
 

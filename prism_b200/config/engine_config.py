@@ -51,7 +51,11 @@ class EngineConfig:
                                         # model is loaded as its file has it (both have room on the device for a moment)
     act_bits: int = 16                  # with it: products take activations as they are (16) or brought to 4 bits too;
                                         # layers of experts take them as they are in any case
+    max_adapters: int = 0               # low-rank adapters that may be loaded at once (``Engine.load_adapter``); their room is taken at the start
+    max_adapter_rank: int = 16          # the largest rank among them
 
     def __post_init__(self):
+        from ..weights.adapters import check_adapter_room
+        check_adapter_room(self.max_adapters, self.max_adapter_rank)
         from ..weights.four_bit import check_weight_format
         check_weight_format(self.weight_format, self.act_bits)

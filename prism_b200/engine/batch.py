@@ -9,9 +9,10 @@ cache, described by int32 arrays that are packed on the host in pinned memory
 and reach the device in one copy:
 
     token_ids[T] positions[T] tok_seg[T] seg_start[S+1] cached_len[S]
-    q_len[S] state_slots[S] logit_rows[R] block_tables[G][S, W]
+    q_len[S] state_slots[S] logit_rows[R] adapter_ids[T] block_tables[G][S, W]
     decode_items[G][n_g, 4] decode_starts[G][S]
 
+``adapter_ids`` (only where the step has adapters): the low-rank adapter of each token's request, -1 for none.
 ``decode_items[g]`` is the decode attention kernel's work in paged cache group g
 for the single-token segments at the head of the batch: one item
 ``{token, split | used << 16, position, segment}`` per CTA and kv head, as many
@@ -33,10 +34,11 @@ import torch
 @dataclass
 class Segment:
     """A request's next tokens in this step.  ``want``: places among these
-    tokens whose logits are wanted."""
+    tokens whose logits are wanted.  ``adapter``: the number of its low-rank adapter (-1: none)."""
     req_id: object
     tokens: Sequence[int]
     want: Sequence[int] = ()
+    adapter: int = -1
 
 
 @dataclass
@@ -48,13 +50,14 @@ class BatchLayout:
     W: int
     paged_groups: List[int]
     decode_items: Optional[Dict[int, int]] = None       # group -> items in the descriptor
+    adapters: bool = False                              # whether it has adapter_ids
 
     def __post_init__(self):
         o = 0
         self.off = {}
         for name, n in (("token_ids", self.T), ("positions", self.T), ("tok_seg", self.T),
                         ("seg_start", self.S + 1), ("cached_len", self.S), ("q_len", self.S),
-                        ("state_slots", self.S), ("logit_rows", self.R)):
+                        ("state_slots", self.S), ("logit_rows", self.R)) + ((("adapter_ids", self.T),) if self.adapters else ()):
             self.off[name] = (o, n)
             o += (n + 3) // 4 * 4               # keep every array 16-byte aligned
         for g in self.paged_groups:
@@ -90,6 +93,7 @@ class StepContext:
         self.token_ids, self.positions, self.tok_seg = v("token_ids"), v("positions"), v("tok_seg")
         self.seg_start, self.cached_len, self.q_len = v("seg_start"), v("cached_len"), v("q_len")
         self.state_slots, self.logit_rows = v("state_slots"), v("logit_rows")
+        self.adapter_ids = v("adapter_ids") if layout.adapters else None
         self.block_tables = {g: v(f"bt{g}").view(layout.S, layout.W) for g in layout.paged_groups}
         # group -> (items [n, 4], starts [S], most items of a token (1: no merge kernel), tokens the items are for);
         # the runner sets the last two
@@ -102,7 +106,7 @@ class StepContext:
 
 def pack_batch(layout: BatchLayout, token_ids, positions, tok_seg, seg_start, cached_len, q_len,
                slots, logit_rows, block_rows: Dict[int, List[List[int]]], pad_page: Dict[int, int],
-               decode_work: Optional[Dict[int, tuple]] = None):
+               decode_work: Optional[Dict[int, tuple]] = None, adapter_ids=()):
     """Fill a pinned int32 tensor with the descriptor.  ``block_rows[g][s]`` is
     request s's logical-page -> physical-page list in group g; entries beyond
     it (and pages already given back) read ``pad_page[g]``, the scratch page.
@@ -113,7 +117,7 @@ def pack_batch(layout: BatchLayout, token_ids, positions, tok_seg, seg_start, ca
     a[:] = 0
     for name, vals in (("token_ids", token_ids), ("positions", positions), ("tok_seg", tok_seg),
                        ("seg_start", seg_start), ("cached_len", cached_len), ("q_len", q_len),
-                       ("state_slots", slots), ("logit_rows", logit_rows)):
+                       ("state_slots", slots), ("logit_rows", logit_rows)) + ((("adapter_ids", adapter_ids),) if layout.adapters else ()):
         o, n = layout.off[name]
         if n:
             a[o:o + n] = np.asarray(vals, dtype=np.int32)

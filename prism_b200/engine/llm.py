@@ -20,6 +20,7 @@ from ..config.engine_config import EngineConfig, ModelConfig
 from ..cache.manager import pool_sizes
 from ..model_registry import build_model
 from ..sampling.sampler import Sampler, SamplingParams
+from ..weights.adapters import AdapterSet
 from ..weights.four_bit import check_weight_format, to_four_bits, written_out_bytes
 from ..weights.loader import load_model_folder
 from ..weights.random_init import random_pool
@@ -61,12 +62,14 @@ class Engine:
         if ec.weight_format is not None:
             self.pool = to_four_bits(self.model, self.pool, self.device, self.dtype, ec.act_bits)
             torch.cuda.empty_cache()             # the matrices as they were: free memory, not torch's, when the cache is sized
+        # room for adapters is taken before the cache is sized
+        self.adapters = AdapterSet(self.model, ec.max_adapters, ec.max_adapter_rank, self.device, self.dtype) if ec.max_adapters else None
         spec = self.model.spec
         max_seq_len = min(ec.max_seq_len or spec.max_positions, spec.max_positions)
         num_pages = self._pages_per_group(ec, max_seq_len)
         self.runner = ModelRunner(self.model, self.device, self.dtype, ec.kv_page_size, num_pages,
                                   ec.scheduler.max_num_seqs, max_seq_len, ec.use_cuda_graph,
-                                  ec.graph_batch_sizes)
+                                  ec.graph_batch_sizes, adapters=self.adapters)
         self.sampler = Sampler(self.device)
         self.scheduler = Scheduler(self.runner, self.sampler, ec.scheduler, spec.eos_token_id, ec.seed)
 
@@ -84,16 +87,47 @@ class Engine:
 
     # ---- generation ---------------------------------------------------------------
     def generate(self, prompts: Sequence[Sequence[int]],
-                 sampling: Union[SamplingParams, Sequence[SamplingParams], None] = None) -> List[GenerationResult]:
+                 sampling: Union[SamplingParams, Sequence[SamplingParams], None] = None,
+                 adapters: Union[str, Sequence[Optional[str]], None] = None) -> List[GenerationResult]:
         """Generate for every prompt (lists of token ids); requests are batched
-        continuously.  Returns results in the order of the prompts."""
+        continuously, whatever adapters they use.  Returns results in the order of the prompts.  ``adapters``: the name of a loaded
+        adapter for all prompts, or one (or None) for each."""
         if sampling is None or isinstance(sampling, SamplingParams):
             sampling = [sampling or SamplingParams()] * len(prompts)
-        reqs = [self.scheduler.add_request(p, s) for p, s in zip(prompts, sampling)]
+        if adapters is None or isinstance(adapters, str):
+            adapters = [adapters] * len(prompts)
+        if len(adapters) != len(prompts):
+            raise ValueError(f"{len(adapters)} adapters for {len(prompts)} prompts")
+        numbers = [self._adapter_number(name) for name in adapters]
+        reqs = [self.scheduler.add_request(p, s, a) for p, s, a in zip(prompts, sampling, numbers)]
         self.scheduler.run_to_completion()
         self.runner.check_errors()
-        return [GenerationResult(r.generated_tokens, r.finish_reason, r.ttft, r.tbt, r.num_preemptions, r.error)
+        return [GenerationResult(r.generated_tokens, r.finish_reason, r.ttft, r.tbt, r.num_preemptions, r.error,
+                                 r.logprobs if r.params.logprobs else None)
                 for r in reqs]
+
+    # ---- adapters -----------------------------------------------------------------
+    def _adapter_number(self, name: Optional[str]) -> int:
+        if name is None:
+            return -1
+        if self.adapters is None:
+            raise ValueError(f"adapter {name!r}: this engine has no room for adapters (EngineConfig.max_adapters)")
+        return self.adapters.number(name)
+
+    def load_adapter(self, name: str, folder: str) -> None:
+        """Load the low-rank adapter in ``folder`` (``weights.adapters.read_adapter_folder``) under ``name``; requests use it from then on by that
+        name.  A name that is taken is refused, and so is one adapter more than ``EngineConfig.max_adapters``."""
+        if self.adapters is None:
+            raise ValueError(f"adapter {name!r}: this engine has no room for adapters (EngineConfig.max_adapters)")
+        self.adapters.load(name, folder)
+
+    def unload_adapter(self, name: str) -> None:
+        """Forget an adapter and give its place to the next one.  Refused while a request that uses it is waiting or running."""
+        number = self._adapter_number(name)
+        if number >= 0 and any(r.adapter == number for r in list(self.scheduler.waiting) + list(self.scheduler.running)):
+            raise ValueError(f"adapter {name!r} is in use")
+        if self.adapters is not None:
+            self.adapters.remove(name)
 
     def warmup(self, batch_sizes: Optional[Sequence[int]] = None) -> None:
         """Capture the decode graphs before the first request (engine/executor.py:312-318 does it for a list of

@@ -33,6 +33,8 @@ class Request:
     arrival_time: float = 0.0
     first_token_time: float = 0.0
     done_time: float = 0.0
+    adapter: int = -1                     # number of its low-rank adapter, -1: none
+    logprobs: List[float] = field(default_factory=list)      # of the generated tokens, where its params ask for them
 
     @property
     def tokens(self) -> List[int]:
@@ -73,3 +75,4 @@ class GenerationResult:
     tbt: float
     num_preemptions: int = 0
     error: Optional[str] = None
+    logprobs: Optional[List[float]] = None       # with SamplingParams.logprobs: one a token

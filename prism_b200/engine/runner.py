@@ -43,8 +43,8 @@ def cache_groups(model: DecoderModel):
 class ModelRunner:
     def __init__(self, model: DecoderModel, device, dtype: torch.dtype, page_size: int, num_pages,
                  max_seqs: int, max_seq_len: Optional[int] = None, use_cuda_graph: bool = False,
-                 graph_batch_sizes: Sequence[int] = (1, 2, 4, 8, 16, 32, 64)):
-        """``num_pages``: the pool size of every paged cache group, or one size per group (in the order
+                 graph_batch_sizes: Sequence[int] = (1, 2, 4, 8, 16, 32, 64), adapters=None):
+        """``adapters``: the model's ``weights.adapters.AdapterSet``, if it has one.  ``num_pages``: the pool size of every paged cache group, or one size per group (in the order
         of ``cache_groups(model)``; entries of groups that are not paged are ignored): a group whose
         layers see a window of keys needs far fewer pages than one that keeps them all."""
         if not torch.cuda.is_available():
@@ -72,7 +72,8 @@ class ModelRunner:
         self.graph_batch_sizes = sorted(set(int(b) for b in graph_batch_sizes if b <= max_seqs)) or [1]
         from .. import ops
         self._sms = ops.num_sms(self.device)
-        self._graphs: Dict[tuple, dict] = {}     # (bucket, decode attention places, merge kernels) -> captured step
+        self._graphs: Dict[tuple, dict] = {}     # (bucket, decode attention places, merge kernels, adapters) -> captured step
+        self.adapters = adapters
         self._work_memo: Dict[int, dict] = {}    # per cache group: the last step's decode work items
         self.graph_kernel_launches = 0       # kernels of this library replayed inside graphs
         self.last_h2d_bytes = 0              # bytes of the last step's batch descriptor (host to device)
@@ -109,13 +110,17 @@ class ModelRunner:
                 raise ValueError(f"request {s.req_id!r}: a segment needs at least one token")
         if len({s.req_id for s in segments}) != len(segments):
             raise ValueError("a request may appear once per step")
+        adapted = any(s.adapter >= 0 for s in segments)
+        most = 0 if self.adapters is None else self.adapters.count
+        if adapted and not all(s.adapter < most for s in segments):
+            raise ValueError(f"a segment names an adapter beyond the {most} there are")
         if not self.can_run(segments):
             raise OutOfPages("Out of KV cache pages for this step")
         for s in segments:
             self.cache.append(s.req_id, len(s.tokens))
         self.storage.clear_slots(self.cache.drain_fresh_slots())
 
-        tok, pos, seg_of, seg_start, cached, qlen, slots, rows = [], [], [], [0], [], [], [], []
+        tok, pos, seg_of, seg_start, cached, qlen, slots, rows, ids = [], [], [], [0], [], [], [], [], []
         for i, s in enumerate(segments):
             c = self.cache.length(s.req_id)
             n = len(s.tokens)
@@ -130,19 +135,20 @@ class ModelRunner:
             cached.append(c)
             qlen.append(n)
             slots.append(self.cache.slot(s.req_id))
+            ids.extend([s.adapter] * n)
         block_rows = {g: [self.cache.block_table_row(s.req_id, g) for s in segments] for g in self.paged_groups}
         max_q, max_kv = max(qlen), max(c + n for c, n in zip(cached, qlen))
         host_meta = dict(seg_start=seg_start, cached_len=cached, q_len=qlen, slots=slots, tok_seg=seg_of)
 
         S = len(segments)
         if self.use_cuda_graph and max_q == 1 and S <= self.graph_batch_sizes[-1]:
-            logits = self._step_graph(tok, pos, cached, slots, rows, block_rows, token_source)
+            logits = self._step_graph(tok, pos, cached, slots, rows, block_rows, token_source, ids if adapted else None)
         else:
             work = self._decode_work(cached, qlen)
             layout = BatchLayout(len(tok), S, len(rows), self.cache.table_width, self.paged_groups,
-                                 {g: len(w[0]) for g, w in work.items()})
+                                 {g: len(w[0]) for g, w in work.items()}, adapted)
             host = pack_batch(layout, tok, pos, seg_of, seg_start, cached, qlen, slots, rows,
-                              block_rows, self.pad_page, work)
+                              block_rows, self.pad_page, work, ids)
             dev = host.to(self.device, non_blocking=True)
             self.last_h2d_bytes = host.numel() * 4
             if token_source is not None:
@@ -153,10 +159,16 @@ class ModelRunner:
             for g, w in work.items():                  # the host knows whether any request has more than one item
                 ctx.decode_work[g] = ctx.decode_work[g][:2] + (w[2], len(w[1]))
             views = self.storage.views(ctx.block_tables, ctx.state_slots, slots)
-            logits = self.model.forward(ctx, views)
+            logits = self._forward(ctx, views, next((i for i, n in enumerate(qlen) if n != 1), S))
         for s in segments:
             self.cache.commit(s.req_id, len(s.tokens))
         return logits
+
+    def _forward(self, ctx, views, singles: int):
+        """The model's step; ``singles``: the tokens from the first on that are each a request of its own."""
+        if self.adapters is not None:
+            self.adapters.step.ids, self.adapters.step.singles = ctx.adapter_ids, singles
+        return self.model.forward(ctx, views)
 
     def _decode_work(self, cached, qlen, n_real: Optional[int] = None) -> Dict[int, tuple]:
         """The decode attention kernel's work items for the single-token segments at the head of the batch, per
@@ -193,17 +205,18 @@ class ModelRunner:
             out.append(-(-max(1, items[g]) // wave) * wave)
         return tuple(out)
 
-    def _capture(self, B: int, places: tuple, merge: bool) -> dict:
+    def _capture(self, B: int, places: tuple, merge: bool, adapted: bool = False) -> dict:
         """Capture the decode step for a bucket of B one-token segments: static
         descriptor buffer, every row's logits computed.  ``places``: the decode attention
         kernel's places for work items in each paged group (``_graph_places``); ``merge``: whether
-        a request may have more than one item (else the graph has no merge kernels)."""
-        layout = BatchLayout(B, B, B, self.cache.table_width, self.paged_groups, dict(zip(self.paged_groups, places)))
+        a request may have more than one item (else the graph has no merge kernels); ``adapted``: whether it may have an
+        adapter (else the graph has none of their kernels)."""
+        layout = BatchLayout(B, B, B, self.cache.table_width, self.paged_groups, dict(zip(self.paged_groups, places)), adapted)
         dev = torch.zeros(layout.total, dtype=torch.int32, device=self.device)
         pad_rows = {g: [[] for _ in range(B)] for g in self.paged_groups}
         host = pack_batch(layout, [0] * B, [0] * B, list(range(B)), list(range(B + 1)), [0] * B, [1] * B,
                           [self.cache.max_seqs] * B, list(range(B)), pad_rows, self.pad_page,
-                          self._decode_work([0] * B, [1] * B))
+                          self._decode_work([0] * B, [1] * B), [-1] * B)
         dev.copy_(host)
         def fresh_ctx():
             # every run gets its own context: values parts keep for the length of a step (the
@@ -217,7 +230,7 @@ class ModelRunner:
         stream.wait_stream(torch.cuda.current_stream(self.device))
         with torch.cuda.stream(stream):
             for _ in range(2):                       # warm-up: lazy library set-up happens outside capture
-                self.model.forward(*fresh_ctx())
+                self._forward(*fresh_ctx(), B)
         torch.cuda.current_stream(self.device).wait_stream(stream)
         torch.cuda.synchronize(self.device)
         graph = torch.cuda.CUDAGraph()
@@ -225,15 +238,15 @@ class ModelRunner:
         before = ops.launch_count
         ctx, views = fresh_ctx()
         with torch.cuda.graph(graph, stream=stream):
-            out = self.model.forward(ctx, views)
+            out = self._forward(ctx, views, B)
         torch.cuda.synchronize(self.device)
         return dict(graph=graph, layout=layout, dev=dev, out=out, launches=ops.launch_count - before)
 
-    def _step_graph(self, tok, pos, cached, slots, rows, block_rows, token_source=None):
+    def _step_graph(self, tok, pos, cached, slots, rows, block_rows, token_source=None, ids=None):
         S = len(tok)
         B = self._bucket(S)
         work = self._decode_work(cached + [0] * (B - S), [1] * B, S)    # padded rows: one item each, at position 0
-        key = (B, self._graph_places({g: len(w[0]) for g, w in work.items()}), any(w[2] > 1 for w in work.values()))
+        key = (B, self._graph_places({g: len(w[0]) for g, w in work.items()}), any(w[2] > 1 for w in work.values()), ids is not None)
         g = self._graphs.get(key)
         if g is None:
             g = self._graphs[key] = self._capture(*key)
@@ -242,7 +255,7 @@ class ModelRunner:
         br = {k: v + [[] for _ in range(pad)] for k, v in block_rows.items()}
         host = pack_batch(g["layout"], tok + [0] * pad, pos + [0] * pad, list(range(B)), list(range(B + 1)),
                           cached + [0] * pad, [1] * B, slots + [scratch_slot] * pad, list(range(B)),
-                          br, self.pad_page, work)
+                          br, self.pad_page, work, (ids or []) + [-1] * pad)
         g["dev"].copy_(host, non_blocking=True)
         self.last_h2d_bytes = host.numel() * 4
         if token_source is not None:
@@ -267,9 +280,10 @@ class ModelRunner:
                 work = self._decode_work([0] * b, [1] * b)
                 places = self._graph_places({g: len(w[0]) for g, w in work.items()})
                 for merge in ((True, False) if work else (False,)):
-                    key = (b, places, merge)
-                    if key not in self._graphs:
-                        self._graphs[key] = self._capture(*key)
+                    for adapted in ((False, True) if self.adapters is not None else (False,)):
+                        key = (b, places, merge, adapted)
+                        if key not in self._graphs:
+                            self._graphs[key] = self._capture(*key)
 
     def invalidate_graphs(self) -> None:
         self._graphs.clear()

@@ -83,7 +83,7 @@ class Scheduler:
         self._next_id = 0
 
     # ---- submission ---------------------------------------------------------------
-    def add_request(self, prompt_tokens, params: Optional[SamplingParams] = None) -> Request:
+    def add_request(self, prompt_tokens, params: Optional[SamplingParams] = None, adapter: int = -1) -> Request:
         params = params or SamplingParams()
         prompt = [int(t) for t in prompt_tokens]
         if not prompt:
@@ -98,7 +98,7 @@ class Scheduler:
         for g in self.cache.groups:
             if g.kind == "paged" and g.need.window is None and pages > self.cache.allocators[g.index].num_pages:
                 raise ValueError(f"request needs {pages} pages, the pool has {self.cache.allocators[g.index].num_pages}")
-        req = Request(self._next_id, prompt, params, arrival_time=time.time())
+        req = Request(self._next_id, prompt, params, arrival_time=time.time(), adapter=adapter)
         self._next_id += 1
         self.waiting.append(req)
         return req
@@ -210,7 +210,7 @@ class Scheduler:
         for req, n in batch:
             toks = req.next_tokens(n)
             last = req.num_computed + n == len(req.prompt_tokens) + len(req.generated_tokens)
-            segs.append(Segment(req.id, toks, [n - 1] if last else []))
+            segs.append(Segment(req.id, toks, [n - 1] if last else [], req.adapter))
             if last:
                 sampled.append(req)
             if n == 1 and req.num_computed >= len(req.prompt_tokens):
@@ -226,7 +226,12 @@ class Scheduler:
             temps = [r.params.temperature for r in sampled]
             us = [uniform(r.params.seed if r.params.seed is not None else self.seed, r.id,
                           len(r.generated_tokens)) for r in sampled]
-            tokens = self.sampler.sample(logits, temps, us)
+            if any(r.params.by_filters for r in sampled):
+                h = self.sampler.sample_async(logits, temps, us, [r.params for r in sampled])
+                tokens = self.sampler.read(h)
+                self._keep_logprobs(sampled, h)
+            else:
+                tokens = self.sampler.sample(logits, temps, us)
             now = time.time()
             for req, tok in zip(sampled, tokens):
                 req.generated_tokens.append(int(tok))
@@ -237,6 +242,12 @@ class Scheduler:
                 out.append((req, int(tok)))
                 self._maybe_finish(req, int(tok), now)
         return out
+
+    def _keep_logprobs(self, reqs, handle) -> None:
+        """Of the rows of a read handle, for the requests that ask for them and still run."""
+        for i, req in enumerate(reqs):
+            if req.params.logprobs and req.state != RequestState.FINISHED:
+                req.logprobs.append(float(handle.host_logprobs[i]))
 
     def _ends(self, req: Request, tok: int) -> bool:
         """Whether ``tok`` is an end-of-sequence token for this request."""
@@ -279,6 +290,7 @@ class Scheduler:
         reqs = list(self.running)
         seed_of = [r.params.seed if r.params.seed is not None else self.seed for r in reqs]
         temps = [r.params.temperature for r in reqs]
+        filters = ([r.params for r in reqs],) if any(r.params.by_filters for r in reqs) else ()
         n_launched = [len(r.generated_tokens) for r in reqs]       # tokens sampled or in flight, per request
         inflight = []                                                  # sample handles, oldest first
         source = None
@@ -292,10 +304,10 @@ class Scheduler:
                         [Segment(r.id, [0], [0]) for r in reqs]):
                     stop = True
             if not stop:
-                segs = [Segment(r.id, [r.generated_tokens[-1] if source is None else 0], [0]) for r in reqs]
+                segs = [Segment(r.id, [r.generated_tokens[-1] if source is None else 0], [0], r.adapter) for r in reqs]
                 logits = self.runner.step(segs, token_source=source)
                 us = [uniform(sd, r.id, n) for sd, r, n in zip(seed_of, reqs, n_launched)]
-                h = self.sampler.sample_async(logits, temps, us)
+                h = self.sampler.sample_async(logits, temps, us, *filters)
                 source = h.device_tokens
                 inflight.append(h)
                 for i in range(len(reqs)):
@@ -306,7 +318,10 @@ class Scheduler:
                 return False
             if len(inflight) < 2 and not stop:
                 continue                                               # keep one step ahead
-            tokens = self.sampler.read(inflight.pop(0))
+            h = inflight.pop(0)
+            tokens = self.sampler.read(h)
+            if filters:
+                self._keep_logprobs(reqs, h)
             now = time.time()
             for req, tok in zip(reqs, tokens):
                 if req.state == RequestState.FINISHED:

@@ -457,7 +457,13 @@ def linear_delta(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] 
     """A projection whose result will be added to the residual stream by the
     next norm: like ``linear``, but it may return a float32 stack ``[k, M, N]``
     of partial sums over K, which the fused add + norm kernel adds up.  ``f32``: the
-    result is float32 in any case (never rounded to 16 bits before the residual sum)."""
+    result is float32 in any case (never rounded to 16 bits before the residual sum).
+    Adapters' part joins the (first partial) sum in float32."""
+    w = in_use(w)
+    if type(w) is Adapted:
+        out = linear_delta(x, w.base, bias, True)
+        w.add_to(x, out[0] if out.dim() == 3 else out)
+        return out
     if tc_gemm_ok(x, w):
         N, K = w.shape
         ks = tc_ksplit(N, K, M=x.shape[0])
@@ -475,7 +481,11 @@ def linear(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = None
     (a tensor the model file stores in 32-bit), go through the true-float32
     kernel; bf16 x bf16 goes to the library matrix product (cuBLAS through
     torch), as in andre-fu/prism (executor.py:109).  ``w`` may be an
-    ``Mxfp4``: bf16 activations by ``mxfp4_linear``, with its ``act_bits``."""
+    ``Mxfp4``: bf16 activations by ``mxfp4_linear``, with its ``act_bits``; or an
+    ``Adapted``: the shared product in the result's dtype, then the adapters' part added to it."""
+    w = in_use(w)
+    if type(w) is Adapted:
+        return w.add_to(x, linear(x, w.base, bias, out, out_dtype))
     if isinstance(w, Mxfp4):
         want = out_dtype or (out.dtype if out is not None else x.dtype)
         if out is None or out.dtype == want:
@@ -627,6 +637,9 @@ def qkv_rotate_store(ctx, x: torch.Tensor, qkv_w: torch.Tensor, qkv_b: Optional[
     T = x.shape[0]
     qs, kvs = nh * hd, nkv * hd
     table = None
+    qkv_w = in_use(qkv_w)
+    adapted = qkv_w if type(qkv_w) is Adapted else None
+    qkv_w = qkv_w if adapted is None else adapted.base
     if rot is not None and rot.rotary_dim:
         key = ("rotary_table", rot.inv_freq.data_ptr())          # one table per step for all layers
         table = ctx.scratch.get(key)
@@ -640,6 +653,8 @@ def qkv_rotate_store(ctx, x: torch.Tensor, qkv_w: torch.Tensor, qkv_b: Optional[
         if ks > 1:
             parts = ctx.alloc((ks, T, qs + 2 * kvs), torch.float32)
             gemm_tc(x, qkv_w, None, parts, EPI_PARTIAL, ksplit=ks)
+            if adapted is not None:
+                adapted.add_to(x, parts[0])
             q = ctx.alloc((T, nh, hd), x.dtype)
             rope_kv_write_partial(parts, qkv_b, q, ctx.positions, ctx.tok_seg, table, rot.rotary_dim, kc, vc,
                                   cache.block_table, cache.num_pages, ctx.max_positions, nkv, ctx.err)
@@ -649,6 +664,8 @@ def qkv_rotate_store(ctx, x: torch.Tensor, qkv_w: torch.Tensor, qkv_b: Optional[
         qkv = torch.nn.functional.linear(x, qkv_w, b)
     else:
         qkv = linear(x, qkv_w, qkv_b)
+    if adapted is not None:
+        adapted.add_to(x, qkv)
     q = qkv[:, :qs].view(T, nh, hd)
     k = qkv[:, qs:qs + kvs].view(T, nkv, hd)
     v = qkv[:, qs + kvs:].view(T, nkv, hd)
@@ -1269,6 +1286,7 @@ def qkv_attention(ctx, x: torch.Tensor, qkv_w: torch.Tensor, qkv_b: Optional[tor
     ``qkv_rotate_store`` followed by ``attention``; with ``QKV_IN_ATTENTION`` a pure decode step of a few
     tokens runs as two kernels (K-split projection, attention that finishes the projection)."""
     T = x.shape[0]
+    qkv_w = in_use(qkv_w)
     if (QKV_IN_ATTENTION and QKV_PARTIAL and ctx.decode_only and cache.write and rot is not None
             and rot.rotary_dim == hd and x.dtype == torch.bfloat16 and cache.k.dtype == torch.bfloat16
             and not FORCE_GENERIC_ATTENTION and tc_gemm_ok(x, qkv_w)
@@ -1294,6 +1312,7 @@ def qkv_attention(ctx, x: torch.Tensor, qkv_w: torch.Tensor, qkv_b: Optional[tor
 def feed_forward_swiglu(ctx, x: torch.Tensor, gate_up_w: torch.Tensor, down_w: torch.Tensor):
     """``down(silu(gate(x)) * up(x))`` with the fused gate/up weight."""
     M, I = x.shape[0], gate_up_w.shape[0] // 2
+    gate_up_w = in_use(gate_up_w)
     if tc_gemm_ok(x, gate_up_w, TC_GEMM_MAX_M_SWIGLU):
         act = ctx.alloc((M, I), x.dtype)
         gemm_tc(x, gate_up_w, None, act, EPI_SWIGLU, ksplit=tc_ksplit_paired(I, x.shape[1], M=M))    # the SwiGLU in its epilogue
@@ -1542,6 +1561,7 @@ def glu_hidden(ctx, x: torch.Tensor, gate_up_w: torch.Tensor, kind: str, limit: 
     """The hidden layer of a gated feed-forward (``glu`` of the product with the fused gate/up weight); for a few tokens
     the gated activation is the product's epilogue.  ``bias``: on the product's rows (gate, then up)."""
     act = ctx.alloc((x.shape[0], gate_up_w.shape[0] // 2), x.dtype)
+    gate_up_w = in_use(gate_up_w)
     if tc_gemm_ok(x, gate_up_w, TC_GEMM_MAX_M_SWIGLU):
         gemm_tc(x, gate_up_w, bias, act, {"silu": EPI_SWIGLU, "gelu_tanh": EPI_GEGLU, "clamped": EPI_CLAMPED}[kind],
                 ksplit=tc_ksplit_paired(act.shape[1], x.shape[1], M=x.shape[0]), limit=limit)
@@ -2545,4 +2565,4 @@ def moe_feed_forward(ctx, x: torch.Tensor, logits: torch.Tensor, gate_up_w: torc
 
 from . import mxfp4      # noqa: E402
 from .mxfp4 import Mxfp4, mxfp4_linear, mxfp4_moe, mxfp4_quantize      # noqa: E402,F401
-from .low_rank import LowRank, low_rank      # noqa: E402,F401
+from .low_rank import Adapted, AdapterStep, LowRank, in_use, low_rank, low_rank_limits      # noqa: E402,F401

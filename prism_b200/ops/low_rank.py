@@ -21,6 +21,11 @@ MOST_RANK, MOST_SLICES = 128, 8      # csrc/low_rank.cu
 RANK_UNIT, WIDTH_UNIT = 16, 8        # an adapter's rank in memory, and its A's rows, are whole numbers of these
 
 
+def low_rank_limits():
+    """``(largest rank, most slices)`` of a stack of adapters."""
+    return MOST_RANK, MOST_SLICES
+
+
 def _up(n: int, unit: int) -> int:
     return -(-n // unit) * unit
 
@@ -84,6 +89,47 @@ class LowRank:
                 rank, at = ab[0].shape[0], self._first[g]
                 self.a[index, g, :rank, :self.k].copy_(ab[0])
                 self.b[index, at:at + self.rows[g], :rank].copy_(ab[1])
+
+
+class AdapterStep:
+    """What the adapters of a model are told of a step before it runs: ``ids``, each token's adapter (int32 on the device), or None where no
+    token has one; and ``low_rank``'s ``singles``."""
+
+    __slots__ = ("ids", "singles")
+
+    def __init__(self):
+        self.ids, self.singles = None, 0
+
+
+class Adapted:
+    """A projection's matrix ``base`` (or an ``Mxfp4``) with its adapters: ``linear`` and what is built on it take it in the matrix's place.  In a
+    step without adapters the matrix alone is used, by whichever kernel it would be used by; else the shared product runs as it does for a
+    matrix by itself and the adapters' part is added to its result."""
+
+    __slots__ = ("base", "low", "step")
+    dtype = "adapted"                        # no kernel's: products that look for a dtype leave it to ``linear``
+
+    def __init__(self, base, low: LowRank, step: AdapterStep):
+        if tuple(base.shape) != (low.n, low.k):
+            raise ops.KernelError(f"adapters for a matrix [{low.n}, {low.k}] beside one {tuple(base.shape)}")
+        self.base, self.low, self.step = base, low, step
+
+    @property
+    def shape(self):
+        return self.base.shape
+
+    def dim(self) -> int:
+        return 2
+
+    def add_to(self, x: torch.Tensor, result: torch.Tensor) -> torch.Tensor:
+        """The step's adapters' part, added to the shared product's result in place."""
+        x = x if x.dtype is self.low.a.dtype else x.to(self.low.a.dtype)
+        return low_rank(x, self.low, self.step.ids, result, result, self.step.singles)
+
+
+def in_use(w):
+    """``w`` itself, or the matrix alone of an ``Adapted`` whose adapters the step does not use."""
+    return w.base if type(w) is Adapted and w.step.ids is None else w
 
 
 SINGLES = 64                 # without a word from the caller, so many tokens are taken one by one

@@ -68,7 +68,7 @@ class GQAAttention(Mixer):
     for each distance below ``B / 2``, the rest shared in steps that grow like a logarithm up to D.  ``names``: the tensors' names in the model file (keys
     q, k, v, o, q_b, k_b, v_b, o_b, sink, q_norm, k_norm, g)."""
 
-    four_bit = ("qkv_w", "o_w")
+    four_bit = adaptable = ("qkv_w", "o_w")
     NAMES = dict(q="q_proj.weight", k="k_proj.weight", v="v_proj.weight", o="o_proj.weight",
                  q_b="q_proj.bias", k_b="k_proj.bias", v_b="v_proj.bias", o_b="o_proj.bias", sink="sinks",
                  q_norm="q_norm.weight", k_norm="k_norm.weight", g="g_proj.weight", rel="rel")

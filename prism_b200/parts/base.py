@@ -189,6 +189,7 @@ class Part:
     category = ""
     prefix = ""
     four_bit: Tuple[str, ...] = ()       # own parameters that may be kept in 4 bits (``ops.Mxfp4``)
+    adaptable: Tuple[str, ...] = ()      # own parameters that may have low-rank adapters beside them (``ops.Adapted``)
 
     @property
     def children(self) -> Dict[str, "Part"]:

@@ -18,7 +18,7 @@ class SwiGLU(FeedForward):
     through, ``silu`` or ``gelu_tanh``; or ``clamped``, the form with both projections limited by ``limit``
     (``ops.glu``).  ``biases``: the names of the gate's, the up and the down projection's biases, or None."""
 
-    four_bit = ("gate_up_w", "down_w")
+    four_bit = adaptable = ("gate_up_w", "down_w")
 
     def __init__(self, hidden_size: int, intermediate_size: int,
                  names=("gate_proj.weight", "up_proj.weight", "down_proj.weight"), activation: str = "silu",
@@ -59,7 +59,7 @@ class ActMLP(FeedForward):
     """``down(act(up(x)))`` without gate.  ``activation``: one of ``ops.ACTIVATIONS`` (``relu2``: the square of
     relu; ``gelu_tanh``; ``silu``; ``relu``).  ``names``: the up and down tensors' names in the model file."""
 
-    four_bit = ("up_w", "down_w")
+    four_bit = adaptable = ("up_w", "down_w")
 
     def __init__(self, hidden_size: int, intermediate_size: int, activation: str = "relu2",
                  names=("up_proj.weight", "down_proj.weight")):
