@@ -5,18 +5,21 @@
 // neighbouring result columns.  a [L, G, r, Kp]: r rows of a slice's A, zeros beyond K; b [L, N, r]: the rows of all slices' B.  r is a
 // multiple of 16, Kp of 8 (rows start on 16 bytes), zeros beyond an adapter's own rank.  Sums in float32, one rounding where a result is stored.
 //
-// Here: a few tokens at a time on CUDA cores - decoding requests, each with an adapter of its own, where every byte of A and B is used once and
-// the kernel is bound by reading them, and 32-bit floats.  low_rank_tile.cu has the portions of prompts.
+// Here, on CUDA cores: decoding requests, each with an adapter of its own, where every byte of A and B is used once and the kernel is bound by
+// reading them; and portions of prompts in 32-bit floats, or of sizes that TMA does not take.  low_rank_tile.cu has the portions on tensor cores.
 //
-// A cluster of eight CTAs takes one token (or eight neighbours) and a range of one slice's columns: each computes an eighth of the hidden values
-// over the whole K and writes them into all CTAs' shared memory, then all have the hidden vector and share the columns.  So it is one launch, no
-// sum crosses CTAs, and B's first 32 KB a CTA are asked for before the hidden values are waited for.
+// Decoding: a cluster of eight CTAs takes one token and a range of one slice's columns; each computes an eighth of the hidden values over the whole K
+// and writes them into all CTAs' shared memory, then all have the hidden vector and share the columns.  So it is one launch, no sum crosses
+// CTAs, and B's first 64 KB a CTA and the results that they are added to are asked for before the hidden values are waited for.
+//
+// Portions: 32 tokens at a time, hidden values (a cluster shares K, its sums meet through distributed shared memory) and results in a launch
+// each.  A tile's tokens may have several adapters: it is gone through once for each of them.
 #include "vec.cuh"
 
 namespace prism {
 namespace lowrank {
 
-constexpr int THREADS = 256, WARPS = THREADS / 32;
+constexpr int THREADS = 512, WARPS = THREADS / 32;
 constexpr int CTAS = 8;                       // of a cluster
 constexpr int AHEAD = 8;                      // 16-byte loads of B in flight a thread
 constexpr int MOST_RANK = 128, MOST_SLICES = 8;
@@ -52,171 +55,132 @@ template <> struct Chunk<__nv_bfloat16> {
     }
 };
 
-// TT: tokens a cluster takes.  Tokens of several adapters among them are taken one adapter after the other.
-template <typename T, typename O, int TT>
-__global__ void __launch_bounds__(THREADS)
-low_rank_kernel(const T* __restrict__ x_, long long ldx, int x_whole, const T* __restrict__ a, const T* __restrict__ b, const float* __restrict__ scale,
-                const int* __restrict__ ids_, const O* __restrict__ base_, long long ldb, O* out_, long long ldo, int first_token, int tokens, int K, int Kp,
-                int r, int L, Slices slices, int parts, int* err) {
+__device__ __forceinline__ void cluster_barrier() { asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory"); }
+__device__ __forceinline__ uint32_t peer(const void* p, int cta) {
+    uint32_t at;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(cta));
+    return at;
+}
+__device__ __forceinline__ uint32_t rank_in_cluster() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+
+// ---- one token ----------------------------------------------------------------------------------------------
+
+template <typename T, typename O>
+__global__ void __launch_bounds__(THREADS, 1)
+low_rank_token_kernel(const T* __restrict__ x_, long long ldx, int x_whole, const T* __restrict__ a, const T* __restrict__ b,
+                      const float* __restrict__ scale, const int* __restrict__ ids_, const O* __restrict__ base_, long long ldb, O* out_, long long ldo,
+                      int K, int Kp, int r, int L, Slices slices, int parts, int* err) {
     constexpr int E = Chunk<T>::E;
-    __shared__ float hidden[TT][MOST_RANK];
-    __shared__ float partial[WARPS][TT];
+    __shared__ float hidden[MOST_RANK];
+    __shared__ float partial[WARPS];
     asm volatile("barrier.cluster.arrive.aligned;" ::: "memory");              // here: peers may write into this CTA's memory
     pdl_trigger();
     pdl_wait();
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    uint32_t me;
-    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(me));
-    const int g = blockIdx.y / parts, part = blockIdx.y % parts, N = slices.first[slices.n];
-    const int t0 = first_token + blockIdx.z * TT, here = min(TT, first_token + tokens - t0);
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, me = (int)rank_in_cluster();
+    const int g = blockIdx.y / parts, part = blockIdx.y % parts, N = slices.first[slices.n], t = blockIdx.z;
     // this CTA's columns: an eighth of its cluster's share of the slice
     const int wide = slices.first[g + 1] - slices.first[g], shares = parts * CTAS, each = (wide + shares - 1) / shares;
-    const int n0 = slices.first[g] + min(wide, (part * CTAS + (int)me) * each), n1 = min(slices.first[g + 1], n0 + each);
-    const T* x = pdl_fresh(x_) + (size_t)t0 * ldx;
-    const O* base = base_ ? pdl_fresh(base_) + (size_t)t0 * ldb : nullptr;
-    O* out = out_ + (size_t)t0 * ldo;
-
-    int id[TT];
-#pragma unroll
-    for (int i = 0; i < TT; ++i) id[i] = i < here ? adapter_of(pdl_fresh(ids_), t0 + i, L, err) : -1;
-#pragma unroll
-    for (int i = 0; i < TT; ++i)
-        if (i < here && id[i] < 0 && out_ != base_)
-            for (int n = n0 + tid; n < n1; n += THREADS) out[(size_t)i * ldo + n] = base ? base[(size_t)i * ldb + n] : from_float<O>(0.f);
-    bool all_here = false;
-
+    const int n0 = slices.first[g] + min(wide, (part * CTAS + me) * each), mine = min(slices.first[g + 1], n0 + each) - n0;
+    const T* x = pdl_fresh(x_) + (size_t)t * ldx;
+    const O* base = base_ ? pdl_fresh(base_) + (size_t)t * ldb + n0 : nullptr;
+    O* out = out_ + (size_t)t * ldo + n0;
+    const int l = adapter_of(pdl_fresh(ids_), t, L, err);
+    if (l < 0) {                                                   // the same for the whole cluster
+        if (out_ != base_)
+            for (int n = tid; n < mine; n += THREADS) out[n] = base ? base[n] : from_float<O>(0.f);
+        asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+        return;
+    }
     // B's chunks: `lanes` neighbours share a row, each with the same part of every row that it meets
     const int chunks = r / E;
     int lanes = 1;
     while (lanes < chunks) lanes *= 2;
     const int chunk = lane % lanes, rows_at_once = THREADS / lanes, row0 = tid / lanes;
     const bool holds = chunk < chunks;
-
-#pragma unroll 1
-    for (int p = 0; p < TT; ++p) {
-        int l = -1;
-        bool mine[TT];
-        {
-            bool again = false;
+    const T* B = b + ((size_t)l * N + n0) * r + chunk * E;
+    uint4 ahead[AHEAD];
+    float old[AHEAD];
 #pragma unroll
-            for (int i = 0; i < TT; ++i) {
-                if (i == p) l = id[i];
-            }
-#pragma unroll
-            for (int i = 0; i < TT; ++i) {
-                mine[i] = id[i] == l;
-                again |= i < p && mine[i];
-            }
-            if (l < 0 || again) continue;                          // the same for the whole cluster
-        }
-        const T* B = b + ((size_t)l * N + n0) * r + chunk * E;
-        uint4 ahead[AHEAD];
-#pragma unroll
-        for (int j = 0; j < AHEAD; ++j) {
-            const int n = row0 + j * rows_at_once;
-            ahead[j] = holds && n < n1 - n0 ? __ldg(reinterpret_cast<const uint4*>(B + (size_t)n * r)) : make_uint4(0, 0, 0, 0);
-        }
-        // an eighth of the hidden values, several warps a row where there are fewer rows than warps
-        const int rows = r / CTAS;
-        int split = 1;
-        while (split * 2 * rows <= WARPS) split *= 2;
-        const int sub = warp % split;
-        const T* A = a + (((size_t)l * slices.n + g) * r + me * rows) * Kp;
-        for (int j0 = 0; j0 < rows; j0 += WARPS / split) {
-            const int j = j0 + warp / split;
-            float s[TT];
-#pragma unroll
-            for (int i = 0; i < TT; ++i) s[i] = 0.f;
-            if (j < rows) {
-                const T* row = A + (size_t)j * Kp;
-#pragma unroll TT == 1 ? 8 : 2
-                for (int k = (sub * 32 + lane) * E; k < K; k += split * 32 * E) {
-                    float w[E];
-                    Chunk<T>::unpack(__ldg(reinterpret_cast<const uint4*>(row + k)), w);
-#pragma unroll
-                    for (int i = 0; i < TT; ++i) {
-                        if (TT > 1 && !mine[i]) continue;
-                        float v[E];
-                        const T* xi = x + (size_t)i * ldx + k;
-                        if (x_whole && k + E <= K) {
-                            Chunk<T>::unpack(*reinterpret_cast<const uint4*>(xi), v);
-                        } else {
-#pragma unroll
-                            for (int e = 0; e < E; ++e) v[e] = k + e < K ? to_float(xi[e]) : 0.f;
-                        }
-#pragma unroll
-                        for (int e = 0; e < E; ++e) s[i] = fmaf(v[e], w[e], s[i]);
-                    }
-                }
-            }
-#pragma unroll
-            for (int i = 0; i < TT; ++i) {
-                s[i] = warp_sum(s[i]);
-                if (lane == 0) partial[warp][i] = s[i];
-            }
-            __syncthreads();
-            if (!all_here) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
-            all_here = true;
-            for (int task = tid; task < TT * (WARPS / split) * CTAS; task += THREADS) {          // a hidden value, for one of the CTAs
-                const int c = task % CTAS, i = task / CTAS % TT, q = task / CTAS / TT;
-                if (j0 + q < rows) {
-                    float h = 0.f;
-                    for (int w = 0; w < split; ++w) h += partial[q * split + w][i];
-                    uint32_t at;
-                    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;"
-                                 : "=r"(at) : "r"((uint32_t)__cvta_generic_to_shared(&hidden[i][me * rows + j0 + q])), "r"(c));
-                    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(at), "f"(h * scale[l]) : "memory");
-                }
-            }
-            __syncthreads();
-        }
-        asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
-        float h[TT][E];
-#pragma unroll
-        for (int i = 0; i < TT; ++i)
-#pragma unroll
-            for (int e = 0; e < E; ++e) h[i][e] = holds ? hidden[i][chunk * E + e] : 0.f;
-        for (int m = 0; m < n1 - n0; m += AHEAD * rows_at_once) {
-#pragma unroll
-            for (int j = 0; j < AHEAD; ++j) {
-                const int n = m + j * rows_at_once + row0;
-                if (m + j * rows_at_once >= n1 - n0) break;
-                float w[E];
-                Chunk<T>::unpack(ahead[j], w);
-                const int next = n + AHEAD * rows_at_once;
-                if (holds && next < n1 - n0) ahead[j] = __ldg(reinterpret_cast<const uint4*>(B + (size_t)next * r));
-#pragma unroll
-                for (int i = 0; i < TT; ++i) {
-                    if (TT > 1 && !mine[i]) continue;
-                    float s = 0.f;
-#pragma unroll
-                    for (int e = 0; e < E; ++e) s = fmaf(h[i][e], w[e], s);
-                    for (int o = 1; o < lanes; o <<= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-                    if (chunk == 0 && n < n1 - n0)
-                        out[(size_t)i * ldo + n0 + n] = from_float<O>(base ? to_float(base[(size_t)i * ldb + n0 + n]) + s : s);
-                }
-            }
-        }
-        if (TT > 1) asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");      // `hidden` is written again
+    for (int j = 0; j < AHEAD; ++j) {
+        const int n = row0 + j * rows_at_once;
+        ahead[j] = holds && n < mine ? __ldg(reinterpret_cast<const uint4*>(B + (size_t)n * r)) : make_uint4(0, 0, 0, 0);
+        old[j] = chunk == 0 && n < mine && base ? to_float(base[n]) : 0.f;
     }
-    if (!all_here) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+    // an eighth of the hidden values, several warps a row where there are fewer rows than warps
+    const int rows = r / CTAS;
+    int split = 1;
+    while (split * 2 * rows <= WARPS) split *= 2;
+    const int sub = warp % split, j = warp / split;                // r / 8 is at most 16: a row a warp at least
+    float s = 0.f;
+    if (j < rows) {
+        const T* row = a + (((size_t)l * slices.n + g) * r + me * rows + j) * Kp;
+#pragma unroll 8
+        for (int k = (sub * 32 + lane) * E; k < K; k += split * 32 * E) {
+            float w[E], v[E];
+            Chunk<T>::unpack(__ldg(reinterpret_cast<const uint4*>(row + k)), w);
+            if (x_whole && k + E <= K) {
+                Chunk<T>::unpack(*reinterpret_cast<const uint4*>(x + k), v);
+            } else {
+#pragma unroll
+                for (int e = 0; e < E; ++e) v[e] = k + e < K ? to_float(x[k + e]) : 0.f;
+            }
+#pragma unroll
+            for (int e = 0; e < E; ++e) s = fmaf(v[e], w[e], s);
+        }
+    }
+    s = warp_sum(s);
+    if (lane == 0) partial[warp] = s;
+    __syncthreads();
+    asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+    if (tid < rows * CTAS) {                                       // a hidden value, for one of the CTAs
+        const int c = tid % CTAS, q = tid / CTAS;
+        float h = 0.f;
+        for (int w = 0; w < split; ++w) h += partial[q * split + w];
+        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(peer(&hidden[me * rows + q], c)), "f"(h * scale[l]) : "memory");
+    }
+    __syncwarp();
+    cluster_barrier();
+    float h[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) h[e] = holds ? hidden[chunk * E + e] : 0.f;
+    for (int m = 0; m < mine; m += AHEAD * rows_at_once) {
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+            if (m + i * rows_at_once >= mine) break;
+            const int n = m + i * rows_at_once + row0, next = n + AHEAD * rows_at_once;
+            float w[E], sum = 0.f;
+            const float was = old[i];
+            Chunk<T>::unpack(ahead[i], w);
+            if (next < mine) {
+                if (holds) ahead[i] = __ldg(reinterpret_cast<const uint4*>(B + (size_t)next * r));
+                if (chunk == 0 && base) old[i] = to_float(base[next]);
+            }
+#pragma unroll
+            for (int e = 0; e < E; ++e) sum = fmaf(h[e], w[e], sum);
+            for (int o = 1; o < lanes; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            if (chunk == 0 && n < mine) out[n] = from_float<O>(was + sum);
+        }
+    }
 }
 
-template <typename T, typename O, int TT>
-int launch(const void* x, long long ldx, const void* a, const void* b, const float* scale, const int* ids, const void* base, long long ldb, void* out,
-           long long ldo, int first_token, int tokens, int K, int Kp, int r, int L, const Slices& s, int* err, int sms, cudaStream_t stream) {
+template <typename T, typename O>
+int launch_tokens(const void* x, long long ldx, const void* a, const void* b, const float* scale, const int* ids, const void* base, long long ldb, void* out,
+                  long long ldo, int tokens, int K, int Kp, int r, int L, const Slices& s, int* err, int sms, cudaStream_t stream) {
     if (tokens <= 0) return 0;
-    const int groups = (tokens + TT - 1) / TT;
-    if (groups > 65535) return (int)cudaErrorInvalidValue;
+    if (tokens > 65535) return (int)cudaErrorInvalidValue;
     // clusters that share a slice's columns: as many as keep B's part of a CTA within what it asks for ahead, while all CTAs together are no
-    // more than four an SM
+    // more than two an SM
     int widest = 0;
     for (int g = 0; g < s.n; ++g) widest = max(widest, s.first[g + 1] - s.first[g]);
     const long long bytes = (long long)widest * r * (int)sizeof(T), ahead = (long long)CTAS * THREADS * AHEAD * 16;
-    const int parts = (int)max(1ll, min((bytes + ahead - 1) / ahead, 4ll * sms / ((long long)CTAS * s.n * groups)));
-    const int whole = (reinterpret_cast<uintptr_t>(x) % 16 == 0) && (ldx * (long long)sizeof(T) % 16 == 0 || tokens + first_token == 1);
+    const int parts = (int)max(1ll, min((bytes + ahead - 1) / ahead, 2ll * sms / ((long long)CTAS * s.n * tokens)));
+    const int whole = (reinterpret_cast<uintptr_t>(x) % 16 == 0) && (ldx * (long long)sizeof(T) % 16 == 0 || tokens == 1);
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(CTAS, s.n * parts, groups);
+    cfg.gridDim = dim3(CTAS, s.n * parts, tokens);
     cfg.blockDim = dim3(THREADS);
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
@@ -226,34 +190,221 @@ int launch(const void* x, long long ldx, const void* a, const void* b, const flo
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = prism::pdl_enabled() ? 2 : 1;
-    return (int)cudaLaunchKernelEx(&cfg, low_rank_kernel<T, O, TT>, (const T*)x, ldx, whole, (const T*)a, (const T*)b, scale, ids, (const O*)base, ldb, (O*)out,
-                                   ldo, first_token, tokens, K, Kp, r, L, s, parts, err);
+    return (int)cudaLaunchKernelEx(&cfg, low_rank_token_kernel<T, O>, (const T*)x, ldx, whole, (const T*)a, (const T*)b, scale, ids, (const O*)base, ldb, (O*)out,
+                                   ldo, K, Kp, r, L, s, parts, err);
+}
+
+// ---- portions -----------------------------------------------------------------------------------------------
+
+constexpr int TOKENS = 32;                    // of a tile
+constexpr int DEEP = 64;                      // of K at a time
+constexpr int HT = 512, PT = 256;             // threads of either launch
+constexpr int COLUMNS = 128;                  // results of a tile
+
+// The tokens' adapters (-1: none, or beyond the end) and the different ones among them, in order.  By the first warp.
+__device__ __forceinline__ void list_adapters(const int* ids, int t0, int tokens, int L, int* own, int* list, int* count, int* err) {
+    const int lane = threadIdx.x;
+    const int id = t0 + lane < tokens ? adapter_of(ids, t0 + lane, L, err) : -1;
+    own[lane] = id;
+    const uint32_t same = __match_any_sync(0xffffffffu, id);
+    const bool first = id >= 0 && __ffs(same) - 1 == lane;
+    const uint32_t found = __ballot_sync(0xffffffffu, first);
+    if (first) list[__popc(found & ((1u << lane) - 1))] = id;
+    if (lane == 0) *count = __popc(found);
+}
+
+// hidden [tokens, G r] float32.  A thread: two tokens by up to four of a slice's hidden values.
+template <typename T>
+__global__ void __launch_bounds__(HT)
+low_rank_plain_hidden_kernel(const T* __restrict__ x_, long long ldx, const T* __restrict__ a, const float* __restrict__ scale,
+                             const int* __restrict__ ids_, float* __restrict__ hidden, int tokens, int K, int Kp, int r, int G, int L, int* err) {
+    __shared__ float xs[TOKENS][DEEP + 1];
+    __shared__ float as[MOST_RANK][DEEP + 1];                      // behind the last block, this CTA's sums
+    float* sums = &as[0][0];                                       // [TOKENS][r]
+    __shared__ int own[TOKENS], list[TOKENS], count;
+    pdl_trigger();
+    pdl_wait();
+    const int tid = threadIdx.x, lane = tid & 31, q = tid >> 5, me = (int)rank_in_cluster(), t0 = blockIdx.y * TOKENS, g = blockIdx.z;
+    if (q == 0) list_adapters(pdl_fresh(ids_), t0, tokens, L, own, list, &count, me == 0 && g == 0 ? err : nullptr);
+    __syncthreads();
+    const T* x = pdl_fresh(x_) + (size_t)t0 * ldx;
+    constexpr int XN = TOKENS * DEEP / HT, AN = MOST_RANK * DEEP / HT;         // values a thread brings of a block
+    for (int p = 0; p < count; ++p) {
+        const int l = list[p];
+        const T* A = a + ((size_t)l * G + g) * r * Kp;
+        float acc[2][4] = {};
+        float xv[XN];
+        T av[AN];
+        auto bring = [&](int k0) {
+#pragma unroll
+            for (int i = 0; i < XN; ++i) {
+                const int row = (tid + i * HT) / DEEP, k = k0 + (tid + i * HT) % DEEP;
+                xv[i] = t0 + row < tokens && k < K ? to_float(x[(size_t)row * ldx + k]) : 0.f;
+            }
+#pragma unroll
+            for (int i = 0; i < AN; ++i) {
+                const int row = (tid + i * HT) / DEEP, k = k0 + (tid + i * HT) % DEEP;
+                if (row < r) av[i] = k < K ? A[(size_t)row * Kp + k] : from_float<T>(0.f);
+            }
+        };
+        bring(me * DEEP);
+        for (int k0 = me * DEEP; k0 < K; k0 += CTAS * DEEP) {
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < XN; ++i) xs[(tid + i * HT) / DEEP][(tid + i * HT) % DEEP] = xv[i];
+#pragma unroll
+            for (int i = 0; i < AN; ++i)
+                if ((tid + i * HT) / DEEP < r) as[(tid + i * HT) / DEEP][(tid + i * HT) % DEEP] = to_float(av[i]);
+            __syncthreads();
+            if (k0 + CTAS * DEEP < K) bring(k0 + CTAS * DEEP);     // the next block's, while this one's are used
+#pragma unroll 4
+            for (int k = 0; k < DEEP; ++k) {
+                float u[2], w[4];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) u[i] = xs[q * 2 + i][k];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) w[i] = lane + 32 * i < r ? as[lane + 32 * i][k] : 0.f;
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) acc[i][c] = fmaf(u[i], w[c], acc[i][c]);
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+                if (lane + 32 * c < r) sums[(q * 2 + i) * r + lane + 32 * c] = acc[i][c];
+        cluster_barrier();
+        // a CTA adds up four tokens' sums
+        for (int v = tid; v < TOKENS / CTAS * r; v += HT) {
+            const int row = me * (TOKENS / CTAS) + v / r, c = v % r;
+            if (own[row] != l) continue;
+            float part[CTAS], s = 0.f;
+#pragma unroll
+            for (int i = 0; i < CTAS; ++i) asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(part[i]) : "r"(peer(sums + row * r + c, i)) : "memory");
+#pragma unroll
+            for (int i = 0; i < CTAS; ++i) s += part[i];
+            hidden[((size_t)(t0 + row) * G + g) * r + c] = s * scale[l];
+        }
+        __syncwarp();
+        cluster_barrier();
+    }
+}
+
+// A thread: four tokens by four columns
+template <typename T, typename O>
+__global__ void __launch_bounds__(PT)
+low_rank_plain_result_kernel(const float* __restrict__ hidden_, const T* __restrict__ b, const int* __restrict__ ids_, const O* base, long long ldb, O* out,
+                             long long ldo, int tokens, int r, int L, Slices slices) {
+    extern __shared__ float plain_smem[];
+    __shared__ int own[TOKENS], list[TOKENS], count;
+    const int pitch = r + 1;
+    float* hs = plain_smem;                                        // [TOKENS][r]
+    float* bs = plain_smem + TOKENS * r;                           // [COLUMNS][pitch]
+    pdl_trigger();
+    pdl_wait();
+    const int tid = threadIdx.x, lane = tid & 31, q = tid >> 5, t0 = blockIdx.y * TOKENS, N = slices.first[slices.n];
+    int g = 0, tile = blockIdx.x;
+    while (g + 1 < slices.n && tile >= (slices.first[g + 1] - slices.first[g] + COLUMNS - 1) / COLUMNS)
+        tile -= (slices.first[g + 1] - slices.first[g] + COLUMNS - 1) / COLUMNS, ++g;
+    const int n0 = slices.first[g] + tile * COLUMNS, wide = min(COLUMNS, slices.first[g + 1] - n0);
+    if (q == 0) list_adapters(pdl_fresh(ids_), t0, tokens, L, own, list, &count, nullptr);
+    float old[4][4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+            old[i][c] = base && t0 + q * 4 + i < tokens && lane + 32 * c < wide ? to_float(base[(size_t)(t0 + q * 4 + i) * ldb + n0 + lane + 32 * c]) : 0.f;
+    __syncthreads();
+    const float* hidden = pdl_fresh(hidden_) + ((size_t)t0 * slices.n + g) * r;
+    for (int p = 0; p < count; ++p) {
+        const int l = list[p];
+        __syncthreads();
+        for (int i = tid; i < TOKENS * r; i += PT) hs[i] = own[i / r] == l ? hidden[(size_t)(i / r) * slices.n * r + i % r] : 0.f;
+        const T* B = b + ((size_t)l * N + n0) * r;
+#pragma unroll 8
+        for (int i = tid; i < wide * r; i += PT) bs[i / r * pitch + i % r] = to_float(B[i]);
+        __syncthreads();
+        float acc[4][4] = {};
+#pragma unroll 4
+        for (int k = 0; k < r; ++k) {
+            float u[4], w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) u[i] = hs[(q * 4 + i) * r + k];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) w[c] = bs[(lane + 32 * c) * pitch + k];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) acc[i][c] = fmaf(u[i], w[c], acc[i][c]);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (own[q * 4 + i] == l)
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+                    if (lane + 32 * c < wide) out[(size_t)(t0 + q * 4 + i) * ldo + n0 + lane + 32 * c] = from_float<O>(old[i][c] + acc[i][c]);
+    }
+    if ((const O*)out != base)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (own[q * 4 + i] < 0 && t0 + q * 4 + i < tokens)
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+                    if (lane + 32 * c < wide) out[(size_t)(t0 + q * 4 + i) * ldo + n0 + lane + 32 * c] = from_float<O>(old[i][c]);
+}
+
+template <typename T, typename O>
+int launch_portions(const void* x, long long ldx, const void* a, const void* b, const float* scale, const int* ids, const void* base, long long ldb, void* out,
+                    long long ldo, int tokens, int K, int Kp, int r, int L, const Slices& s, void* hidden, int* err, cudaStream_t stream) {
+    if (tokens <= 0) return 0;
+    const int tiles = (tokens + TOKENS - 1) / TOKENS;
+    if (tiles > 65535 || hidden == nullptr) return (int)cudaErrorInvalidValue;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(CTAS, tiles, s.n);
+    cfg.blockDim = dim3(HT);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = CTAS, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = prism::pdl_enabled() ? 2 : 1;
+    int code = (int)cudaLaunchKernelEx(&cfg, low_rank_plain_hidden_kernel<T>, (const T*)x, ldx, (const T*)a, scale, ids, (float*)hidden, tokens, K, Kp, r, s.n, L,
+                                       err);
+    if (code != 0) return code;
+    int columns = 0;
+    for (int g = 0; g < s.n; ++g) columns += (s.first[g + 1] - s.first[g] + COLUMNS - 1) / COLUMNS;
+    const size_t smem = ((size_t)TOKENS * r + (size_t)COLUMNS * (r + 1)) * 4;
+    prism::open_smem(low_rank_plain_result_kernel<T, O>, smem);
+    return (int)prism::launch_kernel(low_rank_plain_result_kernel<T, O>, dim3(columns, tiles), dim3(PT), smem, stream, (const float*)hidden, (const T*)b, ids,
+                                     (const O*)base, ldb, (O*)out, ldo, tokens, r, L, s);
 }
 
 }  // namespace lowrank
 }  // namespace prism
 
-// first: G + 1 column borders (host memory).  base may be null (nothing to add to), or out itself.  The first `singles` tokens one by one, the
-// others eight at a time.
+// first: G + 1 column borders (host memory).  base may be null (nothing to add to), or out itself.  hidden null: all T tokens one by one; else in
+// tiles, with T G r floats of workspace there.
 PRISM_EXPORT int prism_low_rank(const void* x, long long ldx, int dtype, const void* a, const void* b, const float* scale, const int* ids,
                                 const void* base, long long ldb, void* out, long long ldo, int out_dtype, int T, int K, int Kp, int r, int L, int G,
-                                const int* first, int singles, int sms, int* err, cudaStream_t stream) {
+                                const int* first, void* hidden, int sms, int* err, cudaStream_t stream) {
     using namespace prism::lowrank;
     typedef __nv_bfloat16 bf16;
     if (T <= 0) return 0;
-    if (G < 1 || G > MOST_SLICES || r < 16 || r % 16 || r > MOST_RANK || K < 1 || Kp < K || Kp % 8 || L < 1 || singles < 0 || singles > T || sms < 1)
-        return (int)cudaErrorInvalidValue;
+    if (G < 1 || G > MOST_SLICES || r < 16 || r % 16 || r > MOST_RANK || K < 1 || Kp < K || Kp % 8 || L < 1 || sms < 1) return (int)cudaErrorInvalidValue;
     Slices s;
     s.n = G;
     for (int g = 0; g <= G; ++g) s.first[g] = first[g];
     for (int g = 0; g < G; ++g)
         if (s.first[g] >= s.first[g + 1]) return (int)cudaErrorInvalidValue;
-#define PRISM_LOW_RANK(TX, TO, TT, at, n) launch<TX, TO, TT>(x, ldx, a, b, scale, ids, base, ldb, out, ldo, at, n, K, Kp, r, L, s, err, sms, stream)
-#define PRISM_LOW_RANK_TYPES(TT, at, n)                                                                                          \
-    (dtype == PRISM_DTYPE_F32 ? (out_dtype == PRISM_DTYPE_F32 ? PRISM_LOW_RANK(float, float, TT, at, n) : PRISM_LOW_RANK(float, bf16, TT, at, n)) \
-                              : (out_dtype == PRISM_DTYPE_F32 ? PRISM_LOW_RANK(bf16, float, TT, at, n) : PRISM_LOW_RANK(bf16, bf16, TT, at, n)))
-    const int code = PRISM_LOW_RANK_TYPES(1, 0, singles);
-    return code != 0 ? code : PRISM_LOW_RANK_TYPES(8, singles, T - singles);
-#undef PRISM_LOW_RANK_TYPES
+#define PRISM_LOW_RANK(TX, TO)                                                                                                           \
+    (hidden ? launch_portions<TX, TO>(x, ldx, a, b, scale, ids, base, ldb, out, ldo, T, K, Kp, r, L, s, hidden, err, stream)              \
+            : launch_tokens<TX, TO>(x, ldx, a, b, scale, ids, base, ldb, out, ldo, T, K, Kp, r, L, s, err, sms, stream))
+    if (dtype == PRISM_DTYPE_F32) return out_dtype == PRISM_DTYPE_F32 ? PRISM_LOW_RANK(float, float) : PRISM_LOW_RANK(float, bf16);
+    return out_dtype == PRISM_DTYPE_F32 ? PRISM_LOW_RANK(bf16, float) : PRISM_LOW_RANK(bf16, bf16);
 #undef PRISM_LOW_RANK
 }

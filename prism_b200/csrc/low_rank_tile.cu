@@ -29,10 +29,12 @@ struct Tiles {
 // The tokens' adapters (-1: none, or beyond the end) and the different ones among them, in order.  By one warp.
 __device__ __forceinline__ void list_adapters(const int* ids, int t0, int tokens, int L, int* own, int* list, int* count, int* err) {
     const int lane = threadIdx.x & 31;
-    int n = 0;
+    int n = 0, all[TILE / 32];
+#pragma unroll
+    for (int q = 0; q < TILE / 32; ++q) all[q] = t0 + q * 32 + lane < tokens ? ids[t0 + q * 32 + lane] : -1;
+#pragma unroll
     for (int q = 0; q < TILE / 32; ++q) {
-        const int t = t0 + q * 32 + lane;
-        int id = t < tokens ? ids[t] : -1;
+        int id = all[q];
         if (id >= L) {
             report_error(err, PRISM_ERR_ADAPTER_RANGE);
             id = -1;
@@ -50,6 +52,7 @@ __device__ __forceinline__ void list_adapters(const int* ids, int t0, int tokens
     if (lane == 0) *count = n;
 }
 
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* map) { asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory"); }
 __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(bar)) : "memory");
 }
@@ -77,6 +80,7 @@ low_rank_hidden_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_c
     volatile int* abortp = &abort_flag;
 
     if (threadIdx.x == 0) {
+        prefetch_map(&map_x), prefetch_map(&map_a);
         abort_flag = 0;
         for (int s = 0; s < stages; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
         mbar_init(&done, 1);
@@ -223,7 +227,7 @@ template <> struct Eight<float> {
 };
 
 template <typename O>
-__global__ void __launch_bounds__(ALL_THREADS)
+__global__ void __launch_bounds__(ALL_THREADS, sizeof(O) == 2 ? 2 : 1)
 low_rank_result_kernel(const __grid_constant__ CUtensorMap map_b, const __nv_bfloat16* __restrict__ hidden_, const int* __restrict__ ids_,
                        const O* base, long long ldb, O* out, long long ldo, int aligned, int tokens, int r, int N, int L, Tiles tiles, int* err) {
     constexpr int STAGES = 2;
@@ -246,6 +250,7 @@ low_rank_result_kernel(const __grid_constant__ CUtensorMap map_b, const __nv_bfl
     const int j0 = (int)((long long)all * unit / units), j1 = (int)((long long)all * (unit + 1) / units);
 
     if (threadIdx.x == 0) {
+        prefetch_map(&map_b);
         abort_flag = 0;
         for (int s = 0; s < STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
         for (int s = 0; s < 2; ++s) { mbar_init(&acc_full[s], 1); mbar_init(&acc_empty[s], EPI_WARPS); }
@@ -325,58 +330,65 @@ low_rank_result_kernel(const __grid_constant__ CUtensorMap map_b, const __nv_bfl
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 mbar_arrive(&h_full);
             }
-            for (int j = j0; j < j1; ++j, ++i) {
-                const int buf = i & 1;
+            // Steps of 64 columns.  What a step adds to is asked for a step ahead: eight columns of four rows a thread.
+            const int c = tid % 8 * 8, row0 = tid / 8, steps = 2 * (j1 - j0);
+            Eight<O> old[4], ahead[4];
+            auto ask = [&](Eight<O> (&e)[4], int step) {
+                const int n0 = n_first + j0 * TILE + step * CHUNK;
+                const bool whole = aligned && n0 % 8 == 0 && step < steps && n0 + c + 8 <= n_end;
+#pragma unroll
+                for (int m = 0; m < 4; ++m) {
+                    const int row = row0 + 32 * m;
+                    e[m].zero();
+                    if (whole && base && own[row] == l) e[m].load(base + (size_t)(t0 + row) * ldb + n0 + c);
+                }
+            };
+            ask(ahead, 0);
 #pragma unroll 1
-                for (int c0 = 0; c0 < TILE; c0 += CHUNK) {
-                    const int n0 = n_first + j * TILE + c0, wide = min(CHUNK, n_end - n0);
-                    // what the result is added to, asked for before the sums are waited for: eight columns of four rows a thread
-                    const int c = tid % 8 * 8, row0 = tid / 8;
+            for (int step = 0; step < steps; ++step) {
+                const int buf = i & 1, half = step & 1, n0 = n_first + j0 * TILE + step * CHUNK, wide = min(CHUNK, n_end - n0);
+#pragma unroll
+                for (int m = 0; m < 4; ++m) old[m] = ahead[m];
+                ask(ahead, step + 1);
+                if (half == 0) {
+                    ok = __all_sync(0xffffffffu, mbar_wait(&acc_full[buf], (i / 2) & 1, abortp)) && ok;
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                }
+                if (wide > 0 && ok) {
+                    float v[32];
+                    tmem_load<32>(tmem + ((uint32_t)(q * 32) << 16) + buf * TILE + half * CHUNK + part * 32, v);
+                    float* row = sums + (q * 32 + lane) * CHUNK_LD + part * 32;
+#pragma unroll
+                    for (int e = 0; e < 32; e += 4) *reinterpret_cast<float4*>(row + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+                }
+                if (half == 1) {                                   // the accumulator has been read
+                    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&acc_empty[buf]);
+                    ++i;
+                }
+                epilogue_barrier();
+                if (ok && c < wide) {
                     const bool whole = aligned && n0 % 8 == 0 && c + 8 <= wide;
-                    Eight<O> old[4];
 #pragma unroll
                     for (int m = 0; m < 4; ++m) {
                         const int row = row0 + 32 * m;
-                        old[m].zero();
-                        if (whole && base && own[row] == l) old[m].load(base + (size_t)(t0 + row) * ldb + n0 + c);
-                    }
-                    if (c0 == 0) {
-                        ok = __all_sync(0xffffffffu, mbar_wait(&acc_full[buf], (i / 2) & 1, abortp)) && ok;
-                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    }
-                    if (wide > 0 && ok) {
-                        float v[32];
-                        tmem_load<32>(tmem + ((uint32_t)(q * 32) << 16) + buf * TILE + c0 + part * 32, v);
-                        float* row = sums + (q * 32 + lane) * CHUNK_LD + part * 32;
+                        if (own[row] != l) continue;
+                        float v[8], s[8];
+                        load8(sums + row * CHUNK_LD + c, s);
+                        O* to = out + (size_t)(t0 + row) * ldo + n0 + c;
+                        if (whole) {
+                            old[m].get(v);
 #pragma unroll
-                        for (int e = 0; e < 32; e += 4) *reinterpret_cast<float4*>(row + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
-                    }
-                    if (c0 + CHUNK >= TILE) {                      // the accumulator has been read
-                        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(&acc_empty[buf]);
-                    }
-                    epilogue_barrier();
-                    if (ok)
-#pragma unroll
-                        for (int m = 0; m < 4; ++m) {
-                            const int row = row0 + 32 * m;
-                            if (own[row] != l || c >= wide) continue;
-                            float v[8], s[8];
-                            load8(sums + row * CHUNK_LD + c, s);
-                            O* to = out + (size_t)(t0 + row) * ldo + n0 + c;
-                            if (whole) {
-                                old[m].get(v);
-#pragma unroll
-                                for (int e = 0; e < 8; ++e) v[e] += s[e];
-                                store8(to, v);
-                            } else {
-                                for (int e = 0; e < min(8, wide - c); ++e)
-                                    to[e] = from_float<O>(base ? to_float(base[(size_t)(t0 + row) * ldb + n0 + c + e]) + s[e] : s[e]);
-                            }
+                            for (int e = 0; e < 8; ++e) v[e] += s[e];
+                            store8(to, v);
+                        } else {
+                            for (int e = 0; e < min(8, wide - c); ++e)
+                                to[e] = from_float<O>(base ? to_float(base[(size_t)(t0 + row) * ldb + n0 + c + e]) + s[e] : s[e]);
                         }
-                    epilogue_barrier();
+                    }
                 }
+                epilogue_barrier();
             }
         }
         if ((const O*)out != base) {          // tokens without an adapter
@@ -454,7 +466,7 @@ PRISM_EXPORT int prism_low_rank_tile(const void* x, long long ldx, const void* a
     // the second launch: two CTAs an SM, as their shared memory allows, share the tiles of results; a CTA has some columns of one slice
     const int kblocks = (r + prism::tc::TILE_K - 1) / prism::tc::TILE_K;
     smem = 1024 + (size_t)(2 + 2) * kblocks * BLOCK_BYTES + sums;
-    const int slots = (smem <= 110 * 1024 ? 2 : 1) * sms;
+    const int slots = (smem <= 110 * 1024 && out_dtype == PRISM_DTYPE_BF16 ? 2 : 1) * sms;
     const double per = all <= slots / tiles ? 1.0 : (double)all * tiles / slots;       // tiles of columns a CTA
     s.units[0] = 0;
     for (int g = 0; g < G; ++g) {

@@ -133,7 +133,7 @@ def in_use(w):
 
 
 SINGLES = 64                 # without a word from the caller, so many tokens are taken one by one
-TILE_FROM = 16               # so many tokens of portions, and they are taken in tiles of 128
+TILE_FROM = 16               # so many tokens of portions, and they are taken in tiles of 128 on tensor cores
 
 
 def low_rank(x: torch.Tensor, low: LowRank, ids: torch.Tensor, base: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
@@ -171,19 +171,21 @@ def low_rank(x: torch.Tensor, low: LowRank, ids: torch.Tensor, base: Optional[to
     what = (low.scale.data_ptr(), ids.data_ptr())
     sizes = (low.k, a.shape[3], low.rank, low.count, len(low.rows), low._address)
     sms, err, stream, dt, odt = ops.num_sms(x.device), ops.mxfp4._err_word(x.device), ops._stream(), ops._dt(x), ops._dt(out)
-    tiled = 0
-    if T - singles >= TILE_FROM and dt == ops.BF16:
-        skip = singles * xs * 2
-        if L.prism_low_rank_tile_supported(low.k, low.rank, len(low.rows), (xp + skip) % 16 == 0 and (xs % 8 == 0 or T - singles == 1)):
-            tiled = T - singles
-    if T > tiled:
-        ops._check(L.prism_low_rank(xp, xs, dt, a.data_ptr(), low.b.data_ptr(), *what, bp or None, bs, op, os_, odt, T - tiled, *sizes,
-                                    min(singles, T - tiled), sms, err, stream), "low_rank")
-    if tiled:
-        size = 2 if odt == ops.BF16 else 4
-        hidden = torch.empty(2 * tiled * len(low.rows) * low.rank, dtype=torch.bfloat16, device=x.device)
-        ops._check(L.prism_low_rank_tile(xp + singles * xs * 2, xs, a.data_ptr(), low.b.data_ptr(), what[0], what[1] + 4 * singles,
-                                         bp + singles * bs * size if bp else None, bs, op + singles * os_ * size, os_, odt, tiled, *sizes,
-                                         hidden.data_ptr(), sms, err, stream), "low_rank_tile")
-        ops.launch_count += 1                # two kernels
+    if singles:
+        ops._check(L.prism_low_rank(xp, xs, dt, a.data_ptr(), low.b.data_ptr(), *what, bp or None, bs, op, os_, odt, singles, *sizes, None, sms, err, stream),
+                   "low_rank")
+    rest = T - singles
+    if rest == 0:
+        return out
+    # behind the singles, in tiles
+    size, G = 2 if odt == ops.BF16 else 4, len(low.rows)
+    xp, op, bp = xp + singles * xs * (2 if dt == ops.BF16 else 4), op + singles * os_ * size, bp + singles * bs * size if bp else None
+    args = (low.scale.data_ptr(), ids.data_ptr() + 4 * singles, bp, bs, op, os_, odt, rest, *sizes)
+    if dt == ops.BF16 and rest >= TILE_FROM and L.prism_low_rank_tile_supported(low.k, low.rank, G, xp % 16 == 0 and (xs % 8 == 0 or rest == 1)):
+        hidden = torch.empty(2 * rest * G * low.rank, dtype=torch.bfloat16, device=x.device)
+        ops._check(L.prism_low_rank_tile(xp, xs, a.data_ptr(), low.b.data_ptr(), *args, hidden.data_ptr(), sms, err, stream), "low_rank_tile")
+    else:
+        hidden = torch.empty(rest * G * low.rank, dtype=torch.float32, device=x.device)
+        ops._check(L.prism_low_rank(xp, xs, dt, a.data_ptr(), low.b.data_ptr(), *args, hidden.data_ptr(), sms, err, stream), "low_rank")
+    ops.launch_count += 1                    # two kernels
     return out

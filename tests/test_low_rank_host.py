@@ -62,11 +62,11 @@ def test_the_library_refuses_sizes():
     first = (ctypes.c_int * 3)(0, 8, 12)
     p = ctypes.addressof(first)
 
-    def low_rank(T=4, K=20, Kp=24, r=16, L=2, G=2, first=p, singles=4, sms=148):
-        return lib.prism_low_rank(p, 24, 0, p, p, p, p, p, 12, p, 12, 0, T, K, Kp, r, L, G, first, singles, sms, p, None)
+    def low_rank(T=4, K=20, Kp=24, r=16, L=2, G=2, first=p, hidden=None, sms=148):
+        return lib.prism_low_rank(p, 24, 0, p, p, p, p, p, 12, p, 12, 0, T, K, Kp, r, L, G, first, hidden, sms, p, None)
     assert low_rank(T=0) == 0
     back = (ctypes.c_int * 3)(0, 8, 8)
-    for change in (dict(G=0), dict(G=9), dict(r=8), dict(r=0), dict(r=144), dict(r=24), dict(K=0), dict(Kp=16), dict(Kp=20, K=20), dict(L=0), dict(singles=-1), dict(singles=5), dict(sms=0),
+    for change in (dict(G=0), dict(G=9), dict(r=8), dict(r=0), dict(r=144), dict(r=24), dict(K=0), dict(Kp=16), dict(Kp=20, K=20), dict(L=0), dict(sms=0),
                    dict(first=ctypes.addressof(back))):
         assert low_rank(**change) == 1, change
 
