@@ -10,7 +10,7 @@
 //
 // Decoding: a cluster of eight CTAs takes one token and a range of one slice's columns; each computes an eighth of the hidden values over the whole K
 // and writes them into all CTAs' shared memory, then all have the hidden vector and share the columns.  So it is one launch, no sum crosses
-// CTAs, and B's first 64 KB a CTA and the results that they are added to are asked for before the hidden values are waited for.
+// CTAs, and B's first 32 KB a CTA and the results that they are added to are asked for before the hidden values are waited for.
 //
 // Portions: 32 tokens at a time, hidden values (a cluster shares K, its sums meet through distributed shared memory) and results in a launch
 // each.  A tile's tokens may have several adapters: it is gone through once for each of them.
@@ -21,7 +21,7 @@ namespace lowrank {
 
 constexpr int THREADS = 512, WARPS = THREADS / 32;
 constexpr int CTAS = 8;                       // of a cluster
-constexpr int AHEAD = 8;                      // 16-byte loads of B in flight a thread
+constexpr int AHEAD = 4;                      // 16-byte loads of B in flight a thread
 constexpr int MOST_RANK = 128, MOST_SLICES = 8;
 
 struct Slices {
@@ -70,7 +70,7 @@ __device__ __forceinline__ uint32_t rank_in_cluster() {
 // ---- one token ----------------------------------------------------------------------------------------------
 
 template <typename T, typename O>
-__global__ void __launch_bounds__(THREADS, 1)
+__global__ void __launch_bounds__(THREADS, 2)
 low_rank_token_kernel(const T* __restrict__ x_, long long ldx, int x_whole, const T* __restrict__ a, const T* __restrict__ b,
                       const float* __restrict__ scale, const int* __restrict__ ids_, const O* __restrict__ base_, long long ldb, O* out_, long long ldo,
                       int K, int Kp, int r, int L, Slices slices, int parts, int* err) {
@@ -118,7 +118,7 @@ low_rank_token_kernel(const T* __restrict__ x_, long long ldx, int x_whole, cons
     float s = 0.f;
     if (j < rows) {
         const T* row = a + (((size_t)l * slices.n + g) * r + me * rows + j) * Kp;
-#pragma unroll 8
+#pragma unroll 4
         for (int k = (sub * 32 + lane) * E; k < K; k += split * 32 * E) {
             float w[E], v[E];
             Chunk<T>::unpack(__ldg(reinterpret_cast<const uint4*>(row + k)), w);
@@ -173,11 +173,11 @@ int launch_tokens(const void* x, long long ldx, const void* a, const void* b, co
     if (tokens <= 0) return 0;
     if (tokens > 65535) return (int)cudaErrorInvalidValue;
     // clusters that share a slice's columns: as many as keep B's part of a CTA within what it asks for ahead, while all CTAs together are no
-    // more than two an SM
+    // more than four an SM
     int widest = 0;
     for (int g = 0; g < s.n; ++g) widest = max(widest, s.first[g + 1] - s.first[g]);
     const long long bytes = (long long)widest * r * (int)sizeof(T), ahead = (long long)CTAS * THREADS * AHEAD * 16;
-    const int parts = (int)max(1ll, min((bytes + ahead - 1) / ahead, 2ll * sms / ((long long)CTAS * s.n * tokens)));
+    const int parts = (int)max(1ll, min((bytes + ahead - 1) / ahead, 4ll * sms / ((long long)CTAS * s.n * tokens)));
     const int whole = (reinterpret_cast<uintptr_t>(x) % 16 == 0) && (ldx * (long long)sizeof(T) % 16 == 0 || tokens == 1);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(CTAS, s.n * parts, tokens);

@@ -4,9 +4,12 @@
 // slices' A (TMA, 128-byte swizzle, tcgen05.mma with the tokens as M); their sums meet through distributed shared memory, are scaled and leave as
 // two bfloat16 terms, high and low (2^-16 of a hidden value is lost; one term alone would lose 2^-8, as much as rounding the result does).  The
 // second multiplies them with B, 128 columns at a time, and adds the shared result: it is bound by reading and writing that - the 7B shape's gate
-// and up for 2,048 tokens are 310 MB against 28 MB of everything else.
+// and up for 2,048 tokens are 310 MB against 28 MB of everything else.  So the shared result comes and goes by TMA, boxes of 128 rows by 128 bytes, some
+// of them ahead, and a thread adds its row's sums where they lie in shared memory.
 //
-// A tile's tokens may have several adapters: it is gone through once for each of them, and only that adapter's rows are stored.
+// A tile's tokens may have several adapters, or some of them none.  The first launch goes through it once for each adapter; the second has up to four
+// adapters' products side by side in tensor memory.  With more than four, or where base and out are no place for TMA, it goes through the tile
+// once for each adapter, and the threads store that adapter's rows.
 #include "tcgen05.cuh"
 #include "vec.cuh"
 
@@ -20,6 +23,7 @@ constexpr int CTAS = 8;                       // that share a tile's K
 constexpr int EPI_WARPS = 8, EPI_THREADS = EPI_WARPS * 32, ALL_THREADS = EPI_THREADS + 64;
 constexpr int MOST_RANK = 128, MOST_SLICES = 8, MOST_HIDDEN = 512;
 constexpr int CHUNK = 64, CHUNK_LD = CHUNK + 4;                   // columns of sums on their way through shared memory, and their pitch
+constexpr int WIDE = 128, WIDE_LD = WIDE + 4;                     // the same of hidden values
 
 struct Tiles {
     int n, first[MOST_SLICES + 1];            // slice g has the result columns first[g] .. first[g + 1] - 1
@@ -63,7 +67,7 @@ __device__ __forceinline__ void epilogue_barrier() { asm volatile("bar.sync 1, %
 
 // ---- hidden values ------------------------------------------------------------------------------------------
 
-// hidden: [2][tokens][G r], high terms and low ones
+// hidden: [tokens][2][G r], high terms and low ones
 __global__ void __launch_bounds__(ALL_THREADS)
 low_rank_hidden_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_a, const float* __restrict__ scale,
                        const int* __restrict__ ids_, __nv_bfloat16* __restrict__ hidden, int tokens, int K, int r, int G, int L, int stages,
@@ -86,18 +90,18 @@ low_rank_hidden_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_c
         mbar_init(&done, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    pdl_wait();                               // before tensor memory is taken: a kernel that this one waits for may still want it
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&tmem_slot)), "r"(tmem_cols));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
     }
-    pdl_wait();
     if (warp == 2) list_adapters(pdl_fresh(ids_), t0, tokens, L, own, list, &count, me == 0 ? err : nullptr);
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = tmem_slot;
     const int passes = count;
-    pdl_trigger();                            // not before this CTA has its tensor memory: a kernel that waits for this one may hold the rest
+    pdl_trigger();                            // not before this CTA has its tensor memory: the next kernel may take the rest and wait
 
     int it = 0;                               // blocks so far, over all passes
     bool go = true;                           // no wait of this warp has run out
@@ -149,29 +153,33 @@ low_rank_hidden_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_c
             if (mine > 0) go = __all_sync(0xffffffffu, mbar_wait(&done, p & 1, abortp)) && go;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         }
-        for (int c0 = 0; c0 < H; c0 += CHUNK) {
+        for (int c0 = 0; c0 < H; c0 += WIDE) {
             if (warp >= 2) {
                 // this CTA's sums: a thread's row is its tensor memory lane
-                const int c = c0 + half * 32;
-                if (c < H) {
+#pragma unroll
+                for (int m = 0; m < WIDE / 64; ++m) {
+                    const int at = m * 64 + half * 32;
+                    if (c0 + at >= H) break;
                     float v[32];
                     if (mine > 0 && go) {
-                        tmem_load<32>(tmem + ((uint32_t)(q * 32) << 16) + c, v);       // columns beyond H are allocated, and not used
+                        tmem_load<32>(tmem + ((uint32_t)(q * 32) << 16) + c0 + at, v);       // columns beyond H are allocated, and not used
                     } else {
 #pragma unroll
                         for (int i = 0; i < 32; ++i) v[i] = 0.f;
                     }
-                    float* row = sums + (q * 32 + lane) * CHUNK_LD + half * 32;
+                    float* row = sums + (q * 32 + lane) * WIDE_LD + at;
 #pragma unroll
                     for (int i = 0; i < 32; i += 4) *reinterpret_cast<float4*>(row + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
                 }
             }
             asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
             if (warp >= 2) {
-                // sixteen rows of all CTAs' sums: four columns a thread
-                const int row = me * (TILE / CTAS) + tid / (CHUNK / 4), c = tid % (CHUNK / 4) * 4, t = t0 + row;
-                if (c0 + c < H && own[row] == l && go) {
-                    const uint32_t at = smem_addr(sums + row * CHUNK_LD + c);
+                // sixteen rows of all CTAs' sums: four columns a thread at a time
+                const int wide = min(WIDE, H - c0) / 4;
+                for (int e = tid; e < TILE / CTAS * wide; e += EPI_THREADS) {
+                    const int row = me * (TILE / CTAS) + e / wide, c = e % wide * 4, t = t0 + row;
+                    if (own[row] != l || !go) continue;
+                    const uint32_t at = smem_addr(sums + row * WIDE_LD + c);
                     float4 part[CTAS];
 #pragma unroll
                     for (int j = 0; j < CTAS; ++j) {
@@ -192,11 +200,12 @@ low_rank_hidden_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_c
                         const float rest = h - __bfloat162float(hi[i]);
                         lo[i] = __float2bfloat16_rn(rest == rest ? rest : 0.f);        // an infinity's rest is none
                     }
-                    __nv_bfloat16* to = hidden + (size_t)t * H + c0 + c;
+                    __nv_bfloat16* to = hidden + (size_t)t * 2 * H + c0 + c;
                     *reinterpret_cast<uint2*>(to) = *reinterpret_cast<uint2*>(hi);
-                    *reinterpret_cast<uint2*>(to + (size_t)tokens * H) = *reinterpret_cast<uint2*>(lo);
+                    *reinterpret_cast<uint2*>(to + H) = *reinterpret_cast<uint2*>(lo);
                 }
             }
+            __syncwarp();
             asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
         }
         it += mine;
@@ -226,18 +235,30 @@ template <> struct Eight<float> {
     }
 };
 
+struct Boxes { CUtensorMap base[MOST_SLICES], out[MOST_SLICES]; };         // a slice's columns each
+
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, const void* src, int c0, int c1) {
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(map), "r"(smem_addr(src)), "r"(c0), "r"(c1) : "memory");
+}
+
+constexpr int B_STAGES = 2, MOST_BOXES = 6, ACCS = 4;              // ACCS: accumulators, all of tensor memory
+constexpr int RESULT_THREADS = ALL_THREADS + 32;                  // one more warp, that asks for boxes
+
+// by_box: a bit a slice, whether its columns of base and out can go by TMA; depth: how many boxes there is memory for
 template <typename O>
-__global__ void __launch_bounds__(ALL_THREADS, sizeof(O) == 2 ? 2 : 1)
-low_rank_result_kernel(const __grid_constant__ CUtensorMap map_b, const __nv_bfloat16* __restrict__ hidden_, const int* __restrict__ ids_,
-                       const O* base, long long ldb, O* out, long long ldo, int aligned, int tokens, int r, int N, int L, Tiles tiles, int* err) {
-    constexpr int STAGES = 2;
+__global__ void __launch_bounds__(RESULT_THREADS, 1)
+low_rank_result_kernel(const __grid_constant__ CUtensorMap map_h, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ Boxes boxes,
+                       const int* __restrict__ ids_, const O* base, long long ldb, O* out, long long ldo, int by_box, int depth, int aligned, int tokens, int r, int N,
+                       int L, Tiles tiles, int* err) {
+    constexpr int BOX_COLS = 128 / (int)sizeof(O), PER_TILE = TILE / BOX_COLS;         // columns of a box of 128 bytes a row
     extern __shared__ unsigned char raw[];
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
     const int kblocks = (r + TILE_K - 1) / TILE_K;
-    unsigned char* h_hi = smem;
-    unsigned char* ring = smem + 2 * kblocks * BLOCK_BYTES;                            // behind the low terms
-    float* sums = reinterpret_cast<float*>(ring + STAGES * kblocks * BLOCK_BYTES);
-    __shared__ uint64_t full[STAGES], empty[STAGES], acc_full[2], acc_empty[2], h_full;
+    unsigned char* h_hi = smem;                                                        // high terms, then low ones
+    unsigned char* ring = smem + 2 * kblocks * BLOCK_BYTES;
+    unsigned char* box = ring + B_STAGES * kblocks * BLOCK_BYTES;
+    float* sums = reinterpret_cast<float*>(box);                                       // where no boxes are used
+    __shared__ uint64_t full[B_STAGES], empty[B_STAGES], acc_full[ACCS], acc_empty[ACCS], h_full, box_full[MOST_BOXES], box_empty[MOST_BOXES];
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_flag, own[TILE], list[TILE], count;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, t0 = blockIdx.y * TILE;
@@ -250,160 +271,284 @@ low_rank_result_kernel(const __grid_constant__ CUtensorMap map_b, const __nv_bfl
     const int j0 = (int)((long long)all * unit / units), j1 = (int)((long long)all * (unit + 1) / units);
 
     if (threadIdx.x == 0) {
-        prefetch_map(&map_b);
+        prefetch_map(&map_h), prefetch_map(&map_b), prefetch_map(&boxes.base[g]), prefetch_map(&boxes.out[g]);
         abort_flag = 0;
-        for (int s = 0; s < STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
-        for (int s = 0; s < 2; ++s) { mbar_init(&acc_full[s], 1); mbar_init(&acc_empty[s], EPI_WARPS); }
-        mbar_init(&h_full, EPI_THREADS);
+        for (int s = 0; s < B_STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+        for (int s = 0; s < ACCS; ++s) { mbar_init(&acc_full[s], 1); mbar_init(&acc_empty[s], EPI_WARPS); }
+        for (int s = 0; s < MOST_BOXES; ++s) { mbar_init(&box_full[s], 1); mbar_init(&box_empty[s], EPI_WARPS / 2); }
+        mbar_init(&h_full, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    pdl_wait();
     if (warp == 1) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&tmem_slot)), "r"(2 * TILE));
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&tmem_slot)), "r"(ACCS * TILE));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
     }
-    pdl_wait();
     if (warp == 2) list_adapters(pdl_fresh(ids_), t0, tokens, L, own, list, &count, nullptr);
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = tmem_slot;
     const int passes = count;
-    pdl_trigger();                            // not before this CTA has its tensor memory: a kernel that waits for this one may hold the rest
+    // Up to ACCS adapters: their products with a tile of columns lie side by side in tensor memory, a thread takes its row's, and the results go by
+    // boxes.  Else one adapter after the other.
+    const bool by_boxes = passes > 0 && passes <= ACCS && (by_box >> g & 1);
+    pdl_trigger();                            // not before this CTA has its tensor memory: the next kernel may take the rest and wait
+    // products are numbered: tile by tile and in it adapter by adapter, or adapter by adapter
+    const int products = passes * (j1 - j0);
+    auto adapter_of_product = [&](int i) { return list[by_boxes ? i % passes : i / (j1 - j0)]; };
+    auto tile_of_product = [&](int i) { return j0 + (by_boxes ? i / passes : i % (j1 - j0)); };
 
     if (warp == 0) {
-        if (lane == 0) {
+        if (lane == 0 && products > 0) {
+            // a token's hidden values are its own adapter's, whichever B they are multiplied with: other rows of a product are not used
+            mbar_expect_tx(&h_full, 2 * kblocks * BLOCK_BYTES);
+            for (int term = 0; term < 2; ++term)
+                for (int k = 0; k < kblocks; ++k)
+                    tma_load_2d(h_hi + (term * kblocks + k) * BLOCK_BYTES, &map_h, &h_full, (term * tiles.n + g) * r + k * TILE_K, t0);
             int i = 0;
-            for (int p = 0; p < passes && !*abortp; ++p)
-                for (int j = j0; j < j1; ++j, ++i) {
-                    const int s = i % STAGES;
-                    if (i >= STAGES && !mbar_wait(&empty[s], (i / STAGES - 1) & 1, abortp)) break;
-                    mbar_expect_tx(&full[s], kblocks * BLOCK_BYTES);
-                    for (int k = 0; k < kblocks; ++k)
-                        tma_load_2d(ring + (s * kblocks + k) * BLOCK_BYTES, &map_b, &full[s], k * TILE_K, list[p] * N + n_first + j * TILE);
-                }
-            if (*abortp)
-                for (int k = max(0, i - STAGES); k < i; ++k) mbar_wait(&full[k % STAGES], (k / STAGES) & 1, abortp);
+            for (; i < products; ++i) {
+                const int s = i % B_STAGES;
+                if (i >= B_STAGES && !mbar_wait(&empty[s], (i / B_STAGES - 1) & 1, abortp)) break;
+                mbar_expect_tx(&full[s], kblocks * BLOCK_BYTES);
+                for (int k = 0; k < kblocks; ++k)
+                    tma_load_2d(ring + (s * kblocks + k) * BLOCK_BYTES, &map_b, &full[s], k * TILE_K, adapter_of_product(i) * N + n_first + tile_of_product(i) * TILE);
+            }
+            if (*abortp) {                    // copies in flight get a bounded chance to land
+                mbar_wait(&h_full, 0, abortp);
+                for (int k = max(0, i - B_STAGES); k < i; ++k) mbar_wait(&full[k % B_STAGES], (k / B_STAGES) & 1, abortp);
+            }
         }
     } else if (warp == 1) {
-        if (lane == 0) {
+        if (lane == 0 && products > 0) {
             const uint32_t idesc = instruction(TILE);
-            int i = 0;
-            bool ok = true;
-            for (int p = 0; p < passes && ok; ++p) {
-                ok = mbar_wait(&h_full, p & 1, abortp);
-                for (int j = j0; j < j1 && ok; ++j, ++i) {
-                    const int s = i % STAGES, buf = i & 1;
-                    ok = mbar_wait(&full[s], (i / STAGES) & 1, abortp) && (i < 2 || mbar_wait(&acc_empty[buf], (i / 2 - 1) & 1, abortp));
-                    if (!ok) break;
-                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    const uint32_t d = tmem + buf * TILE;
-                    for (int k = 0; k < r / UMMA_K; ++k) {
-                        const int block = k / 4, in = k % 4;
-                        const uint64_t db = umma_desc(smem_addr(ring + (s * kblocks + block) * BLOCK_BYTES)) + (uint64_t)(in * UMMA_K * 2 >> 4);
-                        const uint64_t dh = umma_desc(smem_addr(h_hi + block * BLOCK_BYTES)) + (uint64_t)(in * UMMA_K * 2 >> 4);
-                        const uint64_t dl = umma_desc(smem_addr(h_hi + (kblocks + block) * BLOCK_BYTES)) + (uint64_t)(in * UMMA_K * 2 >> 4);
-                        umma_bf16(d, dh, db, idesc, k > 0 ? 1u : 0u);
-                        umma_bf16(d, dl, db, idesc, 1u);
-                    }
-                    umma_commit(&empty[s]);
-                    umma_commit(&acc_full[buf]);
+            bool ok = mbar_wait(&h_full, 0, abortp);
+            for (int i = 0; i < products && ok; ++i) {
+                const int s = i % B_STAGES, acc = i % ACCS;
+                ok = mbar_wait(&full[s], (i / B_STAGES) & 1, abortp) && (i < ACCS || mbar_wait(&acc_empty[acc], (i / ACCS - 1) & 1, abortp));
+                if (!ok) break;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const uint32_t d = tmem + acc * TILE;
+                for (int k = 0; k < r / UMMA_K; ++k) {
+                    const int block = k / 4, in = k % 4;
+                    const uint64_t db = umma_desc(smem_addr(ring + (s * kblocks + block) * BLOCK_BYTES)) + (uint64_t)(in * UMMA_K * 2 >> 4);
+                    const uint64_t dh = umma_desc(smem_addr(h_hi + block * BLOCK_BYTES)) + (uint64_t)(in * UMMA_K * 2 >> 4);
+                    const uint64_t dl = umma_desc(smem_addr(h_hi + (kblocks + block) * BLOCK_BYTES)) + (uint64_t)(in * UMMA_K * 2 >> 4);
+                    umma_bf16(d, dh, db, idesc, k > 0 ? 1u : 0u);
+                    umma_bf16(d, dl, db, idesc, 1u);
                 }
+                umma_commit(&empty[s]);
+                umma_commit(&acc_full[acc]);
             }
         }
+    } else if (warp == RESULT_THREADS / 32 - 1) {
+        if (lane == 0 && by_boxes && base) {
+            const int steps = PER_TILE * (j1 - j0);
+            int i = 0;
+            for (; i < steps; ++i) {
+                const int s = i % depth;
+                if (i >= depth && !mbar_wait(&box_empty[s], (i / depth - 1) & 1, abortp)) break;
+                mbar_expect_tx(&box_full[s], BLOCK_BYTES);
+                tma_load_2d(box + s * BLOCK_BYTES, &boxes.base[g], &box_full[s], j0 * TILE + i * BOX_COLS, t0);
+            }
+            if (*abortp)
+                for (int k = max(0, i - depth); k < i; ++k) mbar_wait(&box_full[k % depth], (k / depth) & 1, abortp);
+        }
     } else {
-        const int tid = threadIdx.x - 64, q = warp & 3, part = (warp - 2) >> 2;
-        const int H = tiles.n * r;
         // after a wait that ran out the loops go on, as the barriers of these threads count on all of them, but touch nothing
+        const int tid = threadIdx.x - 64, q = warp & 3, part = (warp - 2) >> 2;
         int i = 0;
         bool ok = true;
-        for (int p = 0; p < passes; ++p) {
-            const int l = list[p];
-            {
-                // the adapter's hidden rows as operands, the others zero: high terms by one half of the threads, low ones by the other
-                const int row = tid % TILE, term = tid / TILE;
-                const bool mine = own[row] == l;
-                const uint4* from = reinterpret_cast<const uint4*>(pdl_fresh(hidden_) + ((size_t)term * tokens + (mine ? t0 + row : 0)) * H + g * r);
-                unsigned char* to = h_hi + term * kblocks * BLOCK_BYTES + row * 128;
-#pragma unroll 4
-                for (int c = 0; c < r / 8; ++c)
-                    *reinterpret_cast<uint4*>(to + c / 8 * BLOCK_BYTES + ((c % 8) ^ (row & 7)) * 16) = mine ? from[c] : make_uint4(0, 0, 0, 0);
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                mbar_arrive(&h_full);
-            }
-            // Steps of 64 columns.  What a step adds to is asked for a step ahead: eight columns of four rows a thread.
-            const int c = tid % 8 * 8, row0 = tid / 8, steps = 2 * (j1 - j0);
-            Eight<O> old[4], ahead[4];
-            auto ask = [&](Eight<O> (&e)[4], int step) {
-                const int n0 = n_first + j0 * TILE + step * CHUNK;
-                const bool whole = aligned && n0 % 8 == 0 && step < steps && n0 + c + 8 <= n_end;
-#pragma unroll
-                for (int m = 0; m < 4; ++m) {
-                    const int row = row0 + 32 * m;
-                    e[m].zero();
-                    if (whole && base && own[row] == l) e[m].load(base + (size_t)(t0 + row) * ldb + n0 + c);
-                }
-            };
-            ask(ahead, 0);
+        auto wait_for_sums = [&](int product) {
+            ok = __all_sync(0xffffffffu, mbar_wait(&acc_full[product % ACCS], (product / ACCS) & 1, abortp)) && ok;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        };
+        auto sums_read = [&](int product) {
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&acc_empty[product % ACCS]);
+        };
+        if (by_boxes) {
+            // A thread has a row of a box; four warps have one, the other four the next, and no warp waits for another: each sends its 32 rows off.
+            // 16 bytes of a row lie at their place xor the row's number: no bank conflicts.
+            constexpr int E = 16 / (int)sizeof(O);
+            const int row = q * 32 + lane;
+            int which = -1;                   // the row's adapter among the tile's
+            for (int p = 0; p < passes; ++p)
+                if (own[row] == list[p]) which = p;
+            int last = -1;                    // the box of this warp's last store
 #pragma unroll 1
-            for (int step = 0; step < steps; ++step) {
-                const int buf = i & 1, half = step & 1, n0 = n_first + j0 * TILE + step * CHUNK, wide = min(CHUNK, n_end - n0);
+            for (int t = 0; t < j1 - j0; ++t) {
+                for (int p = 0; p < passes; ++p) wait_for_sums(t * passes + p);
+#pragma unroll 1
+                for (int in = part; in < PER_TILE; in += 2) {
+                    const int step = t * PER_TILE + in, s = step % depth;
+                    float v[BOX_COLS];
 #pragma unroll
-                for (int m = 0; m < 4; ++m) old[m] = ahead[m];
-                ask(ahead, step + 1);
-                if (half == 0) {
-                    ok = __all_sync(0xffffffffu, mbar_wait(&acc_full[buf], (i / 2) & 1, abortp)) && ok;
-                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                }
-                if (wide > 0 && ok) {
-                    float v[32];
-                    tmem_load<32>(tmem + ((uint32_t)(q * 32) << 16) + buf * TILE + half * CHUNK + part * 32, v);
-                    float* row = sums + (q * 32 + lane) * CHUNK_LD + part * 32;
+                    for (int c = 0; c < BOX_COLS; ++c) v[c] = 0.f;
+                    if (ok)
+#pragma unroll 1
+                        for (int p = 0; p < passes; ++p) {
+                            float w[BOX_COLS];
+                            tmem_load<BOX_COLS>(tmem + ((uint32_t)(q * 32) << 16) + (t * passes + p) % ACCS * TILE + in * BOX_COLS, w);
 #pragma unroll
-                    for (int e = 0; e < 32; e += 4) *reinterpret_cast<float4*>(row + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
-                }
-                if (half == 1) {                                   // the accumulator has been read
-                    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                            for (int c = 0; c < BOX_COLS; ++c) v[c] = which == p ? w[c] : v[c];
+                        }
+                    if (in + 2 >= PER_TILE)
+                        for (int p = 0; p < passes; ++p) sums_read(t * passes + p);
+                    if (base) {
+                        ok = __all_sync(0xffffffffu, mbar_wait(&box_full[s], (step / depth) & 1, abortp)) && ok;
+                    } else if (step >= depth) {                    // the stores that had this box's memory have read it
+                        ok = __all_sync(0xffffffffu, mbar_wait(&box_empty[s], (step / depth - 1) & 1, abortp)) && ok;
+                    }
+                    if (ok)
+#pragma unroll
+                        for (int c = 0; c < 8; ++c) {
+                            O* at = reinterpret_cast<O*>(box + s * BLOCK_BYTES + row * 128 + ((c ^ (row & 7)) * 16));
+                            __align__(16) O w[E];
+                            if (base) *reinterpret_cast<uint4*>(w) = *reinterpret_cast<uint4*>(at);
+#pragma unroll
+                            for (int e = 0; e < E; ++e) w[e] = from_float<O>(base ? to_float(w[e]) + v[c * E + e] : v[c * E + e]);
+                            *reinterpret_cast<uint4*>(at) = *reinterpret_cast<uint4*>(w);
+                        }
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(&acc_empty[buf]);
-                    ++i;
+                    if (lane == 0) {
+                        const int c = j0 * TILE + step * BOX_COLS;
+                        if (ok && c < n_end - n_first && t0 + q * 32 < tokens)
+                            tma_store_2d(&boxes.out[g], box + s * BLOCK_BYTES + q * 32 * 128, c, t0 + q * 32);
+                        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+                        // this warp's store before this one has read its rows
+                        asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+                        if (last >= 0) mbar_arrive(&box_empty[last]);
+                        last = s;
+                    }
                 }
-                epilogue_barrier();
-                if (ok && c < wide) {
-                    const bool whole = aligned && n0 % 8 == 0 && c + 8 <= wide;
+            }
+            if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+        } else {
+            for (int p = 0; p < passes; ++p) {
+                const int l = list[p];
+                // Steps of 64 columns.  What a step adds to is asked for a step ahead: eight columns of four rows a thread.
+                const int c = tid % 8 * 8, row0 = tid / 8, steps = 2 * (j1 - j0);
+                Eight<O> old[4], ahead[4];
+                auto ask = [&](Eight<O> (&e)[4], int step) {
+                    const int n0 = n_first + j0 * TILE + step * CHUNK;
+                    const bool whole = aligned && n0 % 8 == 0 && step < steps && n0 + c + 8 <= n_end;
 #pragma unroll
                     for (int m = 0; m < 4; ++m) {
                         const int row = row0 + 32 * m;
-                        if (own[row] != l) continue;
-                        float v[8], s[8];
-                        load8(sums + row * CHUNK_LD + c, s);
-                        O* to = out + (size_t)(t0 + row) * ldo + n0 + c;
-                        if (whole) {
-                            old[m].get(v);
+                        e[m].zero();
+                        if (whole && base && own[row] == l) e[m].load(base + (size_t)(t0 + row) * ldb + n0 + c);
+                    }
+                };
+                ask(ahead, 0);
+#pragma unroll 1
+                for (int step = 0; step < steps; ++step) {
+                    const int acc = i % ACCS, half = step & 1, n0 = n_first + j0 * TILE + step * CHUNK, wide = min(CHUNK, n_end - n0);
 #pragma unroll
-                            for (int e = 0; e < 8; ++e) v[e] += s[e];
-                            store8(to, v);
-                        } else {
-                            for (int e = 0; e < min(8, wide - c); ++e)
-                                to[e] = from_float<O>(base ? to_float(base[(size_t)(t0 + row) * ldb + n0 + c + e]) + s[e] : s[e]);
+                    for (int m = 0; m < 4; ++m) old[m] = ahead[m];
+                    ask(ahead, step + 1);
+                    if (half == 0) wait_for_sums(i);
+                    if (wide > 0 && ok) {
+                        float v[32];
+                        tmem_load<32>(tmem + ((uint32_t)(q * 32) << 16) + acc * TILE + half * CHUNK + part * 32, v);
+                        float* row = sums + (q * 32 + lane) * CHUNK_LD + part * 32;
+#pragma unroll
+                        for (int e = 0; e < 32; e += 4) *reinterpret_cast<float4*>(row + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+                    }
+                    if (half == 1) sums_read(i++);
+                    epilogue_barrier();
+                    if (ok && c < wide) {
+                        const bool whole = aligned && n0 % 8 == 0 && c + 8 <= wide;
+#pragma unroll
+                        for (int m = 0; m < 4; ++m) {
+                            const int row = row0 + 32 * m;
+                            if (own[row] != l) continue;
+                            float v[8], s[8];
+                            load8(sums + row * CHUNK_LD + c, s);
+                            O* to = out + (size_t)(t0 + row) * ldo + n0 + c;
+                            if (whole) {
+                                old[m].get(v);
+#pragma unroll
+                                for (int e = 0; e < 8; ++e) v[e] += s[e];
+                                store8(to, v);
+                            } else {
+                                for (int e = 0; e < min(8, wide - c); ++e)
+                                    to[e] = from_float<O>(base ? to_float(base[(size_t)(t0 + row) * ldb + n0 + c + e]) + s[e] : s[e]);
+                            }
                         }
                     }
+                    epilogue_barrier();
                 }
-                epilogue_barrier();
             }
-        }
-        if ((const O*)out != base) {          // tokens without an adapter
-            const int n0 = n_first + j0 * TILE, n1 = min(n_end, n_first + j1 * TILE);
-            for (int row = warp - 2; row < TILE; row += EPI_WARPS)
-                if (own[row] < 0 && t0 + row < tokens)
-                    for (int n = n0 + lane; n < n1; n += 32)
-                        out[(size_t)(t0 + row) * ldo + n] = base ? base[(size_t)(t0 + row) * ldb + n] : from_float<O>(0.f);
+            if ((const O*)out != base) {      // tokens without an adapter
+                const int n0 = n_first + j0 * TILE, n1 = min(n_end, n_first + j1 * TILE);
+                for (int row = warp - 2; row < TILE; row += EPI_WARPS)
+                    if (own[row] < 0 && t0 + row < tokens)
+                        for (int n = n0 + lane; n < n1; n += 32)
+                            out[(size_t)(t0 + row) * ldo + n] = base ? base[(size_t)(t0 + row) * ldb + n] : from_float<O>(0.f);
+            }
         }
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     if (threadIdx.x == 0 && abort_flag) report_error(err, PRISM_ERR_WAIT_TIMEOUT);
-    if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * TILE));
+    if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(ACCS * TILE));
+}
+
+// Columns of base or out as boxes of rows of 128 bytes
+template <typename O> int make_box_map(CUtensorMap* map, const void* ptr, long long rows, long long cols, long long ld, int box_rows) {
+    if (sizeof(O) == 2) return prism::tc::make_map(map, ptr, rows, cols, ld, box_rows);
+    EncodeTiledFn fn = encode_fn();
+    if (fn == nullptr) return (int)cudaErrorNotSupported;
+    cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+    cuuint64_t strides[1] = {(cuuint64_t)ld * 4};
+    cuuint32_t size[2] = {32, (cuuint32_t)box_rows};
+    cuuint32_t estr[2] = {1, 1};
+    const CUresult code = fn(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, const_cast<void*>(ptr), dims, strides, size, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return code == CUDA_SUCCESS ? 0 : (int)cudaErrorInvalidValue;
+}
+
+template <typename O>
+int launch_results(const void* hidden, const CUtensorMap& map_b, const int* ids, const void* base, long long ldb, void* out, long long ldo, int T, int r, int L,
+                   Tiles s, int* err, int sms, cudaStream_t stream) {
+    const int tiles = (T + TILE - 1) / TILE, G = s.n, N = s.first[G], kblocks = (r + TILE_K - 1) / TILE_K;
+    CUtensorMap map_h;
+    int code = prism::tc::make_map(&map_h, hidden, T, 2ll * G * r, 2ll * G * r, TILE);
+    if (code != 0) return code;
+    Boxes boxes;
+    int by_box = 0;
+    const long long row_b = T > 1 ? ldb : (N + 7) / 8 * 8, row_o = T > 1 ? ldo : (N + 7) / 8 * 8;
+    for (int g = 0; g < G; ++g) {
+        const int n0 = s.first[g], wide = s.first[g + 1] - n0;
+        const O* b = base ? (const O*)base + n0 : nullptr;
+        O* o = (O*)out + n0;
+        bool fits = reinterpret_cast<uintptr_t>(b) % 16 == 0 && reinterpret_cast<uintptr_t>(o) % 16 == 0 && row_b * (long long)sizeof(O) % 16 == 0 &&
+                    row_o * (long long)sizeof(O) % 16 == 0 && wide * sizeof(O) % 16 == 0;      // a box that ends inside 16 bytes writes more of them
+        fits = fits && make_box_map<O>(&boxes.out[g], o, T, wide, row_o, 32) == 0 &&
+               make_box_map<O>(&boxes.base[g], b ? b : o, T, wide, b ? row_b : row_o, TILE) == 0;
+        if (fits) by_box |= 1 << g;
+        else boxes.out[g] = boxes.base[g] = map_h;                 // never followed
+    }
+    // a CTA an SM shares the tiles of results; it has some columns of one slice
+    int all = 0;
+    for (int g = 0; g < G; ++g) all += (s.first[g + 1] - s.first[g] + TILE - 1) / TILE;
+    const double per = all <= sms / tiles ? 1.0 : (double)all * tiles / sms;           // tiles of columns a CTA
+    s.units[0] = 0;
+    for (int g = 0; g < G; ++g) {
+        const int mine = (s.first[g + 1] - s.first[g] + TILE - 1) / TILE;
+        s.units[g + 1] = s.units[g] + max(1, min(mine, (int)(mine / per)));
+    }
+    const int aligned = reinterpret_cast<uintptr_t>(out) % 16 == 0 && reinterpret_cast<uintptr_t>(base) % 16 == 0 &&
+                        (T == 1 || (ldo % 8 == 0 && (base == nullptr || ldb % 8 == 0)));
+    const int depth = kblocks == 1 ? MOST_BOXES : 4;
+    const size_t smem = 1024 + (size_t)((2 + B_STAGES) * kblocks + depth) * BLOCK_BYTES;
+    prism::open_smem(low_rank_result_kernel<O>, smem);
+    return (int)prism::launch_kernel(low_rank_result_kernel<O>, dim3(s.units[G], tiles), dim3(RESULT_THREADS), smem, stream, map_h, map_b, boxes, ids, (const O*)base,
+                                     ldb, (O*)out, ldo, by_box, depth, aligned, T, r, N, L, s, err);
 }
 
 }  // namespace lowrank
@@ -428,11 +573,8 @@ PRISM_EXPORT int prism_low_rank_tile(const void* x, long long ldx, const void* a
     Tiles s;
     s.n = G;
     for (int g = 0; g <= G; ++g) s.first[g] = first[g];
-    long long all = 0;
-    for (int g = 0; g < G; ++g) {
+    for (int g = 0; g < G; ++g)
         if (s.first[g] >= s.first[g + 1]) return (int)cudaErrorInvalidValue;
-        all += (s.first[g + 1] - s.first[g] + TILE - 1) / TILE;
-    }
     const int N = first[G], tiles = (T + TILE - 1) / TILE, H = G * r;
     if ((long long)L * N >= 1ll << 31 || (long long)L * H >= 1ll << 31) return (int)cudaErrorInvalidValue;
     CUtensorMap map_x, map_a, map_b;
@@ -442,8 +584,8 @@ PRISM_EXPORT int prism_low_rank_tile(const void* x, long long ldx, const void* a
     if (code == 0) code = prism::tc::make_map(&map_b, b, (long long)L * N, r, r, TILE);
     if (code != 0) return code;
 
-    const int stage = BLOCK_BYTES + H * prism::tc::TILE_K * 2, sums = TILE * CHUNK_LD * 4;
-    const int stages = min(6, (190 * 1024 - sums) / stage);
+    const int stage = BLOCK_BYTES + H * prism::tc::TILE_K * 2, sums = TILE * WIDE_LD * 4;
+    const int stages = min(6, (198 * 1024 - sums) / stage);
     int cols = 32;
     while (cols < H) cols *= 2;
     size_t smem = 1024 + (size_t)stages * stage + sums;
@@ -463,25 +605,6 @@ PRISM_EXPORT int prism_low_rank_tile(const void* x, long long ldx, const void* a
     code = (int)cudaLaunchKernelEx(&cfg, low_rank_hidden_kernel, map_x, map_a, scale, ids, (bf16*)hidden, T, K, r, G, L, stages, cols, err);
     if (code != 0) return code;
 
-    // the second launch: two CTAs an SM, as their shared memory allows, share the tiles of results; a CTA has some columns of one slice
-    const int kblocks = (r + prism::tc::TILE_K - 1) / prism::tc::TILE_K;
-    smem = 1024 + (size_t)(2 + 2) * kblocks * BLOCK_BYTES + sums;
-    const int slots = (smem <= 110 * 1024 && out_dtype == PRISM_DTYPE_BF16 ? 2 : 1) * sms;
-    const double per = all <= slots / tiles ? 1.0 : (double)all * tiles / slots;       // tiles of columns a CTA
-    s.units[0] = 0;
-    for (int g = 0; g < G; ++g) {
-        const int mine = (s.first[g + 1] - s.first[g] + TILE - 1) / TILE;
-        s.units[g + 1] = s.units[g] + max(1, min(mine, (int)(mine / per)));
-    }
-    const int aligned = reinterpret_cast<uintptr_t>(out) % 16 == 0 && reinterpret_cast<uintptr_t>(base) % 16 == 0 &&
-                        (T == 1 || (ldo % 8 == 0 && (base == nullptr || ldb % 8 == 0)));
-    const dim3 grid(s.units[G], tiles);
-    if (out_dtype == PRISM_DTYPE_F32) {
-        prism::open_smem(low_rank_result_kernel<float>, smem);
-        return (int)prism::launch_kernel(low_rank_result_kernel<float>, grid, dim3(ALL_THREADS), smem, stream, map_b, (const bf16*)hidden, ids, (const float*)base,
-                                         ldb, (float*)out, ldo, aligned, T, r, N, L, s, err);
-    }
-    prism::open_smem(low_rank_result_kernel<bf16>, smem);
-    return (int)prism::launch_kernel(low_rank_result_kernel<bf16>, grid, dim3(ALL_THREADS), smem, stream, map_b, (const bf16*)hidden, ids, (const bf16*)base, ldb,
-                                     (bf16*)out, ldo, aligned, T, r, N, L, s, err);
+    if (out_dtype == PRISM_DTYPE_F32) return launch_results<float>(hidden, map_b, ids, base, ldb, out, ldo, T, r, L, s, err, sms, stream);
+    return launch_results<bf16>(hidden, map_b, ids, base, ldb, out, ldo, T, r, L, s, err, sms, stream);
 }
