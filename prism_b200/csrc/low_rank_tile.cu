@@ -292,7 +292,7 @@ low_rank_result_kernel(const __grid_constant__ CUtensorMap map_h, const __grid_c
     const int passes = count;
     // Up to ACCS adapters: their products with a tile of columns lie side by side in tensor memory, a thread takes its row's, and the results go by
     // boxes.  Else one adapter after the other.
-    const bool by_boxes = passes > 0 && passes <= ACCS && (by_box >> g & 1);
+    const bool nothing = passes == 0 && (const O*)out == base, by_boxes = !nothing && passes <= ACCS && (by_box >> g & 1);
     pdl_trigger();                            // not before this CTA has its tensor memory: the next kernel may take the rest and wait
     // products are numbered: tile by tile and in it adapter by adapter, or adapter by adapter
     const int products = passes * (j1 - j0);
@@ -485,9 +485,21 @@ low_rank_result_kernel(const __grid_constant__ CUtensorMap map_h, const __grid_c
             if ((const O*)out != base) {      // tokens without an adapter
                 const int n0 = n_first + j0 * TILE, n1 = min(n_end, n_first + j1 * TILE);
                 for (int row = warp - 2; row < TILE; row += EPI_WARPS)
-                    if (own[row] < 0 && t0 + row < tokens)
-                        for (int n = n0 + lane; n < n1; n += 32)
-                            out[(size_t)(t0 + row) * ldo + n] = base ? base[(size_t)(t0 + row) * ldb + n] : from_float<O>(0.f);
+                    if (own[row] < 0 && t0 + row < tokens) {
+                        O* to = out + (size_t)(t0 + row) * ldo;
+                        const O* from = base ? base + (size_t)(t0 + row) * ldb : nullptr;
+                        const bool eights = aligned && n0 % 8 == 0;
+#pragma unroll 2
+                        for (int n = n0 + lane * 8; eights && n + 8 <= n1; n += 256) {
+                            Eight<O> e;
+                            e.zero();
+                            if (from) e.load(from + n);
+                            float v[8];
+                            e.get(v);
+                            store8(to + n, v);
+                        }
+                        for (int n = (eights ? n1 - (n1 - n0) % 8 : n0) + lane; n < n1; n += 32) to[n] = from ? from[n] : from_float<O>(0.f);
+                    }
             }
         }
     }
