@@ -241,14 +241,47 @@ __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, const void*
     asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(map), "r"(smem_addr(src)), "r"(c0), "r"(c1) : "memory");
 }
 
-constexpr int B_STAGES = 2, MOST_BOXES = 6, ACCS = 4;              // ACCS: accumulators, all of tensor memory
-constexpr int RESULT_THREADS = ALL_THREADS + 32;                  // one more warp, that asks for boxes
+constexpr int MOST_STAGES = 4, MOST_BOXES = 6, ACCS = 4;           // ACCS: accumulators, all of tensor memory
+constexpr int PARTS = 4;                                          // groups of four warps that each have a box
+constexpr int RESULT_THREADS = 64 + PARTS * 128 + 32;             // and one more warp, that asks for boxes
 
-// by_box: a bit a slice, whether its columns of base and out can go by TMA; depth: how many boxes there is memory for
+// 32 columns of a warp's lanes in one load
+__device__ __forceinline__ void tmem_load_wide(uint32_t at, float (&v)[32]) {
+    uint32_t r[32];
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,"
+                 "%28,%29,%30,%31}, [%32];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+                   "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]),
+                   "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]),
+                   "=r"(r[31])
+                 : "r"(at));
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void tmem_load_wide(uint32_t at, float (&v)[16]) { tmem_load<16>(at, v); }
+
+// 16 bytes of results, plus sums
+__device__ __forceinline__ uint4 plus(const uint4& old, const float* v, __nv_bfloat16) {
+    const uint32_t u[4] = {old.x, old.y, old.z, old.w};
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const __nv_bfloat162 t = __floats2bfloat162_rn(__uint_as_float(u[i] << 16) + v[2 * i], __uint_as_float(u[i] & 0xffff0000u) + v[2 * i + 1]);
+        w[i] = *reinterpret_cast<const uint32_t*>(&t);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+__device__ __forceinline__ uint4 plus(const uint4& old, const float* v, float) {
+    return make_uint4(__float_as_uint(__uint_as_float(old.x) + v[0]), __float_as_uint(__uint_as_float(old.y) + v[1]),
+                      __float_as_uint(__uint_as_float(old.z) + v[2]), __float_as_uint(__uint_as_float(old.w) + v[3]));
+}
+
+// by_box: a bit a slice, whether its columns of base and out can go by TMA; depth, stages: how many boxes and tiles of B there is memory for
 template <typename O>
 __global__ void __launch_bounds__(RESULT_THREADS, 1)
 low_rank_result_kernel(const __grid_constant__ CUtensorMap map_h, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ Boxes boxes,
-                       const int* __restrict__ ids_, const O* base, long long ldb, O* out, long long ldo, int by_box, int depth, int aligned, int tokens, int r, int N,
+                       const int* __restrict__ ids_, const O* base, long long ldb, O* out, long long ldo, int by_box, int depth, int stages, int aligned, int tokens, int r, int N,
                        int L, Tiles tiles, int* err) {
     constexpr int BOX_COLS = 128 / (int)sizeof(O), PER_TILE = TILE / BOX_COLS;         // columns of a box of 128 bytes a row
     extern __shared__ unsigned char raw[];
@@ -256,9 +289,9 @@ low_rank_result_kernel(const __grid_constant__ CUtensorMap map_h, const __grid_c
     const int kblocks = (r + TILE_K - 1) / TILE_K;
     unsigned char* h_hi = smem;                                                        // high terms, then low ones
     unsigned char* ring = smem + 2 * kblocks * BLOCK_BYTES;
-    unsigned char* box = ring + B_STAGES * kblocks * BLOCK_BYTES;
+    unsigned char* box = ring + stages * kblocks * BLOCK_BYTES;
     float* sums = reinterpret_cast<float*>(box);                                       // where no boxes are used
-    __shared__ uint64_t full[B_STAGES], empty[B_STAGES], acc_full[ACCS], acc_empty[ACCS], h_full, box_full[MOST_BOXES], box_empty[MOST_BOXES];
+    __shared__ uint64_t full[MOST_STAGES], empty[MOST_STAGES], acc_full[ACCS], acc_empty[ACCS], h_full, box_full[MOST_BOXES], box_empty[MOST_BOXES];
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_flag, own[TILE], list[TILE], count;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, t0 = blockIdx.y * TILE;
@@ -273,9 +306,9 @@ low_rank_result_kernel(const __grid_constant__ CUtensorMap map_h, const __grid_c
     if (threadIdx.x == 0) {
         prefetch_map(&map_h), prefetch_map(&map_b), prefetch_map(&boxes.base[g]), prefetch_map(&boxes.out[g]);
         abort_flag = 0;
-        for (int s = 0; s < B_STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
-        for (int s = 0; s < ACCS; ++s) { mbar_init(&acc_full[s], 1); mbar_init(&acc_empty[s], EPI_WARPS); }
-        for (int s = 0; s < MOST_BOXES; ++s) { mbar_init(&box_full[s], 1); mbar_init(&box_empty[s], EPI_WARPS / 2); }
+        for (int s = 0; s < MOST_STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+        for (int s = 0; s < ACCS; ++s) { mbar_init(&acc_full[s], 1); mbar_init(&acc_empty[s], 4 * min(PARTS, PER_TILE)); }
+        for (int s = 0; s < MOST_BOXES; ++s) { mbar_init(&box_full[s], 1); mbar_init(&box_empty[s], 4); }
         mbar_init(&h_full, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -308,15 +341,15 @@ low_rank_result_kernel(const __grid_constant__ CUtensorMap map_h, const __grid_c
                     tma_load_2d(h_hi + (term * kblocks + k) * BLOCK_BYTES, &map_h, &h_full, (term * tiles.n + g) * r + k * TILE_K, t0);
             int i = 0;
             for (; i < products; ++i) {
-                const int s = i % B_STAGES;
-                if (i >= B_STAGES && !mbar_wait(&empty[s], (i / B_STAGES - 1) & 1, abortp)) break;
+                const int s = i % stages;
+                if (i >= stages && !mbar_wait(&empty[s], (i / stages - 1) & 1, abortp)) break;
                 mbar_expect_tx(&full[s], kblocks * BLOCK_BYTES);
                 for (int k = 0; k < kblocks; ++k)
                     tma_load_2d(ring + (s * kblocks + k) * BLOCK_BYTES, &map_b, &full[s], k * TILE_K, adapter_of_product(i) * N + n_first + tile_of_product(i) * TILE);
             }
             if (*abortp) {                    // copies in flight get a bounded chance to land
                 mbar_wait(&h_full, 0, abortp);
-                for (int k = max(0, i - B_STAGES); k < i; ++k) mbar_wait(&full[k % B_STAGES], (k / B_STAGES) & 1, abortp);
+                for (int k = max(0, i - stages); k < i; ++k) mbar_wait(&full[k % stages], (k / stages) & 1, abortp);
             }
         }
     } else if (warp == 1) {
@@ -324,8 +357,8 @@ low_rank_result_kernel(const __grid_constant__ CUtensorMap map_h, const __grid_c
             const uint32_t idesc = instruction(TILE);
             bool ok = mbar_wait(&h_full, 0, abortp);
             for (int i = 0; i < products && ok; ++i) {
-                const int s = i % B_STAGES, acc = i % ACCS;
-                ok = mbar_wait(&full[s], (i / B_STAGES) & 1, abortp) && (i < ACCS || mbar_wait(&acc_empty[acc], (i / ACCS - 1) & 1, abortp));
+                const int s = i % stages, acc = i % ACCS;
+                ok = mbar_wait(&full[s], (i / stages) & 1, abortp) && (i < ACCS || mbar_wait(&acc_empty[acc], (i / ACCS - 1) & 1, abortp));
                 if (!ok) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const uint32_t d = tmem + acc * TILE;
@@ -357,76 +390,78 @@ low_rank_result_kernel(const __grid_constant__ CUtensorMap map_h, const __grid_c
     } else {
         // after a wait that ran out the loops go on, as the barriers of these threads count on all of them, but touch nothing
         const int tid = threadIdx.x - 64, q = warp & 3, part = (warp - 2) >> 2;
-        int i = 0;
         bool ok = true;
         auto wait_for_sums = [&](int product) {
             ok = __all_sync(0xffffffffu, mbar_wait(&acc_full[product % ACCS], (product / ACCS) & 1, abortp)) && ok;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         };
-        auto sums_read = [&](int product) {
+        auto sums_read = [&](int product, int times) {
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             __syncwarp();
-            if (lane == 0) mbar_arrive(&acc_empty[product % ACCS]);
+            if (lane == 0)
+                for (int i = 0; i < times; ++i) mbar_arrive(&acc_empty[product % ACCS]);
         };
         if (by_boxes) {
-            // A thread has a row of a box; four warps have one, the other four the next, and no warp waits for another: each sends its 32 rows off.
-            // 16 bytes of a row lie at their place xor the row's number: no bank conflicts.
-            constexpr int E = 16 / (int)sizeof(O);
-            const int row = q * 32 + lane;
+            // A thread has a row of a box; four warps have one, the next four the next, and no warp waits for another: each sends its 32 rows off.
+            // 16 bytes of a row lie at their place xor the row's number: no bank conflicts.  A part has one box of a tile at most.
+            constexpr int E = 16 / (int)sizeof(O), COLS = BOX_COLS / 2;
+            static_assert(PER_TILE <= PARTS && PARTS % PER_TILE == 0, "a part's boxes are of different tiles");
+            const int row = q * 32 + lane, steps = PER_TILE * (j1 - j0);
             int which = -1;                   // the row's adapter among the tile's
             for (int p = 0; p < passes; ++p)
                 if (own[row] == list[p]) which = p;
-            int last = -1;                    // the box of this warp's last store
 #pragma unroll 1
-            for (int t = 0; t < j1 - j0; ++t) {
+            for (int step = part; step < steps; step += PARTS) {
+                const int t = step / PER_TILE, in = step % PER_TILE, s = step % depth;
                 for (int p = 0; p < passes; ++p) wait_for_sums(t * passes + p);
-#pragma unroll 1
-                for (int in = part; in < PER_TILE; in += 2) {
-                    const int step = t * PER_TILE + in, s = step % depth;
-                    float v[BOX_COLS];
-#pragma unroll
-                    for (int c = 0; c < BOX_COLS; ++c) v[c] = 0.f;
-                    if (ok)
-#pragma unroll 1
-                        for (int p = 0; p < passes; ++p) {
-                            float w[BOX_COLS];
-                            tmem_load<BOX_COLS>(tmem + ((uint32_t)(q * 32) << 16) + (t * passes + p) % ACCS * TILE + in * BOX_COLS, w);
-#pragma unroll
-                            for (int c = 0; c < BOX_COLS; ++c) v[c] = which == p ? w[c] : v[c];
-                        }
-                    if (in + 2 >= PER_TILE)
-                        for (int p = 0; p < passes; ++p) sums_read(t * passes + p);
-                    if (base) {
-                        ok = __all_sync(0xffffffffu, mbar_wait(&box_full[s], (step / depth) & 1, abortp)) && ok;
-                    } else if (step >= depth) {                    // the stores that had this box's memory have read it
-                        ok = __all_sync(0xffffffffu, mbar_wait(&box_empty[s], (step / depth - 1) & 1, abortp)) && ok;
-                    }
-                    if (ok)
-#pragma unroll
-                        for (int c = 0; c < 8; ++c) {
-                            O* at = reinterpret_cast<O*>(box + s * BLOCK_BYTES + row * 128 + ((c ^ (row & 7)) * 16));
-                            __align__(16) O w[E];
-                            if (base) *reinterpret_cast<uint4*>(w) = *reinterpret_cast<uint4*>(at);
-#pragma unroll
-                            for (int e = 0; e < E; ++e) w[e] = from_float<O>(base ? to_float(w[e]) + v[c * E + e] : v[c * E + e]);
-                            *reinterpret_cast<uint4*>(at) = *reinterpret_cast<uint4*>(w);
-                        }
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                    __syncwarp();
-                    if (lane == 0) {
-                        const int c = j0 * TILE + step * BOX_COLS;
-                        if (ok && c < n_end - n_first && t0 + q * 32 < tokens)
-                            tma_store_2d(&boxes.out[g], box + s * BLOCK_BYTES + q * 32 * 128, c, t0 + q * 32);
-                        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-                        // this warp's store before this one has read its rows
-                        asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
-                        if (last >= 0) mbar_arrive(&box_empty[last]);
-                        last = s;
-                    }
+                if (base) {
+                    ok = __all_sync(0xffffffffu, mbar_wait(&box_full[s], (step / depth) & 1, abortp)) && ok;
+                } else if (step >= depth) {                        // the stores that had this box's memory have read it
+                    ok = __all_sync(0xffffffffu, mbar_wait(&box_empty[s], (step / depth - 1) & 1, abortp)) && ok;
                 }
+                if (ok)
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+                        float v[COLS];
+                        const uint32_t from = tmem + ((uint32_t)(q * 32) << 16) + in * BOX_COLS + half * COLS;
+                        if (passes == 1) {
+                            tmem_load_wide(from + t % ACCS * TILE, v);
+                            if (which < 0)
+#pragma unroll
+                                for (int c = 0; c < COLS; ++c) v[c] = 0.f;
+                        } else {
+#pragma unroll
+                            for (int c = 0; c < COLS; ++c) v[c] = 0.f;
+#pragma unroll 1
+                            for (int p = 0; p < passes; ++p) {
+                                float w[COLS];
+                                tmem_load_wide(from + (t * passes + p) % ACCS * TILE, w);
+#pragma unroll
+                                for (int c = 0; c < COLS; ++c) v[c] = which == p ? w[c] : v[c];
+                            }
+                        }
+                        if (half == 1)
+                            for (int p = 0; p < passes; ++p) sums_read(t * passes + p, 1);
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) {
+                            uint4* at = reinterpret_cast<uint4*>(box + s * BLOCK_BYTES + row * 128 + (((half * 4 + c) ^ (row & 7)) * 16));
+                            *at = plus(base ? *at : make_uint4(0, 0, 0, 0), v + c * E, O());
+                        }
+                    }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) {
+                    const int c = j0 * TILE + step * BOX_COLS;
+                    if (ok && c < n_end - n_first && t0 + q * 32 < tokens) tma_store_2d(&boxes.out[g], box + s * BLOCK_BYTES + q * 32 * 128, c, t0 + q * 32);
+                    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+                    asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+                    mbar_arrive(&box_empty[s]);
+                }
+                __syncwarp();
             }
             if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
-        } else {
+        } else if (warp < 2 + EPI_WARPS) {
+            int i = 0;
             for (int p = 0; p < passes; ++p) {
                 const int l = list[p];
                 // Steps of 64 columns.  What a step adds to is asked for a step ahead: eight columns of four rows a thread.
@@ -457,7 +492,7 @@ low_rank_result_kernel(const __grid_constant__ CUtensorMap map_h, const __grid_c
 #pragma unroll
                         for (int e = 0; e < 32; e += 4) *reinterpret_cast<float4*>(row + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
                     }
-                    if (half == 1) sums_read(i++);
+                    if (half == 1) sums_read(i++, min(PARTS, PER_TILE) * 4 / EPI_WARPS);
                     epilogue_barrier();
                     if (ok && c < wide) {
                         const bool whole = aligned && n0 % 8 == 0 && c + 8 <= wide;
@@ -557,10 +592,11 @@ int launch_results(const void* hidden, const CUtensorMap& map_b, const int* ids,
     const int aligned = reinterpret_cast<uintptr_t>(out) % 16 == 0 && reinterpret_cast<uintptr_t>(base) % 16 == 0 &&
                         (T == 1 || (ldo % 8 == 0 && (base == nullptr || ldb % 8 == 0)));
     const int depth = kblocks == 1 ? MOST_BOXES : 4;
-    const size_t smem = 1024 + (size_t)((2 + B_STAGES) * kblocks + depth) * BLOCK_BYTES;
+    const int stages = kblocks == 1 ? MOST_STAGES : 2;
+    const size_t smem = 1024 + (size_t)((2 + stages) * kblocks + depth) * BLOCK_BYTES;
     prism::open_smem(low_rank_result_kernel<O>, smem);
     return (int)prism::launch_kernel(low_rank_result_kernel<O>, dim3(s.units[G], tiles), dim3(RESULT_THREADS), smem, stream, map_h, map_b, boxes, ids, (const O*)base,
-                                     ldb, (O*)out, ldo, by_box, depth, aligned, T, r, N, L, s, err);
+                                     ldb, (O*)out, ldo, by_box, depth, stages, aligned, T, r, N, L, s, err);
 }
 
 }  // namespace lowrank
