@@ -19,7 +19,6 @@
 namespace prism {
 namespace lowrank {
 
-constexpr int THREADS = 512, WARPS = THREADS / 32;
 constexpr int CTAS = 8;                       // of a cluster
 constexpr int AHEAD = 4;                      // 16-byte loads of B in flight a thread
 constexpr int MOST_RANK = 128, MOST_SLICES = 8;
@@ -69,14 +68,15 @@ __device__ __forceinline__ uint32_t rank_in_cluster() {
 
 // ---- one token ----------------------------------------------------------------------------------------------
 
-template <typename T, typename O>
-__global__ void __launch_bounds__(THREADS, 2)
+// THREADS: 512, or 256 where there are CTAs enough to fill the SMs all the same: their waits then overlap more finely
+template <typename T, typename O, int THREADS>
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS)
 low_rank_token_kernel(const T* __restrict__ x_, long long ldx, int x_whole, const T* __restrict__ a, const T* __restrict__ b,
                       const float* __restrict__ scale, const int* __restrict__ ids_, const O* __restrict__ base_, long long ldb, O* out_, long long ldo,
                       int K, int Kp, int r, int L, Slices slices, int parts, int* err) {
-    constexpr int E = Chunk<T>::E;
+    constexpr int E = Chunk<T>::E, WARPS = THREADS / 32;
     __shared__ float hidden[MOST_RANK];
-    __shared__ float partial[WARPS];
+    __shared__ float partial[MOST_RANK / CTAS][WARPS];             // a hidden value's share of a warp
     asm volatile("barrier.cluster.arrive.aligned;" ::: "memory");              // here: peers may write into this CTA's memory
     pdl_trigger();
     pdl_wait();
@@ -114,10 +114,10 @@ low_rank_token_kernel(const T* __restrict__ x_, long long ldx, int x_whole, cons
     const int rows = r / CTAS;
     int split = 1;
     while (split * 2 * rows <= WARPS) split *= 2;
-    const int sub = warp % split, j = warp / split;                // r / 8 is at most 16: a row a warp at least
-    float s = 0.f;
-    if (j < rows) {
+    const int sub = warp % split;
+    for (int j = warp / split; j < rows; j += WARPS / split) {
         const T* row = a + (((size_t)l * slices.n + g) * r + me * rows + j) * Kp;
+        float s = 0.f;
 #pragma unroll 4
         for (int k = (sub * 32 + lane) * E; k < K; k += split * 32 * E) {
             float w[E], v[E];
@@ -131,15 +131,15 @@ low_rank_token_kernel(const T* __restrict__ x_, long long ldx, int x_whole, cons
 #pragma unroll
             for (int e = 0; e < E; ++e) s = fmaf(v[e], w[e], s);
         }
+        s = warp_sum(s);
+        if (lane == 0) partial[j][sub] = s;
     }
-    s = warp_sum(s);
-    if (lane == 0) partial[warp] = s;
     __syncthreads();
     asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
     if (tid < rows * CTAS) {                                       // a hidden value, for one of the CTAs
         const int c = tid % CTAS, q = tid / CTAS;
         float h = 0.f;
-        for (int w = 0; w < split; ++w) h += partial[q * split + w];
+        for (int w = 0; w < split; ++w) h += partial[q][w];
         asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(peer(&hidden[me * rows + q], c)), "f"(h * scale[l]) : "memory");
     }
     __syncwarp();
@@ -176,12 +176,13 @@ int launch_tokens(const void* x, long long ldx, const void* a, const void* b, co
     // more than four an SM
     int widest = 0;
     for (int g = 0; g < s.n; ++g) widest = max(widest, s.first[g + 1] - s.first[g]);
-    const long long bytes = (long long)widest * r * (int)sizeof(T), ahead = (long long)CTAS * THREADS * AHEAD * 16;
+    const long long bytes = (long long)widest * r * (int)sizeof(T), ahead = (long long)CTAS * 512 * AHEAD * 16;
     const int parts = (int)max(1ll, min((bytes + ahead - 1) / ahead, 4ll * sms / ((long long)CTAS * s.n * tokens)));
     const int whole = (reinterpret_cast<uintptr_t>(x) % 16 == 0) && (ldx * (long long)sizeof(T) % 16 == 0 || tokens == 1);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(CTAS, s.n * parts, tokens);
-    cfg.blockDim = dim3(THREADS);
+    const bool many = (long long)CTAS * s.n * parts * tokens > 2ll * sms;
+    cfg.blockDim = dim3(many ? 256 : 512);
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -190,7 +191,8 @@ int launch_tokens(const void* x, long long ldx, const void* a, const void* b, co
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = prism::pdl_enabled() ? 2 : 1;
-    return (int)cudaLaunchKernelEx(&cfg, low_rank_token_kernel<T, O>, (const T*)x, ldx, whole, (const T*)a, (const T*)b, scale, ids, (const O*)base, ldb, (O*)out,
+    const auto kernel = many ? low_rank_token_kernel<T, O, 256> : low_rank_token_kernel<T, O, 512>;
+    return (int)cudaLaunchKernelEx(&cfg, kernel, (const T*)x, ldx, whole, (const T*)a, (const T*)b, scale, ids, (const O*)base, ldb, (O*)out,
                                    ldo, K, Kp, r, L, s, parts, err);
 }
 

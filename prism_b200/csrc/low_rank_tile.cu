@@ -14,7 +14,7 @@
 #include "vec.cuh"
 
 namespace prism {
-namespace lowrank {
+namespace lowrank_tile {
 
 using namespace prism::tc;
 constexpr int TILE = 128;                     // tokens of a tile, and columns of one of B
@@ -599,12 +599,12 @@ int launch_results(const void* hidden, const CUtensorMap& map_b, const int* ids,
                                      ldb, (O*)out, ldo, by_box, depth, stages, aligned, T, r, N, L, s, err);
 }
 
-}  // namespace lowrank
+}  // namespace lowrank_tile
 }  // namespace prism
 
 // Whether the tiles take these sizes: x rows that TMA can read, hidden values of all slices in tensor memory.
 PRISM_EXPORT int prism_low_rank_tile_supported(int K, int r, int G, int x_aligned) {
-    using namespace prism::lowrank;
+    using namespace prism::lowrank_tile;
     return x_aligned && K >= 1 && r >= 16 && r % 16 == 0 && r <= MOST_RANK && G >= 1 && G <= MOST_SLICES && G * r <= MOST_HIDDEN;
 }
 
@@ -612,7 +612,7 @@ PRISM_EXPORT int prism_low_rank_tile_supported(int K, int r, int G, int x_aligne
 PRISM_EXPORT int prism_low_rank_tile(const void* x, long long ldx, const void* a, const void* b, const float* scale, const int* ids, const void* base,
                                      long long ldb, void* out, long long ldo, int out_dtype, int T, int K, int Kp, int r, int L, int G, const int* first,
                                      void* hidden, int sms, int* err, cudaStream_t stream) {
-    using namespace prism::lowrank;
+    using namespace prism::lowrank_tile;
     typedef __nv_bfloat16 bf16;
     if (T <= 0) return 0;
     const bool x_aligned = reinterpret_cast<uintptr_t>(x) % 16 == 0 && (ldx % 8 == 0 || T == 1);
