@@ -60,6 +60,12 @@ __device__ __forceinline__ void prefetch_map(const CUtensorMap* map) { asm volat
 __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(bar)) : "memory");
 }
+// After a wait that ran out: whether a copy that is on its way has landed, with a limit of its own (the flag that ends the others is set).  The CTA's
+// shared memory is another one's when it leaves.
+__device__ __forceinline__ void drain(uint64_t* bar, uint32_t parity) {
+    const unsigned long long t0 = globaltimer();
+    while (!mbar_try_wait(bar, parity) && (long long)(globaltimer() - t0) < 200000000ll) {}
+}
 __device__ __forceinline__ uint32_t instruction(int n) {
     return (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(TILE >> 4) << 24);
 }
@@ -108,7 +114,7 @@ low_rank_hidden_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_c
     for (int p = 0; p < passes; ++p) {
         const int l = list[p];
         if (warp == 0) {
-            if (lane == 0) {
+            if (lane == 0 && !*abortp) {
                 int issued = 0;
                 for (int i = 0; i < mine; ++i) {
                     const int s = (it + i) % stages, round = (it + i) / stages;
@@ -121,13 +127,13 @@ low_rank_hidden_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_c
                         tma_load_2d(st + BLOCK_BYTES + (size_t)g * r * TILE_K * 2, &map_a, &full[s], k, (l * G + g) * r);
                     issued = i + 1;
                 }
-                if (*abortp)                  // copies in flight get a bounded chance to land before the memory is used otherwise
-                    for (int i = max(0, issued - stages); i < issued; ++i) mbar_wait(&full[(it + i) % stages], ((it + i) / stages) & 1, abortp);
+                if (*abortp)
+                    for (int i = max(0, issued - stages); i < issued; ++i) drain(&full[(it + i) % stages], ((it + i) / stages) & 1);
             }
         } else if (warp == 1) {
             if (lane == 0) {
                 const uint32_t idesc = instruction(r);
-                bool ok = true;
+                bool ok = !*abortp;
                 for (int i = 0; i < mine && ok; ++i) {
                     const int s = (it + i) % stages;
                     ok = mbar_wait(&full[s], ((it + i) / stages) & 1, abortp);
@@ -144,7 +150,10 @@ low_rank_hidden_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_c
                     }
                     umma_commit(&empty[s]);
                 }
-                umma_commit(&done);
+                if (mine > 0) {
+                    umma_commit(&done);
+                    if (*abortp) drain(&done, p & 1);          // products on their way read shared memory and write tensor memory
+                }
             }
         }
         __syncwarp();
@@ -241,8 +250,14 @@ __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, const void*
     asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(map), "r"(smem_addr(src)), "r"(c0), "r"(c1) : "memory");
 }
 
-constexpr int MOST_STAGES = 4, MOST_BOXES = 6, ACCS = 4;           // ACCS: accumulators, all of tensor memory
+constexpr int MOST_STAGES = 4, ACCS = 4;                          // ACCS: accumulators, all of tensor memory
 constexpr int PARTS = 4;                                          // groups of four warps that each have a box
+// A wait knows a barrier's phase by one bit, so who waits on a barrier has to wait for each of its phases.  Parts take boxes in turn and tiles of
+// columns in turn: a box's memory is always the same part's (the boxes there is memory for are a multiple of the parts), and a product's barrier
+// is its tile's of the next four (one that a tile later comes back to has been seen: it takes ACCS products more at least).  With six boxes a
+// part met a box's third use while the second, another part's, was still on its way, and took it for its own.
+constexpr int MOST_BOXES = 8, TILE_TURNS = 4;
+static_assert(MOST_BOXES % PARTS == 0 && TILE_TURNS % PARTS == 0 && TILE_TURNS >= ACCS, "see above");
 constexpr int RESULT_THREADS = 64 + PARTS * 128 + 32;             // and one more warp, that asks for boxes
 
 // 32 columns of a warp's lanes in one load
@@ -291,7 +306,7 @@ low_rank_result_kernel(const __grid_constant__ CUtensorMap map_h, const __grid_c
     unsigned char* ring = smem + 2 * kblocks * BLOCK_BYTES;
     unsigned char* box = ring + stages * kblocks * BLOCK_BYTES;
     float* sums = reinterpret_cast<float*>(box);                                       // where no boxes are used
-    __shared__ uint64_t full[MOST_STAGES], empty[MOST_STAGES], acc_full[ACCS], acc_empty[ACCS], h_full, box_full[MOST_BOXES], box_empty[MOST_BOXES];
+    __shared__ uint64_t full[MOST_STAGES], empty[MOST_STAGES], acc_full[TILE_TURNS * ACCS], acc_empty[ACCS], h_full, last, box_full[MOST_BOXES], box_empty[MOST_BOXES];
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_flag, own[TILE], list[TILE], count;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, t0 = blockIdx.y * TILE;
@@ -307,9 +322,10 @@ low_rank_result_kernel(const __grid_constant__ CUtensorMap map_h, const __grid_c
         prefetch_map(&map_h), prefetch_map(&map_b), prefetch_map(&boxes.base[g]), prefetch_map(&boxes.out[g]);
         abort_flag = 0;
         for (int s = 0; s < MOST_STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
-        for (int s = 0; s < ACCS; ++s) { mbar_init(&acc_full[s], 1); mbar_init(&acc_empty[s], 4 * min(PARTS, PER_TILE)); }
+        for (int s = 0; s < ACCS; ++s) mbar_init(&acc_empty[s], 4 * min(PARTS, PER_TILE));
+        for (int s = 0; s < TILE_TURNS * ACCS; ++s) mbar_init(&acc_full[s], 1);
         for (int s = 0; s < MOST_BOXES; ++s) { mbar_init(&box_full[s], 1); mbar_init(&box_empty[s], 4); }
-        mbar_init(&h_full, 1);
+        mbar_init(&h_full, 1), mbar_init(&last, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     pdl_wait();
@@ -330,6 +346,8 @@ low_rank_result_kernel(const __grid_constant__ CUtensorMap map_h, const __grid_c
     // products are numbered: tile by tile and in it adapter by adapter, or adapter by adapter
     const int products = passes * (j1 - j0);
     auto adapter_of_product = [&](int i) { return list[by_boxes ? i % passes : i / (j1 - j0)]; };
+    auto barrier_of_product = [&](int i) { return by_boxes ? i / passes % TILE_TURNS * ACCS + i % passes : i % ACCS; };
+    auto phase_of_product = [&](int i) { return (by_boxes ? i / passes / TILE_TURNS : i / ACCS) & 1; };
     auto tile_of_product = [&](int i) { return j0 + (by_boxes ? i / passes : i % (j1 - j0)); };
 
     if (warp == 0) {
@@ -347,9 +365,9 @@ low_rank_result_kernel(const __grid_constant__ CUtensorMap map_h, const __grid_c
                 for (int k = 0; k < kblocks; ++k)
                     tma_load_2d(ring + (s * kblocks + k) * BLOCK_BYTES, &map_b, &full[s], k * TILE_K, adapter_of_product(i) * N + n_first + tile_of_product(i) * TILE);
             }
-            if (*abortp) {                    // copies in flight get a bounded chance to land
-                mbar_wait(&h_full, 0, abortp);
-                for (int k = max(0, i - stages); k < i; ++k) mbar_wait(&full[k % stages], (k / stages) & 1, abortp);
+            if (*abortp) {
+                drain(&h_full, 0);
+                for (int k = max(0, i - stages); k < i; ++k) drain(&full[k % stages], (k / stages) & 1);
             }
         }
     } else if (warp == 1) {
@@ -371,7 +389,11 @@ low_rank_result_kernel(const __grid_constant__ CUtensorMap map_h, const __grid_c
                     umma_bf16(d, dl, db, idesc, 1u);
                 }
                 umma_commit(&empty[s]);
-                umma_commit(&acc_full[acc]);
+                umma_commit(&acc_full[barrier_of_product(i)]);
+            }
+            if (*abortp) {                    // products on their way read shared memory and write tensor memory
+                umma_commit(&last);
+                drain(&last, 0);
             }
         }
     } else if (warp == RESULT_THREADS / 32 - 1) {
@@ -385,14 +407,14 @@ low_rank_result_kernel(const __grid_constant__ CUtensorMap map_h, const __grid_c
                 tma_load_2d(box + s * BLOCK_BYTES, &boxes.base[g], &box_full[s], j0 * TILE + i * BOX_COLS, t0);
             }
             if (*abortp)
-                for (int k = max(0, i - depth); k < i; ++k) mbar_wait(&box_full[k % depth], (k / depth) & 1, abortp);
+                for (int k = max(0, i - depth); k < i; ++k) drain(&box_full[k % depth], (k / depth) & 1);
         }
     } else {
         // after a wait that ran out the loops go on, as the barriers of these threads count on all of them, but touch nothing
         const int tid = threadIdx.x - 64, q = warp & 3, part = (warp - 2) >> 2;
         bool ok = true;
         auto wait_for_sums = [&](int product) {
-            ok = __all_sync(0xffffffffu, mbar_wait(&acc_full[product % ACCS], (product / ACCS) & 1, abortp)) && ok;
+            ok = __all_sync(0xffffffffu, mbar_wait(&acc_full[barrier_of_product(product)], phase_of_product(product), abortp)) && ok;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         };
         auto sums_read = [&](int product, int times) {
@@ -538,6 +560,7 @@ low_rank_result_kernel(const __grid_constant__ CUtensorMap map_h, const __grid_c
             }
         }
     }
+    __syncwarp();                             // a warp whose first thread worked alone is whole again: what follows is for whole warps
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -591,8 +614,7 @@ int launch_results(const void* hidden, const CUtensorMap& map_b, const int* ids,
     }
     const int aligned = reinterpret_cast<uintptr_t>(out) % 16 == 0 && reinterpret_cast<uintptr_t>(base) % 16 == 0 &&
                         (T == 1 || (ldo % 8 == 0 && (base == nullptr || ldb % 8 == 0)));
-    const int depth = kblocks == 1 ? MOST_BOXES : 4;
-    const int stages = kblocks == 1 ? MOST_STAGES : 2;
+    const int depth = kblocks == 1 ? MOST_BOXES : PARTS, stages = 2;
     const size_t smem = 1024 + (size_t)((2 + stages) * kblocks + depth) * BLOCK_BYTES;
     prism::open_smem(low_rank_result_kernel<O>, smem);
     return (int)prism::launch_kernel(low_rank_result_kernel<O>, dim3(s.units[G], tiles), dim3(RESULT_THREADS), smem, stream, map_h, map_b, boxes, ids, (const O*)base,

@@ -49,7 +49,7 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volati
         for (int i = 0; i < 64; ++i)
             if (mbar_try_wait(bar, parity)) return true;
         if (*abort_flag) return false;
-        if (globaltimer() - t0 > WAIT_LIMIT_NS) {
+        if ((long long)(globaltimer() - t0) > (long long)WAIT_LIMIT_NS) {      // signed: the clock may be set back a little meanwhile
             *abort_flag = 1;
             return false;
         }

@@ -226,3 +226,33 @@ def test_stack_and_its_refusals():
         with pytest.raises(E):
             ops.low_rank(**dict(dict(x=x, low=low, ids=ids, base=base), **change))
     assert ops.low_rank(x[:0], low, ids[:0], base[:0]).shape == (0, 96)
+
+
+@pytest.mark.parametrize("ids", [(-1,), (0,), (0, 1, 2, 3), (0, -1, 2)], ids=str)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=str)
+def test_calls_queued_behind_each_other(ids, dtype):
+    """Many calls in flight, with wide rows: every box of the shared result passes through shared memory often, in no fixed order of arrival.  The
+    results of all of them are the first one's, bit by bit, as nothing in a sum depends on time."""
+    from prism_b200 import ops
+    T, K, n, r = 1024, 64, 37888, 16
+    g = torch.Generator(device="cuda").manual_seed(7)
+    a = torch.randn(4, 1, r, K, generator=g, device="cuda").bfloat16()
+    b = torch.randn(4, n, r, generator=g, device="cuda").bfloat16()
+    low = ops.LowRank(a, b, torch.ones(4, device="cuda"), rows=(n,))
+    x = torch.randn(T, K, generator=g, device="cuda").bfloat16()
+    base = torch.randn(T, n, generator=g, device="cuda").to(dtype)
+    at = torch.tensor(ids, dtype=torch.int32, device="cuda").repeat(T)[:T].contiguous()
+    want = ops.low_rank(x, low, at, base=base, singles=0)
+    torch.cuda.synchronize()
+    none = at < 0
+    assert torch.equal(want[none], base[none])
+    wrong = torch.zeros((), dtype=torch.int64, device="cuda")
+    outs = [torch.empty_like(base) for _ in range(3)]
+    for i in range(60):
+        ops.low_rank(x, low, at, base=base, out=outs[i % 3], singles=0)
+        if i % 3 == 2:
+            for o in outs:
+                wrong += (o != want).sum()
+                o.fill_(float("nan"))
+    assert int(wrong) == 0
+    ops.check_tc_errors()
