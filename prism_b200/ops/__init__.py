@@ -198,7 +198,7 @@ launch_count = 0      # kernels of this library launched (or captured) by this p
 
 def _here(t: torch.Tensor, what: str):
     """Launches go to the current device's current stream: a call for another device's tensors is refused."""
-    if t.device.index != torch._C._cuda_getDevice():
+    if t.get_device() != torch._C._cuda_getDevice():
         raise KernelError(f"{what}: tensors on {t.device} while the current device is cuda:{torch._C._cuda_getDevice()}")
 
 
@@ -742,29 +742,28 @@ def sample_filtered(logits: torch.Tensor, temperature: Optional[torch.Tensor], u
     left as they are.  Results by row of ``logits``: ``out`` (int32); ``kept`` (int32): how many tokens it was drawn from (1 if greedy; 0
     for a row of nothing); ``logprob`` (float32): the logarithm of the probability that the token had among them (0 if greedy, -infinity
     for a row of nothing)."""
-    _cuda(logits, temperature, u, out, top_k, top_p, min_p, rows, kept, logprob)
-    if logits.dim() != 2 or logits.dtype != torch.float32 or (logits.stride(1) != 1 and logits.shape[1] > 1) or logits.shape[1] < 1:
-        raise KernelError(f"sample_filtered: logits are float32 rows side by side in memory, got {tuple(logits.shape)} {logits.dtype}, strides "
-                          f"{logits.stride()}")
-    R, V = logits.shape
-    for name, t, dtype in (("temperature", temperature, torch.float32), ("u", u, torch.float32), ("out", out, torch.int32),
-                           ("top_k", top_k, torch.int32), ("top_p", top_p, torch.float32), ("min_p", min_p, torch.float32),
-                           ("kept", kept, torch.int32), ("logprob", logprob, torch.float32), ("rows", rows, torch.int32)):
-        if t is None:
-            if name in ("u", "out"):
-                raise KernelError(f"sample_filtered: no {name}")
-            continue
-        if t.dtype != dtype or not t.is_contiguous() or t.dim() != 1 or (t.shape[0] != R if name != "rows" else t.shape[0] > R) \
-                or t.device != logits.device:
-            raise KernelError(f"sample_filtered: {name} is {dtype} for each of the {R} rows, contiguous, on {logits.device}: got {t.dtype} "
-                              f"{tuple(t.shape)} on {t.device}")
+    d = logits.get_device()
+    shape = logits.shape
+    if d < 0 or len(shape) != 2 or logits.dtype is not torch.float32 or shape[1] < 1 or (logits.stride(1) != 1 and shape[1] > 1):
+        raise KernelError(f"sample_filtered: logits are float32 rows side by side in a CUDA device's memory, got {tuple(shape)} {logits.dtype}, strides "
+                          f"{logits.stride()} on {logits.device}")
+    R, V = shape
+    row, f32, i32 = shape[:1], torch.float32, torch.int32
+    n = R if rows is None else rows.numel()
+    for t, dtype in ((u, f32), (out, i32), (temperature, f32), (top_k, i32), (top_p, f32), (min_p, f32), (kept, i32), (logprob, f32)):
+        if t is not None and (t.dtype is not dtype or t.shape != row or t.get_device() != d or not t.is_contiguous()):
+            raise KernelError(f"sample_filtered: u, temperature, top_p, min_p and logprob are float32, out, top_k and kept int32, one entry for each of the {R} "
+                              f"rows, contiguous on {logits.device}: got {t.dtype} {tuple(t.shape)}, strides {t.stride()} on {t.device}")
+    if u is None or out is None:
+        raise KernelError("sample_filtered: u and out are needed")
+    if rows is not None and (rows.dtype is not i32 or rows.dim() != 1 or n > R or rows.get_device() != d or not rows.is_contiguous()):
+        raise KernelError(f"sample_filtered: rows are int32 numbers of some of the {R} rows, contiguous on {logits.device}: got {rows.dtype} "
+                          f"{tuple(rows.shape)} on {rows.device}")
     _here(logits, "sample_filtered")
-    n = R if rows is None else rows.shape[0]
     if n == 0:
         return
-    _check(lib().prism_sample_filtered(_ptr(logits), logits.stride(0), n, R, V, _ptr(temperature), _ptr(u), _ptr(top_k), _ptr(top_p), _ptr(min_p),
-                                       _ptr(rows), _ptr(out), _ptr(kept), _ptr(logprob), _ptr(_tc_err_word(logits.device)), _stream()),
-           "sample_filtered")
+    _check(lib().prism_sample_filtered(logits.data_ptr(), logits.stride(0), n, R, V, _ptr(temperature), u.data_ptr(), _ptr(top_k), _ptr(top_p), _ptr(min_p),
+                                       _ptr(rows), out.data_ptr(), _ptr(kept), _ptr(logprob), mxfp4._err_word(logits.device), _stream()), "sample_filtered")
 
 
 # --------------------------------------------------------------------------

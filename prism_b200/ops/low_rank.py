@@ -11,6 +11,7 @@ is a model of its own there (engine/weight_manager.py:45).
 from __future__ import annotations
 
 import ctypes
+import itertools
 from typing import Optional, Sequence
 
 import torch
@@ -36,30 +37,32 @@ class LowRank:
     below each other.  ``rows``: how many of the N rows each slice has.  r is a multiple of 16 up to 128, with zeros beyond an adapter's
     own rank; Kp is K rounded up to a multiple of 8 at least, with zeros beyond K.  ``scale``: float32 ``[L]``."""
 
-    __slots__ = ("a", "b", "scale", "rows", "k", "rank", "count", "n", "_first", "_address")
+    __slots__ = ("a", "b", "scale", "rows", "k", "rank", "count", "n", "_first", "_where", "_sizes")
 
     def __init__(self, a: torch.Tensor, b: torch.Tensor, scale: torch.Tensor, rows: Sequence[int], k: Optional[int] = None):
-        rows = tuple(int(n) for n in rows)
-        if a.dim() != 4 or b.dim() != 3 or not rows or min(rows) < 1 or len(rows) > MOST_SLICES:
+        rows = tuple(map(int, rows))
+        sa, sb, dt = a.shape, b.shape, a.dtype
+        if len(sa) != 4 or len(sb) != 3 or not rows or min(rows) < 1 or len(rows) > MOST_SLICES:
             raise ops.KernelError(f"adapters: A is [adapters, slices, rank, width] and B [adapters, rows, rank], of 1 to {MOST_SLICES} slices: got "
-                                  f"{tuple(a.shape)}, {tuple(b.shape)} and rows {rows}")
-        L, G, r, kp = a.shape
-        k = kp if k is None else int(k)
-        if G != len(rows) or b.shape != (L, sum(rows), r) or L < 1:
-            raise ops.KernelError(f"adapters: A {tuple(a.shape)}, B {tuple(b.shape)} and rows {rows} do not belong together")
+                                  f"{tuple(sa)}, {tuple(sb)} and rows {rows}")
+        L, G, r, kp = sa
+        k, n = kp if k is None else int(k), sum(rows)
+        if G != len(rows) or sb != (L, n, r) or L < 1:
+            raise ops.KernelError(f"adapters: A {tuple(sa)}, B {tuple(sb)} and rows {rows} do not belong together")
         if r % RANK_UNIT or not RANK_UNIT <= r <= MOST_RANK or kp % WIDTH_UNIT or not 1 <= k <= kp:
             raise ops.KernelError(f"adapters: a rank in memory is a multiple of {RANK_UNIT} up to {MOST_RANK} and a row of A a multiple of {WIDTH_UNIT} "
                                   f"that holds its {k} entries: got rank {r}, rows of {kp}")
-        if a.dtype not in (torch.bfloat16, torch.float32) or b.dtype != a.dtype or scale.dtype != torch.float32 or scale.shape != (L,):
-            raise ops.KernelError(f"adapters: A and B are both bfloat16 or both float32 and the scales float32 [{L}]: got {a.dtype}, {b.dtype}, "
+        if (dt is not torch.bfloat16 and dt is not torch.float32) or b.dtype is not dt or scale.dtype is not torch.float32 or scale.shape != sa[:1]:
+            raise ops.KernelError(f"adapters: A and B are both bfloat16 or both float32 and the scales float32 [{L}]: got {dt}, {b.dtype}, "
                                   f"{scale.dtype} {tuple(scale.shape)}")
         if not (a.is_contiguous() and b.is_contiguous() and scale.is_contiguous()) or a.data_ptr() % 16 or b.data_ptr() % 16 \
-                or not a.device == b.device == scale.device:
+                or not a.get_device() == b.get_device() == scale.get_device():
             raise ops.KernelError("adapters: A, B and the scales lie contiguous on one device, A and B from a 16-byte border on")
-        self.a, self.b, self.scale, self.rows, self.k, self.rank, self.count, self.n = a, b, scale, rows, k, r, L, sum(rows)
-        first = [sum(rows[:g]) for g in range(G + 1)]
-        self._first = (ctypes.c_int * (G + 1))(*first)
-        self._address = ctypes.addressof(self._first)
+        self.a, self.b, self.scale, self.rows, self.k, self.rank, self.count, self.n = a, b, scale, rows, k, r, L, n
+        self._first = (ctypes.c_int * (G + 1))(0, *itertools.accumulate(rows))
+        # what every call hands over: where A, B and the scales are, and their sizes
+        self._where = (a.data_ptr(), b.data_ptr(), scale.data_ptr())
+        self._sizes = (k, kp, r, L, G, ctypes.addressof(self._first))
 
     @classmethod
     def empty(cls, count: int, rank: int, rows: Sequence[int], k: int, dtype: torch.dtype, device) -> "LowRank":
@@ -144,48 +147,45 @@ def low_rank(x: torch.Tensor, low: LowRank, ids: torch.Tensor, base: Optional[to
     each a request of its own, and the others stand in runs of one adapter (as in a step: decoding requests, then portions of
     prompts); this says how the work is laid out and changes no result's meaning.  An id outside the stack adds nothing and is reported by
     ``check_tc_errors``."""
-    a = low.a
-    if not (x.is_cuda and a.is_cuda and ids.is_cuda and (base is None or base.is_cuda) and (out is None or out.is_cuda)):
-        ops._cuda(x, a, ids, base, out)
-    if x.dim() != 2 or x.shape[1] != low.k or x.dtype is not a.dtype or (x.stride(1) != 1 and low.k > 1):
-        raise ops.KernelError(f"adapters in {a.dtype} for rows of {low.k} side by side in memory: got {tuple(x.shape)} {x.dtype}, strides {x.stride()}")
-    T, N = x.shape[0], low.n
-    if ids.shape != (T,) or ids.dtype is not torch.int32 or not ids.is_contiguous():
-        raise ops.KernelError(f"adapters' numbers are int32 [{T}], contiguous: got {ids.dtype} {tuple(ids.shape)}")
+    d, xs, dt = x.get_device(), x.shape, x.dtype
+    if d < 0 or len(xs) != 2 or xs[1] != low.k or dt is not low.a.dtype or (x.stride(1) != 1 and low.k > 1) or low.a.get_device() != d:
+        raise ops.KernelError(f"adapters in {low.a.dtype} on {low.a.device} for rows of {low.k} side by side in that CUDA device's memory: got {tuple(xs)} "
+                              f"{dt}, strides {x.stride()} on {x.device}")
+    T, N = xs[0], low.n
+    if ids.dtype is not torch.int32 or ids.shape != xs[:1] or ids.get_device() != d or not ids.is_contiguous():
+        raise ops.KernelError(f"adapters' numbers are int32 [{T}], contiguous on {x.device}: got {ids.dtype} {tuple(ids.shape)} on {ids.device}")
     if out is None:
-        out = x.new_empty((T, N), dtype=None if base is None else base.dtype)
-    for t, name in ((base, "base"), (out, "out")):
-        if t is not None and (t.shape != (T, N) or t.dtype not in (torch.bfloat16, torch.float32) or (t.stride(1) != 1 and N > 1)
-                              or (T > 1 and t.stride(0) < N) or t.device != x.device or t.dtype is not out.dtype):
-            raise ops.KernelError(f"{name} of {T} rows and {N} columns, bfloat16 or float32 as the other: got {tuple(t.shape)} {t.dtype}, strides "
-                                  f"{t.stride()} on {t.device}")
-    if a.device != x.device or ids.device != x.device:
-        raise ops.KernelError(f"adapters on {a.device} and their numbers on {ids.device} beside rows on {x.device}")
+        out = torch.empty((T, N), dtype=dt if base is None else base.dtype, device=x.device)
+    odt = out.dtype
+    for t in (out,) if base is None or base is out else (out, base):
+        if t.shape != (T, N) or t.dtype is not odt or (odt is not torch.bfloat16 and odt is not torch.float32) or t.get_device() != d \
+                or (t.stride(1) != 1 and N > 1) or (T > 1 and t.stride(0) < N):
+            raise ops.KernelError(f"base and out are {T} rows of {N} side by side, both bfloat16 or both float32, on {x.device}: got {tuple(t.shape)} {t.dtype}, "
+                                  f"strides {t.stride()} on {t.device}")
     ops._here(x, "low_rank")
     if T == 0:
         return out
     singles = (T if T <= SINGLES else 0) if singles is None else max(0, min(int(singles), T))
-    L = ops.lib()
-    xp, xs, bp, bs, op, os_ = x.data_ptr(), x.stride(0), 0 if base is None else base.data_ptr(), 0 if base is None else base.stride(0), out.data_ptr(), \
-        out.stride(0)
-    what = (low.scale.data_ptr(), ids.data_ptr())
-    sizes = (low.k, a.shape[3], low.rank, low.count, len(low.rows), low._address)
-    sms, err, stream, dt, odt = ops.num_sms(x.device), ops.mxfp4._err_word(x.device), ops._stream(), ops._dt(x), ops._dt(out)
+    L, stream, err = ops.lib(), ops._stream(), ops.mxfp4._err_word(x.device)
+    sms = ops._num_sms.get(d) or ops.num_sms(x.device)
+    (ap, bp, sp), sizes = low._where, low._sizes
+    bf16, out16 = dt is torch.bfloat16, odt is torch.bfloat16
+    xp, x_row, ip, op, o_row = x.data_ptr(), x.stride(0), ids.data_ptr(), out.data_ptr(), out.stride(0)
+    basep, b_row = (None, 0) if base is None else (base.data_ptr(), base.stride(0))
     if singles:
-        ops._check(L.prism_low_rank(xp, xs, dt, a.data_ptr(), low.b.data_ptr(), *what, bp or None, bs, op, os_, odt, singles, *sizes, None, sms, err, stream),
-                   "low_rank")
+        ops._check(L.prism_low_rank(xp, x_row, bf16, ap, bp, sp, ip, basep, b_row, op, o_row, out16, singles, *sizes, None, sms, err, stream), "low_rank")
     rest = T - singles
     if rest == 0:
         return out
     # behind the singles, in tiles
-    size, G = 2 if odt == ops.BF16 else 4, len(low.rows)
-    xp, op, bp = xp + singles * xs * (2 if dt == ops.BF16 else 4), op + singles * os_ * size, bp + singles * bs * size if bp else None
-    args = (low.scale.data_ptr(), ids.data_ptr() + 4 * singles, bp, bs, op, os_, odt, rest, *sizes)
-    if dt == ops.BF16 and rest >= TILE_FROM and L.prism_low_rank_tile_supported(low.k, low.rank, G, xp % 16 == 0 and (xs % 8 == 0 or rest == 1)):
+    size, G = 2 if out16 else 4, len(low.rows)
+    xp, op, basep = xp + singles * x_row * (2 if bf16 else 4), op + singles * o_row * size, basep and basep + singles * b_row * size
+    args = (sp, ip + 4 * singles, basep, b_row, op, o_row, out16, rest, *sizes)
+    if bf16 and rest >= TILE_FROM and L.prism_low_rank_tile_supported(low.k, low.rank, G, xp % 16 == 0 and (x_row % 8 == 0 or rest == 1)):
         hidden = torch.empty(2 * rest * G * low.rank, dtype=torch.bfloat16, device=x.device)
-        ops._check(L.prism_low_rank_tile(xp, xs, a.data_ptr(), low.b.data_ptr(), *args, hidden.data_ptr(), sms, err, stream), "low_rank_tile")
+        ops._check(L.prism_low_rank_tile(xp, x_row, ap, bp, *args, hidden.data_ptr(), sms, err, stream), "low_rank_tile")
     else:
         hidden = torch.empty(rest * G * low.rank, dtype=torch.float32, device=x.device)
-        ops._check(L.prism_low_rank(xp, xs, dt, a.data_ptr(), low.b.data_ptr(), *args, hidden.data_ptr(), sms, err, stream), "low_rank")
+        ops._check(L.prism_low_rank(xp, x_row, bf16, ap, bp, *args, hidden.data_ptr(), sms, err, stream), "low_rank")
     ops.launch_count += 1                    # two kernels
     return out
