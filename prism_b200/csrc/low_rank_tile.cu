@@ -432,6 +432,10 @@ low_rank_result_kernel(const __grid_constant__ CUtensorMap map_h, const __grid_c
             int which = -1;                   // the row's adapter among the tile's
             for (int p = 0; p < passes; ++p)
                 if (own[row] == list[p]) which = p;
+            // of the tile's adapters, those of this warp's rows: a portion's border is seldom among them, so its other products are not loaded
+            const uint32_t present = __reduce_or_sync(0xffffffffu, which < 0 ? 0u : 1u << which);
+            const bool alone = (present & (present - 1)) == 0;
+            const int sole = present ? __ffs(present) - 1 : 0;
 #pragma unroll 1
             for (int step = part; step < steps; step += PARTS) {
                 const int t = step / PER_TILE, in = step % PER_TILE, s = step % depth;
@@ -446,8 +450,8 @@ low_rank_result_kernel(const __grid_constant__ CUtensorMap map_h, const __grid_c
                     for (int half = 0; half < 2; ++half) {
                         float v[COLS];
                         const uint32_t from = tmem + ((uint32_t)(q * 32) << 16) + in * BOX_COLS + half * COLS;
-                        if (passes == 1) {
-                            tmem_load_wide(from + t % ACCS * TILE, v);
+                        if (alone && present) {
+                            tmem_load_wide(from + (t * passes + sole) % ACCS * TILE, v);
                             if (which < 0)
 #pragma unroll
                                 for (int c = 0; c < COLS; ++c) v[c] = 0.f;
@@ -456,6 +460,7 @@ low_rank_result_kernel(const __grid_constant__ CUtensorMap map_h, const __grid_c
                             for (int c = 0; c < COLS; ++c) v[c] = 0.f;
 #pragma unroll 1
                             for (int p = 0; p < passes; ++p) {
+                                if (!(present >> p & 1)) continue;
                                 float w[COLS];
                                 tmem_load_wide(from + (t * passes + p) % ACCS * TILE, w);
 #pragma unroll
@@ -614,7 +619,7 @@ int launch_results(const void* hidden, const CUtensorMap& map_b, const int* ids,
     }
     const int aligned = reinterpret_cast<uintptr_t>(out) % 16 == 0 && reinterpret_cast<uintptr_t>(base) % 16 == 0 &&
                         (T == 1 || (ldo % 8 == 0 && (base == nullptr || ldb % 8 == 0)));
-    const int depth = kblocks == 1 ? MOST_BOXES : PARTS, stages = 2;
+    const int depth = kblocks == 1 ? MOST_BOXES : PARTS, stages = kblocks == 1 ? 3 : 2;
     const size_t smem = 1024 + (size_t)((2 + stages) * kblocks + depth) * BLOCK_BYTES;
     prism::open_smem(low_rank_result_kernel<O>, smem);
     return (int)prism::launch_kernel(low_rank_result_kernel<O>, dim3(s.units[G], tiles), dim3(RESULT_THREADS), smem, stream, map_h, map_b, boxes, ids, (const O*)base,
