@@ -20,7 +20,7 @@ namespace prism {
 namespace lowrank {
 
 constexpr int CTAS = 8;                       // of a cluster
-constexpr int AHEAD = 4;                      // 16-byte loads of B in flight a thread
+constexpr int AHEAD = 2, EACH = 2;            // rows of B in flight a thread, and its 16-byte chunks of each
 constexpr int MOST_RANK = 128, MOST_SLICES = 8;
 
 struct Slices {
@@ -68,9 +68,9 @@ __device__ __forceinline__ uint32_t rank_in_cluster() {
 
 // ---- one token ----------------------------------------------------------------------------------------------
 
-// THREADS: 512, or 256 where there are CTAs enough to fill the SMs all the same: their waits then overlap more finely
+// THREADS: 512 where the CTAs are no more than the SMs, with twice the loads of A in flight; else 256, four CTAs an SM, whose waits overlap
 template <typename T, typename O, int THREADS>
-__global__ void __launch_bounds__(THREADS, 1024 / THREADS)
+__global__ void __launch_bounds__(THREADS, THREADS == 512 ? 1 : 4)
 low_rank_token_kernel(const T* __restrict__ x_, long long ldx, int x_whole, const T* __restrict__ a, const T* __restrict__ b,
                       const float* __restrict__ scale, const int* __restrict__ ids_, const O* __restrict__ base_, long long ldb, O* out_, long long ldo,
                       int K, int Kp, int r, int L, Slices slices, int parts, int* err) {
@@ -95,20 +95,24 @@ low_rank_token_kernel(const T* __restrict__ x_, long long ldx, int x_whole, cons
         asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
         return;
     }
-    // B's chunks: `lanes` neighbours share a row, each with the same part of every row that it meets
+    // B's chunks: `lanes` neighbours share a row, each with the same two parts of every row that it meets
     const int chunks = r / E;
     int lanes = 1;
-    while (lanes < chunks) lanes *= 2;
+    while (lanes * EACH < chunks) lanes *= 2;
     const int chunk = lane % lanes, rows_at_once = THREADS / lanes, row0 = tid / lanes;
-    const bool holds = chunk < chunks;
+    bool holds[EACH];
+#pragma unroll
+    for (int c = 0; c < EACH; ++c) holds[c] = chunk + c * lanes < chunks;
     const T* B = b + ((size_t)l * N + n0) * r + chunk * E;
-    uint4 ahead[AHEAD];
-    float old[AHEAD];
+    uint4 ahead[AHEAD][EACH];
+    O old[AHEAD];                                                  // as they lie in memory: to change their type is to wait for them
 #pragma unroll
     for (int j = 0; j < AHEAD; ++j) {
         const int n = row0 + j * rows_at_once;
-        ahead[j] = holds && n < mine ? __ldg(reinterpret_cast<const uint4*>(B + (size_t)n * r)) : make_uint4(0, 0, 0, 0);
-        old[j] = chunk == 0 && n < mine && base ? to_float(base[n]) : 0.f;
+#pragma unroll
+        for (int c = 0; c < EACH; ++c)
+            ahead[j][c] = holds[c] && n < mine ? __ldg(reinterpret_cast<const uint4*>(B + (size_t)n * r + c * lanes * E)) : make_uint4(0, 0, 0, 0);
+        old[j] = chunk == 0 && n < mine && base ? base[n] : from_float<O>(0.f);
     }
     // an eighth of the hidden values, several warps a row where there are fewer rows than warps
     const int rows = r / CTAS;
@@ -118,8 +122,28 @@ low_rank_token_kernel(const T* __restrict__ x_, long long ldx, int x_whole, cons
     for (int j = warp / split; j < rows; j += WARPS / split) {
         const T* row = a + (((size_t)l * slices.n + g) * r + me * rows + j) * Kp;
         float s = 0.f;
-#pragma unroll 4
-        for (int k = (sub * 32 + lane) * E; k < K; k += split * 32 * E) {
+        int k = (sub * 32 + lane) * E;
+        if (x_whole) {
+            // several chunks of A and x on their way at a time, without a branch between them
+            constexpr int U = THREADS == 512 ? 8 : 2;
+            const int stride = split * 32 * E;
+            for (; k + (U - 1) * stride + E <= K; k += U * stride) {
+                uint4 w[U], v[U];
+#pragma unroll
+                for (int i = 0; i < U; ++i) w[i] = __ldg(reinterpret_cast<const uint4*>(row + k + i * stride));
+#pragma unroll
+                for (int i = 0; i < U; ++i) v[i] = *reinterpret_cast<const uint4*>(x + k + i * stride);
+#pragma unroll
+                for (int i = 0; i < U; ++i) {
+                    float wf[E], vf[E];
+                    Chunk<T>::unpack(w[i], wf), Chunk<T>::unpack(v[i], vf);
+#pragma unroll
+                    for (int e = 0; e < E; ++e) s = fmaf(vf[e], wf[e], s);
+                }
+            }
+        }
+#pragma unroll 2
+        for (; k < K; k += split * 32 * E) {
             float w[E], v[E];
             Chunk<T>::unpack(__ldg(reinterpret_cast<const uint4*>(row + k)), w);
             if (x_whole && k + E <= K) {
@@ -144,25 +168,34 @@ low_rank_token_kernel(const T* __restrict__ x_, long long ldx, int x_whole, cons
     }
     __syncwarp();
     cluster_barrier();
-    float h[E];
+    float h[EACH][E];
 #pragma unroll
-    for (int e = 0; e < E; ++e) h[e] = holds ? hidden[chunk * E + e] : 0.f;
-    for (int m = 0; m < mine; m += AHEAD * rows_at_once) {
+    for (int c = 0; c < EACH; ++c)
 #pragma unroll
-        for (int i = 0; i < AHEAD; ++i) {
+        for (int e = 0; e < E; ++e) h[c][e] = holds[c] ? hidden[(chunk + c * lanes) * E + e] : 0.f;
+    const int pass = AHEAD * rows_at_once;
+    const size_t step = (size_t)rows_at_once * r;
+    const T* next = B + (size_t)(row0 + pass) * r;
+    int n = row0;
+    for (int m = 0; m < mine; m += pass) {
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i, n += rows_at_once, next += step) {
             if (m + i * rows_at_once >= mine) break;
-            const int n = m + i * rows_at_once + row0, next = n + AHEAD * rows_at_once;
-            float w[E], sum = 0.f;
-            const float was = old[i];
-            Chunk<T>::unpack(ahead[i], w);
-            if (next < mine) {
-                if (holds) ahead[i] = __ldg(reinterpret_cast<const uint4*>(B + (size_t)next * r));
-                if (chunk == 0 && base) old[i] = to_float(base[next]);
+            float w[EACH][E], sum = to_float(old[i]);
+#pragma unroll
+            for (int c = 0; c < EACH; ++c) Chunk<T>::unpack(ahead[i][c], w[c]);
+            if (n + pass < mine) {
+#pragma unroll
+                for (int c = 0; c < EACH; ++c)
+                    if (holds[c]) ahead[i][c] = __ldg(reinterpret_cast<const uint4*>(next + c * lanes * E));
+                if (chunk == 0 && base) old[i] = base[n + pass];
             }
 #pragma unroll
-            for (int e = 0; e < E; ++e) sum = fmaf(h[e], w[e], sum);
+            for (int c = 0; c < EACH; ++c)
+#pragma unroll
+                for (int e = 0; e < E; ++e) sum = fmaf(h[c][e], w[c][e], sum);
             for (int o = 1; o < lanes; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-            if (chunk == 0 && n < mine) out[n] = from_float<O>(was + sum);
+            if (chunk == 0 && n < mine) out[n] = from_float<O>(sum);
         }
     }
 }
@@ -172,16 +205,16 @@ int launch_tokens(const void* x, long long ldx, const void* a, const void* b, co
                   long long ldo, int tokens, int K, int Kp, int r, int L, const Slices& s, int* err, int sms, cudaStream_t stream) {
     if (tokens <= 0) return 0;
     if (tokens > 65535) return (int)cudaErrorInvalidValue;
-    // clusters that share a slice's columns: as many as keep B's part of a CTA within what it asks for ahead, while all CTAs together are no
-    // more than four an SM
+    // clusters that share a slice's columns, each with hidden values of its own: as many as keep B's part of a CTA within what it asks for ahead, while
+    // all CTAs together are no more than the SMs
     int widest = 0;
     for (int g = 0; g < s.n; ++g) widest = max(widest, s.first[g + 1] - s.first[g]);
-    const long long bytes = (long long)widest * r * (int)sizeof(T), ahead = (long long)CTAS * 512 * AHEAD * 16;
-    const int parts = (int)max(1ll, min((bytes + ahead - 1) / ahead, 4ll * sms / ((long long)CTAS * s.n * tokens)));
+    const long long bytes = (long long)widest * r * (int)sizeof(T), ahead = (long long)CTAS * 512 * AHEAD * EACH * 16;
+    const int parts = (int)max(1ll, min((bytes + ahead - 1) / ahead, (long long)sms / ((long long)CTAS * s.n * tokens)));
     const int whole = (reinterpret_cast<uintptr_t>(x) % 16 == 0) && (ldx * (long long)sizeof(T) % 16 == 0 || tokens == 1);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(CTAS, s.n * parts, tokens);
-    const bool many = (long long)CTAS * s.n * parts * tokens > 2ll * sms;
+    const bool many = (long long)CTAS * s.n * parts * tokens > sms;
     cfg.blockDim = dim3(many ? 256 : 512);
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
