@@ -250,15 +250,15 @@ __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, const void*
     asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(map), "r"(smem_addr(src)), "r"(c0), "r"(c1) : "memory");
 }
 
-constexpr int MOST_STAGES = 4, ACCS = 4;                          // ACCS: accumulators, all of tensor memory
+constexpr int MOST_STAGES = 7, ACCS = 4;                          // ACCS: accumulators, all of tensor memory
 constexpr int PARTS = 4;                                          // groups of four warps that each have a box
 // A wait knows a barrier's phase by one bit, so who waits on a barrier has to wait for each of its phases.  Parts take boxes in turn and tiles of
 // columns in turn: a box's memory is always the same part's (the boxes there is memory for are a multiple of the parts), and a product's barrier
 // is its tile's of the next four (one that a tile later comes back to has been seen: it takes ACCS products more at least).  With six boxes a
 // part met a box's third use while the second, another part's, was still on its way, and took it for its own.
 constexpr int MOST_BOXES = 8, TILE_TURNS = 4;
-static_assert(MOST_BOXES % PARTS == 0 && TILE_TURNS % PARTS == 0 && TILE_TURNS >= ACCS, "see above");
-constexpr int RESULT_THREADS = 64 + PARTS * 128 + 32;             // and one more warp, that asks for boxes
+static_assert(MOST_BOXES == 8 && PARTS == 4 && TILE_TURNS % PARTS == 0 && TILE_TURNS >= ACCS, "see above");
+constexpr int RESULT_THREADS = 64 + PARTS * 128 + 64;             // and two more warps: one asks for boxes, one sends them off
 
 // 32 columns of a warp's lanes in one load
 __device__ __forceinline__ void tmem_load_wide(uint32_t at, float (&v)[32]) {
@@ -292,11 +292,11 @@ __device__ __forceinline__ uint4 plus(const uint4& old, const float* v, float) {
                       __float_as_uint(__uint_as_float(old.z) + v[2]), __float_as_uint(__uint_as_float(old.w) + v[3]));
 }
 
-// by_box: a bit a slice, whether its columns of base and out can go by TMA; depth, stages: how many boxes and tiles of B there is memory for
+// by_box: a bit a slice, whether its columns of base and out can go by TMA; buffers: of 16 KB there is memory for, beside the hidden values
 template <typename O>
 __global__ void __launch_bounds__(RESULT_THREADS, 1)
 low_rank_result_kernel(const __grid_constant__ CUtensorMap map_h, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ Boxes boxes,
-                       const int* __restrict__ ids_, const O* base, long long ldb, O* out, long long ldo, int by_box, int depth, int stages, int aligned, int tokens, int r, int N,
+                       const int* __restrict__ ids_, const O* base, long long ldb, O* out, long long ldo, int by_box, int buffers, int aligned, int tokens, int r, int N,
                        int L, Tiles tiles, int* err) {
     constexpr int BOX_COLS = 128 / (int)sizeof(O), PER_TILE = TILE / BOX_COLS;         // columns of a box of 128 bytes a row
     extern __shared__ unsigned char raw[];
@@ -304,9 +304,8 @@ low_rank_result_kernel(const __grid_constant__ CUtensorMap map_h, const __grid_c
     const int kblocks = (r + TILE_K - 1) / TILE_K;
     unsigned char* h_hi = smem;                                                        // high terms, then low ones
     unsigned char* ring = smem + 2 * kblocks * BLOCK_BYTES;
-    unsigned char* box = ring + stages * kblocks * BLOCK_BYTES;
-    float* sums = reinterpret_cast<float*>(box);                                       // where no boxes are used
-    __shared__ uint64_t full[MOST_STAGES], empty[MOST_STAGES], acc_full[TILE_TURNS * ACCS], acc_empty[ACCS], h_full, last, box_full[MOST_BOXES], box_empty[MOST_BOXES];
+    __shared__ uint64_t full[MOST_STAGES], empty[MOST_STAGES], acc_full[TILE_TURNS * ACCS], acc_empty[ACCS], h_full, last, box_full[MOST_BOXES],
+        box_done[MOST_BOXES], box_empty[MOST_BOXES];
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_flag, own[TILE], list[TILE], count;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, t0 = blockIdx.y * TILE;
@@ -324,7 +323,7 @@ low_rank_result_kernel(const __grid_constant__ CUtensorMap map_h, const __grid_c
         for (int s = 0; s < MOST_STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
         for (int s = 0; s < ACCS; ++s) mbar_init(&acc_empty[s], 4 * min(PARTS, PER_TILE));
         for (int s = 0; s < TILE_TURNS * ACCS; ++s) mbar_init(&acc_full[s], 1);
-        for (int s = 0; s < MOST_BOXES; ++s) { mbar_init(&box_full[s], 1); mbar_init(&box_empty[s], 4); }
+        for (int s = 0; s < MOST_BOXES; ++s) { mbar_init(&box_full[s], 1); mbar_init(&box_done[s], 4); mbar_init(&box_empty[s], 1); }
         mbar_init(&h_full, 1), mbar_init(&last, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -341,14 +340,25 @@ low_rank_result_kernel(const __grid_constant__ CUtensorMap map_h, const __grid_c
     const int passes = count;
     // Up to ACCS adapters: their products with a tile of columns lie side by side in tensor memory, a thread takes its row's, and the results go by
     // boxes.  Else one adapter after the other.
+    // The memory: twice as many boxes as parts where a tile has one adapter at most, else as many, and the rest for tiles of B, which more adapters
+    // use up faster.
+    const int depth_log = kblocks == 1 && passes <= 1 ? 3 : 2, depth = 1 << depth_log, stages = min(MOST_STAGES, (buffers - depth) / kblocks);
+    unsigned char* box = ring + stages * kblocks * BLOCK_BYTES;
+    float* sums = reinterpret_cast<float*>(box);                                       // where no boxes are used
     const bool nothing = passes == 0 && (const O*)out == base, by_boxes = !nothing && passes <= ACCS && (by_box >> g & 1);
     pdl_trigger();                            // not before this CTA has its tensor memory: the next kernel may take the rest and wait
     // products are numbered: tile by tile and in it adapter by adapter, or adapter by adapter
     const int products = passes * (j1 - j0);
-    auto adapter_of_product = [&](int i) { return list[by_boxes ? i % passes : i / (j1 - j0)]; };
-    auto barrier_of_product = [&](int i) { return by_boxes ? i / passes % TILE_TURNS * ACCS + i % passes : i % ACCS; };
-    auto phase_of_product = [&](int i) { return (by_boxes ? i / passes / TILE_TURNS : i / ACCS) & 1; };
-    auto tile_of_product = [&](int i) { return j0 + (by_boxes ? i / passes : i % (j1 - j0)); };
+    struct Turn {                             // of a product: its tile and its adapter's number among the tile's
+        int tile = 0, adapter = 0;
+        __device__ __forceinline__ void next(bool by_boxes, int tiles, int adapters) {
+            if (by_boxes) {
+                if (++adapter == adapters) adapter = 0, ++tile;
+            } else if (++tile == tiles) {
+                tile = 0, ++adapter;
+            }
+        }
+    };
 
     if (warp == 0) {
         if (lane == 0 && products > 0) {
@@ -357,13 +367,15 @@ low_rank_result_kernel(const __grid_constant__ CUtensorMap map_h, const __grid_c
             for (int term = 0; term < 2; ++term)
                 for (int k = 0; k < kblocks; ++k)
                     tma_load_2d(h_hi + (term * kblocks + k) * BLOCK_BYTES, &map_h, &h_full, (term * tiles.n + g) * r + k * TILE_K, t0);
-            int i = 0;
+            Turn turn;
+            int i = 0, s = 0, round = 0;
             for (; i < products; ++i) {
-                const int s = i % stages;
-                if (i >= stages && !mbar_wait(&empty[s], (i / stages - 1) & 1, abortp)) break;
+                if (round > 0 && !mbar_wait(&empty[s], (round - 1) & 1, abortp)) break;
                 mbar_expect_tx(&full[s], kblocks * BLOCK_BYTES);
                 for (int k = 0; k < kblocks; ++k)
-                    tma_load_2d(ring + (s * kblocks + k) * BLOCK_BYTES, &map_b, &full[s], k * TILE_K, adapter_of_product(i) * N + n_first + tile_of_product(i) * TILE);
+                    tma_load_2d(ring + (s * kblocks + k) * BLOCK_BYTES, &map_b, &full[s], k * TILE_K, list[turn.adapter] * N + n_first + (j0 + turn.tile) * TILE);
+                turn.next(by_boxes, j1 - j0, passes);
+                if (++s == stages) s = 0, ++round;
             }
             if (*abortp) {
                 drain(&h_full, 0);
@@ -373,48 +385,73 @@ low_rank_result_kernel(const __grid_constant__ CUtensorMap map_h, const __grid_c
     } else if (warp == 1) {
         if (lane == 0 && products > 0) {
             const uint32_t idesc = instruction(TILE);
+            // one thread's instructions between products are time that the tensor cores stand still: descriptors differ by addresses in 16 bytes
+            const uint64_t dh = umma_desc(smem_addr(h_hi)), db0 = umma_desc(smem_addr(ring));
+            constexpr uint64_t BLOCK = BLOCK_BYTES >> 4, STEP = UMMA_K * 2 >> 4;
+            Turn turn;
             bool ok = mbar_wait(&h_full, 0, abortp);
+            int s = 0, round = 0;
             for (int i = 0; i < products && ok; ++i) {
-                const int s = i % stages, acc = i % ACCS;
-                ok = mbar_wait(&full[s], (i / stages) & 1, abortp) && (i < ACCS || mbar_wait(&acc_empty[acc], (i / ACCS - 1) & 1, abortp));
+                const int acc = i % ACCS;
+                ok = mbar_wait(&full[s], round & 1, abortp) && (i < ACCS || mbar_wait(&acc_empty[acc], (i / ACCS - 1) & 1, abortp));
                 if (!ok) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const uint32_t d = tmem + acc * TILE;
-                for (int k = 0; k < r / UMMA_K; ++k) {
-                    const int block = k / 4, in = k % 4;
-                    const uint64_t db = umma_desc(smem_addr(ring + (s * kblocks + block) * BLOCK_BYTES)) + (uint64_t)(in * UMMA_K * 2 >> 4);
-                    const uint64_t dh = umma_desc(smem_addr(h_hi + block * BLOCK_BYTES)) + (uint64_t)(in * UMMA_K * 2 >> 4);
-                    const uint64_t dl = umma_desc(smem_addr(h_hi + (kblocks + block) * BLOCK_BYTES)) + (uint64_t)(in * UMMA_K * 2 >> 4);
-                    umma_bf16(d, dh, db, idesc, k > 0 ? 1u : 0u);
-                    umma_bf16(d, dl, db, idesc, 1u);
+                const uint64_t db = db0 + s * kblocks * BLOCK;
+                for (int block = 0; block < kblocks; ++block) {
+                    const int steps = min(r - block * TILE_K, TILE_K) / UMMA_K;
+#pragma unroll
+                    for (int k = 0; k < TILE_K / UMMA_K; ++k)
+                        if (k < steps) {
+                            umma_bf16(d, dh + block * BLOCK + k * STEP, db + block * BLOCK + k * STEP, idesc, block + k > 0 ? 1u : 0u);
+                            umma_bf16(d, dh + (kblocks + block) * BLOCK + k * STEP, db + block * BLOCK + k * STEP, idesc, 1u);
+                        }
                 }
                 umma_commit(&empty[s]);
-                umma_commit(&acc_full[barrier_of_product(i)]);
+                umma_commit(&acc_full[by_boxes ? turn.tile % TILE_TURNS * ACCS + turn.adapter : acc]);
+                turn.next(by_boxes, j1 - j0, passes);
+                if (++s == stages) s = 0, ++round;
             }
             if (*abortp) {                    // products on their way read shared memory and write tensor memory
                 umma_commit(&last);
                 drain(&last, 0);
             }
         }
-    } else if (warp == RESULT_THREADS / 32 - 1) {
+    } else if (warp == RESULT_THREADS / 32 - 2) {
         if (lane == 0 && by_boxes && base) {
             const int steps = PER_TILE * (j1 - j0);
             int i = 0;
             for (; i < steps; ++i) {
-                const int s = i % depth;
-                if (i >= depth && !mbar_wait(&box_empty[s], (i / depth - 1) & 1, abortp)) break;
+                const int s = i & depth - 1;
+                if (i >= depth && !mbar_wait(&box_empty[s], (i >> depth_log) - 1 & 1, abortp)) break;
                 mbar_expect_tx(&box_full[s], BLOCK_BYTES);
                 tma_load_2d(box + s * BLOCK_BYTES, &boxes.base[g], &box_full[s], j0 * TILE + i * BOX_COLS, t0);
             }
             if (*abortp)
-                for (int k = max(0, i - depth); k < i; ++k) drain(&box_full[k % depth], (k / depth) & 1);
+                for (int k = max(0, i - depth); k < i; ++k) drain(&box_full[k & depth - 1], k >> depth_log & 1);
+        }
+    } else if (warp == RESULT_THREADS / 32 - 1) {
+        // sends boxes off; a box's memory is free when the store after it is on its way and its own has read it
+        if (lane == 0 && by_boxes) {
+            const int steps = PER_TILE * (j1 - j0), width = n_end - n_first;
+            for (int i = 0; i < steps; ++i) {
+                const int s = i & depth - 1, c = j0 * TILE + i * BOX_COLS;
+                if (!mbar_wait(&box_done[s], i >> depth_log & 1, abortp) || *abortp) break;
+                if (c < width) tma_store_2d(&boxes.out[g], box + s * BLOCK_BYTES, c, t0);
+                asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+                if (i > 0) {
+                    asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+                    mbar_arrive(&box_empty[i - 1 & depth - 1]);
+                }
+            }
+            asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
         }
     } else {
         // after a wait that ran out the loops go on, as the barriers of these threads count on all of them, but touch nothing
         const int tid = threadIdx.x - 64, q = warp & 3, part = (warp - 2) >> 2;
         bool ok = true;
-        auto wait_for_sums = [&](int product) {
-            ok = __all_sync(0xffffffffu, mbar_wait(&acc_full[barrier_of_product(product)], phase_of_product(product), abortp)) && ok;
+        auto wait_for_sums = [&](int barrier, int phase) {
+            ok = __all_sync(0xffffffffu, mbar_wait(&acc_full[barrier], phase & 1, abortp)) && ok;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         };
         auto sums_read = [&](int product, int times) {
@@ -424,7 +461,7 @@ low_rank_result_kernel(const __grid_constant__ CUtensorMap map_h, const __grid_c
                 for (int i = 0; i < times; ++i) mbar_arrive(&acc_empty[product % ACCS]);
         };
         if (by_boxes) {
-            // A thread has a row of a box; four warps have one, the next four the next, and no warp waits for another: each sends its 32 rows off.
+            // A thread has a row of a box; four warps have one, the next four the next.
             // 16 bytes of a row lie at their place xor the row's number: no bank conflicts.  A part has one box of a tile at most.
             constexpr int E = 16 / (int)sizeof(O), COLS = BOX_COLS / 2;
             static_assert(PER_TILE <= PARTS && PARTS % PER_TILE == 0, "a part's boxes are of different tiles");
@@ -438,14 +475,17 @@ low_rank_result_kernel(const __grid_constant__ CUtensorMap map_h, const __grid_c
             const int sole = present ? __ffs(present) - 1 : 0;
 #pragma unroll 1
             for (int step = part; step < steps; step += PARTS) {
-                const int t = step / PER_TILE, in = step % PER_TILE, s = step % depth;
-                for (int p = 0; p < passes; ++p) wait_for_sums(t * passes + p);
+                const int t = step / PER_TILE, in = step % PER_TILE, s = step & depth - 1;
+                for (int p = 0; p < passes; ++p) wait_for_sums(t % TILE_TURNS * ACCS + p, t / TILE_TURNS);
                 if (base) {
-                    ok = __all_sync(0xffffffffu, mbar_wait(&box_full[s], (step / depth) & 1, abortp)) && ok;
+                    ok = __all_sync(0xffffffffu, mbar_wait(&box_full[s], step >> depth_log & 1, abortp)) && ok;
                 } else if (step >= depth) {                        // the stores that had this box's memory have read it
-                    ok = __all_sync(0xffffffffu, mbar_wait(&box_empty[s], (step / depth - 1) & 1, abortp)) && ok;
+                    ok = __all_sync(0xffffffffu, mbar_wait(&box_empty[s], (step >> depth_log) - 1 & 1, abortp)) && ok;
                 }
-                if (ok)
+                auto release = [&]() {
+                    for (int p = 0; p < passes; ++p) sums_read(t * passes + p, 1);
+                };
+                if (ok && (present || !base))                      // rows without an adapter stay as they came
 #pragma unroll
                     for (int half = 0; half < 2; ++half) {
                         float v[COLS];
@@ -467,26 +507,18 @@ low_rank_result_kernel(const __grid_constant__ CUtensorMap map_h, const __grid_c
                                 for (int c = 0; c < COLS; ++c) v[c] = which == p ? w[c] : v[c];
                             }
                         }
-                        if (half == 1)
-                            for (int p = 0; p < passes; ++p) sums_read(t * passes + p, 1);
+                        if (half == 1) release();
 #pragma unroll
                         for (int c = 0; c < 4; ++c) {
                             uint4* at = reinterpret_cast<uint4*>(box + s * BLOCK_BYTES + row * 128 + (((half * 4 + c) ^ (row & 7)) * 16));
                             *at = plus(base ? *at : make_uint4(0, 0, 0, 0), v + c * E, O());
                         }
                     }
+                else release();
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
-                if (lane == 0) {
-                    const int c = j0 * TILE + step * BOX_COLS;
-                    if (ok && c < n_end - n_first && t0 + q * 32 < tokens) tma_store_2d(&boxes.out[g], box + s * BLOCK_BYTES + q * 32 * 128, c, t0 + q * 32);
-                    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-                    asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-                    mbar_arrive(&box_empty[s]);
-                }
-                __syncwarp();
+                if (lane == 0) mbar_arrive(&box_done[s]);
             }
-            if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
         } else if (warp < 2 + EPI_WARPS) {
             int i = 0;
             for (int p = 0; p < passes; ++p) {
@@ -511,7 +543,7 @@ low_rank_result_kernel(const __grid_constant__ CUtensorMap map_h, const __grid_c
 #pragma unroll
                     for (int m = 0; m < 4; ++m) old[m] = ahead[m];
                     ask(ahead, step + 1);
-                    if (half == 0) wait_for_sums(i);
+                    if (half == 0) wait_for_sums(acc, i / ACCS);
                     if (wide > 0 && ok) {
                         float v[32];
                         tmem_load<32>(tmem + ((uint32_t)(q * 32) << 16) + acc * TILE + half * CHUNK + part * 32, v);
@@ -603,7 +635,7 @@ int launch_results(const void* hidden, const CUtensorMap& map_b, const int* ids,
         O* o = (O*)out + n0;
         bool fits = reinterpret_cast<uintptr_t>(b) % 16 == 0 && reinterpret_cast<uintptr_t>(o) % 16 == 0 && row_b * (long long)sizeof(O) % 16 == 0 &&
                     row_o * (long long)sizeof(O) % 16 == 0 && wide * sizeof(O) % 16 == 0;      // a box that ends inside 16 bytes writes more of them
-        fits = fits && make_box_map<O>(&boxes.out[g], o, T, wide, row_o, 32) == 0 &&
+        fits = fits && make_box_map<O>(&boxes.out[g], o, T, wide, row_o, TILE) == 0 &&
                make_box_map<O>(&boxes.base[g], b ? b : o, T, wide, b ? row_b : row_o, TILE) == 0;
         if (fits) by_box |= 1 << g;
         else boxes.out[g] = boxes.base[g] = map_h;                 // never followed
@@ -619,11 +651,11 @@ int launch_results(const void* hidden, const CUtensorMap& map_b, const int* ids,
     }
     const int aligned = reinterpret_cast<uintptr_t>(out) % 16 == 0 && reinterpret_cast<uintptr_t>(base) % 16 == 0 &&
                         (T == 1 || (ldo % 8 == 0 && (base == nullptr || ldb % 8 == 0)));
-    const int depth = kblocks == 1 ? MOST_BOXES : PARTS, stages = kblocks == 1 ? 3 : 2;
-    const size_t smem = 1024 + (size_t)((2 + stages) * kblocks + depth) * BLOCK_BYTES;
+    const int buffers = kblocks == 1 ? 11 : 8;
+    const size_t smem = 1024 + (size_t)(2 * kblocks + buffers) * BLOCK_BYTES;
     prism::open_smem(low_rank_result_kernel<O>, smem);
     return (int)prism::launch_kernel(low_rank_result_kernel<O>, dim3(s.units[G], tiles), dim3(RESULT_THREADS), smem, stream, map_h, map_b, boxes, ids, (const O*)base,
-                                     ldb, (O*)out, ldo, by_box, depth, stages, aligned, T, r, N, L, s, err);
+                                     ldb, (O*)out, ldo, by_box, buffers, aligned, T, r, N, L, s, err);
 }
 
 }  // namespace lowrank_tile
