@@ -250,7 +250,7 @@ __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, const void*
     asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(map), "r"(smem_addr(src)), "r"(c0), "r"(c1) : "memory");
 }
 
-constexpr int MOST_STAGES = 7, ACCS = 4;                          // ACCS: accumulators, all of tensor memory
+constexpr int MOST_STAGES = 3, ACCS = 4;                          // ACCS: accumulators, all of tensor memory
 constexpr int PARTS = 4;                                          // groups of four warps that each have a box
 // A wait knows a barrier's phase by one bit, so who waits on a barrier has to wait for each of its phases.  Parts take boxes in turn and tiles of
 // columns in turn: a box's memory is always the same part's (the boxes there is memory for are a multiple of the parts), and a product's barrier
@@ -340,9 +340,9 @@ low_rank_result_kernel(const __grid_constant__ CUtensorMap map_h, const __grid_c
     const int passes = count;
     // Up to ACCS adapters: their products with a tile of columns lie side by side in tensor memory, a thread takes its row's, and the results go by
     // boxes.  Else one adapter after the other.
-    // The memory: twice as many boxes as parts where a tile has one adapter at most, else as many, and the rest for tiles of B, which more adapters
-    // use up faster.
-    const int depth_log = kblocks == 1 && passes <= 1 ? 3 : 2, depth = 1 << depth_log, stages = min(MOST_STAGES, (buffers - depth) / kblocks);
+    // The memory: eight boxes, and three tiles of B, or four and two of twice the size (four boxes and seven tiles, where a tile has two adapters
+    // and uses up B faster, took 2,048 tokens of such tiles from 119 to 124 us)
+    const int depth_log = kblocks == 1 ? 3 : 2, depth = 1 << depth_log, stages = (buffers - depth) / kblocks;
     unsigned char* box = ring + stages * kblocks * BLOCK_BYTES;
     float* sums = reinterpret_cast<float*>(box);                                       // where no boxes are used
     const bool nothing = passes == 0 && (const O*)out == base, by_boxes = !nothing && passes <= ACCS && (by_box >> g & 1);
