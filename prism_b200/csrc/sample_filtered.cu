@@ -842,7 +842,7 @@ sample_filtered_kernel(const float* __restrict__ logits_, long long ld, int R, i
     const float* x = pdl_fresh(logits_) + (size_t)row * ld + c0;
     const float T = temperature_ ? pdl_fresh(temperature_)[row] : 0.f;
     const int k = top_k_ ? pdl_fresh(top_k_)[row] : 0;
-    const float p = top_p_ ? pdl_fresh(top_p_)[row] : 1.f, mp = min_p_ ? fminf(pdl_fresh(min_p_)[row], 1.f) : 0.f;
+    const float p = top_p_ ? pdl_fresh(top_p_)[row] : 1.f, min_p = min_p_ ? pdl_fresh(min_p_)[row] : 0.f, mp = min_p > 0.f ? fminf(min_p, 1.f) : 0.f;
     const float u = pdl_fresh(u_)[row];
 
     float top = -INFINITY;
@@ -922,7 +922,7 @@ sample_filtered_kernel(const float* __restrict__ logits_, long long ld, int R, i
     }
     if (tid == 0) {
         sh.top = (double)top;
-        sh.floor = __double2float_ru((double)top - 1000.0 / sh.per);
+        sh.floor = fmaxf(LEAST, __double2float_ru((double)top - 1000.0 / sh.per));           // at an infinite temperature all but -infinity count
     }
     __syncthreads();
     // min_p as the lowest value that it keeps

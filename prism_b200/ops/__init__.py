@@ -729,6 +729,9 @@ def sample(logits: torch.Tensor, temperature: Optional[torch.Tensor], u: Optiona
                               _ptr(out), _stream()), "sample")
 
 
+_MOST_VOCABULARY = 520000     # csrc/sample_filtered.cu: MOST_V
+
+
 def sample_filtered(logits: torch.Tensor, temperature: Optional[torch.Tensor], u: torch.Tensor, out: torch.Tensor,
                     top_k: Optional[torch.Tensor] = None, top_p: Optional[torch.Tensor] = None, min_p: Optional[torch.Tensor] = None,
                     rows: Optional[torch.Tensor] = None, kept: Optional[torch.Tensor] = None, logprob: Optional[torch.Tensor] = None):
@@ -759,6 +762,8 @@ def sample_filtered(logits: torch.Tensor, temperature: Optional[torch.Tensor], u
     if rows is not None and (rows.dtype is not i32 or rows.dim() != 1 or n > R or rows.get_device() != d or not rows.is_contiguous()):
         raise KernelError(f"sample_filtered: rows are int32 numbers of some of the {R} rows, contiguous on {logits.device}: got {rows.dtype} "
                           f"{tuple(rows.shape)} on {rows.device}")
+    if V > _MOST_VOCABULARY or n > 65535:
+        raise KernelError(f"sample_filtered: {n} rows of {V}: up to 65535 rows of up to {_MOST_VOCABULARY}")
     _here(logits, "sample_filtered")
     if n == 0:
         return

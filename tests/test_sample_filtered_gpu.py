@@ -257,3 +257,26 @@ def test_refusals():
     ops.sample_filtered(x[:0], None, one[:0], out[:0])
     ops.sample_filtered(x, None, one, out, rows=out[:0])
     assert out.tolist() == [0, 0]
+
+
+@pytest.mark.parametrize("V", [70, 9001])
+def test_settings_that_are_no_numbers_and_masks_at_any_temperature(V):
+    x = logits(6, V, 41)
+    x[:, ::3] = -math.inf
+    x[:, 1] = float("nan")
+    nan = float("nan")
+    # an infinite temperature makes all tokens alike, save those that are masked; a setting that is NaN is off
+    check(x.to(DEV), [math.inf, math.inf, math.inf, 1.0, 1.0, 3e38], [0.0, 0.5, 1 - 2.0 ** -24, 0.3, 0.6, 0.9], k=[0, 20, 0, 0, 9, 0],
+          p=[1.0, 1.0, 0.5, nan, nan, 0.7], m=[0.0, 0.0, 0.9, nan, 0.01, nan])
+
+
+def test_refuses_more_than_it_takes():
+    ops = _ops()
+    x = torch.zeros(1, 520001, device=DEV)
+    u, out = torch.zeros(1, device=DEV), torch.zeros(1, dtype=torch.int32, device=DEV)
+    with pytest.raises(ops.KernelError, match="520000"):
+        ops.sample_filtered(x, None, u, out)
+    x = torch.zeros(65536, 1, device=DEV)
+    u, out = torch.zeros(65536, device=DEV), torch.zeros(65536, dtype=torch.int32, device=DEV)
+    with pytest.raises(ops.KernelError, match="65536"):
+        ops.sample_filtered(x, None, u, out)
