@@ -485,7 +485,7 @@ low_rank_result_kernel(const __grid_constant__ CUtensorMap map_h, const __grid_c
                 auto release = [&]() {
                     for (int p = 0; p < passes; ++p) sums_read(t * passes + p, 1);
                 };
-                if (ok && (present || !base))                      // rows without an adapter stay as they came
+                if (ok && (present || !base))                      // rows without an adapter stay as they came, bit by bit
 #pragma unroll
                     for (int half = 0; half < 2; ++half) {
                         float v[COLS];
@@ -511,7 +511,7 @@ low_rank_result_kernel(const __grid_constant__ CUtensorMap map_h, const __grid_c
 #pragma unroll
                         for (int c = 0; c < 4; ++c) {
                             uint4* at = reinterpret_cast<uint4*>(box + s * BLOCK_BYTES + row * 128 + (((half * 4 + c) ^ (row & 7)) * 16));
-                            *at = plus(base ? *at : make_uint4(0, 0, 0, 0), v + c * E, O());
+                            if (which >= 0 || !base) *at = plus(base ? *at : make_uint4(0, 0, 0, 0), v + c * E, O());
                         }
                     }
                 else release();

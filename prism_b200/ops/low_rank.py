@@ -37,7 +37,7 @@ class LowRank:
     below each other.  ``rows``: how many of the N rows each slice has.  r is a multiple of 16 up to 128, with zeros beyond an adapter's
     own rank; Kp is K rounded up to a multiple of 8 at least, with zeros beyond K.  ``scale``: float32 ``[L]``."""
 
-    __slots__ = ("a", "b", "scale", "rows", "k", "rank", "count", "n", "_first", "_where", "_sizes")
+    __slots__ = ("a", "b", "scale", "rows", "k", "rank", "count", "n", "_first", "_sizes")
 
     def __init__(self, a: torch.Tensor, b: torch.Tensor, scale: torch.Tensor, rows: Sequence[int], k: Optional[int] = None):
         rows = tuple(map(int, rows))
@@ -60,8 +60,6 @@ class LowRank:
             raise ops.KernelError("adapters: A, B and the scales lie contiguous on one device, A and B from a 16-byte border on")
         self.a, self.b, self.scale, self.rows, self.k, self.rank, self.count, self.n = a, b, scale, rows, k, r, L, n
         self._first = (ctypes.c_int * (G + 1))(0, *itertools.accumulate(rows))
-        # what every call hands over: where A, B and the scales are, and their sizes
-        self._where = (a.data_ptr(), b.data_ptr(), scale.data_ptr())
         self._sizes = (k, kp, r, L, G, ctypes.addressof(self._first))
 
     @classmethod
@@ -143,7 +141,7 @@ def low_rank(x: torch.Tensor, low: LowRank, ids: torch.Tensor, base: Optional[to
              singles: Optional[int] = None) -> torch.Tensor:
     """``out[t] = base[t] + scale[l] (x[t] A_l^T) B_l^T`` with ``l = ids[t]`` (int32 ``[T]`` on the device; negative: ``out[t] = base[t]``).
     ``x [T, K]`` in the adapters' dtype; ``base`` and ``out [T, N]`` both bfloat16 or both float32, rows may have strides of their own;
-    ``base`` None: zeros; ``out`` may be ``base`` itself.  Sums in float32, one rounding.  ``singles``: so many tokens from the first on are
+    ``base`` None: zeros; ``out`` may be ``base`` itself, else it shares no memory with the others.  Adapters are finite.  Sums in float32, one rounding.  ``singles``: so many tokens from the first on are
     each a request of its own, and the others stand in runs of one adapter (as in a step: decoding requests, then portions of
     prompts); this says how the work is laid out and changes no result's meaning.  An id outside the stack adds nothing and is reported by
     ``check_tc_errors``."""
@@ -168,7 +166,7 @@ def low_rank(x: torch.Tensor, low: LowRank, ids: torch.Tensor, base: Optional[to
     singles = (T if T <= SINGLES else 0) if singles is None else max(0, min(int(singles), T))
     L, stream, err = ops.lib(), ops._stream(), ops.mxfp4._err_word(x.device)
     sms = ops._num_sms.get(d) or ops.num_sms(x.device)
-    (ap, bp, sp), sizes = low._where, low._sizes
+    ap, bp, sp, sizes = low.a.data_ptr(), low.b.data_ptr(), low.scale.data_ptr(), low._sizes
     bf16, out16 = dt is torch.bfloat16, odt is torch.bfloat16
     xp, x_row, ip, op, o_row = x.data_ptr(), x.stride(0), ids.data_ptr(), out.data_ptr(), out.stride(0)
     basep, b_row = (None, 0) if base is None else (base.data_ptr(), base.stride(0))
@@ -181,7 +179,7 @@ def low_rank(x: torch.Tensor, low: LowRank, ids: torch.Tensor, base: Optional[to
     size, G = 2 if out16 else 4, len(low.rows)
     xp, op, basep = xp + singles * x_row * (2 if bf16 else 4), op + singles * o_row * size, basep and basep + singles * b_row * size
     args = (sp, ip + 4 * singles, basep, b_row, op, o_row, out16, rest, *sizes)
-    if bf16 and rest >= TILE_FROM and L.prism_low_rank_tile_supported(low.k, low.rank, G, xp % 16 == 0 and (x_row % 8 == 0 or rest == 1)):
+    if bf16 and rest >= TILE_FROM and L.prism_low_rank_tile_supported(low.k, low.rank, G, xp % 16 == 0 and x_row % 8 == 0 and x_row >= low.k):
         hidden = torch.empty(2 * rest * G * low.rank, dtype=torch.bfloat16, device=x.device)
         ops._check(L.prism_low_rank_tile(xp, x_row, ap, bp, *args, hidden.data_ptr(), sms, err, stream), "low_rank_tile")
     else:

@@ -256,3 +256,34 @@ def test_calls_queued_behind_each_other(ids, dtype):
                 o.fill_(float("nan"))
     assert int(wrong) == 0
     ops.check_tc_errors()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=str)
+@pytest.mark.parametrize("T,n,singles", [(200, 256, 0), (200, 100, 0), (40, 256, 40), (150, 257, 10)])
+def test_tokens_without_an_adapter_keep_their_bits(dtype, T, n, singles):
+    ops = _ops()
+    low = stack(3, (n,), 128, 16, torch.bfloat16, 5)
+    g = torch.Generator(device=DEV).manual_seed(9)
+    x = torch.randn(T, 128, generator=g, device=DEV).bfloat16()
+    base = torch.randn(T, n, generator=g, device=DEV).to(dtype)
+    base[:, ::7] = -0.0
+    base[:, 3::11] = float("inf")
+    for ids in (torch.arange(T) % 4 - 1, torch.full((T,), -1), torch.where(torch.arange(T) < T // 2, 1, -1)):
+        ids = ids.int().to(DEV)
+        out = ops.low_rank(x, low, ids, base=base, singles=singles)
+        same = base.clone()
+        ops.low_rank(x, low, ids, base=same, out=same, singles=singles)
+        whole = torch.int16 if dtype is torch.bfloat16 else torch.int32
+        none = ids < 0
+        assert torch.equal(out.view(whole)[none], base.view(whole)[none]) and torch.equal(same.view(whole), out.view(whole))
+
+
+@pytest.mark.parametrize("T", [5, 40, 200])
+def test_one_row_for_all_tokens(T):
+    ops = _ops()
+    low = stack(2, (96,), 64, 16, torch.bfloat16, 6)
+    x, base = inputs(T, 64, 96, torch.bfloat16, torch.bfloat16, 3)
+    x = x[:1].expand(T, 64)
+    ids = (torch.arange(T, device=DEV) % 3 - 1).int()
+    check(ops.low_rank(x, low, ids, base=base, singles=0), *plain(x, low, ids, base))
+    check(ops.low_rank(x, low, ids, base=base, singles=T), *plain(x, low, ids, base))
