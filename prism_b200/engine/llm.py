@@ -123,11 +123,12 @@ class Engine:
 
     def unload_adapter(self, name: str) -> None:
         """Forget an adapter and give its place to the next one.  Refused while a request that uses it is waiting or running."""
+        if name is None:
+            raise ValueError("unload_adapter: which adapter?")
         number = self._adapter_number(name)
-        if number >= 0 and any(r.adapter == number for r in list(self.scheduler.waiting) + list(self.scheduler.running)):
+        if any(r.adapter == number for r in list(self.scheduler.waiting) + list(self.scheduler.running)):
             raise ValueError(f"adapter {name!r} is in use")
-        if self.adapters is not None:
-            self.adapters.remove(name)
+        self.adapters.remove(name)
 
     def warmup(self, batch_sizes: Optional[Sequence[int]] = None) -> None:
         """Capture the decode graphs before the first request (engine/executor.py:312-318 does it for a list of
