@@ -134,7 +134,12 @@ def in_use(w):
 
 
 SINGLES = 64                 # without a word from the caller, so many tokens are taken one by one
-TILE_FROM = 16               # so many tokens of portions, and they are taken in tiles of 128 on tensor cores
+# So many tokens of portions, and they are taken in tiles: of 128 on tensor cores, or of 32 on CUDA cores (32-bit floats, sizes that TMA does not
+# take); fewer one by one.  Microseconds one by one and in tiles, all tokens of one adapter, for gate and up (rank 16), q k v (32) and down (64) of the 7B shape:
+# bfloat16, 32 tokens 13.5/17.3, 14.6/16.7, 23.9/27.2; 64 tokens 24.2/17.8, 23.7/17.0, 29.9/27.5 (two adapters a tile cost the tiles a half more).
+# float32, 64 tokens 28/46, 24/44, 32/194; 128 tokens 51/54, 45/44, 63/194; 512 tokens 200/85 (gate and up).
+TILE_FROM = 48
+PLAIN_TILE_FROM = 128
 
 
 def low_rank(x: torch.Tensor, low: LowRank, ids: torch.Tensor, base: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
@@ -170,16 +175,19 @@ def low_rank(x: torch.Tensor, low: LowRank, ids: torch.Tensor, base: Optional[to
     bf16, out16 = dt is torch.bfloat16, odt is torch.bfloat16
     xp, x_row, ip, op, o_row = x.data_ptr(), x.stride(0), ids.data_ptr(), out.data_ptr(), out.stride(0)
     basep, b_row = (None, 0) if base is None else (base.data_ptr(), base.stride(0))
+    G = len(low.rows)
+    tiles = bf16 and xp % 16 == 0 and x_row % 8 == 0 and x_row >= low.k and L.prism_low_rank_tile_supported(low.k, low.rank, G, True)
+    if T - singles < (TILE_FROM if tiles else PLAIN_TILE_FROM):
+        singles = T
     if singles:
         ops._check(L.prism_low_rank(xp, x_row, bf16, ap, bp, sp, ip, basep, b_row, op, o_row, out16, singles, *sizes, None, sms, err, stream), "low_rank")
     rest = T - singles
     if rest == 0:
         return out
-    # behind the singles, in tiles
-    size, G = 2 if out16 else 4, len(low.rows)
+    size = 2 if out16 else 4
     xp, op, basep = xp + singles * x_row * (2 if bf16 else 4), op + singles * o_row * size, basep and basep + singles * b_row * size
     args = (sp, ip + 4 * singles, basep, b_row, op, o_row, out16, rest, *sizes)
-    if bf16 and rest >= TILE_FROM and L.prism_low_rank_tile_supported(low.k, low.rank, G, xp % 16 == 0 and x_row % 8 == 0 and x_row >= low.k):
+    if tiles:
         hidden = torch.empty(2 * rest * G * low.rank, dtype=torch.bfloat16, device=x.device)
         ops._check(L.prism_low_rank_tile(xp, x_row, ap, bp, *args, hidden.data_ptr(), sms, err, stream), "low_rank_tile")
     else:

@@ -287,3 +287,14 @@ def test_one_row_for_all_tokens(T):
     ids = (torch.arange(T, device=DEV) % 3 - 1).int()
     check(ops.low_rank(x, low, ids, base=base, singles=0), *plain(x, low, ids, base))
     check(ops.low_rank(x, low, ids, base=base, singles=T), *plain(x, low, ids, base))
+
+
+@pytest.mark.parametrize("dtype,out_dtype", TYPES)
+@pytest.mark.parametrize("rows,K,rank", [((130, 65), 1003, 5), ((257,), 70, 100), ((96, 8, 40), 512, 128)])
+@pytest.mark.parametrize("lengths", [(47,), (48,), (127,), (128,), (1, 126), (40, 1, 90, 33, 160), (300, 200)], ids=str)
+def test_portions_of_every_length(dtype, out_dtype, rows, K, rank, lengths):
+    """On both sides of the lengths from which portions are taken in tiles; some have no adapter, some tiles several."""
+    low = stack(3, rows, K, rank, dtype, 11)
+    ids = ids_of([(i % 4 - 1 if len(lengths) > 1 else 1, n) for i, n in enumerate(lengths)])
+    x, base = inputs(ids.numel(), K, sum(rows), dtype, out_dtype, 12)
+    check(_ops().low_rank(x, low, ids, base=base, singles=0), *plain(x, low, ids, base))
