@@ -68,9 +68,12 @@ __device__ __forceinline__ uint32_t rank_in_cluster() {
 
 // ---- one token ----------------------------------------------------------------------------------------------
 
-// THREADS: 512 where the CTAs are no more than the SMs, with twice the loads of A in flight; else 256, four CTAs an SM, whose waits overlap
-template <typename T, typename O, int THREADS>
-__global__ void __launch_bounds__(THREADS, THREADS == 512 ? 1 : 4)
+// Three of it, by the clusters of a launch.  512 threads and an SM's registers, eight loads of A in flight a thread, where all clusters run at a time so
+// (15 on 148 SMs, as a cluster's CTAs are neighbours) or nearly.  512 threads and half an SM's registers up to 33 clusters; else 256 threads, four CTAs an SM, whose
+// waits overlap.  Microseconds of the three (bfloat16, the 7B shape, an adapter a token): down projection of rank 64, 4 tokens 8.4, 10.8, 15.2; 24 tokens
+// 19.9, 20.0, 28.8; gate and up of rank 16, 16 tokens 14.7, 9.4, 12.0; 64 tokens 57, 42, 32.
+template <typename T, typename O, int THREADS, int PER_SM>
+__global__ void __launch_bounds__(THREADS, PER_SM)
 low_rank_token_kernel(const T* __restrict__ x_, long long ldx, int x_whole, const T* __restrict__ a, const T* __restrict__ b,
                       const float* __restrict__ scale, const int* __restrict__ ids_, const O* __restrict__ base_, long long ldb, O* out_, long long ldo,
                       int K, int Kp, int r, int L, Slices slices, int parts, int* err) {
@@ -125,7 +128,7 @@ low_rank_token_kernel(const T* __restrict__ x_, long long ldx, int x_whole, cons
         int k = (sub * 32 + lane) * E;
         if (x_whole) {
             // several chunks of A and x on their way at a time, without a branch between them
-            constexpr int U = THREADS == 512 ? 8 : 2;
+            constexpr int U = PER_SM == 1 ? 8 : PER_SM == 2 ? 4 : 2;
             const int stride = split * 32 * E;
             for (; k + (U - 1) * stride + E <= K; k += U * stride) {
                 uint4 w[U], v[U];
@@ -205,17 +208,21 @@ int launch_tokens(const void* x, long long ldx, const void* a, const void* b, co
                   long long ldo, int tokens, int K, int Kp, int r, int L, const Slices& s, int* err, int sms, cudaStream_t stream) {
     if (tokens <= 0) return 0;
     if (tokens > 65535) return (int)cudaErrorInvalidValue;
+    // Clusters at a time with an SM a CTA, and with half of one.  Up to 18 are launched in the first form all the same: rows without an adapter (of a captured
+    // step that has fewer requests than rows, say) are over at once.  16 tokens, down projection of rank 64: 17.3 us, in the second form 16.0; if one of them
+    // has none 10.9 and 16.3.
+    const int wholes = sms / CTAS * 5 / 6, halves = sms * 9 / (CTAS * 5), first_form = sms / CTAS;
     // clusters that share a slice's columns, each with hidden values of its own: as many as keep B's part of a CTA within what it asks for ahead, while
-    // all CTAs together are no more than the SMs
+    // all run at a time
     int widest = 0;
     for (int g = 0; g < s.n; ++g) widest = max(widest, s.first[g + 1] - s.first[g]);
     const long long bytes = (long long)widest * r * (int)sizeof(T), ahead = (long long)CTAS * 512 * AHEAD * EACH * 16;
-    const int parts = (int)max(1ll, min((bytes + ahead - 1) / ahead, (long long)sms / ((long long)CTAS * s.n * tokens)));
+    const int parts = (int)max(1ll, min((bytes + ahead - 1) / ahead, (long long)wholes / ((long long)s.n * tokens)));
     const int whole = (reinterpret_cast<uintptr_t>(x) % 16 == 0) && (ldx * (long long)sizeof(T) % 16 == 0 || tokens == 1);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(CTAS, s.n * parts, tokens);
-    const bool many = (long long)CTAS * s.n * parts * tokens > sms;
-    cfg.blockDim = dim3(many ? 256 : 512);
+    const int clusters = s.n * parts * tokens;
+    cfg.blockDim = dim3(clusters <= halves ? 512 : 256);
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -224,7 +231,7 @@ int launch_tokens(const void* x, long long ldx, const void* a, const void* b, co
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = prism::pdl_enabled() ? 2 : 1;
-    const auto kernel = many ? low_rank_token_kernel<T, O, 256> : low_rank_token_kernel<T, O, 512>;
+    const auto kernel = clusters <= first_form ? low_rank_token_kernel<T, O, 512, 1> : clusters <= halves ? low_rank_token_kernel<T, O, 512, 2> : low_rank_token_kernel<T, O, 256, 4>;
     return (int)cudaLaunchKernelEx(&cfg, kernel, (const T*)x, ldx, whole, (const T*)a, (const T*)b, scale, ids, (const O*)base, ldb, (O*)out,
                                    ldo, K, Kp, r, L, s, parts, err);
 }

@@ -81,7 +81,7 @@ low_rank_hidden_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_c
     extern __shared__ unsigned char raw[];
     unsigned char* ring = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
     const int H = G * r, stage_bytes = BLOCK_BYTES + H * TILE_K * 2;
-    float* sums = reinterpret_cast<float*>(ring + (size_t)stages * stage_bytes);
+    float* sums = reinterpret_cast<float*>(ring);                  // behind a pass's last product, its sums; there is memory for as many at least
     __shared__ uint64_t full[8], empty[8], done;
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_flag, own[TILE], list[TILE], count;
@@ -218,8 +218,9 @@ low_rank_hidden_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_c
             asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
         }
         it += mine;
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-        __syncthreads();                      // the sums have been read: the next pass may write them
+        __syncthreads();                      // the sums have been read: the next pass's copies may come
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     }
     if (threadIdx.x == 0 && abort_flag) report_error(err, PRISM_ERR_WAIT_TIMEOUT);
@@ -692,10 +693,13 @@ PRISM_EXPORT int prism_low_rank_tile(const void* x, long long ldx, const void* a
     if (code != 0) return code;
 
     const int stage = BLOCK_BYTES + H * prism::tc::TILE_K * 2, sums = TILE * WIDE_LD * 4;
-    const int stages = min(6, (198 * 1024 - sums) / stage);
     int cols = 32;
     while (cols < H) cols *= 2;
-    size_t smem = 1024 + (size_t)stages * stage + sums;
+    // All of a CTA's memory for copies in flight, or a half of an SM's: of clusters of eight CTAs with an SM each, 15 run at a time on 148 SMs, with half of one 33
+    // (2,048 tokens, 16 tiles: 107 -> 97 us).  The CTAs that fit an SM have tensor memory side by side, as a cluster's wait for each other.
+    const int budget = tiles * CTAS > sms * 5 / 6 ? 104 * 1024 : 198 * 1024;
+    const int stages = max(2, min(6, budget / stage));
+    const size_t smem = max(1024 + (size_t)max(stages * stage, sums), (size_t)228 * 1024 / (512 / cols + 1) + 1);
     prism::open_smem(low_rank_hidden_kernel, smem);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(CTAS, tiles);
