@@ -18,6 +18,9 @@ Which of andre-fu/prism's call sites each op replaces:
 ``attention``       ``flash_attn_with_kvcache`` (executor.py:119-120)
 ``swiglu``          ``F.silu(gate) * up`` (executor.py:127)
 ``sample``          argmax / softmax + multinomial (engine/scheduler.py:266-272)
+``sample_filtered`` the same among the tokens that top-k, top-p and min-p keep; the
+                    reference has none of them
+``low_rank``        adapters of requests beside ``linear``; none there
 ==================  ==========================================================
 """
 
