@@ -4,8 +4,12 @@
 // slices' A (TMA, 128-byte swizzle, tcgen05.mma with the tokens as M); their sums meet through distributed shared memory, are scaled and leave as
 // two bfloat16 terms, high and low (2^-16 of a hidden value is lost; one term alone would lose 2^-8, as much as rounding the result does).  The
 // second multiplies them with B, 128 columns at a time, and adds the shared result: it is bound by reading and writing that - the 7B shape's gate
-// and up for 2,048 tokens are 310 MB against 28 MB of everything else.  So the shared result comes and goes by TMA, boxes of 128 rows by 128 bytes, some
-// of them ahead, and a thread adds its row's sums where they lie in shared memory.
+// and up for 2,048 tokens are 310 MB against 28 MB of everything else.  So the shared result comes and goes by TMA, boxes of 128 rows by 128 bytes, eight
+// of them on their way or at work, and a thread adds its row's sums where they lie in shared memory.
+//
+// Measured for that, rank 64, one adapter: 16 us for the hidden values and 71 for the results on their own, 76 together (the floor is 52; torch copies the shared
+// result in 48): 4.4 TB/s.  A launch that only passes boxes through takes 59: what bounds it is how fast an SM's share comes and goes.  Beside it a tile
+// of 128 x 128 moves 208 KB through shared memory, 1,600 cycles at 128 bytes a cycle of some 3,600.
 //
 // A tile's tokens may have several adapters, or some of them none.  The first launch goes through it once for each adapter; the second has up to four
 // adapters' products side by side in tensor memory.  With more than four, or where base and out are no place for TMA, it goes through the tile
@@ -27,7 +31,8 @@ constexpr int WIDE = 128, WIDE_LD = WIDE + 4;                     // the same of
 
 struct Tiles {
     int n, first[MOST_SLICES + 1];            // slice g has the result columns first[g] .. first[g + 1] - 1
-    int units[MOST_SLICES + 1];               // of the second launch: slice g has the CTAs units[g] .. units[g + 1] - 1 of a tile
+    // of the second launch: slice g has the CTAs units[g] .. units[g + 1] - 1 of a tile of tokens, and before[g] tiles of columns lie before it
+    int units[MOST_SLICES + 1], before[MOST_SLICES + 1];
 };
 
 // The tokens' adapters (-1: none, or beyond the end) and the different ones among them, in order.  By one warp.
@@ -73,10 +78,10 @@ __device__ __forceinline__ void epilogue_barrier() { asm volatile("bar.sync 1, %
 
 // ---- hidden values ------------------------------------------------------------------------------------------
 
-// hidden: [tokens][2][G r], high terms and low ones
+// hidden: [tokens][2][G r], high terms and low ones; adapters: how many a tile has
 __global__ void __launch_bounds__(ALL_THREADS)
 low_rank_hidden_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_a, const float* __restrict__ scale,
-                       const int* __restrict__ ids_, __nv_bfloat16* __restrict__ hidden, int tokens, int K, int r, int G, int L, int stages,
+                       const int* __restrict__ ids_, __nv_bfloat16* __restrict__ hidden, int* __restrict__ adapters, int tokens, int K, int r, int G, int L, int stages,
                        int tmem_cols, int* err) {
     extern __shared__ unsigned char raw[];
     unsigned char* ring = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
@@ -107,6 +112,7 @@ low_rank_hidden_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_c
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = tmem_slot;
     const int passes = count;
+    if (me == 0 && threadIdx.x == 0) adapters[blockIdx.y] = passes;
     pdl_trigger();                            // not before this CTA has its tensor memory: the next kernel may take the rest and wait
 
     int it = 0;                               // blocks so far, over all passes
@@ -252,12 +258,13 @@ __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, const void*
 }
 
 constexpr int MOST_STAGES = 3, ACCS = 4;                          // ACCS: accumulators, all of tensor memory
-constexpr int PARTS = 4;                                          // groups of four warps that each have a box
+constexpr int PARTS = 4;                                          // groups of four warps that each have a box; with two of them 2,048 tokens took 112 us, with four 104
 // A wait knows a barrier's phase by one bit, so who waits on a barrier has to wait for each of its phases.  Parts take boxes in turn and tiles of
 // columns in turn: a box's memory is always the same part's (the boxes there is memory for are a multiple of the parts), and a product's barrier
 // is its tile's of the next four (one that a tile later comes back to has been seen: it takes ACCS products more at least).  With six boxes a
 // part met a box's third use while the second, another part's, was still on its way, and took it for its own.
 constexpr int MOST_BOXES = 8, TILE_TURNS = 4;
+constexpr int MOST_EVEN = 64;                                      // tiles of tokens that CTAs share evenly, by what they cost
 static_assert(MOST_BOXES == 8 && PARTS == 4 && TILE_TURNS % PARTS == 0 && TILE_TURNS >= ACCS, "see above");
 constexpr int RESULT_THREADS = 64 + PARTS * 128 + 64;             // and two more warps: one asks for boxes, one sends them off
 
@@ -293,51 +300,49 @@ __device__ __forceinline__ uint4 plus(const uint4& old, const float* v, float) {
                       __float_as_uint(__uint_as_float(old.z) + v[2]), __float_as_uint(__uint_as_float(old.w) + v[3]));
 }
 
+struct Shared {
+    uint64_t full[MOST_STAGES], empty[MOST_STAGES], acc_full[TILE_TURNS * ACCS], acc_empty[ACCS], h_full, last, box_full[MOST_BOXES], box_done[MOST_BOXES],
+        box_empty[MOST_BOXES];
+    uint32_t tmem_slot;
+    int abort_flag, own[TILE], list[TILE], count, start[MOST_EVEN + 1], several;
+};
+constexpr int BARRIERS = 2 * MOST_STAGES + (TILE_TURNS + 1) * ACCS + 2 + 3 * MOST_BOXES;           // the first members, one after the other
+template <int PER_TILE> __device__ __forceinline__ void init_barriers(Shared& sh) {
+    for (int s = 0; s < MOST_STAGES; ++s) mbar_init(&sh.full[s], 1), mbar_init(&sh.empty[s], 1);
+    for (int s = 0; s < ACCS; ++s) mbar_init(&sh.acc_empty[s], 4 * min(PARTS, PER_TILE));
+    for (int s = 0; s < TILE_TURNS * ACCS; ++s) mbar_init(&sh.acc_full[s], 1);
+    for (int s = 0; s < MOST_BOXES; ++s) mbar_init(&sh.box_full[s], 1), mbar_init(&sh.box_done[s], 4), mbar_init(&sh.box_empty[s], 1);
+    mbar_init(&sh.h_full, 1), mbar_init(&sh.last, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+}
+
+// A part of the results: tokens from t0 on, slice g, tiles j0 to j1 - 1 of its columns.
 // by_box: a bit a slice, whether its columns of base and out can go by TMA; buffers: of 16 KB there is memory for, beside the hidden values
 template <typename O>
-__global__ void __launch_bounds__(RESULT_THREADS, 1)
-low_rank_result_kernel(const __grid_constant__ CUtensorMap map_h, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ Boxes boxes,
-                       const int* __restrict__ ids_, const O* base, long long ldb, O* out, long long ldo, int by_box, int buffers, int aligned, int tokens, int r, int N,
-                       int L, Tiles tiles, int* err) {
+__device__ __forceinline__ void result_part(Shared& sh, const CUtensorMap& map_h, const CUtensorMap& map_b, const Boxes& boxes, const int* ids, const O* base,
+                                            long long ldb, O* out, long long ldo, int by_box, int buffers, int aligned, int tokens, int r, int N, int L,
+                                            const Tiles& tiles, int t0, int g, int j0, int j1, bool first) {
     constexpr int BOX_COLS = 128 / (int)sizeof(O), PER_TILE = TILE / BOX_COLS;         // columns of a box of 128 bytes a row
     extern __shared__ unsigned char raw[];
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
     const int kblocks = (r + TILE_K - 1) / TILE_K;
     unsigned char* h_hi = smem;                                                        // high terms, then low ones
     unsigned char* ring = smem + 2 * kblocks * BLOCK_BYTES;
-    __shared__ uint64_t full[MOST_STAGES], empty[MOST_STAGES], acc_full[TILE_TURNS * ACCS], acc_empty[ACCS], h_full, last, box_full[MOST_BOXES],
-        box_done[MOST_BOXES], box_empty[MOST_BOXES];
-    __shared__ uint32_t tmem_slot;
-    __shared__ int abort_flag, own[TILE], list[TILE], count;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, t0 = blockIdx.y * TILE;
-    volatile int* abortp = &abort_flag;
-    int g = 0;
-    while (g + 1 < tiles.n && (int)blockIdx.x >= tiles.units[g + 1]) ++g;
-    // this CTA's tiles of the slice's columns
-    const int n_first = tiles.first[g], n_end = tiles.first[g + 1], all = (n_end - n_first + TILE - 1) / TILE;
-    const int units = tiles.units[g + 1] - tiles.units[g], unit = blockIdx.x - tiles.units[g];
-    const int j0 = (int)((long long)all * unit / units), j1 = (int)((long long)all * (unit + 1) / units);
-
-    if (threadIdx.x == 0) {
-        prefetch_map(&map_h), prefetch_map(&map_b), prefetch_map(&boxes.base[g]), prefetch_map(&boxes.out[g]);
-        abort_flag = 0;
-        for (int s = 0; s < MOST_STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
-        for (int s = 0; s < ACCS; ++s) mbar_init(&acc_empty[s], 4 * min(PARTS, PER_TILE));
-        for (int s = 0; s < TILE_TURNS * ACCS; ++s) mbar_init(&acc_full[s], 1);
-        for (int s = 0; s < MOST_BOXES; ++s) { mbar_init(&box_full[s], 1); mbar_init(&box_done[s], 4); mbar_init(&box_empty[s], 1); }
-        mbar_init(&h_full, 1), mbar_init(&last, 1);
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    }
-    pdl_wait();
-    if (warp == 1) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&tmem_slot)), "r"(ACCS * TILE));
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
-    }
-    if (warp == 2) list_adapters(pdl_fresh(ids_), t0, tokens, L, own, list, &count, nullptr);
+    auto &full = sh.full, &empty = sh.empty;
+    auto& acc_full = sh.acc_full;
+    auto& acc_empty = sh.acc_empty;
+    auto &h_full = sh.h_full, &last = sh.last;
+    auto &box_full = sh.box_full, &box_done = sh.box_done, &box_empty = sh.box_empty;
+    auto &own = sh.own, &list = sh.list;
+    int& count = sh.count;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    volatile int* abortp = &sh.abort_flag;
+    const int n_first = tiles.first[g], n_end = tiles.first[g + 1];
+    if (warp == 2) list_adapters(ids, t0, tokens, L, own, list, &count, nullptr);
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    const uint32_t tmem = tmem_slot;
+    const uint32_t tmem = sh.tmem_slot;
     const int passes = count;
     // Up to ACCS adapters: their products with a tile of columns lie side by side in tensor memory, a thread takes its row's, and the results go by
     // boxes.  Else one adapter after the other.
@@ -347,7 +352,7 @@ low_rank_result_kernel(const __grid_constant__ CUtensorMap map_h, const __grid_c
     unsigned char* box = ring + stages * kblocks * BLOCK_BYTES;
     float* sums = reinterpret_cast<float*>(box);                                       // where no boxes are used
     const bool nothing = passes == 0 && (const O*)out == base, by_boxes = !nothing && passes <= ACCS && (by_box >> g & 1);
-    pdl_trigger();                            // not before this CTA has its tensor memory: the next kernel may take the rest and wait
+    if (first) pdl_trigger();                            // not before this CTA has its tensor memory: the next kernel may take the rest and wait
     // products are numbered: tile by tile and in it adapter by adapter, or adapter by adapter
     const int products = passes * (j1 - j0);
     struct Turn {                             // of a product: its tile and its adapter's number among the tile's
@@ -378,6 +383,8 @@ low_rank_result_kernel(const __grid_constant__ CUtensorMap map_h, const __grid_c
                 turn.next(by_boxes, j1 - j0, passes);
                 if (++s == stages) s = 0, ++round;
             }
+            // the last products have read their tiles of B: nothing is on its way to a barrier when the part ends
+            for (int k = max(0, i - stages); k < i && !*abortp; ++k) mbar_wait(&empty[k % stages], (k / stages) & 1, abortp);
             if (*abortp) {
                 drain(&h_full, 0);
                 for (int k = max(0, i - stages); k < i; ++k) drain(&full[k % stages], (k / stages) & 1);
@@ -598,12 +605,98 @@ low_rank_result_kernel(const __grid_constant__ CUtensorMap map_h, const __grid_c
             }
         }
     }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     __syncwarp();                             // a warp whose first thread worked alone is whole again: what follows is for whole warps
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    if (threadIdx.x == 0 && abort_flag) report_error(err, PRISM_ERR_WAIT_TIMEOUT);
-    if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(ACCS * TILE));
+}
+
+// Results, one way or the other.  A CTA has some columns of one slice of one tile of tokens.  Or, where `adapters` is given and a tile of tokens has several, all
+// CTAs have the same share of the work, parts of neighbouring tiles one after the other: a tile of columns costs more with more adapters, and one tile of tokens
+// with two would hold up all others (2,048 tokens in three portions, gate and up of the 7B shape, rank 64: 107 us, shared evenly 92).  To end a part and begin the
+// next costs 6 to 8 us (2,048 tokens of one adapter 76 us, shared evenly 84; 1,024 tokens 48 and 54), so this is for several adapters, and for 16
+// tiles of columns a CTA and more.
+template <typename O>
+__global__ void __launch_bounds__(RESULT_THREADS, 1)
+low_rank_result_kernel(const __grid_constant__ CUtensorMap map_h, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ Boxes boxes,
+                       const int* __restrict__ ids_, const int* __restrict__ adapters_, const O* base, long long ldb, O* out, long long ldo, int by_box, int buffers,
+                       int aligned, int tokens, int r, int N, int L, const __grid_constant__ Tiles tiles, int* err) {
+    constexpr int PER_TILE = TILE * (int)sizeof(O) / 128;
+    __shared__ Shared sh;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        prefetch_map(&map_h), prefetch_map(&map_b);
+        sh.abort_flag = 0;
+        init_barriers<PER_TILE>(sh);
+    }
+    pdl_wait();
+    const int* ids = pdl_fresh(ids_);
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&sh.tmem_slot)), "r"(ACCS * TILE));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
+    }
+    const int token_tiles = (tokens + TILE - 1) / TILE, columns = tiles.before[tiles.n], units = tiles.units[tiles.n];
+    bool even = false;
+    if (adapters_ != nullptr) {
+        if (warp == 3) {                      // where a tile of tokens starts in the whole, in fifths of what a tile of columns costs with one adapter
+            const int* adapters = pdl_fresh(adapters_);
+            int before = 0;
+            bool several = false;
+            for (int q = 0; q < MOST_EVEN / 32; ++q) {
+                const int at = q * 32 + lane, n = at < token_tiles ? adapters[at] : 0;
+                int sum = at < token_tiles ? columns * (n <= 1 ? 5 : n <= ACCS ? 3 + 2 * n : 5 + 5 * n) : 0;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const int up = __shfl_up_sync(0xffffffffu, sum, o);
+                    if (lane >= o) sum += up;
+                }
+                sh.start[at + 1] = before + sum;
+                before += __shfl_sync(0xffffffffu, sum, 31);
+                several = __any_sync(0xffffffffu, n > 1) || several;
+            }
+            if (lane == 0) sh.start[0] = 0, sh.several = several;
+        }
+        __syncthreads();
+        even = sh.several;
+    }
+    int tile = blockIdx.x / units, g = 0, j0 = 0, j1 = 0, column = 0, low = 0, high = 0;
+    if (even) {
+        const long long whole = sh.start[token_tiles];
+        low = (int)(whole * blockIdx.x / gridDim.x), high = (int)(whole * (blockIdx.x + 1) / gridDim.x);
+        tile = 0;
+        while (sh.start[tile + 1] <= low) ++tile;
+        const int one = (sh.start[tile + 1] - sh.start[tile]) / columns;
+        column = (low - sh.start[tile] + one - 1) / one;           // a tile of columns is the CTA's in whose share it starts
+    } else {
+        const int own = blockIdx.x % units;
+        while (own >= tiles.units[g + 1]) ++g;
+        const int all = tiles.before[g + 1] - tiles.before[g], mine = tiles.units[g + 1] - tiles.units[g], unit = own - tiles.units[g];
+        j0 = (int)((long long)all * unit / mine), j1 = (int)((long long)all * (unit + 1) / mine);
+    }
+#pragma unroll 1
+    for (bool first = true; tile < token_tiles; first = false) {
+        if (even) {
+            if (sh.start[tile] >= high || sh.abort_flag) break;
+            const int one = (sh.start[tile + 1] - sh.start[tile]) / columns, end = min(columns, (high - sh.start[tile] + one - 1) / one);
+            if (column >= end) {
+                ++tile, column = 0;
+                if (first) pdl_trigger();                          // a share that is rounded to nothing
+                continue;
+            }
+            g = 0;
+            while (column >= tiles.before[g + 1]) ++g;
+            j0 = column - tiles.before[g], column = min(end, tiles.before[g + 1]), j1 = column - tiles.before[g];
+            if (!first && threadIdx.x == 0) {
+                for (int i = 0; i < BARRIERS; ++i) asm volatile("mbarrier.inval.shared::cta.b64 [%0];" ::"r"(smem_addr(&sh.full[0] + i)) : "memory");
+                init_barriers<PER_TILE>(sh);
+            }
+        }
+        result_part<O>(sh, map_h, map_b, boxes, ids, base, ldb, out, ldo, by_box, buffers, aligned, tokens, r, N, L, tiles, tile * TILE, g, j0, j1, first);
+        if (!even) break;
+    }
+    if (threadIdx.x == 0 && sh.abort_flag) report_error(err, PRISM_ERR_WAIT_TIMEOUT);
+    if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(sh.tmem_slot), "r"(ACCS * TILE));
 }
 
 // Columns of base or out as boxes of rows of 128 bytes
@@ -621,7 +714,7 @@ template <typename O> int make_box_map(CUtensorMap* map, const void* ptr, long l
 }
 
 template <typename O>
-int launch_results(const void* hidden, const CUtensorMap& map_b, const int* ids, const void* base, long long ldb, void* out, long long ldo, int T, int r, int L,
+int launch_results(const void* hidden, const int* adapters, const CUtensorMap& map_b, const int* ids, const void* base, long long ldb, void* out, long long ldo, int T, int r, int L,
                    Tiles s, int* err, int sms, cudaStream_t stream) {
     const int tiles = (T + TILE - 1) / TILE, G = s.n, N = s.first[G], kblocks = (r + TILE_K - 1) / TILE_K;
     CUtensorMap map_h;
@@ -644,18 +737,23 @@ int launch_results(const void* hidden, const CUtensorMap& map_b, const int* ids,
     // a CTA an SM shares the tiles of results; it has some columns of one slice
     int all = 0;
     for (int g = 0; g < G; ++g) all += (s.first[g + 1] - s.first[g] + TILE - 1) / TILE;
+    const bool even = tiles > 1 && tiles <= MOST_EVEN && (long long)all * tiles >= 16ll * sms && (long long)all * tiles * (5 + 5 * TILE) < 1ll << 31;
     const double per = all <= sms / tiles ? 1.0 : (double)all * tiles / sms;           // tiles of columns a CTA
-    s.units[0] = 0;
+    s.units[0] = s.before[0] = 0;
     for (int g = 0; g < G; ++g) {
         const int mine = (s.first[g + 1] - s.first[g] + TILE - 1) / TILE;
+        s.before[g + 1] = s.before[g] + mine;
         s.units[g + 1] = s.units[g] + max(1, min(mine, (int)(mine / per)));
     }
+    const long long ctas = (long long)s.units[G] * tiles;
+    if (ctas >= 1ll << 31) return (int)cudaErrorInvalidValue;
     const int aligned = reinterpret_cast<uintptr_t>(out) % 16 == 0 && reinterpret_cast<uintptr_t>(base) % 16 == 0 &&
                         (T == 1 || (ldo % 8 == 0 && (base == nullptr || ldb % 8 == 0)));
     const int buffers = kblocks == 1 ? 11 : 8;
     const size_t smem = 1024 + (size_t)(2 * kblocks + buffers) * BLOCK_BYTES;
     prism::open_smem(low_rank_result_kernel<O>, smem);
-    return (int)prism::launch_kernel(low_rank_result_kernel<O>, dim3(s.units[G], tiles), dim3(RESULT_THREADS), smem, stream, map_h, map_b, boxes, ids, (const O*)base,
+    return (int)prism::launch_kernel(low_rank_result_kernel<O>, dim3(even ? max(sms, (int)ctas) : (int)ctas), dim3(RESULT_THREADS), smem, stream, map_h, map_b, boxes, ids,
+                                     even ? adapters : nullptr, (const O*)base,
                                      ldb, (O*)out, ldo, by_box, buffers, aligned, T, r, N, L, s, err);
 }
 
@@ -668,7 +766,8 @@ PRISM_EXPORT int prism_low_rank_tile_supported(int K, int r, int G, int x_aligne
     return x_aligned && K >= 1 && r >= 16 && r % 16 == 0 && r <= MOST_RANK && G >= 1 && G <= MOST_SLICES && G * r <= MOST_HIDDEN;
 }
 
-// bfloat16 x and adapters, all T tokens in tiles; arguments as prism_low_rank's.  hidden: 2 T G r bfloat16 of workspace.
+// bfloat16 x and adapters, all T tokens in tiles; arguments as prism_low_rank's.  hidden: 2 T G r bfloat16 of workspace, and an int for each of the
+// tiles of 128 tokens.
 PRISM_EXPORT int prism_low_rank_tile(const void* x, long long ldx, const void* a, const void* b, const float* scale, const int* ids, const void* base,
                                      long long ldb, void* out, long long ldo, int out_dtype, int T, int K, int Kp, int r, int L, int G, const int* first,
                                      void* hidden, int sms, int* err, cudaStream_t stream) {
@@ -685,6 +784,7 @@ PRISM_EXPORT int prism_low_rank_tile(const void* x, long long ldx, const void* a
         if (s.first[g] >= s.first[g + 1]) return (int)cudaErrorInvalidValue;
     const int N = first[G], tiles = (T + TILE - 1) / TILE, H = G * r;
     if ((long long)L * N >= 1ll << 31 || (long long)L * H >= 1ll << 31) return (int)cudaErrorInvalidValue;
+    int* adapters = reinterpret_cast<int*>((bf16*)hidden + 2ll * T * H);
     CUtensorMap map_x, map_a, map_b;
     // a box of r rows of A: a slice's
     int code = prism::tc::make_map(&map_x, x, T, K, T > 1 ? ldx : (K + 7) / 8 * 8, TILE);
@@ -713,9 +813,9 @@ PRISM_EXPORT int prism_low_rank_tile(const void* x, long long ldx, const void* a
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = prism::pdl_enabled() ? 2 : 1;
-    code = (int)cudaLaunchKernelEx(&cfg, low_rank_hidden_kernel, map_x, map_a, scale, ids, (bf16*)hidden, T, K, r, G, L, stages, cols, err);
+    code = (int)cudaLaunchKernelEx(&cfg, low_rank_hidden_kernel, map_x, map_a, scale, ids, (bf16*)hidden, adapters, T, K, r, G, L, stages, cols, err);
     if (code != 0) return code;
 
-    if (out_dtype == PRISM_DTYPE_F32) return launch_results<float>(hidden, map_b, ids, base, ldb, out, ldo, T, r, L, s, err, sms, stream);
-    return launch_results<bf16>(hidden, map_b, ids, base, ldb, out, ldo, T, r, L, s, err, sms, stream);
+    if (out_dtype == PRISM_DTYPE_F32) return launch_results<float>(hidden, adapters, map_b, ids, base, ldb, out, ldo, T, r, L, s, err, sms, stream);
+    return launch_results<bf16>(hidden, adapters, map_b, ids, base, ldb, out, ldo, T, r, L, s, err, sms, stream);
 }

@@ -188,7 +188,7 @@ def low_rank(x: torch.Tensor, low: LowRank, ids: torch.Tensor, base: Optional[to
     xp, op, basep = xp + singles * x_row * (2 if bf16 else 4), op + singles * o_row * size, basep and basep + singles * b_row * size
     args = (sp, ip + 4 * singles, basep, b_row, op, o_row, out16, rest, *sizes)
     if tiles:
-        hidden = torch.empty(2 * rest * G * low.rank, dtype=torch.bfloat16, device=x.device)
+        hidden = torch.empty(2 * rest * G * low.rank + 2 * (-(-rest // 128)), dtype=torch.bfloat16, device=x.device)
         ops._check(L.prism_low_rank_tile(xp, x_row, ap, bp, *args, hidden.data_ptr(), sms, err, stream), "low_rank_tile")
     else:
         hidden = torch.empty(rest * G * low.rank, dtype=torch.float32, device=x.device)

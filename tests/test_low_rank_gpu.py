@@ -298,3 +298,23 @@ def test_portions_of_every_length(dtype, out_dtype, rows, K, rank, lengths):
     ids = ids_of([(i % 4 - 1 if len(lengths) > 1 else 1, n) for i, n in enumerate(lengths)])
     x, base = inputs(ids.numel(), K, sum(rows), dtype, out_dtype, 12)
     check(_ops().low_rank(x, low, ids, base=base, singles=0), *plain(x, low, ids, base))
+
+
+@pytest.mark.parametrize("out_dtype", [torch.bfloat16, torch.float32], ids=str)
+@pytest.mark.parametrize("rows", [(18944, 18944), (20000, 136, 18000), (40001,)], ids=str)
+@pytest.mark.parametrize("lengths", [(1024, 600, 424), (2048,), (5, 1100, 3, 2, 900), (1,) * 130 + (1000,)], ids=lambda v: str(len(v)))
+def test_wide_results_of_many_tokens(out_dtype, rows, lengths):
+    """Enough for all CTAs to share the work evenly, in parts of several tiles of tokens and slices; also with tiles of more adapters than tensor memory
+    holds side by side, and columns that are no place for TMA."""
+    low = stack(6, rows, 64, 16, torch.bfloat16, 21)
+    ids = ids_of([(i % 7 - 1 if len(lengths) > 1 else 1, n) for i, n in enumerate(lengths)])
+    x, base = inputs(ids.numel(), 64, sum(rows), torch.bfloat16, out_dtype, 22)
+    want, tol = plain(x, low, ids, base)
+    got = _ops().low_rank(x, low, ids, base=base, singles=0)
+    check(got, want, tol)
+    none = ids < 0
+    assert torch.equal(got[none], base[none])
+    for _ in range(3):
+        again = _ops().low_rank(x, low, ids, base=base, singles=0)
+        assert torch.equal(again, got)
+    _ops().check_tc_errors()
