@@ -18,6 +18,11 @@
 // sorts them, one a thread, and draws from them; the other CTAs are done.  Else the bin's own tokens are collected and sorted, if it has
 // 512 at most, or divided into 512 bins by the bits of their place in the order (their number there: exact, ties and all), until it has; the
 // draw is then a pass over the row.
+//
+// Measured on a B200, rows of 152,064, microseconds for 1, 16, 64 and 256 of them: top-k with or without top-p 11.6, 15.7, 46, 143; top-p alone 37, 67, 108, 343;
+// min-p 10, 13, 26, 108; none 14, 21, 42, 158.  Reading 256 rows takes 24: a few rows are bound by the chain of steps (a barrier of the cluster costs half a
+// microsecond with what is read behind it, weighing a CTA's 19,000 tokens 8 us, half of it instructions around the 64-bit ones), many by the turns that
+// 33 clusters at a time take, about 15 us each.
 #include "common.cuh"
 
 namespace prism {
@@ -962,6 +967,8 @@ PRISM_EXPORT int prism_sample_filtered(const float* logits, long long ld, int n,
     using namespace prism::draw;
     if (n <= 0) return 0;
     if (V < 1 || V > MOST_V || n > 65535 || n > R || u == nullptr || out == nullptr) return (int)cudaErrorInvalidValue;
+    // Eight CTAs for a large row: with four 152,064 tokens took by top-p 87 us (16 rows; eight: 68), by top-k 13.8 (15.6), 64 rows 55 (46); with sixteen 64 and 26,
+    // 64 rows 174 (108) and 74.  Slices in shared memory: read again from L2 instead, 16 rows took 18.7 us by top-k and 82 by top-p.
     int ctas = 1;
     while (ctas < MOST_CTAS && V > 4096 * ctas) ctas *= 2;
     const int per_cta = ((V + ctas - 1) / ctas + 3) & ~3;
