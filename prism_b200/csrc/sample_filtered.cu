@@ -19,7 +19,7 @@
 // 512 at most, or divided into 512 bins by the bits of their place in the order (their number there: exact, ties and all), until it has; the
 // draw is then a pass over the row.
 //
-// Measured on a B200, rows of 152,064, microseconds for 1, 16, 64 and 256 of them: top-k with or without top-p 11.6, 15.7, 46, 143; top-p alone 37, 67, 108, 343;
+// Measured on a B200, rows of 152,064, microseconds for 1, 16, 64 and 256 of them: top-k with or without top-p 11.6, 15.7, 46, 143; top-p alone 36, 66, 104, 328;
 // min-p 10, 13, 26, 108; none 14, 21, 42, 158.  Reading 256 rows takes 24: a few rows are bound by the chain of steps (a barrier of the cluster costs half a
 // microsecond with what is read behind it, weighing a CTA's 19,000 tokens 8 us, half of it instructions around the 64-bit ones), many by the turns that
 // 33 clusters at a time take, about 15 us each.
@@ -114,7 +114,7 @@ struct Shared {
     // the row
     const float* x;                            // the CTA's slice
     double top, per, deepest, one;             // largest logit; log2(e) / T; depth of min_p; a weight of 1 as a whole number: 2^46, or less where V of them would not fit
-    float floor;                               // tokens below have no weight: it would be less than 2^-1000
+    float floor;                               // tokens below have no weight: it would be less than 2^-999
     float p, u;
     int n, c0, ctas, me, k, bits, row;
     bool endless;                              // the largest is +infinity: such logits share the probability, as if they were 0 and the others masked
@@ -141,18 +141,20 @@ __device__ __noinline__ uint32_t team_reduce(uint32_t v, bool max, int turn) {
     team_barrier();
     return warp_all(lane < sh.ctas ? read_peer(&sh.part32[turn], lane) : 0, max);
 }
-__device__ __forceinline__ double team_sum(double v, int turn) {
+// A weight and a number at once
+__device__ __forceinline__ void team_sum(double& v, uint32_t& n, int turn) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    v = warp_sum64(v);
-    if (lane == 0) sh.slot[turn][warp] = bits_of(v);
+    v = warp_sum64(v), n = warp_all(n, false);
+    if (lane == 0) sh.slot[turn][warp] = bits_of(v), sh.slot32[turn][warp] = n;
     __syncthreads();
     of_bits(lane < WARPS ? sh.slot[turn][lane] : 0, v);
-    v = warp_sum64(v);
-    if (sh.ctas == 1) return v;
-    if (threadIdx.x == 0) sh.part[turn][0] = bits_of(v);
+    v = warp_sum64(v), n = warp_all(lane < WARPS ? sh.slot32[turn][lane] : 0, false);
+    if (sh.ctas == 1) return;
+    if (threadIdx.x == 0) sh.part[turn][0] = bits_of(v), sh.part32[turn] = n;
     team_barrier();
     of_bits(lane < sh.ctas ? read_peer(&sh.part[turn][0], lane) : 0, v);
-    return warp_sum64(v);
+    n = lane < sh.ctas ? read_peer(&sh.part32[turn], lane) : 0;
+    v = warp_sum64(v), n = warp_all(n, false);
 }
 // Sums over the threads up to this one; `all`: over all of them.  Every thread passes two barriers.
 __device__ __forceinline__ uint32_t scan32(uint32_t v, uint32_t& all) {
@@ -179,23 +181,16 @@ template <typename W> __device__ __noinline__ W scan64(W v) {
     __syncthreads();
     if (lane == 31) sh.scanned[warp] = bits_of(v);
     __syncthreads();
-    W before = 0, t;
-#pragma unroll 1
-    for (int w = 0; w < warp; ++w) {
-        of_bits(sh.scanned[w], t);
-        before += t;
-    }
-    return before + v;
+    W t;
+    of_bits(lane < warp ? sh.scanned[lane] : 0, t);                // 0 is zero of either kind
+    return warp_sum64(t) + v;
 }
 // after a scan64: what it is for the last thread
 template <typename W> __device__ __forceinline__ W scanned_all() {
-    W all = 0, t;
-#pragma unroll 1
-    for (int w = 0; w < WARPS; ++w) {
-        of_bits(sh.scanned[w], t);
-        all += t;
-    }
-    return all;
+    const int lane = threadIdx.x & 31;
+    W t;
+    of_bits(lane < WARPS ? sh.scanned[lane] : 0, t);
+    return warp_sum64(t);
 }
 
 // One number a thread, the largest first.  Only the first `n` threads hold any; the others hold 0 and get 0.
@@ -535,9 +530,9 @@ template <bool RESIDENT> __device__ __noinline__ u64 search(bool by_weight, u64 
         } else {
             fill_first<RESIDENT, false>(tail, tail_n);
         }
-        // the barriers of these sums are those of the bins
-        if (by_weight && level == 0) tail = team_sum(tail, turn ^= 1);
-        tail_n = team_reduce(tail_n, false, turn ^= 1);
+        // the barrier of these sums is that of the bins
+        if (by_weight && level == 0) team_sum(tail, tail_n, turn ^= 1);
+        else tail_n = team_reduce(tail_n, false, turn ^= 1);
         uint32_t in, n_all;
         double w_in = 0, w_all = 0, w_upto = 0;
         if (by_weight) {
@@ -927,7 +922,7 @@ sample_filtered_kernel(const float* __restrict__ logits_, long long ld, int R, i
     }
     if (tid == 0) {
         sh.top = (double)top;
-        sh.floor = fmaxf(LEAST, __double2float_ru((double)top - 1000.0 / sh.per));           // at an infinite temperature all but -infinity count
+        sh.floor = fmaxf(LEAST, __double2float_ru((double)top - 693.0 * (double)T));           // at an infinite temperature all but -infinity count
     }
     __syncthreads();
     // min_p as the lowest value that it keeps
