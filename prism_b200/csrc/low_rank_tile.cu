@@ -796,10 +796,12 @@ PRISM_EXPORT int prism_low_rank_tile(const void* x, long long ldx, const void* a
     int cols = 32;
     while (cols < H) cols *= 2;
     // All of a CTA's memory for copies in flight, or a half of an SM's: of clusters of eight CTAs with an SM each, 15 run at a time on 148 SMs, with half of one 33
-    // (2,048 tokens, 16 tiles: 107 -> 97 us).  The CTAs that fit an SM have tensor memory side by side, as a cluster's wait for each other.
+    // (2,048 tokens, 16 tiles, down projection of the 7B shape: 55 -> 35 us).
+    // CTAs of this kernel that fit an SM have tensor memory side by side, as a cluster's wait for each other: of any two calls, on whatever streams.  None
+    // has less than 68 KB (its sums), so that beside one with 512 columns there is no other, and of three one at most has 256.
     const int budget = tiles * CTAS > sms * 5 / 6 ? 104 * 1024 : 198 * 1024;
     const int stages = max(2, min(6, budget / stage));
-    const size_t smem = max(1024 + (size_t)max(stages * stage, sums), (size_t)228 * 1024 / (512 / cols + 1) + 1);
+    const size_t smem = max(1024 + max(stages * stage, sums), cols > 256 ? 160 * 1024 : cols > 128 ? 80 * 1024 : 0);
     prism::open_smem(low_rank_hidden_kernel, smem);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(CTAS, tiles);

@@ -318,3 +318,20 @@ def test_wide_results_of_many_tokens(out_dtype, rows, lengths):
         again = _ops().low_rank(x, low, ids, base=base, singles=0)
         assert torch.equal(again, got)
     _ops().check_tc_errors()
+
+
+@pytest.mark.parametrize("rows,rank", [((64, 130), 64), ((200, 64, 64, 8), 64), ((64, 40, 200), 128), ((16,) * 8, 64), ((72,) * 4, 128), ((128,), 16)], ids=str)
+@pytest.mark.parametrize("T", [1900, 2200, 5000])
+def test_hidden_values_of_many_tiles(rows, rank, T):
+    """Up to 512 hidden values a token, more clusters than run at a time, one and two CTAs an SM; calls behind each other, with tiles of several adapters."""
+    ops = _ops()
+    low = stack(5, rows, 320, rank, torch.bfloat16, 31)
+    x, base = inputs(T, 320, sum(rows), torch.bfloat16, torch.float32, 32)
+    at = torch.arange(T, device=DEV)
+    several = [(at * 7 // T - 1).clamp(max=4).int(), (at // 50 % 6 - 1).int(), torch.zeros_like(at).int()]
+    outs = [ops.low_rank(x, low, ids, base=base, singles=0) for _ in range(4) for ids in several]
+    for i, ids in enumerate(several):
+        check(outs[i], *plain(x, low, ids, base))
+        for other in outs[i + 3::3]:
+            assert torch.equal(outs[i], other)
+    ops.check_tc_errors()
