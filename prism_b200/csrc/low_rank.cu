@@ -8,7 +8,7 @@
 // Here, on CUDA cores: decoding requests, each with an adapter of its own, where every byte of A and B is used once and the kernel is bound by
 // reading them; and portions of prompts in 32-bit floats, or of sizes that TMA does not take.  low_rank_tile.cu has the portions on tensor cores.
 //
-// Decoding: a cluster of eight CTAs takes one token and a range of one slice's columns; each computes an eighth of the hidden values over the whole K
+// Decoding: a cluster of up to eight CTAs takes one token and a range of one slice's columns; each computes its share of the hidden values over the whole K
 // and writes them into all CTAs' shared memory, then all have the hidden vector and share the columns.  So it is one launch, no sum crosses
 // CTAs, and B's first 16 or 32 KB a CTA and the results that they are added to are asked for before the hidden values are waited for.  A thread has two
 // 16-byte chunks of a row of B: with one each, and four rows ahead, registers were spilled and an instruction in two was not arithmetic (64 tokens, gate and up
@@ -22,7 +22,7 @@
 namespace prism {
 namespace lowrank {
 
-constexpr int CTAS = 8;                       // of a cluster
+constexpr int CTAS = 8;                       // of a cluster that shares K, and of one token's at most
 constexpr int AHEAD = 2, EACH = 2;            // rows of B in flight a thread, and its 16-byte chunks of each
 constexpr int MOST_RANK = 128, MOST_SLICES = 8;
 
@@ -71,11 +71,12 @@ __device__ __forceinline__ uint32_t rank_in_cluster() {
 
 // ---- one token ----------------------------------------------------------------------------------------------
 
-// Three of it, by the clusters of a launch.  512 threads and an SM's registers, eight loads of A in flight a thread, where all clusters run at a time so
+// Five forms of it, by the clusters of a launch.  512 threads and an SM's registers, eight loads of A in flight a thread, where all clusters run at a time so
 // (15 on 148 SMs, as a cluster's CTAs are neighbours) or nearly.  512 threads and half an SM's registers up to 33 clusters; else 256 threads, four CTAs an SM, whose
-// waits overlap.  Microseconds of the three (bfloat16, the 7B shape, an adapter a token): down projection of rank 64, 4 tokens 8.4, 10.8, 15.2; 24 tokens
-// 19.9, 20.0, 28.8; gate and up of rank 16, 16 tokens 14.7, 9.4, 12.0; 64 tokens 57, 42, 32.
-template <typename T, typename O, int THREADS, int PER_SM>
+// waits overlap: clusters of eight up to 71 of them, of four up to 142, of two.  Microseconds (bfloat16, the 7B shape, an adapter a token): down projection of rank 64,
+// by the first three forms, 4 tokens 8.4, 10.8, 15.2; 24 tokens 19.9, 20.0, 28.8; gate and up of rank 16, 16 tokens 14.7, 9.4, 12.0; 64 tokens 57, 42, 32, in clusters
+// of four 30; q, k and v of rank 16 in clusters of eight, four and two, 32 tokens 11.5, 8.9, -, 64 tokens 18.4, 14.0, 11.9, 128 tokens 47, 22, 17.
+template <typename T, typename O, int THREADS, int PER_SM, int CTAS>
 __global__ void __launch_bounds__(THREADS, PER_SM)
 low_rank_token_kernel(const T* __restrict__ x_, long long ldx, int x_whole, const T* __restrict__ a, const T* __restrict__ b,
                       const float* __restrict__ scale, const int* __restrict__ ids_, const O* __restrict__ base_, long long ldb, O* out_, long long ldo,
@@ -214,7 +215,7 @@ int launch_tokens(const void* x, long long ldx, const void* a, const void* b, co
     // Clusters at a time with an SM a CTA, and with half of one.  Up to 18 are launched in the first form all the same: rows without an adapter (of a captured
     // step that has fewer requests than rows, say) are over at once.  16 tokens, down projection of rank 64: 17.3 us, in the second form 16.0; if one of them
     // has none 10.9 and 16.3.
-    const int wholes = sms / CTAS * 5 / 6, halves = sms * 9 / (CTAS * 5), first_form = sms / CTAS;
+    const int wholes = sms / CTAS * 5 / 6, halves = sms * 9 / (CTAS * 5), first_form = sms / CTAS, quarters = sms * 12 / 25;
     // clusters that share a slice's columns, each with hidden values of its own: as many as keep B's part of a CTA within what it asks for ahead, while
     // all run at a time
     int widest = 0;
@@ -223,18 +224,24 @@ int launch_tokens(const void* x, long long ldx, const void* a, const void* b, co
     const int parts = (int)max(1ll, min((bytes + ahead - 1) / ahead, (long long)wholes / ((long long)s.n * tokens)));
     const int whole = (reinterpret_cast<uintptr_t>(x) % 16 == 0) && (ldx * (long long)sizeof(T) % 16 == 0 || tokens == 1);
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(CTAS, s.n * parts, tokens);
+    // the form: kernel, its threads and its clusters' size together
     const int clusters = s.n * parts * tokens;
-    cfg.blockDim = dim3(clusters <= halves ? 512 : 256);
+    auto kernel = low_rank_token_kernel<T, O, 256, 4, 2>;
+    int threads = 256, ctas = 2;
+    if (clusters <= first_form) kernel = low_rank_token_kernel<T, O, 512, 1, 8>, threads = 512, ctas = 8;
+    else if (clusters <= halves) kernel = low_rank_token_kernel<T, O, 512, 2, 8>, threads = 512, ctas = 8;
+    else if (clusters <= quarters) kernel = low_rank_token_kernel<T, O, 256, 4, 8>, ctas = 8;
+    else if (clusters <= 2 * quarters) kernel = low_rank_token_kernel<T, O, 256, 4, 4>, ctas = 4;
+    cfg.gridDim = dim3(ctas, s.n * parts, tokens);
+    cfg.blockDim = dim3(threads);
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = CTAS, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
+    attr[0].val.clusterDim.x = ctas, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = prism::pdl_enabled() ? 2 : 1;
-    const auto kernel = clusters <= first_form ? low_rank_token_kernel<T, O, 512, 1> : clusters <= halves ? low_rank_token_kernel<T, O, 512, 2> : low_rank_token_kernel<T, O, 256, 4>;
     return (int)cudaLaunchKernelEx(&cfg, kernel, (const T*)x, ldx, whole, (const T*)a, (const T*)b, scale, ids, (const O*)base, ldb, (O*)out,
                                    ldo, K, Kp, r, L, s, parts, err);
 }

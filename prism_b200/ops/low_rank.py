@@ -175,10 +175,11 @@ def low_rank(x: torch.Tensor, low: LowRank, ids: torch.Tensor, base: Optional[to
     bf16, out16 = dt is torch.bfloat16, odt is torch.bfloat16
     xp, x_row, ip, op, o_row = x.data_ptr(), x.stride(0), ids.data_ptr(), out.data_ptr(), out.stride(0)
     basep, b_row = (None, 0) if base is None else (base.data_ptr(), base.stride(0))
-    G = len(low.rows)
-    tiles = bf16 and xp % 16 == 0 and x_row % 8 == 0 and x_row >= low.k and L.prism_low_rank_tile_supported(low.k, low.rank, G, True)
-    if T - singles < (TILE_FROM if tiles else PLAIN_TILE_FROM):
-        singles = T
+    G, tiles = len(low.rows), False
+    if singles < T:
+        tiles = bf16 and xp % 16 == 0 and x_row % 8 == 0 and x_row >= low.k and L.prism_low_rank_tile_supported(low.k, low.rank, G, True)
+        if T - singles < (TILE_FROM if tiles else PLAIN_TILE_FROM):
+            singles = T
     if singles:
         ops._check(L.prism_low_rank(xp, x_row, bf16, ap, bp, sp, ip, basep, b_row, op, o_row, out16, singles, *sizes, None, sms, err, stream), "low_rank")
     rest = T - singles
