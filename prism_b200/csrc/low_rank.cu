@@ -212,10 +212,11 @@ int launch_tokens(const void* x, long long ldx, const void* a, const void* b, co
                   long long ldo, int tokens, int K, int Kp, int r, int L, const Slices& s, int* err, int sms, cudaStream_t stream) {
     if (tokens <= 0) return 0;
     if (tokens > 65535) return (int)cudaErrorInvalidValue;
-    // Clusters at a time with an SM a CTA, and with half of one.  Up to 18 are launched in the first form all the same: rows without an adapter (of a captured
-    // step that has fewer requests than rows, say) are over at once.  16 tokens, down projection of rank 64: 17.3 us, in the second form 16.0; if one of them
-    // has none 10.9 and 16.3.
-    const int wholes = sms / CTAS * 5 / 6, halves = sms * 9 / (CTAS * 5), first_form = sms / CTAS, quarters = sms * 12 / 25;
+    // Clusters at a time with an SM a CTA, with half of one and with a quarter.  Where a CTA has much of A, up to 18 are launched in the first form all the same: rows
+    // without an adapter (of a captured step that has fewer requests than rows, say) are over at once.  16 tokens, down projection, 303 KB of A a CTA: 17.3 us, in
+    // the second form 16.0; if one of them has none 10.9 and 16.3.  With 76 KB it is 9.7 and 8.1, with 14 KB 7.7 and 6.1, whoever has none.
+    const int wholes = sms / CTAS * 5 / 6, halves = sms * 9 / (CTAS * 5), quarters = sms * 12 / 25;
+    const int first_form = (long long)r / CTAS * Kp * (int)sizeof(T) >= 128 * 1024 ? sms / CTAS : wholes;
     // clusters that share a slice's columns, each with hidden values of its own: as many as keep B's part of a CTA within what it asks for ahead, while
     // all run at a time
     int widest = 0;
