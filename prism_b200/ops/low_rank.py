@@ -136,10 +136,10 @@ def in_use(w):
 SINGLES = 64                 # without a word from the caller, so many tokens are taken one by one
 # So many tokens of portions, and they are taken in tiles: of 128 on tensor cores, or of 32 on CUDA cores (32-bit floats, sizes that TMA does not
 # take); fewer one by one.  Microseconds one by one and in tiles, all tokens of one adapter, for gate and up (rank 16), q k v (32) and down (64) of the 7B shape:
-# bfloat16, 32 tokens 13.5/17.3, 14.6/16.7, 23.9/27.2; 64 tokens 24.2/17.8, 23.7/17.0, 29.9/27.5 (two adapters a tile cost the tiles a half more).
-# float32, 64 tokens 28/46, 24/44, 32/194; 128 tokens 51/54, 45/44, 63/194; 512 tokens 200/85 (gate and up).
+# bfloat16, 48 tokens 21.9/17.6, 16.3/17.8, 28.9/28.3; 96 tokens 37.5/18.2, 21.3/18.2, 52.4/28.7 (two adapters a tile cost the tiles a half more).
+# float32, 128 tokens 43/54, 35/44, 60/193; 192 tokens 72/61, 44/80, 112/196; 256 tokens 99/106, 57/81, 115/197; 512 tokens 200/85 (gate and up).
 TILE_FROM = 48
-PLAIN_TILE_FROM = 128
+PLAIN_TILE_FROM = 256
 
 
 def low_rank(x: torch.Tensor, low: LowRank, ids: torch.Tensor, base: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
