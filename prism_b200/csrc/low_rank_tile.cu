@@ -11,8 +11,8 @@
 // result in 48): 4.4 TB/s.  A launch that only passes boxes through takes 59: what bounds it is how fast an SM's share comes and goes.  Beside it a tile
 // of 128 x 128 moves 208 KB through shared memory, 1,600 cycles at 128 bytes a cycle of some 3,600.
 //
-// A tile's tokens may have several adapters, or some of them none.  The first launch goes through it once for each adapter; the second has up to four
-// adapters' products side by side in tensor memory.  With more than four, or where base and out are no place for TMA, it goes through the tile
+// A tile's tokens may have several adapters, or some of them none.  Up to four adapters' products lie side by side in tensor memory (in the first launch as many
+// as have 256 hidden values together, and it goes through the tile again for the next).  With more than four, or where base and out are no place for TMA, it goes through the tile
 // once for each adapter, and the threads store that adapter's rows.
 #include "tcgen05.cuh"
 #include "vec.cuh"
@@ -26,6 +26,7 @@ constexpr int BLOCK_BYTES = TILE * TILE_K * 2;
 constexpr int CTAS = 8;                       // that share a tile's K
 constexpr int EPI_WARPS = 8, EPI_THREADS = EPI_WARPS * 32, ALL_THREADS = EPI_THREADS + 64;
 constexpr int MOST_RANK = 128, MOST_SLICES = 8, MOST_HIDDEN = 512;
+constexpr int HIDDEN_STAGES = 6;
 constexpr int CHUNK = 64, CHUNK_LD = CHUNK + 4;                   // columns of sums on their way through shared memory, and their pitch
 constexpr int WIDE = 128, WIDE_LD = WIDE + 4;                     // the same of hidden values
 
@@ -81,13 +82,13 @@ __device__ __forceinline__ void epilogue_barrier() { asm volatile("bar.sync 1, %
 // hidden: [tokens][2][G r], high terms and low ones; adapters: how many a tile has
 __global__ void __launch_bounds__(ALL_THREADS)
 low_rank_hidden_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_a, const float* __restrict__ scale,
-                       const int* __restrict__ ids_, __nv_bfloat16* __restrict__ hidden, int* __restrict__ adapters, int tokens, int K, int r, int G, int L, int stages,
-                       int tmem_cols, int* err) {
+                       const int* __restrict__ ids_, __nv_bfloat16* __restrict__ hidden, int* __restrict__ adapters, int tokens, int K, int r, int G, int L, int ring_bytes,
+                       int most_adapters, int tmem_cols, int* err) {
     extern __shared__ unsigned char raw[];
     unsigned char* ring = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
-    const int H = G * r, stage_bytes = BLOCK_BYTES + H * TILE_K * 2;
+    const int H = G * r;
     float* sums = reinterpret_cast<float*>(ring);                  // behind a pass's last product, its sums; there is memory for as many at least
-    __shared__ uint64_t full[8], empty[8], done;
+    __shared__ uint64_t full[HIDDEN_STAGES], empty[HIDDEN_STAGES], done;
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_flag, own[TILE], list[TILE], count;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, me = blockIdx.x, t0 = blockIdx.y * TILE;
@@ -97,7 +98,7 @@ low_rank_hidden_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_c
     if (threadIdx.x == 0) {
         prefetch_map(&map_x), prefetch_map(&map_a);
         abort_flag = 0;
-        for (int s = 0; s < stages; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+        for (int s = 0; s < HIDDEN_STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
         mbar_init(&done, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -115,10 +116,12 @@ low_rank_hidden_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_c
     if (me == 0 && threadIdx.x == 0) adapters[blockIdx.y] = passes;
     pdl_trigger();                            // not before this CTA has its tensor memory: the next kernel may take the rest and wait
 
+    // Up to most_adapters at a time: their products with a block of x lie side by side in tensor memory, a row has its own.
+    const int side = min(passes, most_adapters), stage_bytes = BLOCK_BYTES + side * H * TILE_K * 2, stages = side > 0 ? min(HIDDEN_STAGES, ring_bytes / stage_bytes) : 1;
     int it = 0;                               // blocks so far, over all passes
     bool go = true;                           // no wait of this warp has run out
-    for (int p = 0; p < passes; ++p) {
-        const int l = list[p];
+    for (int first = 0, p = 0; first < passes; first += side, ++p) {
+        const int adapters_now = min(side, passes - first);
         if (warp == 0) {
             if (lane == 0 && !*abortp) {
                 int issued = 0;
@@ -126,11 +129,12 @@ low_rank_hidden_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_c
                     const int s = (it + i) % stages, round = (it + i) / stages;
                     if (round > 0 && !mbar_wait(&empty[s], (round - 1) & 1, abortp)) break;
                     unsigned char* st = ring + (size_t)s * stage_bytes;
-                    mbar_expect_tx(&full[s], stage_bytes);
+                    mbar_expect_tx(&full[s], BLOCK_BYTES + adapters_now * H * TILE_K * 2);
                     const int k = (me + i * CTAS) * TILE_K;
                     tma_load_2d(st, &map_x, &full[s], k, t0);
-                    for (int g = 0; g < G; ++g)
-                        tma_load_2d(st + BLOCK_BYTES + (size_t)g * r * TILE_K * 2, &map_a, &full[s], k, (l * G + g) * r);
+                    for (int b = 0; b < adapters_now; ++b)
+                        for (int g = 0; g < G; ++g)
+                            tma_load_2d(st + BLOCK_BYTES + (b * H + g * r) * TILE_K * 2, &map_a, &full[s], k, (list[first + b] * G + g) * r);
                     issued = i + 1;
                 }
                 if (*abortp)
@@ -147,12 +151,11 @@ low_rank_hidden_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_c
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                     const uint32_t st = smem_addr(ring + (size_t)s * stage_bytes);
                     const uint64_t dx = umma_desc(st);
-                    for (int g = 0; g < G; ++g) {
-                        // a slice's rows start on 8 rows of 128 bytes, as r is a multiple of 16
-                        const uint64_t da = umma_desc(st + BLOCK_BYTES + g * r * TILE_K * 2);
+                    for (int row = 0; row < adapters_now * H; row += r) {          // a slice's rows start on 8 rows of 128 bytes, as r is a multiple of 16
+                        const uint64_t da = umma_desc(st + BLOCK_BYTES + row * TILE_K * 2);
 #pragma unroll
                         for (int k = 0; k < TILE_K / UMMA_K; ++k)
-                            umma_bf16(tmem + g * r, dx + (uint64_t)(k * UMMA_K * 2 >> 4), da + (uint64_t)(k * UMMA_K * 2 >> 4), idesc, (i > 0 || k > 0) ? 1u : 0u);
+                            umma_bf16(tmem + row, dx + (uint64_t)(k * UMMA_K * 2 >> 4), da + (uint64_t)(k * UMMA_K * 2 >> 4), idesc, (i > 0 || k > 0) ? 1u : 0u);
                     }
                     umma_commit(&empty[s]);
                 }
@@ -168,6 +171,11 @@ low_rank_hidden_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_c
             if (mine > 0) go = __all_sync(0xffffffffu, mbar_wait(&done, p & 1, abortp)) && go;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         }
+        int which = -1;                       // this row's adapter among these
+        if (warp >= 2)
+            for (int b = 0; b < adapters_now; ++b)
+                if (own[q * 32 + lane] == list[first + b]) which = b;
+        const uint32_t present = __reduce_or_sync(0xffffffffu, which < 0 ? 0u : 1u << which);
         for (int c0 = 0; c0 < H; c0 += WIDE) {
             if (warp >= 2) {
                 // this CTA's sums: a thread's row is its tensor memory lane
@@ -176,12 +184,17 @@ low_rank_hidden_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_c
                     const int at = m * 64 + half * 32;
                     if (c0 + at >= H) break;
                     float v[32];
-                    if (mine > 0 && go) {
-                        tmem_load<32>(tmem + ((uint32_t)(q * 32) << 16) + c0 + at, v);       // columns beyond H are allocated, and not used
-                    } else {
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) v[i] = 0.f;
-                    }
+                    for (int i = 0; i < 32; ++i) v[i] = 0.f;
+                    if (mine > 0 && go)
+#pragma unroll 1
+                        for (int b = 0; b < adapters_now; ++b) {
+                            if (!(present >> b & 1)) continue;
+                            float w[32];
+                            tmem_load<32>(tmem + ((uint32_t)(q * 32) << 16) + b * H + c0 + at, w);         // columns beyond H are allocated, and not used
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) v[i] = which == b ? w[i] : v[i];
+                        }
                     float* row = sums + (q * 32 + lane) * WIDE_LD + at;
 #pragma unroll
                     for (int i = 0; i < 32; i += 4) *reinterpret_cast<float4*>(row + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
@@ -193,7 +206,10 @@ low_rank_hidden_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_c
                 const int wide = min(WIDE, H - c0) / 4;
                 for (int e = tid; e < TILE / CTAS * wide; e += EPI_THREADS) {
                     const int row = me * (TILE / CTAS) + e / wide, c = e % wide * 4, t = t0 + row;
-                    if (own[row] != l || !go) continue;
+                    int l = -1;
+                    for (int b = 0; b < adapters_now; ++b)
+                        if (own[row] == list[first + b]) l = own[row];
+                    if (l < 0 || !go) continue;
                     const uint32_t at = smem_addr(sums + row * WIDE_LD + c);
                     float4 part[CTAS];
 #pragma unroll
@@ -792,16 +808,17 @@ PRISM_EXPORT int prism_low_rank_tile(const void* x, long long ldx, const void* a
     if (code == 0) code = prism::tc::make_map(&map_b, b, (long long)L * N, r, r, TILE);
     if (code != 0) return code;
 
-    const int stage = BLOCK_BYTES + H * prism::tc::TILE_K * 2, sums = TILE * WIDE_LD * 4;
+    const int most = max(1, min(4, 256 / H)), sums = TILE * WIDE_LD * 4;           // adapters side by side: in half of tensor memory
+    const int least = 2 * (BLOCK_BYTES + most * H * prism::tc::TILE_K * 2);
     int cols = 32;
-    while (cols < H) cols *= 2;
+    while (cols < most * H + H % 32) cols *= 2;         // sums are read 32 columns at a time
     // All of a CTA's memory for copies in flight, or a half of an SM's: of clusters of eight CTAs with an SM each, 15 run at a time on 148 SMs, with half of one 33
     // (2,048 tokens, 16 tiles, down projection of the 7B shape: 55 -> 35 us).
-    // CTAs of this kernel that fit an SM have tensor memory side by side, as a cluster's wait for each other: of any two calls, on whatever streams.  None
-    // has less than 68 KB (its sums), so that beside one with 512 columns there is no other, and of three one at most has 256.
+    // CTAs of this kernel that fit an SM have tensor memory side by side, as a cluster's wait for each other: of any two calls, on whatever streams.  None has
+    // less than 105 KB, so that there are two at most, of 256 columns, and beside one with 512 columns there is no other.
     const int budget = tiles * CTAS > sms * 5 / 6 ? 104 * 1024 : 198 * 1024;
-    const int stages = max(2, min(6, budget / stage));
-    const size_t smem = max(1024 + max(stages * stage, sums), cols > 256 ? 160 * 1024 : cols > 128 ? 80 * 1024 : 0);
+    const int ring = max(max(budget, least), sums);
+    const size_t smem = max(1024 + ring, cols > 256 ? 160 * 1024 : 0);
     prism::open_smem(low_rank_hidden_kernel, smem);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(CTAS, tiles);
@@ -815,7 +832,7 @@ PRISM_EXPORT int prism_low_rank_tile(const void* x, long long ldx, const void* a
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = prism::pdl_enabled() ? 2 : 1;
-    code = (int)cudaLaunchKernelEx(&cfg, low_rank_hidden_kernel, map_x, map_a, scale, ids, (bf16*)hidden, adapters, T, K, r, G, L, stages, cols, err);
+    code = (int)cudaLaunchKernelEx(&cfg, low_rank_hidden_kernel, map_x, map_a, scale, ids, (bf16*)hidden, adapters, T, K, r, G, L, ring, most, cols, err);
     if (code != 0) return code;
 
     if (out_dtype == PRISM_DTYPE_F32) return launch_results<float>(hidden, adapters, map_b, ids, base, ldb, out, ldo, T, r, L, s, err, sms, stream);
