@@ -7,7 +7,7 @@
 // and up for 2,048 tokens are 310 MB against 28 MB of everything else.  So the shared result comes and goes by TMA, boxes of 128 rows by 128 bytes, eight
 // of them on their way or at work, and a thread adds its row's sums where they lie in shared memory.
 //
-// Measured for that, rank 64, one adapter: 16 us for the hidden values and 71 for the results on their own, 76 together (the floor is 52; torch copies the shared
+// Measured for that, rank 64, one adapter: 17 us for the hidden values and 70 for the results on their own, 77 together (the floor is 52; torch copies the shared
 // result in 48): 4.4 TB/s.  A launch that only passes boxes through takes 59: what bounds it is how fast an SM's share comes and goes.  Beside it a tile
 // of 128 x 128 moves 208 KB through shared memory, 1,600 cycles at 128 bytes a cycle of some 3,600.
 //
