@@ -80,7 +80,7 @@ template <typename T, typename O, int THREADS, int PER_SM, int CTAS>
 __global__ void __launch_bounds__(THREADS, PER_SM)
 low_rank_token_kernel(const T* __restrict__ x_, long long ldx, int x_whole, const T* __restrict__ a, const T* __restrict__ b,
                       const float* __restrict__ scale, const int* __restrict__ ids_, const O* __restrict__ base_, long long ldb, O* out_, long long ldo,
-                      int K, int Kp, int r, int L, Slices slices, int parts, int* err) {
+                      int K, int Kp, int r, int L, const __grid_constant__ Slices slices, int parts, int* err) {
     constexpr int E = Chunk<T>::E, WARPS = THREADS / 32;
     __shared__ float hidden[MOST_RANK];
     __shared__ float partial[MOST_RANK / CTAS][WARPS];             // a hidden value's share of a warp
@@ -107,10 +107,11 @@ low_rank_token_kernel(const T* __restrict__ x_, long long ldx, int x_whole, cons
     int lanes = 1;
     while (lanes * EACH < chunks) lanes *= 2;
     const int chunk = lane % lanes, rows_at_once = THREADS / lanes, row0 = tid / lanes;
-    bool holds[EACH];
+    // a part that is not there: the last one, with hidden values of zero
+    int part_at[EACH];
 #pragma unroll
-    for (int c = 0; c < EACH; ++c) holds[c] = chunk + c * lanes < chunks;
-    const T* B = b + ((size_t)l * N + n0) * r + chunk * E;
+    for (int c = 0; c < EACH; ++c) part_at[c] = min(chunk + c * lanes, chunks - 1) * E;
+    const T* B = b + ((size_t)l * N + n0) * r;
     uint4 ahead[AHEAD][EACH];
     O old[AHEAD];                                                  // as they lie in memory: to change their type is to wait for them
 #pragma unroll
@@ -118,7 +119,7 @@ low_rank_token_kernel(const T* __restrict__ x_, long long ldx, int x_whole, cons
         const int n = row0 + j * rows_at_once;
 #pragma unroll
         for (int c = 0; c < EACH; ++c)
-            ahead[j][c] = holds[c] && n < mine ? __ldg(reinterpret_cast<const uint4*>(B + (size_t)n * r + c * lanes * E)) : make_uint4(0, 0, 0, 0);
+            ahead[j][c] = n < mine ? __ldg(reinterpret_cast<const uint4*>(B + (size_t)n * r + part_at[c])) : make_uint4(0, 0, 0, 0);
         old[j] = chunk == 0 && n < mine && base ? base[n] : from_float<O>(0.f);
     }
     // an eighth of the hidden values, several warps a row where there are fewer rows than warps
@@ -179,7 +180,7 @@ low_rank_token_kernel(const T* __restrict__ x_, long long ldx, int x_whole, cons
 #pragma unroll
     for (int c = 0; c < EACH; ++c)
 #pragma unroll
-        for (int e = 0; e < E; ++e) h[c][e] = holds[c] ? hidden[(chunk + c * lanes) * E + e] : 0.f;
+        for (int e = 0; e < E; ++e) h[c][e] = chunk + c * lanes < chunks ? hidden[part_at[c] + e] : 0.f;
     const int pass = AHEAD * rows_at_once;
     const size_t step = (size_t)rows_at_once * r;
     const T* next = B + (size_t)(row0 + pass) * r;
@@ -194,7 +195,7 @@ low_rank_token_kernel(const T* __restrict__ x_, long long ldx, int x_whole, cons
             if (n + pass < mine) {
 #pragma unroll
                 for (int c = 0; c < EACH; ++c)
-                    if (holds[c]) ahead[i][c] = __ldg(reinterpret_cast<const uint4*>(next + c * lanes * E));
+                    ahead[i][c] = __ldg(reinterpret_cast<const uint4*>(next + part_at[c]));
                 if (chunk == 0 && base) old[i] = base[n + pass];
             }
 #pragma unroll
