@@ -12,7 +12,7 @@
 // and writes them into all CTAs' shared memory, then all have the hidden vector and share the columns.  So it is one launch, no sum crosses
 // CTAs, and B's first 16 or 32 KB a CTA and the results that they are added to are asked for before the hidden values are waited for.  A thread has two
 // 16-byte chunks of a row of B: with one each, and four rows ahead, registers were spilled and an instruction in two was not arithmetic (64 tokens, gate and up
-// of the 7B shape, rank 16: 40 us, so 32, 2.9 TB/s).  One token there takes 4.3 us, four of them launch, first loads and two barriers of the cluster.
+// of the 7B shape, rank 16: 40 us, so 32; without registers in memory 23, 4.1 TB/s).  One token there takes 4.3 us, four of them launch, first loads and two barriers of the cluster.
 //
 // Portions: 32 tokens at a time, hidden values (a cluster shares K, its sums meet through distributed shared memory) and results in a launch
 // each.  A tile's tokens may have several adapters: it is gone through once for each of them.  512 tokens of two adapters, gate and up, rank 16, in float32: 85 us,
@@ -71,11 +71,12 @@ __device__ __forceinline__ uint32_t rank_in_cluster() {
 
 // ---- one token ----------------------------------------------------------------------------------------------
 
-// Five forms of it, by the clusters of a launch.  512 threads and an SM's registers, eight loads of A in flight a thread, where all clusters run at a time so
-// (15 on 148 SMs, as a cluster's CTAs are neighbours) or nearly.  512 threads and half an SM's registers up to 33 clusters; else 256 threads, four CTAs an SM, whose
-// waits overlap: clusters of eight up to 71 of them, of four up to 142, of two.  Microseconds (bfloat16, the 7B shape, an adapter a token): down projection of rank 64,
-// by the first three forms, 4 tokens 8.4, 10.8, 15.2; 24 tokens 19.9, 20.0, 28.8; gate and up of rank 16, 16 tokens 14.7, 9.4, 12.0; 64 tokens 57, 42, 32, in clusters
-// of four 30; q, k and v of rank 16 in clusters of eight, four and two, 32 tokens 11.5, 8.9, -, 64 tokens 18.4, 14.0, 11.9, 128 tokens 47, 22, 17.
+// Forms of it, by the clusters of a launch, as a cluster's CTAs are neighbours and so many run at a time.  512 threads and an SM's registers, eight loads of A in
+// flight a thread: 15 clusters on 148 SMs.  512 threads and half of them, where a CTA has much of A: 33.  Else 256 threads, three or four CTAs an SM (whose registers
+// are short by ten: they spill outside the loops), in clusters of eight, four and two: the fewest CTAs an SM that run at a time.  Microseconds (bfloat16, the 7B shape,
+// an adapter a token): down projection of rank 64, by the first two forms and the third of eight, 4 tokens 8.4, 10.8, 15.2; 24 tokens 19.9, 17.8, 22.9; q, k and v of
+// rank 16, 12 tokens three an SM 4.8, four 5.9; 64 tokens in clusters of eight, four and two 18.4, 14.0, 8.1 (the first two as they were with registers in
+// memory); gate and up, 64 tokens four an SM 23.0, three 27.5, 96 tokens 35.9 and 26.5.
 template <typename T, typename O, int THREADS, int PER_SM, int CTAS>
 __global__ void __launch_bounds__(THREADS, PER_SM)
 low_rank_token_kernel(const T* __restrict__ x_, long long ldx, int x_whole, const T* __restrict__ a, const T* __restrict__ b,
@@ -213,11 +214,12 @@ int launch_tokens(const void* x, long long ldx, const void* a, const void* b, co
                   long long ldo, int tokens, int K, int Kp, int r, int L, const Slices& s, int* err, int sms, cudaStream_t stream) {
     if (tokens <= 0) return 0;
     if (tokens > 65535) return (int)cudaErrorInvalidValue;
-    // Clusters at a time with an SM a CTA, with half of one and with a quarter.  Where a CTA has much of A, up to 18 are launched in the first form all the same: rows
-    // without an adapter (of a captured step that has fewer requests than rows, say) are over at once.  16 tokens, down projection, 303 KB of A a CTA: 17.3 us, in
-    // the second form 16.0; if one of them has none 10.9 and 16.3.  With 76 KB it is 9.7 and 8.1, with 14 KB 7.7 and 6.1, whoever has none.
-    const int wholes = sms / CTAS * 5 / 6, halves = sms * 9 / (CTAS * 5), quarters = sms * 12 / 25;
-    const int first_form = (long long)r / CTAS * Kp * (int)sizeof(T) >= 128 * 1024 ? sms / CTAS : wholes;
+    // Clusters at a time with an SM a CTA, with half of one, a third and a quarter.  Where a CTA has much of A, up to 18 are launched in the first form all the same:
+    // rows without an adapter (of a captured step that has fewer requests than rows, say) are over at once.  16 tokens, down projection, 303 KB of A a CTA: 17.3 us,
+    // in the second form 16.0; if one of them has none 10.9 and 16.3.
+    const bool much = (long long)r / CTAS * Kp * (int)sizeof(T) >= 128 * 1024;
+    const int wholes = sms / CTAS * 5 / 6, halves = much ? sms * 9 / (CTAS * 5) : 0, thirds = sms * 9 / 25, quarters = sms * 12 / 25;
+    const int first_form = much ? sms / CTAS : wholes;
     // clusters that share a slice's columns, each with hidden values of its own: as many as keep B's part of a CTA within what it asks for ahead, while
     // all run at a time
     int widest = 0;
@@ -232,8 +234,11 @@ int launch_tokens(const void* x, long long ldx, const void* a, const void* b, co
     int threads = 256, ctas = 2;
     if (clusters <= first_form) kernel = low_rank_token_kernel<T, O, 512, 1, 8>, threads = 512, ctas = 8;
     else if (clusters <= halves) kernel = low_rank_token_kernel<T, O, 512, 2, 8>, threads = 512, ctas = 8;
+    else if (clusters <= thirds) kernel = low_rank_token_kernel<T, O, 256, 3, 8>, ctas = 8;
     else if (clusters <= quarters) kernel = low_rank_token_kernel<T, O, 256, 4, 8>, ctas = 8;
+    else if (clusters <= 2 * thirds) kernel = low_rank_token_kernel<T, O, 256, 3, 4>, ctas = 4;
     else if (clusters <= 2 * quarters) kernel = low_rank_token_kernel<T, O, 256, 4, 4>, ctas = 4;
+    else if (clusters <= 4 * thirds) kernel = low_rank_token_kernel<T, O, 256, 3, 2>, ctas = 2;
     cfg.gridDim = dim3(ctas, s.n * parts, tokens);
     cfg.blockDim = dim3(threads);
     cfg.stream = stream;
