@@ -136,9 +136,10 @@ def in_use(w):
 SINGLES = 64                 # without a word from the caller, so many tokens are taken one by one
 # So many tokens of portions, and they are taken in tiles: of 128 on tensor cores, or of 32 on CUDA cores (32-bit floats, sizes that TMA does not
 # take); fewer one by one.  Microseconds one by one and in tiles, all tokens of one adapter, for gate and up (rank 16), q k v (32) and down (64) of the 7B shape:
-# bfloat16, 48 tokens 21.9/17.6, 16.3/17.8, 28.9/28.3; 96 tokens 37.5/18.2, 21.3/18.2, 52.4/28.7 (two adapters a tile cost the tiles a half more).
-# float32, 128 tokens 43/54, 35/44, 60/193; 192 tokens 72/61, 44/80, 112/196; 256 tokens 99/106, 57/81, 115/197; 512 tokens 200/85 (gate and up).
-TILE_FROM = 48
+# bfloat16, 64 tokens 16.0/18.7, 13.1/19.1, 27.4/29.6; 96 tokens 17.3/18.9, 19.1/19.3, 35.5/29.9; 128 tokens 26.4/19.0, 25.3/19.7, 51.4/30.3 (two adapters a tile cost
+# the tiles a fifth more).  float32, 128 tokens 35/54, 33/44, 58/193; 192 tokens 63/61, 42/80, 91/196; 256 tokens 91/106, 54/80, 112/197; 512 tokens 200/85 (gate
+# and up).
+TILE_FROM = 96
 PLAIN_TILE_FROM = 256
 
 
