@@ -291,7 +291,7 @@ def test_one_row_for_all_tokens(T):
 
 @pytest.mark.parametrize("dtype,out_dtype", TYPES)
 @pytest.mark.parametrize("rows,K,rank", [((130, 65), 1003, 5), ((257,), 70, 100), ((96, 8, 40), 512, 128)])
-@pytest.mark.parametrize("lengths", [(47,), (48,), (127,), (128,), (1, 126), (40, 1, 90, 33, 160), (300, 200)], ids=str)
+@pytest.mark.parametrize("lengths", [(47,), (95,), (96,), (128,), (255,), (256,), (1, 126), (40, 1, 90, 33, 160), (300, 200)], ids=str)
 def test_portions_of_every_length(dtype, out_dtype, rows, K, rank, lengths):
     """On both sides of the lengths from which portions are taken in tiles; some have no adapter, some tiles several."""
     low = stack(3, rows, K, rank, dtype, 11)
