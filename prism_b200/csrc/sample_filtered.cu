@@ -3,7 +3,8 @@
 // With m the row's largest logit and w_i = exp((x_i - m) / T), tokens stand in the order (logit down, index up).  Kept are
 // the first top_k of them; of these the shortest prefix whose weight reaches top_p of theirs; of these the ones with w_i >= min_p.
 // Each filter keeps a prefix of that order, so together they keep the shortest of the three.  The draw is the inverse CDF in the
-// order of the indices, as in sample.cu: the first kept index whose running weight exceeds u times the weight of all kept.
+// order of the indices, as in sample.cu: the first kept index whose running weight exceeds u times the weight of all kept (u below 0 counts as 0,
+// 1 and more and NaN as the largest float32 below 1).
 // T <= 0: the largest, lowest index on ties.  NaN counts as -infinity, which is never kept; a row with nothing else gives token 0.
 //
 // Weights come from 64-bit arithmetic (relative error below 2^-50).  The draw adds them up as whole numbers, w_i * 2^46 rounded: such sums are exact, so neither
@@ -645,7 +646,9 @@ __device__ __noinline__ void tell(int row, int token, float v, u64 total, int ke
     if (kept_out) kept_out[row] = kept;
     if (logprob_out) logprob_out[row] = (float)(-0.69314718055994530942 * (depth(v) + (log2((double)total) - sh.bits)));
 }
-__device__ __forceinline__ double goal_of(u64 total) { return sh.u < 1.f ? fmax((double)sh.u, 0.0) * (double)total : (double)(total - 1); }
+// The running weight that the drawn token passes: less than all of it by 2^-24, so that one does.  (All but one whole unit would not do: of a total of more than
+// 2^53 a 64-bit float does not tell it.)
+__device__ __forceinline__ double goal_of(u64 total) { return (double)sh.u * (double)total; }
 
 // CTA 0 has all that can be kept, one token a thread.  Up to 128 are compared each with each, four threads a token or more; of more the order is
 // sorted out, cut, then sorted by index.
@@ -878,7 +881,8 @@ sample_filtered_kernel(const float* __restrict__ logits_, long long ld, int R, i
     }
     if (tid == THREADS - 1) {                                      // for all, behind the barrier of the largest logit
         sh.x = x, sh.n = n, sh.c0 = c0, sh.ctas = ctas, sh.me = me, sh.row = row;
-        sh.k = k < V ? k : 0, sh.p = p, sh.u = u;
+        sh.k = k < V ? k : 0, sh.p = p;
+        sh.u = u < 1.f ? fmaxf(u, 0.f) : 1.f - 0x1p-24f;             // what is not in [0, 1), NaN too, as its nearer end there
         sh.per = 1.44269504088896340736 / (double)T;
         sh.deepest = mp > 0.f ? -log2((double)mp) : INFINITY;
         sh.bits = min(46, 63 - (31 - __clz(V)));                   // V weights of 1 stay below 2^64

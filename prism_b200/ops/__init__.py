@@ -739,7 +739,7 @@ def sample_filtered(logits: torch.Tensor, temperature: Optional[torch.Tensor], u
                     top_k: Optional[torch.Tensor] = None, top_p: Optional[torch.Tensor] = None, min_p: Optional[torch.Tensor] = None,
                     rows: Optional[torch.Tensor] = None, kept: Optional[torch.Tensor] = None, logprob: Optional[torch.Tensor] = None):
     """Per row: a token of ``softmax(logits / temperature)`` among those that the row's filters keep, at the uniform number ``u`` (in
-    ``[0, 1)``) of the inverse CDF.  ``top_k`` (int32; 0 or less: off) keeps the largest logits (the lower index of equal ones);
+    ``[0, 1)``; any other as the nearer end, NaN as the upper one, the largest float32 below 1) of the inverse CDF.  ``top_k`` (int32; 0 or less: off) keeps the largest logits (the lower index of equal ones);
     ``top_p`` (float32; 1 or more: off) the shortest run of the likeliest of these whose probability reaches that share of theirs, one at least;
     ``min_p`` (float32; 0 or less: off) of these the ones at least ``min_p`` times as likely as the likeliest.  Temperature 0 or less
     (or None for all rows): the largest, lowest index on ties.  NaN counts as -infinity, which is never kept; rows of nothing else give token

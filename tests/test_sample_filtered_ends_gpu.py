@@ -1,0 +1,41 @@
+"""Uniform numbers beyond the ends of [0, 1), where many tokens are kept (GPU)."""
+
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from test_sample_filtered_gpu import DEV, draw, plain_row
+
+pytestmark = pytest.mark.gpu
+LAST = 1 - 2.0 ** -24                                    # the largest float32 below 1
+KINDS = [("equal", 152064, None, None, None), ("equal", 9001, None, None, None), ("equal", 9001, 300, None, None), ("equal", 520, 400, None, None),
+         ("equal", 152064, 5000, None, None), ("equal", 152064, None, 0.9, None), ("flat", 152064, None, None, None), ("flat", 40000, 300, 0.99, 0.001),
+         ("flat", 400000, None, 0.999, None)]
+
+
+@pytest.mark.parametrize("kind,V,k,p,m", KINDS)
+def test_what_is_not_below_1_is_the_last_number_that_is(kind, V, k, p, m):
+    """The weight of all kept tokens is a whole number of up to 63 bits here: more than a 64-bit float tells from the next one."""
+    ends = [1.0, math.nan, 2.0, math.inf, 1 + 2.0 ** -23]
+    R = len(ends)
+    x = torch.zeros(R, V) if kind == "equal" else torch.randn(1, V, generator=torch.Generator().manual_seed(V)).expand(R, V) * 0.5
+    x = x.contiguous().to(DEV)
+    every = lambda v: None if v is None else [v] * R     # noqa: E731
+    got = draw(x, [1.0] * R, ends, every(k), every(p), every(m))
+    want = draw(x, [1.0] * R, [LAST] * R, every(k), every(p), every(m))
+    assert got == want
+    row = x[0].cpu().numpy()
+    f = np.float32
+    tok, kept, lp = plain_row(row, f(1.0), f(LAST), k or 0, f(1.0 if p is None else p), f(m or 0))
+    for i in range(R):
+        assert got[0][i] == tok and got[1][i] == kept and abs(got[2][i] - lp) <= 2.0 ** -24 * abs(lp) + 2.0 ** -40
+
+
+@pytest.mark.parametrize("V,k", [(152064, None), (520, 400)])
+def test_what_is_below_0_is_0(V, k):
+    ends = [-0.0, -1.0, -math.inf, -1e-30]
+    x = torch.zeros(4, V, device=DEV)
+    k = None if k is None else [k] * 4
+    assert draw(x, [1.0] * 4, ends, k) == draw(x, [1.0] * 4, [0.0] * 4, k)
