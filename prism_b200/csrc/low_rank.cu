@@ -3,7 +3,9 @@
 //
 // A projection that runs as one product over stacked matrices (q, k, v; gate, up) has its adapters' A and B per matrix: "slices", groups of
 // neighbouring result columns.  a [L, G, r, Kp]: r rows of a slice's A, zeros beyond K; b [L, N, r]: the rows of all slices' B.  r is a
-// multiple of 16, Kp of 8 (rows start on 16 bytes), zeros beyond an adapter's own rank.  Sums in float32, one rounding where a result is stored.
+// multiple of 16, Kp of 8 (rows start on 16 bytes).  ranks [L, G]: so many rows of a slice's A, and columns of its B, are the adapter's own, the others
+// zeros; a hidden value beyond them is 0 whatever x is (infinity times a zero that only fills up room would be NaN).  Sums in float32, one
+// rounding where a result is stored.
 //
 // Here, on CUDA cores: decoding requests, each with an adapter of its own, where every byte of A and B is used once and the kernel is bound by
 // reading them; and portions of prompts in 32-bit floats, or of sizes that TMA does not take.  low_rank_tile.cu has the portions on tensor cores.
@@ -38,6 +40,11 @@ __device__ __forceinline__ int adapter_of(const int* ids, int t, int L, int* err
         return -1;
     }
     return l < 0 ? -1 : l;
+}
+
+// four bytes of memory into shared memory, through no register
+__device__ __forceinline__ void async_word(void* to, const void* from) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from) : "memory");
 }
 
 // 16 bytes of a row: E values
@@ -80,11 +87,13 @@ __device__ __forceinline__ uint32_t rank_in_cluster() {
 template <typename T, typename O, int THREADS, int PER_SM, int CTAS>
 __global__ void __launch_bounds__(THREADS, PER_SM)
 low_rank_token_kernel(const T* __restrict__ x_, long long ldx, int x_whole, const T* __restrict__ a, const T* __restrict__ b,
-                      const float* __restrict__ scale, const int* __restrict__ ids_, const O* __restrict__ base_, long long ldb, O* out_, long long ldo,
-                      int K, int Kp, int r, int L, const __grid_constant__ Slices slices, int parts, int* err) {
+                      const float* __restrict__ scale, const int* __restrict__ ranks, const int* __restrict__ ids_, const O* __restrict__ base_, long long ldb,
+                      O* out_, long long ldo, int K, int Kp, int r, int L, const __grid_constant__ Slices slices, int parts, int* err) {
     constexpr int E = Chunk<T>::E, WARPS = THREADS / 32;
     __shared__ float hidden[MOST_RANK];
     __shared__ float partial[MOST_RANK / CTAS][WARPS];             // a hidden value's share of a warp
+    __shared__ float scale_l;                                      // the adapter's, and its rank: asked for here, needed behind the sums
+    __shared__ int own;
     asm volatile("barrier.cluster.arrive.aligned;" ::: "memory");              // here: peers may write into this CTA's memory
     pdl_trigger();
     pdl_wait();
@@ -102,6 +111,11 @@ low_rank_token_kernel(const T* __restrict__ x_, long long ldx, int x_whole, cons
             for (int n = tid; n < mine; n += THREADS) out[n] = base ? base[n] : from_float<O>(0.f);
         asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
         return;
+    }
+    if (tid == 0) {
+        async_word(&scale_l, scale + l);
+        if (ranks) async_word(&own, ranks + l * slices.n + g);
+        else own = r;
     }
     // B's chunks: `lanes` neighbours share a row, each with the same two parts of every row that it meets
     const int chunks = r / E;
@@ -167,13 +181,15 @@ low_rank_token_kernel(const T* __restrict__ x_, long long ldx, int x_whole, cons
         s = warp_sum(s);
         if (lane == 0) partial[j][sub] = s;
     }
+    if (tid == 0) asm volatile("cp.async.wait_all;" ::: "memory");
     __syncthreads();
     asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
     if (tid < rows * CTAS) {                                       // a hidden value, for one of the CTAs
         const int c = tid % CTAS, q = tid / CTAS;
         float h = 0.f;
         for (int w = 0; w < split; ++w) h += partial[q][w];
-        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(peer(&hidden[me * rows + q], c)), "f"(h * scale[l]) : "memory");
+        h = me * rows + q < own ? h * scale_l : 0.f;
+        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(peer(&hidden[me * rows + q], c)), "f"(h) : "memory");
     }
     __syncwarp();
     cluster_barrier();
@@ -210,8 +226,8 @@ low_rank_token_kernel(const T* __restrict__ x_, long long ldx, int x_whole, cons
 }
 
 template <typename T, typename O>
-int launch_tokens(const void* x, long long ldx, const void* a, const void* b, const float* scale, const int* ids, const void* base, long long ldb, void* out,
-                  long long ldo, int tokens, int K, int Kp, int r, int L, const Slices& s, int* err, int sms, cudaStream_t stream) {
+int launch_tokens(const void* x, long long ldx, const void* a, const void* b, const float* scale, const int* ranks, const int* ids, const void* base,
+                  long long ldb, void* out, long long ldo, int tokens, int K, int Kp, int r, int L, const Slices& s, int* err, int sms, cudaStream_t stream) {
     if (tokens <= 0) return 0;
     if (tokens > 65535) return (int)cudaErrorInvalidValue;
     // Clusters at a time with an SM a CTA, with half of one, a third and a quarter.  Where a CTA has much of A, up to 18 are launched in the first form all the same:
@@ -249,7 +265,7 @@ int launch_tokens(const void* x, long long ldx, const void* a, const void* b, co
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = prism::pdl_enabled() ? 2 : 1;
-    return (int)cudaLaunchKernelEx(&cfg, kernel, (const T*)x, ldx, whole, (const T*)a, (const T*)b, scale, ids, (const O*)base, ldb, (O*)out,
+    return (int)cudaLaunchKernelEx(&cfg, kernel, (const T*)x, ldx, whole, (const T*)a, (const T*)b, scale, ranks, ids, (const O*)base, ldb, (O*)out,
                                    ldo, K, Kp, r, L, s, parts, err);
 }
 
@@ -276,7 +292,7 @@ __device__ __forceinline__ void list_adapters(const int* ids, int t0, int tokens
 template <typename T>
 __global__ void __launch_bounds__(HT)
 low_rank_plain_hidden_kernel(const T* __restrict__ x_, long long ldx, const T* __restrict__ a, const float* __restrict__ scale,
-                             const int* __restrict__ ids_, float* __restrict__ hidden, int tokens, int K, int Kp, int r, int G, int L, int* err) {
+                             const int* __restrict__ ranks, const int* __restrict__ ids_, float* __restrict__ hidden, int tokens, int K, int Kp, int r, int G, int L, int* err) {
     __shared__ float xs[TOKENS][DEEP + 1];
     __shared__ float as[MOST_RANK][DEEP + 1];                      // behind the last block, this CTA's sums
     float* sums = &as[0][0];                                       // [TOKENS][r]
@@ -345,7 +361,7 @@ low_rank_plain_hidden_kernel(const T* __restrict__ x_, long long ldx, const T* _
             for (int i = 0; i < CTAS; ++i) asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(part[i]) : "r"(peer(sums + row * r + c, i)) : "memory");
 #pragma unroll
             for (int i = 0; i < CTAS; ++i) s += part[i];
-            hidden[((size_t)(t0 + row) * G + g) * r + c] = s * scale[l];
+            hidden[((size_t)(t0 + row) * G + g) * r + c] = ranks == nullptr || c < ranks[l * G + g] ? s * scale[l] : 0.f;
         }
         __syncwarp();
         cluster_barrier();
@@ -416,8 +432,8 @@ low_rank_plain_result_kernel(const float* __restrict__ hidden_, const T* __restr
 }
 
 template <typename T, typename O>
-int launch_portions(const void* x, long long ldx, const void* a, const void* b, const float* scale, const int* ids, const void* base, long long ldb, void* out,
-                    long long ldo, int tokens, int K, int Kp, int r, int L, const Slices& s, void* hidden, int* err, cudaStream_t stream) {
+int launch_portions(const void* x, long long ldx, const void* a, const void* b, const float* scale, const int* ranks, const int* ids, const void* base,
+                    long long ldb, void* out, long long ldo, int tokens, int K, int Kp, int r, int L, const Slices& s, void* hidden, int* err, cudaStream_t stream) {
     if (tokens <= 0) return 0;
     const int tiles = (tokens + TOKENS - 1) / TOKENS;
     if (tiles > 65535 || hidden == nullptr) return (int)cudaErrorInvalidValue;
@@ -432,7 +448,7 @@ int launch_portions(const void* x, long long ldx, const void* a, const void* b, 
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = prism::pdl_enabled() ? 2 : 1;
-    int code = (int)cudaLaunchKernelEx(&cfg, low_rank_plain_hidden_kernel<T>, (const T*)x, ldx, (const T*)a, scale, ids, (float*)hidden, tokens, K, Kp, r, s.n, L,
+    int code = (int)cudaLaunchKernelEx(&cfg, low_rank_plain_hidden_kernel<T>, (const T*)x, ldx, (const T*)a, scale, ranks, ids, (float*)hidden, tokens, K, Kp, r, s.n, L,
                                        err);
     if (code != 0) return code;
     int columns = 0;
@@ -446,12 +462,12 @@ int launch_portions(const void* x, long long ldx, const void* a, const void* b, 
 }  // namespace lowrank
 }  // namespace prism
 
-// first: G + 1 column borders (host memory).  base may be null (nothing to add to), or out itself.  hidden null: all T tokens one by one; else in
-// tiles, with T G r floats of workspace there.
-PRISM_EXPORT int prism_low_rank(const void* x, long long ldx, int dtype, const void* a, const void* b, const float* scale, const int* ids,
-                                const void* base, long long ldb, void* out, long long ldo, int out_dtype, int T, int K, int Kp, int r, int L, int G,
-                                const int* first, void* hidden, int sms, int* err, cudaStream_t stream) {
-    using namespace prism::lowrank;
+namespace prism {
+namespace lowrank {
+
+int run(const void* x, long long ldx, int dtype, const void* a, const void* b, const float* scale, const int* ranks, const int* ids, const void* base,
+        long long ldb, void* out, long long ldo, int out_dtype, int T, int K, int Kp, int r, int L, int G, const int* first, void* hidden, int sms,
+        int* err, cudaStream_t stream) {
     typedef __nv_bfloat16 bf16;
     if (T <= 0) return 0;
     if (G < 1 || G > MOST_SLICES || r < 16 || r % 16 || r > MOST_RANK || K < 1 || Kp < K || Kp % 8 || L < 1 || sms < 1) return (int)cudaErrorInvalidValue;
@@ -460,10 +476,28 @@ PRISM_EXPORT int prism_low_rank(const void* x, long long ldx, int dtype, const v
     for (int g = 0; g <= G; ++g) s.first[g] = first[g];
     for (int g = 0; g < G; ++g)
         if (s.first[g] >= s.first[g + 1]) return (int)cudaErrorInvalidValue;
-#define PRISM_LOW_RANK(TX, TO)                                                                                                           \
-    (hidden ? launch_portions<TX, TO>(x, ldx, a, b, scale, ids, base, ldb, out, ldo, T, K, Kp, r, L, s, hidden, err, stream)              \
-            : launch_tokens<TX, TO>(x, ldx, a, b, scale, ids, base, ldb, out, ldo, T, K, Kp, r, L, s, err, sms, stream))
+#define PRISM_LOW_RANK(TX, TO)                                                                                                              \
+    (hidden ? launch_portions<TX, TO>(x, ldx, a, b, scale, ranks, ids, base, ldb, out, ldo, T, K, Kp, r, L, s, hidden, err, stream)          \
+            : launch_tokens<TX, TO>(x, ldx, a, b, scale, ranks, ids, base, ldb, out, ldo, T, K, Kp, r, L, s, err, sms, stream))
     if (dtype == PRISM_DTYPE_F32) return out_dtype == PRISM_DTYPE_F32 ? PRISM_LOW_RANK(float, float) : PRISM_LOW_RANK(float, bf16);
     return out_dtype == PRISM_DTYPE_F32 ? PRISM_LOW_RANK(bf16, float) : PRISM_LOW_RANK(bf16, bf16);
 #undef PRISM_LOW_RANK
+}
+
+}  // namespace lowrank
+}  // namespace prism
+
+// first: G + 1 column borders (host memory).  base may be null (nothing to add to), or out itself.  hidden null: all T tokens one by one; else in
+// tiles, with T G r floats of workspace there.  All r rows of every A count.
+PRISM_EXPORT int prism_low_rank(const void* x, long long ldx, int dtype, const void* a, const void* b, const float* scale, const int* ids,
+                                const void* base, long long ldb, void* out, long long ldo, int out_dtype, int T, int K, int Kp, int r, int L, int G,
+                                const int* first, void* hidden, int sms, int* err, cudaStream_t stream) {
+    return prism::lowrank::run(x, ldx, dtype, a, b, scale, nullptr, ids, base, ldb, out, ldo, out_dtype, T, K, Kp, r, L, G, first, hidden, sms, err, stream);
+}
+
+// The same with ranks [L, G]: how many rows of A each adapter has in each slice.
+PRISM_EXPORT int prism_low_rank_ranked(const void* x, long long ldx, int dtype, const void* a, const void* b, const float* scale, const int* ranks,
+                                       const int* ids, const void* base, long long ldb, void* out, long long ldo, int out_dtype, int T, int K, int Kp,
+                                       int r, int L, int G, const int* first, void* hidden, int sms, int* err, cudaStream_t stream) {
+    return prism::lowrank::run(x, ldx, dtype, a, b, scale, ranks, ids, base, ldb, out, ldo, out_dtype, T, K, Kp, r, L, G, first, hidden, sms, err, stream);
 }

@@ -82,7 +82,7 @@ __device__ __forceinline__ void epilogue_barrier() { asm volatile("bar.sync 1, %
 // hidden: [tokens][2][G r], high terms and low ones; adapters: how many a tile has
 __global__ void __launch_bounds__(ALL_THREADS)
 low_rank_hidden_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_a, const float* __restrict__ scale,
-                       const int* __restrict__ ids_, __nv_bfloat16* __restrict__ hidden, int* __restrict__ adapters, int tokens, int K, int r, int G, int L, int ring_bytes,
+                       const int* __restrict__ ranks, const int* __restrict__ ids_, __nv_bfloat16* __restrict__ hidden, int* __restrict__ adapters, int tokens, int K, int r, int G, int L, int ring_bytes,
                        int most_adapters, int tmem_cols, int* err) {
     extern __shared__ unsigned char raw[];
     unsigned char* ring = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
@@ -210,6 +210,12 @@ low_rank_hidden_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_c
                     for (int b = 0; b < adapters_now; ++b)
                         if (own[row] == list[first + b]) l = own[row];
                     if (l < 0 || !go) continue;
+                    const float s = scale[l];
+                    int mine = 4;                                  // of these columns, the adapter's own (low_rank.cu)
+                    if (ranks) {
+                        const int g = (c0 + c) / r;
+                        mine = ranks[l * G + g] - (c0 + c - g * r);
+                    }
                     const uint32_t at = smem_addr(sums + row * WIDE_LD + c);
                     float4 part[CTAS];
 #pragma unroll
@@ -222,14 +228,13 @@ low_rank_hidden_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_c
                     float v[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                     for (int j = 0; j < CTAS; ++j) v[0] += part[j].x, v[1] += part[j].y, v[2] += part[j].z, v[3] += part[j].w;
-                    const float s = scale[l];
                     __nv_bfloat16 hi[4], lo[4];
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const float h = v[i] * s;
+                        const float h = i < mine ? v[i] * s : 0.f;
                         hi[i] = __float2bfloat16_rn(h);
                         const float rest = h - __bfloat162float(hi[i]);
-                        lo[i] = __float2bfloat16_rn(rest == rest ? rest : 0.f);        // an infinity's rest is none
+                        lo[i] = __float2bfloat16_rn(fabsf(rest) < INFINITY ? rest : 0.f);        // an infinity's rest is none
                     }
                     __nv_bfloat16* to = hidden + (size_t)t * 2 * H + c0 + c;
                     *reinterpret_cast<uint2*>(to) = *reinterpret_cast<uint2*>(hi);
@@ -782,10 +787,10 @@ PRISM_EXPORT int prism_low_rank_tile_supported(int K, int r, int G, int x_aligne
     return x_aligned && K >= 1 && r >= 16 && r % 16 == 0 && r <= MOST_RANK && G >= 1 && G <= MOST_SLICES && G * r <= MOST_HIDDEN;
 }
 
-// bfloat16 x and adapters, all T tokens in tiles; arguments as prism_low_rank's.  hidden: 2 T G r bfloat16 of workspace, and an int for each of the
+// bfloat16 x and adapters, all T tokens in tiles; arguments as prism_low_rank_ranked's, ranks may be null.  hidden: 2 T G r bfloat16 of workspace, and an int for each of the
 // tiles of 128 tokens.
-PRISM_EXPORT int prism_low_rank_tile(const void* x, long long ldx, const void* a, const void* b, const float* scale, const int* ids, const void* base,
-                                     long long ldb, void* out, long long ldo, int out_dtype, int T, int K, int Kp, int r, int L, int G, const int* first,
+PRISM_EXPORT int prism_low_rank_tile(const void* x, long long ldx, const void* a, const void* b, const float* scale, const int* ranks, const int* ids,
+                                     const void* base, long long ldb, void* out, long long ldo, int out_dtype, int T, int K, int Kp, int r, int L, int G, const int* first,
                                      void* hidden, int sms, int* err, cudaStream_t stream) {
     using namespace prism::lowrank_tile;
     typedef __nv_bfloat16 bf16;
@@ -832,7 +837,7 @@ PRISM_EXPORT int prism_low_rank_tile(const void* x, long long ldx, const void* a
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = prism::pdl_enabled() ? 2 : 1;
-    code = (int)cudaLaunchKernelEx(&cfg, low_rank_hidden_kernel, map_x, map_a, scale, ids, (bf16*)hidden, adapters, T, K, r, G, L, ring, most, cols, err);
+    code = (int)cudaLaunchKernelEx(&cfg, low_rank_hidden_kernel, map_x, map_a, scale, ranks, ids, (bf16*)hidden, adapters, T, K, r, G, L, ring, most, cols, err);
     if (code != 0) return code;
 
     if (out_dtype == PRISM_DTYPE_F32) return launch_results<float>(hidden, adapters, map_b, ids, base, ldb, out, ldo, T, r, L, s, err, sms, stream);

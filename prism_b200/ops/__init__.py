@@ -171,8 +171,9 @@ class _Sig:
     prism_sample = [_p, _i, _i, _i, _p, _p, _p, _p]
     prism_sample_filtered = [_p, _ll, _i, _i, _i, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p]
     prism_low_rank = [_p, _ll, _i, _p, _p, _p, _p, _p, _ll, _p, _ll, _i, _i, _i, _i, _i, _i, _i, _p, _p, _i, _p, _p]
+    prism_low_rank_ranked = [_p, _ll, _i, _p, _p, _p, _p, _p, _p, _ll, _p, _ll, _i, _i, _i, _i, _i, _i, _i, _p, _p, _i, _p, _p]
     prism_low_rank_tile_supported = [_i, _i, _i, _i]
-    prism_low_rank_tile = [_p, _ll, _p, _p, _p, _p, _p, _ll, _p, _ll, _i, _i, _i, _i, _i, _i, _i, _p, _p, _i, _p, _p]
+    prism_low_rank_tile = [_p, _ll, _p, _p, _p, _p, _p, _p, _ll, _p, _ll, _i, _i, _i, _i, _i, _i, _i, _p, _p, _i, _p, _p]
     prism_argmax_split = [_p, _i, _i, _i, _i, _p, _p, _p, _p, _p]
     prism_set_pdl = [_i]
     prism_gemm_tcgen05_supported = [_i, _i, _i]

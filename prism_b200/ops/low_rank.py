@@ -35,11 +35,14 @@ class LowRank:
     """Adapters of one projection ``[N, K]``.  ``a [L, G, r, Kp]``: the A of each of the L adapters for each of the G slices of the
     projection's rows (the matrices that it stacks: q, k and v, say), r rows each.  ``b [L, N, r]``: the rows of their B, all slices'
     below each other.  ``rows``: how many of the N rows each slice has.  r is a multiple of 16 up to 128, with zeros beyond an adapter's
-    own rank; Kp is K rounded up to a multiple of 8 at least, with zeros beyond K.  ``scale``: float32 ``[L]``."""
+    own rank; Kp is K rounded up to a multiple of 8 at least, with zeros beyond K.  ``scale``: float32 ``[L]``.  ``ranks``: int32 ``[L, G]``, the rank that
+    each adapter has in each slice (0: it has none there); what lies beyond is no part of the formula, and an infinite x meets none of its zeros.
+    None: all r rows of every A count."""
 
-    __slots__ = ("a", "b", "scale", "rows", "k", "rank", "count", "n", "_first", "_sizes")
+    __slots__ = ("a", "b", "scale", "ranks", "rows", "k", "rank", "count", "n", "_first", "_sizes")
 
-    def __init__(self, a: torch.Tensor, b: torch.Tensor, scale: torch.Tensor, rows: Sequence[int], k: Optional[int] = None):
+    def __init__(self, a: torch.Tensor, b: torch.Tensor, scale: torch.Tensor, rows: Sequence[int], k: Optional[int] = None,
+                 ranks: Optional[torch.Tensor] = None):
         rows = tuple(map(int, rows))
         sa, sb, dt = a.shape, b.shape, a.dtype
         if len(sa) != 4 or len(sb) != 3 or not rows or min(rows) < 1 or len(rows) > MOST_SLICES:
@@ -58,16 +61,20 @@ class LowRank:
         if not (a.is_contiguous() and b.is_contiguous() and scale.is_contiguous()) or a.data_ptr() % 16 or b.data_ptr() % 16 \
                 or not a.get_device() == b.get_device() == scale.get_device():
             raise ops.KernelError("adapters: A, B and the scales lie contiguous on one device, A and B from a 16-byte border on")
+        if ranks is not None and (ranks.dtype is not torch.int32 or ranks.shape != sa[:2] or not ranks.is_contiguous() or ranks.get_device() != a.get_device()):
+            raise ops.KernelError(f"adapters: ranks are int32 [{L}, {G}], contiguous on {a.device}: got {ranks.dtype} {tuple(ranks.shape)} on {ranks.device}")
+        self.ranks = ranks
         self.a, self.b, self.scale, self.rows, self.k, self.rank, self.count, self.n = a, b, scale, rows, k, r, L, n
         self._first = (ctypes.c_int * (G + 1))(0, *itertools.accumulate(rows))
         self._sizes = (k, kp, r, L, G, ctypes.addressof(self._first))
 
     @classmethod
     def empty(cls, count: int, rank: int, rows: Sequence[int], k: int, dtype: torch.dtype, device) -> "LowRank":
-        """Room for ``count`` adapters of ranks up to ``rank``, all zero (an adapter of zeros adds nothing)."""
+        """Room for ``count`` adapters of ranks up to ``rank``, all zero (an adapter of zeros adds nothing).  All rows count until ``put`` says how many
+        an adapter has."""
         r, kp = _up(int(rank), RANK_UNIT), _up(int(k), WIDTH_UNIT)
         return cls(torch.zeros((count, len(rows), r, kp), dtype=dtype, device=device), torch.zeros((count, sum(rows), r), dtype=dtype, device=device),
-                   torch.zeros(count, dtype=torch.float32, device=device), rows, k)
+                   torch.zeros(count, dtype=torch.float32, device=device), rows, k, torch.full((count, len(rows)), r, dtype=torch.int32, device=device))
 
     @property
     def nbytes(self) -> int:
@@ -85,6 +92,8 @@ class LowRank:
         self.a[index].zero_()
         self.b[index].zero_()
         self.scale[index] = float(scale)
+        if self.ranks is not None:
+            self.ranks[index].copy_(torch.tensor([0 if ab is None else ab[0].shape[0] for ab in slices], dtype=torch.int32))
         for g, ab in enumerate(slices):
             if ab is not None:
                 rank, at = ab[0].shape[0], self._first[g]
@@ -172,7 +181,9 @@ def low_rank(x: torch.Tensor, low: LowRank, ids: torch.Tensor, base: Optional[to
     singles = (T if T <= SINGLES else 0) if singles is None else max(0, min(int(singles), T))
     L, stream, err = ops.lib(), ops._stream(), ops.mxfp4._err_word(x.device)
     sms = ops._num_sms.get(d) or ops.num_sms(x.device)
-    ap, bp, sp, sizes = low.a.data_ptr(), low.b.data_ptr(), low.scale.data_ptr(), low._sizes
+    sizes, ap, bp, sp = low._sizes, low.a.data_ptr(), low.b.data_ptr(), low.scale.data_ptr()
+    rp = None if low.ranks is None else low.ranks.data_ptr()
+    plain, head = (L.prism_low_rank, (ap, bp, sp)) if rp is None else (L.prism_low_rank_ranked, (ap, bp, sp, rp))
     bf16, out16 = dt is torch.bfloat16, odt is torch.bfloat16
     xp, x_row, ip, op, o_row = x.data_ptr(), x.stride(0), ids.data_ptr(), out.data_ptr(), out.stride(0)
     basep, b_row = (None, 0) if base is None else (base.data_ptr(), base.stride(0))
@@ -182,18 +193,18 @@ def low_rank(x: torch.Tensor, low: LowRank, ids: torch.Tensor, base: Optional[to
         if T - singles < (TILE_FROM if tiles else PLAIN_TILE_FROM):
             singles = T
     if singles:
-        ops._check(L.prism_low_rank(xp, x_row, bf16, ap, bp, sp, ip, basep, b_row, op, o_row, out16, singles, *sizes, None, sms, err, stream), "low_rank")
+        ops._check(plain(xp, x_row, bf16, *head, ip, basep, b_row, op, o_row, out16, singles, *sizes, None, sms, err, stream), "low_rank")
     rest = T - singles
     if rest == 0:
         return out
     size = 2 if out16 else 4
     xp, op, basep = xp + singles * x_row * (2 if bf16 else 4), op + singles * o_row * size, basep and basep + singles * b_row * size
-    args = (sp, ip + 4 * singles, basep, b_row, op, o_row, out16, rest, *sizes)
+    args = (ip + 4 * singles, basep, b_row, op, o_row, out16, rest, *sizes)
     if tiles:
         hidden = torch.empty(2 * rest * G * low.rank + 2 * (-(-rest // 128)), dtype=torch.bfloat16, device=x.device)
-        ops._check(L.prism_low_rank_tile(xp, x_row, ap, bp, *args, hidden.data_ptr(), sms, err, stream), "low_rank_tile")
+        ops._check(L.prism_low_rank_tile(xp, x_row, ap, bp, sp, rp, *args, hidden.data_ptr(), sms, err, stream), "low_rank_tile")
     else:
         hidden = torch.empty(rest * G * low.rank, dtype=torch.float32, device=x.device)
-        ops._check(L.prism_low_rank(xp, x_row, bf16, ap, bp, *args, hidden.data_ptr(), sms, err, stream), "low_rank")
+        ops._check(plain(xp, x_row, bf16, *head, *args, hidden.data_ptr(), sms, err, stream), "low_rank")
     ops.launch_count += 1                    # two kernels
     return out

@@ -1,0 +1,79 @@
+"""Low-rank adapters on the GPU: what is part of an adapter and what only fills up its stack, and what calls may do beside each other."""
+
+import pytest
+import torch
+
+from test_low_rank_gpu import DEV, _ops, check, ids_of, inputs, plain
+
+pytestmark = pytest.mark.gpu
+
+
+def exactly(x, low, ids, base, own):
+    """The definition in 64 bits with each adapter's matrices as they are, without the stack's room: ``own[e][slice]`` is ``(A, B)`` or None."""
+    y = base.double().clone()
+    for e, slices in enumerate(own):
+        tok = torch.nonzero(ids == e).squeeze(1)
+        at = 0
+        for n, ab in zip(low.rows, slices):
+            if ab is not None:
+                a, b = ab[0].to(DEV).double(), ab[1].to(DEV).double()
+                # row by row: a matrix product may add zeros for places that are not there
+                h = low.scale[e].double() * (x[tok].double().unsqueeze(1) * a).sum(2)
+                y[tok, at:at + n] += (h.unsqueeze(1) * b).sum(2)
+            at += n
+    return y
+
+
+@pytest.mark.parametrize("dtype,out_dtype", [(torch.bfloat16, torch.bfloat16), (torch.bfloat16, torch.float32), (torch.float32, torch.float32)], ids=str)
+@pytest.mark.parametrize("T,singles", [(12, 12), (40, 40), (140, 0), (300, 0), (300, 30)])
+@pytest.mark.parametrize("room", [16, 40, 128])
+def test_infinities_do_not_meet_the_room_beyond_an_adapter_s_rank(dtype, out_dtype, T, singles, room):
+    """An infinite activation makes an adapter's own hidden values infinite.  What lies behind its rank in the stack, and slices that it does not have, are
+    not part of the formula: results are infinities there and the shared ones here, not NaN."""
+    ops = _ops()
+    rows, K = (72, 40, 64), 136
+    g = torch.Generator().manual_seed(room)
+    signs = lambda *s: torch.where(torch.rand(*s, generator=g) < 0.5, -1.0, 1.0) * (0.5 + torch.rand(*s, generator=g))          # noqa: E731
+    ab = lambda r, n: ((signs(1, K).expand(r, K) * 0.25).to(dtype), (signs(n, 1).expand(n, r) * 0.5).to(dtype))                 # noqa: E731
+    # of one adapter all hidden values have one sign, and a result's terms too: sums of infinities of one sign
+    own = [[ab(1, 72), None, ab(2, 64)], [None, ab(5, 40), None], [None, None, None], [ab(16, 72), ab(16, 40), ab(16, 64)]]
+    low = ops.LowRank.empty(4, room, rows, K, dtype, DEV)
+    for e, slices in enumerate(own):
+        low.put(e, slices, 0.5 + e)
+    ids = ids_of([(e, 1) for e in (0, 1, 2, 3, -1)] * 2 + [(0, 1), (3, T - 11)])
+    x, base = inputs(T, K, sum(rows), dtype, out_dtype, 5)
+    x[5:10, 17], x[10, 3], x[T - 1, 64] = float("inf"), float("-inf"), float("inf")
+    want = exactly(x, low, ids, base, own)
+    got = ops.low_rank(x, low, ids, base, singles=singles)
+    limits = ~torch.isfinite(want)
+    assert limits[5].any() and not limits[5].all() and not limits[7].any() and not torch.isnan(want).any()
+    assert torch.equal(got[limits].double(), want[limits])
+    clean = x.clone()
+    clean[~torch.isfinite(x)] = 0
+    finite, tol = plain(clean, low, ids, base)
+    rest = ~limits.any(1)
+    check(got[rest], finite[rest], tol[rest])
+    none = torch.zeros_like(limits)                       # slices that the row's adapter does not have
+    none[(ids == 0), 72:112] = none[(ids == 1), :72] = none[(ids == 1), 112:] = none[(ids == 2)] = none[(ids < 0)] = True
+    assert torch.equal(got[none], base[none])
+
+
+def test_a_stack_that_is_not_filled_by_put_counts_whole():
+    """A and B given, or written into an empty stack: all r rows count, until ``put`` says how many an adapter has."""
+    ops = _ops()
+    g = torch.Generator().manual_seed(3)
+    a, b = (torch.randn(2, 2, 16, 72, generator=g) / 8).bfloat16().to(DEV), torch.randn(2, 96, 16, generator=g).bfloat16().to(DEV)
+    given = ops.LowRank(a, b, torch.ones(2, device=DEV), rows=(64, 32))
+    filled = ops.LowRank.empty(2, 16, (64, 32), 72, torch.bfloat16, DEV)
+    filled.a.copy_(a), filled.b.copy_(b), filled.scale.fill_(1.0)
+    for T, singles in ((9, 9), (140, 0)):
+        x, base = inputs(T, 72, 96, torch.bfloat16, torch.float32, 9)
+        ids = (torch.arange(T, device=DEV) % 3 - 1).int()
+        want, tol = plain(x, given, ids, base)
+        for low in (given, filled):
+            check(ops.low_rank(x, low, ids, base, singles=singles), want, tol)
+    filled.put(1, [(a[1, 0, :3].cpu(), b[1, :64, :3].cpu()), None], 2.0)
+    assert filled.ranks.tolist() == [[16, 16], [3, 0]]
+    ids = torch.ones(9, dtype=torch.int32, device=DEV)
+    x, base = inputs(9, 72, 96, torch.bfloat16, torch.float32, 9)
+    check(ops.low_rank(x, filled, ids, base), *plain(x, filled, ids, base))
