@@ -68,6 +68,10 @@ class LowRank:
         self._first = (ctypes.c_int * (G + 1))(0, *itertools.accumulate(rows))
         self._sizes = (k, kp, r, L, G, ctypes.addressof(self._first))
 
+    def __reduce__(self):
+        # copies and what is read back are made anew: the launchers follow the address of the borders, which are this object's
+        return LowRank, (self.a, self.b, self.scale, self.rows, self.k, self.ranks)
+
     @classmethod
     def empty(cls, count: int, rank: int, rows: Sequence[int], k: int, dtype: torch.dtype, device) -> "LowRank":
         """Room for ``count`` adapters of ranks up to ``rank``, all zero (an adapter of zeros adds nothing).  All rows count until ``put`` says how many

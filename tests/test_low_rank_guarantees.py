@@ -1,5 +1,10 @@
 """The adapters' stack on the host (CPU)."""
 
+import copy
+import ctypes
+import gc
+import pickle
+
 import pytest
 import torch
 
@@ -25,3 +30,22 @@ def test_ranks_are_checked():
     for ranks in (torch.ones(2, 2), torch.ones(2, dtype=torch.int32), torch.ones(2, 3, dtype=torch.int32), torch.ones(2, 4, dtype=torch.int32)[:, ::2]):
         with pytest.raises(ops.KernelError):
             ops.LowRank(a, b, s, (8, 4), ranks=ranks)
+
+
+@pytest.mark.parametrize("how", [copy.copy, copy.deepcopy, lambda low: pickle.loads(pickle.dumps(low))], ids=["copy", "deepcopy", "pickle"])
+@pytest.mark.parametrize("filled", [True, False])
+def test_a_copy_has_borders_of_its_own(how, filled):
+    """The slices' borders go to the kernels' launchers by their address in host memory: a copy outlives what it was made from."""
+    low = ops.LowRank.empty(2, 4, (8, 4), 21, torch.float32, "cpu")
+    if not filled:
+        low = ops.LowRank(low.a, low.b, low.scale, (8, 4), 21)
+    else:
+        low.put(1, [(torch.ones(3, 21), torch.ones(8, 3)), None], 2.0)
+    other = how(low)
+    assert other._sizes[-1] == ctypes.addressof(other._first) and other._sizes[:-1] == low._sizes[:-1]
+    want = low.a.clone(), low.b.clone(), None if low.ranks is None else low.ranks.tolist()
+    del low
+    gc.collect()
+    assert list((ctypes.c_int * 3).from_address(other._sizes[-1])) == [0, 8, 12]
+    assert (other.rows, other.k, other.rank, other.count, other.n) == ((8, 4), 21, 16, 2, 12)
+    assert torch.equal(other.a, want[0]) and torch.equal(other.b, want[1]) and (None if other.ranks is None else other.ranks.tolist()) == want[2]
