@@ -84,6 +84,7 @@ class LowRank:
     def nbytes(self) -> int:
         return sum(t.numel() * t.element_size() for t in (self.a, self.b, self.scale))
 
+    @torch.no_grad()
     def put(self, index: int, slices, scale: float) -> None:
         """Adapter ``index``: per slice its ``(A [rank, K], B [rows, rank])``, or None where it has none."""
         if not 0 <= index < self.count or len(slices) != len(self.rows):

@@ -49,3 +49,13 @@ def test_a_copy_has_borders_of_its_own(how, filled):
     assert list((ctypes.c_int * 3).from_address(other._sizes[-1])) == [0, 8, 12]
     assert (other.rows, other.k, other.rank, other.count, other.n) == ((8, 4), 21, 16, 2, 12)
     assert torch.equal(other.a, want[0]) and torch.equal(other.b, want[1]) and (None if other.ranks is None else other.ranks.tolist()) == want[2]
+
+
+def test_matrices_that_want_gradients_leave_nothing_behind():
+    """An adapter as a training loop has it: its values are taken, its graph is not."""
+    low = ops.LowRank.empty(2, 4, (8,), 24, torch.float32, "cpu")
+    a, b = torch.nn.Parameter(torch.randn(3, 24)), torch.nn.Parameter(torch.randn(8, 3))
+    low.put(1, [(a * 2, b)], 1.0)
+    assert torch.equal(low.a[1, 0, :3, :24], a.detach() * 2) and torch.equal(low.b[1, :, :3], b.detach())
+    for t in (low.a, low.b, low.scale, low.ranks):
+        assert not t.requires_grad and t.grad_fn is None
