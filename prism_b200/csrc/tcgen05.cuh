@@ -116,7 +116,14 @@ typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t,
                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
+// The driver's encoder needs a context in the calling thread, which only calls of the runtime that need one bring: a thread whose first call this
+// is has none.
 inline EncodeTiledFn encode_fn() {
+    static thread_local bool bound = false;
+    if (!bound) {
+        int device = 0;
+        bound = cudaGetDevice(&device) == cudaSuccess && cudaSetDevice(device) == cudaSuccess;
+    }
     static EncodeTiledFn fn = nullptr;
     if (fn == nullptr) {
         void* p = nullptr;

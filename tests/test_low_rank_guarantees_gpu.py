@@ -1,9 +1,11 @@
 """Low-rank adapters on the GPU: what is part of an adapter and what only fills up its stack, and what calls may do beside each other."""
 
+import threading
+
 import pytest
 import torch
 
-from test_low_rank_gpu import DEV, _ops, check, ids_of, inputs, plain
+from test_low_rank_gpu import DEV, _ops, check, ids_of, inputs, plain, stack
 
 pytestmark = pytest.mark.gpu
 
@@ -77,3 +79,32 @@ def test_a_stack_that_is_not_filled_by_put_counts_whole():
     ids = torch.ones(9, dtype=torch.int32, device=DEV)
     x, base = inputs(9, 72, 96, torch.bfloat16, torch.float32, 9)
     check(ops.low_rank(x, filled, ids, base), *plain(x, filled, ids, base))
+
+
+def test_the_first_call_of_a_thread():
+    """A thread that has not called CUDA yet has no context there; memory comes from what torch keeps, so nothing before the kernels needs one."""
+    ops = _ops()
+    low = stack(2, (256,), 64, 16, torch.bfloat16, 1)
+    ids = ids_of([(0, 100), (1, 60)])
+    x, base = inputs(160, 64, 256, torch.bfloat16, torch.bfloat16, 1)
+    w, few = torch.randn(256, 64, generator=torch.Generator().manual_seed(2)).bfloat16().to(DEV), x[:8].contiguous()
+    calls = [lambda: ops.low_rank(x, low, ids, base, singles=0), lambda: ops.low_rank(x, low, ids, base, singles=160), lambda: ops.linear(few, w)]
+    want = [call().clone() for call in calls]
+    for call in calls:
+        call()                                       # its result's memory is free again
+    torch.cuda.synchronize()
+    got = [None] * len(calls)
+
+    def work(i):
+        try:
+            got[i] = calls[i]()
+        except Exception as e:                       # noqa: BLE001
+            got[i] = e
+    for i in range(len(calls)):
+        t = threading.Thread(target=work, args=(i,))
+        t.start()
+        t.join()
+    torch.cuda.synchronize()
+    for a, b in zip(got, want):
+        assert torch.is_tensor(a), a
+        assert torch.equal(a, b)
