@@ -772,7 +772,9 @@ int launch_results(const void* hidden, const int* adapters, const CUtensorMap& m
                         (T == 1 || (ldo % 8 == 0 && (base == nullptr || ldb % 8 == 0)));
     const int buffers = kblocks == 1 ? 11 : 8;
     const size_t smem = 1024 + (size_t)(2 * kblocks + buffers) * BLOCK_BYTES;
-    prism::open_smem(low_rank_result_kernel<O>, smem);
+    // one limit for both (it is above open_smem's one value, so every call names the same)
+    constexpr size_t MOST = 1024 + 13 * BLOCK_BYTES;
+    prism::open_smem(low_rank_result_kernel<O>, MOST);
     return (int)prism::launch_kernel(low_rank_result_kernel<O>, dim3(even ? max(sms, (int)ctas) : (int)ctas), dim3(RESULT_THREADS), smem, stream, map_h, map_b, boxes, ids,
                                      even ? adapters : nullptr, (const O*)base,
                                      ldb, (O*)out, ldo, by_box, buffers, aligned, T, r, N, L, s, err);

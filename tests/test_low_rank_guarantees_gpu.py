@@ -108,3 +108,40 @@ def test_the_first_call_of_a_thread():
     for a, b in zip(got, want):
         assert torch.is_tensor(a), a
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("out_dtype", [torch.bfloat16, torch.float32], ids=str)
+def test_threads_with_ranks_of_either_kind(out_dtype):
+    """Ranks up to 64 and above want different amounts of shared memory of one kernel, whose limit belongs to the kernel and not to a call: no thread's call
+    lowers it under another's.  The library's entry is called by itself, as Python's lock between calls would keep them apart."""
+    ops = _ops()
+    T, K, N, G = 160, 64, 256, 1
+    lib, err = ops.lib(), ops.mxfp4._err_word(torch.device(DEV))
+    jobs = []
+    for rank in (16, 128, 64, 80):
+        low = stack(2, (N,), K, rank, torch.bfloat16, rank)
+        ids = ids_of([(0, 100), (1, T - 100)])
+        x, base = inputs(T, K, N, torch.bfloat16, out_dtype, rank)
+        want = ops.low_rank(x, low, ids, base, singles=0)
+        check(want, *plain(x, low, ids, base))
+        out, hidden = torch.empty_like(base), torch.empty(2 * T * G * low.rank + 2 * 2, dtype=torch.bfloat16, device=DEV)
+        stream = torch.cuda.Stream()
+        args = (x.data_ptr(), K, low.a.data_ptr(), low.b.data_ptr(), low.scale.data_ptr(), low.ranks.data_ptr(), ids.data_ptr(), base.data_ptr(), N,
+                out.data_ptr(), N, out_dtype is torch.bfloat16, T, *low._sizes, hidden.data_ptr(), ops.num_sms(), err, stream.cuda_stream)
+        jobs.append((args, want, out, (low, ids, x, base, hidden, stream)))
+    torch.cuda.synchronize()
+    said, start = [], threading.Barrier(len(jobs))
+
+    def work(args):
+        start.wait(30)
+        said.extend(code for code in (lib.prism_low_rank_tile(*args) for _ in range(8000)) if code != 0)
+    threads = [threading.Thread(target=work, args=(j[0],)) for j in jobs]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert said == [], (len(said), set(said))
+    for _, want, out, _ in jobs:
+        assert torch.equal(out, want)
+    ops.check_tc_errors()
