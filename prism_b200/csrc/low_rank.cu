@@ -228,8 +228,13 @@ low_rank_token_kernel(const T* __restrict__ x_, long long ldx, int x_whole, cons
 template <typename T, typename O>
 int launch_tokens(const void* x, long long ldx, const void* a, const void* b, const float* scale, const int* ranks, const int* ids, const void* base,
                   long long ldb, void* out, long long ldo, int tokens, int K, int Kp, int r, int L, const Slices& s, int* err, int sms, cudaStream_t stream) {
-    if (tokens <= 0) return 0;
-    if (tokens > 65535) return (int)cudaErrorInvalidValue;
+    constexpr int MOST = 65535;                // tokens of a launch: its grid's third size
+    int code = 0;
+    for (; tokens > MOST && code == 0; tokens -= MOST) {
+        code = launch_tokens<T, O>(x, ldx, a, b, scale, ranks, ids, base, ldb, out, ldo, MOST, K, Kp, r, L, s, err, sms, stream);
+        x = (const T*)x + MOST * ldx, ids += MOST, base = base ? (const O*)base + MOST * ldb : nullptr, out = (O*)out + MOST * ldo;
+    }
+    if (tokens <= 0 || code != 0) return code;
     // Clusters at a time with an SM a CTA, with half of one, a third and a quarter.  Where a CTA has much of A, up to 18 are launched in the first form all the same:
     // rows without an adapter (of a captured step that has fewer requests than rows, say) are over at once.  16 tokens, down projection, 303 KB of A a CTA: 17.3 us,
     // in the second form 16.0; if one of them has none 10.9 and 16.3.
@@ -434,9 +439,14 @@ low_rank_plain_result_kernel(const float* __restrict__ hidden_, const T* __restr
 template <typename T, typename O>
 int launch_portions(const void* x, long long ldx, const void* a, const void* b, const float* scale, const int* ranks, const int* ids, const void* base,
                     long long ldb, void* out, long long ldo, int tokens, int K, int Kp, int r, int L, const Slices& s, void* hidden, int* err, cudaStream_t stream) {
-    if (tokens <= 0) return 0;
+    constexpr int MOST = 65535 * TOKENS;       // tokens of a launch; the next one's hidden values take the place of its own
+    int code = 0;
+    for (; tokens > MOST && code == 0; tokens -= MOST) {
+        code = launch_portions<T, O>(x, ldx, a, b, scale, ranks, ids, base, ldb, out, ldo, MOST, K, Kp, r, L, s, hidden, err, stream);
+        x = (const T*)x + MOST * ldx, ids += MOST, base = base ? (const O*)base + MOST * ldb : nullptr, out = (O*)out + MOST * ldo;
+    }
+    if (tokens <= 0 || code != 0) return code;
     const int tiles = (tokens + TOKENS - 1) / TOKENS;
-    if (tiles > 65535 || hidden == nullptr) return (int)cudaErrorInvalidValue;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(CTAS, tiles, s.n);
     cfg.blockDim = dim3(HT);
@@ -448,7 +458,7 @@ int launch_portions(const void* x, long long ldx, const void* a, const void* b, 
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = prism::pdl_enabled() ? 2 : 1;
-    int code = (int)cudaLaunchKernelEx(&cfg, low_rank_plain_hidden_kernel<T>, (const T*)x, ldx, (const T*)a, scale, ranks, ids, (float*)hidden, tokens, K, Kp, r, s.n, L,
+    code = (int)cudaLaunchKernelEx(&cfg, low_rank_plain_hidden_kernel<T>, (const T*)x, ldx, (const T*)a, scale, ranks, ids, (float*)hidden, tokens, K, Kp, r, s.n, L,
                                        err);
     if (code != 0) return code;
     int columns = 0;

@@ -796,9 +796,16 @@ PRISM_EXPORT int prism_low_rank_tile(const void* x, long long ldx, const void* a
                                      void* hidden, int sms, int* err, cudaStream_t stream) {
     using namespace prism::lowrank_tile;
     typedef __nv_bfloat16 bf16;
+    constexpr int MOST = 65535 * TILE;        // tokens of a launch; the next one's hidden values take the place of its own
+    const int size = out_dtype == PRISM_DTYPE_F32 ? 4 : 2;
+    for (; T > MOST; T -= MOST) {
+        const int code = prism_low_rank_tile(x, ldx, a, b, scale, ranks, ids, base, ldb, out, ldo, out_dtype, MOST, K, Kp, r, L, G, first, hidden, sms, err, stream);
+        if (code != 0) return code;
+        x = (const bf16*)x + MOST * ldx, ids += MOST, base = base ? (const char*)base + MOST * ldb * size : nullptr, out = (char*)out + MOST * ldo * size;
+    }
     if (T <= 0) return 0;
     const bool x_aligned = reinterpret_cast<uintptr_t>(x) % 16 == 0 && (ldx % 8 == 0 || T == 1);
-    if (!prism_low_rank_tile_supported(K, r, G, x_aligned) || Kp < K || Kp % 8 || L < 1 || sms < 1 || (T + TILE - 1) / TILE > 65535)
+    if (!prism_low_rank_tile_supported(K, r, G, x_aligned) || Kp < K || Kp % 8 || L < 1 || sms < 1)
         return (int)cudaErrorInvalidValue;
     Tiles s;
     s.n = G;

@@ -145,3 +145,31 @@ def test_threads_with_ranks_of_either_kind(out_dtype):
     for _, want, out, _ in jobs:
         assert torch.equal(out, want)
     ops.check_tc_errors()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=str)
+@pytest.mark.parametrize("T,singles", [(65535, 65535), (65536, 65536), (70000, 70000), (131100, 131080), (66000, 65900), (70001, 3)])
+def test_more_single_tokens_than_a_launch_has_room_for(dtype, T, singles):
+    """How the tokens are laid out changes no result's meaning: not with more singles than one launch takes either."""
+    low = stack(3, (24,), 24, 4, dtype, 3)
+    x, base = inputs(T, 24, 24, dtype, dtype, 7)
+    ids = (torch.arange(T, device=DEV) % 4 - 1).int()
+    got = _ops().low_rank(x, low, ids, base, singles=singles)
+    check(got, *plain(x, low, ids, base))
+    assert torch.equal(got[ids < 0], base[ids < 0])
+    again = base.clone()
+    _ops().low_rank(x, low, ids, again, out=again, singles=singles)
+    assert torch.equal(again, got)
+
+
+@pytest.mark.parametrize("dtype,out_dtype,T", [(torch.bfloat16, torch.bfloat16, 65535 * 128 + 300), (torch.bfloat16, torch.float32, 65535 * 128 + 1),
+                                               (torch.float32, torch.float32, 65535 * 32 + 300)], ids=str)
+def test_more_tiles_than_a_launch_has_room_for(dtype, out_dtype, T):
+    ops = _ops()
+    low = stack(3, (8,), 8, 4, dtype, 3)
+    g = torch.Generator(device=DEV).manual_seed(3)
+    x, base = torch.randn(T, 8, generator=g, device=DEV).to(dtype), torch.randn(T, 8, generator=g, device=DEV).to(out_dtype)
+    ids = (torch.arange(T, device=DEV) // 1000 % 4 - 1).int()
+    got = ops.low_rank(x, low, ids, base, singles=0)
+    check(got, *plain(x, low, ids, base))
+    ops.check_tc_errors()
