@@ -19,6 +19,11 @@ import torch
 from .. import ops
 
 CONFIG, TENSORS = "adapter_config.json", "adapter_model.safetensors"
+# settings that, where they are on, change the formula: other scales, ranks or layers, more parameters, tokens that the adapter leaves alone
+OTHER_FORMULAS = ("use_dora", "rank_pattern", "alpha_pattern", "modules_to_save", "fan_in_fan_out", "layer_replication", "lora_bias", "trainable_token_indices",
+                  "alora_invocation_tokens", "arrow_config", "use_qalora", "use_bdlora")
+# of the named ways to begin training those that leave W as it is; others take their product out of W, or round it
+PLAIN_BEGINNINGS = ("gaussian", "eva", "orthogonal")
 
 
 class AdapterError(ValueError):
@@ -52,7 +57,10 @@ def read_adapter_config(folder: str) -> Tuple[int, float]:
         raise AdapterError(f"no {CONFIG} in {folder}")
     with open(path) as f:
         raw = json.load(f)
-    bad = [k for k in ("use_dora", "rank_pattern", "alpha_pattern", "modules_to_save", "fan_in_fan_out", "layer_replication") if raw.get(k)]
+    bad = [k for k in OTHER_FORMULAS if raw.get(k)]
+    begin = raw.get("init_lora_weights")
+    if isinstance(begin, str) and begin.lower() not in PLAIN_BEGINNINGS:
+        bad.append("init_lora_weights")
     if raw.get("bias", "none") != "none":
         bad.append("bias")
     if raw.get("peft_type", "LORA") != "LORA":

@@ -1,0 +1,43 @@
+"""Adapter folders whose configuration says that W + scale B A is not the formula, and how the command answers (CPU)."""
+
+import json
+import os
+
+import pytest
+
+import adapter_helpers as H
+import helpers
+from prism_b200.weights import adapters as A
+
+
+def folder_with(**change):
+    d = H.adapter_folder(helpers.model_folder("B"), change.pop("rank", 3), 12, 1)
+    path = os.path.join(d, "adapter_config.json")
+    with open(path) as f:
+        cfg = json.load(f)
+    with open(path, "w") as f:
+        json.dump(dict(cfg, **change), f)
+    return d
+
+
+@pytest.mark.parametrize("how", ["pissa", "pissa_niter_16", "PiSSA", "olora", "corda", "loftq", "lora_ga", "something new"])
+def test_an_adapter_beside_a_changed_matrix_is_refused(how):
+    """Such a beginning takes its product out of W (or rounds W): the adapter belongs to the matrix that is left."""
+    with pytest.raises(A.AdapterError, match="init_lora_weights"):
+        A.read_adapter_config(folder_with(init_lora_weights=how))
+
+
+@pytest.mark.parametrize("how", [True, False, None, "gaussian", "eva", "orthogonal"])
+def test_a_beginning_that_leaves_the_matrix_is_taken(how):
+    assert A.read_adapter_config(folder_with(init_lora_weights=how)) == (3, 4.0)
+
+
+@pytest.mark.parametrize("change", [dict(alora_invocation_tokens=[5, 6]), dict(arrow_config={"top_k": 2}), dict(use_qalora=True), dict(use_bdlora={"nblocks": 2}),
+                                    dict(lora_bias=True), dict(trainable_token_indices=[1])])
+def test_what_applies_to_some_tokens_or_adds_more_is_refused(change):
+    with pytest.raises(A.AdapterError, match=next(iter(change))):
+        A.read_adapter_config(folder_with(**change))
+
+
+def test_settings_that_are_off_are_taken():
+    assert A.read_adapter_config(folder_with(alora_invocation_tokens=None, arrow_config=None, use_qalora=False, lora_bias=False, trainable_token_indices=None)) == (3, 4.0)
