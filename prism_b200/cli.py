@@ -56,7 +56,7 @@ def main(argv=None) -> int:
     import torch
     from .config.engine_config import EngineConfig, ModelConfig, SchedulerConfig
     from .sampling.sampler import SamplingParams
-    from .weights.adapters import read_adapter_config
+    from .weights.adapters import AdapterError, check_adapter_room, read_adapter_config
     from .weights.four_bit import four_bit_share
 
     raw = None
@@ -75,13 +75,22 @@ def main(argv=None) -> int:
         print("give --model DIR or --random-weights --config-json FILE", file=sys.stderr)
         return 2
 
+    adapter_rank = 16
+    if args.adapter is not None:
+        try:
+            adapter_rank = read_adapter_config(args.adapter)[0]
+            check_adapter_room(1, adapter_rank)
+        except ValueError as e:                      # an AdapterError among them
+            print(f"--adapter {args.adapter}: {e}", file=sys.stderr)
+            return 2
+
     from .engine.llm import Engine
     ec = EngineConfig(gpu_id=args.gpu, kv_page_size=args.page_size, num_pages=args.num_pages,
                       kv_cache_budget_gb=args.kv_budget_gb, max_seq_len=args.max_seq_len,
                       use_cuda_graph=not args.no_cuda_graph, seed=args.sample_seed,
                       scheduler=SchedulerConfig(args.max_batch_tokens, args.max_num_seqs, args.prefill_chunk),
                       weight_format=args.weight_format, act_bits=args.act_bits, max_adapters=int(args.adapter is not None),
-                      max_adapter_rank=read_adapter_config(args.adapter)[0] if args.adapter else 16)
+                      max_adapter_rank=adapter_rank)
     t0 = time.perf_counter()
     if raw is not None:
         eng = Engine(None, ec, dtype=args.dtype, config=raw, random_seed=args.seed)
@@ -89,7 +98,11 @@ def main(argv=None) -> int:
         eng = Engine(ModelConfig(args.model, args.name, args.dtype), ec)
     adapter = None if args.adapter is None else "adapter"
     if adapter:
-        eng.load_adapter(adapter, args.adapter)
+        try:
+            eng.load_adapter(adapter, args.adapter)
+        except AdapterError as e:
+            print(f"--adapter {args.adapter}: {e}", file=sys.stderr)
+            return 2
     t_load = time.perf_counter() - t0
     vocab = eng.model.spec.vocab_size
 

@@ -41,3 +41,12 @@ def test_what_applies_to_some_tokens_or_adds_more_is_refused(change):
 
 def test_settings_that_are_off_are_taken():
     assert A.read_adapter_config(folder_with(alora_invocation_tokens=None, arrow_config=None, use_qalora=False, lora_bias=False, trainable_token_indices=None)) == (3, 4.0)
+
+
+@pytest.mark.parametrize("make,say", [(lambda: folder_with(r=129), "129"), (lambda: folder_with(use_dora=True), "use_dora"), (lambda: "/nonexistent", "adapter_config")])
+def test_the_command_says_what_is_wrong_with_an_adapter(make, say, capsys):
+    """Before it loads a model, in a line."""
+    from prism_b200.cli import main
+    assert main(["--model", "/nonexistent", "--adapter", make()]) == 2
+    err = capsys.readouterr().err
+    assert say in err and "Traceback" not in err and err.count("\n") == 1
