@@ -84,14 +84,14 @@ __device__ __forceinline__ uint32_t rank_in_cluster() {
 // an adapter a token): down projection of rank 64, by the first two forms and the third of eight, 4 tokens 8.4, 10.8, 15.2; 24 tokens 19.9, 17.8, 22.9; q, k and v of
 // rank 16, 12 tokens three an SM 4.8, four 5.9; 64 tokens in clusters of eight, four and two 18.4, 14.0, 8.1 (the first two as they were with registers in
 // memory); gate and up, 64 tokens four an SM 23.0, three 27.5, 96 tokens 35.9 and 26.5.
-template <typename T, typename O, int THREADS, int PER_SM, int CTAS>
+template <typename T, typename O, int THREADS, int PER_SM, int TEAM>
 __global__ void __launch_bounds__(THREADS, PER_SM)
 low_rank_token_kernel(const T* __restrict__ x_, long long ldx, int x_whole, const T* __restrict__ a, const T* __restrict__ b,
                       const float* __restrict__ scale, const int* __restrict__ ranks, const int* __restrict__ ids_, const O* __restrict__ base_, long long ldb,
                       O* out_, long long ldo, int K, int Kp, int r, int L, const __grid_constant__ Slices slices, int parts, int* err) {
     constexpr int E = Chunk<T>::E, WARPS = THREADS / 32;
     __shared__ float hidden[MOST_RANK];
-    __shared__ float partial[MOST_RANK / CTAS][WARPS];             // a hidden value's share of a warp
+    __shared__ float partial[MOST_RANK / TEAM][WARPS];             // a hidden value's share of a warp
     __shared__ float scale_l;                                      // the adapter's, and its rank: asked for here, needed behind the sums
     __shared__ int own;
     asm volatile("barrier.cluster.arrive.aligned;" ::: "memory");              // here: peers may write into this CTA's memory
@@ -99,9 +99,9 @@ low_rank_token_kernel(const T* __restrict__ x_, long long ldx, int x_whole, cons
     pdl_wait();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, me = (int)rank_in_cluster();
     const int g = blockIdx.y / parts, part = blockIdx.y % parts, N = slices.first[slices.n], t = blockIdx.z;
-    // this CTA's columns: an eighth of its cluster's share of the slice
-    const int wide = slices.first[g + 1] - slices.first[g], shares = parts * CTAS, each = (wide + shares - 1) / shares;
-    const int n0 = slices.first[g] + min(wide, (part * CTAS + me) * each), mine = min(slices.first[g + 1], n0 + each) - n0;
+    // this CTA's columns: its part of its cluster's share of the slice
+    const int wide = slices.first[g + 1] - slices.first[g], shares = parts * TEAM, each = (wide + shares - 1) / shares;
+    const int n0 = slices.first[g] + min(wide, (part * TEAM + me) * each), mine = min(slices.first[g + 1], n0 + each) - n0;
     const T* x = pdl_fresh(x_) + (size_t)t * ldx;
     const O* base = base_ ? pdl_fresh(base_) + (size_t)t * ldb + n0 : nullptr;
     O* out = out_ + (size_t)t * ldo + n0;
@@ -137,8 +137,8 @@ low_rank_token_kernel(const T* __restrict__ x_, long long ldx, int x_whole, cons
             ahead[j][c] = n < mine ? __ldg(reinterpret_cast<const uint4*>(B + (size_t)n * r + part_at[c])) : make_uint4(0, 0, 0, 0);
         old[j] = chunk == 0 && n < mine && base ? base[n] : from_float<O>(0.f);
     }
-    // an eighth of the hidden values, several warps a row where there are fewer rows than warps
-    const int rows = r / CTAS;
+    // this CTA's part of the hidden values, several warps a row where there are fewer rows than warps
+    const int rows = r / TEAM;
     int split = 1;
     while (split * 2 * rows <= WARPS) split *= 2;
     const int sub = warp % split;
@@ -184,8 +184,8 @@ low_rank_token_kernel(const T* __restrict__ x_, long long ldx, int x_whole, cons
     if (tid == 0) asm volatile("cp.async.wait_all;" ::: "memory");
     __syncthreads();
     asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
-    if (tid < rows * CTAS) {                                       // a hidden value, for one of the CTAs
-        const int c = tid % CTAS, q = tid / CTAS;
+    if (tid < rows * TEAM) {                                       // a hidden value, for one of the CTAs
+        const int c = tid % TEAM, q = tid / TEAM;
         float h = 0.f;
         for (int w = 0; w < split; ++w) h += partial[q][w];
         h = me * rows + q < own ? h * scale_l : 0.f;

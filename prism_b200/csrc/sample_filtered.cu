@@ -433,7 +433,6 @@ __device__ __forceinline__ bool put(const Range& r, u64 at, float v, double w, i
 template <bool RESIDENT, bool BY_WEIGHT> __device__ __noinline__ void fill_first(double& tail_out, uint32_t& tail_n_out) {
     const Weigher weigh;
     const bool endless = sh.endless;
-    const float top = (float)sh.top;
     const int nv = (sh.n + 3) / 4;
     double tail = 0;
     uint32_t tail_n = 0;

@@ -173,3 +173,60 @@ def test_more_tiles_than_a_launch_has_room_for(dtype, out_dtype, T):
     got = ops.low_rank(x, low, ids, base, singles=0)
     check(got, *plain(x, low, ids, base))
     ops.check_tc_errors()
+
+
+def narrow(x, low, ids, base):
+    """``(result, bound)`` in 64 bits where hidden values stay in float32: any order of additions of K, r and one more products, 2^-23 of the sum of
+    the magnitudes each, as in test_low_rank_gpu, but nothing for two bfloat16 terms."""
+    x, a, b, scale = x.double(), low.a.double(), low.b.double(), low.scale.double()
+    y = base.double().clone()
+    tol = 2.0 ** -23 * y.abs()
+    for e in range(low.count):
+        tok = torch.nonzero(ids == e).squeeze(1)
+        at = 0
+        for g, n in enumerate(low.rows):
+            A, B = a[e, g, :, :low.k], b[e, at:at + n]
+            h = scale[e] * (x[tok] @ A.t())
+            y[tok, at:at + n] += h @ B.t()
+            tol[tok, at:at + n] += 2.0 ** -23 * ((low.k + 2) * (scale[e] * (x[tok].abs() @ A.abs().t()) @ B.abs().t()) + (low.rank + 4) * (h.abs() @ B.abs().t()))
+            at += n
+    return y, tol
+
+
+@pytest.mark.parametrize("rows,K,rank", [((64,), 64, 16), ((501, 77), 1003, 5), ((130, 64, 8), 520, 33), ((896, 128, 128), 896, 128)])
+@pytest.mark.parametrize("dtype,T,singles", [(torch.float32, 1, 1), (torch.float32, 40, 40), (torch.float32, 200, 200), (torch.float32, 300, 0), (torch.float32, 300, 20),
+                                             (torch.bfloat16, 1, 1), (torch.bfloat16, 40, 40), (torch.bfloat16, 64, 64), (torch.bfloat16, 200, 200)], ids=str)
+def test_hidden_values_keep_32_bits_off_the_tensor_cores(rows, K, rank, dtype, T, singles):
+    """Beside the bound of every result the whole's relative 2-norm error stays below 2^-20: roundings of half a step, 2^-24, that are not all of one
+    sign, in chains of K / 8 products at most (1,003: sqrt(125 / 3) half steps of a hidden value, 2^-21.3).  Two bfloat16 terms leave 2^-17 of a hidden value each
+    and would pass neither."""
+    low = stack(4, rows, K, rank, dtype, K)
+    x, base = inputs(T, K, sum(rows), dtype, torch.float32, T)
+    base *= 2.0 ** -6                                     # so that the adapters' part is most of the result
+    ids = torch.sort(torch.randint(0, 4, (T,), generator=torch.Generator().manual_seed(T)).int()).values.to(DEV)
+    want, tol = narrow(x, low, ids, base)
+    err = (_ops().low_rank(x, low, ids, base, singles=singles).double() - want).abs()
+    assert (err <= tol + 2.0 ** -24 * (want.abs() + tol)).all()
+    assert err.norm() <= 2.0 ** -20 * want.norm()
+
+
+@pytest.mark.parametrize("dtype,out_dtype", [(torch.bfloat16, torch.bfloat16), (torch.bfloat16, torch.float32), (torch.float32, torch.float32)], ids=str)
+@pytest.mark.parametrize("T,singles", [(1, 1), (40, 40), (64, 64), (200, 0), (300, 0), (300, 40), (1000, 0)])
+def test_a_token_s_bits_do_not_depend_on_its_neighbours(dtype, out_dtype, T, singles):
+    """With as many tokens laid out in the same way: whatever the others' activations and adapters are, how many adapters share a tile, and beside NaN."""
+    ops = _ops()
+    rows, K = (700, 130, 24), 500
+    low = stack(8, rows, K, 32, dtype, 23)
+    x, base = inputs(T, K, sum(rows), dtype, out_dtype, 29)
+    g = torch.Generator().manual_seed(T)
+    ids = torch.sort(torch.randint(-1, 3, (T,), generator=g).int()).values.to(DEV)
+    kept = (torch.rand(T, generator=g) < 0.3).to(DEV)
+    kept[0] = True
+    want = ops.low_rank(x, low, ids, base, singles=singles)
+    for others in (torch.full((T,), -1), torch.full((T,), 7), torch.randint(-1, 8, (T,), generator=g), torch.arange(T) % 9 - 1):
+        x2, base2 = inputs(T, K, sum(rows), dtype, out_dtype, 31)
+        x2[::3] = float("nan")
+        x2[kept], base2[kept] = x[kept], base[kept]
+        ids2 = torch.where(kept, ids, others.int().to(DEV))
+        got = ops.low_rank(x2, low, ids2, base2, singles=singles)
+        assert torch.equal(got[kept], want[kept])
