@@ -17,8 +17,8 @@
 // of the 7B shape, rank 16: 40 us, so 32; without registers in memory 23, 4.1 TB/s).  One token there takes 4.3 us, four of them launch, first loads and two barriers of the cluster.
 //
 // Portions: 32 tokens at a time, hidden values (a cluster shares K, its sums meet through distributed shared memory) and results in a launch
-// each.  A tile's tokens may have several adapters: it is gone through once for each of them.  512 tokens of two adapters, gate and up, rank 16, in float32: 85 us,
-// as long as the products' multiply-adds through shared memory take; one by one they would take 200.
+// each.  A tile's tokens may have several adapters: it is gone through once for each of them.  512 tokens of one adapter, gate and up of the 7B shape, rank 16, in
+// float32: 173 us, of two 176; one by one 207.  Reading and writing the shared result takes 24 of them, the rest are loads of single values from shared memory.
 #include "vec.cuh"
 
 namespace prism {
@@ -79,8 +79,9 @@ __device__ __forceinline__ uint32_t rank_in_cluster() {
 // ---- one token ----------------------------------------------------------------------------------------------
 
 // Forms of it, by the clusters of a launch, as a cluster's CTAs are neighbours and so many run at a time.  512 threads and an SM's registers, eight loads of A in
-// flight a thread: 15 clusters on 148 SMs.  512 threads and half of them, where a CTA has much of A: 33.  Else 256 threads, three or four CTAs an SM (whose registers
-// are short by ten: they spill outside the loops), in clusters of eight, four and two: the fewest CTAs an SM that run at a time.  Microseconds (bfloat16, the 7B shape,
+// flight a thread: 15 clusters on 148 SMs.  512 threads and half of them, where a CTA has much of A: 33.  Else 256 threads, three or four CTAs an SM, in clusters of eight,
+// four and two: the fewest CTAs an SM that run at a time.  With four an SM registers are short: of a thread's 44 bytes go through memory, 56 with float32 results, 20
+// with float32 adapters (36 to 68 and 12 in the second form, 8 to 12 and none with three an SM).  Microseconds (bfloat16, the 7B shape,
 // an adapter a token): down projection of rank 64, by the first two forms and the third of eight, 4 tokens 8.4, 10.8, 15.2; 24 tokens 19.9, 17.8, 22.9; q, k and v of
 // rank 16, 12 tokens three an SM 4.8, four 5.9; 64 tokens in clusters of eight, four and two 18.4, 14.0, 8.1 (the first two as they were with registers in
 // memory); gate and up, 64 tokens four an SM 23.0, three 27.5, 96 tokens 35.9 and 26.5.
@@ -241,8 +242,8 @@ int launch_tokens(const void* x, long long ldx, const void* a, const void* b, co
     }
     if (tokens <= 0 || code != 0) return code;
     // Clusters at a time with an SM a CTA, with half of one, a third and a quarter.  Where a CTA has much of A, up to 18 are launched in the first form all the same:
-    // rows without an adapter (of a captured step that has fewer requests than rows, say) are over at once.  16 tokens, down projection, 303 KB of A a CTA: 17.3 us,
-    // in the second form 16.0; if one of them has none 10.9 and 16.3.
+    // rows without an adapter (of a captured step that has fewer requests than rows, say) are over at once.  16 tokens, down projection, 303 KB of A a CTA, eight
+    // adapters: 17.3 us if all 16 have one, in the second form 16.0; if one of them has none 10.9 and 16.3.
     const bool much = (long long)r / CTAS * Kp * (int)sizeof(T) >= 128 * 1024;
     const int wholes = sms / CTAS * 5 / 6, halves = much ? sms * 9 / (CTAS * 5) : 0, thirds = sms * 9 / 25, quarters = sms * 12 / 25;
     const int first_form = much ? sms / CTAS : wholes;

@@ -7,7 +7,7 @@
 // 1 and more and NaN as the largest float32 below 1).
 // T <= 0: the largest, lowest index on ties.  NaN counts as -infinity, which is never kept; a row with nothing else gives token 0.
 //
-// Weights come from 64-bit arithmetic (relative error below 2^-50).  The draw adds them up as whole numbers, w_i * 2^46 rounded: such sums are exact, so neither
+// Weights come from 64-bit arithmetic (relative error below 2^-48 + 2^-51 |x_i - m| / T: the series and the rounded 1 / T).  The draw adds them up as whole numbers, w_i * 2^46 rounded: such sums are exact, so neither
 // the order of additions nor the number of CTAs that share a row can change them, and every thread sees the same running weight; a draw is decided
 // to about 1e-12 of the weight (in float32 one row in thirty over 150,000 tokens would be decided by rounding).  top_p = 0.9999999 ends a
 // prefix among weights that such steps do not resolve: its sums are 64-bit floats, added in an order that V alone fixes.

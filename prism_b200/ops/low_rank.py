@@ -149,10 +149,13 @@ def in_use(w):
 
 SINGLES = 64                 # without a word from the caller, so many tokens are taken one by one
 # So many tokens of portions, and they are taken in tiles: of 128 on tensor cores, or of 32 on CUDA cores (32-bit floats, sizes that TMA does not
-# take); fewer one by one.  Microseconds one by one and in tiles, all tokens of one adapter, for gate and up (rank 16), q k v (32) and down (64) of the 7B shape:
-# bfloat16, 64 tokens 16.0/18.7, 13.1/19.1, 27.4/29.6; 96 tokens 17.3/18.9, 19.1/19.3, 35.5/29.9; 128 tokens 26.4/19.0, 25.3/19.7, 51.4/30.3 (two adapters a tile cost
-# the tiles a fifth more).  float32, 128 tokens 35/54, 33/44, 58/193; 192 tokens 63/61, 42/80, 91/196; 256 tokens 91/106, 54/80, 112/197; 512 tokens 200/85 (gate
-# and up).
+# take); fewer one by one.  Microseconds one by one and in tiles, all tokens of one adapter, for gate and up, q k v and down of the 7B shape.
+# bfloat16, rank 16: 64 tokens 15.5/18.6, 7.7/17.3, 10.4/28.1; 96 tokens 19.6/18.9, 10.6/17.6, 12.1/28.2; 128 tokens 32/19, 15.1/17.8, 16.5/28.4 (two adapters a
+# tile cost the tiles a fifth more).  Rank 64: 64 tokens 68/20, 22/21, 27/29; 96 tokens 77/21, 34/22, 35/29.  Rank 128: 64 tokens 121/26, 43/27, 51/31.
+# float32, rank 16: 192 tokens 110/62, 28/75, 51/178; 256 tokens 115/105, 42/76, 68/179; 384 tokens 170/122, 65/115, 127/181.  Rank 64: 128 tokens 220/81,
+# 78/48, 85/185; 256 tokens 417/156, 147/84, 263/189.
+# One border for all ranks and widths: it is near where the two meet for rank 16 and for the narrower matrices of rank 64; wide matrices of larger ranks would
+# go in tiles from 32 tokens on (gate and up of rank 64: 35/19), q k v and down of rank 16 stay one by one longer.
 TILE_FROM = 96
 PLAIN_TILE_FROM = 256
 
@@ -161,10 +164,12 @@ def low_rank(x: torch.Tensor, low: LowRank, ids: torch.Tensor, base: Optional[to
              singles: Optional[int] = None) -> torch.Tensor:
     """``out[t] = base[t] + scale[l] (x[t] A_l^T) B_l^T`` with ``l = ids[t]`` (int32 ``[T]`` on the device; negative: ``out[t] = base[t]``).
     ``x [T, K]`` in the adapters' dtype; ``base`` and ``out [T, N]`` both bfloat16 or both float32, rows may have strides of their own;
-    ``base`` None: zeros; ``out`` may be ``base`` itself, else it shares no memory with the others.  Adapters are finite.  Sums in float32, one rounding.  ``singles``: so many tokens from the first on are
-    each a request of its own, and the others stand in runs of one adapter (as in a step: decoding requests, then portions of
-    prompts); this says how the work is laid out and changes no result's meaning.  An id outside the stack adds nothing and is reported by
-    ``check_tc_errors``."""
+    ``base`` None: zeros; ``out`` may be ``base`` itself, else it shares no memory with the others.  Adapters are finite.  Sums in float32, one rounding; portions in
+    bfloat16 that go by tensor cores keep a hidden value (``x A^T``) as two bfloat16 terms, off by 2^-16 of it at most.  ``singles``: so many tokens from the first on
+    are each a request of its own, and the others stand in runs of one adapter (as in a step: decoding requests, then portions of
+    prompts); this says how the work is laid out and changes no result's meaning, though with the layout, and with how many tokens there are, the
+    order of additions changes: a token's last bits may (among as many tokens in the same layout its neighbours change none).  An id outside the stack adds
+    nothing and is reported by ``check_tc_errors``."""
     d, xs, dt = x.get_device(), x.shape, x.dtype
     if d < 0 or len(xs) != 2 or xs[1] != low.k or dt is not low.a.dtype or (x.stride(1) != 1 and low.k > 1) or low.a.get_device() != d:
         raise ops.KernelError(f"adapters in {low.a.dtype} on {low.a.device} for rows of {low.k} side by side in that CUDA device's memory: got {tuple(xs)} "
