@@ -511,7 +511,7 @@ PRISM_EXPORT int prism_low_rank(const void* x, long long ldx, int dtype, const v
     return prism::lowrank::run(x, ldx, dtype, a, b, scale, nullptr, ids, base, ldb, out, ldo, out_dtype, T, K, Kp, r, L, G, first, hidden, sms, err, stream);
 }
 
-// The same with ranks [L, G]: how many rows of A each adapter has in each slice.
+// The same with ranks [L, G]: how many rows of A each adapter has in each slice; null: all r.
 PRISM_EXPORT int prism_low_rank_ranked(const void* x, long long ldx, int dtype, const void* a, const void* b, const float* scale, const int* ranks,
                                        const int* ids, const void* base, long long ldb, void* out, long long ldo, int out_dtype, int T, int K, int Kp,
                                        int r, int L, int G, const int* first, void* hidden, int sms, int* err, cudaStream_t stream) {

@@ -191,30 +191,30 @@ def low_rank(x: torch.Tensor, low: LowRank, ids: torch.Tensor, base: Optional[to
     singles = (T if T <= SINGLES else 0) if singles is None else max(0, min(int(singles), T))
     L, stream, err = ops.lib(), ops._stream(), ops.mxfp4._err_word(x.device)
     sms = ops._num_sms.get(d) or ops.num_sms(x.device)
-    sizes, ap, bp, sp = low._sizes, low.a.data_ptr(), low.b.data_ptr(), low.scale.data_ptr()
-    rp = None if low.ranks is None else low.ranks.data_ptr()
-    plain, head = (L.prism_low_rank, (ap, bp, sp)) if rp is None else (L.prism_low_rank_ranked, (ap, bp, sp, rp))
+    ap, bp, sp, sizes, ranks = low.a.data_ptr(), low.b.data_ptr(), low.scale.data_ptr(), low._sizes, low.ranks
     bf16, out16 = dt is torch.bfloat16, odt is torch.bfloat16
     xp, x_row, ip, op, o_row = x.data_ptr(), x.stride(0), ids.data_ptr(), out.data_ptr(), out.stride(0)
     basep, b_row = (None, 0) if base is None else (base.data_ptr(), base.stride(0))
-    G, tiles = len(low.rows), False
     if singles < T:
+        G = len(low.rows)
         tiles = bf16 and xp % 16 == 0 and x_row % 8 == 0 and x_row >= low.k and L.prism_low_rank_tile_supported(low.k, low.rank, G, True)
         if T - singles < (TILE_FROM if tiles else PLAIN_TILE_FROM):
             singles = T
     if singles:
-        ops._check(plain(xp, x_row, bf16, *head, ip, basep, b_row, op, o_row, out16, singles, *sizes, None, sms, err, stream), "low_rank")
-    rest = T - singles
-    if rest == 0:
-        return out
-    size = 2 if out16 else 4
+        ops._check(L.prism_low_rank(xp, x_row, bf16, ap, bp, sp, ip, basep, b_row, op, o_row, out16, singles, *sizes, None, sms, err, stream)
+                   if ranks is None else
+                   L.prism_low_rank_ranked(xp, x_row, bf16, ap, bp, sp, ranks.data_ptr(), ip, basep, b_row, op, o_row, out16, singles, *sizes, None, sms, err, stream),
+                   "low_rank")
+        if singles == T:
+            return out
+    rest, size = T - singles, 2 if out16 else 4
     xp, op, basep = xp + singles * x_row * (2 if bf16 else 4), op + singles * o_row * size, basep and basep + singles * b_row * size
-    args = (ip + 4 * singles, basep, b_row, op, o_row, out16, rest, *sizes)
+    args = (ops._ptr(ranks), ip + 4 * singles, basep, b_row, op, o_row, out16, rest, *sizes)
     if tiles:
         hidden = torch.empty(2 * rest * G * low.rank + 2 * (-(-rest // 128)), dtype=torch.bfloat16, device=x.device)
-        ops._check(L.prism_low_rank_tile(xp, x_row, ap, bp, sp, rp, *args, hidden.data_ptr(), sms, err, stream), "low_rank_tile")
+        ops._check(L.prism_low_rank_tile(xp, x_row, ap, bp, sp, *args, hidden.data_ptr(), sms, err, stream), "low_rank_tile")
     else:
         hidden = torch.empty(rest * G * low.rank, dtype=torch.float32, device=x.device)
-        ops._check(plain(xp, x_row, bf16, *head, *args, hidden.data_ptr(), sms, err, stream), "low_rank")
+        ops._check(L.prism_low_rank_ranked(xp, x_row, bf16, ap, bp, sp, *args, hidden.data_ptr(), sms, err, stream), "low_rank")
     ops.launch_count += 1                    # two kernels
     return out
