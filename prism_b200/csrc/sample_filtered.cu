@@ -391,7 +391,8 @@ __device__ __forceinline__ int bin_of(bool by_weight, int octave, float v, int s
 __device__ __noinline__ float border(bool by_weight, int octave, int b) {
     const double d = octave + (b + (by_weight ? 0.5 : 1.0)) / STEPS;
     const double v = sh.top - (by_weight ? d / sh.per : d * 0.69314718055994530942), room = 1e-6 * (fabs(v) + fabs(sh.top));
-    uint32_t out = key_of(fmaxf(LEAST, (float)(v - room))), in = key_of(fminf((float)sh.top, fmaxf(LEAST, (float)(v + room))));
+    // rounded outwards: among the smallest numbers a float's step is wider than the room
+    uint32_t out = key_of(fmaxf(LEAST, __double2float_rd(v - room))), in = key_of(fminf((float)sh.top, fmaxf(LEAST, __double2float_ru(v + room))));
     if (out > in) out = in;
     // `in` has a bin up to b; the border is not below `out`
 #pragma unroll 1

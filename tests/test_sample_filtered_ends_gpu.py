@@ -6,7 +6,7 @@ import numpy as np
 import pytest
 import torch
 
-from test_sample_filtered_gpu import DEV, draw, plain_row
+from test_sample_filtered_gpu import DEV, check, draw, plain_row
 
 pytestmark = pytest.mark.gpu
 LAST = 1 - 2.0 ** -24                                    # the largest float32 below 1
@@ -39,3 +39,16 @@ def test_what_is_below_0_is_0(V, k):
     x = torch.zeros(4, V, device=DEV)
     k = None if k is None else [k] * 4
     assert draw(x, [1.0] * 4, ends, k) == draw(x, [1.0] * 4, [0.0] * 4, k)
+
+
+@pytest.mark.parametrize("V", [300, 9001, 50257, 152064])
+@pytest.mark.parametrize("scale", [3e-42, 2e-40, 4e-39, 1e-37])
+def test_logits_and_temperatures_that_are_nearly_nothing(V, scale):
+    """Below 2^-126 float32 has steps of 2^-149, whatever the value: borders between bins are values too."""
+    R = 12
+    g = torch.Generator().manual_seed(V)
+    rng = np.random.RandomState(V % 1000)
+    x = (torch.randn(R, V, generator=g, dtype=torch.float64) * scale).float().to(DEV)
+    t = (scale * (0.1 + rng.rand(R))).astype(np.float32)
+    check(x, t, 0.02 + 0.96 * rng.rand(R), k=[0, 0, 0, V // 2, 0, V // 3, 0, 300, 0, 0, V // 4, 0],
+          p=[0.3, 0.6, 0.9, 0.99, 0.9999994, 0.5, 0.04, 0.97, 0.8, 0.25, 0.9, 0.75], m=[0, 0, 0, 0, 0, 1e-6, 0, 0, 1e-4, 0, 0, 0.01])
