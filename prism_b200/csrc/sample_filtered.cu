@@ -9,7 +9,7 @@
 //
 // Weights come from 64-bit arithmetic (relative error below 2^-48 + 2^-51 |x_i - m| / T: the series and the rounded 1 / T).  The draw adds them up as whole numbers, w_i * 2^46 rounded: such sums are exact, so neither
 // the order of additions nor the number of CTAs that share a row can change them, and every thread sees the same running weight; a draw is decided
-// to about 1e-12 of the weight (in float32 one row in thirty over 150,000 tokens would be decided by rounding).  top_p = 0.9999999 ends a
+// to about 1e-12 of the weight (in float32 one row in thirty over 150,000 tokens would be decided by rounding), and a token of less than 2^-47 is never drawn.  top_p = 0.9999999 ends a
 // prefix among weights that such steps do not resolve: its sums are 64-bit floats, added in an order that V alone fixes.
 //
 // One cluster of CTAs a row: each keeps its slice of the logits in shared memory, so that the row is read once, and the CTAs' sums meet

@@ -739,15 +739,18 @@ _MOST_VOCABULARY = 520000     # csrc/sample_filtered.cu: MOST_V
 def sample_filtered(logits: torch.Tensor, temperature: Optional[torch.Tensor], u: torch.Tensor, out: torch.Tensor,
                     top_k: Optional[torch.Tensor] = None, top_p: Optional[torch.Tensor] = None, min_p: Optional[torch.Tensor] = None,
                     rows: Optional[torch.Tensor] = None, kept: Optional[torch.Tensor] = None, logprob: Optional[torch.Tensor] = None):
-    """Per row: a token of ``softmax(logits / temperature)`` among those that the row's filters keep, at the uniform number ``u`` (in
-    ``[0, 1)``; any other as the nearer end, NaN as the upper one, the largest float32 below 1) of the inverse CDF.  ``top_k`` (int32; 0 or less: off) keeps the largest logits (the lower index of equal ones);
+    """Per row: a token of ``softmax(logits / temperature)`` among those that the row's filters keep, at the uniform number ``u`` of the
+    inverse CDF (in ``[0, 1)``; any other counts as the nearer end, the upper one being the largest float32 below 1, and so does NaN).
+    ``top_k`` (int32; 0 or less: off) keeps the largest logits (the lower index of equal ones);
     ``top_p`` (float32; 1 or more: off) the shortest run of the likeliest of these whose probability reaches that share of theirs, one at least;
     ``min_p`` (float32; 0 or less: off) of these the ones at least ``min_p`` times as likely as the likeliest.  Temperature 0 or less
     (or None for all rows): the largest, lowest index on ties.  NaN counts as -infinity, which is never kept; rows of nothing else give token
     0.  +infinity leaves the probability to such logits alone.  Decided in 64-bit arithmetic and whole-number sums: a row's result
-    depends on its own logits and settings only.  ``rows`` (int32): only these rows of ``logits``, each at most once; the others' results are
-    left as they are.  Results by row of ``logits``: ``out`` (int32); ``kept`` (int32): how many tokens it was drawn from (1 if greedy; 0
-    for a row of nothing); ``logprob`` (float32): the logarithm of the probability that the token had among them (0 if greedy, -infinity
+    depends on its own logits and settings only.  Those numbers' steps are 2^-46 of the likeliest token's weight (2^-45 from 262,144 tokens
+    on): a token of less than half of one counts where filters cut and is never drawn, and ``logprob`` is off by half of one a kept token
+    at most, beside its rounding.  ``rows`` (int32): only these rows of ``logits``, each at most once; the others' results are left as they
+    are.  Results by row of ``logits``: ``out`` (int32); ``kept`` (int32): how many tokens it was drawn from (1 if greedy; 0 for a row of
+    nothing); ``logprob`` (float32): the logarithm of the probability that the token had among them (0 if greedy, -infinity
     for a row of nothing)."""
     d = logits.get_device()
     shape = logits.shape

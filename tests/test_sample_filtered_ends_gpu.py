@@ -52,3 +52,13 @@ def test_logits_and_temperatures_that_are_nearly_nothing(V, scale):
     t = (scale * (0.1 + rng.rand(R))).astype(np.float32)
     check(x, t, 0.02 + 0.96 * rng.rand(R), k=[0, 0, 0, V // 2, 0, V // 3, 0, 300, 0, 0, V // 4, 0],
           p=[0.3, 0.6, 0.9, 0.99, 0.9999994, 0.5, 0.04, 0.97, 0.8, 0.25, 0.9, 0.75], m=[0, 0, 0, 0, 0, 1e-6, 0, 0, 1e-4, 0, 0, 0.01])
+
+
+@pytest.mark.parametrize("V", [6, 700, 40000])
+def test_what_is_too_unlikely_is_kept_and_never_drawn(V):
+    """A token's weight counts in steps of 2^-46 of the largest one's: 2^-48 of it is none, 2^-45 is two."""
+    x = torch.full((2, V), -math.inf)
+    x[:, 0], x[:, V // 2], x[:, V - 1] = -48 * math.log(2), -45 * math.log(2), 0.0
+    tok, kept, lp = draw(x.to(DEV), [1.0, 1.0], [0.0, 0.5])
+    assert tok == [V // 2, V - 1] and kept == [3, 3]
+    assert abs(lp[0] + 45 * math.log(2)) < 1e-5 and abs(lp[1]) < 2.0 ** -40
