@@ -59,3 +59,21 @@ def test_matrices_that_want_gradients_leave_nothing_behind():
     assert torch.equal(low.a[1, 0, :3, :24], a.detach() * 2) and torch.equal(low.b[1, :, :3], b.detach())
     for t in (low.a, low.b, low.scale, low.ranks):
         assert not t.requires_grad and t.grad_fn is None
+
+
+def test_the_library_refuses_sizes_with_ranks_and_in_tiles():
+    lib = ops.lib()
+    first, back = (ctypes.c_int * 3)(0, 8, 12), (ctypes.c_int * 3)(0, 8, 8)
+    p, q = ctypes.addressof(first), ctypes.addressof(back)
+
+    def ranked(T=4, K=20, Kp=24, r=16, L=2, G=2, first=p, hidden=None, sms=148):
+        return lib.prism_low_rank_ranked(p, 24, 0, p, p, p, p, p, p, 12, p, 12, 0, T, K, Kp, r, L, G, first, hidden, sms, p, None)
+
+    def tile(T=4, K=20, Kp=24, r=16, L=2, G=2, first=p, hidden=p, sms=148):
+        return lib.prism_low_rank_tile(p, 24, p, p, p, p, p, p, 12, p, 12, 0, T, K, Kp, r, L, G, first, hidden, sms, p, None)
+    assert ranked(T=0) == 0 and tile(T=0) == 0
+    for change in (dict(G=0), dict(G=9), dict(r=8), dict(r=0), dict(r=144), dict(r=24), dict(K=0), dict(Kp=16), dict(Kp=20, K=20), dict(L=0), dict(sms=0), dict(first=q)):
+        for T in (4, 70000):
+            assert ranked(T=T, **change) == 1, change
+        for T in (4, 65535 * 128 + 5):
+            assert tile(T=T, **change) == 1, change
