@@ -55,8 +55,13 @@ def read_adapter_config(folder: str) -> Tuple[int, float]:
     path = os.path.join(folder, CONFIG)
     if not os.path.isfile(path):
         raise AdapterError(f"no {CONFIG} in {folder}")
-    with open(path) as f:
-        raw = json.load(f)
+    try:
+        with open(path) as f:
+            raw = json.load(f)
+    except ValueError as e:                          # no text, or no JSON
+        raise AdapterError(f"{path}: {e}") from None
+    if not isinstance(raw, dict):
+        raise AdapterError(f"{path}: an object with the adapter's settings is needed, got {type(raw).__name__}")
     bad = [k for k in OTHER_FORMULAS if raw.get(k)]
     begin = raw.get("init_lora_weights")
     if isinstance(begin, str) and begin.lower() not in PLAIN_BEGINNINGS:

@@ -50,3 +50,14 @@ def test_the_command_says_what_is_wrong_with_an_adapter(make, say, capsys):
     assert main(["--model", "/nonexistent", "--adapter", make()]) == 2
     err = capsys.readouterr().err
     assert say in err and "Traceback" not in err and err.count("\n") == 1
+
+
+@pytest.mark.parametrize("text", ["", "{", "[1, 2]", "3", "null", "\xff\xfe"])
+def test_a_configuration_that_is_none_is_refused(text, capsys):
+    from prism_b200.cli import main
+    d = folder_with()
+    with open(os.path.join(d, "adapter_config.json"), "w", encoding="latin-1") as f:
+        f.write(text)
+    with pytest.raises(A.AdapterError, match="adapter_config"):
+        A.read_adapter_config(d)
+    assert main(["--model", "/nonexistent", "--adapter", d]) == 2 and "adapter_config" in capsys.readouterr().err
