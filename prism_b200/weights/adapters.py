@@ -82,24 +82,29 @@ def read_adapter_folder(folder: str) -> Tuple[Dict[str, Tuple[torch.Tensor, torc
     """``({module: (A [rank, in], B [out, rank])}, scale)`` of a folder with ``adapter_config.json`` (``r``, ``lora_alpha``) and
     ``adapter_model.safetensors`` (``[base_model.model.]<module>.lora_A.weight`` and ``.lora_B.weight`` for the model file's tensor
     ``<module>.weight``, or ``<module>`` in a design whose tensors are named without that ending)."""
-    from safetensors import safe_open
+    from safetensors import SafetensorError, safe_open
     rank, scale = read_adapter_config(folder)
     path = os.path.join(folder, TENSORS)
     if not os.path.isfile(path):
         raise AdapterError(f"no {TENSORS} in {folder}")
     halves: Dict[str, Dict[str, torch.Tensor]] = {}
     wrong: List[str] = []
-    with safe_open(path, framework="pt", device="cpu") as f:
-        for name in f.keys():
-            module, _, half = name.rpartition(".lora_")
-            if half not in ("A.weight", "B.weight") or not module:
-                wrong.append(f"unexpected tensor {name}")
-                continue
-            module = module[len("base_model.model."):] if module.startswith("base_model.model.") else module
-            t = f.get_tensor(name)
-            if t.dim() != 2 or t.dtype not in (torch.float32, torch.float16, torch.bfloat16):
-                wrong.append(f"{name}: a matrix in float32, float16 or bfloat16 is needed, got {t.dtype} {tuple(t.shape)}")
-            halves.setdefault(module, {})[half[0]] = t
+    try:
+        with safe_open(path, framework="pt", device="cpu") as f:
+            tensors = {name: f.get_tensor(name) for name in f.keys()}
+    except SafetensorError as e:
+        raise AdapterError(f"{path}: {e}") from None
+    for name, t in tensors.items():
+        module, _, half = name.rpartition(".lora_")
+        if half not in ("A.weight", "B.weight") or not module:
+            wrong.append(f"unexpected tensor {name}")
+            continue
+        module = module[len("base_model.model."):] if module.startswith("base_model.model.") else module
+        if t.dim() != 2 or t.dtype not in (torch.float32, torch.float16, torch.bfloat16):
+            wrong.append(f"{name}: a matrix in float32, float16 or bfloat16 is needed, got {t.dtype} {tuple(t.shape)}")
+        if half[0] in halves.setdefault(module, {}):
+            wrong.append(f"{name}: {module} is named twice")
+        halves[module][half[0]] = t
     for name, ab in halves.items():
         if len(ab) != 2:
             wrong.append(f"{name}: only its {next(iter(ab))} is there")

@@ -4,6 +4,7 @@ import json
 import os
 
 import pytest
+from safetensors.torch import load_file, save_file
 
 import adapter_helpers as H
 import helpers
@@ -61,3 +62,25 @@ def test_a_configuration_that_is_none_is_refused(text, capsys):
     with pytest.raises(A.AdapterError, match="adapter_config"):
         A.read_adapter_config(d)
     assert main(["--model", "/nonexistent", "--adapter", d]) == 2 and "adapter_config" in capsys.readouterr().err
+
+
+@pytest.mark.parametrize("keep", [0, 5, 40, -16])
+def test_tensors_that_are_cut_off_are_refused(keep):
+    d = folder_with()
+    path = os.path.join(d, "adapter_model.safetensors")
+    with open(path, "rb") as f:
+        data = f.read()
+    with open(path, "wb") as f:
+        f.write(data[:keep])
+    with pytest.raises(A.AdapterError, match="adapter_model"):
+        A.read_adapter_folder(d)
+
+
+def test_a_matrix_that_is_named_twice_is_refused():
+    d = folder_with()
+    path = os.path.join(d, "adapter_model.safetensors")
+    tensors = {n: v.clone() for n, v in load_file(path).items()}
+    first = sorted(tensors)[0]
+    save_file(dict(tensors, **{first.removeprefix("base_model.model."): tensors[first] * 2}), path)
+    with pytest.raises(A.AdapterError, match="twice"):
+        A.read_adapter_folder(d)
